@@ -45,6 +45,8 @@ extern "C" {
  * the same buffer by the float32 scales s_r [B][Hq][T].  Buffer bytes:
  * B*Hq*T*(2*D + 4).  Eight times finer than bf16 at half float32's size. */
 #define NSA_F16S 2
+/* Only for the rows of nsa_norm_fwd in 8 bits: OCP e4m3 (448 the largest). */
+#define NSA_E4M3 3
 
 #define NSA_MODE_WINDOW 0
 #define NSA_MODE_COMPRESS 1
@@ -520,6 +522,74 @@ int nsa_decode_step(void* kc, void* vc, void* ks, void* vs, void* kw, void* vw, 
                     void* out, int32_t* block_idx, void* workspace, size_t workspace_bytes, int B, int Hq, int Hkv,
                     int D, int Tcap, int Ncap, int cmp_block, int cmp_stride, int sel_block, int n_sel, int window,
                     int force_init, int n_local, int dtype, void* stream);
+
+/* ---- residual addition with root-mean-square norm ----------------------------
+ * Replaces x + branch followed by the norm in Block.forward
+ * (nsa_model.py:449-452) for decoders whose norm is the root mean square:
+ *   h = x + res (float, rounded once to h_dtype),  y = h / sqrt(mean h^2 + eps) * w
+ * over `rows` rows of D elements at any element-aligned address.  res null:
+ * h = x (h is not written, h_dtype = x_dtype).  y_dtype NSA_E4M3: y [rows][D]
+ * bytes hold y / scale[row], scale = max(row's |y|, 2^-100) / 448 (float).
+ * rstd (float [rows], nullable): 1 / sqrt(mean h^2 + eps), for the backward.
+ * x, h / res and w are NSA_F32 or NSA_BF16, each on its own.  D <= 2^24. */
+int nsa_norm_fwd(const void* x, const void* res, const void* w, void* h, void* y, float* scale, float* rstd,
+                 int64_t rows, int D, float eps, int x_dtype, int h_dtype, int w_dtype, int y_dtype, void* stream);
+/* Its backward: dy in y_dtype, dh (nullable) the gradient of h in h_dtype; dx
+ * in x_dtype, dres (nullable: dx serves both) in h_dtype, dw (nullable) in
+ * w_dtype, summed over the rows in an order fixed by the shape.  workspace:
+ * nsa_norm_bwd_workspace bytes (0: unsupported shape); not read where dw is
+ * null. */
+size_t nsa_norm_bwd_workspace(int64_t rows, int D, void* stream);
+int nsa_norm_bwd(const void* dy, const void* dh, const void* h, const void* w, const float* rstd, void* dx, void* dres,
+                 void* dw, void* workspace, size_t workspace_bytes, int64_t rows, int D, int x_dtype, int h_dtype,
+                 int w_dtype, int y_dtype, void* stream);
+
+/* ---- log probabilities of tokens ----------------------------------------------
+ * Replaces the loss over the vocabulary (nsa_model.py:504-507) and gives what a
+ * server reports beside a token.  Logits z [rows][V] at any element-aligned
+ * address, -inf where a token is banned; per row:
+ *   logp     ln softmax(z)[target]; 0 where the target is outside 0 .. V-1
+ *   entropy  - sum p ln p (tokens of weight 0 add nothing)
+ *   top_logp, top_idx [rows][k]: the k largest, equal logits by ascending index
+ *   stat     float [rows][2]: (max z, ln sum e^(z - max)), for the backward
+ * logp and entropy may be null.  A row of -inf alone has logp -inf (and top_logp),
+ * entropy 0 and no gradient.  k <= 64, k <= V, V <= 2^28, rows <= 2^25.
+ * workspace: nsa_logprob_workspace bytes (0: unsupported shape). */
+size_t nsa_logprob_workspace(int64_t rows, int V, int k, void* stream);
+int nsa_logprob_fwd(const void* z, const int64_t* target, float* logp, float* entropy, float* stat, float* top_logp,
+                    int64_t* top_idx, void* workspace, size_t workspace_bytes, int64_t rows, int V, int k, int dtype,
+                    void* stream);
+/* dz = dlogp (1[target] - p) - dent p (ln p + entropy), in dtype; dlogp and dent
+ * float [rows], each nullable (dent needs the forward's entropy). */
+int nsa_logprob_bwd(const void* z, const int64_t* target, const float* stat, const float* entropy, const float* dlogp,
+                    const float* dent, void* dz, int64_t rows, int V, int dtype, void* stream);
+
+/* ---- one new token over a paged key-value cache -------------------------------
+ * The generation step of the dense arm (FullAttention, nsa_model.py:377-419;
+ * the reference has none).
+ *   k_pages, v_pages [n_pages][Hkv][P][D]; P a multiple of 16
+ *   table [B][max_pages] int32: the page of positions i P .. i P + P - 1
+ *   lens  [B] int32 on the device: keys held; negative: no sequence here
+ * out [B][Hq][D] = softmax(scale q K^T) V over each sequence's keys; zeros where
+ * it has none.  With k_new, v_new [B][Hkv][D]: the rows are written to
+ * position lens[b] first and attended too, lens_out[b] = lens[b] + 1; a
+ * sequence whose position has no page (past the table, or an entry outside
+ * 0 .. n_pages - 1) keeps its length and rows and attends what it holds.
+ * Keys whose table entry is outside 0 .. n_pages - 1 are not attended; rows past
+ * a length are never read.  lse (float [B][Hq], nullable): ln sum e^score, -1e9
+ * where there is no key.  lens and lens_out are different buffers.
+ * workspace: nsa_paged_workspace bytes (0: unsupported shape). */
+size_t nsa_paged_workspace(int B, int Hq, int Hkv, int D, int P, int max_pages, void* stream);
+int nsa_paged_attend(const void* q, const void* k_new, const void* v_new, void* k_pages, void* v_pages,
+                     const int32_t* table, const int32_t* lens, int32_t* lens_out, void* out, float* lse,
+                     void* workspace, size_t workspace_bytes, int B, int Hq, int Hkv, int D, int P, int max_pages,
+                     int n_pages, float scale, int dtype, void* stream);
+/* Rows [B][Hkv][T][D] of a prompt (count[b] of them, null: T) to positions
+ * lens[b] ..; lens_out[b] = lens[b] + count[b].  A sequence whose rows do not all
+ * have a page keeps its length and pages. */
+int nsa_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* table,
+                     const int32_t* lens, const int32_t* count, int32_t* lens_out, int B, int Hkv, int T, int D, int P,
+                     int max_pages, int n_pages, int dtype, void* stream);
 
 
 #ifdef __cplusplus

@@ -25,6 +25,7 @@ NSA_ERR_WORKSPACE = -5
 NSA_F32 = 0
 NSA_BF16 = 1
 NSA_F16S = 2
+NSA_E4M3 = 3
 MODE_WINDOW = 0
 MODE_COMPRESS = 1
 
@@ -32,6 +33,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
 _Z = ctypes.c_size_t
+_F = ctypes.c_float
 
 # name -> (restype, argtypes); mirrors include/nsa_hip.h
 SIGNATURES = {
@@ -100,6 +102,15 @@ SIGNATURES = {
     "nsa_decode_fwd": (_I, [_P] * 15 + [_Z] + [_I] * 14 + [_P]),
     "nsa_decode_append": (_I, [_P] * 16 + [_I] * 8 + [_P]),
     "nsa_decode_step": (_I, [_P] * 21 + [_Z] + [_I] * 14 + [_P]),
+    "nsa_norm_fwd": (_I, [_P] * 7 + [_L, _I, _F, _I, _I, _I, _I, _P]),
+    "nsa_norm_bwd_workspace": (_Z, [_L, _I, _P]),
+    "nsa_norm_bwd": (_I, [_P] * 9 + [_Z, _L, _I, _I, _I, _I, _I, _P]),
+    "nsa_logprob_workspace": (_Z, [_L, _I, _I, _P]),
+    "nsa_logprob_fwd": (_I, [_P] * 8 + [_Z, _L, _I, _I, _I, _P]),
+    "nsa_logprob_bwd": (_I, [_P] * 7 + [_L, _I, _I, _P]),
+    "nsa_paged_workspace": (_Z, [_I] * 6 + [_P]),
+    "nsa_paged_attend": (_I, [_P] * 11 + [_Z] + [_I] * 7 + [_F, _I, _P]),
+    "nsa_paged_append": (_I, [_P] * 8 + [_I] * 8 + [_P]),
 }
 
 _lib = None

@@ -1,0 +1,481 @@
+// Log probabilities of given tokens, the entropy and the best alternatives of
+// every row of logits z [rows][V], in one pass over the row, and the gradient.
+//
+//   m = max z,  l = sum e^(z-m),  s = sum e^(z-m) (z-m)
+//   logp = (z_t - m) - ln l,   H = ln l - s / l,   top: z descending, index ascending
+//   dz_j = dlogp (1[j = t] - p_j) - dH p_j (ln p_j + H),   p_j = e^(z_j - m) / l
+//
+// m is the row's own maximum, never a sentinel: it starts at the lowest finite
+// value, so that minus infinity has weight 0 against it (e^-inf) while a row
+// masked with the type's lowest value still sums to its length.  NaN and plus
+// infinity make l NaN, and with it the row's results.
+//
+// The forward reads the row once.  A lane keeps its own (m, l, s) and rescales
+// them when a run of 32 elements raises its maximum.  For the alternatives the
+// k-th largest of the lanes' maxima is a lower bound of the row's k-th value
+// (k lanes hold one such element each): elements below it are dropped, the
+// few others go to a list in LDS as (value, ~index) keys, which are all
+// different, and are ranked by counting.  The bound is formed after the
+// first chunk, which is still in registers, and again whenever the chunks done
+// have grown fourfold.  A row that overfills the list (long ties, a rising
+// row) is selected exactly by eight radix passes over the keys instead.
+//
+// One wave takes a row of up to 2048 elements; a workgroup of four takes a
+// longer one.  Where the rows are too few to fill the chip, a row is split
+// over workgroups and a second launch joins their (m, l, s) and lists.
+#include "nsa_launch.h"
+#include "nsa_rows.h"
+
+namespace nsa {
+
+constexpr int kLpTopMax = 64;        // most alternatives
+constexpr int kLpCap = 1024;         // candidate list
+constexpr float kLowest = -3.402823466e38f;
+constexpr float kFar = -1.0e30f;     // stands for the logarithm of weight 0 where it is multiplied by 0
+
+struct LpArgs {
+  const void* z;
+  const int64_t* target;   // or null
+  float *logp, *entropy;
+  float2* stat;            // (m, ln l)
+  float* top_logp;         // [rows][k]
+  int64_t* top_idx;
+  float4* part;            // [rows][nsp] (m, l, s) of a split row
+  uint64_t* part_top;      // [rows][nsp][k] keys, descending, 0 past the part's elements
+  int64_t rows;
+  int V, k, nsp, seg;      // parts a row, elements a part
+};
+
+// z's key: the order of the values, -0 with 0, NaN above infinity; ties to the lower index
+__device__ __forceinline__ uint32_t value_key(float z) {
+  return z != z ? 0xffffffffu : order_key(z + 0.0f);
+}
+__device__ __forceinline__ uint64_t elem_key(float z, int idx) {
+  return ((uint64_t)value_key(z) << 32) | (uint32_t)~idx;
+}
+__device__ __forceinline__ float key_value(uint64_t key) {
+  const uint32_t u = (uint32_t)(key >> 32);
+  return __uint_as_float((u & 0x80000000u) ? (u ^ 0x80000000u) : ~u);
+}
+
+struct LpState {
+  float m, l, s;
+};
+__device__ __forceinline__ void lp_raise(LpState& a, float m) {   // a's sums against the maximum m >= a.m
+  const float d = a.m - m;
+  const float f = fast_exp2(d * kLog2e);
+  a.l *= f;
+  a.s = a.s * f + a.l * fmaxf(d, kFar);
+  a.m = m;
+}
+__device__ __forceinline__ void lp_join(LpState& a, LpState b) {
+  const float m = fmaxf(a.m, b.m);
+  lp_raise(a, m);
+  lp_raise(b, m);
+  a.l += b.l;
+  a.s += b.s;
+}
+__device__ __forceinline__ LpState lp_wave(LpState a) {
+#pragma unroll
+  for (int x = 1; x < kWave; x <<= 1) {
+    LpState b{__shfl_xor(a.m, x, kWave), __shfl_xor(a.l, x, kWave), __shfl_xor(a.s, x, kWave)};
+    lp_join(a, b);
+  }
+  return a;
+}
+
+// Results of one row from its sums (one thread).
+__device__ __forceinline__ float lp_finish(const LpArgs& a, int64_t row, LpState st, float zt, bool has_t) {
+  const float logl = st.l == 0.0f ? -__builtin_inff() : logf(st.l);
+  a.stat[row] = make_float2(st.m, logl);
+  if (a.entropy != nullptr) a.entropy[row] = st.l == 0.0f ? 0.0f : logl - st.s / st.l;
+  if (a.logp != nullptr) a.logp[row] = has_t ? (st.l == 0.0f ? -__builtin_inff() : (zt - st.m) - logl) : 0.0f;
+  return logl;
+}
+
+// The target's logit: asked for at the start, so that its load is not waited for at the end.
+template <typename T>
+__device__ __forceinline__ bool lp_target(const LpArgs& a, int64_t row, float& zt) {
+  if (a.target == nullptr) return false;
+  const int64_t t = a.target[row];
+  if (t < 0 || t >= a.V) return false;
+  zt = (float)static_cast<const T*>(a.z)[row * a.V + t];
+  return true;
+}
+
+// The k best of the `count` keys in LDS, by rank: THR threads; place[rank] = key
+template <int THR, typename F>
+__device__ __forceinline__ void lp_rank(const uint64_t* list, int count, int k, int t, F place) {
+  for (int i = t; i < count; i += THR) {
+    const uint64_t mine = list[i];
+    int rank = 0;
+    for (int j = 0; j < count; ++j) rank += list[j] > mine ? 1 : 0;
+    if (rank < k) place(rank, mine);
+  }
+}
+
+// W waves a row (1: four rows a workgroup); U runs of 8 a lane and chunk.
+template <typename T, int W, int U, bool TOP>
+__global__ __launch_bounds__(256) void k_logprob(const LpArgs a) {
+  constexpr int THR = 64 * W;               // threads a row
+  constexpr int ROWS = 256 / THR;           // rows a workgroup
+  constexpr int CAP = W > 1 ? kLpCap : 512;
+  __shared__ uint64_t list_s[TOP ? ROWS : 1][TOP ? CAP : 1];
+  __shared__ uint32_t keys_s[TOP ? ROWS : 1][TOP ? THR : 1];
+  __shared__ uint32_t hist[TOP ? ROWS : 1][TOP ? 256 : 1];
+  __shared__ int count_s[ROWS];
+  __shared__ uint32_t thr_s[ROWS];
+  __shared__ LpState st_s[W];
+  const int t = threadIdx.x & (THR - 1), sub = threadIdx.x / THR;
+  const int64_t unit = (int64_t)blockIdx.x * ROWS + sub;
+  const int64_t row = ROWS > 1 ? unit : unit / a.nsp;
+  const int part = ROWS > 1 ? 0 : (int)(unit % a.nsp);
+  const bool live = row < a.rows;           // (whole waves; the barriers below are for every wave)
+  const int c0 = part * a.seg;
+  const int c1 = live ? min(a.V, c0 + a.seg) : c0;
+  const T* z = static_cast<const T*>(a.z) + (live ? row : 0) * a.V;
+  float zt = 0.0f;
+  const bool has_t = live && t == 0 && lp_target<T>(a, row, zt);
+  uint64_t* list = list_s[TOP ? sub : 0];
+  auto sync = [] {
+    if (W > 1)
+      __syncthreads();
+    else
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  };
+  if (TOP && t == 0) count_s[sub] = 0;
+
+  LpState st{kLowest, 0.0f, 0.0f};
+  uint32_t thr = 0;             // keys below it are no alternatives
+  float thr_z = -__builtin_inff();
+  int next = 1;                 // chunks done at the bound's next forming
+  int done = 0;
+  constexpr int CH = THR * 8 * U;
+  for (int c = c0; c < c1; c += CH) {
+    float x[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = c + 8 * (u * THR + t);
+      load_run8(z + at, c1 - at, x[u], -__builtin_inff());
+    }
+    float mx = x[0][0];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mx = fmaxf(mx, x[u][j]);
+    if (mx > st.m) lp_raise(st, mx);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float d = x[u][j] - st.m;
+        const float e = fast_exp2(d * kLog2e);
+        st.l += e;
+        st.s += e * fmaxf(d, kFar);
+      }
+    if (TOP) {
+      ++done;
+      if (done == next) {
+        // the k-th largest of the lanes' maxima
+        const bool any = c0 + 8 * t < c1;
+        // (a lane that holds NaN counts with its largest other value: still one of its elements' keys or less)
+        const uint32_t mine = any ? value_key(st.l == 0.0f ? -__builtin_inff() : st.m) : 0u;
+        keys_s[sub][t] = mine;
+        sync();
+        int rank = 0;
+        for (int i = 0; i < THR; ++i) {
+          const uint32_t o = keys_s[sub][i];
+          rank += (o > mine || (o == mine && i < t)) ? 1 : 0;
+        }
+        if (rank == a.k - 1) thr_s[sub] = mine;
+        sync();
+        thr = thr_s[sub];
+        thr_z = thr == 0u ? -__builtin_inff() : key_value((uint64_t)thr << 32);
+        next *= 4;
+      }
+      if (!(mx < thr_z) || st.l != st.l) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int at = c + 8 * (u * THR + t) + j;
+            if (at < c1 && value_key(x[u][j]) >= thr) {
+              const int i = atomicAdd(&count_s[sub], 1);
+              if (i < CAP) list[i] = elem_key(x[u][j], at);
+            }
+          }
+      }
+    }
+  }
+
+  // the row's (or the part's) sums
+  st = lp_wave(st);
+  if (W > 1) {
+    if ((threadIdx.x & 63) == 0) st_s[threadIdx.x >> 6] = st;
+    __syncthreads();
+    st = st_s[0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) lp_join(st, st_s[i]);
+  }
+  const bool split = ROWS == 1 && a.nsp > 1;
+  float logl = 0.0f;
+  if (live && t == 0 && split) a.part[row * a.nsp + part] = make_float4(st.m, st.l, st.s, 0.0f);
+  if (live && !split) {
+    if (t == 0) lp_finish(a, row, st, zt, has_t);
+    logl = st.l == 0.0f ? -__builtin_inff() : logf(st.l);
+  }
+
+  if (TOP) {
+    sync();
+    int count = count_s[sub];
+    if (count > CAP) {
+      // exact selection: the k-th key digit by digit from the top, then the keys at or above it
+      uint64_t prefix = 0;
+      int want = a.k;
+      for (int sh = 56; sh >= 0; sh -= 8) {
+        for (int i = t; i < 256; i += THR) hist[sub][i] = 0;
+        sync();
+        for (int at = c0 + t; at < c1; at += THR) {
+          const uint64_t key = elem_key((float)z[at], at);
+          if (sh == 56 || (key >> (sh + 8)) == (prefix >> (sh + 8))) atomicAdd(&hist[sub][(key >> sh) & 255], 1u);
+        }
+        sync();
+        int d = 255;      // every lane walks the digits: the same walk
+        uint32_t above = 0;
+        for (; d > 0; --d) {
+          const uint32_t n = hist[sub][d];
+          if (above + n >= (uint32_t)want) break;
+          above += n;
+        }
+        want -= (int)above;
+        prefix |= (uint64_t)d << sh;
+        sync();
+      }
+      if (t == 0) count_s[sub] = 0;
+      sync();
+      for (int at = c0 + t; at < c1; at += THR) {
+        const uint64_t key = elem_key((float)z[at], at);
+        if (key >= prefix) list[atomicAdd(&count_s[sub], 1)] = key;   // k of them: the keys are all different
+      }
+      sync();
+      count = a.k;
+    }
+    if (live) {
+      if (split) {
+        uint64_t* out = a.part_top + (row * a.nsp + part) * a.k;
+        for (int i = count + t; i < a.k; i += THR) out[i] = 0;
+        lp_rank<THR>(list, count, a.k, t, [&](int r, uint64_t key) { out[r] = key; });
+      } else {
+        lp_rank<THR>(list, count, a.k, t, [&](int r, uint64_t key) {
+          a.top_logp[row * a.k + r] = st.l == 0.0f ? -__builtin_inff() : (key_value(key) - st.m) - logl;
+          a.top_idx[row * a.k + r] = (int64_t)(uint32_t)~(uint32_t)key;
+        });
+      }
+    }
+  }
+}
+
+// Joins the parts of split rows: one workgroup a row.
+template <typename T>
+__global__ __launch_bounds__(256) void k_logprob_join(const LpArgs a) {
+  extern __shared__ uint64_t jlist[];
+  __shared__ LpState st_s[4];
+  const int64_t row = blockIdx.x;
+  const int t = threadIdx.x;
+  float zt = 0.0f;
+  const bool has_t = t == 0 && lp_target<T>(a, row, zt);
+  LpState st{kLowest, 0.0f, 0.0f};
+  for (int i = t; i < a.nsp; i += 256) {
+    const float4 p = a.part[row * a.nsp + i];
+    lp_join(st, LpState{p.x, p.y, p.z});
+  }
+  const int n = a.nsp * a.k;
+  for (int i = t; i < n; i += 256) jlist[i] = a.part_top[row * n + i];
+  st = lp_wave(st);
+  if ((t & 63) == 0) st_s[t >> 6] = st;
+  __syncthreads();
+  st = st_s[0];
+#pragma unroll
+  for (int i = 1; i < 4; ++i) lp_join(st, st_s[i]);
+  const float logl = st.l == 0.0f ? -__builtin_inff() : logf(st.l);
+  if (t == 0) lp_finish(a, row, st, zt, has_t);
+  for (int i = t; i < n; i += 256) {
+    const uint64_t mine = jlist[i];
+    if (mine == 0) continue;
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += jlist[j] > mine ? 1 : 0;
+    if (rank < a.k) {
+      a.top_logp[row * a.k + rank] = st.l == 0.0f ? -__builtin_inff() : (key_value(mine) - st.m) - logl;
+      a.top_idx[row * a.k + rank] = (int64_t)(uint32_t)~(uint32_t)mine;
+    }
+  }
+}
+
+struct LpBwdArgs {
+  const void* z;
+  const int64_t* target;        // or null
+  const float2* stat;
+  const float *entropy, *dlogp, *dent;   // dlogp, dent: or null
+  void* dz;
+  int64_t rows;
+  int V, units;                 // units of a row
+};
+
+constexpr int kLpBwdRuns = 4;
+constexpr int kLpBwdUnit = 64 * 8 * kLpBwdRuns;   // elements a wave takes
+
+template <typename T, bool ENT>
+__global__ __launch_bounds__(256) void k_logprob_bwd(const LpBwdArgs a) {
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t row = unit / a.units;
+  if (row >= a.rows) return;
+  const int lane = threadIdx.x & 63;
+  const int c = (int)(unit % a.units) * kLpBwdUnit + 8 * lane;
+  const T* z = static_cast<const T*>(a.z) + row * a.V;
+  T* dz = static_cast<T*>(a.dz) + row * a.V;
+  int64_t tg = a.target == nullptr ? -1 : a.target[row];
+  const float2 st = a.stat[row];
+  const bool empty = st.y == -__builtin_inff();   // nothing in the row: no gradient
+  const float dl = a.dlogp == nullptr || tg < 0 || tg >= a.V || empty ? 0.0f : a.dlogp[row];
+  if (dl == 0.0f) tg = -1;
+  const float dh = ENT && !empty ? a.dent[row] : 0.0f;
+  const bool zero = dl == 0.0f && dh == 0.0f;
+  const float log2l = st.y * kLog2e;
+  const float hh = ENT ? a.entropy[row] - st.y : 0.0f;
+  float x[kLpBwdRuns][8];
+  if (!zero) {
+#pragma unroll
+    for (int u = 0; u < kLpBwdRuns; ++u) {
+      const int at = c + 512 * u;
+      load_run8(z + at, a.V - at, x[u]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kLpBwdRuns; ++u) {
+    const int at = c + 512 * u;
+    if (at >= a.V) break;
+    float d[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (zero) {
+        d[j] = 0.0f;
+      } else {
+        const float y = x[u][j] - st.x;
+        const float p = fast_exp2(y * kLog2e - log2l);
+        d[j] = ENT ? -p * (dl + dh * (fmaxf(y, kFar) + hh)) : -p * dl;
+      }
+      if (tg == at + j) d[j] += dl;
+    }
+    store_run8(dz + at, a.V - at, d);
+  }
+}
+
+// Parts of a row: as many as bring the launch to four workgroups a compute
+// unit, each a whole number of 2048-element chunks; at most as many as the
+// join's list in LDS holds.
+static int lp_parts(int64_t rows, int V, int k, int cu) {
+  if (V <= 2048) return 1;
+  int64_t want = (4LL * cu + rows - 1) / rows;
+  const int chunks = (V + 2047) / 2048;
+  if (want > chunks) want = chunks;
+  const int most = k > 0 ? (4096 / k < 64 ? 4096 / k : 64) : 64;
+  if (want > most) want = most;
+  if (want <= 1) return 1;
+  const int per = (int)((chunks + want - 1) / want);
+  return (chunks + per - 1) / per;
+}
+static int lp_seg(int V, int nsp) {
+  if (nsp <= 1) return V;
+  const int chunks = (V + 2047) / 2048;
+  return ((chunks + nsp - 1) / nsp) * 2048;
+}
+
+template <typename T>
+static int logprob_launch(LpArgs a, hipStream_t s) {
+  if (a.V <= 2048) {
+    const int64_t grid = (a.rows + 3) / 4;
+    if (a.k > 0)
+      k_logprob<T, 1, 4, true><<<(unsigned)grid, 256, 0, s>>>(a);
+    else
+      k_logprob<T, 1, 4, false><<<(unsigned)grid, 256, 0, s>>>(a);
+    return nsa_launch_status();
+  }
+  const int64_t grid = a.rows * a.nsp;
+  // a part of one or two chunks takes its elements as runs of its own chunks; a long row four runs at a time
+  const bool small = a.seg <= 4096;
+  if (a.k > 0) {
+    if (small)
+      k_logprob<T, 4, 1, true><<<(unsigned)grid, 256, 0, s>>>(a);
+    else
+      k_logprob<T, 4, 4, true><<<(unsigned)grid, 256, 0, s>>>(a);
+  } else {
+    if (small)
+      k_logprob<T, 4, 1, false><<<(unsigned)grid, 256, 0, s>>>(a);
+    else
+      k_logprob<T, 4, 4, false><<<(unsigned)grid, 256, 0, s>>>(a);
+  }
+  if (a.nsp > 1) k_logprob_join<T><<<(unsigned)a.rows, 256, (size_t)a.nsp * a.k * 8, s>>>(a);
+  return nsa_launch_status();
+}
+
+}  // namespace nsa
+
+static bool lp_shape_ok(int64_t rows, int V, int k) {
+  return rows >= 0 && rows <= (1LL << 25) && V >= 1 && V <= (1 << 28) && k >= 0 && k <= nsa::kLpTopMax && k <= V;
+}
+
+extern "C" size_t nsa_logprob_workspace(int64_t rows, int V, int k, void* stream) {
+  using namespace nsa;
+  if (!lp_shape_ok(rows, V, k)) return 0;
+  if (rows == 0) return 16;
+  const int nsp = lp_parts(rows, V, k, device_cu_count(static_cast<hipStream_t>(stream)));
+  return nsp <= 1 ? 16 : (size_t)rows * nsp * (16 + 8 * (size_t)k);
+}
+
+extern "C" int nsa_logprob_fwd(const void* z, const int64_t* target, float* logp, float* entropy, float* stat,
+                               float* top_logp, int64_t* top_idx, void* workspace, size_t workspace_bytes,
+                               int64_t rows, int V, int k, int dtype, void* stream) {
+  using namespace nsa;
+  NSA_CHECK(lp_shape_ok(rows, V, k), NSA_ERR_SHAPE);
+  NSA_CHECK(dtype == NSA_F32 || dtype == NSA_BF16, NSA_ERR_DTYPE);
+  if (rows == 0) return NSA_OK;
+  NSA_CHECK(z != nullptr && stat != nullptr && (logp == nullptr || target != nullptr), NSA_ERR_ARG);
+  NSA_CHECK(k == 0 || (top_logp != nullptr && top_idx != nullptr), NSA_ERR_ARG);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const int nsp = lp_parts(rows, V, k, device_cu_count(s));
+  LpArgs a{z, target, logp, entropy, reinterpret_cast<float2*>(stat), top_logp, top_idx, nullptr, nullptr, rows, V,
+           k, nsp, lp_seg(V, nsp)};
+  if (nsp > 1) {
+    NSA_CHECK(workspace != nullptr && workspace_bytes >= (size_t)rows * nsp * (16 + 8 * (size_t)k), NSA_ERR_WORKSPACE);
+    a.part = static_cast<float4*>(workspace);
+    a.part_top = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + (size_t)rows * nsp * 16);
+  }
+  return dtype == NSA_BF16 ? logprob_launch<bf16>(a, s) : logprob_launch<float>(a, s);
+}
+
+extern "C" int nsa_logprob_bwd(const void* z, const int64_t* target, const float* stat, const float* entropy,
+                               const float* dlogp, const float* dent, void* dz, int64_t rows, int V, int dtype,
+                               void* stream) {
+  using namespace nsa;
+  NSA_CHECK(lp_shape_ok(rows, V, 0), NSA_ERR_SHAPE);
+  NSA_CHECK(dtype == NSA_F32 || dtype == NSA_BF16, NSA_ERR_DTYPE);
+  if (rows == 0) return NSA_OK;
+  NSA_CHECK(z != nullptr && stat != nullptr && dz != nullptr && (dent == nullptr || entropy != nullptr), NSA_ERR_ARG);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const int units = (V + kLpBwdUnit - 1) / kLpBwdUnit;
+  const int64_t grid = (rows * units + 3) / 4;
+  NSA_CHECK(grid <= 0x7fffffffLL, NSA_ERR_SHAPE);
+  const LpBwdArgs a{z, target, reinterpret_cast<const float2*>(stat), entropy, dlogp, dent, dz, rows, V, units};
+  if (dtype == NSA_BF16) {
+    if (dent != nullptr)
+      k_logprob_bwd<bf16, true><<<(unsigned)grid, 256, 0, s>>>(a);
+    else
+      k_logprob_bwd<bf16, false><<<(unsigned)grid, 256, 0, s>>>(a);
+  } else {
+    if (dent != nullptr)
+      k_logprob_bwd<float, true><<<(unsigned)grid, 256, 0, s>>>(a);
+    else
+      k_logprob_bwd<float, false><<<(unsigned)grid, 256, 0, s>>>(a);
+  }
+  return nsa_launch_status();
+}

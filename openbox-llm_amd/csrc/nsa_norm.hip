@@ -1,0 +1,445 @@
+// Residual addition with root-mean-square norm, rows of D elements:
+//
+//   h = x + r  (float32, rounded once to r's type; h = x without a residual)
+//   rstd = 1 / sqrt(mean_j h_j^2 + eps),   y = (h rstd) w
+//
+// or, with the output in 8 bits, q = e4m3(y 448 / amax), scale = amax / 448
+// with amax the row's largest |y| (at least 2^-100: a row of zeros has a finite
+// scale).  The norm is taken of the stored h, so that the backward recomputes
+// it from what the forward left.  With g = dy w:
+//
+//   dh = dh_out + rstd (g - n mean_j(g_j n_j)),  n = h rstd;   dx = dr = dh;   dw = sum over rows of dy n
+//
+// Every kernel is bound by the bytes it moves: one read of x and r (dy, dh_out
+// and h in the backward), one write of h and y (dx, dr).  A row stays in
+// registers between its reduction and its output, so nothing is read twice
+// (past 32768 elements a row is read again, through the cache).
+//
+// Threads per row: one wave up to 2048 elements (no barrier at all), 256 or
+// 1024 threads above, in runs of 8 elements.  Where the rows are too few to
+// fill the chip, a row takes as many threads as it has runs.
+//
+// The backward's workgroups walk over rows in a stride of the grid and keep
+// their columns' part of dw in registers; the parts are added in workgroup
+// order by a second launch, so that dw has the same bits on every run.
+#include "nsa_launch.h"
+#include "nsa_rows.h"
+
+namespace nsa {
+
+constexpr float kQ8Max = 448.0f;            // largest e4m3 value
+constexpr float kQ8Floor = 0x1p-100f;
+constexpr int kNormWaveMax = 2048;           // widest row of one wave
+constexpr int kNormRegMax = 32768;           // widest row held in registers
+constexpr int kNormMax = 1 << 24;            // widest row
+
+struct NormArgs {
+  const void *x, *res, *w;
+  void *h, *y;
+  float *scale, *rstd;
+  int64_t rows;
+  int D;
+  float eps, inv_d;
+  bool w_bf16, y_bf16;
+};
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// 8 floats as e4m3 (round to nearest even; |v| <= 448 but for NaN)
+__device__ __forceinline__ void store_q8(uint8_t* p, int n, const float (&f)[8]) {
+  typedef uint32_t u32x2u __attribute__((ext_vector_type(2), aligned(1)));
+  int a = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
+  a = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], a, true);
+  int b = __builtin_amdgcn_cvt_pk_fp8_f32(f[4], f[5], 0, false);
+  b = __builtin_amdgcn_cvt_pk_fp8_f32(f[6], f[7], b, true);
+  if (n >= 8) {
+    *reinterpret_cast<u32x2u*>(p) = (u32x2u){(uint32_t)a, (uint32_t)b};
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) p[j] = (uint8_t)((uint32_t)(j < 4 ? a : b) >> (8 * (j & 3)));
+  }
+}
+
+// h of one run: x + r rounded to r's type (RES), or x itself
+template <typename XT, typename RT, bool RES>
+__device__ __forceinline__ void norm_sum8(const NormArgs& a, int64_t at, int n, float (&h)[8]) {
+  load_run8(static_cast<const XT*>(a.x) + at, n, h);
+  if (RES) {
+    float r[8];
+    load_run8(static_cast<const RT*>(a.res) + at, n, r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[j] = (float)(RT)(h[j] + r[j]);
+  }
+}
+
+// TPR threads a row, NV runs of 8 a thread (NV = 0: any length, h formed again for every pass).
+template <typename XT, typename RT, bool RES, bool Q8, int TPR, int NV>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(const NormArgs a) {
+  constexpr int W = TPR / kWave;
+  __shared__ float red[2][W];
+  __shared__ uint32_t redm[W];
+  const int t = threadIdx.x & (TPR - 1);
+  const int64_t row = TPR < 256 ? (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR : (int64_t)blockIdx.x;
+  if (TPR < 256 && row >= a.rows) return;   // whole waves; no barrier follows for TPR == 64
+  const int D = a.D;
+  const int64_t base = row * D;
+  const int nrun = NV > 0 ? NV : (D + 8 * TPR - 1) / (8 * TPR);
+  float h[NV > 0 ? NV : 1][8];
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < nrun; ++i) {
+    float(&hi)[8] = h[NV > 0 ? i : 0];
+    const int c = 8 * (i * TPR + t), n = D - c;
+    norm_sum8<XT, RT, RES>(a, base + c, n, hi);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss += hi[j] * hi[j];
+    if (RES && n > 0) store_run8(static_cast<RT*>(a.h) + base + c, n, hi);
+  }
+  ss = group_sum<W>(ss, red[0]);
+  const float rstd = 1.0f / sqrtf(ss * a.inv_d + a.eps);
+  if (a.rstd != nullptr && t == 0) a.rstd[row] = rstd;
+  uint32_t am = 0;   // |y| as bits: the order of the magnitudes, NaN above infinity
+#pragma unroll
+  for (int i = 0; i < nrun; ++i) {
+    float(&hi)[8] = h[NV > 0 ? i : 0];
+    const int c = 8 * (i * TPR + t), n = D - c;
+    if (NV == 0) norm_sum8<XT, RT, RES>(a, base + c, n, hi);
+    float wv[8];
+    load_run8_of(a.w, a.w_bf16, c, n, wv);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      hi[j] = (hi[j] * rstd) * wv[j];
+      if (Q8 && j < n) am = max(am, abs_bits(hi[j]));
+    }
+    if (!Q8 && n > 0) {
+      if (a.y_bf16)
+        store_run8(static_cast<bf16*>(a.y) + base + c, n, hi);
+      else
+        store_run8(static_cast<float*>(a.y) + base + c, n, hi);
+    }
+  }
+  if (Q8) {
+    am = wave_reduce_u32<true>(am);
+    if (W > 1) {
+      if ((threadIdx.x & (kWave - 1)) == 0) redm[threadIdx.x / kWave] = am;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < W; ++i) am = max(am, redm[i]);
+    }
+    const float amax = __uint_as_float(max(am, __float_as_uint(kQ8Floor)));
+    const float inv = kQ8Max / amax;
+    if (t == 0) a.scale[row] = amax / kQ8Max;
+#pragma unroll
+    for (int i = 0; i < nrun; ++i) {
+      float(&hi)[8] = h[NV > 0 ? i : 0];
+      const int c = 8 * (i * TPR + t), n = D - c;
+      if (NV == 0) {
+        norm_sum8<XT, RT, RES>(a, base + c, n, hi);
+        float wv[8];
+        load_run8_of(a.w, a.w_bf16, c, n, wv);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) hi[j] = (hi[j] * rstd) * wv[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) hi[j] *= inv;
+      if (n > 0) store_q8(static_cast<uint8_t*>(a.y) + base + c, n, hi);
+    }
+  }
+}
+
+struct NormBwdArgs {
+  const void *dy, *dh, *h, *w;
+  const float* rstd;
+  void *dx, *dres;
+  float* part;            // [gridDim.x][D], or null
+  int64_t rows;
+  int D;
+  float inv_d;
+  bool w_bf16, dx_bf16;
+};
+
+// YT: dy; RT: h, dh and dres.  dres is null where dx serves both (one type).
+template <typename YT, typename RT, int TPR, int NV>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormBwdArgs a) {
+  constexpr int W = TPR / kWave;
+  constexpr int RPG = TPR < 256 ? 256 / TPR : 1;   // rows at a time
+  __shared__ float red[2][W];
+  __shared__ float dws[TPR < 256 ? 2048 : 1];
+  const int t = threadIdx.x & (TPR - 1);
+  const int sub = threadIdx.x / TPR;
+  const int D = a.D;
+  float w[NV][8], dw[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    load_run8_of(a.w, a.w_bf16, 8 * (i * TPR + t), D - 8 * (i * TPR + t), w[i]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dw[i][j] = 0.0f;
+  }
+  int turn = 0;
+  for (int64_t row = (int64_t)blockIdx.x * RPG + sub; row < a.rows; row += (int64_t)gridDim.x * RPG) {
+    const int64_t base = row * D;
+    const float rstd = a.rstd[row];
+    float n_[NV][8], g[NV][8];
+    float dot = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + t), n = D - c;
+      load_run8(static_cast<const RT*>(a.h) + base + c, n, n_[i]);
+      load_run8(static_cast<const YT*>(a.dy) + base + c, n, g[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        n_[i][j] *= rstd;
+        dw[i][j] += g[i][j] * n_[i][j];
+        g[i][j] *= w[i][j];
+        dot += g[i][j] * n_[i][j];
+      }
+    }
+    // two buffers in turn: the next row's sum is not written over one still being read
+    dot = group_sum<W>(dot, red[turn & 1]) * a.inv_d;
+    ++turn;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + t), n = D - c;
+      float d[8];
+      if (a.dh != nullptr) {
+        load_run8(static_cast<const RT*>(a.dh) + base + c, n, d);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] = 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[j] += rstd * (g[i][j] - n_[i][j] * dot);
+      if (n > 0) {
+        if (a.dx_bf16)
+          store_run8(static_cast<bf16*>(a.dx) + base + c, n, d);
+        else
+          store_run8(static_cast<float*>(a.dx) + base + c, n, d);
+        if (a.dres != nullptr) store_run8(static_cast<RT*>(a.dres) + base + c, n, d);
+      }
+    }
+  }
+  if (a.part == nullptr) return;
+  float* out = a.part + (int64_t)blockIdx.x * D;
+  if constexpr (RPG == 1) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + t);
+      if (c < D) store_run8(out + c, D - c, dw[i]);
+    }
+  } else {
+    // the waves' parts, added in wave order
+    for (int s = 0; s < RPG; ++s) {
+      if (sub == s) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int c = 8 * (i * TPR + t) + j;
+            if (c < D) dws[c] = s == 0 ? dw[i][j] : dws[c] + dw[i][j];
+          }
+        }
+      }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < D; c += 256) out[c] = dws[c];
+  }
+}
+
+// Rows past kNormRegMax: one workgroup a row, read twice.
+template <typename YT, typename RT>
+__global__ __launch_bounds__(1024) void k_norm_bwd_long(const NormBwdArgs a) {
+  __shared__ float red[16];
+  const int64_t row = blockIdx.x;
+  const int D = a.D;
+  const int64_t base = row * D;
+  const float rstd = a.rstd[row];
+  float dot = 0.0f;
+  for (int c = 8 * threadIdx.x; c < D; c += 8 * 1024) {
+    float h[8], g[8], w[8];
+    load_run8(static_cast<const RT*>(a.h) + base + c, D - c, h);
+    load_run8(static_cast<const YT*>(a.dy) + base + c, D - c, g);
+    load_run8_of(a.w, a.w_bf16, c, D - c, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dot += g[j] * w[j] * (h[j] * rstd);
+  }
+  dot = group_sum<16>(dot, red) * a.inv_d;
+  for (int c = 8 * threadIdx.x; c < D; c += 8 * 1024) {
+    const int n = D - c;
+    float h[8], g[8], w[8], d[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    load_run8(static_cast<const RT*>(a.h) + base + c, n, h);
+    load_run8(static_cast<const YT*>(a.dy) + base + c, n, g);
+    load_run8_of(a.w, a.w_bf16, c, n, w);
+    if (a.dh != nullptr) load_run8(static_cast<const RT*>(a.dh) + base + c, n, d);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) d[j] += rstd * (g[j] * w[j] - h[j] * rstd * dot);
+    if (a.dx_bf16)
+      store_run8(static_cast<bf16*>(a.dx) + base + c, n, d);
+    else
+      store_run8(static_cast<float*>(a.dx) + base + c, n, d);
+    if (a.dres != nullptr) store_run8(static_cast<RT*>(a.dres) + base + c, n, d);
+  }
+}
+
+// dw of rows past kNormRegMax: a thread a column, the rows in order.
+template <typename YT, typename RT>
+__global__ __launch_bounds__(256) void k_norm_dw_long(const NormBwdArgs a, void* dw) {
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c >= a.D) return;
+  float s = 0.0f;
+  for (int64_t r = 0; r < a.rows; ++r)
+    s += (float)static_cast<const YT*>(a.dy)[r * a.D + c] *
+         ((float)static_cast<const RT*>(a.h)[r * a.D + c] * a.rstd[r]);
+  if (a.w_bf16)
+    static_cast<bf16*>(dw)[c] = (bf16)s;
+  else
+    static_cast<float*>(dw)[c] = s;
+}
+
+// dw[c] = sum of part[p][c], p ascending within each of 16 interleaved sums, those in order
+__global__ __launch_bounds__(1024) void k_norm_dw(const float* __restrict__ part, int nparts, int D, void* dw,
+                                                  bool w_bf16) {
+  __shared__ float acc[16][64];
+  const int lane = threadIdx.x & 63, s = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + lane;
+  float v = 0.0f;
+  if (c < D)
+    for (int p = s; p < nparts; p += 16) v += part[(int64_t)p * D + c];
+  acc[s][lane] = v;
+  __syncthreads();
+  if (s == 0 && c < D) {
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += acc[i][lane];
+    if (w_bf16)
+      static_cast<bf16*>(dw)[c] = (bf16)t;
+    else
+      static_cast<float*>(dw)[c] = t;
+  }
+}
+
+// Threads a row and runs a thread.  A row takes the fewest threads that hold
+// it (one wave to 2048 elements, 256 threads to 8192, 1024 above), which keeps
+// several rows in flight on a compute unit; fewer rows than compute units
+// take as many threads as they have runs.
+struct NormShape {
+  int tpr, nv;
+};
+static NormShape norm_shape(int64_t rows, int D, int cu) {
+  const int runs = (D + 7) / 8;
+  int tpr = D <= kNormWaveMax ? 64 : D <= 8192 ? 256 : 1024;
+  if (rows <= cu) tpr = runs <= 64 ? 64 : runs <= 256 ? 256 : 1024;
+  if (D > kNormRegMax) return {1024, 0};
+  const int nv = (runs + tpr - 1) / tpr;
+  return {tpr, nv == 3 ? (tpr == 64 ? 3 : 4) : nv};
+}
+
+template <typename XT, typename RT, bool RES, bool Q8>
+static int norm_fwd_launch(const NormArgs& a, hipStream_t s) {
+  const NormShape sh = norm_shape(a.rows, a.D, device_cu_count(s));
+#define NSA_NORM_CASE(TPR, NV)                                                                             \
+  if (sh.tpr == TPR && sh.nv == NV) {                                                                      \
+    const int64_t grid = TPR < 256 ? (a.rows + 256 / TPR - 1) / (256 / TPR) : a.rows;                      \
+    k_norm_fwd<XT, RT, RES, Q8, TPR, NV><<<(unsigned)grid, TPR < 256 ? 256 : TPR, 0, s>>>(a);              \
+    return nsa_launch_status();                                                                            \
+  }
+  NSA_NORM_CASE(64, 1) NSA_NORM_CASE(64, 2) NSA_NORM_CASE(64, 3) NSA_NORM_CASE(64, 4)
+  NSA_NORM_CASE(256, 1) NSA_NORM_CASE(256, 2) NSA_NORM_CASE(256, 4)
+  NSA_NORM_CASE(1024, 1) NSA_NORM_CASE(1024, 2) NSA_NORM_CASE(1024, 4) NSA_NORM_CASE(1024, 0)
+#undef NSA_NORM_CASE
+  return NSA_ERR_SHAPE;
+}
+
+template <typename XT, typename RT>
+static int norm_fwd_as(const NormArgs& a, bool q8, hipStream_t s) {
+  if (a.res != nullptr) return q8 ? norm_fwd_launch<XT, RT, true, true>(a, s) : norm_fwd_launch<XT, RT, true, false>(a, s);
+  if constexpr (sizeof(XT) == sizeof(RT))
+    return q8 ? norm_fwd_launch<XT, RT, false, true>(a, s) : norm_fwd_launch<XT, RT, false, false>(a, s);
+  return NSA_ERR_DTYPE;
+}
+
+// Workgroups of the backward: four to a compute unit, each with a part of dw.
+static int64_t norm_bwd_groups(int64_t rows, int D, int cu) {
+  const NormShape sh = norm_shape(rows, D, cu);
+  const int64_t groups = sh.tpr == 64 ? (rows + 3) / 4 : rows;
+  const int64_t most = (int64_t)cu * (sh.tpr == 1024 ? 2 : 4);
+  return groups < most ? groups : most;
+}
+
+template <typename YT, typename RT>
+static int norm_bwd_launch(NormBwdArgs a, void* dw, hipStream_t s) {
+  const int cu = device_cu_count(s);
+  const NormShape sh = norm_shape(a.rows, a.D, cu);
+  if (sh.nv == 0) {
+    k_norm_bwd_long<YT, RT><<<(unsigned)a.rows, 1024, 0, s>>>(a);
+    if (dw != nullptr) k_norm_dw_long<YT, RT><<<(unsigned)((a.D + 255) / 256), 256, 0, s>>>(a, dw);
+    return nsa_launch_status();
+  }
+  const int64_t grid = norm_bwd_groups(a.rows, a.D, cu);
+  bool done = false;
+#define NSA_NORM_CASE(TPR, NV)                                                                        \
+  if (sh.tpr == TPR && sh.nv == NV) {                                                                 \
+    k_norm_bwd<YT, RT, TPR, NV><<<(unsigned)grid, TPR < 256 ? 256 : TPR, 0, s>>>(a);                  \
+    done = true;                                                                                      \
+  }
+  NSA_NORM_CASE(64, 1) NSA_NORM_CASE(64, 2) NSA_NORM_CASE(64, 3) NSA_NORM_CASE(64, 4)
+  NSA_NORM_CASE(256, 1) NSA_NORM_CASE(256, 2) NSA_NORM_CASE(256, 4)
+  NSA_NORM_CASE(1024, 1) NSA_NORM_CASE(1024, 2) NSA_NORM_CASE(1024, 4)
+#undef NSA_NORM_CASE
+  if (!done) return NSA_ERR_SHAPE;
+  if (dw != nullptr)
+    k_norm_dw<<<(unsigned)((a.D + 63) / 64), 1024, 0, s>>>(a.part, (int)grid, a.D, dw, a.w_bf16);
+  return nsa_launch_status();
+}
+
+static bool norm_type(int dtype) { return dtype == NSA_F32 || dtype == NSA_BF16; }
+
+}  // namespace nsa
+
+extern "C" int nsa_norm_fwd(const void* x, const void* res, const void* w, void* h, void* y, float* scale,
+                            float* rstd, int64_t rows, int D, float eps, int x_dtype, int h_dtype, int w_dtype,
+                            int y_dtype, void* stream) {
+  using namespace nsa;
+  NSA_CHECK(rows >= 0 && rows <= 0x7fffffffLL && D >= 1 && D <= kNormMax, NSA_ERR_SHAPE);
+  NSA_CHECK(norm_type(x_dtype) && norm_type(h_dtype) && norm_type(w_dtype), NSA_ERR_DTYPE);
+  NSA_CHECK(norm_type(y_dtype) || y_dtype == NSA_E4M3, NSA_ERR_DTYPE);
+  NSA_CHECK(res != nullptr || x_dtype == h_dtype, NSA_ERR_DTYPE);
+  if (rows == 0) return NSA_OK;
+  NSA_CHECK(x != nullptr && w != nullptr && y != nullptr, NSA_ERR_ARG);
+  NSA_CHECK(res == nullptr || h != nullptr, NSA_ERR_ARG);
+  NSA_CHECK(y_dtype != NSA_E4M3 || scale != nullptr, NSA_ERR_ARG);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const NormArgs a{x, res, w, h, y, scale, rstd, rows, D, eps, 1.0f / (float)D, w_dtype == NSA_BF16,
+                   y_dtype == NSA_BF16};
+  const bool q8 = y_dtype == NSA_E4M3;
+  if (x_dtype == NSA_BF16)
+    return h_dtype == NSA_BF16 ? norm_fwd_as<bf16, bf16>(a, q8, s) : norm_fwd_as<bf16, float>(a, q8, s);
+  return h_dtype == NSA_BF16 ? norm_fwd_as<float, bf16>(a, q8, s) : norm_fwd_as<float, float>(a, q8, s);
+}
+
+extern "C" size_t nsa_norm_bwd_workspace(int64_t rows, int D, void* stream) {
+  using namespace nsa;
+  if (rows < 0 || rows > 0x7fffffffLL || D < 1 || D > kNormMax) return 0;
+  if (rows == 0 || D > kNormRegMax) return 16;
+  return (size_t)norm_bwd_groups(rows, D, device_cu_count(static_cast<hipStream_t>(stream))) * D * sizeof(float);
+}
+
+extern "C" int nsa_norm_bwd(const void* dy, const void* dh, const void* h, const void* w, const float* rstd, void* dx,
+                            void* dres, void* dw, void* workspace, size_t workspace_bytes, int64_t rows, int D,
+                            int x_dtype, int h_dtype, int w_dtype, int y_dtype, void* stream) {
+  using namespace nsa;
+  NSA_CHECK(rows >= 1 && rows <= 0x7fffffffLL && D >= 1 && D <= kNormMax, NSA_ERR_SHAPE);
+  NSA_CHECK(norm_type(x_dtype) && norm_type(h_dtype) && norm_type(w_dtype) && norm_type(y_dtype), NSA_ERR_DTYPE);
+  NSA_CHECK(dy != nullptr && h != nullptr && w != nullptr && rstd != nullptr && dx != nullptr, NSA_ERR_ARG);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  float* part = nullptr;
+  if (dw != nullptr && D <= kNormRegMax) {
+    NSA_CHECK(workspace != nullptr && workspace_bytes >= nsa_norm_bwd_workspace(rows, D, stream), NSA_ERR_WORKSPACE);
+    part = static_cast<float*>(workspace);
+  }
+  const NormBwdArgs a{dy, dh, h, w, rstd, dx, dres, part, rows, D, 1.0f / (float)D, w_dtype == NSA_BF16,
+                      x_dtype == NSA_BF16};
+  if (y_dtype == NSA_BF16)
+    return h_dtype == NSA_BF16 ? norm_bwd_launch<bf16, bf16>(a, dw, s) : norm_bwd_launch<bf16, float>(a, dw, s);
+  return h_dtype == NSA_BF16 ? norm_bwd_launch<float, bf16>(a, dw, s) : norm_bwd_launch<float, float>(a, dw, s);
+}

@@ -144,6 +144,14 @@ def _lib():
     return L.load()
 
 
+def device_of(t):
+    """Context in which t's device is the current one (launches, stream and
+    device queries then go there)."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
 def _stream(t):
     return L.stream_of(t)
 

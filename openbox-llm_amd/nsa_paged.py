@@ -1,0 +1,230 @@
+"""Generation over a paged key-value cache on MI355X: one new token of every
+sequence against keys and values that lie in pages.
+
+The reference runs whole sequences only (FullAttention.forward,
+nsa_model.py:377-419).  A step here computes that function's newest row for
+every sequence of a batch.
+
+* ``paged_step`` appends the new tokens' key and value rows and attends;
+  ``paged_attend`` attends alone; ``paged_append`` writes a prompt's rows.
+* ``PagedKVCache`` holds one layer's pages, the page table and the lengths, and
+  hands pages out to sequences as they grow.
+
+Layout: ``k_pages, v_pages [n_pages, Hkv, page, D]`` (float32 or bfloat16,
+``page`` a multiple of 16, ``D`` in 16, 32, 64, 128), ``table [B, max_pages]``
+int32 (the page that holds positions ``i page ..``) and ``lens [B]`` int32, all
+on the device: a generation loop never waits for the host, and a step can be
+captured into a graph.  Query head h reads KV head ``h // (Hq // Hkv)``.
+
+Table entries outside ``0 .. n_pages-1`` are no pages: keys there are not
+attended and rows are not written.  Rows past a length are never read.  A
+negative length stands for no sequence: its output is zeros, its length stays.
+"""
+
+import torch
+
+import _nsa_lib as L
+import nsa_hip_ops as _ops
+
+
+def _check_pages(k_pages, v_pages, table, lens):
+    assert k_pages.dim() == 4 and k_pages.is_cuda, "paged: pages must be [n_pages, Hkv, page, D] on the GPU"
+    assert v_pages.shape == k_pages.shape and v_pages.dtype == k_pages.dtype and v_pages.device == k_pages.device, \
+        "paged: key and value pages differ in shape, dtype or device"
+    n, Hkv, P, D = k_pages.shape
+    assert n >= 1 and Hkv >= 1 and P >= 16 and P % 16 == 0, "paged: the page size must be a multiple of 16"
+    assert D in (16, 32, 64, 128), "head dim must be a power of two <= 128"
+    assert k_pages.dtype in (torch.float32, torch.bfloat16), \
+        f"dtype {k_pages.dtype} is not supported (float32 or bfloat16)"
+    for p in (k_pages, v_pages):
+        assert p.is_contiguous() and p.data_ptr() % 16 == 0, "paged: pages must be dense and 16-byte aligned"
+    assert table.dim() == 2 and table.dtype == torch.int32 and table.device == k_pages.device, \
+        "paged: table int32 [B, max_pages] on the pages' device"
+    assert table.shape[1] >= 1 and table.shape[1] * P <= 1 << 30, "paged: table of 1 page to 2^30 positions"
+    assert lens.dtype == torch.int32 and lens.shape == table.shape[:1] and lens.device == k_pages.device, \
+        "paged: lens int32 [B] on the pages' device"
+
+
+def _attend(q, rows, k_pages, v_pages, table, lens, scale, return_lse):
+    _check_pages(k_pages, v_pages, table, lens)
+    n, Hkv, P, D = k_pages.shape
+    B, mp = table.shape
+    assert q.dim() == 3 and q.shape[0] == B and q.shape[2] == D, "paged: q must be [B, Hq, D]"
+    assert q.dtype == k_pages.dtype and q.device == k_pages.device, "paged: q in the pages' dtype and device"
+    Hq = q.shape[1]
+    assert Hq >= 1 and Hq % Hkv == 0, "GQA needs n_q_heads divisible by n_kv_heads"
+    assert Hq <= 4096 and B <= 65536, "paged: at most 4096 heads and 65536 sequences"
+    q, table, lens = _ops._contig(q), table.contiguous(), lens.contiguous()
+    kn = vn = lens_out = None
+    if rows is not None:
+        for r in rows:
+            assert r.shape == (B, Hkv, D) and r.dtype == q.dtype and r.device == q.device, \
+                "paged: new rows must be [B, Hkv, D] in the pages' dtype"
+        kn, vn = (_ops._contig(r) for r in rows)
+        lens_out = torch.empty_like(lens)
+    out = torch.empty_like(q)
+    lse = torch.empty(B, Hq, device=q.device, dtype=torch.float32) if return_lse else None
+    if B > 0:
+        with _ops.device_of(q):
+            lib, stream = _ops._lib(), _ops._stream(q)
+            nbytes = int(lib.nsa_paged_workspace(B, Hq, Hkv, D, P, mp, stream))
+            ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
+            _ops._call("nsa_paged_attend", lib.nsa_paged_attend, L.ptr(q), L.ptr(kn), L.ptr(vn), L.ptr(k_pages),
+                       L.ptr(v_pages), L.ptr(table), L.ptr(lens), L.ptr(lens_out), L.ptr(out), L.ptr(lse), L.ptr(ws),
+                       nbytes, B, Hq, Hkv, D, P, mp, n, D ** -0.5 if scale is None else float(scale),
+                       L.dtype_code(q), stream)
+    return out, lse, lens_out
+
+
+def paged_attend(q, k_pages, v_pages, table, lens, scale=None, return_lse=False):
+    """``softmax(scale q K^T) V`` of one query per sequence, ``q [B, Hq, D]``, over
+    the first ``lens[b]`` positions -> ``out [B, Hq, D]`` (zeros where there are
+    none).  ``scale`` defaults to ``D ** -0.5``; ``return_lse`` adds
+    ``ln sum e^score`` (float32 ``[B, Hq]``, -1e9 without keys)."""
+    out, lse, _ = _attend(q, None, k_pages, v_pages, table, lens, scale, return_lse)
+    return (out, lse) if return_lse else out
+
+
+def paged_step(q, k_new, v_new, k_pages, v_pages, table, lens, scale=None):
+    """One generation step: the new rows ``[B, Hkv, D]`` go to position
+    ``lens[b]`` (in place, in the pages), then ``q [B, Hq, D]`` attends the
+    ``lens[b] + 1`` positions -> ``(out, new lens)``; the lengths are a new
+    tensor.  A sequence whose position has no page keeps its pages and length
+    and attends what it holds.  Pages that are written may not be shared with
+    another sequence of the call."""
+    out, _, lens_out = _attend(q, (k_new, v_new), k_pages, v_pages, table, lens, scale, False)
+    return out, lens_out
+
+
+def paged_append(k, v, k_pages, v_pages, table, lens, count=None):
+    """Write rows ``k, v [B, Hkv, T, D]`` (the first ``count[b]`` of them: int32
+    ``[B]``, default T) to positions ``lens[b] ..`` -> the new lengths.  A
+    sequence whose rows do not all have a page keeps its pages and length."""
+    _check_pages(k_pages, v_pages, table, lens)
+    n, Hkv, P, D = k_pages.shape
+    B, mp = table.shape
+    assert k.dim() == 4 and k.shape[:2] == (B, Hkv) and k.shape[3] == D and v.shape == k.shape, \
+        "paged: rows must be [B, Hkv, T, D]"
+    assert all(t.dtype == k_pages.dtype and t.device == k_pages.device for t in (k, v)), \
+        "paged: rows in the pages' dtype and device"
+    assert Hkv <= 4096 and B <= 65536, "paged: at most 4096 heads and 65536 sequences"
+    k, v, table, lens = _ops._contig(k), _ops._contig(v), table.contiguous(), lens.contiguous()
+    if count is not None:
+        assert count.dtype == torch.int32 and count.shape == (B,) and count.device == lens.device, \
+            "paged: count int32 [B] on the pages' device"
+        count = count.contiguous()
+    lens_out = torch.empty_like(lens)
+    if B > 0:
+        with _ops.device_of(k_pages):
+            _ops._call("nsa_paged_append", _ops._lib().nsa_paged_append, L.ptr(k), L.ptr(v), L.ptr(k_pages),
+                       L.ptr(v_pages), L.ptr(table), L.ptr(lens), L.ptr(count), L.ptr(lens_out), B, Hkv, k.shape[2], D,
+                       P, mp, n, L.dtype_code(k_pages), _ops._stream(k_pages))
+    return lens_out
+
+
+class _PageAccount:
+    """The table of a set of caches, and the host's account of who holds which page."""
+
+    def __init__(self, batch, max_pages, n_pages, device):
+        self.table = torch.full((batch, max_pages), -1, device=device, dtype=torch.int32)
+        self.free = list(range(n_pages - 1, -1, -1))
+        self.held = [[] for _ in range(batch)]
+        self.caches = []
+
+
+class PagedKVCache:
+    """Pages, table and lengths of one dense attention layer for ``batch``
+    sequences of up to ``max_len`` tokens (``n_kv_heads`` x ``head_dim``).
+
+    ``n_pages`` pages in all (default: enough for every sequence at
+    ``max_len``).  Sequences take pages with ``reserve`` and give them back with
+    ``release``, on the host's own account of the table (neither reads the
+    device).  ``step`` needs the new position reserved.  ``like``, another
+    layer's cache of the same sizes: both lie under one table, and reserving or
+    releasing on either serves both; each has its own pages and lengths."""
+
+    def __init__(self, batch, n_kv_heads, head_dim, max_len, page_size=64, n_pages=None, dtype=torch.bfloat16,
+                 device="cuda", like=None):
+        assert page_size >= 16 and page_size % 16 == 0, "paged: the page size must be a multiple of 16"
+        assert batch >= 1 and max_len >= 1, "paged: a cache of at least one sequence and one token"
+        self.page_size = page_size
+        self.max_pages = -(-max_len // page_size)
+        n_pages = batch * self.max_pages if n_pages is None else n_pages
+        shape = (n_pages, n_kv_heads, page_size, head_dim)
+        if like is not None:
+            assert (like.batch, like.page_size, like.max_pages, like.k_pages.shape[0]) == \
+                (batch, page_size, self.max_pages, n_pages), "paged: caches under one table differ in size"
+        self.k_pages = torch.zeros(shape, device=device, dtype=dtype)
+        self.v_pages = torch.zeros(shape, device=device, dtype=dtype)
+        self.lens = torch.zeros(batch, device=device, dtype=torch.int32)
+        self._account = _PageAccount(batch, self.max_pages, n_pages, device) if like is None else like._account
+        self._account.caches.append(self)
+        _check_pages(self.k_pages, self.v_pages, self.table, self.lens)
+
+    @property
+    def table(self):
+        return self._account.table
+
+    @property
+    def batch(self):
+        return len(self._account.held)
+
+    @property
+    def capacity(self):
+        return self.max_pages * self.page_size
+
+    @property
+    def free_pages(self):
+        return len(self._account.free)
+
+    def reserve(self, lengths):
+        """Pages for ``lengths`` tokens (an int for all sequences, or one per
+        sequence); what a sequence holds already stays.  Raises RuntimeError,
+        and takes nothing, where the pages do not suffice."""
+        acc = self._account
+        lengths = [lengths] * self.batch if isinstance(lengths, int) else [int(n) for n in lengths]
+        assert len(lengths) == self.batch, "paged: one length for each sequence"
+        need = [-(-n // self.page_size) for n in lengths]
+        assert max(need) <= self.max_pages, "paged: longer than max_len"
+        more = [max(0, n - len(h)) for n, h in zip(need, acc.held)]
+        if sum(more) > len(acc.free):
+            raise RuntimeError(f"paged: {sum(more)} pages needed, {len(acc.free)} free")
+        rows, cols, pages = [], [], []
+        for b, m in enumerate(more):
+            for _ in range(m):
+                rows.append(b)
+                cols.append(len(acc.held[b]))
+                pages.append(acc.free.pop())
+                acc.held[b].append(pages[-1])
+        if rows:
+            at = torch.tensor([rows, cols, pages], dtype=torch.int64).to(self.table.device)
+            self.table[at[0], at[1]] = at[2].to(torch.int32)
+
+    def release(self, seq):
+        """Give back sequence ``seq``'s pages; its length becomes 0."""
+        acc = self._account
+        assert 0 <= seq < self.batch, "paged: no such sequence"
+        acc.free.extend(reversed(acc.held[seq]))
+        acc.held[seq] = []
+        acc.table[seq].fill_(-1)
+        for cache in acc.caches:
+            cache.lens[seq].zero_()
+
+    def prefill(self, k, v, lens=None):
+        """Append a prompt's rows ``[B, Hkv, T, D]``, ``lens`` of them a sequence
+        (int32 ``[B]`` on the device, or host ints; default T); the pages must
+        be reserved."""
+        if lens is not None and not torch.is_tensor(lens):
+            lens = torch.as_tensor(lens, dtype=torch.int32).expand(self.batch)
+        if lens is not None:
+            lens = lens.to(device=self.lens.device, dtype=torch.int32)
+        self.lens = paged_append(k, v, self.k_pages, self.v_pages, self.table, self.lens, lens)
+
+    def step(self, q, k_new, v_new, scale=None):
+        """``paged_step`` on this cache -> ``out [B, Hq, D]``."""
+        out, self.lens = paged_step(q, k_new, v_new, self.k_pages, self.v_pages, self.table, self.lens, scale)
+        return out
+
+    def attend(self, q, scale=None, return_lse=False):
+        """``paged_attend`` on this cache."""
+        return paged_attend(q, self.k_pages, self.v_pages, self.table, self.lens, scale, return_lse)
