@@ -44,7 +44,13 @@ Keyword-only extensions, off by default (none is in the reference):
   ``ffn='swiglu'`` with ``ffn_hidden``, ``pos='rope'`` (rotary position on
   queries and keys of every branch, keys rotated before pooling),
   ``tie_embeddings``, ``dense_impl='sdpa'`` (the dense arm through
-  ``torch.nn.functional.scaled_dot_product_attention``).
+  ``torch.nn.functional.scaled_dot_product_attention``);
+* ``norm_impl='fused'`` and ``loss_impl='fused'``: the residual additions with
+  the RMS norms, and the loss over the vocabulary, on the MI355X kernels
+  (``nsa_lm``);
+* generation with the dense arm over paged caches (``nsa_paged``):
+  ``NSATransformer.paged_caches``, ``prefill`` and ``step``; ``score`` for the log
+  probabilities of given tokens.
 """
 
 
@@ -210,6 +216,13 @@ class MLPCompressor(nn.Module):
                                 self.block_size, stride)
 
 
+def _rotate(x, cos, sin):
+    """The halves of x's last dimension as rotated pairs."""
+    h = x.shape[-1] // 2
+    a, b = x[..., :h], x[..., h:]
+    return torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1)
+
+
 class Rotary(nn.Module):
     """Rotary position embedding (RoFormer, arXiv:2104.09864) in the half-split
     layout: the first and second halves of the head dim form the rotated
@@ -242,10 +255,7 @@ class Rotary(nn.Module):
         """``x [B,H,T,D]`` rotated by position ``t``."""
         T = x.shape[2]
         ang = torch.arange(T, device=x.device, dtype=torch.float32)[:, None] * self.inv_freq[None, :]
-        cos, sin = ang.cos().to(x.dtype), ang.sin().to(x.dtype)
-        h = x.shape[-1] // 2
-        a, b = x[..., :h], x[..., h:]
-        return torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1)
+        return _rotate(x, ang.cos().to(x.dtype), ang.sin().to(x.dtype))
 
 
 class SwiGLU(nn.Module):
@@ -541,7 +551,8 @@ class FullAttention(nn.Module):
         B, T, _ = y.shape
         return y.view(B, T, n_heads, self.dh).transpose(1, 2)
 
-    def forward(self, x):
+    def _qkv(self, x):
+        """q, k, v ``[B, H, T, dh]`` of ``x [B, T, d_model]``, rotated by position."""
         B, T, _ = x.shape
         ws = (self.q_proj.weight, self.k_proj.weight, self.v_proj.weight)
         if self.impl == "sdpa" and x.is_cuda:
@@ -552,18 +563,21 @@ class FullAttention(nn.Module):
             y = _linear(x, _stacked_padded(ws))
             r = self.rope is not None
             cos, sin = self.rope.tables(T, y.device, y.dtype) if r else (None, None)
-            q, k, v = ops.split_heads(y, ((self.Hq, self.dh, r), (self.Hkv, self.dh, r), (self.Hkv, self.dh, False)),
-                                      cos, sin)
+            return ops.split_heads(y, ((self.Hq, self.dh, r), (self.Hkv, self.dh, r), (self.Hkv, self.dh, False)),
+                                   cos, sin)
+        if self.impl == "sdpa":
+            yq, yk, yv = torch.split(F.linear(x, torch.cat(ws, dim=0)), [w.shape[0] for w in ws], dim=-1)
         else:
-            if self.impl == "sdpa":
-                yq, yk, yv = torch.split(F.linear(x, torch.cat(ws, dim=0)), [w.shape[0] for w in ws], dim=-1)
-            else:
-                yq, yk, yv = self.q_proj(x), self.k_proj(x), self.v_proj(x)
-            q = self._heads(yq, self.Hq)
-            k = self._heads(yk, self.Hkv)
-            v = self._heads(yv, self.Hkv)
-            if self.rope is not None:
-                q, k = self.rope(q), self.rope(k)
+            yq, yk, yv = self.q_proj(x), self.k_proj(x), self.v_proj(x)
+        q = self._heads(yq, self.Hq)
+        k = self._heads(yk, self.Hkv)
+        v = self._heads(yv, self.Hkv)
+        if self.rope is not None:
+            q, k = self.rope(q), self.rope(k)
+        return q, k, v
+
+    def _causal(self, q, k, v):
+        B, _, T, _ = q.shape
         if self.impl == "sdpa":
             # fused kernels only (the unfused math fallback forms batched
             # products with transposed operands, avoided on this GPU), with
@@ -574,9 +588,41 @@ class FullAttention(nn.Module):
                                                    enable_gqa=self.G > 1)
         else:
             k, v = expand_kv(k, self.G), expand_kv(v, self.G)
-            causal = torch.ones(T, T, dtype=torch.bool, device=x.device).tril()
+            causal = torch.ones(T, T, dtype=torch.bool, device=q.device).tril()
             o = masked_softmax(_scores(q, k, self.scale), causal[None, None]) @ v
         return self.out_proj(o.transpose(1, 2).reshape(B, T, self.Hq * self.dh))
+
+    def forward(self, x):
+        return self._causal(*self._qkv(x))
+
+    def paged_cache(self, batch, max_len, page_size=64, n_pages=None, dtype=None, device=None, like=None):
+        """A ``PagedKVCache`` for this layer (``nsa_paged``)."""
+        import nsa_paged
+        p = next(self.parameters())
+        return nsa_paged.PagedKVCache(batch, self.Hkv, self.dh, max_len, page_size, n_pages, dtype or p.dtype,
+                                      device or p.device, like)
+
+    def prefill(self, x, cache, lens=None):
+        """``forward(x)``, its keys and values kept in the (empty) cache, ``lens``
+        tokens of each sequence (default all); the pages must be reserved."""
+        q, k, v = self._qkv(x)
+        cache.prefill(k.to(cache.k_pages.dtype), v.to(cache.v_pages.dtype), lens)
+        return self._causal(q, k, v)
+
+    def step(self, x, cache):
+        """The row of ``forward`` at the cache's next position: ``x [B, d_model]``
+        -> ``[B, d_model]``, its key and value appended."""
+        B, dt = x.shape[0], cache.k_pages.dtype
+        q = self.q_proj(x).view(B, self.Hq, self.dh)
+        k = self.k_proj(x).view(B, self.Hkv, self.dh)
+        v = self.v_proj(x).view(B, self.Hkv, self.dh)
+        if self.rope is not None:
+            cos, sin = self.rope.tables(cache.capacity, x.device, q.dtype)
+            at = cache.lens.long().clamp(0, cache.capacity - 1)
+            cos, sin = cos[at][:, None].to(q.dtype), sin[at][:, None].to(q.dtype)
+            q, k = _rotate(q, cos, sin), _rotate(k, cos, sin)
+        o = cache.step(q.to(dt), k.to(dt), v.to(dt))
+        return self.out_proj(o.reshape(B, self.Hq * self.dh).to(x.dtype))
 
 
 def make_attention(attn_type, d_model, n_q_heads, n_kv_heads, **nsa_kw):
@@ -601,8 +647,11 @@ class Block(nn.Module):
     and ``ffn='swiglu'`` give the Llama-style variant."""
 
     def __init__(self, d_model, n_q_heads, n_kv_heads, ffn_mult=4, attn_type="nsa", *, norm="layer",
-                 ffn="gelu", ffn_hidden=None, **nsa_kw):
+                 ffn="gelu", ffn_hidden=None, norm_impl="ref", **nsa_kw):
         super().__init__()
+        assert norm_impl in ("ref", "fused"), "norm_impl must be 'ref' or 'fused'"
+        assert norm_impl == "ref" or norm == "rms", "norm_impl='fused' needs norm='rms'"
+        self.norm_impl = norm_impl
         if attn_type == "full":
             nsa_kw = {k: v for k, v in nsa_kw.items() if k not in _NSA_ONLY}
         else:
@@ -618,13 +667,43 @@ class Block(nn.Module):
             self.ffn = nn.Sequential(Linear(d_model, hidden), nn.GELU(), Linear(hidden, d_model))
 
     def forward(self, x):
+        if self.norm_impl == "fused":
+            x, f = self.pending(x, None)
+            return x + f
         x = x + self.attn(self.ln1(x))
         return x + self.ffn(self.ln2(x))
+
+    def pending(self, x, branch, attn=None):
+        """The block with its additions left to the norms that follow them
+        (``norm_impl='fused'``): ``x`` and the branch still to be added to it
+        (None: nothing) -> the same pair behind the block.  ``attn`` stands in
+        for the attention (a generation step's)."""
+        y, x = _fused_norm(self.ln1, branch, x)
+        y, x = _fused_norm(self.ln2, (attn or self.attn)(y), x)
+        return x, self.ffn(y)
+
+    def step(self, x, branch, cache):
+        """One token of every sequence, ``x [B, d_model]``: the pair of
+        ``pending`` (with ``norm_impl='ref'`` the branch is None throughout)."""
+        if self.norm_impl == "fused":
+            return self.pending(x, branch, lambda y: self.attn.step(y, cache))
+        x = x + self.attn.step(self.ln1(x), cache)
+        return x + self.ffn(self.ln2(x)), None
 
 
 def _norm(kind, d_model):
     assert kind in ("layer", "rms"), "norm must be 'layer' or 'rms'"
     return nn.LayerNorm(d_model) if kind == "layer" else nn.RMSNorm(d_model)
+
+
+def _fused_norm(ln, branch, x):
+    """``(ln(x + branch), x + branch)`` in one kernel; the norm's rows in the
+    dtype the products after it compute in (autocast's, where it is on)."""
+    import nsa_lm
+    out = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+    if branch is None:
+        return nsa_lm.add_rms_norm(x, None, ln.weight, ln.eps, out)
+    return nsa_lm.add_rms_norm(branch, x, ln.weight, ln.eps, out)
 
 
 class NSATransformer(nn.Module):
@@ -638,8 +717,11 @@ class NSATransformer(nn.Module):
                  ffn_mult=4, block_size=16, n_selected_blocks=4, window=32, attn_type="nsa", attn_impl="ref", *,
                  norm="layer", ffn="gelu", ffn_hidden=None, pos="learned", rope_base=10000.0, tie_embeddings=True,
                  dense_impl="ref", cmp_stride=None, sel_block=None, force_init=False, n_local=0, compressor="mean",
-                 cmp_hidden=None):
+                 cmp_hidden=None, norm_impl="ref", loss_impl="ref"):
         super().__init__()
+        assert loss_impl in ("ref", "fused"), "loss_impl must be 'ref' or 'fused'"
+        self.norm_impl = norm_impl
+        self.loss_impl = loss_impl
         assert pos in ("learned", "rope"), "pos must be 'learned' or 'rope'"
         self.max_seq_len = max_seq_len
         self.attn_type = attn_type
@@ -653,7 +735,7 @@ class NSATransformer(nn.Module):
                   cmp_stride=cmp_stride, sel_block=sel_block, force_init=force_init, n_local=n_local, rope=rope,
                   dense_impl=dense_impl, compressor=compressor, cmp_hidden=cmp_hidden)
         self.blocks = nn.ModuleList([Block(d_model, n_q_heads, n_kv_heads, ffn_mult=ffn_mult, attn_type=attn_type,
-                                           norm=norm, ffn=ffn, ffn_hidden=ffn_hidden, **kw)
+                                           norm=norm, ffn=ffn, ffn_hidden=ffn_hidden, norm_impl=norm_impl, **kw)
                                      for _ in range(n_layers)])
         self.ln_f = _norm(norm, d_model)
         self.lm_head = Linear(d_model, vocab_size, bias=False)
@@ -676,16 +758,88 @@ class NSATransformer(nn.Module):
         x = self.tok_emb(idx)
         if hasattr(self, "pos_emb"):
             x = x + self.pos_emb(torch.arange(T, device=idx.device))[None]
+        logits = self.lm_head(self._run_blocks(x))
+        loss = None
+        if targets is not None:
+            loss = self._loss(logits, targets)
+        return logits, loss
+
+    def _run_blocks(self, x):
+        """The blocks and the final norm."""
+        ckpt = self.grad_checkpoint and self.training
+        if self.norm_impl == "fused":
+            branch = None
+            for blk in self.blocks:
+                if ckpt:
+                    x, branch = torch.utils.checkpoint.checkpoint(blk.pending, x, branch, use_reentrant=False)
+                else:
+                    x, branch = blk.pending(x, branch)
+            return _fused_norm(self.ln_f, branch, x)[0]
         for blk in self.blocks:
-            if self.grad_checkpoint and self.training:
+            if ckpt:
                 x = torch.utils.checkpoint.checkpoint(blk, x, use_reentrant=False)
             else:
                 x = blk(x)
-        logits = self.lm_head(self.ln_f(x))
-        loss = None
-        if targets is not None:
-            loss = F.cross_entropy(logits.view(-1, logits.size(-1)), targets.view(-1))
-        return logits, loss
+        return self.ln_f(x)
+
+    def _loss(self, logits, targets):
+        """The mean negative log probability of the targets; -100 is left out."""
+        if self.loss_impl == "fused":
+            import nsa_lm
+            logp = nsa_lm.token_logprobs(logits, targets).logp
+            return -logp.sum() / (targets != -100).sum()
+        return F.cross_entropy(logits.view(-1, logits.size(-1)), targets.view(-1))
+
+    @torch.no_grad()
+    def score(self, idx, targets, top=0):
+        """``TokenLogprobs`` of the targets ``[B, T]`` behind the tokens ``idx [B, T]``:
+        log probabilities, entropies and the ``top`` best alternatives."""
+        import nsa_lm
+        return nsa_lm.token_logprobs(self.forward(idx)[0], targets, top)
+
+    # -- generation with the dense arm over paged caches ----------------------
+    def paged_caches(self, batch, max_len=None, page_size=64, n_pages=None, dtype=None):
+        """One ``PagedKVCache`` a block, all under one page table: ``reserve`` and
+        ``release`` on the first serve all."""
+        assert self.attn_type == "full", "paged caches serve the dense arm (attn_type='full')"
+        max_len = self.max_seq_len if max_len is None else max_len
+        assert max_len <= self.max_seq_len, "longer than the model's max_seq_len"
+        caches = []
+        for blk in self.blocks:
+            caches.append(blk.attn.paged_cache(batch, max_len, page_size, n_pages, dtype,
+                                               like=caches[0] if caches else None))
+        return caches
+
+    @torch.no_grad()
+    def prefill(self, idx, caches, lens=None):
+        """``forward(idx)``'s logits ``[B, T, V]``, the keys and values of the first
+        ``lens[b]`` tokens (default all) kept in the (empty, reserved) caches."""
+        B, T = idx.shape
+        assert T <= self.max_seq_len
+        x = self.tok_emb(idx)
+        if hasattr(self, "pos_emb"):
+            x = x + self.pos_emb(torch.arange(T, device=idx.device))[None]
+        branch = None
+        for blk, cache in zip(self.blocks, caches):
+            if self.norm_impl == "fused":
+                x, branch = blk.pending(x, branch, lambda y: blk.attn.prefill(y, cache, lens))
+            else:
+                x = x + blk.attn.prefill(blk.ln1(x), cache, lens)
+                x = x + blk.ffn(blk.ln2(x))
+        return self.lm_head(_fused_norm(self.ln_f, branch, x)[0] if self.norm_impl == "fused" else self.ln_f(x))
+
+    @torch.no_grad()
+    def step(self, tokens, caches):
+        """One generation step: ``tokens [B]`` at each sequence's next position
+        -> logits ``[B, V]``; the caches grow by one (their pages reserved).  No
+        host synchronisation: the loop can be captured into a graph."""
+        x = self.tok_emb(tokens)
+        if hasattr(self, "pos_emb"):
+            x = x + self.pos_emb(caches[0].lens.long().clamp(0, self.max_seq_len - 1))
+        branch = None
+        for blk, cache in zip(self.blocks, caches):
+            x, branch = blk.step(x, branch, cache)
+        return self.lm_head(_fused_norm(self.ln_f, branch, x)[0] if self.norm_impl == "fused" else self.ln_f(x))
 
     def num_params(self):
         """The reference's parameter count (nsa_model.py:508-511): the unique
