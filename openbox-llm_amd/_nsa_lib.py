@@ -163,5 +163,10 @@ def ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
+def addr(t):
+    """A tensor's address as ctypes takes it fastest (None: a null pointer)."""
+    return None if t is None else t.data_ptr()
+
+
 def stream_of(t):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)

@@ -17,7 +17,7 @@
 // few others go to a list in LDS as (value, ~index) keys, which are all
 // different, and are ranked by counting.  The bound is formed after the
 // first chunk, which is still in registers, and again whenever the chunks done
-// have grown fourfold.  A row that overfills the list (long ties, a rising
+// have doubled: 16 ballots, one for each of the upper bits of a value's key.  A row that overfills the list (long ties, a rising
 // row) is selected exactly by eight radix passes over the keys instead.
 //
 // One wave takes a row of up to 2048 elements; a workgroup of four takes a
@@ -121,10 +121,9 @@ __global__ __launch_bounds__(256) void k_logprob(const LpArgs a) {
   constexpr int ROWS = 256 / THR;           // rows a workgroup
   constexpr int CAP = W > 1 ? kLpCap : 512;
   __shared__ uint64_t list_s[TOP ? ROWS : 1][TOP ? CAP : 1];
-  __shared__ uint32_t keys_s[TOP ? ROWS : 1][TOP ? THR : 1];
+  __shared__ uint32_t keys_s[2][TOP && W > 1 ? THR : 1];
   __shared__ uint32_t hist[TOP ? ROWS : 1][TOP ? 256 : 1];
   __shared__ int count_s[ROWS];
-  __shared__ uint32_t thr_s[ROWS];
   __shared__ LpState st_s[W];
   const int t = threadIdx.x & (THR - 1), sub = threadIdx.x / THR;
   const int64_t unit = (int64_t)blockIdx.x * ROWS + sub;
@@ -143,13 +142,13 @@ __global__ __launch_bounds__(256) void k_logprob(const LpArgs a) {
     else
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
-  if (TOP && t == 0) count_s[sub] = 0;
+  if (TOP && t == 0) count_s[sub] = 0;   // (added to only behind the first bound's barrier)
 
   LpState st{kLowest, 0.0f, 0.0f};
   uint32_t thr = 0;             // keys below it are no alternatives
   float thr_z = -__builtin_inff();
   int next = 1;                 // chunks done at the bound's next forming
-  int done = 0;
+  int done = 0, turn = 0;
   constexpr int CH = THR * 8 * U;
   for (int c = c0; c < c1; c += CH) {
     float x[U][8];
@@ -158,11 +157,14 @@ __global__ __launch_bounds__(256) void k_logprob(const LpArgs a) {
       const int at = c + 8 * (u * THR + t);
       load_run8(z + at, c1 - at, x[u], -__builtin_inff());
     }
-    float mx = x[0][0];
+    float mxu[U], mx;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      mxu[u] = x[u][0];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) mx = fmaxf(mx, x[u][j]);
+      for (int j = 1; j < 8; ++j) mxu[u] = fmaxf(mxu[u], x[u][j]);
+      mx = u == 0 ? mxu[0] : fmaxf(mx, mxu[u]);
+    }
     if (mx > st.m) lp_raise(st, mx);
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -176,26 +178,37 @@ __global__ __launch_bounds__(256) void k_logprob(const LpArgs a) {
     if (TOP) {
       ++done;
       if (done == next) {
-        // the k-th largest of the lanes' maxima
+        // The k-th largest of the lanes' maxima, by the upper halves of their keys.  (A lane that
+        // holds NaN counts with its largest other value: still one of its elements' keys or less.)
         const bool any = c0 + 8 * t < c1;
-        // (a lane that holds NaN counts with its largest other value: still one of its elements' keys or less)
-        const uint32_t mine = any ? value_key(st.l == 0.0f ? -__builtin_inff() : st.m) : 0u;
-        keys_s[sub][t] = mine;
-        sync();
-        int rank = 0;
-        for (int i = 0; i < THR; ++i) {
-          const uint32_t o = keys_s[sub][i];
-          rank += (o > mine || (o == mine && i < t)) ? 1 : 0;
-        }
-        if (rank == a.k - 1) thr_s[sub] = mine;
-        sync();
-        thr = thr_s[sub];
-        thr_z = thr == 0u ? -__builtin_inff() : key_value((uint64_t)thr << 32);
-        next *= 4;
-      }
-      if (!(mx < thr_z) || st.l != st.l) {
+        uint32_t v[W];
+        v[0] = any ? value_key(st.l == 0.0f ? -__builtin_inff() : st.m) >> 16 : 0u;
+        if (W > 1) {
+          // two buffers in turn: the next bound's maxima are not written over ones still being read
+          keys_s[turn][t] = v[0];
+          __syncthreads();
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+          for (int i = 0; i < W; ++i) v[i] = keys_s[turn][64 * i + (t & 63)];
+          turn ^= 1;
+        }
+        uint32_t kth = 0;
+#pragma unroll
+        for (int bit = 15; bit >= 0; --bit) {
+          const uint32_t cand = kth | (1u << bit);
+          int n = 0;
+#pragma unroll
+          for (int i = 0; i < W; ++i) n += __popcll(__ballot(v[i] >= cand));
+          kth = n >= a.k ? cand : kth;
+        }
+        thr = kth << 16;
+        thr_z = thr == 0u ? -__builtin_inff() : key_value((uint64_t)thr << 32);
+        next *= 2;
+      }
+      const bool nan = st.l != st.l;
+      if (!(mx < thr_z) || nan) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (mxu[u] < thr_z && !nan) continue;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const int at = c + 8 * (u * THR + t) + j;
@@ -204,6 +217,7 @@ __global__ __launch_bounds__(256) void k_logprob(const LpArgs a) {
               if (i < CAP) list[i] = elem_key(x[u][j], at);
             }
           }
+        }
       }
     }
   }
@@ -275,39 +289,47 @@ __global__ __launch_bounds__(256) void k_logprob(const LpArgs a) {
   }
 }
 
-// Joins the parts of split rows: one workgroup a row.
+// Larger of two keys over the wave, in every lane.
+__device__ __forceinline__ uint64_t wave_max_key(uint64_t key) {
+  const uint32_t hi = wave_reduce_u32<true>((uint32_t)(key >> 32));
+  const uint32_t lo = wave_reduce_u32<true>((uint32_t)(key >> 32) == hi ? (uint32_t)key : 0u);
+  return ((uint64_t)hi << 32) | lo;
+}
+
+// Joins the parts of a split row: one wave a row, one lane a part.  The parts'
+// lists are sorted, so the k best come off their heads one after the other.
 template <typename T>
-__global__ __launch_bounds__(256) void k_logprob_join(const LpArgs a) {
+__global__ __launch_bounds__(64) void k_logprob_join(const LpArgs a) {
   extern __shared__ uint64_t jlist[];
-  __shared__ LpState st_s[4];
   const int64_t row = blockIdx.x;
   const int t = threadIdx.x;
   float zt = 0.0f;
   const bool has_t = t == 0 && lp_target<T>(a, row, zt);
   LpState st{kLowest, 0.0f, 0.0f};
-  for (int i = t; i < a.nsp; i += 256) {
-    const float4 p = a.part[row * a.nsp + i];
-    lp_join(st, LpState{p.x, p.y, p.z});
+  if (t < a.nsp) {
+    const float4 p = a.part[row * a.nsp + t];
+    st = LpState{p.x, p.y, p.z};
   }
   const int n = a.nsp * a.k;
-  for (int i = t; i < n; i += 256) jlist[i] = a.part_top[row * n + i];
+  for (int i = t; i < n; i += 64) jlist[i] = a.part_top[row * n + i];
   st = lp_wave(st);
-  if ((t & 63) == 0) st_s[t >> 6] = st;
-  __syncthreads();
-  st = st_s[0];
-#pragma unroll
-  for (int i = 1; i < 4; ++i) lp_join(st, st_s[i]);
   const float logl = st.l == 0.0f ? -__builtin_inff() : logf(st.l);
   if (t == 0) lp_finish(a, row, st, zt, has_t);
-  for (int i = t; i < n; i += 256) {
-    const uint64_t mine = jlist[i];
-    if (mine == 0) continue;
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += jlist[j] > mine ? 1 : 0;
-    if (rank < a.k) {
-      a.top_logp[row * a.k + rank] = st.l == 0.0f ? -__builtin_inff() : (key_value(mine) - st.m) - logl;
-      a.top_idx[row * a.k + rank] = (int64_t)(uint32_t)~(uint32_t)mine;
+  __syncthreads();
+  int at = t * a.k;
+  const int end = t < a.nsp ? at + a.k : at;
+  uint64_t head = at < end ? jlist[at] : 0, out = 0;
+  for (int r = 0; r < a.k; ++r) {
+    const uint64_t best = wave_max_key(head);
+    if (t == r) out = best;
+    if (head == best) {      // one lane: keys are all different (and k of them are no 0)
+      ++at;
+      head = at < end ? jlist[at] : 0;
     }
+  }
+  if (t < a.k) {
+    a.top_logp[row * a.k + t] = st.l == 0.0f ? -__builtin_inff() : (key_value(out) - st.m) - logl;
+    a.top_idx[row * a.k + t] = (int64_t)(uint32_t)~(uint32_t)out;
   }
 }
 
@@ -414,7 +436,7 @@ static int logprob_launch(LpArgs a, hipStream_t s) {
     else
       k_logprob<T, 4, 4, false><<<(unsigned)grid, 256, 0, s>>>(a);
   }
-  if (a.nsp > 1) k_logprob_join<T><<<(unsigned)a.rows, 256, (size_t)a.nsp * a.k * 8, s>>>(a);
+  if (a.nsp > 1) k_logprob_join<T><<<(unsigned)a.rows, 64, (size_t)a.nsp * a.k * 8, s>>>(a);
   return nsa_launch_status();
 }
 

@@ -13,7 +13,8 @@
 // Every kernel is bound by the bytes it moves: one read of x and r (dy, dh_out
 // and h in the backward), one write of h and y (dx, dr).  A row stays in
 // registers between its reduction and its output, so nothing is read twice
-// (past 32768 elements a row is read again, through the cache).
+// (past 32768 elements, 16384 in the backward, a row is read again, through the
+// cache).
 //
 // Threads per row: one wave up to 2048 elements (no barrier at all), 256 or
 // 1024 threads above, in runs of 8 elements.  Where the rows are too few to
@@ -30,7 +31,8 @@ namespace nsa {
 constexpr float kQ8Max = 448.0f;            // largest e4m3 value
 constexpr float kQ8Floor = 0x1p-100f;
 constexpr int kNormWaveMax = 2048;           // widest row of one wave
-constexpr int kNormRegMax = 32768;           // widest row held in registers
+constexpr int kNormRegMax = 32768;           // widest row held in registers (forward)
+constexpr int kNormBwdMax = 16384;           // ... and with its gradient and its part of dw (backward)
 constexpr int kNormMax = 1 << 24;            // widest row
 
 struct NormArgs {
@@ -180,13 +182,27 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormBw
   for (int64_t row = (int64_t)blockIdx.x * RPG + sub; row < a.rows; row += (int64_t)gridDim.x * RPG) {
     const int64_t base = row * D;
     const float rstd = a.rstd[row];
-    float n_[NV][8], g[NV][8];
+    constexpr bool kEarly = NV * TPR <= 1024;   // dh asked for with the rest, where the registers hold it
+    float n_[NV][8], g[NV][8], d[kEarly ? NV : 1][8];
     float dot = 0.0f;
+    auto load_dh = [&](int i, float(&v)[8]) {
+      const int c = 8 * (i * TPR + t);
+      if (a.dh != nullptr) {
+        load_run8(static_cast<const RT*>(a.dh) + base + c, D - c, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+      }
+    };
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = 8 * (i * TPR + t), n = D - c;
       load_run8(static_cast<const RT*>(a.h) + base + c, n, n_[i]);
       load_run8(static_cast<const YT*>(a.dy) + base + c, n, g[i]);
+      if (kEarly) load_dh(i, d[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         n_[i][j] *= rstd;
@@ -201,21 +217,16 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormBw
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = 8 * (i * TPR + t), n = D - c;
-      float d[8];
-      if (a.dh != nullptr) {
-        load_run8(static_cast<const RT*>(a.dh) + base + c, n, d);
-      } else {
+      float(&di)[8] = d[kEarly ? i : 0];
+      if (!kEarly) load_dh(i, di);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] = 0.0f;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) d[j] += rstd * (g[i][j] - n_[i][j] * dot);
+      for (int j = 0; j < 8; ++j) di[j] += rstd * (g[i][j] - n_[i][j] * dot);
       if (n > 0) {
         if (a.dx_bf16)
-          store_run8(static_cast<bf16*>(a.dx) + base + c, n, d);
+          store_run8(static_cast<bf16*>(a.dx) + base + c, n, di);
         else
-          store_run8(static_cast<float*>(a.dx) + base + c, n, d);
-        if (a.dres != nullptr) store_run8(static_cast<RT*>(a.dres) + base + c, n, d);
+          store_run8(static_cast<float*>(a.dx) + base + c, n, di);
+        if (a.dres != nullptr) store_run8(static_cast<RT*>(a.dres) + base + c, n, di);
       }
     }
   }
@@ -246,7 +257,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormBw
   }
 }
 
-// Rows past kNormRegMax: one workgroup a row, read twice.
+// Rows past kNormBwdMax: one workgroup a row, read twice.
 template <typename YT, typename RT>
 __global__ __launch_bounds__(1024) void k_norm_bwd_long(const NormBwdArgs a) {
   __shared__ float red[16];
@@ -281,40 +292,50 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(const NormBwdArgs a) {
   }
 }
 
-// dw of rows past kNormRegMax: a thread a column, the rows in order.
+// Parts of dw for such rows: 2048 columns and every gridDim.y-th row a workgroup.
 template <typename YT, typename RT>
-__global__ __launch_bounds__(256) void k_norm_dw_long(const NormBwdArgs a, void* dw) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= a.D) return;
-  float s = 0.0f;
-  for (int64_t r = 0; r < a.rows; ++r)
-    s += (float)static_cast<const YT*>(a.dy)[r * a.D + c] *
-         ((float)static_cast<const RT*>(a.h)[r * a.D + c] * a.rstd[r]);
-  if (a.w_bf16)
-    static_cast<bf16*>(dw)[c] = (bf16)s;
-  else
-    static_cast<float*>(dw)[c] = s;
+__global__ __launch_bounds__(256) void k_norm_dw_wide(const NormBwdArgs a) {
+  const int c = 8 * ((int)blockIdx.x * 256 + (int)threadIdx.x), n = a.D - c;
+  if (n <= 0) return;
+  float dw[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 2
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    float h[8], g[8];
+    load_run8(static_cast<const RT*>(a.h) + row * a.D + c, n, h);
+    load_run8(static_cast<const YT*>(a.dy) + row * a.D + c, n, g);
+    const float rstd = a.rstd[row];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dw[j] += g[j] * (h[j] * rstd);
+  }
+  store_run8(a.part + (int64_t)blockIdx.y * a.D + c, n, dw);
 }
 
-// dw[c] = sum of part[p][c], p ascending within each of 16 interleaved sums, those in order
+// dw[c] = sum of part[p][c]: 16 columns a workgroup (64-byte pieces of a part), 64
+// interleaved sums over the parts, added in order.
 __global__ __launch_bounds__(1024) void k_norm_dw(const float* __restrict__ part, int nparts, int D, void* dw,
                                                   bool w_bf16) {
-  __shared__ float acc[16][64];
-  const int lane = threadIdx.x & 63, s = threadIdx.x >> 6;
-  const int c = blockIdx.x * 64 + lane;
+  __shared__ float acc[64][17];
+  const int x = threadIdx.x & 15, s = threadIdx.x >> 4;
+  const int c = blockIdx.x * 16 + x;
   float v = 0.0f;
-  if (c < D)
-    for (int p = s; p < nparts; p += 16) v += part[(int64_t)p * D + c];
-  acc[s][lane] = v;
+  if (c < D) {
+#pragma unroll 8
+    for (int p = s; p < nparts; p += 64) v += part[(int64_t)p * D + c];
+  }
+  acc[s][x] = v;
   __syncthreads();
-  if (s == 0 && c < D) {
+  if (s < 4) {   // 16 sums each by the first wave, then those four
     float t = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t += acc[i][lane];
-    if (w_bf16)
-      static_cast<bf16*>(dw)[c] = (bf16)t;
-    else
-      static_cast<float*>(dw)[c] = t;
+    for (int i = 0; i < 16; ++i) t += acc[16 * s + i][x];
+    t += __shfl_xor(t, 16, kWave);
+    t += __shfl_xor(t, 32, kWave);
+    if (s == 0 && c < D) {
+      if (w_bf16)
+        static_cast<bf16*>(dw)[c] = (bf16)t;
+      else
+        static_cast<float*>(dw)[c] = t;
+    }
   }
 }
 
@@ -358,11 +379,13 @@ static int norm_fwd_as(const NormArgs& a, bool q8, hipStream_t s) {
   return NSA_ERR_DTYPE;
 }
 
-// Workgroups of the backward: four to a compute unit, each with a part of dw.
+// Parts of dw: a workgroup of the backward each, as many as fill the chip's
+// waves (eight of 256 threads to a compute unit); past kNormBwdMax a row group of k_norm_dw_wide.
 static int64_t norm_bwd_groups(int64_t rows, int D, int cu) {
+  if (D > kNormBwdMax) return rows < 128 ? rows : 128;
   const NormShape sh = norm_shape(rows, D, cu);
   const int64_t groups = sh.tpr == 64 ? (rows + 3) / 4 : rows;
-  const int64_t most = (int64_t)cu * (sh.tpr == 1024 ? 2 : 4);
+  const int64_t most = (int64_t)cu * (sh.tpr == 1024 ? 2 : 8);
   return groups < most ? groups : most;
 }
 
@@ -370,25 +393,26 @@ template <typename YT, typename RT>
 static int norm_bwd_launch(NormBwdArgs a, void* dw, hipStream_t s) {
   const int cu = device_cu_count(s);
   const NormShape sh = norm_shape(a.rows, a.D, cu);
-  if (sh.nv == 0) {
-    k_norm_bwd_long<YT, RT><<<(unsigned)a.rows, 1024, 0, s>>>(a);
-    if (dw != nullptr) k_norm_dw_long<YT, RT><<<(unsigned)((a.D + 255) / 256), 256, 0, s>>>(a, dw);
-    return nsa_launch_status();
-  }
   const int64_t grid = norm_bwd_groups(a.rows, a.D, cu);
   bool done = false;
+  if (a.D > kNormBwdMax) {
+    k_norm_bwd_long<YT, RT><<<(unsigned)a.rows, 1024, 0, s>>>(a);
+    if (dw != nullptr)
+      k_norm_dw_wide<YT, RT><<<dim3((unsigned)((a.D + 2047) / 2048), (unsigned)grid), 256, 0, s>>>(a);
+    done = true;
+  }
 #define NSA_NORM_CASE(TPR, NV)                                                                        \
-  if (sh.tpr == TPR && sh.nv == NV) {                                                                 \
+  if (!done && sh.tpr == TPR && sh.nv == NV) {                                                        \
     k_norm_bwd<YT, RT, TPR, NV><<<(unsigned)grid, TPR < 256 ? 256 : TPR, 0, s>>>(a);                  \
     done = true;                                                                                      \
   }
   NSA_NORM_CASE(64, 1) NSA_NORM_CASE(64, 2) NSA_NORM_CASE(64, 3) NSA_NORM_CASE(64, 4)
   NSA_NORM_CASE(256, 1) NSA_NORM_CASE(256, 2) NSA_NORM_CASE(256, 4)
-  NSA_NORM_CASE(1024, 1) NSA_NORM_CASE(1024, 2) NSA_NORM_CASE(1024, 4)
+  NSA_NORM_CASE(1024, 1) NSA_NORM_CASE(1024, 2)
 #undef NSA_NORM_CASE
   if (!done) return NSA_ERR_SHAPE;
   if (dw != nullptr)
-    k_norm_dw<<<(unsigned)((a.D + 63) / 64), 1024, 0, s>>>(a.part, (int)grid, a.D, dw, a.w_bf16);
+    k_norm_dw<<<(unsigned)((a.D + 15) / 16), 1024, 0, s>>>(a.part, (int)grid, a.D, dw, a.w_bf16);
   return nsa_launch_status();
 }
 
@@ -420,7 +444,7 @@ extern "C" int nsa_norm_fwd(const void* x, const void* res, const void* w, void*
 extern "C" size_t nsa_norm_bwd_workspace(int64_t rows, int D, void* stream) {
   using namespace nsa;
   if (rows < 0 || rows > 0x7fffffffLL || D < 1 || D > kNormMax) return 0;
-  if (rows == 0 || D > kNormRegMax) return 16;
+  if (rows == 0) return 16;
   return (size_t)norm_bwd_groups(rows, D, device_cu_count(static_cast<hipStream_t>(stream))) * D * sizeof(float);
 }
 
@@ -433,7 +457,7 @@ extern "C" int nsa_norm_bwd(const void* dy, const void* dh, const void* h, const
   NSA_CHECK(dy != nullptr && h != nullptr && w != nullptr && rstd != nullptr && dx != nullptr, NSA_ERR_ARG);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   float* part = nullptr;
-  if (dw != nullptr && D <= kNormRegMax) {
+  if (dw != nullptr) {
     NSA_CHECK(workspace != nullptr && workspace_bytes >= nsa_norm_bwd_workspace(rows, D, stream), NSA_ERR_WORKSPACE);
     part = static_cast<float*>(workspace);
   }

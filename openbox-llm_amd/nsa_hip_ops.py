@@ -144,12 +144,24 @@ def _lib():
     return L.load()
 
 
-def device_of(t):
-    """Context in which t's device is the current one (launches, stream and
-    device queries then go there)."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def launch(t, name, *args):
+    """Library call ``name(*args, stream)`` on t's device and its current
+    stream; addresses as integers.  The short way round for calls whose host
+    time counts: the raw stream query and integer addresses take 0.2 us where
+    ``stream_of`` and a dozen ``ptr`` take 4."""
+    dev = t.get_device()
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return launch(t, name, *args)
+    fn = getattr(_lib(), name)
+    if _TIMER is not None:
+        with _span(name):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc < 0:
+        L.check(rc, name)
+    return rc
 
 
 def _stream(t):

@@ -27,6 +27,7 @@ import _nsa_lib as L
 import nsa_hip_ops as _ops
 
 _FLOATS = (torch.float32, torch.bfloat16)
+_CODE = {torch.float32: L.NSA_F32, torch.bfloat16: L.NSA_BF16, torch.float8_e4m3fn: L.NSA_E4M3}
 TOP_MAX = 64     # most alternatives of a row
 
 
@@ -35,8 +36,8 @@ def _check(t, what):
     assert t.dtype in _FLOATS, f"{what}: dtype {t.dtype} is not supported (float32 or bfloat16)"
 
 
-def _code(dtype):
-    return {torch.float32: L.NSA_F32, torch.bfloat16: L.NSA_BF16, torch.float8_e4m3fn: L.NSA_E4M3}[dtype]
+def _wants_grad(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
 # ---------------------------------------------------------------------------
@@ -46,8 +47,9 @@ def _code(dtype):
 def _norm_args(x, residual, weight, eps, what):
     _check(x, f"{what}: x")
     _check(weight, f"{what}: weight")
-    assert x.dim() >= 1 and x.shape[-1] >= 1, f"{what}: x must be [..., D]"
-    assert weight.shape == x.shape[-1:], f"{what}: weight must be [D]"
+    D = x.shape[-1] if x.dim() else 0
+    assert 1 <= D <= 1 << 24, f"{what}: x must be [..., D]"
+    assert weight.shape == (D,), f"{what}: weight must be [D]"
     assert weight.device == x.device, f"{what}: x and weight on different devices"
     if residual is not None:
         _check(residual, f"{what}: residual")
@@ -55,24 +57,60 @@ def _norm_args(x, residual, weight, eps, what):
     if eps is None:
         eps = torch.finfo(x.dtype if residual is None else residual.dtype).eps
     assert eps >= 0, f"{what}: eps must not be negative"
-    return float(eps)
+    return eps
 
 
 def _norm_fwd(x, residual, weight, eps, out_dtype, want_rstd):
     """-> (y, h, scale, rstd); h is x without a residual."""
     x, weight = x.contiguous(), weight.contiguous()
-    D, rows = x.shape[-1], x.numel() // x.shape[-1]
-    res = None if residual is None else residual.contiguous()
-    h = x if res is None else torch.empty_like(res)
-    y = torch.empty(x.shape, device=x.device, dtype=out_dtype)
-    f32 = dict(device=x.device, dtype=torch.float32)
-    scale = torch.empty(x.shape[:-1], **f32) if out_dtype == torch.float8_e4m3fn else None
-    rstd = torch.empty(rows, **f32) if want_rstd else None
-    with _ops.device_of(x):
-        _ops._call("nsa_norm_fwd", _ops._lib().nsa_norm_fwd, L.ptr(x), L.ptr(res), L.ptr(weight),
-                   L.ptr(None if res is None else h), L.ptr(y), L.ptr(scale), L.ptr(rstd), rows, D, eps,
-                   _code(x.dtype), _code(h.dtype), _code(weight.dtype), _code(out_dtype), _ops._stream(x))
+    D = x.shape[-1]
+    rows = x.numel() // D
+    if residual is None:
+        h, r_at, h_at = x, None, None
+    else:
+        residual = residual.contiguous()
+        h = torch.empty_like(residual)
+        r_at, h_at = residual.data_ptr(), h.data_ptr()
+    y = torch.empty_like(x, dtype=out_dtype)
+    scale = rstd = None
+    if out_dtype == torch.float8_e4m3fn:
+        scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    if want_rstd:
+        rstd = torch.empty(rows, device=x.device, dtype=torch.float32)
+    _ops.launch(x, "nsa_norm_fwd", x.data_ptr(), r_at, weight.data_ptr(), h_at, y.data_ptr(), L.addr(scale),
+                L.addr(rstd), rows, D, eps, _CODE[x.dtype], _CODE[h.dtype], _CODE[weight.dtype], _CODE[out_dtype])
     return y, h, scale, rstd
+
+
+def _norm_bwd(ctx, dy, dh=None):
+    h, weight, rstd = ctx.saved_tensors
+    x_dt, added = ctx.meta
+    need_x, need_r, need_w = ctx.needs_input_grad[:3]
+    if dy is None:       # only the sum was used: its gradient passes through
+        if dh is None:
+            return None, None, None, None, None
+        return (dh.to(x_dt) if need_x else None, dh if need_r else None, torch.zeros_like(weight) if need_w else None,
+                None, None)
+    D = h.shape[-1]
+    rows = h.numel() // D
+    dy = dy.contiguous()
+    dh = None if dh is None else dh.contiguous()
+    dx = torch.empty_like(h, dtype=x_dt)
+    dr = dx if added else None
+    if added and x_dt != h.dtype:
+        dr = torch.empty_like(h)
+    if rows == 0:
+        return dx, dr, torch.zeros_like(weight) if need_w else None, None, None
+    dw = ws = None
+    nbytes = 0
+    if need_w:
+        dw = torch.empty_like(weight)
+        nbytes = _ops.launch(h, "nsa_norm_bwd_workspace", rows, D)
+        ws = torch.empty(nbytes, device=h.device, dtype=torch.uint8)
+    _ops.launch(h, "nsa_norm_bwd", dy.data_ptr(), L.addr(dh), h.data_ptr(), weight.data_ptr(), rstd.data_ptr(),
+                dx.data_ptr(), None if dr is dx else L.addr(dr), L.addr(dw), L.addr(ws), nbytes, rows, D,
+                _CODE[x_dt], _CODE[h.dtype], _CODE[weight.dtype], _CODE[dy.dtype])
+    return dx, dr, dw, None, None
 
 
 class AddRmsNormHIP(torch.autograd.Function):
@@ -81,39 +119,17 @@ class AddRmsNormHIP(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, eps, out_dtype):
         ctx.set_materialize_grads(False)
-        y, h, _, rstd = _norm_fwd(x, residual, weight, eps, out_dtype, any(ctx.needs_input_grad))
+        weight = weight.contiguous()
+        y, h, _, rstd = _norm_fwd(x, residual, weight, eps, out_dtype, True)
         ctx.save_for_backward(h, weight, rstd)
         ctx.meta = (x.dtype, residual is not None)
         return y if residual is None else (y, h)
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dh=None):
-        h, weight, rstd = ctx.saved_tensors
-        x_dt, added = ctx.meta
-        need_x, need_r, need_w = ctx.needs_input_grad[:3]
-        if dy is None:       # only the sum was used: its gradient passes through
-            if dh is None:
-                return None, None, None, None, None
-            return (dh.to(x_dt) if need_x else None, dh if need_r else None,
-                    torch.zeros_like(weight) if need_w else None, None, None)
-        D, rows = h.shape[-1], h.numel() // h.shape[-1]
-        h, weight, dy = h.contiguous(), weight.contiguous(), dy.contiguous()
-        dh = None if dh is None else dh.contiguous()
-        dx = torch.empty(h.shape, device=h.device, dtype=x_dt)
-        dres = torch.empty_like(h) if added and x_dt != h.dtype else None
-        dw = torch.empty_like(weight) if need_w else None
-        if rows == 0:
-            return dx, dres if dres is not None else (dx if added else None), \
-                torch.zeros_like(weight) if need_w else None, None, None
-        with _ops.device_of(h):
-            nbytes = int(_ops._lib().nsa_norm_bwd_workspace(rows, D, _ops._stream(h))) if need_w else 0
-            ws = torch.empty(nbytes, device=h.device, dtype=torch.uint8) if need_w else None
-            _ops._call("nsa_norm_bwd", _ops._lib().nsa_norm_bwd, L.ptr(dy), L.ptr(dh), L.ptr(h), L.ptr(weight),
-                       L.ptr(rstd), L.ptr(dx), L.ptr(dres), L.ptr(dw), L.ptr(ws), nbytes, rows, D, _code(x_dt),
-                       _code(h.dtype), _code(weight.dtype), _code(dy.dtype), _ops._stream(h))
-        dr = None if not added else dx if dres is None else dres
-        return dx, dr, dw, None, None
+    def backward(ctx, *grads):
+        if torch.is_grad_enabled():      # (create_graph: a second derivative is refused when it is taken)
+            return once_differentiable(_norm_bwd)(ctx, *grads)
+        return _norm_bwd(ctx, *grads)
 
 
 def add_rms_norm(x, residual, weight, eps=None, out_dtype=None):
@@ -132,6 +148,9 @@ def add_rms_norm(x, residual, weight, eps=None, out_dtype=None):
     if out_dtype is None:
         out_dtype = x.dtype if residual is None else residual.dtype
     assert out_dtype in _FLOATS, "add_rms_norm: out_dtype must be float32 or bfloat16"
+    if not _wants_grad(x, residual, weight):
+        y, h, _, _ = _norm_fwd(x, residual, weight, eps, out_dtype, False)
+        return y, x if residual is None else h
     if residual is None:
         return AddRmsNormHIP.apply(x, None, weight, eps, out_dtype), x
     return AddRmsNormHIP.apply(x, residual, weight, eps, out_dtype)
@@ -147,8 +166,7 @@ def add_rms_norm_q8(x, residual, weight, eps=None):
     NaN or infinite scale.  For inference: inputs that need a gradient are
     refused."""
     eps = _norm_args(x, residual, weight, eps, "add_rms_norm_q8")
-    assert not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight))), \
-        "add_rms_norm_q8 has no gradient: call it under torch.no_grad()"
+    assert not _wants_grad(x, residual, weight), "add_rms_norm_q8 has no gradient: call it under torch.no_grad()"
     y, h, scale, _ = _norm_fwd(x, residual, weight, eps, torch.float8_e4m3fn, False)
     return y, scale, x if residual is None else h
 
@@ -167,43 +185,54 @@ class TokenLogprobs(NamedTuple):
     top_idx: Optional[torch.Tensor]
 
 
+def _logprob_fwd(z, targets, top):
+    """-> (logp, entropy, top_logp, top_idx, stat) of dense ``z [rows, V]``."""
+    rows, V = z.shape
+    dev, f32 = z.device, torch.float32
+    logp = None if targets is None else torch.empty(rows, device=dev, dtype=f32)
+    ent, stat = torch.empty(rows, device=dev, dtype=f32), torch.empty(rows, 2, device=dev, dtype=f32)
+    top_logp = top_idx = None
+    if top:
+        top_logp = torch.empty(rows, top, device=dev, dtype=f32)
+        top_idx = torch.empty(rows, top, device=dev, dtype=torch.int64)
+    nbytes = _ops.launch(z, "nsa_logprob_workspace", rows, V, top)
+    assert nbytes > 0, "token_logprobs: unsupported shape"
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes > 16 else None
+    _ops.launch(z, "nsa_logprob_fwd", z.data_ptr(), L.addr(targets), L.addr(logp), ent.data_ptr(), stat.data_ptr(),
+                L.addr(top_logp), L.addr(top_idx), L.addr(ws), nbytes, rows, V, top, _CODE[z.dtype])
+    return logp, ent, top_logp, top_idx, stat
+
+
+def _logprob_bwd(ctx, dlogp, dent, _dtop=None, _didx=None):
+    z, targets, stat, ent = ctx.saved_tensors
+    if dlogp is None and dent is None:
+        return None, None, None
+    rows, V = z.shape
+    dz = torch.empty_like(z)
+    dlogp = None if dlogp is None else dlogp.contiguous()
+    dent = None if dent is None else dent.contiguous()
+    _ops.launch(z, "nsa_logprob_bwd", z.data_ptr(), L.addr(targets), stat.data_ptr(), ent.data_ptr(), L.addr(dlogp),
+                L.addr(dent), dz.data_ptr(), rows, V, _CODE[z.dtype])
+    return dz, None, None
+
+
 class TokenLogprobsHIP(torch.autograd.Function):
     """``(logp, entropy, top_logp, top_idx)`` of dense ``z [rows, V]``."""
 
     @staticmethod
     def forward(ctx, z, targets, top):
         ctx.set_materialize_grads(False)
-        z = z.contiguous()
-        rows, V = z.shape
-        f32 = dict(device=z.device, dtype=torch.float32)
-        logp = None if targets is None else torch.empty(rows, **f32)
-        ent, stat = torch.empty(rows, **f32), torch.empty(rows, 2, **f32)
-        top_logp = torch.empty(rows, top, **f32)
-        top_idx = torch.empty(rows, top, device=z.device, dtype=torch.int64)
-        with _ops.device_of(z):
-            nbytes = int(_ops._lib().nsa_logprob_workspace(rows, V, top, _ops._stream(z)))
-            assert nbytes > 0, "token_logprobs: unsupported shape"
-            ws = torch.empty(nbytes, device=z.device, dtype=torch.uint8)
-            _ops._call("nsa_logprob_fwd", _ops._lib().nsa_logprob_fwd, L.ptr(z), L.ptr(targets), L.ptr(logp),
-                       L.ptr(ent), L.ptr(stat), L.ptr(top_logp), L.ptr(top_idx), L.ptr(ws), nbytes, rows, V, top,
-                       _code(z.dtype), _ops._stream(z))
+        logp, ent, top_logp, top_idx, stat = _logprob_fwd(z, targets, top)
         ctx.save_for_backward(z, targets, stat, ent)
-        ctx.mark_non_differentiable(top_logp, top_idx)
+        if top:
+            ctx.mark_non_differentiable(top_logp, top_idx)
         return logp, ent, top_logp, top_idx
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, dlogp, dent, _dtop, _didx):
-        z, targets, stat, ent = ctx.saved_tensors
-        if dlogp is None and dent is None:
-            return None, None, None
-        rows, V = z.shape
-        dz = torch.empty_like(z)
-        dlogp, dent = (None if d is None else d.float().contiguous() for d in (dlogp, dent))
-        with _ops.device_of(z):
-            _ops._call("nsa_logprob_bwd", _ops._lib().nsa_logprob_bwd, L.ptr(z), L.ptr(targets), L.ptr(stat),
-                       L.ptr(ent), L.ptr(dlogp), L.ptr(dent), L.ptr(dz), rows, V, _code(z.dtype), _ops._stream(z))
-        return dz, None, None
+    def backward(ctx, *grads):
+        if torch.is_grad_enabled():      # (create_graph: a second derivative is refused when it is taken)
+            return once_differentiable(_logprob_bwd)(ctx, *grads)
+        return _logprob_bwd(ctx, *grads)
 
 
 def token_logprobs(logits, targets=None, top=0):
@@ -230,7 +259,13 @@ def token_logprobs(logits, targets=None, top=0):
         assert targets.dtype in (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8), \
             "token_logprobs: targets must be integers"
         assert targets.shape == lead, "token_logprobs: one target for each row"
-        targets = targets.reshape(-1).long().contiguous()
-    logp, ent, top_logp, top_idx = TokenLogprobsHIP.apply(logits.reshape(-1, V), targets, top)
+        targets = targets.reshape(-1).long()
+    z = logits.reshape(-1, V).contiguous()
+    if _wants_grad(logits):
+        logp, ent, top_logp, top_idx = TokenLogprobsHIP.apply(z, targets, top)
+    else:
+        logp, ent, top_logp, top_idx, _ = _logprob_fwd(z, targets, top)
+    if len(lead) == 1:
+        return TokenLogprobs(logp, ent, top_logp, top_idx)
     return TokenLogprobs(None if logp is None else logp.view(lead), ent.view(lead),
                          top_logp.view(*lead, top) if top else None, top_idx.view(*lead, top) if top else None)

@@ -65,14 +65,12 @@ def _attend(q, rows, k_pages, v_pages, table, lens, scale, return_lse):
     out = torch.empty_like(q)
     lse = torch.empty(B, Hq, device=q.device, dtype=torch.float32) if return_lse else None
     if B > 0:
-        with _ops.device_of(q):
-            lib, stream = _ops._lib(), _ops._stream(q)
-            nbytes = int(lib.nsa_paged_workspace(B, Hq, Hkv, D, P, mp, stream))
-            ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
-            _ops._call("nsa_paged_attend", lib.nsa_paged_attend, L.ptr(q), L.ptr(kn), L.ptr(vn), L.ptr(k_pages),
-                       L.ptr(v_pages), L.ptr(table), L.ptr(lens), L.ptr(lens_out), L.ptr(out), L.ptr(lse), L.ptr(ws),
-                       nbytes, B, Hq, Hkv, D, P, mp, n, D ** -0.5 if scale is None else float(scale),
-                       L.dtype_code(q), stream)
+        nbytes = _ops.launch(q, "nsa_paged_workspace", B, Hq, Hkv, D, P, mp)
+        ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes > 16 else None
+        _ops.launch(q, "nsa_paged_attend", q.data_ptr(), L.addr(kn), L.addr(vn), k_pages.data_ptr(),
+                    v_pages.data_ptr(), table.data_ptr(), lens.data_ptr(), L.addr(lens_out), out.data_ptr(),
+                    L.addr(lse), L.addr(ws), nbytes, B, Hq, Hkv, D, P, mp, n, D ** -0.5 if scale is None else scale,
+                    L.NSA_BF16 if q.dtype == torch.bfloat16 else L.NSA_F32)
     return out, lse, lens_out
 
 
@@ -115,10 +113,9 @@ def paged_append(k, v, k_pages, v_pages, table, lens, count=None):
         count = count.contiguous()
     lens_out = torch.empty_like(lens)
     if B > 0:
-        with _ops.device_of(k_pages):
-            _ops._call("nsa_paged_append", _ops._lib().nsa_paged_append, L.ptr(k), L.ptr(v), L.ptr(k_pages),
-                       L.ptr(v_pages), L.ptr(table), L.ptr(lens), L.ptr(count), L.ptr(lens_out), B, Hkv, k.shape[2], D,
-                       P, mp, n, L.dtype_code(k_pages), _ops._stream(k_pages))
+        _ops.launch(k_pages, "nsa_paged_append", k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                    table.data_ptr(), lens.data_ptr(), L.addr(count), lens_out.data_ptr(), B, Hkv, k.shape[2], D, P, mp,
+                    n, L.NSA_BF16 if k.dtype == torch.bfloat16 else L.NSA_F32)
     return lens_out
 
 
