@@ -20,9 +20,11 @@
 // have doubled: 16 ballots, one for each of the upper bits of a value's key.  A row that overfills the list (long ties, a rising
 // row) is selected exactly by eight radix passes over the keys instead.
 //
-// One wave takes a row of up to 2048 elements; a workgroup of four takes a
-// longer one.  Where the rows are too few to fill the chip, a row is split
-// over workgroups and a second launch joins their (m, l, s) and lists.
+// One wave takes a row of up to 2048 elements, a workgroup of four or sixteen a
+// longer one; few and very long rows are split over workgroups, whose (m, l, s)
+// and lists a second launch joins.
+#include <type_traits>
+
 #include "nsa_launch.h"
 #include "nsa_rows.h"
 
@@ -114,11 +116,11 @@ __device__ __forceinline__ void lp_rank(const uint64_t* list, int count, int k, 
   }
 }
 
-// W waves a row (1: four rows a workgroup); U runs of 8 a lane and chunk.
+// W waves a row (1: four rows a workgroup of 256 threads); U runs of 8 a lane and chunk.
 template <typename T, int W, int U, bool TOP>
-__global__ __launch_bounds__(256) void k_logprob(const LpArgs a) {
+__global__ __launch_bounds__(W > 4 ? 64 * W : 256, W > 4 ? 4 : 8) void k_logprob(const LpArgs a) {
   constexpr int THR = 64 * W;               // threads a row
-  constexpr int ROWS = 256 / THR;           // rows a workgroup
+  constexpr int ROWS = W > 1 ? 1 : 4;       // rows a workgroup
   constexpr int CAP = W > 1 ? kLpCap : 512;
   __shared__ uint64_t list_s[TOP ? ROWS : 1][TOP ? CAP : 1];
   __shared__ uint32_t keys_s[2][TOP && W > 1 ? THR : 1];
@@ -150,12 +152,33 @@ __global__ __launch_bounds__(256) void k_logprob(const LpArgs a) {
   int next = 1;                 // chunks done at the bound's next forming
   int done = 0, turn = 0;
   constexpr int CH = THR * 8 * U;
-  for (int c = c0; c < c1; c += CH) {
+  // runs start at 16-byte addresses, the first one up to 7 elements before c0: odd rows otherwise cost a second
+  // cache line a run
+  const int cs = c0 - (int)((reinterpret_cast<uintptr_t>(z + c0) & 15) / sizeof(T));
+  // Elements at .. at + 7 of the row, -inf for those outside [c0, c1).
+  auto load = [&](int at, float(&y)[8]) {
+    if (at >= c0 && at + 8 <= c1) {
+      load_run8(z + at, y);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = -__builtin_inff();
+      if (at + 8 > c0 && at < c1) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (at + j >= c0 && at + j < c1) y[j] = (float)z[at + j];
+      }
+    }
+  };
+  auto chunk = [&](auto whole, int c) {   // whole: every run of the chunk is
+    constexpr bool kWhole = decltype(whole)::value;
     float x[U][8];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int at = c + 8 * (u * THR + t);
-      load_run8(z + at, c1 - at, x[u], -__builtin_inff());
+      if (kWhole)
+        load_run8(z + at, x[u]);
+      else
+        load(at, x[u]);
     }
     float mxu[U], mx;
 #pragma unroll
@@ -176,11 +199,14 @@ __global__ __launch_bounds__(256) void k_logprob(const LpArgs a) {
         st.s += e * fmaxf(d, kFar);
       }
     if (TOP) {
+      // the sums end here: left to itself the compiler carries their 32 terms past the bound, at 117 registers and
+      // half the waves (69 registers with this line)
+      asm volatile("" : "+v"(st.l), "+v"(st.s));
       ++done;
       if (done == next) {
         // The k-th largest of the lanes' maxima, by the upper halves of their keys.  (A lane that
         // holds NaN counts with its largest other value: still one of its elements' keys or less.)
-        const bool any = c0 + 8 * t < c1;
+        const bool any = cs + 8 * t < c1;
         uint32_t v[W];
         v[0] = any ? value_key(st.l == 0.0f ? -__builtin_inff() : st.m) >> 16 : 0u;
         if (W > 1) {
@@ -204,23 +230,34 @@ __global__ __launch_bounds__(256) void k_logprob(const LpArgs a) {
         thr_z = thr == 0u ? -__builtin_inff() : key_value((uint64_t)thr << 32);
         next *= 2;
       }
-      const bool nan = st.l != st.l;
-      if (!(mx < thr_z) || nan) {
+      // the runs with an element at or above the bound: few, read again through the cache so that the
+      // streaming loop keeps its registers
+      uint32_t runs = 0;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (mxu[u] < thr_z && !nan) continue;
+      for (int u = 0; u < U; ++u) runs |= (mxu[u] < thr_z ? 0u : 1u) << u;
+      if (st.l != st.l) runs = (1u << U) - 1;
+      while (runs != 0) {
+        const int at = c + 8 * ((__ffs(runs) - 1) * THR + t);
+        runs &= runs - 1;
+        float y[8];
+        load(at, y);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int at = c + 8 * (u * THR + t) + j;
-            if (at < c1 && value_key(x[u][j]) >= thr) {
-              const int i = atomicAdd(&count_s[sub], 1);
-              if (i < CAP) list[i] = elem_key(x[u][j], at);
-            }
+        for (int j = 0; j < 8; ++j) {
+          if (at + j >= c0 && at + j < c1 && value_key(y[j]) >= thr) {
+            const int i = atomicAdd(&count_s[sub], 1);
+            if (i < CAP) list[i] = elem_key(y[j], at + j);
           }
         }
       }
     }
+  };
+  int c = cs;
+  if (c < c0 && c < c1) {
+    chunk(std::false_type{}, c);
+    c += CH;
   }
+  for (; c + CH <= c1; c += CH) chunk(std::true_type{}, c);
+  if (c < c1) chunk(std::false_type{}, c);
 
   // the row's (or the part's) sums
   st = lp_wave(st);
@@ -392,50 +429,38 @@ __global__ __launch_bounds__(256) void k_logprob_bwd(const LpBwdArgs a) {
   }
 }
 
-// Parts of a row: as many as bring the launch to four workgroups a compute
-// unit, each a whole number of 2048-element chunks; at most as many as the
-// join's list in LDS holds.
-static int lp_parts(int64_t rows, int V, int k, int cu) {
-  if (V <= 2048) return 1;
-  int64_t want = (4LL * cu + rows - 1) / rows;
-  const int chunks = (V + 2047) / 2048;
+// Waves of a row: one up to 2048 elements; sixteen where the rows leave most of
+// the chip's waves idle (a row of 32000 in 16 bits is then one chunk); else four.
+// A row of more than 256 KiB is split where there are not enough of them
+// either, into parts of 8192 elements or more, two for every compute unit: one
+// workgroup's loads would take longer than the second launch.
+static int lp_waves(int64_t rows, int V, int cu) { return V <= 2048 ? 1 : rows <= 2 * cu ? 16 : 4; }
+static int lp_parts(int64_t rows, int V, int esize, int cu) {
+  if ((int64_t)V * esize <= 256 * 1024 || rows >= 2 * cu) return 1;
+  int64_t want = (2LL * cu + rows - 1) / rows;
+  const int chunks = (V + 8191) / 8192;
   if (want > chunks) want = chunks;
-  const int most = k > 0 ? (4096 / k < 64 ? 4096 / k : 64) : 64;
-  if (want > most) want = most;
-  if (want <= 1) return 1;
+  if (want > 64) want = 64;   // a lane each in the join
   const int per = (int)((chunks + want - 1) / want);
   return (chunks + per - 1) / per;
 }
 static int lp_seg(int V, int nsp) {
   if (nsp <= 1) return V;
-  const int chunks = (V + 2047) / 2048;
-  return ((chunks + nsp - 1) / nsp) * 2048;
+  const int chunks = (V + 8191) / 8192;
+  return ((chunks + nsp - 1) / nsp) * 8192;
 }
 
-template <typename T>
+template <typename T, bool TOP>
 static int logprob_launch(LpArgs a, hipStream_t s) {
-  if (a.V <= 2048) {
-    const int64_t grid = (a.rows + 3) / 4;
-    if (a.k > 0)
-      k_logprob<T, 1, 4, true><<<(unsigned)grid, 256, 0, s>>>(a);
-    else
-      k_logprob<T, 1, 4, false><<<(unsigned)grid, 256, 0, s>>>(a);
-    return nsa_launch_status();
-  }
-  const int64_t grid = a.rows * a.nsp;
-  // a part of one or two chunks takes its elements as runs of its own chunks; a long row four runs at a time
-  const bool small = a.seg <= 4096;
-  if (a.k > 0) {
-    if (small)
-      k_logprob<T, 4, 1, true><<<(unsigned)grid, 256, 0, s>>>(a);
-    else
-      k_logprob<T, 4, 4, true><<<(unsigned)grid, 256, 0, s>>>(a);
-  } else {
-    if (small)
-      k_logprob<T, 4, 1, false><<<(unsigned)grid, 256, 0, s>>>(a);
-    else
-      k_logprob<T, 4, 4, false><<<(unsigned)grid, 256, 0, s>>>(a);
-  }
+  const int w = a.nsp > 1 ? 4 : lp_waves(a.rows, a.V, device_cu_count(s));
+  if (w == 1)
+    k_logprob<T, 1, 4, TOP><<<(unsigned)((a.rows + 3) / 4), 256, 0, s>>>(a);
+  else if (w == 4)
+    // runs in flight against waves: 2047 x 50257 with 5 alternatives takes 58 us at four runs, 54 at three, 56 at
+    // two; 8192 x 32000 without them 105, 109 and 101
+    k_logprob<T, 4, TOP ? 3 : 2, TOP><<<(unsigned)(a.rows * a.nsp), 256, 0, s>>>(a);
+  else
+    k_logprob<T, 16, 4, TOP><<<(unsigned)a.rows, 1024, 0, s>>>(a);
   if (a.nsp > 1) k_logprob_join<T><<<(unsigned)a.rows, 64, (size_t)a.nsp * a.k * 8, s>>>(a);
   return nsa_launch_status();
 }
@@ -450,7 +475,7 @@ extern "C" size_t nsa_logprob_workspace(int64_t rows, int V, int k, void* stream
   using namespace nsa;
   if (!lp_shape_ok(rows, V, k)) return 0;
   if (rows == 0) return 16;
-  const int nsp = lp_parts(rows, V, k, device_cu_count(static_cast<hipStream_t>(stream)));
+  const int nsp = lp_parts(rows, V, 4, device_cu_count(static_cast<hipStream_t>(stream)));   // (float32: no fewer)
   return nsp <= 1 ? 16 : (size_t)rows * nsp * (16 + 8 * (size_t)k);
 }
 
@@ -464,7 +489,7 @@ extern "C" int nsa_logprob_fwd(const void* z, const int64_t* target, float* logp
   NSA_CHECK(z != nullptr && stat != nullptr && (logp == nullptr || target != nullptr), NSA_ERR_ARG);
   NSA_CHECK(k == 0 || (top_logp != nullptr && top_idx != nullptr), NSA_ERR_ARG);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const int nsp = lp_parts(rows, V, k, device_cu_count(s));
+  const int nsp = lp_parts(rows, V, dtype == NSA_BF16 ? 2 : 4, device_cu_count(s));
   LpArgs a{z, target, logp, entropy, reinterpret_cast<float2*>(stat), top_logp, top_idx, nullptr, nullptr, rows, V,
            k, nsp, lp_seg(V, nsp)};
   if (nsp > 1) {
@@ -472,7 +497,8 @@ extern "C" int nsa_logprob_fwd(const void* z, const int64_t* target, float* logp
     a.part = static_cast<float4*>(workspace);
     a.part_top = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + (size_t)rows * nsp * 16);
   }
-  return dtype == NSA_BF16 ? logprob_launch<bf16>(a, s) : logprob_launch<float>(a, s);
+  if (dtype == NSA_BF16) return k > 0 ? logprob_launch<bf16, true>(a, s) : logprob_launch<bf16, false>(a, s);
+  return k > 0 ? logprob_launch<float, true>(a, s) : logprob_launch<float, false>(a, s);
 }
 
 extern "C" int nsa_logprob_bwd(const void* z, const int64_t* target, const float* stat, const float* entropy,

@@ -211,8 +211,15 @@ def test_shapes_strides_and_types():
     off[1:] = zd.flatten()
     for other in (wide[:, 3:336], off[1:].view(24, 333), zd.t().contiguous().t()):
         o = nsa_lm.token_logprobs(other, td, 4)
-        for a, b in zip(o, ref):
-            assert torch.equal(a.flatten(), b.flatten())
+        # the lanes' runs follow the addresses, and the order of a row's sum with them: each result is within
+        # (CHAIN + 6) u (logp, top_logp; 2 u of its terms, below 20, besides) and (2 CHAIN + 20) u 20 (entropy, S
+        # below 20) of the value, so two of them are within twice that
+        assert torch.equal(o.top_idx, ref.top_idx)
+        C = _chain(333)
+        for a, b, tol in ((o.logp, ref.logp, C + 46), (o.top_logp, ref.top_logp, C + 46),
+                          (o.entropy, ref.entropy, C + 46 + (2 * C + 20) * 20)):
+            fin = torch.isfinite(b)
+            assert torch.equal(fin, torch.isfinite(a)) and float((a - b)[fin].abs().max()) <= 2 * tol * U
     for a, b in zip(got, ref):
         assert torch.equal(a.flatten(), b.flatten())
     one = nsa_lm.token_logprobs(zd[0], td[0], 2)
