@@ -579,7 +579,7 @@ int nsa_logprob_bwd(const void* z, const int64_t* target, const float* stat, con
  * a length are never read.  lse (float [B][Hq], nullable): ln sum e^score, -1e9
  * where there is no key.  lens and lens_out are different buffers.
  * workspace: nsa_paged_workspace bytes (0: unsupported shape). */
-size_t nsa_paged_workspace(int B, int Hq, int Hkv, int D, int P, int max_pages, void* stream);
+size_t nsa_paged_workspace(int B, int Hq, int Hkv, int D, int P, int max_pages, int dtype, void* stream);
 int nsa_paged_attend(const void* q, const void* k_new, const void* v_new, void* k_pages, void* v_pages,
                      const int32_t* table, const int32_t* lens, int32_t* lens_out, void* out, float* lse,
                      void* workspace, size_t workspace_bytes, int B, int Hq, int Hkv, int D, int P, int max_pages,

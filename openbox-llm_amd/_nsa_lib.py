@@ -108,7 +108,7 @@ SIGNATURES = {
     "nsa_logprob_workspace": (_Z, [_L, _I, _I, _P]),
     "nsa_logprob_fwd": (_I, [_P] * 8 + [_Z, _L, _I, _I, _I, _P]),
     "nsa_logprob_bwd": (_I, [_P] * 7 + [_L, _I, _I, _P]),
-    "nsa_paged_workspace": (_Z, [_I] * 6 + [_P]),
+    "nsa_paged_workspace": (_Z, [_I] * 7 + [_P]),
     "nsa_paged_attend": (_I, [_P] * 11 + [_Z] + [_I] * 7 + [_F, _I, _P]),
     "nsa_paged_append": (_I, [_P] * 8 + [_I] * 8 + [_P]),
 }

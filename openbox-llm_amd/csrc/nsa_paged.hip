@@ -6,12 +6,15 @@
 //   lens   [B]                   keys of each sequence before the step
 //   out[b][h] = softmax(scale q K^T) V over the keys 0 .. n-1 of KV head h / (Hq / Hkv)
 //
-// A step is bound by reading each key and value row once.  A workgroup of four
-// waves takes a chunk of one sequence's keys for one KV head (and up to 32 of
-// its query heads); each wave takes tiles of 32 keys in turn, with the running
-// maximum and sum of the softmax, and the four are joined in LDS.  With more
-// than one chunk the unnormalised outputs go to the workspace and a second
-// launch joins them.
+// A step is bound by reading each key and value row once.  The keys of all
+// sequences and KV heads (and head tiles of up to 32 query heads) are one list
+// of units of 128 keys, cut into equal shares, one to a workgroup: sequences of
+// unlike lengths then end together.  A share is a few pieces, each of one
+// sequence and head; within a piece each of the four waves takes tiles of 32
+// keys in turn, with the running maximum and sum of the softmax, and the four
+// are joined in LDS.  A sequence and head whose keys are one piece is written
+// out at once; else the pieces' unnormalised outputs go to the workspace and a
+// second launch joins them.
 //
 // Rows go from memory to the matrix operands without LDS.  K: lane (g, c) of
 // S^T = K Q^T holds 8 d of key c, so 16 bytes of the row.  V: O^T = V^T P^T wants 8
@@ -34,6 +37,8 @@
 
 namespace nsa {
 
+constexpr int kUnit = 128;   // keys of a unit: a tile for each wave
+
 struct PagedArgs {
   const void *q, *k_new, *v_new;     // [B][Hq][D], [B][Hkv][D] (null: no append)
   void *kp, *vp;
@@ -41,12 +46,32 @@ struct PagedArgs {
   int32_t* lens_out;                 // or null
   void* out;
   float* lse;                        // or null
-  float* part_o;                     // [B][Hq][nsp][D]
-  float2* part_ml;                   // [B][Hq][nsp]
+  float* part_o;                     // [W + R][16 NT][D]: piece of share w and row r at w + r
+  float2* part_ml;                   // [W + R][16 NT]
+  int2* row_info;                    // [R] first and last share of a row in pieces, (-1, -1) of one piece
   int B, Hq, Hkv, G, HT, P, rpp;     // HT: head tiles of a KV head; rpp: runs of 16 in a page
-  int max_pages, n_pages, nsp, chunk;
+  int max_pages, n_pages, W;         // W: shares of the list, or 0: a workgroup a row
   float sl2;                         // scale * log2 e
 };
+
+// Keys that sequence b attends, twice, plus 1 where the last of them is the row it appends.
+__device__ __forceinline__ uint32_t paged_keys(const PagedArgs& a, int b) {
+  const int cap = a.max_pages * a.P;
+  const int len = a.lens[b];
+  if (a.k_new != nullptr &&
+      paged_new_pos(a.table + (int64_t)b * a.max_pages, len, a.P, a.max_pages, a.n_pages) >= 0)
+    return 2u * ((uint32_t)len + 1u) + 1u;
+  return 2u * (uint32_t)(len < 0 ? 0 : (len < cap ? len : cap));
+}
+// Units of a row of n keys: one at least, so that an empty row is written too.
+__device__ __forceinline__ int paged_units(uint32_t keys) {
+  const int n = (int)(keys >> 1);
+  return n <= kUnit ? 1 : (n + kUnit - 1) / kUnit;
+}
+
+__device__ __forceinline__ float paged_lse(float m, float l) {
+  return l > 0.0f ? (m + __log2f(l)) * kLn2 : (l == 0.0f ? kLseEmpty : l);   // (NaN stays)
+}
 
 __device__ __forceinline__ int64_t run_base(const PagedArgs& a, int b, int hkv, int run, int D) {
   return paged_run(a.table + (int64_t)b * a.max_pages, run, a.rpp, a.max_pages, a.n_pages, a.Hkv, hkv, D);
@@ -87,263 +112,391 @@ template <typename T, int VL> __device__ __forceinline__ VRun<T, VL> vrun_zero()
   return r;
 }
 
-// K operands and V rows of one tile of 32 keys
-template <typename T, int D> struct KVTile {
-  Frag<T> k[2][Dims<D>::KC];
-  VRun<T, D / 16> v[8];
-};
-
 // NT: tiles of 16 query heads.
 template <typename T, int D, int NT>
-__global__ __launch_bounds__(256) void k_paged(const PagedArgs a) {
+__global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
   constexpr int KC = Dims<D>::KC, DT = Dims<D>::DT, VL = D / 16;
   constexpr bool SPLIT_P = sizeof(T) == 2;
+  constexpr int QF = sizeof(Frag<T>) / 16;           // 16-byte pieces of an operand
+  __shared__ f32x4 qs[NT][KC][QF][64];                // the queries as operands, one piece a lane
+  __shared__ float so[4][16][D + 4];                  // the waves' outputs
+  __shared__ float sm[4][16], sl[4][16];
+  __shared__ int64_t wsum[4], found[2];
+  __shared__ uint32_t seq_keys[256];                  // of every sequence, where there are no more than 256
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int64_t bid = blockIdx.x;
-  const int sp = (int)(bid % a.nsp);
-  bid /= a.nsp;
-  const int ht = (int)(bid % a.HT);
-  bid /= a.HT;
-  const int hkv = (int)(bid % a.Hkv), b = (int)(bid / a.Hkv);
-
-  const int cap = a.max_pages * a.P;
-  const int len = a.lens[b];
-  int n = len < 0 ? 0 : (len < cap ? len : cap);     // keys attended
-  int pos = -1;                                      // the appended row's position
-  if (a.k_new != nullptr) {
-    pos = paged_new_pos(a.table + (int64_t)b * a.max_pages, len, a.P, a.max_pages, a.n_pages);
-    if (pos >= 0) n = len + 1;
-  }
-  if (a.lens_out != nullptr && sp == 0 && ht == 0 && hkv == 0 && threadIdx.x == 0) a.lens_out[b] = pos >= 0 ? n : len;
-  const int c0 = sp * a.chunk;
-  const int c1 = n < c0 + a.chunk ? n : c0 + a.chunk;
-  if (c0 >= c1 && sp > 0) return;                    // (uniform; part 0 of an empty sequence writes its zeros)
-
+  const int M = a.Hkv * a.HT;                         // rows of a sequence
   const T* kp = static_cast<const T*>(a.kp);
   const T* vp = static_cast<const T*>(a.vp);
-  const T* kn = static_cast<const T*>(a.k_new) + ((int64_t)b * a.Hkv + hkv) * D;
-  const T* vn = static_cast<const T*>(a.v_new) + ((int64_t)b * a.Hkv + hkv) * D;
 
-  // the append: one wave of the first head tile whose chunk holds the position
-  if (pos >= c0 && pos < c1 && ht == 0 && w == 0) {
-    const int64_t at = run_base(a, b, hkv, pos >> 4, D) + (int64_t)(pos & 15) * D;
-    for (int d = lane; d < D; d += 64) {
-      static_cast<T*>(a.kp)[at + d] = kn[d];
-      static_cast<T*>(a.vp)[at + d] = vn[d];
+  // This workgroup's units: [x, x1) of the list, the first of them in row m of
+  // sequence b, whose `units` units start at row0.
+  int64_t x, x1, row0, U = 0, W = 0;
+  int b, m, units;
+  uint32_t keys;
+  if (a.W == 0) {                                     // a row each: the list is that row
+    b = (int)(blockIdx.x / (unsigned)M);
+    m = (int)(blockIdx.x % (unsigned)M);
+    keys = paged_keys(a, b);
+    units = paged_units(keys);
+    x = row0 = 0;
+    x1 = units;
+  } else {
+    // Each thread counts the units of its sequences; the one whose range holds x finds the sequence.
+    const int per = (a.B + 255) / 256;
+    const int b_lo = min(a.B, (int)threadIdx.x * per), b_hi = min(a.B, b_lo + per);
+    int64_t mine = 0;
+    for (int i = b_lo; i < b_hi; ++i) {
+      keys = paged_keys(a, i);
+      mine += paged_units(keys);
     }
-  }
-
-  Frag<T> qf[NT][KC];
+    if (per == 1 && b_lo < b_hi) seq_keys[b_lo] = keys;
+    int64_t incl = mine;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int hg = ht * 16 * NT + 16 * nt + c;
-    const T* row = hg < a.G ? static_cast<const T*>(a.q) + ((int64_t)b * a.Hq + (int64_t)hkv * a.G + hg) * D : nullptr;
-    load_row_frags<T, D>(qf[nt], row, g);
-  }
-  FwdAcc<D> acc[NT];
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t v = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 63) wsum[w] = incl;
+    __syncthreads();
+    int64_t before = incl - mine;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) acc[nt].init();
-
-  // this wave's tiles: 32 keys every 128; lane i looks up run i of them
-  const int my0 = c0 + 32 * w;
-  const int ntile = c1 > my0 ? (c1 - my0 + 127) / 128 : 0;
-  int64_t base = -1;
-  {
-    const int key = my0 + 128 * (lane >> 1) + 16 * (lane & 1);
-    if ((lane >> 1) < ntile && key < c1) base = run_base(a, b, hkv, key >> 4, D);
-  }
-  const int kofs0 = ((8 * (c >> 2)) & 15) + (c & 3);
-  for (int i = 0; i < ntile; ++i) {
-    const int kb = my0 + 128 * i;
-    const int64_t b0 = __shfl(base, 2 * i, 64), b1 = __shfl(base, 2 * i + 1, 64);
-    KVTile<T, D> t;
-    const int64_t bk = c >= 8 ? b1 : b0, bv = g >= 2 ? b1 : b0;
-    // keys of this tile that this lane's K rows (m) and V rows may be read for
-    const bool whole = kb + 32 <= c1 && b0 >= 0 && b1 >= 0 && !(pos >= kb && pos < kb + 32);
-    if (whole) {
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int kc = 0; kc < KC; ++kc) {
-          if (32 * kc + 8 * g < D)
-            t.k[mt][kc].load(kp + bk + (kofs0 + 4 * mt) * D + 32 * kc + 8 * g);
-          else
-            t.k[mt][kc].zero();
-        }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) t.v[j] = vrun_load<T, VL>(vp + bv + (((8 * g) & 15) + j) * D + VL * c);
-    } else {
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        const int key = kb + 8 * (c >> 2) + 4 * mt + (c & 3);
-        const T* row = key == pos ? kn : (key < c1 && bk >= 0 ? kp + bk + (kofs0 + 4 * mt) * D : nullptr);
-#pragma unroll
-        for (int kc = 0; kc < KC; ++kc) {
-          if (row != nullptr && 32 * kc + 8 * g < D)
-            t.k[mt][kc].load(row + 32 * kc + 8 * g);
-          else
-            t.k[mt][kc].zero();
+    for (int i = 0; i < 4; ++i) {
+      if (i < w) before += wsum[i];
+      U += wsum[i];
+    }
+    U *= M;
+    before *= M;
+    W = U < a.W ? U : a.W;                            // shares of one unit at least: a row's pieces have no gaps
+    if (blockIdx.x >= W) return;                      // (uniform)
+    x = (int64_t)blockIdx.x * U / W;
+    x1 = ((int64_t)blockIdx.x + 1) * U / W;
+    if (x >= before && x < before + mine * M) {
+      int i = b_lo;
+      if (per > 1) {
+        for (;; ++i) {
+          const int64_t u = (int64_t)paged_units(paged_keys(a, i)) * M;
+          if (x < before + u) break;
+          before += u;
         }
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int key = kb + 8 * g + j;
-        const T* row = key == pos ? vn : (key < c1 && bv >= 0 ? vp + bv + (((8 * g) & 15) + j) * D : nullptr);
-        t.v[j] = row != nullptr ? vrun_load<T, VL>(row + VL * c) : vrun_zero<T, VL>();
-      }
+      found[0] = i;
+      found[1] = before;
     }
-    // visible keys kb + 8 g .. + 7 of this lane
-    const uint32_t vm = bv >= 0 ? range_mask(kb + 8 * g, 0, c1 - 1) : 0u;
-    Frag<T> vf[DT];
+    __syncthreads();
+    b = __builtin_amdgcn_readfirstlane((int)found[0]);
+    keys = a.B <= 256 ? (uint32_t)__builtin_amdgcn_readfirstlane((int)seq_keys[b]) : paged_keys(a, b);
+    units = paged_units(keys);
+    m = (int)((x - found[1]) / units);
+    row0 = found[1] + (int64_t)m * units;
+  }
+
+  while (x < x1) {
+    const int hkv = m / a.HT, ht = m - hkv * a.HT;
+    const int t0 = (int)(x - row0);
+    const int t1 = x1 - row0 < units ? (int)(x1 - row0) : units;
+    const bool one = t0 == 0 && t1 == units;          // the row in one piece
+    const int n = (int)(keys >> 1), pos = (keys & 1u) ? n - 1 : -1;
+    const int c0 = kUnit * t0, c1 = min(n, kUnit * t1);
+    const int row = b * M + m;
+    if (t0 == 0 && threadIdx.x == 0) {
+      if (a.row_info != nullptr)
+        a.row_info[row] = one ? make_int2(-1, -1) : make_int2((int)blockIdx.x, (int)(((row0 + units) * W - 1) / U));
+      if (a.lens_out != nullptr && m == 0) a.lens_out[b] = pos >= 0 ? n : a.lens[b];
+    }
+    const T* kn = static_cast<const T*>(a.k_new) + ((int64_t)b * a.Hkv + hkv) * D;
+    const T* vn = static_cast<const T*>(a.v_new) + ((int64_t)b * a.Hkv + hkv) * D;
+
+    // this wave's tiles: 32 keys every 128; lane i looks up run i of the current 32 tiles
+    const int my0 = c0 + 32 * w;
+    const int ntile = c1 > my0 ? (c1 - my0 + kUnit - 1) / kUnit : 0;
+    int64_t base = -1;
+    auto look_up = [&](int i) {   // runs of tiles i .. i + 31
+      const int tile = i + (lane >> 1), key = my0 + kUnit * tile + 16 * (lane & 1);
+      base = tile < ntile && key < c1 ? run_base(a, b, hkv, key >> 4, D) : -1;
+    };
+    auto run_at = [&](int i) -> int64_t {   // (i uniform, of the current 32 tiles)
+      const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)base, i & 63);
+      const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)base >> 32), i & 63);
+      return (int64_t)(((uint64_t)hi << 32) | lo);
+    };
+    // whether all of tile i's rows may be read from their pages
+    auto whole = [&](int i) {
+      const int kb = my0 + kUnit * i;
+      return kb + 32 <= c1 && run_at(2 * i) >= 0 && run_at(2 * i + 1) >= 0 && !(pos >= kb && pos < kb + 32);
+    };
+    Frag<T> kf[2][KC];       // keys kb + 8 (c >> 2) + 4 mt + (c & 3)
+    VRun<T, VL> vr[8];       // keys kb + 8 g + j
+    auto load_k = [&](int i) {
+      const int64_t base_k = c >= 8 ? run_at(2 * i + 1) : run_at(2 * i);
+      const int ofs = ((8 * (c >> 2)) & 15) + (c & 3);
+      if (whole(i)) {
+        const T* row = kp + base_k + ofs * D + 8 * g;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      if constexpr (sizeof(T) == 2) {
+        for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) vf[dt].v[j] = vrun_elem<T, VL>(t.v[j], dt);
+          for (int kc = 0; kc < KC; ++kc) {
+            if (32 * kc + 8 * g < D)
+              kf[mt][kc].load(row + 4 * mt * D + 32 * kc);
+            else
+              kf[mt][kc].zero();
+          }
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          vf[dt].lo[j] = vrun_elem<T, VL>(t.v[j], dt);
-          vf[dt].hi[j] = vrun_elem<T, VL>(t.v[4 + j], dt);
+        for (int mt = 0; mt < 2; ++mt) {
+          const int key = my0 + kUnit * i + 8 * (c >> 2) + 4 * mt + (c & 3);
+          const T* row = key == pos ? kn : (key < c1 && base_k >= 0 ? kp + base_k + (ofs + 4 * mt) * D : nullptr);
+#pragma unroll
+          for (int kc = 0; kc < KC; ++kc) {
+            if (row != nullptr && 32 * kc + 8 * g < D)
+              kf[mt][kc].load(row + 32 * kc + 8 * g);
+            else
+              kf[mt][kc].zero();
+          }
         }
       }
+    };
+    auto load_v = [&](int i) {
+      const int64_t base_v = g >= 2 ? run_at(2 * i + 1) : run_at(2 * i);
+      const int ofs = (8 * g) & 15;
+      if (whole(i)) {
+        const T* row = vp + base_v + ofs * D + VL * c;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) vr[j] = vrun_load<T, VL>(row + j * D);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int key = my0 + kUnit * i + 8 * g + j;
+          const T* row = key == pos ? vn : (key < c1 && base_v >= 0 ? vp + base_v + (ofs + j) * D : nullptr);
+          vr[j] = row != nullptr ? vrun_load<T, VL>(row + VL * c) : vrun_zero<T, VL>();
+        }
+      }
+    };
+    if (ntile > 0) {
+      look_up(0);
+      load_k(0);
+      load_v(0);
     }
+
+    // the append: one wave of the first head tile's piece that holds the position
+    if (pos >= c0 && pos < c1 && ht == 0 && w == 0) {
+      const int64_t at = run_base(a, b, hkv, pos >> 4, D) + (int64_t)(pos & 15) * D;
+      for (int d = lane; d < D; d += 64) {
+        static_cast<T*>(a.kp)[at + d] = kn[d];
+        static_cast<T*>(a.vp)[at + d] = vn[d];
+      }
+    }
+
+    // queries to LDS: wave w takes every fourth operand
+#pragma unroll
+    for (int f = 0; f < NT * KC; ++f) {
+      if ((f & 3) == w) {
+        const int nt = f / KC, kc = f % KC;
+        const int hg = ht * 16 * NT + 16 * nt + c;
+        Frag<T> q;
+        if (hg < a.G && 32 * kc + 8 * g < D)
+          q.load(static_cast<const T*>(a.q) + ((int64_t)b * a.Hq + (int64_t)hkv * a.G + hg) * D + 32 * kc + 8 * g);
+        else
+          q.zero();
+#pragma unroll
+        for (int i = 0; i < QF; ++i) qs[nt][kc][i][lane] = reinterpret_cast<const f32x4*>(&q)[i];
+      }
+    }
+    __syncthreads();
+
+    FwdAcc<D> acc[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) acc[nt].init();
+    for (int i = 0; i < ntile; ++i) {
+      // the next tile's keys are asked for as soon as this one's are used, its values likewise: a wave has
+      // one or the other in flight at all times, in the registers of one tile
+      f32x4 s[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        s[nt][0] = zero4();
+        s[nt][1] = zero4();
+#pragma unroll
+        for (int kc = 0; kc < KC; ++kc) {
+          Frag<T> q;
+#pragma unroll
+          for (int y = 0; y < QF; ++y) reinterpret_cast<f32x4*>(&q)[y] = qs[nt][kc][y][lane];
+          mma(s[nt][0], kf[0][kc], q);
+          mma(s[nt][1], kf[1][kc], q);
+        }
+      }
+      // visible keys kb + 8 g .. + 7 of this lane
+      const int kb = my0 + kUnit * i;
+      const uint32_t vm = (g >= 2 ? run_at(2 * i + 1) : run_at(2 * i)) >= 0 ? range_mask(kb + 8 * g, 0, c1 - 1) : 0u;
+      if (i + 1 < ntile) {
+        if (((i + 1) & 31) == 0) look_up(i + 1);
+        load_k(i + 1);
+      }
+      Frag<T> ph[NT], pl[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        FwdAcc<D>& A = acc[nt];
+        float sv[8], mx = kMaskScore;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          sv[j] = ((vm >> j) & 1u) ? s[nt][j >> 2][j & 3] * a.sl2 : kMaskScore;
+          mx = fmaxf(mx, sv[j]);
+        }
+        mx = group4_max(mx);
+        if (__any(mx > A.m)) {
+          const float mn = fmaxf(A.m, mx);
+          const float alpha = fast_exp2(A.m - mn);
+          A.l *= alpha;
+          A.m = mn;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) A.o[dt] *= alpha;
+        }
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          p[j] = ((vm >> j) & 1u) ? fast_exp2(sv[j] - A.m) : 0.0f;
+          A.l += p[j];
+        }
+        ph[nt].set(p);
+        if constexpr (SPLIT_P) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) p[j] -= (float)ph[nt].elem(j);
+          pl[nt].set(p);
+        }
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        Frag<T> vf;
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) vf.v[j] = vrun_elem<T, VL>(vr[j], dt);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            vf.lo[j] = vrun_elem<T, VL>(vr[j], dt);
+            vf.hi[j] = vrun_elem<T, VL>(vr[4 + j], dt);
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma(acc[nt].o[dt], vf, ph[nt]);
+          if constexpr (SPLIT_P) mma(acc[nt].o[dt], vf, pl[nt]);
+        }
+      }
+      if (i + 1 < ntile) load_v(i + 1);
+    }
+
+    // join the four waves: their outputs against the common maximum, added in wave order
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       FwdAcc<D>& A = acc[nt];
-      f32x4 s0 = zero4(), s1 = zero4();
+      A.l = group4_sum(A.l);
+      if (nt > 0) __syncthreads();
+      if (g == 0) sm[w][c] = A.m, sl[w][c] = A.l;
 #pragma unroll
-      for (int kc = 0; kc < KC; ++kc) {
-        mma(s0, t.k[0][kc], qf[nt][kc]);
-        mma(s1, t.k[1][kc], qf[nt][kc]);
-      }
-      float sv[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
-      float mx = kMaskScore;
+      for (int r = 0; r < 4; ++r) {
+        float* p = &so[w][c][VL * (4 * g + r)];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        sv[j] = ((vm >> j) & 1u) ? sv[j] * a.sl2 : kMaskScore;
-        mx = fmaxf(mx, sv[j]);
-      }
-      mx = group4_max(mx);
-      const float mn = fmaxf(A.m, mx);
-      const float alpha = fast_exp2(A.m - mn);
-      float p[8], ps = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[j] = ((vm >> j) & 1u) ? fast_exp2(sv[j] - mn) : 0.0f;
-        ps += p[j];
-      }
-      A.l = A.l * alpha + ps;
-      A.m = mn;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) A.o[dt] *= alpha;
-      Frag<T> pf;
-      pf.set(p);
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) mma(A.o[dt], vf[dt], pf);
-      if constexpr (SPLIT_P) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] -= (float)pf.elem(j);
-        pf.set(p);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) mma(A.o[dt], vf[dt], pf);
-      }
-    }
-  }
-
-  // join the four waves: their outputs against the common maximum, added in wave order
-  __shared__ float so[16][D + 4];
-  __shared__ float sm[4][16], sl[4][16];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    FwdAcc<D>& A = acc[nt];
-    A.l = group4_sum(A.l);
-    if (nt > 0) __syncthreads();
-    if (g == 0) sm[w][c] = A.m, sl[w][c] = A.l;
-    __syncthreads();
-    const float m = fmaxf(fmaxf(sm[0][c], sm[1][c]), fmaxf(sm[2][c], sm[3][c]));
-    float l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) l += sl[i][c] * fast_exp2(sm[i][c] - m);
-    const float f = fast_exp2(A.m - m);
-    for (int i = 0; i < 4; ++i) {
-      if (i == w) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
-            float* p = &so[c][VL * (4 * g + r) + dt];
-            const float v = A.o[dt][r] * f;
-            *p = i == 0 ? v : *p + v;
-          }
+        for (int dt = 0; dt < DT; ++dt) p[dt] = A.o[dt][r];
       }
       __syncthreads();
+      // 16 threads a head
+      const int hr = threadIdx.x >> 4, y = threadIdx.x & 15;
+      const int hg = ht * 16 * NT + 16 * nt + hr;
+      if (hg < a.G) {
+        const float mj = fmaxf(fmaxf(sm[0][hr], sm[1][hr]), fmaxf(sm[2][hr], sm[3][hr]));
+        float f[4], l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f[i] = fast_exp2(sm[i][hr] - mj);
+          l += sl[i][hr] * f[i];
+        }
+        const float inv = !one ? 1.0f : (l > 0.0f ? 1.0f / l : 0.0f);
+        float o[VL];
+#pragma unroll
+        for (int e = 0; e < VL; ++e) {
+          const int d = VL * y + e;
+          o[e] = (((so[0][hr][d] * f[0] + so[1][hr][d] * f[1]) + so[2][hr][d] * f[2]) + so[3][hr][d] * f[3]) * inv;
+        }
+        if (!one) {
+          const int64_t slot = ((int64_t)blockIdx.x + row) * (16 * NT) + 16 * nt + hr;
+          float* out = a.part_o + slot * D + VL * y;
+#pragma unroll
+          for (int e = 0; e < VL; ++e) out[e] = o[e];
+          if (y == 0) a.part_ml[slot] = make_float2(mj, l);
+        } else {
+          const int64_t head = (int64_t)b * a.Hq + (int64_t)hkv * a.G + hg;
+          T* out = static_cast<T*>(a.out) + head * D + VL * y;
+#pragma unroll
+          for (int e = 0; e < VL; ++e) out[e] = (T)o[e];
+          if (a.lse != nullptr && y == 0) a.lse[head] = paged_lse(mj, l);
+        }
+      }
     }
-    // 16 threads a head
-    const int hr = threadIdx.x >> 4, x = threadIdx.x & 15;
-    const int hg = ht * 16 * NT + 16 * nt + hr;
-    const float lt = __shfl(l, hr & 15, 64), mt = __shfl(m, hr & 15, 64);   // (lane hr of each wave holds column hr)
-    if (hg < a.G) {
-      const int64_t head = (int64_t)b * a.Hq + (int64_t)hkv * a.G + hg;
-      if (a.nsp == 1) {
-        const float inv = lt > 0.0f ? 1.0f / lt : 0.0f;
-        T* out = static_cast<T*>(a.out) + head * D;
-        for (int d = x; d < D; d += 16) out[d] = (T)(lt > 0.0f ? so[hr][d] * inv : so[hr][d] * 0.0f);
-        if (a.lse != nullptr && x == 0) a.lse[head] = lt > 0.0f ? (mt + __log2f(lt)) * kLn2 : (lt == 0.0f ? kLseEmpty : lt);
-      } else {
-        float* out = a.part_o + (head * a.nsp + sp) * D;
-        for (int d = x; d < D; d += 16) out[d] = so[hr][d];
-        if (x == 0) a.part_ml[head * a.nsp + sp] = make_float2(mt, lt);
+
+    x += t1 - t0;
+    if (x < x1) {                                     // on to the next row
+      row0 += units;
+      if (++m == M) {
+        m = 0;
+        ++b;
+        keys = a.B <= 256 ? (uint32_t)__builtin_amdgcn_readfirstlane((int)seq_keys[b]) : paged_keys(a, b);
+        units = paged_units(keys);
       }
     }
   }
 }
 
-// Joins a head's parts: one workgroup of four waves; the waves take parts in turn.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void k_paged_join(const PagedArgs a) {
-  __shared__ float so[4][D], sl[4];
+// Joins the pieces of a head: one workgroup of W waves, which take pieces in
+// turn.  Heads written in one piece are left as they are.
+template <typename T, int D, int W>
+__global__ __launch_bounds__(64 * W) void k_paged_join(const PagedArgs a, int NT) {
+  __shared__ float so[W][D], sl[W];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t head = blockIdx.x;
-  const int b = (int)(head / a.Hq);
-  const int cap = a.max_pages * a.P;
-  const int len = a.lens_out != nullptr ? a.lens_out[b] : a.lens[b];
-  const int n = len < 0 ? 0 : (len < cap ? len : cap);
-  int np = (n + a.chunk - 1) / a.chunk;
-  np = np < 1 ? 1 : np;
-  const float2* ml = a.part_ml + head * a.nsp;
-  const float* po = a.part_o + head * a.nsp * D;
+  const int b = (int)(head / a.Hq), h = (int)(head % a.Hq);
+  const int hkv = h / a.G, hg = h % a.G, ht = hg / (16 * NT);
+  const int row = (b * a.Hkv + hkv) * a.HT + ht;
+  const int2 ri = a.row_info[row];
+  if (ri.x < 0) return;                               // (uniform)
+  const int np = ri.y - ri.x + 1;
+  const int64_t slot0 = ((int64_t)ri.x + row) * (16 * NT) + (hg - ht * 16 * NT);
+  const float2* ml = a.part_ml + slot0;
+  const float* po = a.part_o + slot0 * D;
+  const int step = 16 * NT;                           // slots from a piece to the next
   float m = kMaskScore;
-  for (int i = lane; i < np; i += 64) m = fmaxf(m, ml[i].x);
+  for (int i = lane; i < np; i += 64) m = fmaxf(m, ml[(int64_t)i * step].x);
 #pragma unroll
   for (int x = 1; x < 64; x <<= 1) m = xor_max(m, x);
   constexpr int E = D >= 64 ? D / 64 : 1;
   float o[E], l = 0.0f;
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.0f;
-#pragma unroll 4
-  for (int i = w; i < np; i += 4) {
-    const float2 s = ml[i];
+#pragma unroll 8
+  for (int i = w; i < np; i += W) {
+    const float2 s = ml[(int64_t)i * step];
     const float f = fast_exp2(s.x - m);
     l += s.y * f;
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      if (E * lane + e < D) o[e] += po[(int64_t)i * D + E * lane + e] * f;
+      if (E * lane + e < D) o[e] += po[(int64_t)i * step * D + E * lane + e] * f;
   }
 #pragma unroll
   for (int e = 0; e < E; ++e)
     if (E * lane + e < D) so[w][E * lane + e] = o[e];
   if (lane == 0) sl[w] = l;
   __syncthreads();
-  l = ((sl[0] + sl[1]) + sl[2]) + sl[3];
+  l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < W; ++i) l += sl[i];
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
   if ((int)threadIdx.x < D) {
     const int d = threadIdx.x;
-    const float v = ((so[0][d] + so[1][d]) + so[2][d]) + so[3][d];
+    float v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) v += so[i][d];
     static_cast<T*>(a.out)[head * D + d] = (T)(v * inv);
   }
-  if (a.lse != nullptr && threadIdx.x == 0) a.lse[head] = l > 0.0f ? (m + __log2f(l)) * kLn2 : (l == 0.0f ? kLseEmpty : l);
+  if (a.lse != nullptr && threadIdx.x == 0) a.lse[head] = paged_lse(m, l);
 }
 
 // Rows [B][Hkv][Tn][D] to positions lens[b] .. lens[b] + count[b] - 1: all of a
@@ -386,19 +539,23 @@ __global__ __launch_bounds__(256) void k_paged_append(const T* __restrict__ k, c
 }
 
 struct PagedPlan {
-  int NT, HT, chunk, nsp;
+  int NT, HT, W;
+  int64_t R;             // rows: sequences x KV heads x head tiles
+  bool joined;           // there may be pieces to join
 };
-// Chunk: as long as leaves four workgroups for every compute unit (fewer
-// parts to join), from 128 keys (a tile for each wave) to 2048.
-static PagedPlan paged_plan(int B, int Hq, int Hkv, int D, int64_t cap, int cu) {
+// Shares: two for every compute unit.  Where the rows fill the chip and none can
+// be long (1 MiB of keys and values), a workgroup takes a row instead (W = 0):
+// nothing is counted and nothing joined.
+static PagedPlan paged_plan(int B, int Hq, int Hkv, int row_bytes, int64_t cap, int cu) {
   PagedPlan p;
   const int G = Hq / Hkv;
-  p.NT = G > 16 ? 2 : 1;
+  p.NT = G > 16 && row_bytes <= 256 ? 2 : 1;   // (two tiles of 512-byte rows do not fit the registers)
   p.HT = (G + 16 * p.NT - 1) / (16 * p.NT);
-  const int64_t rows = (int64_t)B * Hkv * p.HT;
-  p.chunk = 2048;
-  while (p.chunk > 128 && rows * ((cap + p.chunk - 1) / p.chunk) < 4LL * cu) p.chunk /= 2;
-  p.nsp = (int)((cap + p.chunk - 1) / p.chunk);
+  p.R = (int64_t)B * Hkv * p.HT;
+  const int64_t most = p.R * ((cap + kUnit - 1) / kUnit);
+  const bool rows = cap <= kUnit || (p.R >= cu && cap * 2 * row_bytes <= (1 << 20));
+  p.W = rows ? 0 : (int)(most < 2LL * cu ? most : 2LL * cu);
+  p.joined = !rows;
   return p;
 }
 static bool paged_shape_ok(int B, int Hq, int Hkv, int D, int P, int max_pages, int n_pages) {
@@ -408,34 +565,44 @@ static bool paged_shape_ok(int B, int Hq, int Hkv, int D, int P, int max_pages, 
 }
 
 template <typename T, int D>
-static int paged_launch(const PagedArgs& a, int NT, hipStream_t s) {
-  const int64_t grid = (int64_t)a.B * a.Hkv * a.HT * a.nsp;
-  NSA_CHECK(grid <= 0x7fffffffLL, NSA_ERR_SHAPE);
-  if (NT == 2)
-    k_paged<T, D, 2><<<(unsigned)grid, 256, 0, s>>>(a);
-  else
-    k_paged<T, D, 1><<<(unsigned)grid, 256, 0, s>>>(a);
-  if (a.nsp > 1) k_paged_join<T, D><<<(unsigned)(a.B * a.Hq), 256, 0, s>>>(a);
+static int paged_launch(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
+  const unsigned grid = (unsigned)(p.W > 0 ? p.W : p.R);
+  if (p.NT == 1)
+    k_paged<T, D, 1><<<grid, 256, 0, s>>>(a);
+  else if constexpr (D * sizeof(T) <= 256)
+    k_paged<T, D, 2><<<grid, 256, 0, s>>>(a);
+  if (p.joined) {
+    // few rows are many pieces each: sixteen waves a head
+    if (p.R * 16 <= p.W)
+      k_paged_join<T, D, 16><<<(unsigned)(a.B * a.Hq), 1024, 0, s>>>(a, p.NT);
+    else
+      k_paged_join<T, D, 4><<<(unsigned)(a.B * a.Hq), 256, 0, s>>>(a, p.NT);
+  }
   return nsa_launch_status();
 }
 template <typename T>
-static int paged_dim(const PagedArgs& a, int NT, int D, hipStream_t s) {
+static int paged_dim(const PagedArgs& a, const PagedPlan& p, int D, hipStream_t s) {
   switch (D) {
-    case 16: return paged_launch<T, 16>(a, NT, s);
-    case 32: return paged_launch<T, 32>(a, NT, s);
-    case 64: return paged_launch<T, 64>(a, NT, s);
-    case 128: return paged_launch<T, 128>(a, NT, s);
+    case 16: return paged_launch<T, 16>(a, p, s);
+    case 32: return paged_launch<T, 32>(a, p, s);
+    case 64: return paged_launch<T, 64>(a, p, s);
+    case 128: return paged_launch<T, 128>(a, p, s);
   }
   return NSA_ERR_SHAPE;
 }
 
 }  // namespace nsa
 
-extern "C" size_t nsa_paged_workspace(int B, int Hq, int Hkv, int D, int P, int max_pages, void* stream) {
+static size_t paged_ws_bytes(int D, const nsa::PagedPlan& p) {
+  return p.joined ? (size_t)(p.W + p.R) * 16 * p.NT * (D * sizeof(float) + sizeof(float2)) + (size_t)p.R * sizeof(int2)
+                  : 16;
+}
+
+extern "C" size_t nsa_paged_workspace(int B, int Hq, int Hkv, int D, int P, int max_pages, int dtype, void* stream) {
   using namespace nsa;
-  if (!paged_shape_ok(B, Hq, Hkv, D, P, max_pages, 1)) return 0;
-  const PagedPlan p = paged_plan(B, Hq, Hkv, D, (int64_t)max_pages * P, device_cu_count(static_cast<hipStream_t>(stream)));
-  return p.nsp == 1 ? 16 : (size_t)B * Hq * p.nsp * (D * sizeof(float) + sizeof(float2)) + 16;
+  if (!paged_shape_ok(B, Hq, Hkv, D, P, max_pages, 1) || (dtype != NSA_F32 && dtype != NSA_BF16)) return 0;
+  return paged_ws_bytes(D, paged_plan(B, Hq, Hkv, D * (dtype == NSA_BF16 ? 2 : 4), (int64_t)max_pages * P,
+                                      device_cu_count(static_cast<hipStream_t>(stream))));
 }
 
 extern "C" int nsa_paged_attend(const void* q, const void* k_new, const void* v_new, void* k_pages, void* v_pages,
@@ -451,16 +618,18 @@ extern "C" int nsa_paged_attend(const void* q, const void* k_new, const void* v_
   NSA_CHECK((k_new == nullptr) == (v_new == nullptr) && (k_new == nullptr) == (lens_out == nullptr) &&
                 lens_out != lens, NSA_ERR_ARG);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const PagedPlan p = paged_plan(B, Hq, Hkv, D, (int64_t)max_pages * P, device_cu_count(s));
-  PagedArgs a{q, k_new, v_new, k_pages, v_pages, table, lens, lens_out, out, lse, nullptr, nullptr, B, Hq, Hkv,
-              Hq / Hkv, p.HT, P, P / 16, max_pages, n_pages, p.nsp, p.chunk, scale * kLog2e};
-  if (p.nsp > 1) {
-    NSA_CHECK(workspace != nullptr && workspace_bytes >= nsa_paged_workspace(B, Hq, Hkv, D, P, max_pages, stream),
-              NSA_ERR_WORKSPACE);
+  const PagedPlan p =
+      paged_plan(B, Hq, Hkv, D * (dtype == NSA_BF16 ? 2 : 4), (int64_t)max_pages * P, device_cu_count(s));
+  PagedArgs a{q, k_new, v_new, k_pages, v_pages, table, lens, lens_out, out, lse, nullptr, nullptr, nullptr, B, Hq, Hkv,
+              Hq / Hkv, p.HT, P, P / 16, max_pages, n_pages, p.W, scale * kLog2e};
+  if (p.joined) {
+    NSA_CHECK(workspace != nullptr && workspace_bytes >= paged_ws_bytes(D, p), NSA_ERR_WORKSPACE);
+    const size_t slots = (size_t)(p.W + p.R) * 16 * p.NT;
     a.part_o = static_cast<float*>(workspace);
-    a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)B * Hq * p.nsp * D);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + slots * D);
+    a.row_info = reinterpret_cast<int2*>(a.part_ml + slots);
   }
-  return dtype == NSA_BF16 ? paged_dim<bf16>(a, p.NT, D, s) : paged_dim<float>(a, p.NT, D, s);
+  return dtype == NSA_BF16 ? paged_dim<bf16>(a, p, D, s) : paged_dim<float>(a, p, D, s);
 }
 
 extern "C" int nsa_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* table,

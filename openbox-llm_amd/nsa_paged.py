@@ -65,12 +65,13 @@ def _attend(q, rows, k_pages, v_pages, table, lens, scale, return_lse):
     out = torch.empty_like(q)
     lse = torch.empty(B, Hq, device=q.device, dtype=torch.float32) if return_lse else None
     if B > 0:
-        nbytes = _ops.launch(q, "nsa_paged_workspace", B, Hq, Hkv, D, P, mp)
+        code = L.NSA_BF16 if q.dtype == torch.bfloat16 else L.NSA_F32
+        nbytes = _ops.launch(q, "nsa_paged_workspace", B, Hq, Hkv, D, P, mp, code)
         ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes > 16 else None
         _ops.launch(q, "nsa_paged_attend", q.data_ptr(), L.addr(kn), L.addr(vn), k_pages.data_ptr(),
                     v_pages.data_ptr(), table.data_ptr(), lens.data_ptr(), L.addr(lens_out), out.data_ptr(),
                     L.addr(lse), L.addr(ws), nbytes, B, Hq, Hkv, D, P, mp, n, D ** -0.5 if scale is None else scale,
-                    L.NSA_BF16 if q.dtype == torch.bfloat16 else L.NSA_F32)
+                    code)
     return out, lse, lens_out
 
 

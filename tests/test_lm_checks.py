@@ -65,7 +65,7 @@ def test_paged_refusals():
                 dict(P=1 << 20, mp=1 << 20), dict(Hq=8192), dict(B=70000)):
         assert attend(**bad) == SHAPE, bad
         assert "n" in bad or "B" in bad and bad["B"] < 0 or \
-            lib.nsa_paged_workspace(*{**dict(B=1, Hq=4, Hkv=2, D=64, P=16, mp=3), **bad}.values(), None) == 0
+            lib.nsa_paged_workspace(*{**dict(B=1, Hq=4, Hkv=2, D=64, P=16, mp=3), **bad}.values(), 1, None) == 0
     assert attend(dt=2) == DTYPE
     assert attend() == ARG
     no = [None] * 8
