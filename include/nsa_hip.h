@@ -552,7 +552,7 @@ int nsa_norm_bwd(const void* dy, const void* dh, const void* h, const void* w, c
  *   entropy  - sum p ln p (tokens of weight 0 add nothing)
  *   top_logp, top_idx [rows][k]: the k largest, equal logits by ascending index
  *   stat     float [rows][2]: (max z, ln sum e^(z - max)), for the backward
- * logp and entropy may be null.  A row of -inf alone has logp -inf (and top_logp),
+ * logp, entropy and stat may be null.  A row of -inf alone has logp -inf (and top_logp),
  * entropy 0 and no gradient.  k <= 64, k <= V, V <= 2^28, rows <= 2^25.
  * workspace: nsa_logprob_workspace bytes (0: unsupported shape). */
 size_t nsa_logprob_workspace(int64_t rows, int V, int k, void* stream);

@@ -39,7 +39,7 @@ struct LpArgs {
   const void* z;
   const int64_t* target;   // or null
   float *logp, *entropy;
-  float2* stat;            // (m, ln l)
+  float2* stat;            // (m, ln l); or null
   float* top_logp;         // [rows][k]
   int64_t* top_idx;
   float4* part;            // [rows][nsp] (m, l, s) of a split row
@@ -89,7 +89,7 @@ __device__ __forceinline__ LpState lp_wave(LpState a) {
 // Results of one row from its sums (one thread).
 __device__ __forceinline__ float lp_finish(const LpArgs& a, int64_t row, LpState st, float zt, bool has_t) {
   const float logl = st.l == 0.0f ? -__builtin_inff() : logf(st.l);
-  a.stat[row] = make_float2(st.m, logl);
+  if (a.stat != nullptr) a.stat[row] = make_float2(st.m, logl);
   if (a.entropy != nullptr) a.entropy[row] = st.l == 0.0f ? 0.0f : logl - st.s / st.l;
   if (a.logp != nullptr) a.logp[row] = has_t ? (st.l == 0.0f ? -__builtin_inff() : (zt - st.m) - logl) : 0.0f;
   return logl;
@@ -486,7 +486,7 @@ extern "C" int nsa_logprob_fwd(const void* z, const int64_t* target, float* logp
   NSA_CHECK(lp_shape_ok(rows, V, k), NSA_ERR_SHAPE);
   NSA_CHECK(dtype == NSA_F32 || dtype == NSA_BF16, NSA_ERR_DTYPE);
   if (rows == 0) return NSA_OK;
-  NSA_CHECK(z != nullptr && stat != nullptr && (logp == nullptr || target != nullptr), NSA_ERR_ARG);
+  NSA_CHECK(z != nullptr && (logp == nullptr || target != nullptr), NSA_ERR_ARG);
   NSA_CHECK(k == 0 || (top_logp != nullptr && top_idx != nullptr), NSA_ERR_ARG);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int nsp = lp_parts(rows, V, dtype == NSA_BF16 ? 2 : 4, device_cu_count(s));

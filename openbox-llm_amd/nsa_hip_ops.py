@@ -15,6 +15,7 @@ case ``cmp_block == cmp_stride == block_size``).
 from __future__ import annotations
 
 import contextlib
+import functools
 from collections import defaultdict
 from dataclasses import dataclass
 
@@ -159,9 +160,16 @@ def launch(t, name, *args):
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    if rc < 0:
+    if rc:
         L.check(rc, name)
-    return rc
+
+
+@functools.lru_cache(maxsize=4096)
+def workspace_bytes(dev, name, *sizes):
+    """The library's answer to the size query ``name(*sizes, stream)`` for device
+    ``dev``: it depends on the sizes and the device alone, so it is asked once."""
+    with torch.cuda.device(dev):
+        return int(getattr(_lib(), name)(*sizes, torch._C._cuda_getCurrentRawStream(dev)))
 
 
 def _stream(t):

@@ -105,7 +105,7 @@ def _norm_bwd(ctx, dy, dh=None):
     nbytes = 0
     if need_w:
         dw = torch.empty_like(weight)
-        nbytes = _ops.launch(h, "nsa_norm_bwd_workspace", rows, D)
+        nbytes = _ops.workspace_bytes(h.get_device(), "nsa_norm_bwd_workspace", rows, D)
         ws = torch.empty(nbytes, device=h.device, dtype=torch.uint8)
     _ops.launch(h, "nsa_norm_bwd", dy.data_ptr(), L.addr(dh), h.data_ptr(), weight.data_ptr(), rstd.data_ptr(),
                 dx.data_ptr(), None if dr is dx else L.addr(dr), L.addr(dw), L.addr(ws), nbytes, rows, D,
@@ -185,20 +185,21 @@ class TokenLogprobs(NamedTuple):
     top_idx: Optional[torch.Tensor]
 
 
-def _logprob_fwd(z, targets, top):
+def _logprob_fwd(z, targets, top, want_stat):
     """-> (logp, entropy, top_logp, top_idx, stat) of dense ``z [rows, V]``."""
     rows, V = z.shape
     dev, f32 = z.device, torch.float32
     logp = None if targets is None else torch.empty(rows, device=dev, dtype=f32)
-    ent, stat = torch.empty(rows, device=dev, dtype=f32), torch.empty(rows, 2, device=dev, dtype=f32)
+    ent = torch.empty(rows, device=dev, dtype=f32)
+    stat = torch.empty(rows, 2, device=dev, dtype=f32) if want_stat else None
     top_logp = top_idx = None
     if top:
         top_logp = torch.empty(rows, top, device=dev, dtype=f32)
         top_idx = torch.empty(rows, top, device=dev, dtype=torch.int64)
-    nbytes = _ops.launch(z, "nsa_logprob_workspace", rows, V, top)
+    nbytes = _ops.workspace_bytes(z.get_device(), "nsa_logprob_workspace", rows, V, top)
     assert nbytes > 0, "token_logprobs: unsupported shape"
     ws = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes > 16 else None
-    _ops.launch(z, "nsa_logprob_fwd", z.data_ptr(), L.addr(targets), L.addr(logp), ent.data_ptr(), stat.data_ptr(),
+    _ops.launch(z, "nsa_logprob_fwd", z.data_ptr(), L.addr(targets), L.addr(logp), ent.data_ptr(), L.addr(stat),
                 L.addr(top_logp), L.addr(top_idx), L.addr(ws), nbytes, rows, V, top, _CODE[z.dtype])
     return logp, ent, top_logp, top_idx, stat
 
@@ -222,7 +223,7 @@ class TokenLogprobsHIP(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, targets, top):
         ctx.set_materialize_grads(False)
-        logp, ent, top_logp, top_idx, stat = _logprob_fwd(z, targets, top)
+        logp, ent, top_logp, top_idx, stat = _logprob_fwd(z, targets, top, True)
         ctx.save_for_backward(z, targets, stat, ent)
         if top:
             ctx.mark_non_differentiable(top_logp, top_idx)
@@ -259,12 +260,13 @@ def token_logprobs(logits, targets=None, top=0):
         assert targets.dtype in (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8), \
             "token_logprobs: targets must be integers"
         assert targets.shape == lead, "token_logprobs: one target for each row"
-        targets = targets.reshape(-1).long()
-    z = logits.reshape(-1, V).contiguous()
+        if targets.dim() != 1 or targets.dtype != torch.int64 or not targets.is_contiguous():
+            targets = targets.reshape(-1).long().contiguous()
+    z = logits if logits.dim() == 2 and logits.is_contiguous() else logits.reshape(-1, V).contiguous()
     if _wants_grad(logits):
         logp, ent, top_logp, top_idx = TokenLogprobsHIP.apply(z, targets, top)
     else:
-        logp, ent, top_logp, top_idx, _ = _logprob_fwd(z, targets, top)
+        logp, ent, top_logp, top_idx, _ = _logprob_fwd(z, targets, top, False)
     if len(lead) == 1:
         return TokenLogprobs(logp, ent, top_logp, top_idx)
     return TokenLogprobs(None if logp is None else logp.view(lead), ent.view(lead),

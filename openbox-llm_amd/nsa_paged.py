@@ -28,27 +28,29 @@ import nsa_hip_ops as _ops
 
 
 def _check_pages(k_pages, v_pages, table, lens):
+    """The asserts; -> (n_pages, Hkv, page, D, B, max_pages)."""
     assert k_pages.dim() == 4 and k_pages.is_cuda, "paged: pages must be [n_pages, Hkv, page, D] on the GPU"
-    assert v_pages.shape == k_pages.shape and v_pages.dtype == k_pages.dtype and v_pages.device == k_pages.device, \
+    dev, shape = k_pages.device, k_pages.shape
+    assert v_pages.shape == shape and v_pages.dtype == k_pages.dtype and v_pages.device == dev, \
         "paged: key and value pages differ in shape, dtype or device"
-    n, Hkv, P, D = k_pages.shape
+    n, Hkv, P, D = shape
     assert n >= 1 and Hkv >= 1 and P >= 16 and P % 16 == 0, "paged: the page size must be a multiple of 16"
     assert D in (16, 32, 64, 128), "head dim must be a power of two <= 128"
     assert k_pages.dtype in (torch.float32, torch.bfloat16), \
         f"dtype {k_pages.dtype} is not supported (float32 or bfloat16)"
-    for p in (k_pages, v_pages):
-        assert p.is_contiguous() and p.data_ptr() % 16 == 0, "paged: pages must be dense and 16-byte aligned"
-    assert table.dim() == 2 and table.dtype == torch.int32 and table.device == k_pages.device, \
+    assert k_pages.is_contiguous() and v_pages.is_contiguous() and k_pages.data_ptr() % 16 == 0 and \
+        v_pages.data_ptr() % 16 == 0, "paged: pages must be dense and 16-byte aligned"
+    assert table.dim() == 2 and table.dtype == torch.int32 and table.device == dev, \
         "paged: table int32 [B, max_pages] on the pages' device"
-    assert table.shape[1] >= 1 and table.shape[1] * P <= 1 << 30, "paged: table of 1 page to 2^30 positions"
-    assert lens.dtype == torch.int32 and lens.shape == table.shape[:1] and lens.device == k_pages.device, \
+    B, mp = table.shape
+    assert mp >= 1 and mp * P <= 1 << 30, "paged: table of 1 page to 2^30 positions"
+    assert lens.dtype == torch.int32 and lens.shape == (B,) and lens.device == dev, \
         "paged: lens int32 [B] on the pages' device"
+    return n, Hkv, P, D, B, mp
 
 
 def _attend(q, rows, k_pages, v_pages, table, lens, scale, return_lse):
-    _check_pages(k_pages, v_pages, table, lens)
-    n, Hkv, P, D = k_pages.shape
-    B, mp = table.shape
+    n, Hkv, P, D, B, mp = _check_pages(k_pages, v_pages, table, lens)
     assert q.dim() == 3 and q.shape[0] == B and q.shape[2] == D, "paged: q must be [B, Hq, D]"
     assert q.dtype == k_pages.dtype and q.device == k_pages.device, "paged: q in the pages' dtype and device"
     Hq = q.shape[1]
@@ -66,7 +68,7 @@ def _attend(q, rows, k_pages, v_pages, table, lens, scale, return_lse):
     lse = torch.empty(B, Hq, device=q.device, dtype=torch.float32) if return_lse else None
     if B > 0:
         code = L.NSA_BF16 if q.dtype == torch.bfloat16 else L.NSA_F32
-        nbytes = _ops.launch(q, "nsa_paged_workspace", B, Hq, Hkv, D, P, mp, code)
+        nbytes = _ops.workspace_bytes(q.get_device(), "nsa_paged_workspace", B, Hq, Hkv, D, P, mp, code)
         ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes > 16 else None
         _ops.launch(q, "nsa_paged_attend", q.data_ptr(), L.addr(kn), L.addr(vn), k_pages.data_ptr(),
                     v_pages.data_ptr(), table.data_ptr(), lens.data_ptr(), L.addr(lens_out), out.data_ptr(),
@@ -99,9 +101,7 @@ def paged_append(k, v, k_pages, v_pages, table, lens, count=None):
     """Write rows ``k, v [B, Hkv, T, D]`` (the first ``count[b]`` of them: int32
     ``[B]``, default T) to positions ``lens[b] ..`` -> the new lengths.  A
     sequence whose rows do not all have a page keeps its pages and length."""
-    _check_pages(k_pages, v_pages, table, lens)
-    n, Hkv, P, D = k_pages.shape
-    B, mp = table.shape
+    n, Hkv, P, D, B, mp = _check_pages(k_pages, v_pages, table, lens)
     assert k.dim() == 4 and k.shape[:2] == (B, Hkv) and k.shape[3] == D and v.shape == k.shape, \
         "paged: rows must be [B, Hkv, T, D]"
     assert all(t.dtype == k_pages.dtype and t.device == k_pages.device for t in (k, v)), \
