@@ -7,6 +7,7 @@ unloadable library raises.
 """
 
 import ctypes
+import importlib.util
 import os
 
 import torch
@@ -113,6 +114,10 @@ SIGNATURES = {
     "nsa_paged_append": (_I, [_P] * 8 + [_I] * 8 + [_P]),
 }
 
+# entry points that csrc/nsa_torch.cpp calls
+_TORCH_SIDE = ("nsa_norm_fwd", "nsa_norm_bwd", "nsa_norm_bwd_workspace", "nsa_logprob_fwd", "nsa_logprob_bwd",
+               "nsa_logprob_workspace", "nsa_paged_attend", "nsa_paged_workspace")
+
 _lib = None
 
 
@@ -132,6 +137,28 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+_torch_side = None
+
+
+def torch_side():
+    """The C++ module of the operators around the attention (csrc/nsa_torch.cpp:
+    their checks, allocations and autograd nodes), bound once to the loaded
+    library's entry points; raises if it is not built."""
+    global _torch_side
+    if _torch_side is None:
+        lib = load()
+        path = os.path.join(_HERE, "_nsa_torch.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is not built: run `make -C openbox-llm_amd` or "
+                               "`python -c 'import __graft_entry__ as g; g.build()'` first")
+        spec = importlib.util.spec_from_file_location("_nsa_torch", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _TORCH_SIDE})
+        _torch_side = mod
+    return _torch_side
 
 
 def check(rc, what):
@@ -161,11 +188,6 @@ def dtype_code(t):
 
 def ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
-
-
-def addr(t):
-    """A tensor's address as ctypes takes it fastest (None: a null pointer)."""
-    return None if t is None else t.data_ptr()
 
 
 def stream_of(t):

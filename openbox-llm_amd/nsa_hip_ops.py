@@ -15,7 +15,6 @@ case ``cmp_block == cmp_stride == block_size``).
 from __future__ import annotations
 
 import contextlib
-import functools
 from collections import defaultdict
 from dataclasses import dataclass
 
@@ -145,31 +144,11 @@ def _lib():
     return L.load()
 
 
-def launch(t, name, *args):
-    """Library call ``name(*args, stream)`` on t's device and its current
-    stream; addresses as integers.  The short way round for calls whose host
-    time counts: the raw stream query and integer addresses take 0.2 us where
-    ``stream_of`` and a dozen ``ptr`` take 4."""
-    dev = t.get_device()
-    if dev != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return launch(t, name, *args)
-    fn = getattr(_lib(), name)
-    if _TIMER is not None:
-        with _span(name):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    if rc:
-        L.check(rc, name)
-
-
-@functools.lru_cache(maxsize=4096)
-def workspace_bytes(dev, name, *sizes):
-    """The library's answer to the size query ``name(*sizes, stream)`` for device
-    ``dev``: it depends on the sizes and the device alone, so it is asked once."""
-    with torch.cuda.device(dev):
-        return int(getattr(_lib(), name)(*sizes, torch._C._cuda_getCurrentRawStream(dev)))
+def device_of(t):
+    """Context in which t's device is the current one."""
+    if t.get_device() == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
 
 
 def _stream(t):

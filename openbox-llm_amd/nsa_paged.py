@@ -27,54 +27,12 @@ import _nsa_lib as L
 import nsa_hip_ops as _ops
 
 
-def _check_pages(k_pages, v_pages, table, lens):
-    """The asserts; -> (n_pages, Hkv, page, D, B, max_pages)."""
-    assert k_pages.dim() == 4 and k_pages.is_cuda, "paged: pages must be [n_pages, Hkv, page, D] on the GPU"
-    dev, shape = k_pages.device, k_pages.shape
-    assert v_pages.shape == shape and v_pages.dtype == k_pages.dtype and v_pages.device == dev, \
-        "paged: key and value pages differ in shape, dtype or device"
-    n, Hkv, P, D = shape
-    assert n >= 1 and Hkv >= 1 and P >= 16 and P % 16 == 0, "paged: the page size must be a multiple of 16"
-    assert D in (16, 32, 64, 128), "head dim must be a power of two <= 128"
-    assert k_pages.dtype in (torch.float32, torch.bfloat16), \
-        f"dtype {k_pages.dtype} is not supported (float32 or bfloat16)"
-    assert k_pages.is_contiguous() and v_pages.is_contiguous() and k_pages.data_ptr() % 16 == 0 and \
-        v_pages.data_ptr() % 16 == 0, "paged: pages must be dense and 16-byte aligned"
-    assert table.dim() == 2 and table.dtype == torch.int32 and table.device == dev, \
-        "paged: table int32 [B, max_pages] on the pages' device"
-    B, mp = table.shape
-    assert mp >= 1 and mp * P <= 1 << 30, "paged: table of 1 page to 2^30 positions"
-    assert lens.dtype == torch.int32 and lens.shape == (B,) and lens.device == dev, \
-        "paged: lens int32 [B] on the pages' device"
-    return n, Hkv, P, D, B, mp
-
-
-def _attend(q, rows, k_pages, v_pages, table, lens, scale, return_lse):
-    n, Hkv, P, D, B, mp = _check_pages(k_pages, v_pages, table, lens)
-    assert q.dim() == 3 and q.shape[0] == B and q.shape[2] == D, "paged: q must be [B, Hq, D]"
-    assert q.dtype == k_pages.dtype and q.device == k_pages.device, "paged: q in the pages' dtype and device"
-    Hq = q.shape[1]
-    assert Hq >= 1 and Hq % Hkv == 0, "GQA needs n_q_heads divisible by n_kv_heads"
-    assert Hq <= 4096 and B <= 65536, "paged: at most 4096 heads and 65536 sequences"
-    q, table, lens = _ops._contig(q), table.contiguous(), lens.contiguous()
-    kn = vn = lens_out = None
-    if rows is not None:
-        for r in rows:
-            assert r.shape == (B, Hkv, D) and r.dtype == q.dtype and r.device == q.device, \
-                "paged: new rows must be [B, Hkv, D] in the pages' dtype"
-        kn, vn = (_ops._contig(r) for r in rows)
-        lens_out = torch.empty_like(lens)
-    out = torch.empty_like(q)
-    lse = torch.empty(B, Hq, device=q.device, dtype=torch.float32) if return_lse else None
-    if B > 0:
-        code = L.NSA_BF16 if q.dtype == torch.bfloat16 else L.NSA_F32
-        nbytes = _ops.workspace_bytes(q.get_device(), "nsa_paged_workspace", B, Hq, Hkv, D, P, mp, code)
-        ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes > 16 else None
-        _ops.launch(q, "nsa_paged_attend", q.data_ptr(), L.addr(kn), L.addr(vn), k_pages.data_ptr(),
-                    v_pages.data_ptr(), table.data_ptr(), lens.data_ptr(), L.addr(lens_out), out.data_ptr(),
-                    L.addr(lse), L.addr(ws), nbytes, B, Hq, Hkv, D, P, mp, n, D ** -0.5 if scale is None else scale,
-                    code)
-    return out, lse, lens_out
+def _attend(q, k_new, v_new, k_pages, v_pages, table, lens, scale, return_lse):
+    f = L.torch_side().paged
+    if _ops._TIMER is None:
+        return f(q, k_new, v_new, k_pages, v_pages, table, lens, scale, return_lse)
+    with _ops._span("nsa_paged_attend"):
+        return f(q, k_new, v_new, k_pages, v_pages, table, lens, scale, return_lse)
 
 
 def paged_attend(q, k_pages, v_pages, table, lens, scale=None, return_lse=False):
@@ -82,7 +40,7 @@ def paged_attend(q, k_pages, v_pages, table, lens, scale=None, return_lse=False)
     the first ``lens[b]`` positions -> ``out [B, Hq, D]`` (zeros where there are
     none).  ``scale`` defaults to ``D ** -0.5``; ``return_lse`` adds
     ``ln sum e^score`` (float32 ``[B, Hq]``, -1e9 without keys)."""
-    out, lse, _ = _attend(q, None, k_pages, v_pages, table, lens, scale, return_lse)
+    out, lse, _ = _attend(q, None, None, k_pages, v_pages, table, lens, scale, return_lse)
     return (out, lse) if return_lse else out
 
 
@@ -93,7 +51,7 @@ def paged_step(q, k_new, v_new, k_pages, v_pages, table, lens, scale=None):
     tensor.  A sequence whose position has no page keeps its pages and length
     and attends what it holds.  Pages that are written may not be shared with
     another sequence of the call."""
-    out, _, lens_out = _attend(q, (k_new, v_new), k_pages, v_pages, table, lens, scale, False)
+    out, _, lens_out = _attend(q, k_new, v_new, k_pages, v_pages, table, lens, scale, False)
     return out, lens_out
 
 
@@ -101,7 +59,9 @@ def paged_append(k, v, k_pages, v_pages, table, lens, count=None):
     """Write rows ``k, v [B, Hkv, T, D]`` (the first ``count[b]`` of them: int32
     ``[B]``, default T) to positions ``lens[b] ..`` -> the new lengths.  A
     sequence whose rows do not all have a page keeps its pages and length."""
-    n, Hkv, P, D, B, mp = _check_pages(k_pages, v_pages, table, lens)
+    L.torch_side().check_pages(k_pages, v_pages, table, lens)
+    n, Hkv, P, D = k_pages.shape
+    B, mp = table.shape
     assert k.dim() == 4 and k.shape[:2] == (B, Hkv) and k.shape[3] == D and v.shape == k.shape, \
         "paged: rows must be [B, Hkv, T, D]"
     assert all(t.dtype == k_pages.dtype and t.device == k_pages.device for t in (k, v)), \
@@ -114,9 +74,10 @@ def paged_append(k, v, k_pages, v_pages, table, lens, count=None):
         count = count.contiguous()
     lens_out = torch.empty_like(lens)
     if B > 0:
-        _ops.launch(k_pages, "nsa_paged_append", k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                    table.data_ptr(), lens.data_ptr(), L.addr(count), lens_out.data_ptr(), B, Hkv, k.shape[2], D, P, mp,
-                    n, L.NSA_BF16 if k.dtype == torch.bfloat16 else L.NSA_F32)
+        with _ops.device_of(k_pages):
+            _ops._call("nsa_paged_append", _ops._lib().nsa_paged_append, L.ptr(k), L.ptr(v), L.ptr(k_pages),
+                       L.ptr(v_pages), L.ptr(table), L.ptr(lens), L.ptr(count), L.ptr(lens_out), B, Hkv, k.shape[2], D,
+                       P, mp, n, L.dtype_code(k_pages), _ops._stream(k_pages))
     return lens_out
 
 
@@ -157,7 +118,7 @@ class PagedKVCache:
         self.lens = torch.zeros(batch, device=device, dtype=torch.int32)
         self._account = _PageAccount(batch, self.max_pages, n_pages, device) if like is None else like._account
         self._account.caches.append(self)
-        _check_pages(self.k_pages, self.v_pages, self.table, self.lens)
+        L.torch_side().check_pages(self.k_pages, self.v_pages, self.table, self.lens)
 
     @property
     def table(self):
