@@ -11,10 +11,10 @@
 // infinity make l NaN, and with it the row's results.
 //
 // The forward reads the row once.  A lane keeps its own (m, l, s) and rescales
-// them when a run of 32 elements raises its maximum.  For the alternatives the
-// k-th largest of the lanes' maxima is a lower bound of the row's k-th value
-// (k lanes hold one such element each): elements below it are dropped, the
-// few others go to a list in LDS as (value, ~index) keys, which are all
+// them when its runs of a chunk raise its maximum.  For the alternatives the k-th
+// largest of 64 or 256 maxima over parts of the row is a lower bound of the
+// row's k-th value (k parts hold one such element each): elements below it are
+// dropped, the few others (24 of 32000 for 20 alternatives) go to a list in LDS as (value, ~index) keys, which are all
 // different, and are ranked by counting.  The bound is formed after the
 // first chunk, which is still in registers, and again whenever the chunks done
 // have doubled: 16 ballots, one for each of the upper bits of a value's key.  A row that overfills the list (long ties, a rising
@@ -70,18 +70,28 @@ __device__ __forceinline__ void lp_raise(LpState& a, float m) {   // a's sums ag
   a.s = a.s * f + a.l * fmaxf(d, kFar);
   a.m = m;
 }
-__device__ __forceinline__ void lp_join(LpState& a, LpState b) {
-  const float m = fmaxf(a.m, b.m);
-  lp_raise(a, m);
-  lp_raise(b, m);
-  a.l += b.l;
-  a.s += b.s;
-}
-__device__ __forceinline__ LpState lp_wave(LpState a) {
+// The sums of W waves (W > 1: two barriers, buf is free before and after):
+// the common maximum first, so that every lane rescales once.
+template <int W>
+__device__ __forceinline__ LpState lp_group(LpState a, float (&buf)[3][W]) {
+  const int w = threadIdx.x >> 6;
+  const bool first = (threadIdx.x & 63) == 0;
+  float m = wave_max(a.m);
+  if (W > 1) {
+    if (first) buf[0][w] = m;
+    __syncthreads();
 #pragma unroll
-  for (int x = 1; x < kWave; x <<= 1) {
-    LpState b{__shfl_xor(a.m, x, kWave), __shfl_xor(a.l, x, kWave), __shfl_xor(a.s, x, kWave)};
-    lp_join(a, b);
+    for (int i = 0; i < W; ++i) m = fmaxf(m, buf[0][i]);
+  }
+  lp_raise(a, m);
+  a.l = wave_sum(a.l);
+  a.s = wave_sum(a.s);
+  if (W > 1) {
+    if (first) buf[1][w] = a.l, buf[2][w] = a.s;
+    __syncthreads();
+    a.l = a.s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) a.l += buf[1][i], a.s += buf[2][i];
   }
   return a;
 }
@@ -116,6 +126,21 @@ __device__ __forceinline__ void lp_rank(const uint64_t* list, int count, int k, 
   }
 }
 
+// The k-th largest of 16-bit values, N a lane: bit by bit from the top.
+template <int N>
+__device__ __forceinline__ uint32_t lp_kth(const uint32_t (&v)[N], int k) {
+  uint32_t kth = 0;
+#pragma unroll
+  for (int bit = 15; bit >= 0; --bit) {
+    const uint32_t cand = kth | (1u << bit);
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) n += __popcll(__ballot(v[i] >= cand));
+    kth = n >= k ? cand : kth;
+  }
+  return kth;
+}
+
 // W waves a row (1: four rows a workgroup of 256 threads); U runs of 8 a lane and chunk.
 template <typename T, int W, int U, bool TOP>
 __global__ __launch_bounds__(W > 4 ? 64 * W : 256, W > 4 ? 4 : 8) void k_logprob(const LpArgs a) {
@@ -126,7 +151,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256, W > 4 ? 4 : 8) void k_logprob
   __shared__ uint32_t keys_s[2][TOP && W > 1 ? THR : 1];
   __shared__ uint32_t hist[TOP ? ROWS : 1][TOP ? 256 : 1];
   __shared__ int count_s[ROWS];
-  __shared__ LpState st_s[W];
+  __shared__ float st_s[3][W];
   const int t = threadIdx.x & (THR - 1), sub = threadIdx.x / THR;
   const int64_t unit = (int64_t)blockIdx.x * ROWS + sub;
   const int64_t row = ROWS > 1 ? unit : unit / a.nsp;
@@ -204,27 +229,34 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256, W > 4 ? 4 : 8) void k_logprob
       asm volatile("" : "+v"(st.l), "+v"(st.s));
       ++done;
       if (done == next) {
-        // The k-th largest of the lanes' maxima, by the upper halves of their keys.  (A lane that
-        // holds NaN counts with its largest other value: still one of its elements' keys or less.)
+        // The k-th largest of 64 maxima (256 for more than 24 alternatives), by the upper halves of
+        // their keys: those of the waves' lanes together, lane by lane.  (A lane that holds NaN counts
+        // with its largest other value: still one of its elements' keys or less.)
         const bool any = cs + 8 * t < c1;
-        uint32_t v[W];
-        v[0] = any ? value_key(st.l == 0.0f ? -__builtin_inff() : st.m) >> 16 : 0u;
-        if (W > 1) {
+        const uint32_t mine = any ? value_key(st.l == 0.0f ? -__builtin_inff() : st.m) >> 16 : 0u;
+        uint32_t kth;
+        if (W == 1) {
+          const uint32_t v[1] = {mine};
+          kth = lp_kth<1>(v, a.k);
+        } else {
           // two buffers in turn: the next bound's maxima are not written over ones still being read
-          keys_s[turn][t] = v[0];
+          keys_s[turn][t] = mine;
           __syncthreads();
+          uint32_t v[4] = {0, 0, 0, 0};
 #pragma unroll
-          for (int i = 0; i < W; ++i) v[i] = keys_s[turn][64 * i + (t & 63)];
+          for (int i = 0; i < W; ++i) {
+            const uint32_t o = keys_s[turn][64 * i + (t & 63)];
+            v[i & 3] = o > v[i & 3] ? o : v[i & 3];
+          }
           turn ^= 1;
-        }
-        uint32_t kth = 0;
+          if (a.k > 24) {
+            kth = lp_kth<4>(v, a.k);
+          } else {
+            uint32_t u[1] = {v[0]};
 #pragma unroll
-        for (int bit = 15; bit >= 0; --bit) {
-          const uint32_t cand = kth | (1u << bit);
-          int n = 0;
-#pragma unroll
-          for (int i = 0; i < W; ++i) n += __popcll(__ballot(v[i] >= cand));
-          kth = n >= a.k ? cand : kth;
+            for (int i = 1; i < 4; ++i) u[0] = v[i] > u[0] ? v[i] : u[0];
+            kth = lp_kth<1>(u, a.k);
+          }
         }
         thr = kth << 16;
         thr_z = thr == 0u ? -__builtin_inff() : key_value((uint64_t)thr << 32);
@@ -260,14 +292,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256, W > 4 ? 4 : 8) void k_logprob
   if (c < c1) chunk(std::false_type{}, c);
 
   // the row's (or the part's) sums
-  st = lp_wave(st);
-  if (W > 1) {
-    if ((threadIdx.x & 63) == 0) st_s[threadIdx.x >> 6] = st;
-    __syncthreads();
-    st = st_s[0];
-#pragma unroll
-    for (int i = 1; i < W; ++i) lp_join(st, st_s[i]);
-  }
+  st = lp_group<W>(st, st_s);
   const bool split = ROWS == 1 && a.nsp > 1;
   float logl = 0.0f;
   if (live && t == 0 && split) a.part[row * a.nsp + part] = make_float4(st.m, st.l, st.s, 0.0f);
@@ -349,7 +374,8 @@ __global__ __launch_bounds__(64) void k_logprob_join(const LpArgs a) {
   }
   const int n = a.nsp * a.k;
   for (int i = t; i < n; i += 64) jlist[i] = a.part_top[row * n + i];
-  st = lp_wave(st);
+  float none[3][1];
+  st = lp_group<1>(st, none);
   const float logl = st.l == 0.0f ? -__builtin_inff() : logf(st.l);
   if (t == 0) lp_finish(a, row, st, zt, has_t);
   __syncthreads();

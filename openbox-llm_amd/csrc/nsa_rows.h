@@ -7,6 +7,8 @@
 // of element alignment, the row's last run element by element.
 #pragma once
 
+#include <type_traits>
+
 #include "nsa_common.h"
 
 namespace nsa {
@@ -70,16 +72,29 @@ __device__ __forceinline__ void load_run8_of(const void* p, bool is_bf16, int64_
     load_run8(static_cast<const float*>(p) + at, n, f);
 }
 
-// Combine the lanes of a wave; every lane gets the result, in the same order
-// of operations, so that all lanes hold the same bits.
+// Combine the lanes of a wave by register moves alone (within rows of 16 by
+// DPP, across rows by the row swaps); op is commutative, so that all lanes end
+// with the same bits.
 template <typename Op>
 __device__ __forceinline__ float wave_all(float v, Op op) {
-#pragma unroll
-  for (int m = 1; m < kWave; m <<= 1) v = op(v, __shfl_xor(v, m, kWave));
-  return v;
+  auto dpp = [](float x, auto ctrl) {
+    return __uint_as_float(
+        (uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), decltype(ctrl)::value, 0xF, 0xF, false));
+  };
+  v = op(v, dpp(v, std::integral_constant<int, 0xB1>{}));    // quad_perm [1,0,3,2]
+  v = op(v, dpp(v, std::integral_constant<int, 0x4E>{}));    // quad_perm [2,3,0,1]
+  v = op(v, dpp(v, std::integral_constant<int, 0x141>{}));   // row_half_mirror
+  v = op(v, dpp(v, std::integral_constant<int, 0x140>{}));   // row_mirror
+  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = op(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return op(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
 __device__ __forceinline__ float wave_sum(float v) {
   return wave_all(v, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float wave_max(float v) {
+  return wave_all(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
 // Sum over a workgroup of W waves: `buf` holds W floats in LDS and is free
