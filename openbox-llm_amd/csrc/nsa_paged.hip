@@ -54,13 +54,12 @@ struct PagedArgs {
   float sl2;                         // scale * log2 e
 };
 
-// Keys that sequence b attends, twice, plus 1 where the last of them is the row it appends.
+// Keys that sequence b attends, twice, plus 1 where the last of them is the row it would append.  (Where
+// that row has no page, its run has none either: it is neither attended nor written.)
 __device__ __forceinline__ uint32_t paged_keys(const PagedArgs& a, int b) {
   const int cap = a.max_pages * a.P;
   const int len = a.lens[b];
-  if (a.k_new != nullptr &&
-      paged_new_pos(a.table + (int64_t)b * a.max_pages, len, a.P, a.max_pages, a.n_pages) >= 0)
-    return 2u * ((uint32_t)len + 1u) + 1u;
+  if (a.k_new != nullptr && len >= 0 && len < cap) return 2u * ((uint32_t)len + 1u) + 1u;
   return 2u * (uint32_t)(len < 0 ? 0 : (len < cap ? len : cap));
 }
 // Units of a row of n keys: one at least, so that an empty row is written too.
@@ -121,7 +120,7 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
   __shared__ f32x4 qs[NT][KC][QF][64];                // the queries as operands, one piece a lane
   __shared__ float so[4][16][D + 4];                  // the waves' outputs
   __shared__ float sm[4][16], sl[4][16];
-  __shared__ int64_t wsum[4], found[2];
+  __shared__ int wsum[4], found[2];
   __shared__ uint32_t seq_keys[256];                  // of every sequence, where there are no more than 256
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -131,7 +130,7 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
 
   // This workgroup's units: [x, x1) of the list, the first of them in row m of
   // sequence b, whose `units` units start at row0.
-  int64_t x, x1, row0, U = 0, W = 0;
+  int x, x1, row0, W = 0, share = 0, more = 0;        // W shares: `more` of share + 1 units, then of share
   int b, m, units;
   uint32_t keys;
   if (a.W == 0) {                                     // a row each: the list is that row
@@ -145,21 +144,21 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
     // Each thread counts the units of its sequences; the one whose range holds x finds the sequence.
     const int per = (a.B + 255) / 256;
     const int b_lo = min(a.B, (int)threadIdx.x * per), b_hi = min(a.B, b_lo + per);
-    int64_t mine = 0;
+    int mine = 0;
     for (int i = b_lo; i < b_hi; ++i) {
       keys = paged_keys(a, i);
       mine += paged_units(keys);
     }
     if (per == 1 && b_lo < b_hi) seq_keys[b_lo] = keys;
-    int64_t incl = mine;
+    int incl = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-      const int64_t v = __shfl_up(incl, o, 64);
+      const int v = __shfl_up(incl, o, 64);
       if (lane >= o) incl += v;
     }
     if (lane == 63) wsum[w] = incl;
     __syncthreads();
-    int64_t before = incl - mine;
+    int before = incl - mine, U = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (i < w) before += wsum[i];
@@ -168,14 +167,16 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
     U *= M;
     before *= M;
     W = U < a.W ? U : a.W;                            // shares of one unit at least: a row's pieces have no gaps
-    if (blockIdx.x >= W) return;                      // (uniform)
-    x = (int64_t)blockIdx.x * U / W;
-    x1 = ((int64_t)blockIdx.x + 1) * U / W;
+    if ((int)blockIdx.x >= W) return;                 // (uniform)
+    share = U / W;
+    more = U - share * W;
+    x = (int)blockIdx.x * share + min((int)blockIdx.x, more);
+    x1 = x + share + ((int)blockIdx.x < more ? 1 : 0);
     if (x >= before && x < before + mine * M) {
       int i = b_lo;
       if (per > 1) {
         for (;; ++i) {
-          const int64_t u = (int64_t)paged_units(paged_keys(a, i)) * M;
+          const int u = paged_units(paged_keys(a, i)) * M;
           if (x < before + u) break;
           before += u;
         }
@@ -184,26 +185,21 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
       found[1] = before;
     }
     __syncthreads();
-    b = __builtin_amdgcn_readfirstlane((int)found[0]);
+    b = __builtin_amdgcn_readfirstlane(found[0]);
     keys = a.B <= 256 ? (uint32_t)__builtin_amdgcn_readfirstlane((int)seq_keys[b]) : paged_keys(a, b);
     units = paged_units(keys);
-    m = (int)((x - found[1]) / units);
-    row0 = found[1] + (int64_t)m * units;
+    m = (x - found[1]) / units;
+    row0 = found[1] + m * units;
   }
 
   while (x < x1) {
     const int hkv = m / a.HT, ht = m - hkv * a.HT;
-    const int t0 = (int)(x - row0);
-    const int t1 = x1 - row0 < units ? (int)(x1 - row0) : units;
+    const int t0 = x - row0;
+    const int t1 = x1 - row0 < units ? x1 - row0 : units;
     const bool one = t0 == 0 && t1 == units;          // the row in one piece
     const int n = (int)(keys >> 1), pos = (keys & 1u) ? n - 1 : -1;
     const int c0 = kUnit * t0, c1 = min(n, kUnit * t1);
     const int row = b * M + m;
-    if (t0 == 0 && threadIdx.x == 0) {
-      if (a.row_info != nullptr)
-        a.row_info[row] = one ? make_int2(-1, -1) : make_int2((int)blockIdx.x, (int)(((row0 + units) * W - 1) / U));
-      if (a.lens_out != nullptr && m == 0) a.lens_out[b] = pos >= 0 ? n : a.lens[b];
-    }
     const T* kn = static_cast<const T*>(a.k_new) + ((int64_t)b * a.Hkv + hkv) * D;
     const T* vn = static_cast<const T*>(a.v_new) + ((int64_t)b * a.Hkv + hkv) * D;
 
@@ -227,79 +223,98 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
     };
     Frag<T> kf[2][KC];       // keys kb + 8 (c >> 2) + 4 mt + (c & 3)
     VRun<T, VL> vr[8];       // keys kb + 8 g + j
+    uint32_t vm;             // which of keys kb + 8 g .. + 7 are visible
     auto load_k = [&](int i) {
+      if ((i & 31) == 0) look_up(i);
+      const int kb = my0 + kUnit * i;
       const int64_t base_k = c >= 8 ? run_at(2 * i + 1) : run_at(2 * i);
+      vm = (g >= 2 ? run_at(2 * i + 1) : run_at(2 * i)) >= 0 ? range_mask(kb + 8 * g, 0, c1 - 1) : 0u;
       const int ofs = ((8 * (c >> 2)) & 15) + (c & 3);
       if (whole(i)) {
-        const T* row = kp + base_k + ofs * D + 8 * g;
+        const T* at = kp + base_k + ofs * D + 8 * g;
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
           for (int kc = 0; kc < KC; ++kc) {
             if (32 * kc + 8 * g < D)
-              kf[mt][kc].load(row + 4 * mt * D + 32 * kc);
+              kf[mt][kc].load(at + 4 * mt * D + 32 * kc);
             else
               kf[mt][kc].zero();
           }
       } else {
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
-          const int key = my0 + kUnit * i + 8 * (c >> 2) + 4 * mt + (c & 3);
-          const T* row = key == pos ? kn : (key < c1 && base_k >= 0 ? kp + base_k + (ofs + 4 * mt) * D : nullptr);
+          const int key = kb + 8 * (c >> 2) + 4 * mt + (c & 3);
+          const T* at = key == pos ? kn : (key < c1 && base_k >= 0 ? kp + base_k + (ofs + 4 * mt) * D : nullptr);
 #pragma unroll
           for (int kc = 0; kc < KC; ++kc) {
-            if (row != nullptr && 32 * kc + 8 * g < D)
-              kf[mt][kc].load(row + 32 * kc + 8 * g);
+            if (at != nullptr && 32 * kc + 8 * g < D)
+              kf[mt][kc].load(at + 32 * kc + 8 * g);
             else
               kf[mt][kc].zero();
           }
         }
       }
     };
-    auto load_v = [&](int i) {
+    auto load_v = [&](int i) {   // (behind load_k of the same tile)
       const int64_t base_v = g >= 2 ? run_at(2 * i + 1) : run_at(2 * i);
       const int ofs = (8 * g) & 15;
       if (whole(i)) {
-        const T* row = vp + base_v + ofs * D + VL * c;
+        const T* at = vp + base_v + ofs * D + VL * c;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) vr[j] = vrun_load<T, VL>(row + j * D);
+        for (int j = 0; j < 8; ++j) vr[j] = vrun_load<T, VL>(at + j * D);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int key = my0 + kUnit * i + 8 * g + j;
-          const T* row = key == pos ? vn : (key < c1 && base_v >= 0 ? vp + base_v + (ofs + j) * D : nullptr);
-          vr[j] = row != nullptr ? vrun_load<T, VL>(row + VL * c) : vrun_zero<T, VL>();
+          const T* at = key == pos ? vn : (key < c1 && base_v >= 0 ? vp + base_v + (ofs + j) * D : nullptr);
+          vr[j] = at != nullptr ? vrun_load<T, VL>(at + VL * c) : vrun_zero<T, VL>();
         }
       }
     };
+    // queries to LDS as operands: wave w takes every fourth.  They are asked for first: loads return in order.
+    Frag<T> qf[(NT * KC + 3) / 4];
+#pragma unroll
+    for (int f = 0; f < NT * KC; f += 4) {
+      const int nt = (f + w) / KC, kc = (f + w) % KC, hg = ht * 16 * NT + 16 * nt + c;
+      if (f + w < NT * KC && hg < a.G && 32 * kc + 8 * g < D)
+        qf[f / 4].load(static_cast<const T*>(a.q) + ((int64_t)b * a.Hq + (int64_t)hkv * a.G + hg) * D + 32 * kc + 8 * g);
+      else
+        qf[f / 4].zero();
+    }
     if (ntile > 0) {
-      look_up(0);
       load_k(0);
       load_v(0);
     }
-
-    // the append: one wave of the first head tile's piece that holds the position
-    if (pos >= c0 && pos < c1 && ht == 0 && w == 0) {
-      const int64_t at = run_base(a, b, hkv, pos >> 4, D) + (int64_t)(pos & 15) * D;
-      for (int d = lane; d < D; d += 64) {
-        static_cast<T*>(a.kp)[at + d] = kn[d];
-        static_cast<T*>(a.vp)[at + d] = vn[d];
+#pragma unroll
+    for (int f = 0; f < NT * KC; f += 4) {
+      if (f + w < NT * KC) {
+#pragma unroll
+        for (int i = 0; i < QF; ++i)
+          qs[(f + w) / KC][(f + w) % KC][i][lane] = reinterpret_cast<const f32x4*>(&qf[f / 4])[i];
       }
     }
 
-    // queries to LDS: wave w takes every fourth operand
-#pragma unroll
-    for (int f = 0; f < NT * KC; ++f) {
-      if ((f & 3) == w) {
-        const int nt = f / KC, kc = f % KC;
-        const int hg = ht * 16 * NT + 16 * nt + c;
-        Frag<T> q;
-        if (hg < a.G && 32 * kc + 8 * g < D)
-          q.load(static_cast<const T*>(a.q) + ((int64_t)b * a.Hq + (int64_t)hkv * a.G + hg) * D + 32 * kc + 8 * g);
-        else
-          q.zero();
-#pragma unroll
-        for (int i = 0; i < QF; ++i) qs[nt][kc][i][lane] = reinterpret_cast<const f32x4*>(&q)[i];
+    if (t0 == 0 && threadIdx.x == 0) {
+      if (a.row_info != nullptr) {
+        const int last = row0 + units - 1, big = more * (share + 1);   // the share of the row's last unit
+        const int wl = last < big ? last / (share + 1) : more + (last - big) / share;
+        a.row_info[row] = one ? make_int2(-1, -1) : make_int2((int)blockIdx.x, wl);
+      }
+      if (a.lens_out != nullptr && m == 0) {
+        const int len = a.lens[b];
+        a.lens_out[b] =
+            paged_new_pos(a.table + (int64_t)b * a.max_pages, len, a.P, a.max_pages, a.n_pages) >= 0 ? len + 1 : len;
+      }
+    }
+    // the append: one wave of the first head tile's piece that holds the position
+    if (pos >= c0 && pos < c1 && ht == 0 && w == 0) {
+      const int64_t at = run_base(a, b, hkv, pos >> 4, D);
+      if (at >= 0) {
+        for (int d = lane; d < D; d += 64) {
+          static_cast<T*>(a.kp)[at + (int64_t)(pos & 15) * D + d] = kn[d];
+          static_cast<T*>(a.vp)[at + (int64_t)(pos & 15) * D + d] = vn[d];
+        }
       }
     }
     __syncthreads();
@@ -308,8 +323,9 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) acc[nt].init();
     for (int i = 0; i < ntile; ++i) {
-      // the next tile's keys are asked for as soon as this one's are used, its values likewise: a wave has
-      // one or the other in flight at all times, in the registers of one tile
+      // The next tile's keys are asked for as soon as this one's are used, its values likewise: a wave has one or
+      // the other in flight at all times, in the registers of one tile.  (Two tiles ahead measured slower: 232
+      // against 220 us for 32 sequences of up to 32K.)
       f32x4 s[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -324,13 +340,8 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
           mma(s[nt][1], kf[1][kc], q);
         }
       }
-      // visible keys kb + 8 g .. + 7 of this lane
-      const int kb = my0 + kUnit * i;
-      const uint32_t vm = (g >= 2 ? run_at(2 * i + 1) : run_at(2 * i)) >= 0 ? range_mask(kb + 8 * g, 0, c1 - 1) : 0u;
-      if (i + 1 < ntile) {
-        if (((i + 1) & 31) == 0) look_up(i + 1);
-        load_k(i + 1);
-      }
+      const uint32_t seen = vm;
+      if (i + 1 < ntile) load_k(i + 1);
       Frag<T> ph[NT], pl[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -338,7 +349,7 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
         float sv[8], mx = kMaskScore;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          sv[j] = ((vm >> j) & 1u) ? s[nt][j >> 2][j & 3] * a.sl2 : kMaskScore;
+          sv[j] = ((seen >> j) & 1u) ? s[nt][j >> 2][j & 3] * a.sl2 : kMaskScore;
           mx = fmaxf(mx, sv[j]);
         }
         mx = group4_max(mx);
@@ -353,7 +364,7 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
         float p[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          p[j] = ((vm >> j) & 1u) ? fast_exp2(sv[j] - A.m) : 0.0f;
+          p[j] = ((seen >> j) & 1u) ? fast_exp2(sv[j] - A.m) : 0.0f;
           A.l += p[j];
         }
         ph[nt].set(p);
@@ -450,7 +461,7 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
 // turn.  Heads written in one piece are left as they are.
 template <typename T, int D, int W>
 __global__ __launch_bounds__(64 * W) void k_paged_join(const PagedArgs a, int NT) {
-  __shared__ float so[W][D], sl[W];
+  __shared__ float so[W][D], sm[W], sl[W];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t head = blockIdx.x;
   const int b = (int)(head / a.Hq), h = (int)(head % a.Hq);
@@ -463,37 +474,54 @@ __global__ __launch_bounds__(64 * W) void k_paged_join(const PagedArgs a, int NT
   const float2* ml = a.part_ml + slot0;
   const float* po = a.part_o + slot0 * D;
   const int step = 16 * NT;                           // slots from a piece to the next
-  float m = kMaskScore;
-  for (int i = lane; i < np; i += 64) m = fmaxf(m, ml[(int64_t)i * step].x);
-#pragma unroll
-  for (int x = 1; x < 64; x <<= 1) m = xor_max(m, x);
+  // Pieces w, w + W, ... eight at a time, all asked for at once; a running maximum, the waves' own joined below.
   constexpr int E = D >= 64 ? D / 64 : 1;
-  float o[E], l = 0.0f;
+  float m = kMaskScore, l = 0.0f, o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.0f;
-#pragma unroll 8
-  for (int i = w; i < np; i += W) {
-    const float2 s = ml[(int64_t)i * step];
-    const float f = fast_exp2(s.x - m);
-    l += s.y * f;
+  for (int i0 = w; i0 < np; i0 += 8 * W) {
+    float2 s[8];
+    float v[8][E], mx = m;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (E * lane + e < D) o[e] += po[(int64_t)i * step * D + E * lane + e] * f;
+    for (int j = 0; j < 8; ++j) {
+      const int i = i0 + j * W;
+      s[j] = i < np ? ml[(int64_t)i * step] : make_float2(kMaskScore, 0.0f);
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        v[j][e] = i < np && E * lane + e < D ? po[(int64_t)i * step * D + E * lane + e] : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mx = fmaxf(mx, s[j].x);
+    const float f0 = fast_exp2(m - mx);
+    l *= f0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] *= f0;
+    m = mx;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float f = fast_exp2(s[j].x - m);
+      l += s[j].y * f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] += v[j][e] * f;
+    }
   }
 #pragma unroll
   for (int e = 0; e < E; ++e)
     if (E * lane + e < D) so[w][E * lane + e] = o[e];
-  if (lane == 0) sl[w] = l;
+  if (lane == 0) sm[w] = m, sl[w] = l;
   __syncthreads();
+  m = sm[0];
+#pragma unroll
+  for (int i = 1; i < W; ++i) m = fmaxf(m, sm[i]);
   l = 0.0f;
 #pragma unroll
-  for (int i = 0; i < W; ++i) l += sl[i];
+  for (int i = 0; i < W; ++i) l += sl[i] * fast_exp2(sm[i] - m);
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
   if ((int)threadIdx.x < D) {
     const int d = threadIdx.x;
     float v = 0.0f;
 #pragma unroll
-    for (int i = 0; i < W; ++i) v += so[i][d];
+    for (int i = 0; i < W; ++i) v += so[i][d] * fast_exp2(sm[i] - m);
     static_cast<T*>(a.out)[head * D + d] = (T)(v * inv);
   }
   if (a.lse != nullptr && threadIdx.x == 0) a.lse[head] = paged_lse(m, l);
@@ -561,7 +589,8 @@ static PagedPlan paged_plan(int B, int Hq, int Hkv, int row_bytes, int64_t cap, 
 static bool paged_shape_ok(int B, int Hq, int Hkv, int D, int P, int max_pages, int n_pages) {
   return B >= 0 && B <= 65536 && Hkv >= 1 && Hq >= Hkv && Hq % Hkv == 0 && Hq <= 4096 &&
          (D == 16 || D == 32 || D == 64 || D == 128) && P >= 16 && P % 16 == 0 && max_pages >= 1 && n_pages >= 1 &&
-         (int64_t)max_pages * P <= (1 << 30);
+         (int64_t)max_pages * P <= (1 << 30) &&
+         (int64_t)B * Hq * (((int64_t)max_pages * P + kUnit - 1) / kUnit) <= INT32_MAX;   // units are counted in 32 bits
 }
 
 template <typename T, int D>
