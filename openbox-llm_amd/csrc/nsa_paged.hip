@@ -120,6 +120,7 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
   __shared__ f32x4 qs[NT][KC][QF][64];                // the queries as operands, one piece a lane
   __shared__ float so[4][16][D + 4];                  // the waves' outputs
   __shared__ float sm[4][16], sl[4][16];
+  __shared__ __align__(16) T rows_new[2][D];          // the appended row
   __shared__ int wsum[4], found[2];
   __shared__ uint32_t seq_keys[256];                  // of every sequence, where there are no more than 256
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
@@ -216,60 +217,52 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
       const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)base >> 32), i & 63);
       return (int64_t)(((uint64_t)hi << 32) | lo);
     };
-    // whether all of tile i's rows may be read from their pages
-    auto whole = [&](int i) {
-      const int kb = my0 + kUnit * i;
-      return kb + 32 <= c1 && run_at(2 * i) >= 0 && run_at(2 * i + 1) >= 0 && !(pos >= kb && pos < kb + 32);
-    };
+    // Loads of a tile: always the same number, whatever the tile holds, so that waiting for the keys does not
+    // wait for what was asked for behind them.  Runs without a page read page 0 instead, and rows past the
+    // length their own page's; fix() then takes out what is not there.
     Frag<T> kf[2][KC];       // keys kb + 8 (c >> 2) + 4 mt + (c & 3)
     VRun<T, VL> vr[8];       // keys kb + 8 g + j
     uint32_t vm;             // which of keys kb + 8 g .. + 7 are visible
     auto load_k = [&](int i) {
       if ((i & 31) == 0) look_up(i);
-      const int kb = my0 + kUnit * i;
-      const int64_t base_k = c >= 8 ? run_at(2 * i + 1) : run_at(2 * i);
-      vm = (g >= 2 ? run_at(2 * i + 1) : run_at(2 * i)) >= 0 ? range_mask(kb + 8 * g, 0, c1 - 1) : 0u;
-      const int ofs = ((8 * (c >> 2)) & 15) + (c & 3);
-      if (whole(i)) {
-        const T* at = kp + base_k + ofs * D + 8 * g;
+      const int64_t b0 = run_at(2 * i), b1 = run_at(2 * i + 1);
+      vm = (g >= 2 ? b1 : b0) >= 0 ? range_mask(my0 + kUnit * i + 8 * g, 0, c1 - 1) : 0u;
+      const int64_t base_k = c >= 8 ? b1 : b0;
+      const T* at = kp + (base_k >= 0 ? base_k : 0) + (((8 * (c >> 2)) & 15) + (c & 3)) * D + 8 * g;
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+      for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-          for (int kc = 0; kc < KC; ++kc) {
-            if (32 * kc + 8 * g < D)
-              kf[mt][kc].load(at + 4 * mt * D + 32 * kc);
-            else
-              kf[mt][kc].zero();
-          }
-      } else {
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          const int key = kb + 8 * (c >> 2) + 4 * mt + (c & 3);
-          const T* at = key == pos ? kn : (key < c1 && base_k >= 0 ? kp + base_k + (ofs + 4 * mt) * D : nullptr);
-#pragma unroll
-          for (int kc = 0; kc < KC; ++kc) {
-            if (at != nullptr && 32 * kc + 8 * g < D)
-              kf[mt][kc].load(at + 32 * kc + 8 * g);
-            else
-              kf[mt][kc].zero();
-          }
+        for (int kc = 0; kc < KC; ++kc) {
+          if (32 * kc + 8 * g < D)
+            kf[mt][kc].load(at + 4 * mt * D + 32 * kc);
+          else
+            kf[mt][kc].zero();
         }
-      }
     };
     auto load_v = [&](int i) {   // (behind load_k of the same tile)
       const int64_t base_v = g >= 2 ? run_at(2 * i + 1) : run_at(2 * i);
-      const int ofs = (8 * g) & 15;
-      if (whole(i)) {
-        const T* at = vp + base_v + ofs * D + VL * c;
+      const T* at = vp + (base_v >= 0 ? base_v : 0) + ((8 * g) & 15) * D + VL * c;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) vr[j] = vrun_load<T, VL>(at + j * D);
-      } else {
+      for (int j = 0; j < 8; ++j) vr[j] = vrun_load<T, VL>(at + j * D);
+    };
+    // The appended row in place of its page's, which another workgroup may be writing.
+    auto new_k = [&](int i) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int key = my0 + kUnit * i + 8 * g + j;
-          const T* at = key == pos ? vn : (key < c1 && base_v >= 0 ? vp + base_v + (ofs + j) * D : nullptr);
-          vr[j] = at != nullptr ? vrun_load<T, VL>(at + VL * c) : vrun_zero<T, VL>();
+      for (int mt = 0; mt < 2; ++mt) {
+        if (my0 + kUnit * i + 8 * (c >> 2) + 4 * mt + (c & 3) == pos) {
+#pragma unroll
+          for (int kc = 0; kc < KC; ++kc)
+            if (32 * kc + 8 * g < D) kf[mt][kc].load(&rows_new[0][32 * kc + 8 * g]);
         }
+      }
+    };
+    // The values of keys that are not visible to 0 (a weight of 0 does not take NaN out), and the appended row.
+    auto fix_v = [&](int i, uint32_t seen) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (my0 + kUnit * i + 8 * g + j == pos)
+          vr[j] = vrun_load<T, VL>(&rows_new[1][VL * c]);
+        if (((seen >> j) & 1u) == 0u) vr[j] = vrun_zero<T, VL>();
       }
     };
     // queries to LDS as operands: wave w takes every fourth.  They are asked for first: loads return in order.
@@ -307,14 +300,16 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
             paged_new_pos(a.table + (int64_t)b * a.max_pages, len, a.P, a.max_pages, a.n_pages) >= 0 ? len + 1 : len;
       }
     }
-    // the append: one wave of the first head tile's piece that holds the position
-    if (pos >= c0 && pos < c1 && ht == 0 && w == 0) {
+    // the appended row: to LDS for this piece's tiles, and by the first head tile to its page
+    if (pos >= c0 && pos < c1 && threadIdx.x < D) {
+      const int d = threadIdx.x;
+      const T k1 = kn[d], v1 = vn[d];
+      rows_new[0][d] = k1;
+      rows_new[1][d] = v1;
       const int64_t at = run_base(a, b, hkv, pos >> 4, D);
-      if (at >= 0) {
-        for (int d = lane; d < D; d += 64) {
-          static_cast<T*>(a.kp)[at + (int64_t)(pos & 15) * D + d] = kn[d];
-          static_cast<T*>(a.vp)[at + (int64_t)(pos & 15) * D + d] = vn[d];
-        }
+      if (ht == 0 && at >= 0) {
+        static_cast<T*>(a.kp)[at + (int64_t)(pos & 15) * D + d] = k1;
+        static_cast<T*>(a.vp)[at + (int64_t)(pos & 15) * D + d] = v1;
       }
     }
     __syncthreads();
@@ -326,6 +321,9 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
       // The next tile's keys are asked for as soon as this one's are used, its values likewise: a wave has one or
       // the other in flight at all times, in the registers of one tile.  (Two tiles ahead measured slower: 232
       // against 220 us for 32 sequences of up to 32K.)
+      const int kb = my0 + kUnit * i;
+      const bool has_new = pos >= kb && pos < kb + 32;
+      if (has_new) new_k(i);
       f32x4 s[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -341,6 +339,7 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
         }
       }
       const uint32_t seen = vm;
+      const bool all = __all(seen == 0xffu);
       if (i + 1 < ntile) load_k(i + 1);
       Frag<T> ph[NT], pl[NT];
 #pragma unroll
@@ -374,6 +373,7 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
           pl[nt].set(p);
         }
       }
+      if (has_new || !all) fix_v(i, seen);
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         Frag<T> vf;
