@@ -32,6 +32,7 @@ namespace nsa {
 
 constexpr int kLpTopMax = 64;        // most alternatives
 constexpr int kLpCap = 1024;         // candidate list
+constexpr int64_t kLpSlice = 1 << 21;   // rows of one launch
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kFar = -1.0e30f;     // stands for the logarithm of weight 0 where it is multiplied by 0
 
@@ -523,8 +524,27 @@ extern "C" int nsa_logprob_fwd(const void* z, const int64_t* target, float* logp
     a.part = static_cast<float4*>(workspace);
     a.part_top = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + (size_t)rows * nsp * 16);
   }
-  if (dtype == NSA_BF16) return k > 0 ? logprob_launch<bf16, true>(a, s) : logprob_launch<bf16, false>(a, s);
-  return k > 0 ? logprob_launch<float, true>(a, s) : logprob_launch<float, false>(a, s);
+  // 2^21 rows a launch: a grid holds less than 2^32 threads (rows that are split are far fewer)
+  for (int64_t r0 = 0; r0 < rows; r0 += kLpSlice) {
+    LpArgs b = a;
+    b.rows = rows - r0 < kLpSlice ? rows - r0 : kLpSlice;
+    b.z = static_cast<const char*>(z) + r0 * V * (dtype == NSA_BF16 ? 2 : 4);
+    if (target != nullptr) b.target = target + r0;
+    if (logp != nullptr) b.logp = logp + r0;
+    if (entropy != nullptr) b.entropy = entropy + r0;
+    if (stat != nullptr) b.stat = a.stat + r0;
+    if (k > 0) {
+      b.top_logp = top_logp + r0 * k;
+      b.top_idx = top_idx + r0 * k;
+    }
+    int rc;
+    if (dtype == NSA_BF16)
+      rc = k > 0 ? logprob_launch<bf16, true>(b, s) : logprob_launch<bf16, false>(b, s);
+    else
+      rc = k > 0 ? logprob_launch<float, true>(b, s) : logprob_launch<float, false>(b, s);
+    if (rc != NSA_OK) return rc;
+  }
+  return NSA_OK;
 }
 
 extern "C" int nsa_logprob_bwd(const void* z, const int64_t* target, const float* stat, const float* entropy,
@@ -537,19 +557,32 @@ extern "C" int nsa_logprob_bwd(const void* z, const int64_t* target, const float
   NSA_CHECK(z != nullptr && stat != nullptr && dz != nullptr && (dent == nullptr || entropy != nullptr), NSA_ERR_ARG);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int units = (V + kLpBwdUnit - 1) / kLpBwdUnit;
-  const int64_t grid = (rows * units + 3) / 4;
-  NSA_CHECK(grid <= 0x7fffffffLL, NSA_ERR_SHAPE);
-  const LpBwdArgs a{z, target, reinterpret_cast<const float2*>(stat), entropy, dlogp, dent, dz, rows, V, units};
-  if (dtype == NSA_BF16) {
-    if (dent != nullptr)
-      k_logprob_bwd<bf16, true><<<(unsigned)grid, 256, 0, s>>>(a);
-    else
-      k_logprob_bwd<bf16, false><<<(unsigned)grid, 256, 0, s>>>(a);
-  } else {
-    if (dent != nullptr)
-      k_logprob_bwd<float, true><<<(unsigned)grid, 256, 0, s>>>(a);
-    else
-      k_logprob_bwd<float, false><<<(unsigned)grid, 256, 0, s>>>(a);
+  const int64_t slice = (1LL << 25) / units > 1 ? (1LL << 25) / units : 1;   // rows of one launch: 2^31 threads
+  const size_t es = dtype == NSA_BF16 ? 2 : 4;
+  for (int64_t r0 = 0; r0 < rows; r0 += slice) {
+    const int64_t n = rows - r0 < slice ? rows - r0 : slice;
+    const unsigned grid = (unsigned)((n * units + 3) / 4);
+    const LpBwdArgs a{static_cast<const char*>(z) + r0 * V * es,
+                      target == nullptr ? nullptr : target + r0,
+                      reinterpret_cast<const float2*>(stat) + r0,
+                      entropy == nullptr ? nullptr : entropy + r0,
+                      dlogp == nullptr ? nullptr : dlogp + r0,
+                      dent == nullptr ? nullptr : dent + r0,
+                      static_cast<char*>(dz) + r0 * V * es,
+                      n, V, units};
+    if (dtype == NSA_BF16) {
+      if (dent != nullptr)
+        k_logprob_bwd<bf16, true><<<grid, 256, 0, s>>>(a);
+      else
+        k_logprob_bwd<bf16, false><<<grid, 256, 0, s>>>(a);
+    } else {
+      if (dent != nullptr)
+        k_logprob_bwd<float, true><<<grid, 256, 0, s>>>(a);
+      else
+        k_logprob_bwd<float, false><<<grid, 256, 0, s>>>(a);
+    }
+    const int rc = nsa_launch_status();
+    if (rc != NSA_OK) return rc;
   }
-  return nsa_launch_status();
+  return NSA_OK;
 }

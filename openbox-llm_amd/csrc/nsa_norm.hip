@@ -34,6 +34,7 @@ constexpr int kNormWaveMax = 2048;           // widest row of one wave
 constexpr int kNormRegMax = 32768;           // widest row held in registers (forward)
 constexpr int kNormBwdMax = 16384;           // ... and with its gradient and its part of dw (backward)
 constexpr int kNormMax = 1 << 24;            // widest row
+constexpr int64_t kNormSlice = 1 << 21;      // rows of one launch
 
 struct NormArgs {
   const void *x, *res, *w;
@@ -171,10 +172,12 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormBw
   const int t = threadIdx.x & (TPR - 1);
   const int sub = threadIdx.x / TPR;
   const int D = a.D;
-  float w[NV][8], dw[NV][8];
+  // where the registers hold them: the weights for all rows, and dh asked for with the rest of a row
+  constexpr bool kHold = NV * TPR <= 1024;
+  float w[kHold ? NV : 1][8], dw[NV][8];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    load_run8_of(a.w, a.w_bf16, 8 * (i * TPR + t), D - 8 * (i * TPR + t), w[i]);
+    if (kHold) load_run8_of(a.w, a.w_bf16, 8 * (i * TPR + t), D - 8 * (i * TPR + t), w[kHold ? i : 0]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) dw[i][j] = 0.0f;
   }
@@ -182,8 +185,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormBw
   for (int64_t row = (int64_t)blockIdx.x * RPG + sub; row < a.rows; row += (int64_t)gridDim.x * RPG) {
     const int64_t base = row * D;
     const float rstd = a.rstd[row];
-    constexpr bool kEarly = NV * TPR <= 1024;   // dh asked for with the rest, where the registers hold it
-    float n_[NV][8], g[NV][8], d[kEarly ? NV : 1][8];
+    float n_[NV][8], g[NV][8], d[kHold ? NV : 1][8];
     float dot = 0.0f;
     auto load_dh = [&](int i, float(&v)[8]) {
       const int c = 8 * (i * TPR + t);
@@ -199,15 +201,17 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormBw
       const int c = 8 * (i * TPR + t), n = D - c;
       load_run8(static_cast<const RT*>(a.h) + base + c, n, n_[i]);
       load_run8(static_cast<const YT*>(a.dy) + base + c, n, g[i]);
-      if (kEarly) load_dh(i, d[i]);
+      if (kHold) load_dh(i, d[i]);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      float(&wi)[8] = w[kHold ? i : 0];
+      if (!kHold) load_run8_of(a.w, a.w_bf16, 8 * (i * TPR + t), D - 8 * (i * TPR + t), wi);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         n_[i][j] *= rstd;
         dw[i][j] += g[i][j] * n_[i][j];
-        g[i][j] *= w[i][j];
+        g[i][j] *= wi[j];
         dot += g[i][j] * n_[i][j];
       }
     }
@@ -217,8 +221,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormBw
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = 8 * (i * TPR + t), n = D - c;
-      float(&di)[8] = d[kEarly ? i : 0];
-      if (!kEarly) load_dh(i, di);
+      float(&di)[8] = d[kHold ? i : 0];
+      if (!kHold) load_dh(i, di);
 #pragma unroll
       for (int j = 0; j < 8; ++j) di[j] += rstd * (g[i][j] - n_[i][j] * dot);
       if (n > 0) {
@@ -260,35 +264,37 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormBw
 // Rows past kNormBwdMax: one workgroup a row, read twice.
 template <typename YT, typename RT>
 __global__ __launch_bounds__(1024) void k_norm_bwd_long(const NormBwdArgs a) {
-  __shared__ float red[16];
-  const int64_t row = blockIdx.x;
+  __shared__ float red[2][16];
   const int D = a.D;
-  const int64_t base = row * D;
-  const float rstd = a.rstd[row];
-  float dot = 0.0f;
-  for (int c = 8 * threadIdx.x; c < D; c += 8 * 1024) {
-    float h[8], g[8], w[8];
-    load_run8(static_cast<const RT*>(a.h) + base + c, D - c, h);
-    load_run8(static_cast<const YT*>(a.dy) + base + c, D - c, g);
-    load_run8_of(a.w, a.w_bf16, c, D - c, w);
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, ++turn) {
+    const int64_t base = row * D;
+    const float rstd = a.rstd[row];
+    float dot = 0.0f;
+    for (int c = 8 * threadIdx.x; c < D; c += 8 * 1024) {
+      float h[8], g[8], w[8];
+      load_run8(static_cast<const RT*>(a.h) + base + c, D - c, h);
+      load_run8(static_cast<const YT*>(a.dy) + base + c, D - c, g);
+      load_run8_of(a.w, a.w_bf16, c, D - c, w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) dot += g[j] * w[j] * (h[j] * rstd);
-  }
-  dot = group_sum<16>(dot, red) * a.inv_d;
-  for (int c = 8 * threadIdx.x; c < D; c += 8 * 1024) {
-    const int n = D - c;
-    float h[8], g[8], w[8], d[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    load_run8(static_cast<const RT*>(a.h) + base + c, n, h);
-    load_run8(static_cast<const YT*>(a.dy) + base + c, n, g);
-    load_run8_of(a.w, a.w_bf16, c, n, w);
-    if (a.dh != nullptr) load_run8(static_cast<const RT*>(a.dh) + base + c, n, d);
+      for (int j = 0; j < 8; ++j) dot += g[j] * w[j] * (h[j] * rstd);
+    }
+    dot = group_sum<16>(dot, red[turn & 1]) * a.inv_d;
+    for (int c = 8 * threadIdx.x; c < D; c += 8 * 1024) {
+      const int n = D - c;
+      float h[8], g[8], w[8], d[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      load_run8(static_cast<const RT*>(a.h) + base + c, n, h);
+      load_run8(static_cast<const YT*>(a.dy) + base + c, n, g);
+      load_run8_of(a.w, a.w_bf16, c, n, w);
+      if (a.dh != nullptr) load_run8(static_cast<const RT*>(a.dh) + base + c, n, d);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) d[j] += rstd * (g[j] * w[j] - h[j] * rstd * dot);
-    if (a.dx_bf16)
-      store_run8(static_cast<bf16*>(a.dx) + base + c, n, d);
-    else
-      store_run8(static_cast<float*>(a.dx) + base + c, n, d);
-    if (a.dres != nullptr) store_run8(static_cast<RT*>(a.dres) + base + c, n, d);
+      for (int j = 0; j < 8; ++j) d[j] += rstd * (g[j] * w[j] - h[j] * rstd * dot);
+      if (a.dx_bf16)
+        store_run8(static_cast<bf16*>(a.dx) + base + c, n, d);
+      else
+        store_run8(static_cast<float*>(a.dx) + base + c, n, d);
+      if (a.dres != nullptr) store_run8(static_cast<RT*>(a.dres) + base + c, n, d);
+    }
   }
 }
 
@@ -396,7 +402,7 @@ static int norm_bwd_launch(NormBwdArgs a, void* dw, hipStream_t s) {
   const int64_t grid = norm_bwd_groups(a.rows, a.D, cu);
   bool done = false;
   if (a.D > kNormBwdMax) {
-    k_norm_bwd_long<YT, RT><<<(unsigned)a.rows, 1024, 0, s>>>(a);
+    k_norm_bwd_long<YT, RT><<<(unsigned)(a.rows < 8192 ? a.rows : 8192), 1024, 0, s>>>(a);
     if (dw != nullptr)
       k_norm_dw_wide<YT, RT><<<dim3((unsigned)((a.D + 2047) / 2048), (unsigned)grid), 256, 0, s>>>(a);
     done = true;
@@ -433,12 +439,28 @@ extern "C" int nsa_norm_fwd(const void* x, const void* res, const void* w, void*
   NSA_CHECK(res == nullptr || h != nullptr, NSA_ERR_ARG);
   NSA_CHECK(y_dtype != NSA_E4M3 || scale != nullptr, NSA_ERR_ARG);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const NormArgs a{x, res, w, h, y, scale, rstd, rows, D, eps, 1.0f / (float)D, w_dtype == NSA_BF16,
-                   y_dtype == NSA_BF16};
   const bool q8 = y_dtype == NSA_E4M3;
-  if (x_dtype == NSA_BF16)
-    return h_dtype == NSA_BF16 ? norm_fwd_as<bf16, bf16>(a, q8, s) : norm_fwd_as<bf16, float>(a, q8, s);
-  return h_dtype == NSA_BF16 ? norm_fwd_as<float, bf16>(a, q8, s) : norm_fwd_as<float, float>(a, q8, s);
+  const size_t xs = x_dtype == NSA_BF16 ? 2 : 4, hs = h_dtype == NSA_BF16 ? 2 : 4;
+  const size_t ys = q8 ? 1 : y_dtype == NSA_BF16 ? 2 : 4;
+  // 2^21 rows a launch: a grid holds less than 2^32 threads
+  for (int64_t r0 = 0; r0 < rows; r0 += kNormSlice) {
+    const int64_t n = rows - r0 < kNormSlice ? rows - r0 : kNormSlice, at = r0 * D;
+    const NormArgs a{static_cast<const char*>(x) + at * xs,
+                     res == nullptr ? nullptr : static_cast<const char*>(res) + at * hs,
+                     w,
+                     h == nullptr ? nullptr : static_cast<char*>(h) + at * hs,
+                     static_cast<char*>(y) + at * ys,
+                     scale == nullptr ? nullptr : scale + r0,
+                     rstd == nullptr ? nullptr : rstd + r0,
+                     n, D, eps, 1.0f / (float)D, w_dtype == NSA_BF16, y_dtype == NSA_BF16};
+    int rc;
+    if (x_dtype == NSA_BF16)
+      rc = h_dtype == NSA_BF16 ? norm_fwd_as<bf16, bf16>(a, q8, s) : norm_fwd_as<bf16, float>(a, q8, s);
+    else
+      rc = h_dtype == NSA_BF16 ? norm_fwd_as<float, bf16>(a, q8, s) : norm_fwd_as<float, float>(a, q8, s);
+    if (rc != NSA_OK) return rc;
+  }
+  return NSA_OK;
 }
 
 extern "C" size_t nsa_norm_bwd_workspace(int64_t rows, int D, void* stream) {

@@ -595,6 +595,7 @@ static bool paged_shape_ok(int B, int Hq, int Hkv, int D, int P, int max_pages, 
 
 template <typename T, int D>
 static int paged_launch(const PagedArgs& a, const PagedPlan& p, hipStream_t s) {
+  NSA_CHECK(p.R < (1 << 24) && (int64_t)a.B * a.Hq < (1 << 22), NSA_ERR_SHAPE);   // grids hold less than 2^32 threads
   const unsigned grid = (unsigned)(p.W > 0 ? p.W : p.R);
   if (p.NT == 1)
     k_paged<T, D, 1><<<grid, 256, 0, s>>>(a);
@@ -672,7 +673,7 @@ extern "C" int nsa_paged_append(const void* k, const void* v, void* k_pages, voi
                 lens != lens_out && (T == 0 || (k != nullptr && v != nullptr)), NSA_ERR_ARG);
   const int nchunk = T > 64 ? (T + 63) / 64 : 1;
   const int64_t grid = (int64_t)B * Hkv * nchunk;
-  NSA_CHECK(grid <= 0x7fffffffLL, NSA_ERR_SHAPE);
+  NSA_CHECK(grid < (1 << 24), NSA_ERR_SHAPE);   // a grid holds less than 2^32 threads
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == NSA_BF16)
     k_paged_append<bf16><<<(unsigned)grid, 256, 0, s>>>(

@@ -106,7 +106,7 @@ class PagedKVCache:
                  device="cuda", like=None):
         assert page_size >= 16 and page_size % 16 == 0, "paged: the page size must be a multiple of 16"
         assert batch >= 1 and max_len >= 1, "paged: a cache of at least one sequence and one token"
-        self.page_size = page_size
+        self.page_size, self.max_len = page_size, max_len
         self.max_pages = -(-max_len // page_size)
         n_pages = batch * self.max_pages if n_pages is None else n_pages
         shape = (n_pages, n_kv_heads, page_size, head_dim)
@@ -143,8 +143,8 @@ class PagedKVCache:
         acc = self._account
         lengths = [lengths] * self.batch if isinstance(lengths, int) else [int(n) for n in lengths]
         assert len(lengths) == self.batch, "paged: one length for each sequence"
+        assert 0 <= min(lengths) and max(lengths) <= self.max_len, "paged: lengths of 0 to max_len"
         need = [-(-n // self.page_size) for n in lengths]
-        assert max(need) <= self.max_pages, "paged: longer than max_len"
         more = [max(0, n - len(h)) for n, h in zip(need, acc.held)]
         if sum(more) > len(acc.free):
             raise RuntimeError(f"paged: {sum(more)} pages needed, {len(acc.free)} free")

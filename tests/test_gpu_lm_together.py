@@ -86,16 +86,16 @@ def test_training_step_autocast():
         _near(a, b, 16 * 2.0 ** -8)
 
 
-@pytest.mark.parametrize("kw", [dict(pos="rope"), dict(pos="learned"), dict(pos="rope", norm_impl="fused"),
-                                dict(pos="rope", norm="layer"), dict(pos="rope", dense_impl="sdpa", norm_impl="fused")],
-                         ids=str)
-@pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
+KINDS = [dict(pos="rope"), dict(pos="learned"), dict(pos="rope", norm_impl="fused"), dict(pos="rope", norm="layer")]
+
+
+# (the library's attention kernels take 16-bit inputs only)
+@pytest.mark.parametrize("kw,dtype", [(k, d) for k in KINDS for d in (F32, BF)] +
+                         [(dict(pos="rope", dense_impl="sdpa", norm_impl="fused"), BF)], ids=str)
 def test_generation_is_the_forward(kw, dtype):
     """Prefill and steps over paged caches give the forward's logits row by row,
     with sequences of unlike lengths and pages taken as they grow."""
     require_gpu()
-    if dtype == F32 and kw.get("dense_impl") == "sdpa":
-        pytest.skip("the library's attention kernels take 16-bit inputs only")
     m = _model(attn_type="full", dtype=dtype, **kw).eval()
     B, T = 3, 80
     x = _tokens(B, T, 4)

@@ -264,6 +264,40 @@ def test_same_bits_captured_and_replayed():
                 assert torch.equal(a, b)
 
 
+def test_more_rows_than_one_launch():
+    """2^21 rows go to one launch; the rows around the seam and the last ones."""
+    dev = require_gpu()
+    import nsa_lm
+    rows, V = (1 << 21) + 5, 7
+    g = torch.Generator(device=dev).manual_seed(0)
+    z = torch.randn(rows, V, generator=g, device=dev).requires_grad_()
+    t = torch.randint(0, V, (rows,), generator=g, device=dev)
+    dl, dH = torch.randn(rows, generator=g, device=dev), torch.randn(rows, generator=g, device=dev)
+    got = nsa_lm.token_logprobs(z, t, 2)
+    dz, = torch.autograd.grad((got.logp, got.entropy), z, (dl, dH))
+    C = _chain(V)
+    for at in (slice(0, 4), slice((1 << 21) - 3, rows)):
+        lp, lp0, p, H, logp, _ = _ref(z[at].detach(), t[at])
+        # 7 elements: all terms below 8 in magnitude
+        assert ((got.logp[at].double() - logp).abs() <= (C + 6 + 2 * 16) * U).all()
+        assert ((got.entropy[at].double() - H).abs() <= (C + 6 + (2 * C + 20) * 8) * U).all()
+        assert torch.equal(got.top_idx[at], torch.sort(z[at].detach(), dim=1, descending=True, stable=True).indices[:, :2])
+        L, h = dl[at].double()[:, None], dH[at].double()[:, None]
+        ref = (-p * (L + h * (lp0 + H[:, None]))).scatter_add(1, t[at][:, None], L)
+        tol = (p * (L.abs() + 16 * h.abs()) * (C + 12 + 4 * 16) + 2 * L.abs() + p * h.abs() * (2 * C + 20) * 8) * U
+        assert ((dz[at].double() - ref).abs() <= tol + ref.abs() * U).all()
+
+
+def test_second_derivatives_are_refused():
+    import nsa_lm
+    dev = require_gpu()
+    z = torch.randn(4, 30, device=dev, requires_grad=True)
+    got = nsa_lm.token_logprobs(z, torch.zeros(4, device=dev, dtype=torch.long))
+    g, = torch.autograd.grad(got.logp.sum(), z, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.square().sum().backward()
+
+
 def test_refusals():
     import nsa_lm
     dev = require_gpu()

@@ -278,6 +278,78 @@ def test_captured_and_replayed():
                                q.float() if q.dtype == torch.float8_e4m3fn else q)
 
 
+def test_more_rows_than_one_launch():
+    """2^21 rows go to one launch; the rows around the seam and the last ones."""
+    import nsa_lm
+    dev = require_gpu()
+    rows, D = (1 << 21) + 3, 5
+    g = torch.Generator(device=dev).manual_seed(0)
+    x, r = (torch.randn(rows, D, generator=g, device=dev) for _ in range(2))
+    w = torch.rand(D, generator=g, device=dev) + 0.5
+    dy = torch.randn(rows, D, generator=g, device=dev)
+    xs = [t.requires_grad_() for t in (x, r, w)]
+    y, h = nsa_lm.add_rms_norm(*xs, eps=1e-5)
+    q, s, _ = nsa_lm.add_rms_norm_q8(x.detach(), r.detach(), w.detach(), eps=1e-5)
+    dx, = torch.autograd.grad(y, x, dy)
+    C = _chain(D)
+    for at in (slice(0, 4), slice((1 << 21) - 3, rows)):
+        hh = (x[at] + r[at]).detach()
+        assert torch.equal(h[at], hh)
+        ref = _norm64(hh, w.detach(), 1e-5)
+        assert ((y[at].double() - ref).abs() <= _tol(ref, F32, (C / 2 + 7) * U)).all()
+        assert ((s[at].double() * 448 - ref.abs().amax(1)).abs() <= ref.abs().amax(1) * ((C / 2 + 9) * U)).all()
+        h64, g64 = hh.double(), dy[at].double() * w.detach().double()
+        rstd = 1 / torch.sqrt((h64 * h64).mean(1, keepdim=True) + 1e-5)
+        n = h64 * rstd
+        d = rstd * (g64 - n * (g64 * n).mean(1, keepdim=True))
+        mag = rstd * (g64.abs() + n.abs() * (g64 * n).abs().mean(1, keepdim=True))
+        assert ((dx[at].double() - d).abs() <= mag * (2 * C + 14) * U).all()
+
+
+def test_one_tensor_twice_and_second_derivatives():
+    import nsa_lm
+    dev = require_gpu()
+    x = torch.randn(7, 40, device=dev, requires_grad=True)
+    w = torch.rand(40, device=dev, requires_grad=True)
+    y, h = nsa_lm.add_rms_norm(x, x, w, eps=1e-5)
+    assert torch.equal(h, x + x)
+    gx, = torch.autograd.grad((y, h), x, (torch.ones_like(y), torch.ones_like(h)))
+    a, b = x.detach().clone().requires_grad_(), x.detach().clone().requires_grad_()
+    y2, h2 = nsa_lm.add_rms_norm(a, b, w.detach(), eps=1e-5)
+    ga, gb = torch.autograd.grad((y2, h2), (a, b), (torch.ones_like(y), torch.ones_like(h)))
+    assert torch.equal(ga, gb) and torch.equal(gx, ga + gb)
+    y, _ = nsa_lm.add_rms_norm(x, None, w, eps=1e-5)
+    g, = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+def test_two_streams_at_once():
+    """Calls in flight on two streams share nothing."""
+    import nsa_lm
+    dev = require_gpu()
+    sets = [tuple(t.to(dev) for t in _inputs(4000, 1024, BF, F32, F32, seed=s)) for s in range(2)]
+    dy = torch.randn(4000, 1024, device=dev).to(BF)
+
+    def once(x, r, w):
+        a = [t.detach().requires_grad_() for t in (x, r, w)]
+        y, h = nsa_lm.add_rms_norm(*a, eps=1e-5, out_dtype=BF)
+        return (y, h, *torch.autograd.grad((y, h), a, (dy, r)))
+    want = [once(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(once(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o in got[i]:
+            for a, b in zip(o, want[i]):
+                assert torch.equal(a, b)
+
+
 def test_refusals():
     import nsa_lm
     dev = require_gpu()

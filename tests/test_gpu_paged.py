@@ -293,6 +293,42 @@ def test_other_stream_and_same_bits():
     assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
 
 
+def test_two_streams_at_once():
+    """Steps in flight on two streams, over caches of their own, share nothing."""
+    import nsa_paged
+    dev = require_gpu()
+    sets = [[t.to(dev) if torch.is_tensor(t) else t
+             for t in _setup(5, [900 + 300 * s, 3000, 0, 17, 400], 64, 4, 128, 64, 50, BF, seed=s, fill=0.0)]
+            for s in range(2)]
+    want = [nsa_paged.paged_step(*[t.clone() for t in s[:7]]) for s in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(nsa_paged.paged_step(*sets[i][:7]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out, lens in got[i]:
+            assert torch.equal(out, want[i][0]) and torch.equal(lens, want[i][1])
+
+
+def test_many_sequences_and_shares():
+    """More sequences than threads count at once, shares of many rows and rows of many shares."""
+    import nsa_paged
+    dev = require_gpu()
+    lens = [(i * 7919) % 60 for i in range(700)]
+    lens[350] = 3000
+    q, kn, vn, kp, vp, table, L, ks, vs = _setup(700, lens, 4, 1, 32, 16, 200, BF, seed=1, extra=1)
+    kp, vp = kp[:1 + int(table.max())], vp[:1 + int(table.max())]
+    # a capacity past 1 MiB a row: shares, not a row to a workgroup
+    table = torch.nn.functional.pad(table, (0, 400), value=-1)
+    out, new = nsa_paged.paged_step(*(t.to(dev) for t in (q, kn, vn, kp, vp, table, L)))
+    _compare(out, q, [torch.cat([k, n[:, None]], 1) for k, n in zip(ks, kn)],
+             [torch.cat([v, n[:, None]], 1) for v, n in zip(vs, vn)])
+    assert new.tolist() == [n + 1 for n in lens]
+
+
 def test_cache_pages():
     import nsa_paged
     dev = require_gpu()
@@ -302,8 +338,9 @@ def test_cache_pages():
     assert c.free_pages == 4 and two.table is c.table and (c.table.cpu() >= 0).sum(1).tolist() == [3, 1]
     with pytest.raises(RuntimeError):
         c.reserve([33, 100])
-    with pytest.raises(AssertionError):
-        c.reserve(113)
+    for bad in (101, -1, [5]):
+        with pytest.raises(AssertionError):
+            c.reserve(bad)
     assert c.free_pages == 4
     two.reserve([40, 80])                 # 3 held already, 4 more for the second
     ids = c.table.cpu()
