@@ -571,7 +571,10 @@ struct PagedPlan {
   int64_t R;             // rows: sequences x KV heads x head tiles
   bool joined;           // there may be pieces to join
 };
-// Shares: two for every compute unit.  Where the rows fill the chip and none can
+// Shares: two for every compute unit, so that one loads while the other starts
+// or ends a piece (16 x 4K with a KV head for every head: 65 us, 82 with one);
+// one where the rows are few and long (one sequence of 32K: 19.9 us, 20.9 with
+// two; 32 of up to 32K: 215, 217).  Where the rows fill the chip and none can
 // be long (1 MiB of keys and values), a workgroup takes a row instead (W = 0):
 // nothing is counted and nothing joined.
 static PagedPlan paged_plan(int B, int Hq, int Hkv, int row_bytes, int64_t cap, int cu) {
@@ -582,7 +585,8 @@ static PagedPlan paged_plan(int B, int Hq, int Hkv, int row_bytes, int64_t cap, 
   p.R = (int64_t)B * Hkv * p.HT;
   const int64_t most = p.R * ((cap + kUnit - 1) / kUnit);
   const bool rows = cap <= kUnit || (p.R >= cu && cap * 2 * row_bytes <= (1 << 20));
-  p.W = rows ? 0 : (int)(most < 2LL * cu ? most : 2LL * cu);
+  const int64_t shares = p.R <= cu / 2 && cap >= 32 * kUnit ? cu : 2LL * cu;
+  p.W = rows ? 0 : (int)(most < shares ? most : shares);
   p.joined = !rows;
   return p;
 }
