@@ -14,11 +14,18 @@
 // them when its runs of a chunk raise its maximum.  For the alternatives the k-th
 // largest of 64 or 256 maxima over parts of the row is a lower bound of the
 // row's k-th value (k parts hold one such element each): elements below it are
-// dropped, the few others (24 of 32000 for 20 alternatives) go to a list in LDS as (value, ~index) keys, which are all
-// different, and are ranked by counting.  The bound is formed after the
-// first chunk, which is still in registers, and again whenever the chunks done
-// have doubled: 16 ballots, one for each of the upper bits of a value's key.  A row that overfills the list (long ties, a rising
-// row) is selected exactly by eight radix passes over the keys instead.
+// dropped, the few others (24 of 32000 for 20 alternatives) go to a list in LDS
+// as (value, ~index) keys, which are all different, and are ranked by counting.
+// The bound is formed after the first chunk and again whenever the chunks done
+// have doubled: 16 ballots, one for each of the upper bits of a value's key.  A
+// row that overfills the list (long ties, a rising row) is selected exactly by
+// eight radix passes over the keys instead.
+//
+// Measured (MI355X): 32768 x 32000 in bf16 384 us forward and 737 backward, 5.5
+// and 5.7 TB/s, bound by memory; 2047 x 50257 with 5 alternatives 48 us (38 at
+// the rate of a large copy: all rows start and end together, so their bounds,
+// sums and rankings are not hidden); 32 x 32000 with 20 8.5 us, a row's own
+// chain of load, sums, bound and ranking.
 //
 // One wave takes a row of up to 2048 elements, a workgroup of four or sixteen a
 // longer one; few and very long rows are split over workgroups, whose (m, l, s)
@@ -98,12 +105,11 @@ __device__ __forceinline__ LpState lp_group(LpState a, float (&buf)[3][W]) {
 }
 
 // Results of one row from its sums (one thread).
-__device__ __forceinline__ float lp_finish(const LpArgs& a, int64_t row, LpState st, float zt, bool has_t) {
+__device__ __forceinline__ void lp_finish(const LpArgs& a, int64_t row, LpState st, float zt, bool has_t) {
   const float logl = st.l == 0.0f ? -__builtin_inff() : logf(st.l);
   if (a.stat != nullptr) a.stat[row] = make_float2(st.m, logl);
   if (a.entropy != nullptr) a.entropy[row] = st.l == 0.0f ? 0.0f : logl - st.s / st.l;
   if (a.logp != nullptr) a.logp[row] = has_t ? (st.l == 0.0f ? -__builtin_inff() : (zt - st.m) - logl) : 0.0f;
-  return logl;
 }
 
 // The target's logit: asked for at the start, so that its load is not waited for at the end.

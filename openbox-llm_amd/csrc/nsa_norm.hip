@@ -16,6 +16,10 @@
 // (past 32768 elements, 16384 in the backward, a row is read again, through the
 // cache).
 //
+// Measured (MI355X): 32768 x 768, float32 stream and bf16 branch, 58 us forward
+// and 78 backward, 5.2 TB/s, and 7 for dw; 8191 x 8192 in bf16 with rows in 8
+// bits 95 us, 4.9 TB/s (a large copy reaches 4.9 to 5.5); 32 x 8192 3.4 us.
+//
 // Threads per row: one wave up to 2048 elements (no barrier at all), 256 or
 // 1024 threads above, in runs of 8 elements.  Where the rows are too few to
 // fill the chip, a row takes as many threads as it has runs.

@@ -17,8 +17,8 @@ on the device: a generation loop never waits for the host, and a step can be
 captured into a graph.  Query head h reads KV head ``h // (Hq // Hkv)``.
 
 Table entries outside ``0 .. n_pages-1`` are no pages: keys there are not
-attended and rows are not written.  Rows past a length are never read.  A
-negative length stands for no sequence: its output is zeros, its length stays.
+attended and rows are not written.  Rows past a length have no influence,
+whatever they hold.  A negative length stands for no sequence: its output is zeros, its length stays.
 """
 
 import torch
