@@ -16,13 +16,12 @@
 // (past 32768 elements, 16384 in the backward, a row is read again, through the
 // cache).
 //
-// Measured (MI355X): 32768 x 768, float32 stream and bf16 branch, 58 us forward
-// and 78 backward, 5.2 TB/s, and 7 for dw; 8191 x 8192 in bf16 with rows in 8
-// bits 95 us, 4.9 TB/s (a large copy reaches 4.9 to 5.5); 32 x 8192 3.4 us.
+// Measured (MI355X): 32768 x 768, float32 stream and bf16 branch, 138 us
+// forward and backward, 5.1 TB/s; 8191 x 8192 in bf16 with rows in 8 bits 88 us,
+// 5.3 TB/s (a large copy reaches 4.9 to 5.5); 32 x 8192 3.4 us.
 //
-// Threads per row: one wave up to 2048 elements (no barrier at all), 256 or
-// 1024 threads above, in runs of 8 elements.  Where the rows are too few to
-// fill the chip, a row takes as many threads as it has runs.
+// Threads per row: one wave to sixteen, a run of 8 elements each to 8192
+// elements (norm_shape); up to one wave there is no barrier at all.
 //
 // The backward's workgroups walk over rows in a stride of the grid and keep
 // their columns' part of dw in registers; the parts are added in workgroup
@@ -34,7 +33,6 @@ namespace nsa {
 
 constexpr float kQ8Max = 448.0f;            // largest e4m3 value
 constexpr float kQ8Floor = 0x1p-100f;
-constexpr int kNormWaveMax = 2048;           // widest row of one wave
 constexpr int kNormRegMax = 32768;           // widest row held in registers (forward)
 constexpr int kNormBwdMax = 16384;           // ... and with its gradient and its part of dw (backward)
 constexpr int kNormMax = 1 << 24;            // widest row
@@ -82,13 +80,13 @@ __device__ __forceinline__ void norm_sum8(const NormArgs& a, int64_t at, int n, 
 
 // TPR threads a row, NV runs of 8 a thread (NV = 0: any length, h formed again for every pass).
 template <typename XT, typename RT, bool RES, bool Q8, int TPR, int NV>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(const NormArgs a) {
-  constexpr int W = TPR / kWave;
+__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void k_norm_fwd(const NormArgs a) {
+  constexpr int W = TPR > kWave ? TPR / kWave : 1;
   __shared__ float red[2][W];
   __shared__ uint32_t redm[W];
   const int t = threadIdx.x & (TPR - 1);
-  const int64_t row = TPR < 256 ? (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR : (int64_t)blockIdx.x;
-  if (TPR < 256 && row >= a.rows) return;   // whole waves; no barrier follows for TPR == 64
+  const int64_t row = TPR == 64 ? (int64_t)blockIdx.x * 4 + threadIdx.x / 64 : (int64_t)blockIdx.x;
+  if (TPR == 64 && row >= a.rows) return;   // (whole waves; no barrier follows for these)
   const int D = a.D;
   const int64_t base = row * D;
   const int nrun = NV > 0 ? NV : (D + 8 * TPR - 1) / (8 * TPR);
@@ -103,7 +101,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(const NormAr
     for (int j = 0; j < 8; ++j) ss += hi[j] * hi[j];
     if (RES && n > 0) store_run8(static_cast<RT*>(a.h) + base + c, n, hi);
   }
-  ss = group_sum<W>(ss, red[0]);
+  ss = row_sum<TPR>(ss, red[0]);
   const float rstd = 1.0f / sqrtf(ss * a.inv_d + a.eps);
   if (a.rstd != nullptr && t == 0) a.rstd[row] = rstd;
   uint32_t am = 0;   // |y| as bits: the order of the magnitudes, NaN above infinity
@@ -127,6 +125,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_fwd(const NormAr
     }
   }
   if (Q8) {
+    // (a non-negative float's bits have its order, NaN's above infinity's)
     am = wave_reduce_u32<true>(am);
     if (W > 1) {
       if ((threadIdx.x & (kWave - 1)) == 0) redm[threadIdx.x / kWave] = am;
@@ -168,11 +167,11 @@ struct NormBwdArgs {
 
 // YT: dy; RT: h, dh and dres.  dres is null where dx serves both (one type).
 template <typename YT, typename RT, int TPR, int NV>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormBwdArgs a) {
-  constexpr int W = TPR / kWave;
-  constexpr int RPG = TPR < 256 ? 256 / TPR : 1;   // rows at a time
+__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void k_norm_bwd(const NormBwdArgs a) {
+  constexpr int W = TPR > kWave ? TPR / kWave : 1;
+  constexpr int RPG = TPR == 64 ? 4 : 1;   // rows at a time
   __shared__ float red[2][W];
-  __shared__ float dws[TPR < 256 ? 2048 : 1];
+  __shared__ float dws[RPG > 1 ? 8 * TPR * NV : 1];
   const int t = threadIdx.x & (TPR - 1);
   const int sub = threadIdx.x / TPR;
   const int D = a.D;
@@ -220,7 +219,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_bwd(const NormBw
       }
     }
     // two buffers in turn: the next row's sum is not written over one still being read
-    dot = group_sum<W>(dot, red[turn & 1]) * a.inv_d;
+    dot = row_sum<TPR>(dot, red[turn & 1]) * a.inv_d;
     ++turn;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -283,7 +282,7 @@ __global__ __launch_bounds__(1024) void k_norm_bwd_long(const NormBwdArgs a) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) dot += g[j] * w[j] * (h[j] * rstd);
     }
-    dot = group_sum<16>(dot, red[turn & 1]) * a.inv_d;
+    dot = row_sum<1024>(dot, red[turn & 1]) * a.inv_d;
     for (int c = 8 * threadIdx.x; c < D; c += 8 * 1024) {
       const int n = D - c;
       float h[8], g[8], w[8], d[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -349,34 +348,33 @@ __global__ __launch_bounds__(1024) void k_norm_dw(const float* __restrict__ part
   }
 }
 
-// Threads a row and runs a thread.  A row takes the fewest threads that hold
-// it (one wave to 2048 elements, 256 threads to 8192, 1024 above), which keeps
-// several rows in flight on a compute unit; fewer rows than compute units
-// take as many threads as they have runs.
+// Threads a row and runs a thread: the fewest threads that hold the row with one
+// run each (8192 x 8192 in bf16: 93 us with 1024 threads, 104 with four runs in
+// 256; 32768 x 768 forward and backward, float32 stream: 138 us with 128 threads,
+// 142 with two runs in 64); past 8192 elements two or four runs in 1024.
 struct NormShape {
   int tpr, nv;
 };
-static NormShape norm_shape(int64_t rows, int D, int cu) {
+#define NSA_NORM_SHAPES(X) X(64, 1) X(128, 1) X(256, 1) X(512, 1) X(1024, 1) X(1024, 2)
+static NormShape norm_shape(int D) {
   const int runs = (D + 7) / 8;
-  int tpr = D <= kNormWaveMax ? 64 : D <= 8192 ? 256 : 1024;
-  if (rows <= cu) tpr = runs <= 64 ? 64 : runs <= 256 ? 256 : 1024;
-  if (D > kNormRegMax) return {1024, 0};
-  const int nv = (runs + tpr - 1) / tpr;
-  return {tpr, nv == 3 ? (tpr == 64 ? 3 : 4) : nv};
+#define NSA_NORM_FITS(TPR, NV) \
+  if (runs <= TPR * NV) return {TPR, NV};
+  NSA_NORM_SHAPES(NSA_NORM_FITS)
+#undef NSA_NORM_FITS
+  return {1024, D <= kNormRegMax ? 4 : 0};
 }
 
 template <typename XT, typename RT, bool RES, bool Q8>
 static int norm_fwd_launch(const NormArgs& a, hipStream_t s) {
-  const NormShape sh = norm_shape(a.rows, a.D, device_cu_count(s));
-#define NSA_NORM_CASE(TPR, NV)                                                                             \
-  if (sh.tpr == TPR && sh.nv == NV) {                                                                      \
-    const int64_t grid = TPR < 256 ? (a.rows + 256 / TPR - 1) / (256 / TPR) : a.rows;                      \
-    k_norm_fwd<XT, RT, RES, Q8, TPR, NV><<<(unsigned)grid, TPR < 256 ? 256 : TPR, 0, s>>>(a);              \
-    return nsa_launch_status();                                                                            \
+  const NormShape sh = norm_shape(a.D);
+#define NSA_NORM_CASE(TPR, NV)                                                                    \
+  if (sh.tpr == TPR && sh.nv == NV) {                                                             \
+    const int64_t grid = TPR == 64 ? (a.rows + 3) / 4 : a.rows;                      \
+    k_norm_fwd<XT, RT, RES, Q8, TPR, NV><<<(unsigned)grid, TPR == 64 ? 256 : TPR, 0, s>>>(a);     \
+    return nsa_launch_status();                                                                   \
   }
-  NSA_NORM_CASE(64, 1) NSA_NORM_CASE(64, 2) NSA_NORM_CASE(64, 3) NSA_NORM_CASE(64, 4)
-  NSA_NORM_CASE(256, 1) NSA_NORM_CASE(256, 2) NSA_NORM_CASE(256, 4)
-  NSA_NORM_CASE(1024, 1) NSA_NORM_CASE(1024, 2) NSA_NORM_CASE(1024, 4) NSA_NORM_CASE(1024, 0)
+  NSA_NORM_SHAPES(NSA_NORM_CASE) NSA_NORM_CASE(1024, 4) NSA_NORM_CASE(1024, 0)
 #undef NSA_NORM_CASE
   return NSA_ERR_SHAPE;
 }
@@ -389,20 +387,21 @@ static int norm_fwd_as(const NormArgs& a, bool q8, hipStream_t s) {
   return NSA_ERR_DTYPE;
 }
 
-// Parts of dw: a workgroup of the backward each, as many as fill the chip's
-// waves (eight of 256 threads to a compute unit); past kNormBwdMax a row group of k_norm_dw_wide.
+// Parts of dw: a workgroup of the backward each, eight to a compute unit or what
+// its waves hold; past kNormBwdMax a row group of k_norm_dw_wide.
 static int64_t norm_bwd_groups(int64_t rows, int D, int cu) {
   if (D > kNormBwdMax) return rows < 128 ? rows : 128;
-  const NormShape sh = norm_shape(rows, D, cu);
-  const int64_t groups = sh.tpr == 64 ? (rows + 3) / 4 : rows;
-  const int64_t most = (int64_t)cu * (sh.tpr == 1024 ? 2 : 8);
+  const NormShape sh = norm_shape(D);
+  const int rpg = sh.tpr == 64 ? 4 : 1;
+  const int64_t groups = (rows + rpg - 1) / rpg;
+  const int64_t most = (int64_t)cu * (sh.tpr <= 256 ? 8 : 2048 / sh.tpr);
   return groups < most ? groups : most;
 }
 
 template <typename YT, typename RT>
 static int norm_bwd_launch(NormBwdArgs a, void* dw, hipStream_t s) {
   const int cu = device_cu_count(s);
-  const NormShape sh = norm_shape(a.rows, a.D, cu);
+  const NormShape sh = norm_shape(a.D);
   const int64_t grid = norm_bwd_groups(a.rows, a.D, cu);
   bool done = false;
   if (a.D > kNormBwdMax) {
@@ -411,14 +410,12 @@ static int norm_bwd_launch(NormBwdArgs a, void* dw, hipStream_t s) {
       k_norm_dw_wide<YT, RT><<<dim3((unsigned)((a.D + 2047) / 2048), (unsigned)grid), 256, 0, s>>>(a);
     done = true;
   }
-#define NSA_NORM_CASE(TPR, NV)                                                                        \
-  if (!done && sh.tpr == TPR && sh.nv == NV) {                                                        \
-    k_norm_bwd<YT, RT, TPR, NV><<<(unsigned)grid, TPR < 256 ? 256 : TPR, 0, s>>>(a);                  \
-    done = true;                                                                                      \
+#define NSA_NORM_CASE(TPR, NV)                                                            \
+  if (!done && sh.tpr == TPR && sh.nv == NV) {                                            \
+    k_norm_bwd<YT, RT, TPR, NV><<<(unsigned)grid, TPR == 64 ? 256 : TPR, 0, s>>>(a);      \
+    done = true;                                                                          \
   }
-  NSA_NORM_CASE(64, 1) NSA_NORM_CASE(64, 2) NSA_NORM_CASE(64, 3) NSA_NORM_CASE(64, 4)
-  NSA_NORM_CASE(256, 1) NSA_NORM_CASE(256, 2) NSA_NORM_CASE(256, 4)
-  NSA_NORM_CASE(1024, 1) NSA_NORM_CASE(1024, 2)
+  NSA_NORM_SHAPES(NSA_NORM_CASE)
 #undef NSA_NORM_CASE
   if (!done) return NSA_ERR_SHAPE;
   if (dw != nullptr)

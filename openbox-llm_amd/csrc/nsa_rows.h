@@ -97,17 +97,17 @@ __device__ __forceinline__ float wave_max(float v) {
   return wave_all(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
-// Sum over a workgroup of W waves: `buf` holds W floats in LDS and is free
-// again after the next barrier that follows.
-template <int W>
-__device__ __forceinline__ float group_sum(float v, float* buf) {
+// Sum over the N threads of a row: a wave, or a workgroup of several (`buf` then
+// holds a float a wave in LDS and is free again after the next barrier that follows).
+template <int N>
+__device__ __forceinline__ float row_sum(float v, float* buf) {
   v = wave_sum(v);
-  if (W == 1) return v;
+  if (N == kWave) return v;
   if ((threadIdx.x & (kWave - 1)) == 0) buf[threadIdx.x / kWave] = v;
   __syncthreads();
   float s = 0.0f;
 #pragma unroll
-  for (int i = 0; i < W; ++i) s += buf[i];
+  for (int i = 0; i < N / kWave; ++i) s += buf[i];
   return s;
 }
 
