@@ -20,8 +20,8 @@
 // forward and backward, 5.1 TB/s; 8191 x 8192 in bf16 with rows in 8 bits 88 us,
 // 5.3 TB/s (a large copy reaches 4.9 to 5.5); 32 x 8192 3.4 us.
 //
-// Threads per row: one wave to sixteen, a run of 8 elements each to 8192
-// elements (norm_shape); up to one wave there is no barrier at all.
+// Threads per row: eight to 1024, a run of 8 elements each to 8192 elements
+// (norm_shape); up to one wave there is no barrier at all.
 //
 // The backward's workgroups walk over rows in a stride of the grid and keep
 // their columns' part of dw in registers; the parts are added in workgroup
@@ -80,13 +80,13 @@ __device__ __forceinline__ void norm_sum8(const NormArgs& a, int64_t at, int n, 
 
 // TPR threads a row, NV runs of 8 a thread (NV = 0: any length, h formed again for every pass).
 template <typename XT, typename RT, bool RES, bool Q8, int TPR, int NV>
-__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void k_norm_fwd(const NormArgs a) {
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_norm_fwd(const NormArgs a) {
   constexpr int W = TPR > kWave ? TPR / kWave : 1;
   __shared__ float red[2][W];
   __shared__ uint32_t redm[W];
   const int t = threadIdx.x & (TPR - 1);
-  const int64_t row = TPR == 64 ? (int64_t)blockIdx.x * 4 + threadIdx.x / 64 : (int64_t)blockIdx.x;
-  if (TPR == 64 && row >= a.rows) return;   // (whole waves; no barrier follows for these)
+  const int64_t row = TPR <= 64 ? (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR : (int64_t)blockIdx.x;
+  if (TPR <= 64 && row >= a.rows) return;   // (all of a row's lanes; no barrier follows for these)
   const int D = a.D;
   const int64_t base = row * D;
   const int nrun = NV > 0 ? NV : (D + 8 * TPR - 1) / (8 * TPR);
@@ -126,7 +126,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void k_norm_fwd(const NormAr
   }
   if (Q8) {
     // (a non-negative float's bits have its order, NaN's above infinity's)
-    am = wave_reduce_u32<true>(am);
+    am = lanes_all<(TPR < kWave ? TPR : kWave)>(am, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
     if (W > 1) {
       if ((threadIdx.x & (kWave - 1)) == 0) redm[threadIdx.x / kWave] = am;
       __syncthreads();
@@ -167,9 +167,9 @@ struct NormBwdArgs {
 
 // YT: dy; RT: h, dh and dres.  dres is null where dx serves both (one type).
 template <typename YT, typename RT, int TPR, int NV>
-__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void k_norm_bwd(const NormBwdArgs a) {
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_norm_bwd(const NormBwdArgs a) {
   constexpr int W = TPR > kWave ? TPR / kWave : 1;
-  constexpr int RPG = TPR == 64 ? 4 : 1;   // rows at a time
+  constexpr int RPG = TPR <= 64 ? 256 / TPR : 1;   // rows at a time
   __shared__ float red[2][W];
   __shared__ float dws[RPG > 1 ? 8 * TPR * NV : 1];
   const int t = threadIdx.x & (TPR - 1);
@@ -246,16 +246,19 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void k_norm_bwd(const NormBw
       if (c < D) store_run8(out + c, D - c, dw[i]);
     }
   } else {
-    // the waves' parts, added in wave order
-    for (int s = 0; s < RPG; ++s) {
-      if (sub == s) {
+    static_assert(NV == 1, "a row of at most a wave is one run a lane");
+    // the rows of a wave by halves, then the waves' parts in wave order
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
+    for (int x = TPR; x < kWave; x <<= 1)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int c = 8 * (i * TPR + t) + j;
-            if (c < D) dws[c] = s == 0 ? dw[i][j] : dws[c] + dw[i][j];
-          }
+      for (int j = 0; j < 8; ++j) dw[0][j] += __shfl_xor(dw[0][j], x, kWave);
+    const int w = threadIdx.x / kWave;
+    for (int s = 0; s < 4; ++s) {
+      if (w == s && (threadIdx.x & (kWave - 1)) < TPR) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int c = 8 * t + j;
+          if (c < D) dws[c] = s == 0 ? dw[0][j] : dws[c] + dw[0][j];
         }
       }
       __syncthreads();
@@ -355,7 +358,7 @@ __global__ __launch_bounds__(1024) void k_norm_dw(const float* __restrict__ part
 struct NormShape {
   int tpr, nv;
 };
-#define NSA_NORM_SHAPES(X) X(64, 1) X(128, 1) X(256, 1) X(512, 1) X(1024, 1) X(1024, 2)
+#define NSA_NORM_SHAPES(X) X(8, 1) X(16, 1) X(32, 1) X(64, 1) X(128, 1) X(256, 1) X(512, 1) X(1024, 1) X(1024, 2)
 static NormShape norm_shape(int D) {
   const int runs = (D + 7) / 8;
 #define NSA_NORM_FITS(TPR, NV) \
@@ -370,8 +373,8 @@ static int norm_fwd_launch(const NormArgs& a, hipStream_t s) {
   const NormShape sh = norm_shape(a.D);
 #define NSA_NORM_CASE(TPR, NV)                                                                    \
   if (sh.tpr == TPR && sh.nv == NV) {                                                             \
-    const int64_t grid = TPR == 64 ? (a.rows + 3) / 4 : a.rows;                      \
-    k_norm_fwd<XT, RT, RES, Q8, TPR, NV><<<(unsigned)grid, TPR == 64 ? 256 : TPR, 0, s>>>(a);     \
+    const int64_t grid = TPR <= 64 ? (a.rows + 256 / TPR - 1) / (256 / TPR) : a.rows;             \
+    k_norm_fwd<XT, RT, RES, Q8, TPR, NV><<<(unsigned)grid, TPR <= 64 ? 256 : TPR, 0, s>>>(a);     \
     return nsa_launch_status();                                                                   \
   }
   NSA_NORM_SHAPES(NSA_NORM_CASE) NSA_NORM_CASE(1024, 4) NSA_NORM_CASE(1024, 0)
@@ -392,7 +395,7 @@ static int norm_fwd_as(const NormArgs& a, bool q8, hipStream_t s) {
 static int64_t norm_bwd_groups(int64_t rows, int D, int cu) {
   if (D > kNormBwdMax) return rows < 128 ? rows : 128;
   const NormShape sh = norm_shape(D);
-  const int rpg = sh.tpr == 64 ? 4 : 1;
+  const int rpg = sh.tpr <= 64 ? 256 / sh.tpr : 1;
   const int64_t groups = (rows + rpg - 1) / rpg;
   const int64_t most = (int64_t)cu * (sh.tpr <= 256 ? 8 : 2048 / sh.tpr);
   return groups < most ? groups : most;
@@ -412,7 +415,7 @@ static int norm_bwd_launch(NormBwdArgs a, void* dw, hipStream_t s) {
   }
 #define NSA_NORM_CASE(TPR, NV)                                                            \
   if (!done && sh.tpr == TPR && sh.nv == NV) {                                            \
-    k_norm_bwd<YT, RT, TPR, NV><<<(unsigned)grid, TPR == 64 ? 256 : TPR, 0, s>>>(a);      \
+    k_norm_bwd<YT, RT, TPR, NV><<<(unsigned)grid, TPR <= 64 ? 256 : TPR, 0, s>>>(a);      \
     done = true;                                                                          \
   }
   NSA_NORM_SHAPES(NSA_NORM_CASE)

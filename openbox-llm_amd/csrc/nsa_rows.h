@@ -72,37 +72,47 @@ __device__ __forceinline__ void load_run8_of(const void* p, bool is_bf16, int64_
     load_run8(static_cast<const float*>(p) + at, n, f);
 }
 
-// Combine the lanes of a wave by register moves alone (within rows of 16 by
-// DPP, across rows by the row swaps); op is commutative, so that all lanes end
-// with the same bits.
-template <typename Op>
-__device__ __forceinline__ float wave_all(float v, Op op) {
-  auto dpp = [](float x, auto ctrl) {
-    return __uint_as_float(
-        (uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), decltype(ctrl)::value, 0xF, 0xF, false));
+// Combine each N = 8, 16, 32 or 64 neighbouring lanes of a wave by register
+// moves alone (within rows of 16 by DPP, across rows by the row swaps); op is
+// commutative, so that all of them end with the same bits.
+template <int N, typename Op>
+__device__ __forceinline__ uint32_t lanes_all(uint32_t v, Op op) {
+  auto dpp = [](uint32_t x, auto ctrl) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, decltype(ctrl)::value, 0xF, 0xF, false);
   };
-  v = op(v, dpp(v, std::integral_constant<int, 0xB1>{}));    // quad_perm [1,0,3,2]
-  v = op(v, dpp(v, std::integral_constant<int, 0x4E>{}));    // quad_perm [2,3,0,1]
-  v = op(v, dpp(v, std::integral_constant<int, 0x141>{}));   // row_half_mirror
-  v = op(v, dpp(v, std::integral_constant<int, 0x140>{}));   // row_mirror
-  const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = op(__uint_as_float(p[0]), __uint_as_float(p[1]));
-  const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return op(__uint_as_float(q[0]), __uint_as_float(q[1]));
+  v = op(v, dpp(v, std::integral_constant<int, 0xB1>{}));     // quad_perm [1,0,3,2]
+  v = op(v, dpp(v, std::integral_constant<int, 0x4E>{}));     // quad_perm [2,3,0,1]
+  v = op(v, dpp(v, std::integral_constant<int, 0x141>{}));    // row_half_mirror: 8
+  if (N >= 16) v = op(v, dpp(v, std::integral_constant<int, 0x140>{}));   // row_mirror: 16
+  if (N >= 32) {
+    const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = op(p[0], p[1]);
+  }
+  if (N >= 64) {
+    const auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = op(p[0], p[1]);
+  }
+  return v;
 }
+template <int N = kWave>
 __device__ __forceinline__ float wave_sum(float v) {
-  return wave_all(v, [](float a, float b) { return a + b; });
+  return __uint_as_float(lanes_all<N>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
 }
 __device__ __forceinline__ float wave_max(float v) {
-  return wave_all(v, [](float a, float b) { return fmaxf(a, b); });
+  return __uint_as_float(lanes_all<kWave>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
 }
 
-// Sum over the N threads of a row: a wave, or a workgroup of several (`buf` then
-// holds a float a wave in LDS and is free again after the next barrier that follows).
+// Sum over the N threads of a row: part of a wave, a wave, or a workgroup of
+// several (`buf` then holds a float a wave in LDS and is free again after the
+// next barrier that follows).
 template <int N>
 __device__ __forceinline__ float row_sum(float v, float* buf) {
-  v = wave_sum(v);
-  if (N == kWave) return v;
+  v = wave_sum<(N < kWave ? N : kWave)>(v);
+  if (N <= kWave) return v;
   if ((threadIdx.x & (kWave - 1)) == 0) buf[threadIdx.x / kWave] = v;
   __syncthreads();
   float s = 0.0f;

@@ -54,7 +54,7 @@ TYPES = [(BF, BF, BF, BF), (BF, F32, F32, BF), (F32, F32, F32, F32), (F32, BF, F
          (F32, F32, BF, BF)]
 SHAPES = [(1, 1), (3, 7), (5, 8), (2, 64), (1, 511), (300, 512), (257, 768), (9, 1001), (700, 1537), (4, 2048),
           (600, 2049), (3, 4095), (300, 4104), (300, 8192), (2, 8200), (260, 9001), (2, 16384), (260, 20001),
-          (2, 32768), (3, 33001)]
+          (2, 32768), (3, 33001), (1003, 64), (517, 128), (301, 250), (5000, 30)]
 
 
 @pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(str(x)[6:] for x in t))
