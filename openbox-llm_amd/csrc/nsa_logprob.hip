@@ -27,8 +27,8 @@
 // sums and rankings are not hidden); 32 x 32000 with 20 8.5 us, a row's own
 // chain of load, sums, bound and ranking.
 //
-// One wave takes a row of up to 2048 elements, a workgroup of four or sixteen a
-// longer one; few and very long rows are split over workgroups, whose (m, l, s)
+// One wave takes a row of up to 2048 elements (8192 where the rows are many), a
+// workgroup of four or sixteen a longer one; few and very long rows are split over workgroups, whose (m, l, s)
 // and lists a second launch joins.
 #include <type_traits>
 
@@ -462,12 +462,20 @@ __global__ __launch_bounds__(256) void k_logprob_bwd(const LpBwdArgs a) {
   }
 }
 
-// Waves of a row: one up to 2048 elements; sixteen where the rows leave most of
+// Waves of a row: one up to 2048 elements, and up to 8192 where the rows give
+// every compute unit sixteen waves by themselves: no barriers, and no idle lanes
+// where a row is little more than a workgroup's chunk (32768 x 2500 in bf16 with
+// one wave 48 us, with four 80; 8192 x 8192 with 5 alternatives 36 and 50,
+// without them 30 and 29; more than 24 alternatives need four waves' maxima;
+// longer rows gain a tenth, at four times the additions in a lane).  Sixteen where the rows leave most of
 // the chip's waves idle (a row of 32000 in 16 bits is then one chunk); else four.
 // A row of more than 256 KiB is split where there are not enough of them
 // either, into parts of 8192 elements or more, two for every compute unit: one
 // workgroup's loads would take longer than the second launch.
-static int lp_waves(int64_t rows, int V, int cu) { return V <= 2048 ? 1 : rows <= 2 * cu ? 16 : 4; }
+static int lp_waves(int64_t rows, int V, int k, int cu) {
+  if (V <= 2048 || (V <= 8192 && k <= 24 && rows >= 16 * cu)) return 1;
+  return rows <= 2 * cu ? 16 : 4;
+}
 static int lp_parts(int64_t rows, int V, int esize, int cu) {
   if ((int64_t)V * esize <= 256 * 1024 || rows >= 2 * cu) return 1;
   int64_t want = (2LL * cu + rows - 1) / rows;
@@ -485,15 +493,23 @@ static int lp_seg(int V, int nsp) {
 
 template <typename T, bool TOP>
 static int logprob_launch(LpArgs a, hipStream_t s) {
-  const int w = a.nsp > 1 ? 4 : lp_waves(a.rows, a.V, device_cu_count(s));
-  if (w == 1)
-    k_logprob<T, 1, 4, TOP><<<(unsigned)((a.rows + 3) / 4), 256, 0, s>>>(a);
-  else if (w == 4)
+  const int w = a.nsp > 1 ? 4 : lp_waves(a.rows, a.V, a.k, device_cu_count(s));
+  if (w == 1) {
+    // as many runs in flight as the row has: 32768 x 512 takes 13 us with one run, 22 with four
+    const unsigned grid = (unsigned)((a.rows + 3) / 4);
+    if (a.V <= 512)
+      k_logprob<T, 1, 1, TOP><<<grid, 256, 0, s>>>(a);
+    else if (a.V <= 1024)
+      k_logprob<T, 1, 2, TOP><<<grid, 256, 0, s>>>(a);
+    else
+      k_logprob<T, 1, 4, TOP><<<grid, 256, 0, s>>>(a);
+  } else if (w == 4) {
     // runs in flight against waves: 2047 x 50257 with 5 alternatives takes 58 us at four runs, 54 at three, 56 at
     // two; 8192 x 32000 without them 105, 109 and 101
     k_logprob<T, 4, TOP ? 3 : 2, TOP><<<(unsigned)(a.rows * a.nsp), 256, 0, s>>>(a);
-  else
+  } else {
     k_logprob<T, 16, 4, TOP><<<(unsigned)a.rows, 1024, 0, s>>>(a);
+  }
   if (a.nsp > 1) k_logprob_join<T><<<(unsigned)a.rows, 64, (size_t)a.nsp * a.k * 8, s>>>(a);
   return nsa_launch_status();
 }

@@ -7,7 +7,8 @@ of a row takes at most CHAIN additions of positive terms, so that l is within
   logp = (z_t - m) - ln l:          that, and 2 u of either term;
   H = ln l - s / l:                 that, with s within (CHAIN + 8) u of sum e |z-m|;
   dz = -p (dl + dH (ln p + H)):      p within (CHAIN + 10 + 4 |ln p|) u, H's error, half a step.
-CHAIN: V / 256 elements of a lane (32 for one wave's rows) + 6 + 4 + 64 parts.
+CHAIN: V / 256 elements of a lane (32 for one wave's rows) + 6 + 4 + 64 parts + 32;
+a wave that takes a row of up to 8192 by itself has V / 64 + 6, no more than that.
 """
 
 import pytest
@@ -102,7 +103,8 @@ def _check(z, t, top, dev, grad=True):
 
 SHAPES = [(1, 1, 1), (1, 2, 2), (5, 7, 3), (3, 64, 64), (9, 100, 20), (4, 511, 64), (6, 513, 5), (7, 2048, 64),
           (3, 2049, 1), (2, 4097, 64), (1, 8191, 20), (5, 8193, 33), (1, 50257, 20), (33, 32000, 5), (1, 131072, 64),
-          (2, 200001, 7), (1100, 4100, 3), (1030, 20011, 10)]
+          (2, 200001, 7), (1100, 4100, 3), (1030, 20011, 10),
+          (9, 1000, 7), (2001, 129, 2), (4099, 2300, 24), (4096, 8191, 5)]
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
@@ -131,6 +133,14 @@ def test_rows_that_overfill_the_candidate_list(V):
         _check(z, t, top, dev, grad=False)
     _check(z[:7].to(BF), t[:7], 64, dev, grad=False)
     _check(z[:2], t[:2], 64, dev, grad=False)
+
+
+def test_many_rows_of_one_wave_that_overfill_the_list():
+    dev = require_gpu()
+    V = 3000
+    r = torch.arange(V).float()
+    z = torch.stack([torch.zeros(V), r / V, -(r / 97).floor(), (r >= V // 2).float()]).repeat(1025, 1)
+    _check(z, torch.arange(4100) % V, 20, dev, grad=False)
 
 
 def test_signed_zeros_tie():
