@@ -531,12 +531,14 @@ int nsa_decode_step(void* kc, void* vc, void* ks, void* vs, void* kw, void* vw, 
  * h = x (h is not written, h_dtype = x_dtype).  y_dtype NSA_E4M3: y [rows][D]
  * bytes hold y / scale[row], scale = max(row's |y|, 2^-100) / 448 (float).
  * rstd (float [rows], nullable): 1 / sqrt(mean h^2 + eps), for the backward.
- * x, h / res and w are NSA_F32 or NSA_BF16, each on its own.  D <= 2^24. */
+ * x, h / res and w are NSA_F32 or NSA_BF16, each on its own.  D <= 2^24.  The
+ * outputs are buffers of their own: a long row is read after its sum is written. */
 int nsa_norm_fwd(const void* x, const void* res, const void* w, void* h, void* y, float* scale, float* rstd,
                  int64_t rows, int D, float eps, int x_dtype, int h_dtype, int w_dtype, int y_dtype, void* stream);
 /* Its backward: dy in y_dtype, dh (nullable) the gradient of h in h_dtype; dx
  * in x_dtype, dres (nullable: dx serves both) in h_dtype, dw (nullable) in
- * w_dtype, summed over the rows in an order fixed by the shape.  workspace:
+ * w_dtype, summed over the rows in an order fixed by the shape; no output
+ * overlaps an input.  workspace:
  * nsa_norm_bwd_workspace bytes (0: unsupported shape); not read where dw is
  * null. */
 size_t nsa_norm_bwd_workspace(int64_t rows, int D, void* stream);

@@ -379,6 +379,10 @@ std::tuple<Tensor, OptTensor, OptTensor> paged(const Tensor& q_, const OptTensor
   const int64_t Hq = q_.size(1);
   NSA_ASSERT(Hq >= 1 && Hq % Hkv == 0, "GQA needs n_q_heads divisible by n_kv_heads");
   NSA_ASSERT(Hq <= 4096 && B <= 65536, "paged: at most 4096 heads and 65536 sequences");
+  if (at::GradMode::is_enabled())
+    NSA_ASSERT(!q_.requires_grad() && !(k_new && (k_new->requires_grad() || v_new->requires_grad())) &&
+                   !kp.requires_grad() && !vp.requires_grad(),
+               "paged: attention over pages has no gradient: call it under torch.no_grad()");
   const Tensor q = aligned(q_), table = table_.contiguous(), lens = lens_.contiguous();
   Tensor kn, vn, lens_out, lse;
   if (k_new) {

@@ -15,7 +15,8 @@ rows that are not dense are made contiguous.  Sums and statistics are float32.
 Violations raise ``AssertionError``; a missing library raises ``RuntimeError``.
 Every call launches on the current stream of its tensors' device, allocates
 its outputs and workspace with torch, and never waits for the host: calls can
-be captured into a graph.  First derivatives only; the checks, allocations and
+be captured into a graph (a backward, as any torch function's, with no eager
+graph of the same leaves alive).  First derivatives only; the checks, allocations and
 autograd nodes are C++ (csrc/nsa_torch.cpp).
 """
 

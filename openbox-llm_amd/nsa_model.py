@@ -238,7 +238,8 @@ class Rotary(nn.Module):
     def tables(self, T, device, dtype):
         """The factors ``forward`` multiplies by, ``cos, sin [T, dim/2]`` with
         the values of ``dtype``, held as float32 (the fused head split's
-        tables); cached per length, device, dtype and frequency buffer."""
+        tables); cached per length, device, dtype and frequency buffer, but for
+        those that a graph's capture only records."""
         inv = self.inv_freq
         key = (T, str(device), dtype, inv.dtype, inv.data_ptr(), inv._version)
         hit = self._tables.get(key)
@@ -246,10 +247,18 @@ class Rotary(nn.Module):
             with torch.no_grad(), torch.autocast(device_type=torch.device(device).type, enabled=False):
                 ang = torch.arange(T, device=device, dtype=torch.float32)[:, None] * inv.to(device)[None, :]
                 hit = (ang.cos().to(dtype).float().contiguous(), ang.sin().to(dtype).float().contiguous())
+            if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+                return hit
             if len(self._tables) > 8:
                 self._tables.clear()
             self._tables[key] = hit
         return hit
+
+    def at(self, pos, dtype):
+        """The same factors for one token a sequence at ``pos [B]``: ``[B, 1, dim/2]``."""
+        with torch.autocast(device_type=pos.device.type, enabled=False):
+            ang = pos.float()[:, None, None] * self.inv_freq
+            return ang.cos().to(dtype), ang.sin().to(dtype)
 
     def forward(self, x):
         """``x [B,H,T,D]`` rotated by position ``t``."""
@@ -604,22 +613,22 @@ class FullAttention(nn.Module):
 
     def prefill(self, x, cache, lens=None):
         """``forward(x)``, its keys and values kept in the (empty) cache, ``lens``
-        tokens of each sequence (default all); the pages must be reserved."""
+        tokens of each sequence (default all); the pages must be reserved.
+        Gradients are the forward's; none pass through the cache."""
         q, k, v = self._qkv(x)
-        cache.prefill(k.to(cache.k_pages.dtype), v.to(cache.v_pages.dtype), lens)
+        cache.prefill(k.detach().to(cache.k_pages.dtype), v.detach().to(cache.v_pages.dtype), lens)
         return self._causal(q, k, v)
 
+    @torch.no_grad()
     def step(self, x, cache):
         """The row of ``forward`` at the cache's next position: ``x [B, d_model]``
-        -> ``[B, d_model]``, its key and value appended."""
+        -> ``[B, d_model]``, its key and value appended (no gradient)."""
         B, dt = x.shape[0], cache.k_pages.dtype
         q = self.q_proj(x).view(B, self.Hq, self.dh)
         k = self.k_proj(x).view(B, self.Hkv, self.dh)
         v = self.v_proj(x).view(B, self.Hkv, self.dh)
         if self.rope is not None:
-            cos, sin = self.rope.tables(cache.capacity, x.device, q.dtype)
-            at = cache.lens.long().clamp(0, cache.capacity - 1)
-            cos, sin = cos[at][:, None].to(q.dtype), sin[at][:, None].to(q.dtype)
+            cos, sin = self.rope.at(cache.lens, q.dtype)
             q, k = _rotate(q, cos, sin), _rotate(k, cos, sin)
         o = cache.step(q.to(dt), k.to(dt), v.to(dt))
         return self.out_proj(o.reshape(B, self.Hq * self.dh).to(x.dtype))
@@ -682,6 +691,7 @@ class Block(nn.Module):
         y, x = _fused_norm(self.ln2, (attn or self.attn)(y), x)
         return x, self.ffn(y)
 
+    @torch.no_grad()
     def step(self, x, branch, cache):
         """One token of every sequence, ``x [B, d_model]``: the pair of
         ``pending`` (with ``norm_impl='ref'`` the branch is None throughout)."""

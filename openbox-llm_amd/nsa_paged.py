@@ -19,6 +19,8 @@ captured into a graph.  Query head h reads KV head ``h // (Hq // Hkv)``.
 Table entries outside ``0 .. n_pages-1`` are no pages: keys there are not
 attended and rows are not written.  Rows past a length have no influence,
 whatever they hold.  A negative length stands for no sequence: its output is zeros, its length stays.
+
+For inference: inputs that need a gradient are refused.
 """
 
 import torch
@@ -66,6 +68,8 @@ def paged_append(k, v, k_pages, v_pages, table, lens, count=None):
         "paged: rows must be [B, Hkv, T, D]"
     assert all(t.dtype == k_pages.dtype and t.device == k_pages.device for t in (k, v)), \
         "paged: rows in the pages' dtype and device"
+    assert not (torch.is_grad_enabled() and any(t.requires_grad for t in (k, v, k_pages, v_pages))), \
+        "paged: rows in pages have no gradient: call it under torch.no_grad()"
     assert Hkv <= 4096 and B <= 65536, "paged: at most 4096 heads and 65536 sequences"
     k, v, table, lens = _ops._contig(k), _ops._contig(v), table.contiguous(), lens.contiguous()
     if count is not None:
@@ -177,11 +181,13 @@ class PagedKVCache:
             lens = torch.as_tensor(lens, dtype=torch.int32).expand(self.batch)
         if lens is not None:
             lens = lens.to(device=self.lens.device, dtype=torch.int32)
-        self.lens = paged_append(k, v, self.k_pages, self.v_pages, self.table, self.lens, lens)
+        self.lens.copy_(paged_append(k, v, self.k_pages, self.v_pages, self.table, self.lens, lens))
 
     def step(self, q, k_new, v_new, scale=None):
-        """``paged_step`` on this cache -> ``out [B, Hq, D]``."""
-        out, self.lens = paged_step(q, k_new, v_new, self.k_pages, self.v_pages, self.table, self.lens, scale)
+        """``paged_step`` on this cache -> ``out [B, Hq, D]``.  The lengths are
+        updated in place: a captured step advances the cache on every replay."""
+        out, lens = paged_step(q, k_new, v_new, self.k_pages, self.v_pages, self.table, self.lens, scale)
+        self.lens.copy_(lens)
         return out
 
     def attend(self, q, scale=None, return_lse=False):

@@ -163,6 +163,57 @@ def test_captured_generation_with_log_probabilities():
             assert torch.equal(a, b), s
 
 
+def test_eager_steps_beside_a_capture_that_has_not_run():
+    """A step's rotation does not come from memory that a capture has only
+    recorded the writing of."""
+    require_gpu()
+    m = _model(attn_type="full", pos="rope").eval()
+    x = _tokens(2, 30, 5)
+    with torch.no_grad():
+        want = m(x)[0]
+
+    def start(max_len, n):
+        caches = m.paged_caches(2, max_len, page_size=16)
+        caches[0].reserve(max_len)
+        m.prefill(x[:, :n], caches)
+        return caches
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        m.step(x[:, 20], start(64, 20))
+    torch.cuda.current_stream().wait_stream(side)
+    caches = start(96, 25)
+    tok = x[:, 25].contiguous()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = m.step(tok, caches)
+    eager = start(96, 10)
+    for s in range(10, 30):
+        _near(m.step(x[:, s], eager), want[:, s], 1e-4)
+    for s in range(25, 30):       # every replay is a step further
+        tok.copy_(x[:, s])
+        graph.replay()
+        torch.cuda.synchronize()
+        _near(out, want[:, s], 1e-4)
+    assert all(c.lens.tolist() == [30, 30] for c in caches + eager)
+
+
+def test_layers_steps_under_gradients():
+    """A layer's step has no gradient; its prefill has the forward's."""
+    require_gpu()
+    m = _model(attn_type="full", pos="rope")
+    at = m.blocks[0].attn
+    x = torch.randn(2, 20, CFG["d_model"], generator=torch.Generator().manual_seed(0)).cuda().requires_grad_()
+    cache = at.paged_cache(2, 32, page_size=16)
+    cache.reserve(21)
+    y = at.prefill(x, cache)
+    want = at(x)
+    _near(y.detach(), want.detach(), 1e-5)
+    g = torch.ones_like(y)
+    _near(torch.autograd.grad(y, x, g)[0], torch.autograd.grad(want, x, g)[0], 1e-5)
+    assert not at.step(x[:, 0], cache).requires_grad
+
+
 def test_score():
     require_gpu()
     m = _model(attn_type="full", pos="rope").eval()

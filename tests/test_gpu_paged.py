@@ -381,3 +381,20 @@ def test_refusals():
     with pytest.raises(AssertionError):
         nsa_paged.PagedKVCache(2, 1, 48, 100)
     assert math.isfinite(float(nsa_paged.paged_attend(**ok).float().sum()))
+
+
+def test_gradients_are_refused():
+    import nsa_paged
+    dev = require_gpu()
+    q, kn, vn, kp, vp, table, L, _, _ = (t.to(dev) if torch.is_tensor(t) else t
+                                         for t in _setup(2, [5, 20], 4, 2, 64, 16, 3, F32))
+    leaf = q.detach().clone().requires_grad_()
+    row = kn.detach().clone().requires_grad_()
+    with pytest.raises(AssertionError):
+        nsa_paged.paged_attend(leaf, kp, vp, table, L)
+    with pytest.raises(AssertionError):
+        nsa_paged.paged_step(q, row, vn, kp, vp, table, L)
+    with pytest.raises(AssertionError):
+        nsa_paged.paged_append(row[:, :, None], vn[:, :, None], kp, vp, table, L)
+    with torch.no_grad():
+        assert torch.equal(nsa_paged.paged_attend(leaf, kp, vp, table, L), nsa_paged.paged_attend(q, kp, vp, table, L))
