@@ -17,8 +17,8 @@
 // cache).
 //
 // Measured (MI355X): 32768 x 768, float32 stream and bf16 branch, 138 us
-// forward and backward, 5.1 TB/s; 8191 x 8192 in bf16 with rows in 8 bits 88 us,
-// 5.3 TB/s (a large copy reaches 4.9 to 5.5); 32 x 8192 3.4 us.
+// forward and backward, 5.1 TB/s; 8191 x 8192 in bf16 with rows in 8 bits 84 to
+// 87 us, 5.4 TB/s (a large copy reaches 4.9 to 5.5); 32 x 8192 3.5 us.
 //
 // Threads per row: eight to 1024, a run of 8 elements each to 8192 elements
 // (norm_shape); up to one wave there is no barrier at all.
@@ -352,9 +352,9 @@ __global__ __launch_bounds__(1024) void k_norm_dw(const float* __restrict__ part
 }
 
 // Threads a row and runs a thread: the fewest threads that hold the row with one
-// run each (8192 x 8192 in bf16: 93 us with 1024 threads, 104 with four runs in
-// 256; 32768 x 768 forward and backward, float32 stream: 138 us with 128 threads,
-// 142 with two runs in 64); past 8192 elements two or four runs in 1024.
+// run each (8191 x 8192 in bf16 with rows in 8 bits: 84 us with 1024 threads, 95
+// with four runs in 256; 32768 x 768 forward and backward, float32 stream: 138 us
+// with 128 threads, 142 with two runs in 64); past 8192 elements two or four runs in 1024.
 struct NormShape {
   int tpr, nv;
 };
