@@ -13,13 +13,18 @@
 // The forward reads the row once.  A lane keeps its own (m, l, s) and rescales
 // them when its runs of a chunk raise its maximum.  For the alternatives the k-th
 // largest of 64 or 256 maxima over parts of the row is a lower bound of the
-// row's k-th value (k parts hold one such element each): elements below it are
-// dropped, the few others (24 of 32000 for 20 alternatives) go to a list in LDS
-// as (value, ~index) keys, which are all different, and are ranked by counting.
-// The bound is formed after the first chunk and again whenever the chunks done
-// have doubled: 16 ballots, one for each of the upper bits of a value's key.  A
-// row that overfills the list (long ties, a rising row) is selected exactly by
-// eight radix passes over the keys instead.
+// row's k-th value (k parts hold one such element each).  It is formed after the
+// first chunk and again whenever the chunks done are four times as many: 16
+// ballots, one for each of the upper bits of a value's key.  Runs with nothing at
+// or above it are dropped; the others are noted, and at the end read again, all
+// at once: the loop waits for no load but its own.  Their elements (24 of 32000
+// for 20 alternatives) go to a list in LDS as (value, ~index) keys, which are all
+// different, and are ranked by counting.  Masked elements (-inf, the type's
+// lowest value) are never noted.  A row that overfills a list (long ties, a
+// rising row), or that has fewer than k unmasked elements, is selected exactly
+// by up to eight radix passes over the keys instead (32 x 32000 with five tokens
+// left and 20 alternatives: 50 us; 238 with every lane's own LDS atomics and all
+// eight passes).
 //
 // Measured (MI355X): 32768 x 32000 in bf16 384 us forward and 737 backward, 5.5
 // and 5.7 TB/s, bound by memory; 2047 x 50257 with 5 alternatives 48 us (38 at
@@ -148,16 +153,23 @@ __device__ __forceinline__ uint32_t lp_kth(const uint32_t (&v)[N], int k) {
   return kth;
 }
 
+// The lowest finite value of a type's key.
+template <typename T>
+__device__ constexpr uint32_t lowest_key() {
+  return sizeof(T) == 2 ? 0x0080ffffu : 0x00800000u;   // ~0xff7f0000, ~0xff7fffff
+}
+
 // W waves a row (1: four rows a workgroup of 256 threads); U runs of 8 a lane and chunk.
 template <typename T, int W, int U, bool TOP>
 __global__ __launch_bounds__(W > 4 ? 64 * W : 256, W > 4 ? 4 : 8) void k_logprob(const LpArgs a) {
   constexpr int THR = 64 * W;               // threads a row
   constexpr int ROWS = W > 1 ? 1 : 4;       // rows a workgroup
   constexpr int CAP = W > 1 ? kLpCap : 512;
+  constexpr int RUNS = W > 1 ? kLpCap : 256;   // list of runs, in the place of the radix passes' counts
   __shared__ uint64_t list_s[TOP ? ROWS : 1][TOP ? CAP : 1];
   __shared__ uint32_t keys_s[2][TOP && W > 1 ? THR : 1];
-  __shared__ uint32_t hist[TOP ? ROWS : 1][TOP ? 256 : 1];
-  __shared__ int count_s[ROWS];
+  __shared__ __align__(16) uint32_t hist[TOP ? ROWS : 1][TOP ? RUNS : 1];
+  __shared__ int nruns_s[ROWS], count_s[ROWS];
   __shared__ float st_s[3][W];
   const int t = threadIdx.x & (THR - 1), sub = threadIdx.x / THR;
   const int64_t unit = (int64_t)blockIdx.x * ROWS + sub;
@@ -176,11 +188,12 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256, W > 4 ? 4 : 8) void k_logprob
     else
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
-  if (TOP && t == 0) count_s[sub] = 0;   // (added to only behind the first bound's barrier)
+  if (TOP && t == 0) nruns_s[sub] = count_s[sub] = 0;   // (added to only behind the first bound's barrier)
 
   LpState st{kLowest, 0.0f, 0.0f};
-  uint32_t thr = 0;             // keys below it are no alternatives
-  float thr_z = -__builtin_inff();
+  constexpr uint32_t kMasked = lowest_key<T>();
+  uint32_t thr = kMasked + 1;   // keys below it are no alternatives: masked elements least of all
+  float thr_z = key_value((uint64_t)thr << 32);
   int next = 1;                 // chunks done at the bound's next forming
   int done = 0, turn = 0;
   constexpr int CH = THR * 8 * U;
@@ -265,28 +278,19 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256, W > 4 ? 4 : 8) void k_logprob
             kth = lp_kth<1>(u, a.k);
           }
         }
-        thr = kth << 16;
-        thr_z = thr == 0u ? -__builtin_inff() : key_value((uint64_t)thr << 32);
-        next *= 2;
+        thr = max(kth << 16, kMasked + 1);
+        thr_z = key_value((uint64_t)thr << 32);
+        next *= 4;
       }
-      // the runs with an element at or above the bound: few, read again through the cache so that the
-      // streaming loop keeps its registers
+      // the runs with an element at or above the bound: few, noted for the end
       uint32_t runs = 0;
 #pragma unroll
       for (int u = 0; u < U; ++u) runs |= (mxu[u] < thr_z ? 0u : 1u) << u;
       if (st.l != st.l) runs = (1u << U) - 1;
       while (runs != 0) {
-        const int at = c + 8 * ((__ffs(runs) - 1) * THR + t);
+        const int i = atomicAdd(&nruns_s[sub], 1);
+        if (i < RUNS) hist[sub][i] = (uint32_t)(c + 8 * ((__ffs(runs) - 1) * THR + t));
         runs &= runs - 1;
-        float y[8];
-        load(at, y);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (at + j >= c0 && at + j < c1 && value_key(y[j]) >= thr) {
-            const int i = atomicAdd(&count_s[sub], 1);
-            if (i < CAP) list[i] = elem_key(y[j], at + j);
-          }
-        }
       }
     }
   };
@@ -310,38 +314,94 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256, W > 4 ? 4 : 8) void k_logprob
 
   if (TOP) {
     sync();
+    const int nruns = nruns_s[sub], want_all = min(a.k, c1 - c0);
+    if (nruns <= RUNS) {
+      for (int i = t; i < nruns; i += THR) {
+        const int at = (int)hist[sub][i];
+        float y[8];
+        load(at, y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (at + j >= c0 && at + j < c1 && value_key(y[j]) >= thr) {
+            const int n = atomicAdd(&count_s[sub], 1);
+            if (n < CAP) list[n] = elem_key(y[j], at + j);
+          }
+        }
+      }
+      sync();
+    }
     int count = count_s[sub];
-    if (count > CAP) {
+    if (nruns > RUNS || count > CAP || count < want_all) {
       // exact selection: the k-th key digit by digit from the top, then the keys at or above it
+      const int lane = t & 63;
       uint64_t prefix = 0;
-      int want = a.k;
+      uint32_t want = (uint32_t)want_all;
+      sync();
       for (int sh = 56; sh >= 0; sh -= 8) {
+        // digits that all keys of the prefix share: a short row's upper index bits, the lower half of a bf16 value's
+        // key (ones below zero and for NaN)
+        const bool low = sizeof(T) == 2 && (sh == 40 || sh == 32);
+        if (low || (sh == 24 && a.V <= 1 << 24) || (sh == 16 && a.V <= 1 << 16)) {
+          const bool ones = !low || prefix >> 63 == 0 || prefix >> 48 == 0xffff;
+          prefix |= (uint64_t)(ones ? 255 : 0) << sh;
+          continue;
+        }
         for (int i = t; i < 256; i += THR) hist[sub][i] = 0;
         sync();
-        for (int at = c0 + t; at < c1; at += THR) {
-          const uint64_t key = elem_key((float)z[at], at);
-          if (sh == 56 || (key >> (sh + 8)) == (prefix >> (sh + 8))) atomicAdd(&hist[sub][(key >> sh) & 255], 1u);
+        for (int at = cs + 8 * t; at < c1; at += 8 * THR) {
+          float y[8];
+          load(at, y);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint64_t key = elem_key(y[j], at + j);
+            const bool in = at + j >= c0 && at + j < c1 && (sh == 56 || (key >> (sh + 8)) == (prefix >> (sh + 8)));
+            const uint32_t digit = (key >> sh) & 255;
+            // ties are what comes here most: the lanes with the first one's digit are counted together
+            if (in) {
+              const uint32_t first = __builtin_amdgcn_readfirstlane(digit);
+              const uint64_t same = __ballot(digit == first);
+              if (digit != first)
+                atomicAdd(&hist[sub][digit], 1u);
+              else if (lane == __ffsll((unsigned long long)same) - 1)
+                atomicAdd(&hist[sub][first], (uint32_t)__popcll(same));
+            }
+          }
         }
         sync();
-        int d = 255;      // every lane walks the digits: the same walk
-        uint32_t above = 0;
-        for (; d > 0; --d) {
-          const uint32_t n = hist[sub][d];
-          if (above + n >= (uint32_t)want) break;
-          above += n;
+        // the digit: every wave by itself, four digits a lane, the keys above a lane's by a scan
+        uint32_t n[4], suf = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) suf += n[i] = hist[sub][4 * lane + i];
+        const uint32_t own = suf;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const uint32_t v = __shfl_down(suf, o, kWave);
+          suf += lane + o < 64 ? v : 0u;
         }
-        want -= (int)above;
-        prefix |= (uint64_t)d << sh;
+        uint32_t above = suf - own, d = 3, in = n[3];
+        const uint64_t here = __ballot(above < want && suf >= want);
+        for (int i = 2; i >= 0; --i)
+          if (above + in < want) above += in, d = i, in = n[i];
+        const int src = here == 0 ? 0 : __ffsll((unsigned long long)here) - 1;
+        want -= __shfl(above, src, kWave);
+        prefix |= (uint64_t)(4 * src + __shfl(d, src, kWave)) << sh;
         sync();
+        if (__shfl(in, src, kWave) == want) break;   // every key of this prefix is one of the k best
       }
       if (t == 0) count_s[sub] = 0;
       sync();
-      for (int at = c0 + t; at < c1; at += THR) {
-        const uint64_t key = elem_key((float)z[at], at);
-        if (key >= prefix) list[atomicAdd(&count_s[sub], 1)] = key;   // k of them: the keys are all different
+      for (int at = cs + 8 * t; at < c1; at += 8 * THR) {
+        float y[8];
+        load(at, y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint64_t key = elem_key(y[j], at + j);
+          if (at + j >= c0 && at + j < c1 && key >= prefix)
+            list[atomicAdd(&count_s[sub], 1)] = key;   // k of them: the keys are all different
+        }
       }
       sync();
-      count = a.k;
+      count = want_all;
     }
     if (live) {
       if (split) {

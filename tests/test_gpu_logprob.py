@@ -37,10 +37,11 @@ def _rows(rows, V, dtype, seed=0, banned=True):
 
 def _ref(z, t):
     # against the maximum first: beside the lowest float32 value even 64 bits lose ln l
+    # (a row of -inf alone: log probabilities of -inf, entropy 0)
     z = z.double()
     m = z.amax(1, keepdim=True)
-    d = z - m
-    lp = d - torch.log(torch.exp(d).sum(1, keepdim=True))
+    d = z - m.masked_fill(m == -INF, 0)
+    lp = d - torch.log(torch.exp(d).sum(1, keepdim=True).masked_fill(m == -INF, 1))
     lp0 = lp.masked_fill(lp == -INF, 0)
     p = lp.exp()
     H = -(p * lp0).sum(1)
@@ -57,7 +58,8 @@ def _check(z, t, top, dev, grad=True):
     lp, lp0, p, H, logp, ok = _ref(z, t)
     C = _chain(V)
     m = z.double().amax(1)
-    logl = torch.logsumexp(z.double() - m[:, None], 1)
+    m = m.masked_fill(m == -INF, 0)
+    logl = torch.logsumexp(z.double() - m[:, None], 1).clamp(min=0)   # (0: a row of -inf alone)
     S = (p * (z.double() - m[:, None]).abs().masked_fill(z.double() == -INF, 0)).sum(1)
     zt = z.double().gather(1, t.clamp(0, V - 1)[:, None])[:, 0]
     tl = (C + 6) * U
@@ -133,6 +135,23 @@ def test_rows_that_overfill_the_candidate_list(V):
         _check(z, t, top, dev, grad=False)
     _check(z[:7].to(BF), t[:7], 64, dev, grad=False)
     _check(z[:2], t[:2], 64, dev, grad=False)
+
+
+@pytest.mark.parametrize("rows,V,top", [(4, 700, 5), (3, 9000, 24), (33, 32000, 20), (2, 140000, 40), (4200, 4096, 8)])
+def test_masked_vocabularies(rows, V, top):
+    """All but a few tokens masked, with -inf or the type's lowest value: fewer left than alternatives
+    asked for (the masked ones follow by index), as many, and more."""
+    dev = require_gpu()
+    for dtype in (BF, F32):
+        for mask in (-INF, torch.finfo(dtype).min):
+            z, t = _rows(rows, V, dtype, seed=V, banned=False)
+            g = torch.Generator().manual_seed(rows)
+            order = torch.rand(rows, V, generator=g).argsort(1) if rows < 100 else \
+                (torch.arange(V)[None] * 7919 + torch.randint(0, V, (rows, 1), generator=g)) % V
+            left = torch.tensor([0, 1, top - 1, top, top + 1, 100]).repeat(rows // 6 + 1)[:rows]
+            keep = torch.zeros(rows, V, dtype=torch.bool).scatter_(1, order, torch.arange(V)[None] < left[:, None])
+            z = z.masked_fill(~keep, mask)
+            _check(z, t, top, dev, grad=False)
 
 
 def test_many_rows_of_one_wave_that_overfill_the_list():
