@@ -27,14 +27,14 @@
 // eight passes).
 //
 // Measured (MI355X): 32768 x 32000 in bf16 384 us forward and 737 backward, 5.5
-// and 5.7 TB/s, bound by memory; 2047 x 50257 with 5 alternatives 48 us (38 at
-// the rate of a large copy: all rows start and end together, so their bounds,
-// sums and rankings are not hidden); 32 x 32000 with 20 8.5 us, a row's own
+// and 5.7 TB/s, bound by memory; 2047 x 50257 47 us, 50 with 5 or 20
+// alternatives (38 at the rate of a large copy: all rows are resident at once,
+// so that they start and end together); 32 x 32000 with 20 8.5 us, a row's own
 // chain of load, sums, bound and ranking.
 //
 // One wave takes a row of up to 2048 elements (8192 where the rows are many), a
-// workgroup of four or sixteen a longer one; few and very long rows are split over workgroups, whose (m, l, s)
-// and lists a second launch joins.
+// workgroup of four or sixteen a longer one; few and very long rows are split over
+// workgroups, whose (m, l, s) and lists a second launch joins.
 #include <type_traits>
 
 #include "nsa_launch.h"
@@ -525,9 +525,9 @@ __global__ __launch_bounds__(256) void k_logprob_bwd(const LpBwdArgs a) {
 // Waves of a row: one up to 2048 elements, and up to 8192 where the rows give
 // every compute unit sixteen waves by themselves: no barriers, and no idle lanes
 // where a row is little more than a workgroup's chunk (32768 x 2500 in bf16 with
-// one wave 48 us, with four 80; 8192 x 8192 with 5 alternatives 36 and 50,
-// without them 30 and 29; more than 24 alternatives need four waves' maxima;
-// longer rows gain a tenth, at four times the additions in a lane).  Sixteen where the rows leave most of
+// one wave 48 to 53 us, with four 82; 8192 x 8192 with 5 alternatives 33 and 39,
+// without them 30 and 29; more than 24 alternatives overfill one wave's list:
+// 97 us with 40, and 49 with four waves; longer rows gain a tenth, at four times the additions in a lane).  Sixteen where the rows leave most of
 // the chip's waves idle (a row of 32000 in 16 bits is then one chunk); else four.
 // A row of more than 256 KiB is split where there are not enough of them
 // either, into parts of 8192 elements or more, two for every compute unit: one
@@ -564,11 +564,11 @@ static int logprob_launch(LpArgs a, hipStream_t s) {
     else
       k_logprob<T, 1, 4, TOP><<<grid, 256, 0, s>>>(a);
   } else if (w == 4) {
-    // runs in flight against waves: 2047 x 50257 with 5 alternatives takes 58 us at four runs, 54 at three, 56 at
-    // two; 8192 x 32000 without them 105, 109 and 101
-    k_logprob<T, 4, TOP ? 3 : 2, TOP><<<(unsigned)(a.rows * a.nsp), 256, 0, s>>>(a);
+    // runs in flight against waves: 2047 x 50257 with 5 alternatives takes 56 us at four runs, 52 at three, 50 at two
+    k_logprob<T, 4, 2, TOP><<<(unsigned)(a.rows * a.nsp), 256, 0, s>>>(a);
   } else {
-    k_logprob<T, 16, 4, TOP><<<(unsigned)a.rows, 1024, 0, s>>>(a);
+    // 256 x 131072 without alternatives: 13.5 us at two runs, 15.5 at four; 32 x 32000 with 20: 8.8 and 8.5
+    k_logprob<T, 16, TOP ? 4 : 2, TOP><<<(unsigned)a.rows, 1024, 0, s>>>(a);
   }
   if (a.nsp > 1) k_logprob_join<T><<<(unsigned)a.rows, 64, (size_t)a.nsp * a.k * 8, s>>>(a);
   return nsa_launch_status();
