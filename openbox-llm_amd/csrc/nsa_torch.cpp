@@ -214,8 +214,8 @@ double norm_args(const Tensor& x, const OptTensor& res, const Tensor& w, std::op
     check_tensor(*res, what);
     NSA_ASSERT(res->sizes() == x.sizes() && res->device() == x.device(), at + "residual must be like x");
   }
-  const auto ht = res ? res->scalar_type() : x.scalar_type();
-  const double e = eps ? *eps : ht == at::kFloat ? 0x1p-23 : 0x1p-7;
+  // (float32's epsilon for bf16 too: torch.nn.RMSNorm takes that of the type it computes in)
+  const double e = eps ? *eps : 0x1p-23;
   NSA_ASSERT(e >= 0.0, at + "eps must not be negative");
   return e;
 }

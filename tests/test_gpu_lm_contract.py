@@ -1,0 +1,77 @@
+"""What the operators around the attention promise beyond their formulas:
+defaults, what is held and for how long, and where they end.
+"""
+
+import pytest
+import torch
+
+from nsa_testlib import require_gpu
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+CFG = dict(vocab_size=203, d_model=128, n_layers=2, n_q_heads=8, n_kv_heads=2, max_seq_len=96, norm="rms",
+           ffn="swiglu", ffn_hidden=160, tie_embeddings=False, attn_type="full")
+
+
+def _model(seed=0, dtype=F32, **kw):
+    from nsa_model import NSATransformer
+    torch.manual_seed(seed)
+    return NSATransformer(**{**CFG, **kw}).cuda().to(dtype)
+
+
+def _tokens(B, T, seed=0):
+    return torch.randint(0, CFG["vocab_size"], (B, T), generator=torch.Generator().manual_seed(seed)).cuda()
+
+
+# ---------------------------------------------------------------------------
+# norm
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("res", [True, False])
+def test_default_eps_is_rms_norms(dtype, res):
+    """``eps=None`` on rows whose mean square is far below, near and above the
+    candidates for it: torch.nn.RMSNorm's own result, and its formula in 64 bits
+    with 2^-23.
+
+    y: a sum of 200 squares over 25 lanes (8 additions and 6 steps, halved by the
+    root) and 7 roundings besides: 14 u, u = 2^-24; then half a step of its dtype.
+    Two results of dtype within one step of each other, and 8 bits within half
+    a step of e4m3 (2^-4, 2^-10 near zero) and the scale's rounding."""
+    import nsa_lm
+    dev = require_gpu()
+    D, U = 200, 2.0 ** -24
+    size = torch.tensor([2.0 ** -12, 2.0 ** -11, 2.0 ** -6, 0.02, 2.0 ** -3, 1.0])[:, None]
+    x = (torch.randn(6, D, generator=torch.Generator().manual_seed(1)) * size).to(dtype)
+    w = (1 + 0.2 * torch.randn(D, generator=torch.Generator().manual_seed(2))).to(dtype)
+    xd, wd = x.to(dev), w.to(dev)
+    r = torch.zeros_like(xd) if res else None
+    y, _ = nsa_lm.add_rms_norm(xd, r, wd)
+    h = x.double()
+    ref = h / torch.sqrt((h * h).mean(1, keepdim=True) + 2.0 ** -23) * w.double()
+    half = torch.finfo(dtype).eps / 2
+    assert ((y.cpu().double() - ref).abs() <= ref.abs() * (half + 14 * U) * (1 + 1e-6)).all()
+    m = torch.nn.RMSNorm(D).to(dev).to(dtype)
+    with torch.no_grad():
+        m.weight.copy_(wd)
+        t = m(xd)
+    assert ((y.double() - t.double()).abs().cpu() <= 2 * ref.abs() * (half + 14 * U) * (1 + 1e-6)).all()
+    q, s, _ = nsa_lm.add_rms_norm_q8(xd, r, wd)
+    v = q.cpu().double() * s.cpu().double()[:, None]
+    assert ((v - ref).abs() <= torch.maximum(ref.abs() * 2.0 ** -4, s.cpu().double()[:, None] * 2.0 ** -10) +
+            ref.abs() * 40 * U).all()
+
+
+def test_fused_norms_in_bf16_are_the_plain_models():
+    """A bf16 model at its initialisation, where the embedding's rows have a mean
+    square of 4e-4: the fused norms' logits against the plain ones'.  Every
+    product's output carries 2^-8 of its size, eight of them in a row over the two
+    layers; an eps of bf16's step moves these logits by most of their size."""
+    require_gpu()
+    ref = _model(dtype=BF, pos="rope").eval()
+    new = _model(dtype=BF, pos="rope", norm_impl="fused").eval()
+    new.load_state_dict(ref.state_dict())
+    x = _tokens(2, 60)
+    with torch.no_grad():
+        a, b = ref(x)[0].double(), new(x)[0].double()
+    assert float((a - b).abs().max()) <= 8 * 2.0 ** -8 * float(a.abs().max())
