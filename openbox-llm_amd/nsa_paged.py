@@ -23,6 +23,8 @@ whatever they hold.  A negative length stands for no sequence: its output is zer
 For inference: inputs that need a gradient are refused.
 """
 
+import weakref
+
 import torch
 
 import _nsa_lib as L
@@ -86,13 +88,14 @@ def paged_append(k, v, k_pages, v_pages, table, lens, count=None):
 
 
 class _PageAccount:
-    """The table of a set of caches, and the host's account of who holds which page."""
+    """The table of a set of caches, and the host's account of who holds which page.
+    The caches themselves are held weakly: a dropped cache frees its pages at once."""
 
     def __init__(self, batch, max_pages, n_pages, device):
         self.table = torch.full((batch, max_pages), -1, device=device, dtype=torch.int32)
         self.free = list(range(n_pages - 1, -1, -1))
         self.held = [[] for _ in range(batch)]
-        self.caches = []
+        self.caches = weakref.WeakSet()
 
 
 class PagedKVCache:
@@ -121,8 +124,8 @@ class PagedKVCache:
         self.v_pages = torch.zeros(shape, device=device, dtype=dtype)
         self.lens = torch.zeros(batch, device=device, dtype=torch.int32)
         self._account = _PageAccount(batch, self.max_pages, n_pages, device) if like is None else like._account
-        self._account.caches.append(self)
         L.torch_side().check_pages(self.k_pages, self.v_pages, self.table, self.lens)
+        self._account.caches.add(self)
 
     @property
     def table(self):
