@@ -11,15 +11,18 @@
 // tensors' device; nothing waits for the host.
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros_like.h>
+#include <c10/core/AutogradState.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <initializer_list>
 #include <optional>
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "nsa_hip.h"
 
@@ -84,6 +87,16 @@ void check_tensor(const Tensor& t, const char* what) {
   NSA_ASSERT(t.is_cuda(), std::string(what) + ": a GPU tensor is needed");
   NSA_ASSERT(is_float(t), std::string(what) + ": dtype " + c10::toString(t.scalar_type()) +
                               " is not supported (float32 or bfloat16)");
+}
+// Forward-mode derivatives: none of these operators has one, and the raw path
+// would drop a dual tensor's tangent (it does not need requires_grad, and
+// no_grad does not turn it off).
+bool has_tangent(const Tensor& t) {
+  return t.defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined();
+}
+bool has_tangent(const OptTensor& t) { return t && has_tangent(*t); }
+void no_tangent(bool found, const char* what) {
+  NSA_ASSERT(!found, std::string(what) + " has no forward-mode derivative");
 }
 int code_of(at::ScalarType t) {
   return t == at::kFloat ? NSA_F32 : t == at::kBFloat16 ? NSA_BF16 : NSA_E4M3;
@@ -169,6 +182,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
     const bool added = ctx->saved_data["added"].toBool();
     const bool need_w = ctx->needs_input_grad(added ? 2 : 1);
     Tensor dy = grads[0], dh = added ? grads[1] : Tensor(), dx, dr, dw;
+    TORCH_CHECK(!has_tangent(dy) && !has_tangent(dh), "nsa_norm_bwd has no forward-mode derivative");
     if (!dy.defined()) {   // only the sum was used: its gradient passes through
       if (dh.defined()) {
         dx = dh.to(xt);
@@ -205,6 +219,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
 
 double norm_args(const Tensor& x, const OptTensor& res, const Tensor& w, std::optional<double> eps, const char* what) {
   const std::string at = std::string(what) + ": ";
+  no_tangent(has_tangent(x) || has_tangent(res) || has_tangent(w), what);
   check_tensor(x, what);
   check_tensor(w, what);
   NSA_ASSERT(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= (1 << 24), at + "x must be [..., D]");
@@ -291,6 +306,7 @@ struct LogprobFn : torch::autograd::Function<LogprobFn> {
     const Tensor &z = saved[0], &targets = saved[1], &stat = saved[2], &ent = saved[3];
     const bool t = ctx->saved_data["targets"].toBool();
     Tensor dlogp = t ? grads[0] : Tensor(), dent = grads[t ? 1 : 0];
+    TORCH_CHECK(!has_tangent(dlogp) && !has_tangent(dent), "nsa_logprob_bwd has no forward-mode derivative");
     if (!dlogp.defined() && !dent.defined()) return {Tensor(), Tensor(), Tensor()};
     if (dlogp.defined()) dlogp = dlogp.contiguous();
     if (dent.defined()) dent = dent.contiguous();
@@ -306,6 +322,7 @@ struct LogprobFn : torch::autograd::Function<LogprobFn> {
 
 std::tuple<OptTensor, Tensor, OptTensor, OptTensor> token_logprobs(const Tensor& logits, const OptTensor& targets_,
                                                                    int64_t top) {
+  no_tangent(has_tangent(logits), "token_logprobs");
   check_tensor(logits, "token_logprobs: logits");
   NSA_ASSERT(logits.dim() >= 1 && logits.size(-1) >= 1 && logits.size(-1) <= (1 << 28),
              "token_logprobs: logits must be [..., V]");
@@ -370,6 +387,8 @@ void check_pages(const Tensor& kp, const Tensor& vp, const Tensor& table, const 
 std::tuple<Tensor, OptTensor, OptTensor> paged(const Tensor& q_, const OptTensor& k_new, const OptTensor& v_new,
                                                const Tensor& kp, const Tensor& vp, const Tensor& table_,
                                                const Tensor& lens_, std::optional<double> scale, bool want_lse) {
+  no_tangent(has_tangent(q_) || has_tangent(k_new) || has_tangent(v_new) || has_tangent(kp) || has_tangent(vp),
+             "paged attention");
   check_pages(kp, vp, table_, lens_);
   const int64_t n = kp.size(0), Hkv = kp.size(1), P = kp.size(2), D = kp.size(3), B = table_.size(0);
   const int64_t mp = table_.size(1);
@@ -420,5 +439,8 @@ PYBIND11_MODULE(_nsa_torch, m) {
   m.def("add_rms_norm_q8", &add_rms_norm_q8);
   m.def("token_logprobs", &token_logprobs);
   m.def("check_pages", &check_pages);
+  m.def("no_tangent", [](const std::vector<Tensor>& ts, const std::string& what) {
+    for (const Tensor& t : ts) no_tangent(has_tangent(t), what.c_str());
+  });
   m.def("paged", &paged);
 }

@@ -16,8 +16,9 @@ Violations raise ``AssertionError``; a missing library raises ``RuntimeError``.
 Every call launches on the current stream of its tensors' device, allocates
 its outputs and workspace with torch, and never waits for the host: calls can
 be captured into a graph (a backward, as any torch function's, with no eager
-graph of the same leaves alive).  First derivatives only; the checks, allocations and
-autograd nodes are C++ (csrc/nsa_torch.cpp).
+graph of the same leaves alive).  First derivatives only, in reverse mode: dual
+tensors are refused.  The checks, allocations and autograd nodes are C++
+(csrc/nsa_torch.cpp).
 """
 
 from typing import NamedTuple, Optional

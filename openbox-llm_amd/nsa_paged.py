@@ -20,7 +20,7 @@ Table entries outside ``0 .. n_pages-1`` are no pages: keys there are not
 attended and rows are not written.  Rows past a length have no influence,
 whatever they hold.  A negative length stands for no sequence: its output is zeros, its length stays.
 
-For inference: inputs that need a gradient are refused.
+For inference: inputs that need a gradient, or carry a forward-mode one, are refused.
 """
 
 import weakref
@@ -63,7 +63,9 @@ def paged_append(k, v, k_pages, v_pages, table, lens, count=None):
     """Write rows ``k, v [B, Hkv, T, D]`` (the first ``count[b]`` of them: int32
     ``[B]``, default T) to positions ``lens[b] ..`` -> the new lengths.  A
     sequence whose rows do not all have a page keeps its pages and length."""
-    L.torch_side().check_pages(k_pages, v_pages, table, lens)
+    side = L.torch_side()
+    side.no_tangent([k, v, k_pages, v_pages], "paged_append")
+    side.check_pages(k_pages, v_pages, table, lens)
     n, Hkv, P, D = k_pages.shape
     B, mp = table.shape
     assert k.dim() == 4 and k.shape[:2] == (B, Hkv) and k.shape[3] == D and v.shape == k.shape, \

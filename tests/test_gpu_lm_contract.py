@@ -75,3 +75,28 @@ def test_fused_norms_in_bf16_are_the_plain_models():
     with torch.no_grad():
         a, b = ref(x)[0].double(), new(x)[0].double()
     assert float((a - b).abs().max()) <= 8 * 2.0 ** -8 * float(a.abs().max())
+
+
+# ---------------------------------------------------------------------------
+# forward-mode derivatives
+# ---------------------------------------------------------------------------
+
+def test_tangents_of_inputs_and_incoming_gradients_are_refused():
+    import torch.autograd.forward_ad as fa
+    import nsa_lm
+    dev = require_gpu()
+    x, w = torch.randn(3, 16, device=dev), torch.ones(16, device=dev, requires_grad=True)
+    z = torch.randn(3, 16, device=dev, requires_grad=True)
+    with fa.dual_level():
+        for t in (x, x.clone().requires_grad_()):
+            d = fa.make_dual(t, torch.ones_like(t))
+            for call in (lambda: nsa_lm.add_rms_norm(d, None, w), lambda: nsa_lm.token_logprobs(d)):
+                with pytest.raises(AssertionError, match="forward-mode"):
+                    call()
+        y, _ = nsa_lm.add_rms_norm(x, None, w)
+        ent = nsa_lm.token_logprobs(z).entropy
+        for out, at in ((y, w), (ent, z)):
+            g = torch.ones_like(out)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(out, at, fa.make_dual(g, g), retain_graph=True)
+            torch.autograd.grad(out, at, g)

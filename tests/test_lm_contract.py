@@ -52,3 +52,41 @@ def test_a_refused_cache_leaves_nothing_in_the_account(monkeypatch):
     with pytest.raises(AssertionError):
         _cache(like=a, head_dim=48)
     assert list(a._account.caches) == [a]
+
+
+def test_dual_tensors_are_refused():
+    """A tangent would be dropped: refused before anything else is looked at, with
+    gradients on and off, wherever it sits."""
+    import os
+    import torch.autograd.forward_ad as fa
+    import _nsa_lib
+    if not os.path.exists(_nsa_lib.LIB_PATH):
+        pytest.skip("libnsa_hip.so not built")
+    import nsa_lm
+    import nsa_paged
+    x, w = torch.zeros(3, 16), torch.ones(16)
+    q, row, pages = torch.zeros(1, 1, 16), torch.zeros(1, 1, 16), torch.zeros(2, 1, 16, 16)
+    table, lens = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+
+    def calls(d):
+        yield lambda: nsa_lm.add_rms_norm(d(x), x, w)
+        yield lambda: nsa_lm.add_rms_norm(x, d(x), w)
+        yield lambda: nsa_lm.add_rms_norm(x, None, d(w))
+        yield lambda: nsa_lm.add_rms_norm_q8(x, d(x), w)
+        yield lambda: nsa_lm.token_logprobs(d(x))
+        yield lambda: nsa_paged.paged_attend(d(q), pages, pages, table, lens)
+        yield lambda: nsa_paged.paged_attend(q, pages, d(pages), table, lens)
+        yield lambda: nsa_paged.paged_step(q, d(row), row, pages, pages, table, lens)
+        yield lambda: nsa_paged.paged_step(q, row, d(row), pages, pages, table, lens)
+        yield lambda: nsa_paged.paged_append(d(row)[:, :, None], row[:, :, None], pages, pages, table, lens)
+        yield lambda: nsa_paged.paged_append(row[:, :, None], row[:, :, None], pages, d(pages), table, lens)
+    with fa.dual_level():
+        for call in calls(lambda t: fa.make_dual(t, torch.ones_like(t))):
+            with pytest.raises(AssertionError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(AssertionError, match="forward-mode"):
+                call()
+        for call in calls(lambda t: t):      # (no tangent: refused as CPU tensors)
+            with pytest.raises(AssertionError) as e:
+                call()
+            assert "forward-mode" not in str(e.value)
