@@ -793,11 +793,16 @@ class NSATransformer(nn.Module):
         return self.ln_f(x)
 
     def _loss(self, logits, targets):
-        """The mean negative log probability of the targets; -100 is left out."""
+        """The mean negative log probability of the targets; -100 is left out.
+        Any other target outside the vocabulary stops the process on the GPU in
+        ``F.cross_entropy``; fused, it makes the loss and every gradient NaN,
+        without a wait for the host."""
         if self.loss_impl == "fused":
             import nsa_lm
             logp = nsa_lm.token_logprobs(logits, targets).logp
-            return -logp.sum() / (targets != -100).sum()
+            kept = targets != -100
+            wrong = (kept & ((targets < 0) | (targets >= logits.shape[-1]))).any()
+            return -logp.sum() / kept.sum().float().masked_fill(wrong, float("nan"))
         return F.cross_entropy(logits.view(-1, logits.size(-1)), targets.view(-1))
 
     @torch.no_grad()

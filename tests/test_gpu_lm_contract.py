@@ -100,3 +100,27 @@ def test_tangents_of_inputs_and_incoming_gradients_are_refused():
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(out, at, fa.make_dual(g, g), retain_graph=True)
             torch.autograd.grad(out, at, g)
+
+
+# ---------------------------------------------------------------------------
+# the fused loss
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("bad", [-1, -99, -101, CFG["vocab_size"], 1 << 40], ids=str)
+def test_a_target_outside_the_vocabulary_makes_the_loss_nan(bad):
+    """Not a smaller mean: the loss and every gradient it has."""
+    require_gpu()
+    m = _model(pos="rope", loss_impl="fused")
+    x, y = _tokens(2, 20), _tokens(2, 20, 1)
+    y[0, 3] = -100
+    logits, loss = m(x, y)
+    want = torch.nn.functional.cross_entropy(logits.double().view(-1, CFG["vocab_size"]), y.view(-1))
+    # 39 terms below 16 in at most 39 + 8 float32 additions, each term within 32 u of its size
+    assert abs(float(loss.detach()) - float(want)) <= (39 + 8 + 32) * 2.0 ** -24 * 16
+    y[1, 7] = bad
+    loss = m(x, y)[1]
+    assert loss.isnan() and loss.dtype == F32
+    loss.backward()
+    assert m.lm_head.weight.grad.isnan().any(1).all() and m.tok_emb.weight.grad.isnan().any()
+    y[:] = -100
+    assert m(x, y)[1].isnan()       # no target at all: cross_entropy's 0 / 0
