@@ -238,21 +238,28 @@ class Rotary(nn.Module):
     def tables(self, T, device, dtype):
         """The factors ``forward`` multiplies by, ``cos, sin [T, dim/2]`` with
         the values of ``dtype``, held as float32 (the fused head split's
-        tables); cached per length, device, dtype and frequency buffer, but for
-        those that a graph's capture only records."""
-        inv = self.inv_freq
-        key = (T, str(device), dtype, inv.dtype, inv.data_ptr(), inv._version)
-        hit = self._tables.get(key)
-        if hit is None:
-            with torch.no_grad(), torch.autocast(device_type=torch.device(device).type, enabled=False):
-                ang = torch.arange(T, device=device, dtype=torch.float32)[:, None] * inv.to(device)[None, :]
-                hit = (ang.cos().to(dtype).float().contiguous(), ang.sin().to(dtype).float().contiguous())
-            if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+        tables).  Cached per length, dtype, frequency buffer, device and stream:
+        another stream would read them before they are written, or after their
+        memory is another's.  A graph's capture always forms its own, in the
+        graph: the cache is emptied when it is full, and a replay would read
+        what lies there then."""
+        inv, device = self.inv_freq, torch.device(device)
+        key = None
+        if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():
+            stream = torch.cuda.current_stream(device) if device.type == "cuda" else None
+            at = None if stream is None else (stream.device_index, stream.cuda_stream)
+            key = (T, str(device), at, dtype, inv.dtype, inv.data_ptr(), inv._version)
+            hit = self._tables.get(key)
+            if hit is not None:
                 return hit
+        with torch.no_grad(), torch.autocast(device_type=device.type, enabled=False):
+            ang = torch.arange(T, device=device, dtype=torch.float32)[:, None] * inv.to(device)[None, :]
+            made = (ang.cos().to(dtype).float().contiguous(), ang.sin().to(dtype).float().contiguous())
+        if key is not None:
             if len(self._tables) > 8:
                 self._tables.clear()
-            self._tables[key] = hit
-        return hit
+            self._tables[key] = made
+        return made
 
     def at(self, pos, dtype):
         """The same factors for one token a sequence at ``pos [B]``: ``[B, 1, dim/2]``."""

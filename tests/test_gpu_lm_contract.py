@@ -124,3 +124,65 @@ def test_a_target_outside_the_vocabulary_makes_the_loss_nan(bad):
     assert m.lm_head.weight.grad.isnan().any(1).all() and m.tok_emb.weight.grad.isnan().any()
     y[:] = -100
     assert m(x, y)[1].isnan()       # no target at all: cross_entropy's 0 / 0
+
+
+# ---------------------------------------------------------------------------
+# rotation tables
+# ---------------------------------------------------------------------------
+
+def test_rotation_tables_are_a_streams_own():
+    from nsa_model import Rotary
+    dev = require_gpu()
+    rope = Rotary(32).to(dev)
+    cos, sin = rope.tables(50, dev, BF)
+    assert rope.tables(50, dev, BF)[0] is cos
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        other = rope.tables(50, dev, BF)
+        assert other[0].data_ptr() != cos.data_ptr() and rope.tables(50, dev, BF)[0] is other[0]
+    torch.cuda.synchronize()
+    assert torch.equal(other[0], cos) and torch.equal(other[1], sin)
+    assert rope.tables(50, dev, BF)[0] is cos
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):      # made in the graph, and not kept
+        inside = rope.tables(50, dev, BF)
+    assert inside[0].data_ptr() not in (cos.data_ptr(), other[0].data_ptr())
+    with torch.cuda.stream(side):
+        assert rope.tables(50, dev, BF)[0] is other[0]
+    for _ in range(3):
+        inside[0].zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(inside[0], cos) and torch.equal(inside[1], sin)
+
+
+def test_captured_forward_outlives_the_rotation_tables():
+    """A forward of the library arm captured behind a warm-up of the same length,
+    replayed after ten other lengths have passed and their memory is written over."""
+    require_gpu()
+    m = _model(dtype=BF, pos="rope", dense_impl="sdpa").eval()
+    x = _tokens(2, 48)
+    with torch.no_grad():
+        want = m(x)[0]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            m(x)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = m(x)[0]
+        for T in range(50, 60):
+            for stream in (torch.cuda.current_stream(), side):
+                with torch.cuda.stream(stream):
+                    m(_tokens(2, T))
+        torch.cuda.synchronize()
+        junk = [torch.full((48, 8), 7.0, device="cuda") for _ in range(300)]
+        for seed in range(3):
+            x.copy_(_tokens(2, 48, seed))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, m(x)[0]), seed
+            if seed == 0:
+                assert torch.equal(out, want)
+        del junk
