@@ -248,11 +248,13 @@ class Rotary(nn.Module):
         if device.type != "cuda" or not torch.cuda.is_current_stream_capturing():
             stream = torch.cuda.current_stream(device) if device.type == "cuda" else None
             at = None if stream is None else (stream.device_index, stream.cuda_stream)
-            key = (T, str(device), at, dtype, inv.dtype, inv.data_ptr(), inv._version)
+            version = None if inv.is_inference() else inv._version
+            key = (T, str(device), at, dtype, inv.dtype, inv.data_ptr(), version)
             hit = self._tables.get(key)
             if hit is not None:
                 return hit
-        with torch.no_grad(), torch.autocast(device_type=device.type, enabled=False):
+        # (ordinary tensors under inference_mode too: a later training step saves them)
+        with torch.inference_mode(False), torch.no_grad(), torch.autocast(device_type=device.type, enabled=False):
             ang = torch.arange(T, device=device, dtype=torch.float32)[:, None] * inv.to(device)[None, :]
             made = (ang.cos().to(dtype).float().contiguous(), ang.sin().to(dtype).float().contiguous())
         if key is not None:

@@ -186,3 +186,14 @@ def test_captured_forward_outlives_the_rotation_tables():
             if seed == 0:
                 assert torch.equal(out, want)
         del junk
+
+
+def test_training_behind_inference_of_the_same_length():
+    require_gpu()
+    m = _model(dtype=BF, pos="rope", dense_impl="sdpa")
+    x = _tokens(2, 32)
+    with torch.inference_mode():
+        want = m(x)[0].clone()
+    logits, loss = m(x, x)
+    loss.backward()
+    assert torch.equal(logits, want) and m.blocks[0].attn.q_proj.weight.grad.abs().sum() > 0

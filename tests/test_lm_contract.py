@@ -90,3 +90,18 @@ def test_dual_tensors_are_refused():
             with pytest.raises(AssertionError) as e:
                 call()
             assert "forward-mode" not in str(e.value)
+
+
+def test_rotation_tables_of_inference_serve_training():
+    """Tables formed under inference_mode are saved for a later backward."""
+    from nsa_model import Rotary
+    rope = Rotary(16)
+    with torch.inference_mode():
+        cos, _ = rope.tables(5, "cpu", torch.float32)
+    assert rope.tables(5, "cpu", torch.float32)[0] is cos and not cos.is_inference()
+    x = torch.ones(5, 8, requires_grad=True)
+    (x * cos).sum().backward()
+    assert torch.equal(x.grad, cos)
+    with torch.inference_mode():
+        late = Rotary(16)
+        assert torch.equal(late.tables(5, "cpu", torch.float32)[0], cos)
