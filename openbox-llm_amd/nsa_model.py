@@ -843,6 +843,7 @@ class NSATransformer(nn.Module):
         x = self.tok_emb(idx)
         if hasattr(self, "pos_emb"):
             x = x + self.pos_emb(torch.arange(T, device=idx.device))[None]
+        lens = caches[0].counts(lens)
         branch = None
         for blk, cache in zip(self.blocks, caches):
             if self.norm_impl == "fused":

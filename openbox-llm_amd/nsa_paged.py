@@ -13,7 +13,7 @@ every sequence of a batch.
 Layout: ``k_pages, v_pages [n_pages, Hkv, page, D]`` (float32 or bfloat16,
 ``page`` a multiple of 16, ``D`` in 16, 32, 64, 128), ``table [B, max_pages]``
 int32 (the page that holds positions ``i page ..``) and ``lens [B]`` int32, all
-on the device: a generation loop never waits for the host, and a step can be
+on the device: the host never waits for it in a generation loop, and a step can be
 captured into a graph.  Query head h reads KV head ``h // (Hq // Hkv)``.
 
 Table entries outside ``0 .. n_pages-1`` are no pages: keys there are not
@@ -89,6 +89,18 @@ def paged_append(k, v, k_pages, v_pages, table, lens, count=None):
     return lens_out
 
 
+def _staged(numbers, dtype, device):
+    """Host numbers as a tensor on ``device``, with no wait for the device: the copy is
+    made from pinned memory, which torch keeps until it is done."""
+    host, device = torch.as_tensor(numbers, dtype=dtype), torch.device(device)
+    if device.type != "cuda":
+        return host.to(device)
+    assert not torch.cuda.is_current_stream_capturing(), \
+        "paged: a capture would read the host's numbers on every replay: reserve, or hand over lengths, before it"
+    # (memory of its own: a caller's pinned tensor may be changed while the copy waits its turn)
+    return torch.empty(host.shape, dtype=dtype, pin_memory=True).copy_(host).to(device, non_blocking=True)
+
+
 class _PageAccount:
     """The table of a set of caches, and the host's account of who holds which page.
     The caches themselves are held weakly: a dropped cache frees its pages at once."""
@@ -107,7 +119,7 @@ class PagedKVCache:
     ``n_pages`` pages in all (default: enough for every sequence at
     ``max_len``).  Sequences take pages with ``reserve`` and give them back with
     ``release``, on the host's own account of the table (neither reads the
-    device).  ``step`` needs the new position reserved.  ``like``, another
+    device or waits for it).  ``step`` needs the new position reserved.  ``like``, another
     layer's cache of the same sizes: both lie under one table, and reserving or
     releasing on either serves both; each has its own pages and lengths."""
 
@@ -148,7 +160,9 @@ class PagedKVCache:
     def reserve(self, lengths):
         """Pages for ``lengths`` tokens (an int for all sequences, or one per
         sequence); what a sequence holds already stays.  Raises RuntimeError,
-        and takes nothing, where the pages do not suffice."""
+        and takes nothing, where the pages do not suffice.  The table is
+        written on the current stream, with no wait for the device; inside a
+        capture new pages are refused."""
         acc = self._account
         lengths = [lengths] * self.batch if isinstance(lengths, int) else [int(n) for n in lengths]
         assert len(lengths) == self.batch, "paged: one length for each sequence"
@@ -157,16 +171,16 @@ class PagedKVCache:
         more = [max(0, n - len(h)) for n, h in zip(need, acc.held)]
         if sum(more) > len(acc.free):
             raise RuntimeError(f"paged: {sum(more)} pages needed, {len(acc.free)} free")
-        rows, cols, pages = [], [], []
-        for b, m in enumerate(more):
-            for _ in range(m):
-                rows.append(b)
-                cols.append(len(acc.held[b]))
-                pages.append(acc.free.pop())
-                acc.held[b].append(pages[-1])
-        if rows:
-            at = torch.tensor([rows, cols, pages], dtype=torch.int64).to(self.table.device)
-            self.table[at[0], at[1]] = at[2].to(torch.int32)
+        rows = [b for b, m in enumerate(more) for _ in range(m)]
+        if not rows:
+            return
+        cols = [len(h) + i for h, m in zip(acc.held, more) for i in range(m)]
+        pages = acc.free[:-len(rows) - 1:-1]
+        at = _staged([rows, cols, pages], torch.int64, self.table.device)
+        self.table[at[0], at[1]] = at[2].to(torch.int32)
+        del acc.free[-len(rows):]
+        for b, page in zip(rows, pages):
+            acc.held[b].append(page)
 
     def release(self, seq):
         """Give back sequence ``seq``'s pages; its length becomes 0."""
@@ -182,11 +196,14 @@ class PagedKVCache:
         """Append a prompt's rows ``[B, Hkv, T, D]``, ``lens`` of them a sequence
         (int32 ``[B]`` on the device, or host ints; default T); the pages must
         be reserved."""
-        if lens is not None and not torch.is_tensor(lens):
-            lens = torch.as_tensor(lens, dtype=torch.int32).expand(self.batch)
-        if lens is not None:
-            lens = lens.to(device=self.lens.device, dtype=torch.int32)
-        self.lens.copy_(paged_append(k, v, self.k_pages, self.v_pages, self.table, self.lens, lens))
+        self.lens.copy_(paged_append(k, v, self.k_pages, self.v_pages, self.table, self.lens, self.counts(lens)))
+
+    def counts(self, lens):
+        """``prefill``'s ``lens`` as it is handed to the kernel (int32 on the device, or
+        None): converted once for the caches of many layers."""
+        if torch.is_tensor(lens) and lens.device == self.lens.device:
+            return lens.to(torch.int32)
+        return None if lens is None else _staged(lens, torch.int32, self.lens.device).expand(self.batch)
 
     def step(self, q, k_new, v_new, scale=None):
         """``paged_step`` on this cache -> ``out [B, Hq, D]``.  The lengths are

@@ -197,3 +197,79 @@ def test_training_behind_inference_of_the_same_length():
     logits, loss = m(x, x)
     loss.backward()
     assert torch.equal(logits, want) and m.blocks[0].attn.q_proj.weight.grad.abs().sum() > 0
+
+
+# ---------------------------------------------------------------------------
+# paged caches
+# ---------------------------------------------------------------------------
+
+def test_a_generation_loop_never_waits_for_the_device():
+    """Reserving, prefilling with the host's lengths, stepping and releasing all
+    return while the device is still busy with what was asked for before them,
+    and what they wrote is right although their numbers were staged meanwhile."""
+    require_gpu()
+    m = _model(pos="rope").eval()
+    x = _tokens(2, 40)
+    with torch.no_grad():
+        want = m(x)[0]
+    big = torch.randn(8192, 8192, device="cuda", dtype=BF)
+
+    def loop(busy):
+        caches = m.paged_caches(2, 96, page_size=16)
+        lens = [20, 7]
+        if busy:
+            for _ in range(100):            # about 0.1 s of work ahead of the loop
+                big @ big
+        ahead = torch.cuda.Event()
+        ahead.record()
+        caches[0].reserve(lens)
+        mine = torch.tensor(lens, dtype=torch.int32).pin_memory()
+        pre = m.prefill(x[:, :20], caches, mine)
+        mine.zero_()                        # (a pinned tensor of the caller's, changed before the device reads it)
+        outs = []
+        for s in range(12):
+            caches[0].reserve([n + s + 1 for n in lens])
+            at = torch.stack([x[0, 20 + s], x[1, 7 + s]])
+            outs.append(m.step(at, caches))
+        caches[1].release(1)
+        running = not ahead.query()
+        return caches, pre, outs, running
+    loop(False)                             # (pinned memory and workspaces are there)
+    torch.cuda.synchronize()
+    caches, pre, outs, running = loop(True)
+    assert running
+    for b, n in enumerate([20, 7]):
+        assert (pre[b, :n] - want[b, :n]).abs().max() <= 1e-4 * want.abs().max()
+        for s, o in enumerate(outs):
+            assert (o[b] - want[b, n + s]).abs().max() <= 1e-4 * want.abs().max(), (b, s)
+    assert caches[0].lens.tolist() == [32, 0] and (caches[0].table >= 0).sum(1).tolist() == [2, 0]
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        loop(False)
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+
+
+def test_host_numbers_inside_a_capture_are_refused():
+    """A graph would read the staging memory again on every replay."""
+    import nsa_paged
+    dev = require_gpu()
+    c = nsa_paged.PagedKVCache(2, 1, 16, 64, 16, dtype=F32)
+    k = torch.randn(2, 1, 20, 16, device=dev)
+    on_device = torch.tensor([20, 3], device=dev)
+    c.reserve(32)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.reserve(20)                       # nothing new: allowed
+        with pytest.raises(AssertionError, match="capture"):
+            c.reserve(40)
+        with pytest.raises(AssertionError, match="capture"):
+            c.prefill(k, k, [20, 3])
+        c.prefill(k, k, on_device)
+    assert c.free_pages == 4 and c.lens.tolist() == [0, 0]
+    for _ in range(3):
+        c.lens.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert c.lens.tolist() == [20, 3]

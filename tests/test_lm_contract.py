@@ -105,3 +105,27 @@ def test_rotation_tables_of_inference_serve_training():
     with torch.inference_mode():
         late = Rotary(16)
         assert torch.equal(late.tables(5, "cpu", torch.float32)[0], cos)
+
+
+def test_reserving_takes_nothing_where_it_raises(monkeypatch):
+    """The account and the table in step, whatever is refused in between."""
+    import nsa_paged
+    _stub(monkeypatch)
+    c = _cache(n_pages=5)
+    c.reserve([17, 0])
+    staged = nsa_paged._staged
+    monkeypatch.setattr(nsa_paged, "_staged", lambda *a: (_ for _ in ()).throw(AssertionError("capture")))
+    with pytest.raises(AssertionError):
+        c.reserve([17, 40])
+    c.reserve([32, 0])                      # (two pages held already: nothing new, nothing staged)
+    monkeypatch.setattr(nsa_paged, "_staged", staged)
+    assert c.free_pages == 3 and (c.table >= 0).sum(1).tolist() == [2, 0]
+    with pytest.raises(RuntimeError):
+        c.reserve([40, 40])
+    c.reserve([40, 20])
+    assert c.free_pages == 0 and sorted(c.table[c.table >= 0].tolist()) == list(range(5))
+    c.release(0)
+    c.reserve([0, 40])
+    held = [t[t >= 0].tolist() for t in c.table]
+    assert c.free_pages == 2 and [len(h) for h in held] == [0, 3] and held == c._account.held
+    assert c.counts(None) is None and c.counts(3).tolist() == [3, 3] and c.counts([4, 5]).dtype == torch.int32
