@@ -586,12 +586,23 @@ int nsa_paged_attend(const void* q, const void* k_new, const void* v_new, void* 
                      const int32_t* table, const int32_t* lens, int32_t* lens_out, void* out, float* lse,
                      void* workspace, size_t workspace_bytes, int B, int Hq, int Hkv, int D, int P, int max_pages,
                      int n_pages, float scale, int dtype, void* stream);
+/* The same with an end to the sequences: a position at or past max_len (>= 0) has
+ * takes no row, whatever the table holds there (keys that lie there already are
+ * attended).  For a max_len that is not a whole number of pages. */
+int nsa_paged_attend_max(const void* q, const void* k_new, const void* v_new, void* k_pages, void* v_pages,
+                         const int32_t* table, const int32_t* lens, int32_t* lens_out, void* out, float* lse,
+                         void* workspace, size_t workspace_bytes, int B, int Hq, int Hkv, int D, int P, int max_pages,
+                         int n_pages, int max_len, float scale, int dtype, void* stream);
 /* Rows [B][Hkv][T][D] of a prompt (count[b] of them, null: T) to positions
  * lens[b] ..; lens_out[b] = lens[b] + count[b].  A sequence whose rows do not all
  * have a page keeps its length and pages. */
 int nsa_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* table,
                      const int32_t* lens, const int32_t* count, int32_t* lens_out, int B, int Hkv, int T, int D, int P,
                      int max_pages, int n_pages, int dtype, void* stream);
+/* The same up to position max_len (>= 0), as nsa_paged_attend_max. */
+int nsa_paged_append_max(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* table,
+                         const int32_t* lens, const int32_t* count, int32_t* lens_out, int B, int Hkv, int T, int D,
+                         int P, int max_pages, int n_pages, int max_len, int dtype, void* stream);
 
 
 #ifdef __cplusplus

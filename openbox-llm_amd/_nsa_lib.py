@@ -111,12 +111,14 @@ SIGNATURES = {
     "nsa_logprob_bwd": (_I, [_P] * 7 + [_L, _I, _I, _P]),
     "nsa_paged_workspace": (_Z, [_I] * 7 + [_P]),
     "nsa_paged_attend": (_I, [_P] * 11 + [_Z] + [_I] * 7 + [_F, _I, _P]),
+    "nsa_paged_attend_max": (_I, [_P] * 11 + [_Z] + [_I] * 8 + [_F, _I, _P]),
     "nsa_paged_append": (_I, [_P] * 8 + [_I] * 8 + [_P]),
+    "nsa_paged_append_max": (_I, [_P] * 8 + [_I] * 9 + [_P]),
 }
 
 # entry points that csrc/nsa_torch.cpp calls
 _TORCH_SIDE = ("nsa_norm_fwd", "nsa_norm_bwd", "nsa_norm_bwd_workspace", "nsa_logprob_fwd", "nsa_logprob_bwd",
-               "nsa_logprob_workspace", "nsa_paged_attend", "nsa_paged_workspace")
+               "nsa_logprob_workspace", "nsa_paged_attend_max", "nsa_paged_workspace")
 
 _lib = None
 

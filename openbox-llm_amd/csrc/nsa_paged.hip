@@ -58,15 +58,17 @@ struct PagedArgs {
   int2* row_info;                    // [R] first and last share of a row in pieces, (-1, -1) of one piece
   int B, Hq, Hkv, G, HT, P, rpp;     // HT: head tiles of a KV head; rpp: runs of 16 in a page
   int max_pages, n_pages, W;         // W: shares of the list, or 0: a workgroup a row
+  int limit;                         // no row is appended at or past it (at most max_pages * P)
   float sl2;                         // scale * log2 e
 };
 
 // Keys that sequence b attends, twice, plus 1 where the last of them is the row it would append.  (Where
-// that row has no page, its run has none either: it is neither attended nor written.)
+// that row has no page, its run has none either: it is neither attended nor written.  Past the limit there is
+// no such row, page or not.)
 __device__ __forceinline__ uint32_t paged_keys(const PagedArgs& a, int b) {
   const int cap = a.max_pages * a.P;
   const int len = a.lens[b];
-  if (a.k_new != nullptr && len >= 0 && len < cap) return 2u * ((uint32_t)len + 1u) + 1u;
+  if (a.k_new != nullptr && len >= 0 && len < a.limit) return 2u * ((uint32_t)len + 1u) + 1u;
   return 2u * (uint32_t)(len < 0 ? 0 : (len < cap ? len : cap));
 }
 // Units of a row of n keys: one at least, so that an empty row is written too.
@@ -303,8 +305,9 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
       }
       if (a.lens_out != nullptr && m == 0) {
         const int len = a.lens[b];
-        a.lens_out[b] =
-            paged_new_pos(a.table + (int64_t)b * a.max_pages, len, a.P, a.max_pages, a.n_pages) >= 0 ? len + 1 : len;
+        const bool fits = len < a.limit &&
+                          paged_new_pos(a.table + (int64_t)b * a.max_pages, len, a.P, a.max_pages, a.n_pages) >= 0;
+        a.lens_out[b] = fits ? len + 1 : len;
       }
     }
     // the appended row: to LDS for this piece's tiles, and by the first head tile to its page
@@ -541,15 +544,15 @@ __global__ __launch_bounds__(256) void k_paged_append(const T* __restrict__ k, c
                                                       const int32_t* __restrict__ table,
                                                       const int32_t* __restrict__ lens,
                                                       const int32_t* __restrict__ count, int32_t* lens_out, int Hkv,
-                                                      int Tn, int D, int P, int max_pages, int n_pages, int nchunk) {
+                                                      int Tn, int D, int P, int max_pages, int n_pages, int nchunk,
+                                                      int limit) {
   const int b = (int)(blockIdx.x / ((int64_t)Hkv * nchunk));
   const int hc = (int)(blockIdx.x % ((int64_t)Hkv * nchunk));
   const int h = hc / nchunk, ch = hc % nchunk;
-  const int cap = max_pages * P;
   const int len = lens[b];
   int cnt = count == nullptr ? Tn : count[b];
   cnt = cnt < 0 ? 0 : (cnt < Tn ? cnt : Tn);
-  int ok = len >= 0 && len <= cap - cnt;
+  int ok = len >= 0 && len <= limit - cnt;   // (limit: at most max_pages * P)
   if (ok && cnt > 0) {
     const int p1 = (len + cnt - 1) / P;
     for (int p = len / P + threadIdx.x; p <= p1; p += 256) {
@@ -646,12 +649,17 @@ extern "C" size_t nsa_paged_workspace(int B, int Hq, int Hkv, int D, int P, int 
                                       device_cu_count(static_cast<hipStream_t>(stream))));
 }
 
-extern "C" int nsa_paged_attend(const void* q, const void* k_new, const void* v_new, void* k_pages, void* v_pages,
-                                const int32_t* table, const int32_t* lens, int32_t* lens_out, void* out, float* lse,
-                                void* workspace, size_t workspace_bytes, int B, int Hq, int Hkv, int D, int P,
-                                int max_pages, int n_pages, float scale, int dtype, void* stream) {
+static int paged_limit(int max_pages, int P, int max_len) {
+  return max_len < max_pages * P ? max_len : max_pages * P;
+}
+
+extern "C" int nsa_paged_attend_max(const void* q, const void* k_new, const void* v_new, void* k_pages, void* v_pages,
+                                    const int32_t* table, const int32_t* lens, int32_t* lens_out, void* out,
+                                    float* lse, void* workspace, size_t workspace_bytes, int B, int Hq, int Hkv, int D,
+                                    int P, int max_pages, int n_pages, int max_len, float scale, int dtype,
+                                    void* stream) {
   using namespace nsa;
-  NSA_CHECK(paged_shape_ok(B, Hq, Hkv, D, P, max_pages, n_pages), NSA_ERR_SHAPE);
+  NSA_CHECK(paged_shape_ok(B, Hq, Hkv, D, P, max_pages, n_pages) && max_len >= 0, NSA_ERR_SHAPE);
   NSA_CHECK(dtype == NSA_F32 || dtype == NSA_BF16, NSA_ERR_DTYPE);
   if (B == 0) return NSA_OK;
   NSA_CHECK(q != nullptr && k_pages != nullptr && v_pages != nullptr && table != nullptr && lens != nullptr &&
@@ -662,7 +670,7 @@ extern "C" int nsa_paged_attend(const void* q, const void* k_new, const void* v_
   const PagedPlan p =
       paged_plan(B, Hq, Hkv, D * (dtype == NSA_BF16 ? 2 : 4), (int64_t)max_pages * P, device_cu_count(s));
   PagedArgs a{q, k_new, v_new, k_pages, v_pages, table, lens, lens_out, out, lse, nullptr, nullptr, nullptr, B, Hq, Hkv,
-              Hq / Hkv, p.HT, P, P / 16, max_pages, n_pages, p.W, scale * kLog2e};
+              Hq / Hkv, p.HT, P, P / 16, max_pages, n_pages, p.W, paged_limit(max_pages, P, max_len), scale * kLog2e};
   if (p.joined) {
     NSA_CHECK(workspace != nullptr && workspace_bytes >= paged_ws_bytes(D, p), NSA_ERR_WORKSPACE);
     const size_t slots = (size_t)(p.W + p.R) * 16 * p.NT;
@@ -673,11 +681,20 @@ extern "C" int nsa_paged_attend(const void* q, const void* k_new, const void* v_
   return dtype == NSA_BF16 ? paged_dim<bf16>(a, p, D, s) : paged_dim<float>(a, p, D, s);
 }
 
-extern "C" int nsa_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* table,
-                                const int32_t* lens, const int32_t* count, int32_t* lens_out, int B, int Hkv, int T,
-                                int D, int P, int max_pages, int n_pages, int dtype, void* stream) {
+extern "C" int nsa_paged_attend(const void* q, const void* k_new, const void* v_new, void* k_pages, void* v_pages,
+                                const int32_t* table, const int32_t* lens, int32_t* lens_out, void* out, float* lse,
+                                void* workspace, size_t workspace_bytes, int B, int Hq, int Hkv, int D, int P,
+                                int max_pages, int n_pages, float scale, int dtype, void* stream) {
+  return nsa_paged_attend_max(q, k_new, v_new, k_pages, v_pages, table, lens, lens_out, out, lse, workspace,
+                              workspace_bytes, B, Hq, Hkv, D, P, max_pages, n_pages, INT32_MAX, scale, dtype, stream);
+}
+
+extern "C" int nsa_paged_append_max(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* table,
+                                    const int32_t* lens, const int32_t* count, int32_t* lens_out, int B, int Hkv,
+                                    int T, int D, int P, int max_pages, int n_pages, int max_len, int dtype,
+                                    void* stream) {
   using namespace nsa;
-  NSA_CHECK(paged_shape_ok(B, Hkv, Hkv, D, P, max_pages, n_pages) && T >= 0, NSA_ERR_SHAPE);
+  NSA_CHECK(paged_shape_ok(B, Hkv, Hkv, D, P, max_pages, n_pages) && T >= 0 && max_len >= 0, NSA_ERR_SHAPE);
   NSA_CHECK(dtype == NSA_F32 || dtype == NSA_BF16, NSA_ERR_DTYPE);
   if (B == 0) return NSA_OK;
   NSA_CHECK(k_pages != nullptr && v_pages != nullptr && table != nullptr && lens != nullptr && lens_out != nullptr &&
@@ -686,13 +703,23 @@ extern "C" int nsa_paged_append(const void* k, const void* v, void* k_pages, voi
   const int64_t grid = (int64_t)B * Hkv * nchunk;
   NSA_CHECK(grid < (1 << 24), NSA_ERR_SHAPE);   // a grid holds less than 2^32 threads
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  const int limit = paged_limit(max_pages, P, max_len);
   if (dtype == NSA_BF16)
     k_paged_append<bf16><<<(unsigned)grid, 256, 0, s>>>(
         static_cast<const bf16*>(k), static_cast<const bf16*>(v), static_cast<bf16*>(k_pages),
-        static_cast<bf16*>(v_pages), table, lens, count, lens_out, Hkv, T, D, P, max_pages, n_pages, nchunk);
+        static_cast<bf16*>(v_pages), table, lens, count, lens_out, Hkv, T, D, P, max_pages, n_pages, nchunk,
+        limit);
   else
     k_paged_append<float><<<(unsigned)grid, 256, 0, s>>>(
         static_cast<const float*>(k), static_cast<const float*>(v), static_cast<float*>(k_pages),
-        static_cast<float*>(v_pages), table, lens, count, lens_out, Hkv, T, D, P, max_pages, n_pages, nchunk);
+        static_cast<float*>(v_pages), table, lens, count, lens_out, Hkv, T, D, P, max_pages, n_pages, nchunk,
+        limit);
   return nsa_launch_status();
+}
+
+extern "C" int nsa_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* table,
+                                const int32_t* lens, const int32_t* count, int32_t* lens_out, int B, int Hkv, int T,
+                                int D, int P, int max_pages, int n_pages, int dtype, void* stream) {
+  return nsa_paged_append_max(k, v, k_pages, v_pages, table, lens, count, lens_out, B, Hkv, T, D, P, max_pages,
+                              n_pages, INT32_MAX, dtype, stream);
 }

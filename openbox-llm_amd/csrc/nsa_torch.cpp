@@ -42,7 +42,7 @@ NSA_ENTRY(nsa_norm_bwd_workspace);
 NSA_ENTRY(nsa_logprob_fwd);
 NSA_ENTRY(nsa_logprob_bwd);
 NSA_ENTRY(nsa_logprob_workspace);
-NSA_ENTRY(nsa_paged_attend);
+NSA_ENTRY(nsa_paged_attend_max);
 NSA_ENTRY(nsa_paged_workspace);
 #undef NSA_ENTRY
 
@@ -54,7 +54,7 @@ void bind(const py::dict& at) {
   NSA_BIND(nsa_logprob_fwd);
   NSA_BIND(nsa_logprob_bwd);
   NSA_BIND(nsa_logprob_workspace);
-  NSA_BIND(nsa_paged_attend);
+  NSA_BIND(nsa_paged_attend_max);
   NSA_BIND(nsa_paged_workspace);
 #undef NSA_BIND
 }
@@ -386,7 +386,8 @@ void check_pages(const Tensor& kp, const Tensor& vp, const Tensor& table, const 
 // -> (out, lse or None, new lengths or None)
 std::tuple<Tensor, OptTensor, OptTensor> paged(const Tensor& q_, const OptTensor& k_new, const OptTensor& v_new,
                                                const Tensor& kp, const Tensor& vp, const Tensor& table_,
-                                               const Tensor& lens_, std::optional<double> scale, bool want_lse) {
+                                               const Tensor& lens_, std::optional<double> scale, bool want_lse,
+                                               std::optional<int64_t> max_len) {
   no_tangent(has_tangent(q_) || has_tangent(k_new) || has_tangent(v_new) || has_tangent(kp) || has_tangent(vp),
              "paged attention");
   check_pages(kp, vp, table_, lens_);
@@ -402,6 +403,8 @@ std::tuple<Tensor, OptTensor, OptTensor> paged(const Tensor& q_, const OptTensor
     NSA_ASSERT(!q_.requires_grad() && !(k_new && (k_new->requires_grad() || v_new->requires_grad())) &&
                    !kp.requires_grad() && !vp.requires_grad(),
                "paged: attention over pages has no gradient: call it under torch.no_grad()");
+  NSA_ASSERT(!max_len || *max_len >= 0, "paged: max_len must not be negative");
+  const int end = max_len && *max_len < INT32_MAX ? (int)*max_len : INT32_MAX;
   const Tensor q = aligned(q_), table = table_.contiguous(), lens = lens_.contiguous();
   Tensor kn, vn, lens_out, lse;
   if (k_new) {
@@ -421,11 +424,11 @@ std::tuple<Tensor, OptTensor, OptTensor> paged(const Tensor& q_, const OptTensor
     const size_t bytes = p_nsa_paged_workspace((int)B, (int)Hq, (int)Hkv, (int)D, (int)P, (int)mp, code, on.stream);
     const Tensor ws = bytes > 16 ? fresh({(int64_t)bytes}, q, at::kByte) : Tensor();
     const double s = scale ? *scale : 1.0 / std::sqrt((double)D);
-    check_status(p_nsa_paged_attend(q.data_ptr(), at_of(kn), at_of(vn), kp.data_ptr(), vp.data_ptr(),
+    check_status(p_nsa_paged_attend_max(q.data_ptr(), at_of(kn), at_of(vn), kp.data_ptr(), vp.data_ptr(),
                                     static_cast<const int32_t*>(table.data_ptr()),
                                     static_cast<const int32_t*>(lens.data_ptr()), at_as<int32_t>(lens_out),
                                     out.data_ptr(), at_as<float>(lse), at_of(ws), bytes, (int)B, (int)Hq, (int)Hkv,
-                                    (int)D, (int)P, (int)mp, (int)n, (float)s, code, on.stream),
+                                    (int)D, (int)P, (int)mp, (int)n, end, (float)s, code, on.stream),
                  "nsa_paged_attend");
   }
   return {out, want_lse ? OptTensor(lse) : std::nullopt, k_new ? OptTensor(lens_out) : std::nullopt};

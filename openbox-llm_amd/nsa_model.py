@@ -857,7 +857,9 @@ class NSATransformer(nn.Module):
     def step(self, tokens, caches):
         """One generation step: ``tokens [B]`` at each sequence's next position
         -> logits ``[B, V]``; the caches grow by one (their pages reserved).  No
-        host synchronisation: the loop can be captured into a graph."""
+        host synchronisation: the loop can be captured into a graph.  A
+        sequence that is as long as its caches take no longer grows: its
+        length tells (its logits then are of no position)."""
         x = self.tok_emb(tokens)
         if hasattr(self, "pos_emb"):
             x = x + self.pos_emb(caches[0].lens.long().clamp(0, self.max_seq_len - 1))

@@ -31,12 +31,12 @@ import _nsa_lib as L
 import nsa_hip_ops as _ops
 
 
-def _attend(q, k_new, v_new, k_pages, v_pages, table, lens, scale, return_lse):
+def _attend(q, k_new, v_new, k_pages, v_pages, table, lens, scale, return_lse, max_len=None):
     f = L.torch_side().paged
     if _ops._TIMER is None:
-        return f(q, k_new, v_new, k_pages, v_pages, table, lens, scale, return_lse)
+        return f(q, k_new, v_new, k_pages, v_pages, table, lens, scale, return_lse, max_len)
     with _ops._span("nsa_paged_attend"):
-        return f(q, k_new, v_new, k_pages, v_pages, table, lens, scale, return_lse)
+        return f(q, k_new, v_new, k_pages, v_pages, table, lens, scale, return_lse, max_len)
 
 
 def paged_attend(q, k_pages, v_pages, table, lens, scale=None, return_lse=False):
@@ -48,21 +48,23 @@ def paged_attend(q, k_pages, v_pages, table, lens, scale=None, return_lse=False)
     return (out, lse) if return_lse else out
 
 
-def paged_step(q, k_new, v_new, k_pages, v_pages, table, lens, scale=None):
+def paged_step(q, k_new, v_new, k_pages, v_pages, table, lens, scale=None, max_len=None):
     """One generation step: the new rows ``[B, Hkv, D]`` go to position
     ``lens[b]`` (in place, in the pages), then ``q [B, Hq, D]`` attends the
     ``lens[b] + 1`` positions -> ``(out, new lens)``; the lengths are a new
-    tensor.  A sequence whose position has no page keeps its pages and length
-    and attends what it holds.  Pages that are written may not be shared with
+    tensor.  A sequence whose position has no page, or is at or past ``max_len``
+    (default: the table's end), keeps its pages and length and attends what it
+    holds.  Pages that are written may not be shared with
     another sequence of the call."""
-    out, _, lens_out = _attend(q, k_new, v_new, k_pages, v_pages, table, lens, scale, False)
+    out, _, lens_out = _attend(q, k_new, v_new, k_pages, v_pages, table, lens, scale, False, max_len)
     return out, lens_out
 
 
-def paged_append(k, v, k_pages, v_pages, table, lens, count=None):
+def paged_append(k, v, k_pages, v_pages, table, lens, count=None, max_len=None):
     """Write rows ``k, v [B, Hkv, T, D]`` (the first ``count[b]`` of them: int32
     ``[B]``, default T) to positions ``lens[b] ..`` -> the new lengths.  A
-    sequence whose rows do not all have a page keeps its pages and length."""
+    sequence whose rows do not all have a page, or do not all lie before
+    ``max_len`` (default: the table's end), keeps its pages and length."""
     side = L.torch_side()
     side.no_tangent([k, v, k_pages, v_pages], "paged_append")
     side.check_pages(k_pages, v_pages, table, lens)
@@ -75,6 +77,8 @@ def paged_append(k, v, k_pages, v_pages, table, lens, count=None):
     assert not (torch.is_grad_enabled() and any(t.requires_grad for t in (k, v, k_pages, v_pages))), \
         "paged: rows in pages have no gradient: call it under torch.no_grad()"
     assert Hkv <= 4096 and B <= 65536, "paged: at most 4096 heads and 65536 sequences"
+    assert max_len is None or max_len >= 0, "paged: max_len must not be negative"
+    end = 2 ** 31 - 1 if max_len is None else min(max_len, 2 ** 31 - 1)
     k, v, table, lens = _ops._contig(k), _ops._contig(v), table.contiguous(), lens.contiguous()
     if count is not None:
         assert count.dtype == torch.int32 and count.shape == (B,) and count.device == lens.device, \
@@ -83,9 +87,9 @@ def paged_append(k, v, k_pages, v_pages, table, lens, count=None):
     lens_out = torch.empty_like(lens)
     if B > 0:
         with _ops.device_of(k_pages):
-            _ops._call("nsa_paged_append", _ops._lib().nsa_paged_append, L.ptr(k), L.ptr(v), L.ptr(k_pages),
+            _ops._call("nsa_paged_append", _ops._lib().nsa_paged_append_max, L.ptr(k), L.ptr(v), L.ptr(k_pages),
                        L.ptr(v_pages), L.ptr(table), L.ptr(lens), L.ptr(count), L.ptr(lens_out), B, Hkv, k.shape[2], D,
-                       P, mp, n, L.dtype_code(k_pages), _ops._stream(k_pages))
+                       P, mp, n, end, L.dtype_code(k_pages), _ops._stream(k_pages))
     return lens_out
 
 
@@ -196,7 +200,8 @@ class PagedKVCache:
         """Append a prompt's rows ``[B, Hkv, T, D]``, ``lens`` of them a sequence
         (int32 ``[B]`` on the device, or host ints; default T); the pages must
         be reserved."""
-        self.lens.copy_(paged_append(k, v, self.k_pages, self.v_pages, self.table, self.lens, self.counts(lens)))
+        self.lens.copy_(paged_append(k, v, self.k_pages, self.v_pages, self.table, self.lens, self.counts(lens),
+                                     self.max_len))
 
     def counts(self, lens):
         """``prefill``'s ``lens`` as it is handed to the kernel (int32 on the device, or
@@ -207,8 +212,11 @@ class PagedKVCache:
 
     def step(self, q, k_new, v_new, scale=None):
         """``paged_step`` on this cache -> ``out [B, Hq, D]``.  The lengths are
-        updated in place: a captured step advances the cache on every replay."""
-        out, lens = paged_step(q, k_new, v_new, self.k_pages, self.v_pages, self.table, self.lens, scale)
+        updated in place: a captured step advances the cache on every replay.
+        A sequence of ``max_len`` tokens, or whose position is not reserved,
+        keeps its length and attends what it holds."""
+        out, lens = paged_step(q, k_new, v_new, self.k_pages, self.v_pages, self.table, self.lens, scale,
+                               self.max_len)
         self.lens.copy_(lens)
         return out
 

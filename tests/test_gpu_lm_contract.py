@@ -273,3 +273,72 @@ def test_host_numbers_inside_a_capture_are_refused():
         graph.replay()
         torch.cuda.synchronize()
         assert c.lens.tolist() == [20, 3]
+
+
+@pytest.mark.parametrize("B,P", [(3, 144), (3, 64), (300, 64)])
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_a_cache_ends_at_max_len_inside_a_page(dtype, B, P):
+    """max_len 100 over pages of 64 or 144 (equal shares of all keys): position 99 is the last one taken; a step or a
+    prompt past it writes nothing, keeps the length, and attends the 100 keys."""
+    import nsa_paged
+    dev = require_gpu()
+    Hq, Hkv, D = 4, 2, 32
+    c = nsa_paged.PagedKVCache(B, Hkv, D, 100, P, dtype=dtype)
+    c.reserve(100)
+    g = torch.Generator().manual_seed(0)
+    k, v = (torch.randn(B, Hkv, 98, D, generator=g).to(dtype).to(dev) for _ in range(2))
+    start = [98, 97, 50] + [98] * (B - 3)
+    c.prefill(k, v, start)
+    for s in range(5):
+        q, kn, vn = (torch.randn(B, h, D, generator=g).to(dtype).to(dev) for h in (Hq, Hkv, Hkv))
+        before = c.k_pages.clone()
+        want_lens = [min(100, n + s + 1) for n in start]
+        out = c.step(q, kn, vn)
+        assert c.lens.tolist() == want_lens
+        assert torch.equal(out, c.attend(q))                # (the same keys in the same pieces)
+        ids = c.table.cpu()
+        for b in range(3):
+            if start[b] + s < 100:
+                before[int(ids[b, (start[b] + s) // P]), :, (start[b] + s) % P] = kn[b]
+        if B > 3 and s < 2:
+            at = 98 + s
+            before[c.table[3:, at // P].long(), :, at % P] = kn[3:]
+        assert torch.equal(c.k_pages, before)
+    c.prefill(k[:, :, :1], v[:, :, :1], 1)                  # one row more: only where it fits
+    assert c.lens.tolist() == [100, 100, 56] + [100] * (B - 3)
+    c.prefill(k, v, 45)                                     # 56 + 45 = 101
+    assert c.lens.tolist() == [100, 100, 56] + [100] * (B - 3)
+    c.prefill(k, v, 44)
+    assert c.lens.tolist() == [100] * B
+    with pytest.raises(AssertionError):
+        c.reserve(101)
+    lens = torch.full((B,), 100, dtype=torch.int32, device=dev)
+    args = (q, kn, vn, c.k_pages, c.v_pages, c.table, lens)
+    assert nsa_paged.paged_step(*args)[1].tolist() == [101] * B          # the bare pages go to the table's end
+    assert nsa_paged.paged_step(*args, max_len=100)[1].tolist() == [100] * B
+    assert nsa_paged.paged_step(*args, max_len=0)[1].tolist() == [100] * B
+    with pytest.raises(AssertionError):
+        nsa_paged.paged_step(*args, max_len=-1)
+    with pytest.raises(AssertionError):
+        nsa_paged.paged_append(k, v, *args[3:], max_len=-1)
+
+
+@pytest.mark.parametrize("pos", ["learned", "rope"])
+def test_generation_ends_at_the_models_length(pos):
+    """max_seq_len 90 over pages of 64: the last position's logits are the
+    forward's, and no token is appended behind it."""
+    require_gpu()
+    m = _model(pos=pos, max_seq_len=90).eval()
+    x = _tokens(2, 90)
+    with torch.no_grad():
+        want = m(x)[0]
+    caches = m.paged_caches(2)
+    caches[0].reserve(90)
+    m.prefill(x[:, :85], caches)
+    for s in range(85, 90):
+        logits = m.step(x[:, s], caches)
+        assert (logits - want[:, s]).abs().max() <= 1e-4 * want.abs().max()
+    kept = [c.k_pages.clone() for c in caches]
+    m.step(x[:, 0], caches)
+    for c, k in zip(caches, kept):
+        assert c.lens.tolist() == [90, 90] and torch.equal(c.k_pages, k)

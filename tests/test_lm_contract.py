@@ -129,3 +129,16 @@ def test_reserving_takes_nothing_where_it_raises(monkeypatch):
     held = [t[t >= 0].tolist() for t in c.table]
     assert c.free_pages == 2 and [len(h) for h in held] == [0, 3] and held == c._account.held
     assert c.counts(None) is None and c.counts(3).tolist() == [3, 3] and c.counts([4, 5]).dtype == torch.int32
+
+
+def test_an_end_before_the_first_position_is_refused():
+    import os
+    import _nsa_lib
+    if not os.path.exists(_nsa_lib.LIB_PATH):
+        pytest.skip("libnsa_hip.so not built")
+    lib = _nsa_lib.load()
+    shape = (1, 4, 2, 64, 16, 3, 5)
+    assert lib.nsa_paged_attend_max(*[None] * 11, 0, *shape, -1, 0.1, 1, None) == _nsa_lib.NSA_ERR_SHAPE
+    assert lib.nsa_paged_attend_max(*[None] * 11, 0, *shape, 0, 0.1, 1, None) == _nsa_lib.NSA_ERR_ARG
+    assert lib.nsa_paged_append_max(*[None] * 8, 1, 2, 4, 64, 16, 3, 5, -1, 1, None) == _nsa_lib.NSA_ERR_SHAPE
+    assert lib.nsa_paged_append_max(*[None] * 8, 1, 2, 4, 64, 16, 3, 5, 7, 1, None) == _nsa_lib.NSA_ERR_ARG
