@@ -578,7 +578,8 @@ int nsa_logprob_bwd(const void* z, const int64_t* target, const float* stat, con
  * sequence whose position has no page (past the table, or an entry outside
  * 0 .. n_pages - 1) keeps its length and rows and attends what it holds.
  * Keys whose table entry is outside 0 .. n_pages - 1 are not attended; rows past
- * a length have no influence, whatever they hold.  lse (float [B][Hq], nullable): ln sum e^score, -1e9
+ * a length have no influence, whatever they hold.  A score of -inf weighs nothing; a
+ * row of nothing else is one without keys.  lse (float [B][Hq], nullable): ln sum e^score, -1e9
  * where there is no key.  lens and lens_out are different buffers.
  * workspace: nsa_paged_workspace bytes (0: unsupported shape). */
 size_t nsa_paged_workspace(int B, int Hq, int Hkv, int D, int P, int max_pages, int dtype, void* stream);

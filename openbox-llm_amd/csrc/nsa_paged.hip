@@ -45,6 +45,9 @@
 namespace nsa {
 
 constexpr int kUnit = 128;   // keys of a unit: a tile for each wave
+// The running maximum's start, and the score of a key that is not there: at or below every finite score (a sentinel
+// within their range would take weight from rows whose scores are all below it).
+constexpr float kLowScore = -3.402823466e38f;
 
 struct PagedArgs {
   const void *q, *k_new, *v_new;     // [B][Hq][D], [B][Hkv][D] (null: no append)
@@ -326,7 +329,10 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
 
     FwdAcc<D> acc[NT];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) acc[nt].init();
+    for (int nt = 0; nt < NT; ++nt) {
+      acc[nt].init();
+      acc[nt].m = kLowScore;
+    }
     for (int i = 0; i < ntile; ++i) {
       // The next tile's keys are asked for as soon as this one's are used, its values likewise: a wave has one or
       // the other in flight at all times, in the registers of one tile.  (Two tiles ahead measured slower: 232
@@ -355,10 +361,10 @@ __global__ __launch_bounds__(256, 2) void k_paged(const PagedArgs a) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         FwdAcc<D>& A = acc[nt];
-        float sv[8], mx = kMaskScore;
+        float sv[8], mx = kLowScore;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          sv[j] = ((seen >> j) & 1u) ? s[nt][j >> 2][j & 3] * a.sl2 : kMaskScore;
+          sv[j] = ((seen >> j) & 1u) ? s[nt][j >> 2][j & 3] * a.sl2 : kLowScore;
           mx = fmaxf(mx, sv[j]);
         }
         mx = group4_max(mx);
@@ -486,7 +492,7 @@ __global__ __launch_bounds__(64 * W) void k_paged_join(const PagedArgs a, int NT
   const int step = 16 * NT;                           // slots from a piece to the next
   // Pieces w, w + W, ... eight at a time, all asked for at once; a running maximum, the waves' own joined below.
   constexpr int E = D >= 64 ? D / 64 : 1;
-  float m = kMaskScore, l = 0.0f, o[E];
+  float m = kLowScore, l = 0.0f, o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.0f;
   for (int i0 = w; i0 < np; i0 += 8 * W) {
@@ -495,7 +501,7 @@ __global__ __launch_bounds__(64 * W) void k_paged_join(const PagedArgs a, int NT
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int i = i0 + j * W;
-      s[j] = i < np ? ml[(int64_t)i * step] : make_float2(kMaskScore, 0.0f);
+      s[j] = i < np ? ml[(int64_t)i * step] : make_float2(kLowScore, 0.0f);
 #pragma unroll
       for (int e = 0; e < E; ++e)
         v[j][e] = i < np && E * lane + e < D ? po[(int64_t)i * step * D + E * lane + e] : 0.0f;

@@ -19,6 +19,9 @@ captured into a graph.  Query head h reads KV head ``h // (Hq // Hkv)``.
 Table entries outside ``0 .. n_pages-1`` are no pages: keys there are not
 attended and rows are not written.  Rows past a length have no influence,
 whatever they hold.  A negative length stands for no sequence: its output is zeros, its length stays.
+A score of -inf is a key masked out: where every key is, the output is zeros and
+the log sum -1e9, as without keys.  NaN or +inf in a score give NaN, and an
+infinite value in a visible row NaN or an infinity.
 
 For inference: inputs that need a gradient, or carry a forward-mode one, are refused.
 """

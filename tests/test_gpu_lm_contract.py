@@ -342,3 +342,53 @@ def test_generation_ends_at_the_models_length(pos):
     m.step(x[:, 0], caches)
     for c, k in zip(caches, kept):
         assert c.lens.tolist() == [90, 90] and torch.equal(c.k_pages, k)
+
+
+@pytest.mark.parametrize("n", [5, 100, 4000])
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_scores_at_the_ends_of_the_range(dtype, n):
+    """Rows whose scores are all far below -1e30, scores of -inf among finite ones,
+    nothing but -inf, and NaN or +inf; in one piece and joined.
+
+    The scores are powers of two times small whole numbers, so that the weights are
+    exactly equal or 0.  An average over m keys: at most n/16 + 40 additions, one
+    product with 1 / m, and half a step of the output's dtype; bf16 weights in two
+    parts are exact here."""
+    import nsa_paged
+    dev = require_gpu()
+    D, P, U = 16, 48, 2.0 ** -24
+    mp = -(-4100 // P)
+    g = torch.Generator().manual_seed(n)
+    v = torch.randn(1, 1, n, D, generator=g).to(dtype)
+    low = torch.zeros(1, 1, n, D)
+    low[..., 0] = -(2.0 ** 50) * (1 + torch.arange(n) % 3)          # scores of -1e31 to -3e31
+    some = torch.zeros(1, 1, n, D)
+    some[..., 0] = torch.where(torch.arange(n) % 3 == 0, 0.0, -float("inf"))
+    none = torch.zeros(1, 1, n, D)
+    none[..., 0] = -float("inf")
+    q = torch.zeros(1, 2, D)
+    q[..., 0] = 2.0 ** 55
+    c = nsa_paged.PagedKVCache(1, 1, D, mp * P, P, dtype=dtype)
+    c.reserve(n)
+    keep = torch.arange(n) % 3 == 0
+    vk = v[0, 0, keep].double()
+    ref = vk.mean(0)
+    tol = ref.abs() * torch.finfo(dtype).eps / 2 * (1 + 1e-6) + vk.abs().mean(0) * (n / 16 + 42) * U
+    for k, base in ((low, -(2.0 ** 105) / 4), (some, 0.0)):
+        c.lens.zero_()
+        c.prefill(k.to(dtype).to(dev), v.to(dev))
+        out, lse = c.attend(q.to(dtype).to(dev), return_lse=True)
+        assert ((out.cpu().double() - ref).abs() <= tol).all()
+        want = base + torch.tensor(float(keep.sum())).double().log()
+        assert ((lse.cpu().double() - want).abs() <= 8 * U * want.abs() + 8 * U).all()
+    c.lens.zero_()
+    c.prefill(none.to(dtype).to(dev), v.to(dev))
+    out, lse = c.attend(q.to(dtype).to(dev), return_lse=True)
+    assert not out.any() and (lse == -1e9).all()
+    for bad in (float("nan"), float("inf")):
+        k = some.clone()
+        k[0, 0, n // 2, 0] = bad
+        c.lens.zero_()
+        c.prefill(k.to(dtype).to(dev), v.to(dev))
+        out, lse = c.attend(q.to(dtype).to(dev), return_lse=True)
+        assert out.isnan().all()
