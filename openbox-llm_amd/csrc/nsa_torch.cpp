@@ -388,6 +388,7 @@ std::tuple<Tensor, OptTensor, OptTensor> paged(const Tensor& q_, const OptTensor
                                                const Tensor& kp, const Tensor& vp, const Tensor& table_,
                                                const Tensor& lens_, std::optional<double> scale, bool want_lse,
                                                std::optional<int64_t> max_len) {
+  NSA_ASSERT(k_new.has_value() == v_new.has_value(), "paged: a new key row needs its value row, and the other way round");
   no_tangent(has_tangent(q_) || has_tangent(k_new) || has_tangent(v_new) || has_tangent(kp) || has_tangent(vp),
              "paged attention");
   check_pages(kp, vp, table_, lens_);

@@ -59,6 +59,7 @@ def paged_step(q, k_new, v_new, k_pages, v_pages, table, lens, scale=None, max_l
     (default: the table's end), keeps its pages and length and attends what it
     holds.  Pages that are written may not be shared with
     another sequence of the call."""
+    assert k_new is not None and v_new is not None, "paged: a step takes new rows (paged_attend takes none)"
     out, _, lens_out = _attend(q, k_new, v_new, k_pages, v_pages, table, lens, scale, False, max_len)
     return out, lens_out
 

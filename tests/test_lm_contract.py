@@ -142,3 +142,21 @@ def test_an_end_before_the_first_position_is_refused():
     assert lib.nsa_paged_attend_max(*[None] * 11, 0, *shape, 0, 0.1, 1, None) == _nsa_lib.NSA_ERR_ARG
     assert lib.nsa_paged_append_max(*[None] * 8, 1, 2, 4, 64, 16, 3, 5, -1, 1, None) == _nsa_lib.NSA_ERR_SHAPE
     assert lib.nsa_paged_append_max(*[None] * 8, 1, 2, 4, 64, 16, 3, 5, 7, 1, None) == _nsa_lib.NSA_ERR_ARG
+
+
+def test_a_step_takes_both_rows():
+    """A missing row is refused: not read through, and not taken as an attention
+    without one."""
+    import os
+    import _nsa_lib
+    if not os.path.exists(_nsa_lib.LIB_PATH):
+        pytest.skip("libnsa_hip.so not built")
+    import nsa_paged
+    q, row, pages = torch.zeros(1, 1, 16), torch.zeros(1, 1, 16), torch.zeros(2, 1, 16, 16)
+    table, lens = torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    for k, v in ((row, None), (None, row), (None, None)):
+        with pytest.raises(AssertionError, match="row"):
+            nsa_paged.paged_step(q, k, v, pages, pages, table, lens)
+    for k, v in ((row, None), (None, row)):
+        with pytest.raises(AssertionError, match="row"):
+            _nsa_lib.torch_side().paged(q, k, v, pages, pages, table, lens, None, False, None)
