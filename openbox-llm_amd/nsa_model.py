@@ -840,6 +840,7 @@ class NSATransformer(nn.Module):
         ``lens[b]`` tokens (default all) kept in the (empty, reserved) caches."""
         B, T = idx.shape
         assert T <= self.max_seq_len
+        assert len(caches) == len(self.blocks), "one cache for each block"
         x = self.tok_emb(idx)
         if hasattr(self, "pos_emb"):
             x = x + self.pos_emb(torch.arange(T, device=idx.device))[None]
@@ -860,6 +861,7 @@ class NSATransformer(nn.Module):
         host synchronisation: the loop can be captured into a graph.  A
         sequence that is as long as its caches take no longer grows: its
         length tells (its logits then are of no position)."""
+        assert len(caches) == len(self.blocks), "one cache for each block"
         x = self.tok_emb(tokens)
         if hasattr(self, "pos_emb"):
             x = x + self.pos_emb(caches[0].lens.long().clamp(0, self.max_seq_len - 1))

@@ -160,3 +160,15 @@ def test_a_step_takes_both_rows():
     for k, v in ((row, None), (None, row)):
         with pytest.raises(AssertionError, match="row"):
             _nsa_lib.torch_side().paged(q, k, v, pages, pages, table, lens, None, False, None)
+
+
+def test_a_model_takes_one_cache_a_block():
+    """Fewer would leave the blocks behind them out."""
+    from nsa_model import NSATransformer
+    m = NSATransformer(vocab_size=20, d_model=32, n_layers=2, n_q_heads=2, n_kv_heads=1, max_seq_len=16,
+                       attn_type="full")
+    for caches in ([object()], [object()] * 3, []):
+        with pytest.raises(AssertionError, match="one cache"):
+            m.prefill(torch.zeros(1, 4, dtype=torch.long), caches)
+        with pytest.raises(AssertionError, match="one cache"):
+            m.step(torch.zeros(1, dtype=torch.long), caches)
