@@ -191,9 +191,11 @@ class PagedKVCache:
             acc.held[b].append(page)
 
     def release(self, seq):
-        """Give back sequence ``seq``'s pages; its length becomes 0."""
+        """Give back sequence ``seq``'s pages; its length becomes 0.  Refused inside a
+        capture, whose replays the account would not see."""
         acc = self._account
         assert 0 <= seq < self.batch, "paged: no such sequence"
+        assert not (self.lens.is_cuda and torch.cuda.is_current_stream_capturing()), "paged: release inside a capture"
         acc.free.extend(reversed(acc.held[seq]))
         acc.held[seq] = []
         acc.table[seq].fill_(-1)

@@ -392,3 +392,25 @@ def test_scores_at_the_ends_of_the_range(dtype, n):
         c.prefill(k.to(dtype).to(dev), v.to(dev))
         out, lse = c.attend(q.to(dtype).to(dev), return_lse=True)
         assert out.isnan().all()
+
+
+def test_releasing_inside_a_capture_is_refused():
+    """The account would give the pages to another sequence, and every replay take
+    them from it again."""
+    import nsa_paged
+    dev = require_gpu()
+    c = nsa_paged.PagedKVCache(2, 1, 16, 64, 16, dtype=F32)
+    c.reserve(32)
+    x = torch.zeros(4, device=dev)
+    table = c.table.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x += 1
+        with pytest.raises(AssertionError, match="capture"):
+            c.release(0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert c.free_pages == 4 and torch.equal(c.table, table)
+    c.release(0)
+    assert c.free_pages == 6 and (c.table[0] == -1).all()
