@@ -414,3 +414,64 @@ def test_releasing_inside_a_capture_is_refused():
     assert c.free_pages == 4 and torch.equal(c.table, table)
     c.release(0)
     assert c.free_pages == 6 and (c.table[0] == -1).all()
+
+
+# B, lens, Hq, Hkv, D, P
+COUNTS = [(1, [20000], 64, 4, 128, 80), (1, [33000], 16, 1, 64, 256), (5, [1, 127, 128, 129, 5000], 40, 1, 128, 16),
+          (7, [3000, 0, 31, 2049, 4095, 4096, 4097], 12, 2, 32, 48), (300, [(7 * i) % 90 for i in range(300)], 8, 8, 16, 112)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("c", COUNTS, ids=lambda c: f"B{c[0]}-n{max(c[1])}-H{c[2]}:{c[3]}")
+def test_every_key_counts_once(c, dtype):
+    """Equal scores: every weight is exactly 1 before the division and every sum of
+    them a whole number below 2^24, so that only 1 / n, its product (2 u) and the
+    output's half step round.  A key left out or taken twice shows in the log
+    sum (by 1 / n, against its logarithm's and product's 4 u ln n) and, where it
+    has a column of its own at an edge of a tile, share or page, in the output by
+    all of it."""
+    import nsa_paged
+    dev = require_gpu()
+    B, lens, Hq, Hkv, D, P = c
+    U, half = 2.0 ** -24, torch.finfo(dtype).eps / 2
+    g = torch.Generator().manual_seed(B + D)
+    cache = nsa_paged.PagedKVCache(B, Hkv, D, max(lens), P, dtype=dtype)
+    cache.reserve(lens)
+    T = max(lens)
+    k = torch.randn(B, Hkv, T, D, generator=g).to(dtype)
+    whole = torch.randint(-8, 9, (B, Hkv, T, D), generator=g).to(dtype)
+    alone = torch.zeros(B, Hkv, T, D, dtype=dtype)
+    for b, n in enumerate(lens):
+        if n == 0:
+            continue
+        edges = [e for m in (32, 128, P, 1024) for x in (m, n // m * m) for e in (x - 1, x)]
+        edges += [0, n - 1] + torch.randint(0, n, (D,), generator=g).tolist()
+        edges = list(dict.fromkeys(e for e in edges if 0 <= e < n))[:D]
+        alone[b][:, edges, torch.arange(len(edges))] = 2.0 ** 14
+    q = torch.zeros(B, Hq, D, dtype=dtype, device=dev)
+    n = torch.tensor(lens)[:, None, None]
+    for v in (whole, alone):
+        cache.lens.zero_()
+        cache.prefill(k.to(dev), v.to(dev), lens)
+        out, lse = cache.attend(q, return_lse=True)
+        live = torch.arange(T)[None, None, :, None] < n[..., None]
+        ref = (torch.where(live, v.double(), 0.0).sum(2) / n.clamp(min=1)).repeat_interleave(Hq // Hkv, 1)
+        err = (out.cpu().double() - ref).abs()
+        assert (err <= ref.abs() * (half + 2 * U) * (1 + 1e-6)).all(), float(err.max())
+        want = torch.where(n[:, :, 0] > 0, n[:, :, 0].double().log(), -1e9)
+        assert ((lse.cpu().double() - want).abs() <= torch.where(n[:, :, 0] > 0, 4 * U * want, 0.0)).all()
+
+
+@pytest.mark.parametrize("rows,D", [(2, 8), (5, 250), (3, 1001), (4, 2049), (3, 4096), (300, 8192)])
+def test_norm_within_one_run_a_thread(rows, D):
+    """Rows of up to 8192 elements are one run of 8 a thread: 8 additions, 6 steps
+    over the wave, 16 waves, halved by the root, and 7 roundings besides."""
+    import nsa_lm
+    dev = require_gpu()
+    g = torch.Generator().manual_seed(D)
+    x, r = torch.randn(rows, D, generator=g), torch.randn(rows, D, generator=g)
+    w = 1 + 0.2 * torch.randn(D, generator=g)
+    y, h = nsa_lm.add_rms_norm(x.to(dev), r.to(dev), w.to(dev), eps=1e-5)
+    h64 = (x + r).double()
+    ref = h64 / torch.sqrt((h64 * h64).mean(-1, keepdim=True) + 1e-5) * w.double()
+    assert ((y.cpu().double() - ref).abs() <= ref.abs() * (15 + 7 + 1) * 2.0 ** -24).all()
