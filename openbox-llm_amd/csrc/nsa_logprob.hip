@@ -27,10 +27,13 @@
 // eight passes).
 //
 // Measured (MI355X): 32768 x 32000 in bf16 384 us forward and 737 backward, 5.5
-// and 5.7 TB/s, bound by memory; 2047 x 50257 47 us, 50 with 5 or 20
-// alternatives (38 at the rate of a large copy: all rows are resident at once,
-// so that they start and end together); 32 x 32000 with 20 8.5 us, a row's own
-// chain of load, sums, bound and ranking.
+// and 5.7 TB/s, bound by memory; 2047 x 50257 45 us, 49 with 5 and 50 with 20
+// alternatives in a captured loop (38 at the rate of a large copy: all rows are
+// resident at once, so that they start and end together); 32 x 32000 with 20 8.5
+// us, a row's own chain of load, sums, bound and ranking.
+//
+// A weight e^x, x = z - m, is formed as 2^(x log2 e): the product's rounding makes
+// it right to about |x| 2^-24, so that the lighter a weight the less exact it is.
 //
 // One wave takes a row of up to 2048 elements (8192 where the rows are many), a
 // workgroup of four or sixteen a longer one; few and very long rows are split over

@@ -37,7 +37,10 @@
 // 32K 214 us, 5.6 TB/s of keys and values, bound by memory; one of 32K 19.4 us
 // (12.3 at the rate of a large copy), of which the join is 4 and the chain
 // length - table - rows before the first score about 3; 200 chats of up to 900
-// (12:2 heads of 64) 15.4 us, bound by the tiles of the longest.
+// (12:2 heads of 64) 15.7 us, bound by the tiles of the longest.  More than 32
+// heads a KV head are tiles that each read the keys and values again: 64 of up to 2K
+// take 19 us at 16:1, 26 at 32:1, 29 at 40:1.  Prompts go into pages at the rate of a
+// copy (32K of 4 heads of 128 23.5 us, 5.7 TB/s).
 #include "nsa_launch.h"
 #include "nsa_paged_index.h"
 #include "nsa_tiles.h"
@@ -592,7 +595,8 @@ struct PagedPlan {
 // one where the rows are few and long (one sequence of 32K: 19.9 us, 20.9 with
 // two; 32 of up to 32K: 215, 217).  Where the rows fill the chip and none can
 // be long (1 MiB of keys and values), a workgroup takes a row instead (W = 0):
-// nothing is counted and nothing joined.
+// nothing is counted and nothing joined (200 sequences of up to 900 at 12:2 heads
+// of 64: 16.5 us, and 22.4 under a table of 32K positions, which takes shares).
 static PagedPlan paged_plan(int B, int Hq, int Hkv, int row_bytes, int64_t cap, int cu) {
   PagedPlan p;
   const int G = Hq / Hkv;

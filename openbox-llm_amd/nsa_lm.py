@@ -43,9 +43,9 @@ def add_rms_norm(x, residual, weight, eps=None, out_dtype=None):
     rounded once to the residual's dtype; the norm is taken of the rounded
     sum.  ``y`` is in ``out_dtype`` (default: h's dtype).  ``eps`` None is
     float32's machine epsilon 2^-23 whatever the dtypes, what
-    ``torch.nn.RMSNorm`` adds in float32 and in bfloat16.  Differentiable in x,
-    residual and weight, from y and h; the weight's gradient has the same bits
-    on every run."""
+    ``torch.nn.RMSNorm`` adds in float32 and in bfloat16; with 0 a row of zeros
+    is NaN.  Differentiable in x, residual and weight, from y and h; the
+    weight's gradient has the same bits on every run."""
     f = L.torch_side().add_rms_norm
     if _ops._TIMER is None:
         return f(x, residual, weight, eps, out_dtype)

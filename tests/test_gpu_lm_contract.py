@@ -56,6 +56,7 @@ def test_default_eps_is_rms_norms(dtype, res):
         m.weight.copy_(wd)
         t = m(xd)
     assert ((y.double() - t.double()).abs().cpu() <= 2 * ref.abs() * (half + 14 * U) * (1 + 1e-6)).all()
+    assert nsa_lm.add_rms_norm(torch.zeros_like(xd), r, wd, eps=0.0)[0].isnan().all()      # 0 / 0, as the formula
     q, s, _ = nsa_lm.add_rms_norm_q8(xd, r, wd)
     v = q.cpu().double() * s.cpu().double()[:, None]
     assert ((v - ref).abs() <= torch.maximum(ref.abs() * 2.0 ** -4, s.cpu().double()[:, None] * 2.0 ** -10) +
@@ -218,7 +219,7 @@ def test_a_generation_loop_never_waits_for_the_device():
         caches = m.paged_caches(2, 96, page_size=16)
         lens = [20, 7]
         if busy:
-            for _ in range(100):            # about 0.1 s of work ahead of the loop
+            for _ in range(400):            # about 0.4 s of work ahead of the loop
                 big @ big
         ahead = torch.cuda.Event()
         ahead.record()
@@ -475,3 +476,33 @@ def test_norm_within_one_run_a_thread(rows, D):
     h64 = (x + r).double()
     ref = h64 / torch.sqrt((h64 * h64).mean(-1, keepdim=True) + 1e-5) * w.double()
     assert ((y.cpu().double() - ref).abs() <= ref.abs() * (15 + 7 + 1) * 2.0 ** -24).all()
+
+
+def test_the_c_entry_points_without_an_end():
+    """nsa_paged_append and nsa_paged_attend, called as from C, are the functions
+    over bare pages."""
+    import _nsa_lib as L
+    import nsa_paged
+    dev = require_gpu()
+    lib = L.load()
+    B, Hq, Hkv, D, P, mp, T = 2, 8, 2, 64, 16, 6, 90
+    g = torch.Generator().manual_seed(3)
+    k, v = (torch.randn(B, Hkv, T, D, generator=g).to(BF).to(dev) for _ in range(2))
+    q, kn, vn = (torch.randn(B, h, D, generator=g).to(BF).to(dev) for h in (Hq, Hkv, Hkv))
+    table = torch.randperm(B * mp, generator=g).view(B, mp).to(torch.int32).to(dev)
+    zero, count = torch.zeros(B, dtype=torch.int32, device=dev), torch.tensor([T, 37], dtype=torch.int32, device=dev)
+    want = [torch.zeros(B * mp, Hkv, P, D, device=dev, dtype=BF) for _ in range(2)]
+    n = nsa_paged.paged_append(k, v, *want, table, zero, count)
+    out, n1 = nsa_paged.paged_step(q, kn, vn, *want, table, n)
+    pages = [torch.zeros_like(t) for t in want]
+    lens, lens1, o = torch.empty_like(zero), torch.empty_like(zero), torch.empty_like(q)
+    stream = L.stream_of(q)
+    assert lib.nsa_paged_append(L.ptr(k), L.ptr(v), *map(L.ptr, pages), L.ptr(table), L.ptr(zero), L.ptr(count),
+                                L.ptr(lens), B, Hkv, T, D, P, mp, B * mp, L.NSA_BF16, stream) == 0
+    size = lib.nsa_paged_workspace(B, Hq, Hkv, D, P, mp, L.NSA_BF16, stream)
+    ws = torch.empty(max(16, size), dtype=torch.uint8, device=dev)
+    assert lib.nsa_paged_attend(L.ptr(q), L.ptr(kn), L.ptr(vn), *map(L.ptr, pages), L.ptr(table), L.ptr(lens),
+                                L.ptr(lens1), L.ptr(o), None, L.ptr(ws), ws.numel(), B, Hq, Hkv, D, P, mp, B * mp,
+                                D ** -0.5, L.NSA_BF16, stream) == 0
+    assert torch.equal(lens, n) and torch.equal(lens1, n1) and torch.equal(o, out)
+    assert all(torch.equal(a, b) for a, b in zip(pages, want))
