@@ -566,6 +566,67 @@ int nsa_logprob_fwd(const void* z, const int64_t* target, float* logp, float* en
 int nsa_logprob_bwd(const void* z, const int64_t* target, const float* stat, const float* entropy, const float* dlogp,
                     const float* dent, void* dz, int64_t rows, int V, int dtype, void* stream);
 
+/* ---- residual addition with layer norm ------------------------------------------
+ * Replaces x + branch followed by the norm in Block.forward
+ * (nsa_model.py:449-452) for the reference's own norm:
+ *   h = x + res (float, rounded once to h_dtype),
+ *   y = (h - mean h) / sqrt(mean (h - mean h)^2 + eps) * w + b
+ * over `rows` rows of D elements at any element-aligned address.  res null:
+ * h = x (h is not written, h_dtype = x_dtype).  b (nullable) in w_dtype.  stat
+ * (float [rows][2], nullable): mean and 1 / sqrt(variance + eps), for the backward.
+ * x, h / res, w and y are NSA_F32 or NSA_BF16, each on its own.  D <= 2^24.  The
+ * outputs are buffers of their own: a long row is read after its sum is written. */
+int nsa_lnorm_fwd(const void* x, const void* res, const void* w, const void* b, void* h, void* y, float* stat,
+                  int64_t rows, int D, float eps, int x_dtype, int h_dtype, int w_dtype, int y_dtype, void* stream);
+/* Its backward: dy in y_dtype, dh (nullable) the gradient of h in h_dtype; dx in
+ * x_dtype, dres (nullable: dx serves both) in h_dtype, dw and db (each nullable) in
+ * w_dtype, summed over the rows in an order fixed by the shape; no output overlaps
+ * an input.  workspace: nsa_lnorm_bwd_workspace bytes (0: unsupported shape); not
+ * read where dw and db are null. */
+size_t nsa_lnorm_bwd_workspace(int64_t rows, int D, void* stream);
+int nsa_lnorm_bwd(const void* dy, const void* dh, const void* h, const void* w, const float* stat, void* dx,
+                  void* dres, void* dw, void* db, void* workspace, size_t workspace_bytes, int64_t rows, int D,
+                  int x_dtype, int h_dtype, int w_dtype, int y_dtype, void* stream);
+
+/* ---- embedding ----------------------------------------------------------------
+ * Replaces the token and position embeddings of NSATransformer.forward
+ * (nsa_model.py:455-511):
+ *   out[i] = scale w[tokens[i]] + pw[pos[i]]      (float, rounded once to out_dtype)
+ * for n rows of D elements; w [V][D], pw [P][D] (nullable: no positions).  pos null:
+ * position i % T.  A token or position outside its table adds nothing.
+ * n, V, P < 2^31 - 16, D <= 2^20; any element-aligned addresses. */
+int nsa_embed_fwd(const int64_t* tokens, const int64_t* pos, const void* w, const void* pw, void* out, int64_t n,
+                  int64_t T, int64_t V, int64_t P, int D, float scale, int w_dtype, int pw_dtype, int out_dtype,
+                  void* stream);
+/* The gradient of one table, all V rows of it: dw[v] = scale sum of dy[i] over the i
+ * with index[i] = v, summed in an order fixed by the indices (rows without one: 0);
+ * index outside the table: none.  index null: i % T (n a multiple of T, T <= V).
+ * workspace: nsa_embed_bwd_workspace bytes (0: unsupported shape), `sorted` 0 where
+ * index is null. */
+size_t nsa_embed_bwd_workspace(int64_t n, int D, int sorted);
+int nsa_embed_bwd(const int64_t* index, const void* dy, void* dw, void* workspace, size_t workspace_bytes, int64_t n,
+                  int64_t T, int64_t V, int D, float scale, int dy_dtype, int w_dtype, void* stream);
+
+/* ---- log probabilities from the rows behind the last norm -------------------------
+ * Replaces the LM head with the loss over the vocabulary (nsa_model.py:504-507),
+ * without the logits z = x w^T, x [N][D], w [V][D]:
+ *   lse   ln sum_v e^{z_nv},  logp  z_{n, target[n]} - lse_n (0: target outside 0 .. V-1)
+ * float [N] each; target and logp both null: lse alone.  float rows: float's
+ * precision; bf16 rows: products of bf16, summed in float (float weights are rounded
+ * to bf16 first).  N <= 2^22, V <= 2^28, D <= 65536; any element-aligned addresses.
+ * workspace: nsa_head_fwd_workspace bytes (0: unsupported shape); `aligned` 1 only
+ * where x and w lie on 16 bytes. */
+size_t nsa_head_fwd_workspace(int64_t N, int V, int D, int x_dtype, int w_dtype, int aligned, void* stream);
+int nsa_head_fwd(const void* x, const void* w, const int64_t* target, float* logp, float* lse, void* workspace,
+                 size_t workspace_bytes, int64_t N, int V, int D, int x_dtype, int w_dtype, void* stream);
+/* Its backward, from the forward's logp and lse and their gradients dlogp, dlse
+ * (float [N], each nullable): dx in x_dtype, dw in w_dtype (each nullable), with the
+ * same bits on every run. */
+size_t nsa_head_bwd_workspace(int64_t N, int V, int D, int x_dtype, int w_dtype, int aligned, void* stream);
+int nsa_head_bwd(const void* x, const void* w, const int64_t* target, const float* logp, const float* lse,
+                 const float* dlogp, const float* dlse, void* dx, void* dw, void* workspace, size_t workspace_bytes,
+                 int64_t N, int V, int D, int x_dtype, int w_dtype, void* stream);
+
 /* ---- one new token over a paged key-value cache -------------------------------
  * The generation step of the dense arm (FullAttention, nsa_model.py:377-419;
  * the reference has none).

@@ -109,6 +109,16 @@ SIGNATURES = {
     "nsa_logprob_workspace": (_Z, [_L, _I, _I, _P]),
     "nsa_logprob_fwd": (_I, [_P] * 8 + [_Z, _L, _I, _I, _I, _P]),
     "nsa_logprob_bwd": (_I, [_P] * 7 + [_L, _I, _I, _P]),
+    "nsa_lnorm_fwd": (_I, [_P] * 7 + [_L, _I, _F, _I, _I, _I, _I, _P]),
+    "nsa_lnorm_bwd_workspace": (_Z, [_L, _I, _P]),
+    "nsa_lnorm_bwd": (_I, [_P] * 10 + [_Z, _L, _I, _I, _I, _I, _I, _P]),
+    "nsa_embed_fwd": (_I, [_P] * 5 + [_L] * 4 + [_I, _F, _I, _I, _I, _P]),
+    "nsa_embed_bwd_workspace": (_Z, [_L, _I, _I]),
+    "nsa_embed_bwd": (_I, [_P] * 4 + [_Z, _L, _L, _L, _I, _F, _I, _I, _P]),
+    "nsa_head_fwd_workspace": (_Z, [_L, _I, _I, _I, _I, _I, _P]),
+    "nsa_head_fwd": (_I, [_P] * 6 + [_Z, _L, _I, _I, _I, _I, _P]),
+    "nsa_head_bwd_workspace": (_Z, [_L, _I, _I, _I, _I, _I, _P]),
+    "nsa_head_bwd": (_I, [_P] * 10 + [_Z, _L, _I, _I, _I, _I, _P]),
     "nsa_paged_workspace": (_Z, [_I] * 7 + [_P]),
     "nsa_paged_attend": (_I, [_P] * 11 + [_Z] + [_I] * 7 + [_F, _I, _P]),
     "nsa_paged_attend_max": (_I, [_P] * 11 + [_Z] + [_I] * 8 + [_F, _I, _P]),
@@ -118,7 +128,9 @@ SIGNATURES = {
 
 # entry points that csrc/nsa_torch.cpp calls
 _TORCH_SIDE = ("nsa_norm_fwd", "nsa_norm_bwd", "nsa_norm_bwd_workspace", "nsa_logprob_fwd", "nsa_logprob_bwd",
-               "nsa_logprob_workspace", "nsa_paged_attend_max", "nsa_paged_workspace")
+               "nsa_logprob_workspace", "nsa_paged_attend_max", "nsa_paged_workspace", "nsa_lnorm_fwd", "nsa_lnorm_bwd",
+               "nsa_lnorm_bwd_workspace", "nsa_embed_fwd", "nsa_embed_bwd", "nsa_embed_bwd_workspace", "nsa_head_fwd",
+               "nsa_head_fwd_workspace", "nsa_head_bwd", "nsa_head_bwd_workspace")
 
 _lib = None
 

@@ -1,0 +1,812 @@
+// Log probabilities of tokens from the rows behind the last norm, without the
+// logits.  x [N][D], W [V][D]; z = x W^T exists only as tiles in registers:
+//
+//   lse_n = ln sum_v e^{z_nv},   logp_n = x_n . W_{t_n} - lse_n   (0 where t_n is no token)
+//
+// and with a_n = dlse_n - dlogp_n, b_n = dlogp_n (both without dlogp where t_n is none)
+//
+//   dz_nv = a_n e^{z_nv - lse_n} + b_n [v = t_n],   dx = dz W,   dW = dz^T x.
+//
+// Four products, each on v_mfma_f32_32x32x16_bf16 with float32 sums: z for the
+// log sums (a running maximum and sum in registers), z again for dz, and the two
+// of the gradients.  dz exists for a piece of the vocabulary at a time, rounded once
+// to bf16 as the products' operand (the relative rounding of a probability and of
+// an operand are the same; a sum over the vocabulary or the rows averages it).
+//
+// float32 operands go as three bf16 planes p0 + p1 + p2 = x, |x - p0 - p1 - p2| <=
+// 2^-27 |x|: six products of planes (i + j <= 2) leave out terms below 2^-26 of the
+// product, less than float32's own rounding.  A bf16 operand beside float32 rows is
+// one plane; float32 weights beside bf16 rows are rounded to bf16 first.
+//
+// Layout: an operand is read either along its rows (the contraction runs along
+// memory) into a [rows][64] tile, or across them into a [64][columns] tile that
+// the transposed LDS reads turn; no transposed copy is made.  Results have the
+// 32-row tile's rows permuted (perm32), so that a lane holds eight neighbouring
+// elements of an output row.
+#include <algorithm>
+
+#include "nsa_launch.h"
+#include "nsa_rows.h"
+#include "nsa_tile32.h"
+
+namespace nsa {
+
+constexpr int64_t kHeadRows = 1 << 22;       // most rows of x
+constexpr int kHeadVocab = 1 << 28;
+constexpr int kHeadWide = 1 << 16;           // widest row
+constexpr size_t kHeadPiece = 512u << 20;    // bytes of dz held at a time
+constexpr int64_t kHeadPieceMost = 1 << 20;  // most tokens of a piece: offsets within a stage have 32 bits
+constexpr int kStep = 64;                    // contraction elements of a stage
+
+__device__ const uint4 g_head_zero = {0, 0, 0, 0};   // what elements past an end are read from
+
+// An operand of a product: bf16 planes; ROWS: [rows][ld], contraction along a row;
+// otherwise [contraction][ld].
+struct HeadOperand {
+  const bf16* p;
+  int64_t plane;   // elements between planes
+  int64_t ld;      // elements between rows, a multiple of 8
+  int rows;        // rows (ROWS) or columns, for clamping: what lies past them is never stored
+};
+
+// One product C[m][n] = sum over plane pairs and k of A[m][k] B[n][k].
+struct HeadProduct {
+  HeadOperand a, b;
+  int k0, k1;      // contraction range of this workgroup; k0 a multiple of kStep
+  int pa, pb;      // planes
+};
+
+// Plane pairs (of a, of b) in the order they are added, the small ones first.  The
+// rows' side b has three planes where a has.
+__device__ __forceinline__ int head_pairs(int pa, int pb) { return pb == 1 ? 1 : pa == 1 ? 3 : 6; }
+__device__ __forceinline__ void head_pair(int pa, int pb, int i, int& x, int& y) {
+  if (pb == 1) {
+    x = y = 0;
+  } else if (pa == 1) {   // (0,2) (0,1) (0,0)
+    x = 0;
+    y = 2 - i;
+  } else {                // (2,0) (1,1) (0,2) (1,0) (0,1) (0,0)
+    x = i == 0 ? 2 : i == 1 || i == 3 ? 1 : 0;
+    y = i == 2 ? 2 : i == 1 || i == 4 ? 1 : 0;
+  }
+}
+
+// A stage of one operand: T rows (ROWS) or columns x kStep contraction elements.
+// 16-byte chunks swizzled so that 16 neighbouring lanes' 16-byte reads, or the
+// transposed reads' 32-byte pieces of four rows, meet every bank once.
+template <int T, bool ROWS>
+struct HeadTile {
+  static constexpr int kElems = T * kStep;
+  static constexpr int kLoads = T * 8 / 256;   // 16-byte requests a thread
+  static constexpr int kCpr = ROWS ? 8 : T / 8;
+  static_assert(T % 32 == 0 && (ROWS || T >= 128), "a tile of whole requests");
+  static __device__ __forceinline__ int key(int r) {
+    return ROWS ? (r >> 1) & 7 : 4 * (r & 3) + ((r >> 2) & 3);
+  }
+
+  uint32_t off[kLoads];   // bytes from the stage's base
+
+  // rows (columns) first .. first + T - 1 of the operand
+  __device__ __forceinline__ void aim(const HeadOperand& o, int first, int tid) {
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int P = j * 256 + tid, r = P / kCpr, c = (P % kCpr) ^ key(r);
+      if (ROWS) {
+        const int last = o.rows - 1 - first;   // >= 0
+        off[j] = (uint32_t)((r < last ? r : last) * o.ld * 2 + c * 16);
+      } else {
+        const int col = first + 8 * c;
+        off[j] = (uint32_t)(r * o.ld * 2 + (col < o.rows ? 8 * c : 0) * 2);
+      }
+    }
+  }
+  // Request elements k .. k + 63 of plane `pl` (fewer before k1: the rest as zeros).
+  __device__ __forceinline__ void request(const HeadOperand& o, int first, int pl, int k, int k1, bf16* lds,
+                                          int tid) const {
+    const bf16* base = o.p + pl * o.plane + (ROWS ? (int64_t)first * o.ld + k : (int64_t)k * o.ld + first);
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    if (k1 - k >= kStep) {
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) lds_dma16_sbase(base, off[j], lds + (j * 256 + 64 * w) * 8);
+    } else {
+      const int left = k1 - k;
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int P = j * 256 + tid, r = P / kCpr, c = (P % kCpr) ^ key(r);
+        const bool in = ROWS ? 8 * c < left : r < left;
+        const void* src = in ? reinterpret_cast<const char*>(base) + off[j] : reinterpret_cast<const char*>(&g_head_zero);
+        lds_dma16(src, lds + (j * 256 + 64 * w) * 8);
+      }
+    }
+  }
+  // Fragment of the 32-row tile that starts at row r0: row r0 + m (PERM: perm32(m)),
+  // contraction elements 16 s + 8 h .. + 7.
+  template <bool PERM>
+  static __device__ __forceinline__ bf16x8 frag(const bf16* lds, int r0, int s, int lane) {
+    if constexpr (ROWS) {
+      const int m = lane & 31, h = lane >> 5;
+      const int r = r0 + (PERM ? perm32(m) : m);
+      return *reinterpret_cast<const bf16x8*>(lds + r * kStep + (((2 * s + h) ^ key(r)) << 3));
+    } else {
+      typedef short s16x8 __attribute__((ext_vector_type(8)));
+      const int g = lane >> 4, jj = (lane >> 2) & 3;
+      int q = lane & 3;
+      if (PERM) q = ((q & 1) << 1) | (q >> 1);   // perm32 swaps bits 2 and 3 of the row
+      const int col = r0 + 16 * (g & 1) + 4 * q;
+      s16x4 v[2];
+#pragma unroll
+      for (int rd = 0; rd < 2; ++rd) {
+        const int r = 16 * s + 8 * (g >> 1) + 4 * rd + jj;
+        v[rd] = lds_read_tr16(lds + r * T + (((col >> 3) ^ key(r)) << 3) + (col & 7));
+      }
+      const s16x8 f = (s16x8){v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
+      return __builtin_bit_cast(bf16x8, f);
+    }
+  }
+};
+
+// Tile shape: TM x TN of the result over WM x WN waves (four), NS stages.
+template <int TM_, int TN_, int WM_, int WN_, int NS_>
+struct HeadShape {
+  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, NS = NS_;
+  static constexpr int MT = TM / WM / 32, NT = TN / WN / 32;   // 32 x 32 tiles of a wave
+  static_assert(WM * WN == 4 && MT >= 1 && NT >= 1 && NS >= 2, "four waves");
+};
+
+// The product of tiles m = m_first, m_first + m_step, .. < m_tiles (TM rows each) with
+// the tile at column n0; done(m, acc) takes each result.  All stages of all tiles
+// are one pipeline: while a tile is finished, the next one's stages are under way.
+template <class S, bool AROWS, bool BROWS, typename Done>
+__device__ __forceinline__ void head_product(const HeadProduct& pr, int m_first, int m_step, int m_tiles, int n0,
+                                             Done done) {
+  using TA = HeadTile<S::TM, AROWS>;
+  using TB = HeadTile<S::TN, BROWS>;
+  constexpr int kLoads = TA::kLoads + TB::kLoads;
+  __shared__ __align__(1024) bf16 sa[S::NS][TA::kElems];
+  __shared__ __align__(1024) bf16 sb[S::NS][TB::kElems];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = (w % S::WM) * S::MT * 32, wn = (w / S::WM) * S::NT * 32;
+  const int ksteps = (pr.k1 - pr.k0 + kStep - 1) / kStep;
+  const int pairs = head_pairs(pr.pa, pr.pb);
+  const int ntile = m_first < m_tiles ? (m_tiles - m_first + m_step - 1) / m_step : 0;
+  const int64_t total = (int64_t)ntile * pairs * ksteps;
+  // the request's place: tile, plane pair, step
+  TA ta;
+  TB tb;
+  int rm = m_first, rp = 0, rk = 0;
+  ta.aim(pr.a, rm * S::TM, tid);
+  tb.aim(pr.b, n0, tid);
+  int64_t asked = 0;
+  auto request = [&]() {
+    int x, y;
+    head_pair(pr.pa, pr.pb, rp, x, y);
+    const int k = pr.k0 + rk * kStep, st = (int)(asked % S::NS);
+    ta.request(pr.a, rm * S::TM, x, k, pr.k1, sa[st], tid);
+    tb.request(pr.b, n0, y, k, pr.k1, sb[st], tid);
+    ++asked;
+    if (++rk == ksteps) {
+      rk = 0;
+      if (++rp == pairs) {
+        rp = 0;
+        rm += m_step;
+        if (rm < m_tiles) ta.aim(pr.a, rm * S::TM, tid);
+      }
+    }
+  };
+  for (int i = 0; i < S::NS - 1 && asked < total; ++i) request();
+  f32x16 acc[S::MT][S::NT];
+  int64_t it = 0;
+  for (int m = m_first; m < m_tiles; m += m_step) {
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+      for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+    for (int s = 0; s < pairs * ksteps; ++s, ++it) {
+      // stage `it` has arrived when only the NS - 2 younger ones are outstanding
+      if (S::NS > 2 && it + S::NS - 2 < total)
+        vm_wait<(S::NS - 2) * kLoads>();
+      else
+        vm_wait<0>();
+      __syncthreads();   // everybody's part of it has; and nobody reads stage it - 1 any more
+      if (asked < total) request();
+      const bf16* A = sa[it % S::NS];
+      const bf16* B = sb[it % S::NS];
+#pragma unroll
+      for (int ks = 0; ks < kStep / 16; ++ks) {
+        bf16x8 fa[S::MT], fb[S::NT];
+#pragma unroll
+        for (int i = 0; i < S::MT; ++i) fa[i] = TA::template frag<true>(A, wm + 32 * i, ks, lane);
+#pragma unroll
+        for (int j = 0; j < S::NT; ++j) fb[j] = TB::template frag<false>(B, wn + 32 * j, ks, lane);
+#pragma unroll
+        for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+          for (int j = 0; j < S::NT; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+      }
+    }
+    done(m, wm, wn, acc);
+  }
+}
+
+// Workgroup -> (tile of x's rows, one of `split` lanes over the vocabulary's tiles).
+// Workgroups go round-robin over the 8 XCDs: neighbours on one XCD share a tile of
+// rows and walk adjacent vocabulary tiles, so that its L2 serves most of both.
+struct HeadGrid {
+  int n_tiles, split, m_tiles;
+};
+__device__ __forceinline__ bool head_place(const HeadGrid& g, int bid, int& n, int& lane) {
+  if (g.n_tiles >= 8) {
+    const int xcd = bid & 7, slot = bid >> 3;
+    n = (slot / g.split) * 8 + xcd;
+    lane = slot % g.split;
+  } else {
+    n = bid % g.n_tiles;
+    lane = bid / g.n_tiles;
+  }
+  return n < g.n_tiles;
+}
+
+struct HeadFwd {
+  HeadProduct pr;    // a: weights, b: rows
+  HeadGrid g;
+  float2* part;      // [split][N]: maximum (log2 units) and sum of 2^(z - maximum)
+  int N, V;
+};
+
+// Log sums over this workgroup's share of the vocabulary.  A lane holds one row of
+// x for each of its NT tiles and 16 MT logits of it at a time.
+template <class S>
+__global__ __launch_bounds__(256, 1) void k_head_fwd(const HeadFwd a) {
+  int nt, part;
+  if (!head_place(a.g, (int)blockIdx.x, nt, part)) return;
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  float m[S::NT], l[S::NT];
+#pragma unroll
+  for (int j = 0; j < S::NT; ++j) m[j] = kMaskScore, l[j] = 0.0f;
+  head_product<S, true, true>(
+      a.pr, part, a.g.split, a.g.m_tiles, nt * S::TN, [&](int mt, int wm, int wn, f32x16(&acc)[S::MT][S::NT]) {
+        const int v0 = mt * S::TM + wm + 8 * h;
+        if (mt * S::TM + S::TM > a.V) {   // past the vocabulary: no weight
+#pragma unroll
+          for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const bool out = v0 + 32 * i + acc_elem(0, r) >= a.V;
+#pragma unroll
+              for (int j = 0; j < S::NT; ++j)
+                if (out) acc[i][j][r] = -__builtin_inff();
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < S::NT; ++j) {
+          float t = acc[0][j][0];
+#pragma unroll
+          for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) t = fmaxf(t, acc[i][j][r]);
+          const float mn = fmaxf(m[j], t * kLog2e);
+          float s = 0.0f;
+#pragma unroll
+          for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s += fast_exp2(fmaf(acc[i][j][r], kLog2e, -mn));
+          l[j] = l[j] * fast_exp2(m[j] - mn) + s;
+          m[j] = mn;
+        }
+      });
+  // the halves of a wave, then the waves along the vocabulary
+  __shared__ float2 st[S::WM][S::TN];
+  const int w = threadIdx.x >> 6, wmi = w % S::WM, wn = (w / S::WM) * S::NT * 32;
+#pragma unroll
+  for (int j = 0; j < S::NT; ++j) {
+    const float mo = __shfl_xor(m[j], 32, kWave), lo = __shfl_xor(l[j], 32, kWave);
+    const float mx = fmaxf(m[j], mo);
+    const float s = l[j] * fast_exp2(m[j] - mx) + lo * fast_exp2(mo - mx);
+    if (h == 0) st[wmi][wn + 32 * j + (lane & 31)] = make_float2(mx, s);
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < S::TN; c += 256) {
+    const int n = nt * S::TN + c;
+    float mx = kMaskScore, s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < S::WM; ++i) mx = fmaxf(mx, st[i][c].x);
+#pragma unroll
+    for (int i = 0; i < S::WM; ++i) s += st[i][c].y * fast_exp2(st[i][c].x - mx);
+    if (n < a.N) a.part[(int64_t)part * a.N + n] = make_float2(mx, s);
+  }
+}
+
+// Joins the shares and takes the target's own product: a wave a row.
+struct HeadJoin {
+  const float2* part;
+  const void *x, *w;
+  const int64_t* target;   // or null
+  float *logp, *lse;
+  int64_t N;
+  int split, V, D;
+  bool x_bf16, w_bf16, w_round;   // w_round: float32 weights taken as bf16
+};
+__global__ __launch_bounds__(256) void k_head_join(const HeadJoin a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (n >= a.N) return;
+  float m = kMaskScore, l = 0.0f;
+  bool nan = false;
+  for (int s = lane; s < a.split; s += kWave) {
+    const float2 p = a.part[(int64_t)s * a.N + n];
+    const float mx = fmaxf(m, p.x);
+    l = l * fast_exp2(m - mx) + p.y * fast_exp2(p.x - mx);
+    m = mx;
+  }
+  const float mx = wave_max(m);
+  nan = l != l;
+  l = wave_sum(l * fast_exp2(m - mx));
+  if (__any(nan)) l = __builtin_nanf("");
+  const float lse = (mx + __log2f(l)) * kLn2;
+  if (a.target != nullptr) {
+    const int64_t t = a.target[n];
+    float dot = 0.0f;
+    const bool real = t >= 0 && t < a.V;
+    if (real) {
+      for (int c = 8 * lane; c < a.D; c += 8 * kWave) {
+        float u[8], v[8];
+        load_run8_of(a.x, a.x_bf16, n * a.D + c, a.D - c, u);
+        load_run8_of(a.w, a.w_bf16, t * a.D + c, a.D - c, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dot += u[j] * (a.w_round ? (float)(bf16)v[j] : v[j]);
+      }
+      dot = wave_sum(dot);
+    }
+    if (lane == 0) a.logp[n] = real ? dot - lse : 0.0f;
+  }
+  if (lane == 0) a.lse[n] = lse;
+}
+
+// dz of a piece of the vocabulary, as the gradients' operand
+struct HeadDz {
+  HeadProduct pr;
+  HeadGrid g;
+  const float *lse, *dlogp, *dlse;   // dlogp, dlse: or null
+  const int64_t* target;             // or null
+  bf16* dz;                          // [planes][N][ld]
+  int64_t ld, plane;
+  int N, V, v0;                      // the piece starts at token v0 (V: of the whole vocabulary)
+  int vocab;                         // ... and has so many
+  int planes;
+};
+__device__ __forceinline__ bool head_real(const int64_t* target, int64_t n, int V) {
+  return target != nullptr && target[n] >= 0 && target[n] < V;
+}
+template <int PLANES>
+__device__ __forceinline__ void store_planes(bf16* p, int64_t plane, float (&v)[8]) {
+#pragma unroll
+  for (int q = 0; q < PLANES; ++q) {
+    bf16x8 o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      o[j] = (bf16)v[j];
+      v[j] -= (float)o[j];
+    }
+    *reinterpret_cast<bf16x8*>(p + q * plane) = o;
+  }
+}
+template <class S, int PLANES>
+__global__ __launch_bounds__(256, 1) void k_head_dz(const HeadDz a) {
+  int nt, part;
+  if (!head_place(a.g, (int)blockIdx.x, nt, part)) return;
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  const int wn0 = ((threadIdx.x >> 6) / S::WM) * S::NT * 32;
+  float off[S::NT], co[S::NT];   // dz = co 2^(z log2 e - off)
+#pragma unroll
+  for (int j = 0; j < S::NT; ++j) {
+    const int n = nt * S::TN + wn0 + 32 * j + (lane & 31);
+    off[j] = co[j] = 0.0f;
+    if (n < a.N) {
+      off[j] = a.lse[n] * kLog2e;
+      co[j] = a.dlse != nullptr ? a.dlse[n] : 0.0f;
+      if (a.dlogp != nullptr && head_real(a.target, n, a.V)) co[j] -= a.dlogp[n];
+    }
+  }
+  head_product<S, true, true>(
+      a.pr, part, a.g.split, a.g.m_tiles, nt * S::TN, [&](int mt, int wm, int wn, f32x16(&acc)[S::MT][S::NT]) {
+#pragma unroll
+        for (int j = 0; j < S::NT; ++j) {
+          const int n = nt * S::TN + wn + 32 * j + (lane & 31);
+          if (n >= a.N) continue;
+#pragma unroll
+          for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+            for (int r0 = 0; r0 < 16; r0 += 8) {
+              const int v = mt * S::TM + wm + 32 * i + acc_elem(h, r0);
+              float d[8];
+#pragma unroll
+              for (int r = 0; r < 8; ++r) {
+                d[r] = co[j] * fast_exp2(fmaf(acc[i][j][r0 + r], kLog2e, -off[j]));
+                if (v + r >= a.vocab) d[r] = 0.0f;
+              }
+              store_planes<PLANES>(a.dz + (int64_t)n * a.ld + v, a.plane, d);
+            }
+        }
+      });
+}
+
+// The target's own element, where the piece has it: a p_t + b.
+template <int PLANES>
+__global__ __launch_bounds__(256) void k_head_target(const HeadDz a, const float* logp) {
+  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (n >= a.N || a.dlogp == nullptr || !head_real(a.target, n, a.V)) return;
+  const int64_t v = a.target[n] - a.v0;
+  if (v < 0 || v >= a.vocab) return;
+  const float b = a.dlogp[n], dl = a.dlse != nullptr ? a.dlse[n] : 0.0f, lp = logp[n];
+  // (dlse - b) p + b with 1 - p from expm1: p near 1 leaves no digits in 1 - p otherwise
+  float d = dl * expf(lp) - b * expm1f(lp);
+  bf16* p = a.dz + n * a.ld + v;
+#pragma unroll
+  for (int q = 0; q < PLANES; ++q) {
+    const bf16 o = (bf16)d;
+    p[q * a.plane] = o;
+    d -= (float)o;
+  }
+}
+
+// dx (rows of x on n, columns of W on m) and dW's parts (tokens on n, columns of x on m)
+struct HeadGrad {
+  HeadProduct pr;
+  void* out;             // [n][D]: float32 or, out_bf16, bf16
+  const float* add;      // float32 of the same shape to add, or null
+  int64_t part;          // elements between the parts of the contraction (blockIdx.z)
+  int k_part;            // contraction elements a part, a multiple of kStep
+  int N, D, m_tiles, n_tiles;
+  bool out_bf16;
+};
+template <class S, bool BROWS>
+__global__ __launch_bounds__(256, 1) void k_head_grad(const HeadGrad a) {
+  const int bid = (int)xcd_remap(blockIdx.x, gridDim.x);
+  const int mt = bid % a.m_tiles, nt = bid / a.m_tiles;
+  HeadProduct pr = a.pr;
+  pr.k0 = (int)blockIdx.z * a.k_part;
+  pr.k1 = pr.k1 < pr.k0 + a.k_part ? pr.k1 : pr.k0 + a.k_part;
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  const int64_t at = (int64_t)blockIdx.z * a.part;
+  head_product<S, false, BROWS>(
+      pr, mt, 1, mt + 1, nt * S::TN, [&](int m, int wm, int wn, f32x16(&acc)[S::MT][S::NT]) {
+#pragma unroll
+        for (int j = 0; j < S::NT; ++j) {
+          const int64_t n = nt * S::TN + wn + 32 * j + (lane & 31);
+          if (n >= a.N) continue;
+#pragma unroll
+          for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+            for (int r0 = 0; r0 < 16; r0 += 8) {
+              const int d = m * S::TM + wm + 32 * i + acc_elem(h, r0);
+              if (d >= a.D) continue;
+              float v[8];
+#pragma unroll
+              for (int r = 0; r < 8; ++r) v[r] = acc[i][j][r0 + r];
+              if (a.add != nullptr) {
+                float u[8];
+                load_run8(a.add + n * a.D + d, a.D - d, u);
+#pragma unroll
+                for (int r = 0; r < 8; ++r) v[r] += u[r];
+              }
+              if (a.out_bf16)
+                store_run8(static_cast<bf16*>(a.out) + at + n * a.D + d, a.D - d, v);
+              else
+                store_run8(static_cast<float*>(a.out) + at + n * a.D + d, a.D - d, v);
+            }
+        }
+      });
+}
+
+// out[i] = sum over the parts, in order
+__global__ __launch_bounds__(256) void k_head_sum(const float* part, int64_t stride, int nparts, void* out, bool bf,
+                                                  int64_t n) {
+  for (int64_t i = 8 * ((int64_t)blockIdx.x * 256 + threadIdx.x); i < n; i += 8 * 256 * (int64_t)gridDim.x) {
+    float s[8], v[8];
+    load_run8(part + i, (int)std::min<int64_t>(8, n - i), s);
+    for (int p = 1; p < nparts; ++p) {
+      load_run8(part + p * stride + i, (int)std::min<int64_t>(8, n - i), v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] += v[j];
+    }
+    if (bf)
+      store_run8(static_cast<bf16*>(out) + i, (int)std::min<int64_t>(8, n - i), s);
+    else
+      store_run8(static_cast<float*>(out) + i, (int)std::min<int64_t>(8, n - i), s);
+  }
+}
+
+// Rows as bf16 planes with a pitch of ld: [planes][rows][ld], zeros past a row.
+template <int PLANES>
+__global__ __launch_bounds__(256) void k_head_pack(const void* x, bool x_bf16, bf16* out, int64_t rows, int D, int ld) {
+  const int runs = ld / 8;
+  const int64_t total = rows * runs, plane = rows * ld;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / runs;
+    const int c = (int)(i % runs) * 8;
+    float v[8];
+    load_run8_of(x, x_bf16, r * D + c, D - c, v);
+    store_planes<PLANES>(out + r * ld + c, plane, v);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+using HeadBig = HeadShape<256, 256, 2, 2, 2>;
+using HeadMid = HeadShape<128, 128, 2, 2, 3>;
+using HeadFew = HeadShape<128, 32, 4, 1, 4>;
+
+static bool head_type(int dtype) { return dtype == NSA_F32 || dtype == NSA_BF16; }
+static bool head_shape_ok(int64_t N, int V, int D) {
+  return N >= 0 && N <= kHeadRows && V >= 1 && V <= kHeadVocab && D >= 1 && D <= kHeadWide;
+}
+static size_t up16(size_t n) { return (n + 255) / 256 * 256; }
+
+// How the operands lie: as given, or packed (planes, padded rows).
+struct HeadLayout {
+  bool pack_x, pack_w;
+  int px, pw, ld;               // planes; pitch of a packed row
+  size_t x_bytes, w_bytes;      // of the packed copies
+};
+static HeadLayout head_layout(int64_t N, int V, int D, const void* x, const void* w, int x_dtype, int w_dtype) {
+  HeadLayout l;
+  const bool wide = x_dtype == NSA_F32;
+  l.px = wide ? 3 : 1;
+  l.pw = wide && w_dtype == NSA_F32 ? 3 : 1;
+  l.ld = (D + 63) / 64 * 64;
+  // rows are requested in aligned pieces of 16 bytes
+  l.pack_x = wide || D % 8 != 0 || reinterpret_cast<uintptr_t>(x) % 16 != 0;
+  l.pack_w = w_dtype == NSA_F32 || D % 8 != 0 || reinterpret_cast<uintptr_t>(w) % 16 != 0;
+  l.x_bytes = l.pack_x ? up16((size_t)l.px * N * l.ld * 2) : 0;
+  l.w_bytes = l.pack_w ? up16((size_t)l.pw * V * l.ld * 2) : 0;
+  return l;
+}
+static void head_pack(const void* x, int dtype, void* out, int64_t rows, int D, int ld, int planes, hipStream_t s) {
+  const int64_t blocks = (rows * (ld / 8) + 255) / 256;
+  const unsigned grid = (unsigned)(blocks < 65536 ? blocks : 65536);
+  if (planes == 3)
+    k_head_pack<3><<<grid, 256, 0, s>>>(x, dtype == NSA_BF16, static_cast<bf16*>(out), rows, D, ld);
+  else
+    k_head_pack<1><<<grid, 256, 0, s>>>(x, dtype == NSA_BF16, static_cast<bf16*>(out), rows, D, ld);
+}
+
+// Tile of the product over the vocabulary: 256 x 256 where that gives every compute
+// unit a tile, 32 rows of x where there are no more, 128 x 128 between.
+enum { kFew, kMid, kBig };
+static int head_kind(int64_t N, int V, int cu) {
+  if (N <= 32) return kFew;
+  return ((N + 255) / 256) * ((V + 255) / 256) >= cu ? kBig : kMid;
+}
+template <class S>
+static HeadGrid head_grid(int64_t N, int vocab, int cu) {
+  HeadGrid g;
+  g.n_tiles = (int)((N + S::TN - 1) / S::TN);
+  g.m_tiles = (vocab + S::TM - 1) / S::TM;
+  const int want = (4 * cu + g.n_tiles - 1) / g.n_tiles;
+  g.split = want < g.m_tiles ? want : g.m_tiles;
+  return g;
+}
+static unsigned head_blocks(const HeadGrid& g) {
+  return (unsigned)((g.n_tiles >= 8 ? (g.n_tiles + 7) / 8 * 8 : g.n_tiles) * (int64_t)g.split);
+}
+template <typename F>
+static auto head_as(int kind, F f) {
+  if (kind == kFew) return f(HeadFew{});
+  if (kind == kMid) return f(HeadMid{});
+  return f(HeadBig{});
+}
+
+// The backward's pieces: tokens of one, and parts of its contraction over the rows
+struct HeadPlan {
+  int piece;            // tokens of a piece, a multiple of 256
+  int w_parts, k_part;  // dW: parts, rows of x each
+  size_t dz, acc, part; // bytes
+};
+static HeadPlan head_plan(int64_t N, int V, int D, int planes, bool x_bf16, int cu) {
+  HeadPlan p;
+  const int64_t all = ((int64_t)V + 255) / 256 * 256;
+  int64_t fit = (int64_t)(kHeadPiece / ((size_t)N * 2 * planes)) / 256 * 256;
+  fit = fit < 256 ? 256 : fit < kHeadPieceMost ? fit : kHeadPieceMost;
+  const int64_t pieces = (all + fit - 1) / fit;
+  p.piece = (int)(((all + pieces - 1) / pieces + 255) / 256 * 256);
+  const int64_t tiles = (int64_t)(p.piece / 256) * ((D + 255) / 256);
+  int64_t parts = (cu + tiles - 1) / tiles;
+  const int64_t most = (N + 1023) / 1024;
+  if (parts > most) parts = most;
+  p.k_part = (int)(((N + parts - 1) / parts + kStep - 1) / kStep * kStep);
+  p.w_parts = (int)((N + p.k_part - 1) / p.k_part);
+  p.dz = up16((size_t)planes * N * p.piece * 2);
+  p.acc = pieces > 1 && x_bf16 ? up16((size_t)N * D * 4) : 0;
+  p.part = p.w_parts > 1 ? up16((size_t)p.w_parts * p.piece * D * 4) : 0;
+  return p;
+}
+
+}  // namespace nsa
+
+// The workspaces cover any alignment of the operands: a packed copy where the
+// dtypes or D alone need none is only made for pointers off 16 bytes.
+extern "C" size_t nsa_head_fwd_workspace(int64_t N, int V, int D, int x_dtype, int w_dtype, int aligned, void* stream) {
+  using namespace nsa;
+  if (!head_shape_ok(N, V, D) || !head_type(x_dtype) || !head_type(w_dtype)) return 0;
+  if (N == 0) return 16;
+  const void* at = reinterpret_cast<const void*>(aligned ? 16 : 1);
+  const HeadLayout l = head_layout(N, V, D, at, at, x_dtype, w_dtype);
+  const int cu = device_cu_count(static_cast<hipStream_t>(stream));
+  const int split = head_as(head_kind(N, V, cu), [&](auto s) { return head_grid<decltype(s)>(N, V, cu).split; });
+  return l.x_bytes + l.w_bytes + (size_t)split * N * sizeof(float2);
+}
+
+extern "C" int nsa_head_fwd(const void* x, const void* w, const int64_t* target, float* logp, float* lse,
+                            void* workspace, size_t workspace_bytes, int64_t N, int V, int D, int x_dtype, int w_dtype,
+                            void* stream) {
+  using namespace nsa;
+  NSA_CHECK(head_shape_ok(N, V, D), NSA_ERR_SHAPE);
+  NSA_CHECK(head_type(x_dtype) && head_type(w_dtype), NSA_ERR_DTYPE);
+  if (N == 0) return NSA_OK;
+  NSA_CHECK(x != nullptr && w != nullptr && lse != nullptr && (target == nullptr) == (logp == nullptr), NSA_ERR_ARG);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const int cu = device_cu_count(s);
+  const HeadLayout l = head_layout(N, V, D, x, w, x_dtype, w_dtype);
+  return head_as(head_kind(N, V, cu), [&](auto sh) -> int {
+    using S = decltype(sh);
+    const HeadGrid g = head_grid<S>(N, V, cu);
+    NSA_CHECK(workspace != nullptr &&
+                  workspace_bytes >= l.x_bytes + l.w_bytes + (size_t)g.split * N * sizeof(float2),
+              NSA_ERR_WORKSPACE);
+    char* ws = static_cast<char*>(workspace);
+    bf16* xp = reinterpret_cast<bf16*>(ws);
+    bf16* wp = reinterpret_cast<bf16*>(ws + l.x_bytes);
+    float2* part = reinterpret_cast<float2*>(ws + l.x_bytes + l.w_bytes);
+    if (l.pack_x) head_pack(x, x_dtype, xp, N, D, l.ld, l.px, s);
+    if (l.pack_w) head_pack(w, w_dtype, wp, V, D, l.ld, l.pw, s);
+    HeadFwd a;
+    a.pr.a = {l.pack_w ? wp : static_cast<const bf16*>(w), (int64_t)V * l.ld, l.pack_w ? l.ld : D, V};
+    a.pr.b = {l.pack_x ? xp : static_cast<const bf16*>(x), N * l.ld, l.pack_x ? l.ld : D, (int)N};
+    a.pr.k0 = 0;
+    a.pr.k1 = D;
+    a.pr.pa = l.pw;
+    a.pr.pb = l.px;
+    a.g = g;
+    a.part = part;
+    a.N = (int)N;
+    a.V = V;
+    k_head_fwd<S><<<head_blocks(g), 256, 0, s>>>(a);
+    const HeadJoin j{part, x, w, target, logp, lse, N, g.split, V, D, x_dtype == NSA_BF16, w_dtype == NSA_BF16,
+                     x_dtype == NSA_BF16 && w_dtype == NSA_F32};
+    k_head_join<<<(unsigned)((N + 3) / 4), 256, 0, s>>>(j);
+    return nsa_launch_status();
+  });
+}
+
+extern "C" size_t nsa_head_bwd_workspace(int64_t N, int V, int D, int x_dtype, int w_dtype, int aligned, void* stream) {
+  using namespace nsa;
+  if (!head_shape_ok(N, V, D) || !head_type(x_dtype) || !head_type(w_dtype)) return 0;
+  if (N == 0) return 16;
+  const void* at = reinterpret_cast<const void*>(aligned ? 16 : 1);
+  const HeadLayout l = head_layout(N, V, D, at, at, x_dtype, w_dtype);
+  const HeadPlan p = head_plan(N, V, D, l.px, x_dtype == NSA_BF16, device_cu_count(static_cast<hipStream_t>(stream)));
+  return l.x_bytes + l.w_bytes + p.dz + p.acc + p.part;
+}
+
+extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target, const float* logp, const float* lse,
+                            const float* dlogp, const float* dlse, void* dx, void* dw, void* workspace,
+                            size_t workspace_bytes, int64_t N, int V, int D, int x_dtype, int w_dtype, void* stream) {
+  using namespace nsa;
+  NSA_CHECK(head_shape_ok(N, V, D) && N >= 1, NSA_ERR_SHAPE);
+  NSA_CHECK(head_type(x_dtype) && head_type(w_dtype), NSA_ERR_DTYPE);
+  NSA_CHECK(x != nullptr && w != nullptr && lse != nullptr && (dx != nullptr || dw != nullptr), NSA_ERR_ARG);
+  NSA_CHECK(dlogp == nullptr || (target != nullptr && logp != nullptr), NSA_ERR_ARG);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const int cu = device_cu_count(s);
+  const HeadLayout l = head_layout(N, V, D, x, w, x_dtype, w_dtype);
+  const HeadPlan p = head_plan(N, V, D, l.px, x_dtype == NSA_BF16, cu);
+  NSA_CHECK(workspace != nullptr && workspace_bytes >= l.x_bytes + l.w_bytes + p.dz + p.acc + p.part,
+            NSA_ERR_WORKSPACE);
+  char* ws = static_cast<char*>(workspace);
+  bf16* xp = reinterpret_cast<bf16*>(ws);
+  ws += l.x_bytes;
+  bf16* wp = reinterpret_cast<bf16*>(ws);
+  ws += l.w_bytes;
+  bf16* dz = reinterpret_cast<bf16*>(ws);
+  ws += p.dz;
+  float* acc = reinterpret_cast<float*>(ws);
+  ws += p.acc;
+  float* part = reinterpret_cast<float*>(ws);
+  if (l.pack_x) head_pack(x, x_dtype, xp, N, D, l.ld, l.px, s);
+  if (l.pack_w) head_pack(w, w_dtype, wp, V, D, l.ld, l.pw, s);
+  const int ldx = l.pack_x ? l.ld : D, ldw = l.pack_w ? l.ld : D;
+  const bf16* X = l.pack_x ? xp : static_cast<const bf16*>(x);
+  const bf16* W = l.pack_w ? wp : static_cast<const bf16*>(w);
+  const int64_t x_plane = N * (int64_t)l.ld, w_plane = (int64_t)V * l.ld, z_plane = N * (int64_t)p.piece;
+  for (int v0 = 0; v0 < V; v0 += p.piece) {
+    const int vocab = V - v0 < p.piece ? V - v0 : p.piece;
+    HeadDz z;
+    z.pr.a = {W + (int64_t)v0 * ldw, w_plane, ldw, vocab};
+    z.pr.b = {X, x_plane, ldx, (int)N};
+    z.pr.k0 = 0;
+    z.pr.k1 = D;
+    z.pr.pa = l.pw;
+    z.pr.pb = l.px;
+    z.lse = lse;
+    z.dlogp = dlogp;
+    z.dlse = dlse;
+    z.target = target;
+    z.dz = dz;
+    z.ld = p.piece;
+    z.plane = z_plane;
+    z.N = (int)N;
+    z.V = V;
+    z.v0 = v0;
+    z.vocab = vocab;
+    z.planes = l.px;
+    head_as(head_kind(N, vocab, cu), [&](auto sh) {
+      using S = decltype(sh);
+      z.g = head_grid<S>(N, vocab, cu);
+      if (l.px == 3)
+        k_head_dz<S, 3><<<head_blocks(z.g), 256, 0, s>>>(z);
+      else
+        k_head_dz<S, 1><<<head_blocks(z.g), 256, 0, s>>>(z);
+    });
+    if (l.px == 3)
+      k_head_target<3><<<(unsigned)((N + 255) / 256), 256, 0, s>>>(z, logp);
+    else
+      k_head_target<1><<<(unsigned)((N + 255) / 256), 256, 0, s>>>(z, logp);
+    if (dx != nullptr) {
+      HeadGrad g;
+      const bool last = v0 + vocab >= V, lone = p.acc == 0;
+      g.pr.a = {W + (int64_t)v0 * ldw, w_plane, ldw, ldw};
+      g.pr.b = {dz, z_plane, p.piece, (int)N};
+      g.pr.k0 = 0;
+      g.pr.k1 = vocab;
+      g.pr.pa = l.pw;
+      g.pr.pb = l.px;
+      g.out = last || lone ? dx : static_cast<void*>(acc);
+      g.out_bf16 = last && x_dtype == NSA_BF16;
+      g.add = v0 == 0 ? nullptr : lone ? static_cast<const float*>(dx) : acc;
+      g.part = 0;
+      g.k_part = (vocab + kStep - 1) / kStep * kStep;
+      g.N = (int)N;
+      g.D = D;
+      g.m_tiles = (D + 255) / 256;
+      g.n_tiles = (int)((N + 255) / 256);
+      if ((int64_t)g.m_tiles * g.n_tiles >= cu) {
+        k_head_grad<HeadBig, true><<<(unsigned)(g.m_tiles * g.n_tiles), 256, 0, s>>>(g);
+      } else {
+        g.m_tiles = (D + 127) / 128;
+        g.n_tiles = (int)((N + 127) / 128);
+        k_head_grad<HeadMid, true><<<(unsigned)(g.m_tiles * g.n_tiles), 256, 0, s>>>(g);
+      }
+    }
+    if (dw != nullptr) {
+      HeadGrad g;
+      const bool one = p.w_parts == 1, to_bf16 = w_dtype == NSA_BF16;
+      char* to = static_cast<char*>(dw) + (int64_t)v0 * D * (to_bf16 ? 2 : 4);
+      g.pr.a = {X, x_plane, ldx, ldx};
+      g.pr.b = {dz, z_plane, p.piece, p.piece};
+      g.pr.k0 = 0;
+      g.pr.k1 = (int)N;
+      g.pr.pa = l.px;
+      g.pr.pb = l.px;
+      g.out = one ? static_cast<void*>(to) : static_cast<void*>(part);
+      g.out_bf16 = one && to_bf16;
+      g.add = nullptr;
+      g.part = (int64_t)p.piece * D;
+      g.k_part = p.k_part;
+      g.N = vocab;
+      g.D = D;
+      g.m_tiles = (D + 255) / 256;
+      g.n_tiles = (vocab + 255) / 256;
+      k_head_grad<HeadBig, false><<<dim3((unsigned)(g.m_tiles * g.n_tiles), 1, (unsigned)p.w_parts), 256, 0, s>>>(g);
+      if (!one) {
+        const int64_t n = (int64_t)vocab * D, blocks = (n + 2047) / 2048;
+        k_head_sum<<<(unsigned)(blocks < 65536 ? blocks : 65536), 256, 0, s>>>(part, g.part, p.w_parts, to, to_bf16, n);
+      }
+    }
+  }
+  return nsa_launch_status();
+}

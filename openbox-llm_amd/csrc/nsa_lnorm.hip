@@ -1,0 +1,496 @@
+// Residual addition with layer norm, rows of D elements:
+//
+//   h = x + r  (float32, rounded once to r's type; h = x without a residual)
+//   mu = mean_j h_j,  rstd = 1 / sqrt(mean_j (h_j - mu)^2 + eps),  n = (h - mu) rstd,  y = n w + b
+//
+// The norm is taken of the stored h, so that the backward recomputes it from what
+// the forward left.  With g = dy w:
+//
+//   dh = dh_out + rstd (g - mean_j g_j - n mean_j(g_j n_j));   dx = dr = dh
+//   dw = sum over rows of dy n,   db = sum over rows of dy
+//
+// Every kernel is bound by the bytes it moves: one read of x and r (dy, dh_out and
+// h in the backward), one write of h and y (dx, dr).  A row stays in registers, so
+// that the squares are taken about the mean itself (a sum of squares less the
+// squared mean loses the variance of rows far off zero); past 32768 elements, 16384
+// in the backward, a row is read again, through the cache.
+//
+// Threads per row: eight to 1024, a run of 8 elements each to 8192 elements
+// (lnorm_shape); up to one wave there is no barrier at all.
+//
+// The backward's workgroups walk over rows in a stride of the grid and keep their
+// columns' parts of dw and db in registers; the parts are added in workgroup order
+// by a second launch, so that both have the same bits on every run.
+#include "nsa_launch.h"
+#include "nsa_rows.h"
+
+namespace nsa {
+
+constexpr int kLnRegMax = 32768;         // widest row held in registers (forward)
+constexpr int kLnBwdMax = 16384;         // ... and with its gradient and its parts of dw and db (backward)
+constexpr int kLnMax = 1 << 24;          // widest row
+constexpr int64_t kLnSlice = 1 << 21;    // rows of one launch
+
+struct LnArgs {
+  const void *x, *res, *w, *b;
+  void *h, *y;
+  float* stat;      // [rows][2]: mean, rstd; or null
+  int64_t rows;
+  int D;
+  float eps, inv_d;
+  bool w_bf16, y_bf16;
+};
+
+// h of one run: x + r rounded to r's type (RES), or x itself
+template <typename XT, typename RT, bool RES>
+__device__ __forceinline__ void ln_sum8(const LnArgs& a, int64_t at, int n, float (&h)[8]) {
+  load_run8(static_cast<const XT*>(a.x) + at, n, h);
+  if (RES) {
+    float r[8];
+    load_run8(static_cast<const RT*>(a.res) + at, n, r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[j] = (float)(RT)(h[j] + r[j]);
+  }
+}
+
+// TPR threads a row, NV runs of 8 a thread (NV = 0: any length, h formed again for every pass).
+template <typename XT, typename RT, bool RES, int TPR, int NV>
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_ln_fwd(const LnArgs a) {
+  constexpr int W = TPR > kWave ? TPR / kWave : 1;
+  __shared__ float red[2][W];
+  const int t = threadIdx.x & (TPR - 1);
+  const int64_t row = TPR <= 64 ? (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR : (int64_t)blockIdx.x;
+  if (TPR <= 64 && row >= a.rows) return;   // (all of a row's lanes; no barrier follows for these)
+  const int D = a.D;
+  const int64_t base = row * D;
+  const int nrun = NV > 0 ? NV : (D + 8 * TPR - 1) / (8 * TPR);
+  float h[NV > 0 ? NV : 1][8];
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < nrun; ++i) {
+    float(&hi)[8] = h[NV > 0 ? i : 0];
+    const int c = 8 * (i * TPR + t), n = D - c;
+    ln_sum8<XT, RT, RES>(a, base + c, n, hi);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += hi[j];
+    if (RES && n > 0) store_run8(static_cast<RT*>(a.h) + base + c, n, hi);
+  }
+  const float mu = row_sum<TPR>(s, red[0]) * a.inv_d;
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < nrun; ++i) {
+    float(&hi)[8] = h[NV > 0 ? i : 0];
+    const int c = 8 * (i * TPR + t), n = D - c;
+    if (NV == 0) ln_sum8<XT, RT, RES>(a, base + c, n, hi);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      hi[j] -= mu;
+      ss += j < n ? hi[j] * hi[j] : 0.0f;
+    }
+  }
+  ss = row_sum<TPR>(ss, red[1]);
+  const float rstd = 1.0f / sqrtf(ss * a.inv_d + a.eps);
+  if (a.stat != nullptr && t == 0) {
+    a.stat[2 * row] = mu;
+    a.stat[2 * row + 1] = rstd;
+  }
+#pragma unroll
+  for (int i = 0; i < nrun; ++i) {
+    float(&hi)[8] = h[NV > 0 ? i : 0];
+    const int c = 8 * (i * TPR + t), n = D - c;
+    if (NV == 0) {
+      ln_sum8<XT, RT, RES>(a, base + c, n, hi);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) hi[j] -= mu;
+    }
+    float wv[8], bv[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    load_run8_of(a.w, a.w_bf16, c, n, wv);
+    if (a.b != nullptr) load_run8_of(a.b, a.w_bf16, c, n, bv);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) hi[j] = (hi[j] * rstd) * wv[j] + bv[j];
+    if (n > 0) {
+      if (a.y_bf16)
+        store_run8(static_cast<bf16*>(a.y) + base + c, n, hi);
+      else
+        store_run8(static_cast<float*>(a.y) + base + c, n, hi);
+    }
+  }
+}
+
+struct LnBwdArgs {
+  const void *dy, *dh, *h, *w;
+  const float* stat;
+  void *dx, *dres;
+  float* part;            // [2][gridDim.x][D] (dw, db), or null
+  int64_t rows;
+  int D;
+  float inv_d;
+  bool w_bf16, dx_bf16;
+};
+
+// Sums of two values over a row's N threads; `buf` as in row_sum, twice as long.
+template <int N>
+__device__ __forceinline__ void row_sum2(float& u, float& v, float* buf) {
+  u = wave_sum<(N < kWave ? N : kWave)>(u);
+  v = wave_sum<(N < kWave ? N : kWave)>(v);
+  if (N <= kWave) return;
+  if ((threadIdx.x & (kWave - 1)) == 0) {
+    buf[2 * (threadIdx.x / kWave)] = u;
+    buf[2 * (threadIdx.x / kWave) + 1] = v;
+  }
+  __syncthreads();
+  u = v = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N / kWave; ++i) {
+    u += buf[2 * i];
+    v += buf[2 * i + 1];
+  }
+}
+
+// YT: dy; RT: h, dh and dres.  dres is null where dx serves both (one type).
+template <typename YT, typename RT, int TPR, int NV>
+__global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_ln_bwd(const LnBwdArgs a) {
+  constexpr int W = TPR > kWave ? TPR / kWave : 1;
+  constexpr int RPG = TPR <= 64 ? 256 / TPR : 1;   // rows at a time
+  __shared__ float red[2][2 * W];
+  __shared__ float sums[RPG > 1 ? 8 * TPR * NV : 1];
+  const int t = threadIdx.x & (TPR - 1);
+  const int sub = threadIdx.x / TPR;
+  const int D = a.D;
+  // where the registers hold them: the weights for all rows, and dh asked for with the rest of a row
+  constexpr bool kHold = NV * TPR <= 1024;
+  float w[kHold ? NV : 1][8], dw[NV][8], db[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (kHold) load_run8_of(a.w, a.w_bf16, 8 * (i * TPR + t), D - 8 * (i * TPR + t), w[kHold ? i : 0]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dw[i][j] = db[i][j] = 0.0f;
+  }
+  int turn = 0;
+  for (int64_t row = (int64_t)blockIdx.x * RPG + sub; row < a.rows; row += (int64_t)gridDim.x * RPG) {
+    const int64_t base = row * D;
+    const float mu = a.stat[2 * row], rstd = a.stat[2 * row + 1];
+    float n_[NV][8], g[NV][8], d[kHold ? NV : 1][8];
+    float s1 = 0.0f, s2 = 0.0f;
+    auto load_dh = [&](int i, float(&v)[8]) {
+      const int c = 8 * (i * TPR + t);
+      if (a.dh != nullptr) {
+        load_run8(static_cast<const RT*>(a.dh) + base + c, D - c, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + t), n = D - c;
+      load_run8(static_cast<const RT*>(a.h) + base + c, n, n_[i]);
+      load_run8(static_cast<const YT*>(a.dy) + base + c, n, g[i]);   // (0 past the row's end)
+      if (kHold) load_dh(i, d[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float(&wi)[8] = w[kHold ? i : 0];
+      if (!kHold) load_run8_of(a.w, a.w_bf16, 8 * (i * TPR + t), D - 8 * (i * TPR + t), wi);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        n_[i][j] = (n_[i][j] - mu) * rstd;
+        db[i][j] += g[i][j];
+        dw[i][j] += g[i][j] * n_[i][j];
+        g[i][j] *= wi[j];
+        s1 += g[i][j];
+        s2 += g[i][j] * n_[i][j];
+      }
+    }
+    // two buffers in turn: the next row's sums are not written over those still being read
+    row_sum2<TPR>(s1, s2, red[turn & 1]);
+    s1 *= a.inv_d;
+    s2 *= a.inv_d;
+    ++turn;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + t), n = D - c;
+      float(&di)[8] = d[kHold ? i : 0];
+      if (!kHold) load_dh(i, di);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) di[j] += rstd * (g[i][j] - s1 - n_[i][j] * s2);
+      if (n > 0) {
+        if (a.dx_bf16)
+          store_run8(static_cast<bf16*>(a.dx) + base + c, n, di);
+        else
+          store_run8(static_cast<float*>(a.dx) + base + c, n, di);
+        if (a.dres != nullptr) store_run8(static_cast<RT*>(a.dres) + base + c, n, di);
+      }
+    }
+  }
+  if (a.part == nullptr) return;
+  float* out = a.part + (int64_t)blockIdx.x * D;
+  const int64_t next = (int64_t)gridDim.x * D;   // db's parts behind dw's
+  if constexpr (RPG == 1) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = 8 * (i * TPR + t);
+      if (c < D) {
+        store_run8(out + c, D - c, dw[i]);
+        store_run8(out + next + c, D - c, db[i]);
+      }
+    }
+  } else {
+    static_assert(NV == 1, "a row of at most a wave is one run a lane");
+    // the rows of a wave by halves, then the waves' parts in wave order
+    const int wv = threadIdx.x / kWave;
+    auto join = [&](float(&v)[8], float* dst) {
+#pragma unroll
+      for (int x = TPR; x < kWave; x <<= 1)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += __shfl_xor(v[j], x, kWave);
+      for (int s = 0; s < 4; ++s) {
+        if (wv == s && (threadIdx.x & (kWave - 1)) < TPR) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int c = 8 * t + j;
+            if (c < D) sums[c] = s == 0 ? v[j] : sums[c] + v[j];
+          }
+        }
+        __syncthreads();
+      }
+      for (int c = threadIdx.x; c < D; c += 256) dst[c] = sums[c];
+    };
+    join(dw[0], out);
+    __syncthreads();
+    join(db[0], out + next);
+  }
+}
+
+// Rows past kLnBwdMax: one workgroup a row, read twice.
+template <typename YT, typename RT>
+__global__ __launch_bounds__(1024) void k_ln_bwd_long(const LnBwdArgs a) {
+  __shared__ float red[2][32];
+  const int D = a.D;
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, ++turn) {
+    const int64_t base = row * D;
+    const float mu = a.stat[2 * row], rstd = a.stat[2 * row + 1];
+    float s1 = 0.0f, s2 = 0.0f;
+    for (int c = 8 * threadIdx.x; c < D; c += 8 * 1024) {
+      float h[8], g[8], w[8];
+      load_run8(static_cast<const RT*>(a.h) + base + c, D - c, h);
+      load_run8(static_cast<const YT*>(a.dy) + base + c, D - c, g);
+      load_run8_of(a.w, a.w_bf16, c, D - c, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float v = g[j] * w[j];
+        s1 += v;
+        s2 += v * ((h[j] - mu) * rstd);
+      }
+    }
+    row_sum2<1024>(s1, s2, red[turn & 1]);
+    s1 *= a.inv_d;
+    s2 *= a.inv_d;
+    for (int c = 8 * threadIdx.x; c < D; c += 8 * 1024) {
+      const int n = D - c;
+      float h[8], g[8], w[8], d[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      load_run8(static_cast<const RT*>(a.h) + base + c, n, h);
+      load_run8(static_cast<const YT*>(a.dy) + base + c, n, g);
+      load_run8_of(a.w, a.w_bf16, c, n, w);
+      if (a.dh != nullptr) load_run8(static_cast<const RT*>(a.dh) + base + c, n, d);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[j] += rstd * (g[j] * w[j] - s1 - (h[j] - mu) * rstd * s2);
+      if (a.dx_bf16)
+        store_run8(static_cast<bf16*>(a.dx) + base + c, n, d);
+      else
+        store_run8(static_cast<float*>(a.dx) + base + c, n, d);
+      if (a.dres != nullptr) store_run8(static_cast<RT*>(a.dres) + base + c, n, d);
+    }
+  }
+}
+
+// Parts of dw and db for such rows: 2048 columns and every gridDim.y-th row a workgroup.
+template <typename YT, typename RT>
+__global__ __launch_bounds__(256) void k_ln_dw_wide(const LnBwdArgs a) {
+  const int c = 8 * ((int)blockIdx.x * 256 + (int)threadIdx.x), n = a.D - c;
+  if (n <= 0) return;
+  float dw[8] = {0, 0, 0, 0, 0, 0, 0, 0}, db[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 2
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    float h[8], g[8];
+    load_run8(static_cast<const RT*>(a.h) + row * a.D + c, n, h);
+    load_run8(static_cast<const YT*>(a.dy) + row * a.D + c, n, g);
+    const float mu = a.stat[2 * row], rstd = a.stat[2 * row + 1];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      dw[j] += g[j] * ((h[j] - mu) * rstd);
+      db[j] += g[j];
+    }
+  }
+  store_run8(a.part + (int64_t)blockIdx.y * a.D + c, n, dw);
+  store_run8(a.part + ((int64_t)gridDim.y + blockIdx.y) * a.D + c, n, db);
+}
+
+// out[c] = sum of part[p][c] (dw for blockIdx.y = 0, db for 1): 16 columns a workgroup
+// (64-byte pieces of a part), 64 interleaved sums over the parts, added in order.
+__global__ __launch_bounds__(1024) void k_ln_dw(const float* __restrict__ part, int nparts, int D, void* dw, void* db,
+                                                bool w_bf16) {
+  __shared__ float acc[64][17];
+  const int x = threadIdx.x & 15, s = threadIdx.x >> 4;
+  const int c = blockIdx.x * 16 + x;
+  void* out = blockIdx.y == 0 ? dw : db;
+  if (out == nullptr) return;
+  part += (int64_t)blockIdx.y * nparts * D;
+  float v = 0.0f;
+  if (c < D) {
+#pragma unroll 8
+    for (int p = s; p < nparts; p += 64) v += part[(int64_t)p * D + c];
+  }
+  acc[s][x] = v;
+  __syncthreads();
+  if (s < 4) {   // 16 sums each by the first wave, then those four
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += acc[16 * s + i][x];
+    t += __shfl_xor(t, 16, kWave);
+    t += __shfl_xor(t, 32, kWave);
+    if (s == 0 && c < D) {
+      if (w_bf16)
+        static_cast<bf16*>(out)[c] = (bf16)t;
+      else
+        static_cast<float*>(out)[c] = t;
+    }
+  }
+}
+
+// Threads a row and runs a thread: the fewest threads that hold the row with one
+// run each; past 8192 elements two or four runs in 1024.
+struct LnShape {
+  int tpr, nv;
+};
+#define NSA_LN_SHAPES(X) X(8, 1) X(16, 1) X(32, 1) X(64, 1) X(128, 1) X(256, 1) X(512, 1) X(1024, 1) X(1024, 2)
+static LnShape ln_shape(int D) {
+  const int runs = (D + 7) / 8;
+#define NSA_LN_FITS(TPR, NV) \
+  if (runs <= TPR * NV) return {TPR, NV};
+  NSA_LN_SHAPES(NSA_LN_FITS)
+#undef NSA_LN_FITS
+  return {1024, D <= kLnRegMax ? 4 : 0};
+}
+
+template <typename XT, typename RT, bool RES>
+static int ln_fwd_launch(const LnArgs& a, hipStream_t s) {
+  const LnShape sh = ln_shape(a.D);
+#define NSA_LN_CASE(TPR, NV)                                                                 \
+  if (sh.tpr == TPR && sh.nv == NV) {                                                        \
+    const int64_t grid = TPR <= 64 ? (a.rows + 256 / TPR - 1) / (256 / TPR) : a.rows;        \
+    k_ln_fwd<XT, RT, RES, TPR, NV><<<(unsigned)grid, TPR <= 64 ? 256 : TPR, 0, s>>>(a);      \
+    return nsa_launch_status();                                                              \
+  }
+  NSA_LN_SHAPES(NSA_LN_CASE) NSA_LN_CASE(1024, 4) NSA_LN_CASE(1024, 0)
+#undef NSA_LN_CASE
+  return NSA_ERR_SHAPE;
+}
+
+template <typename XT, typename RT>
+static int ln_fwd_as(const LnArgs& a, hipStream_t s) {
+  if (a.res != nullptr) return ln_fwd_launch<XT, RT, true>(a, s);
+  if constexpr (sizeof(XT) == sizeof(RT)) return ln_fwd_launch<XT, RT, false>(a, s);
+  return NSA_ERR_DTYPE;
+}
+
+// Parts of dw and db: a workgroup of the backward each, eight to a compute unit or
+// what its waves hold; past kLnBwdMax a row group of k_ln_dw_wide.
+static int64_t ln_bwd_groups(int64_t rows, int D, int cu) {
+  if (D > kLnBwdMax) return rows < 128 ? rows : 128;
+  const LnShape sh = ln_shape(D);
+  const int rpg = sh.tpr <= 64 ? 256 / sh.tpr : 1;
+  const int64_t groups = (rows + rpg - 1) / rpg;
+  const int64_t most = (int64_t)cu * (sh.tpr <= 256 ? 8 : 2048 / sh.tpr);
+  return groups < most ? groups : most;
+}
+
+template <typename YT, typename RT>
+static int ln_bwd_launch(LnBwdArgs a, void* dw, void* db, hipStream_t s) {
+  const int cu = device_cu_count(s);
+  const LnShape sh = ln_shape(a.D);
+  const int64_t grid = ln_bwd_groups(a.rows, a.D, cu);
+  bool done = false;
+  if (a.D > kLnBwdMax) {
+    k_ln_bwd_long<YT, RT><<<(unsigned)(a.rows < 8192 ? a.rows : 8192), 1024, 0, s>>>(a);
+    if (a.part != nullptr)
+      k_ln_dw_wide<YT, RT><<<dim3((unsigned)((a.D + 2047) / 2048), (unsigned)grid), 256, 0, s>>>(a);
+    done = true;
+  }
+#define NSA_LN_CASE(TPR, NV)                                                            \
+  if (!done && sh.tpr == TPR && sh.nv == NV) {                                          \
+    k_ln_bwd<YT, RT, TPR, NV><<<(unsigned)grid, TPR <= 64 ? 256 : TPR, 0, s>>>(a);      \
+    done = true;                                                                        \
+  }
+  NSA_LN_SHAPES(NSA_LN_CASE)
+#undef NSA_LN_CASE
+  if (!done) return NSA_ERR_SHAPE;
+  if (a.part != nullptr)
+    k_ln_dw<<<dim3((unsigned)((a.D + 15) / 16), 2), 1024, 0, s>>>(a.part, (int)grid, a.D, dw, db, a.w_bf16);
+  return nsa_launch_status();
+}
+
+static bool ln_type(int dtype) { return dtype == NSA_F32 || dtype == NSA_BF16; }
+
+}  // namespace nsa
+
+extern "C" int nsa_lnorm_fwd(const void* x, const void* res, const void* w, const void* b, void* h, void* y,
+                             float* stat, int64_t rows, int D, float eps, int x_dtype, int h_dtype, int w_dtype,
+                             int y_dtype, void* stream) {
+  using namespace nsa;
+  NSA_CHECK(rows >= 0 && rows <= 0x7fffffffLL && D >= 1 && D <= kLnMax, NSA_ERR_SHAPE);
+  NSA_CHECK(ln_type(x_dtype) && ln_type(h_dtype) && ln_type(w_dtype) && ln_type(y_dtype), NSA_ERR_DTYPE);
+  NSA_CHECK(res != nullptr || x_dtype == h_dtype, NSA_ERR_DTYPE);
+  if (rows == 0) return NSA_OK;
+  NSA_CHECK(x != nullptr && w != nullptr && y != nullptr, NSA_ERR_ARG);
+  NSA_CHECK(res == nullptr || h != nullptr, NSA_ERR_ARG);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const size_t xs = x_dtype == NSA_BF16 ? 2 : 4, hs = h_dtype == NSA_BF16 ? 2 : 4, ys = y_dtype == NSA_BF16 ? 2 : 4;
+  // 2^21 rows a launch: a grid holds less than 2^32 threads
+  for (int64_t r0 = 0; r0 < rows; r0 += kLnSlice) {
+    const int64_t n = rows - r0 < kLnSlice ? rows - r0 : kLnSlice, at = r0 * D;
+    const LnArgs a{static_cast<const char*>(x) + at * xs,
+                   res == nullptr ? nullptr : static_cast<const char*>(res) + at * hs,
+                   w,
+                   b,
+                   h == nullptr ? nullptr : static_cast<char*>(h) + at * hs,
+                   static_cast<char*>(y) + at * ys,
+                   stat == nullptr ? nullptr : stat + 2 * r0,
+                   n, D, eps, 1.0f / (float)D, w_dtype == NSA_BF16, y_dtype == NSA_BF16};
+    int rc;
+    if (x_dtype == NSA_BF16)
+      rc = h_dtype == NSA_BF16 ? ln_fwd_as<bf16, bf16>(a, s) : ln_fwd_as<bf16, float>(a, s);
+    else
+      rc = h_dtype == NSA_BF16 ? ln_fwd_as<float, bf16>(a, s) : ln_fwd_as<float, float>(a, s);
+    if (rc != NSA_OK) return rc;
+  }
+  return NSA_OK;
+}
+
+extern "C" size_t nsa_lnorm_bwd_workspace(int64_t rows, int D, void* stream) {
+  using namespace nsa;
+  if (rows < 0 || rows > 0x7fffffffLL || D < 1 || D > kLnMax) return 0;
+  if (rows == 0) return 16;
+  return (size_t)ln_bwd_groups(rows, D, device_cu_count(static_cast<hipStream_t>(stream))) * D * 2 * sizeof(float);
+}
+
+extern "C" int nsa_lnorm_bwd(const void* dy, const void* dh, const void* h, const void* w, const float* stat, void* dx,
+                             void* dres, void* dw, void* db, void* workspace, size_t workspace_bytes, int64_t rows,
+                             int D, int x_dtype, int h_dtype, int w_dtype, int y_dtype, void* stream) {
+  using namespace nsa;
+  NSA_CHECK(rows >= 1 && rows <= 0x7fffffffLL && D >= 1 && D <= kLnMax, NSA_ERR_SHAPE);
+  NSA_CHECK(ln_type(x_dtype) && ln_type(h_dtype) && ln_type(w_dtype) && ln_type(y_dtype), NSA_ERR_DTYPE);
+  NSA_CHECK(dy != nullptr && h != nullptr && w != nullptr && stat != nullptr && dx != nullptr, NSA_ERR_ARG);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  float* part = nullptr;
+  if (dw != nullptr || db != nullptr) {
+    NSA_CHECK(workspace != nullptr && workspace_bytes >= nsa_lnorm_bwd_workspace(rows, D, stream), NSA_ERR_WORKSPACE);
+    part = static_cast<float*>(workspace);
+  }
+  const LnBwdArgs a{dy, dh, h, w, stat, dx, dres, part, rows, D, 1.0f / (float)D, w_dtype == NSA_BF16,
+                    x_dtype == NSA_BF16};
+  if (y_dtype == NSA_BF16)
+    return h_dtype == NSA_BF16 ? ln_bwd_launch<bf16, bf16>(a, dw, db, s) : ln_bwd_launch<bf16, float>(a, dw, db, s);
+  return h_dtype == NSA_BF16 ? ln_bwd_launch<float, bf16>(a, dw, db, s) : ln_bwd_launch<float, float>(a, dw, db, s);
+}

@@ -44,6 +44,16 @@ NSA_ENTRY(nsa_logprob_bwd);
 NSA_ENTRY(nsa_logprob_workspace);
 NSA_ENTRY(nsa_paged_attend_max);
 NSA_ENTRY(nsa_paged_workspace);
+NSA_ENTRY(nsa_lnorm_fwd);
+NSA_ENTRY(nsa_lnorm_bwd);
+NSA_ENTRY(nsa_lnorm_bwd_workspace);
+NSA_ENTRY(nsa_embed_fwd);
+NSA_ENTRY(nsa_embed_bwd);
+NSA_ENTRY(nsa_embed_bwd_workspace);
+NSA_ENTRY(nsa_head_fwd);
+NSA_ENTRY(nsa_head_fwd_workspace);
+NSA_ENTRY(nsa_head_bwd);
+NSA_ENTRY(nsa_head_bwd_workspace);
 #undef NSA_ENTRY
 
 void bind(const py::dict& at) {
@@ -56,6 +66,16 @@ void bind(const py::dict& at) {
   NSA_BIND(nsa_logprob_workspace);
   NSA_BIND(nsa_paged_attend_max);
   NSA_BIND(nsa_paged_workspace);
+  NSA_BIND(nsa_lnorm_fwd);
+  NSA_BIND(nsa_lnorm_bwd);
+  NSA_BIND(nsa_lnorm_bwd_workspace);
+  NSA_BIND(nsa_embed_fwd);
+  NSA_BIND(nsa_embed_bwd);
+  NSA_BIND(nsa_embed_bwd_workspace);
+  NSA_BIND(nsa_head_fwd);
+  NSA_BIND(nsa_head_fwd_workspace);
+  NSA_BIND(nsa_head_bwd);
+  NSA_BIND(nsa_head_bwd_workspace);
 #undef NSA_BIND
 }
 
@@ -361,6 +381,286 @@ std::tuple<OptTensor, Tensor, OptTensor, OptTensor> token_logprobs(const Tensor&
   return {shaped(o.logp, false), *shaped(o.ent, false), shaped(o.top_logp, true), shaped(o.top_idx, true)};
 }
 
+// --- residual addition with layer norm -----------------------------------------
+struct LnOut {
+  Tensor y, h, stat;
+};
+
+LnOut lnorm_forward(const Tensor& x_, const OptTensor& res_, const Tensor& w_, const OptTensor& b_, double eps,
+                    at::ScalarType out, bool want_stat) {
+  const Tensor x = x_.contiguous(), w = w_.contiguous(), res = res_ ? res_->contiguous() : Tensor();
+  const Tensor b = b_ ? b_->contiguous() : Tensor();
+  const int64_t D = x.size(-1), rows = x.numel() / D;
+  LnOut o;
+  o.h = res.defined() ? fresh(res.sizes(), res, res.scalar_type()) : x;
+  o.y = fresh(x.sizes(), x, out);
+  if (want_stat) o.stat = fresh({rows, 2}, x, at::kFloat);
+  On on(x);
+  check_status(p_nsa_lnorm_fwd(x.data_ptr(), at_of(res), w.data_ptr(), at_of(b),
+                               res.defined() ? o.h.data_ptr() : nullptr, o.y.data_ptr(), at_as<float>(o.stat), rows,
+                               (int)D, (float)eps, code_of(x.scalar_type()), code_of(o.h.scalar_type()),
+                               code_of(w.scalar_type()), code_of(out), on.stream),
+               "nsa_lnorm_fwd");
+  return o;
+}
+
+struct LnFn : torch::autograd::Function<LnFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& res, const Tensor& w,
+                               const OptTensor& b, double eps, int64_t out) {
+    ctx->set_materialize_grads(false);
+    LnOut o = lnorm_forward(x, res, w, b, eps, static_cast<at::ScalarType>(out), true);
+    ctx->save_for_backward({o.h, w.contiguous(), o.stat});
+    ctx->saved_data["x"] = static_cast<int64_t>(x.scalar_type());
+    ctx->saved_data["added"] = res.has_value();
+    ctx->saved_data["shifted"] = b.has_value();
+    if (res) return {o.y, o.h};
+    return {o.y};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor h = saved[0].contiguous(), &w = saved[1], &stat = saved[2];
+    const auto xt = static_cast<at::ScalarType>(ctx->saved_data["x"].toInt());
+    const bool added = ctx->saved_data["added"].toBool(), shifted = ctx->saved_data["shifted"].toBool();
+    const bool need_w = ctx->needs_input_grad(added ? 2 : 1);
+    const bool need_b = shifted && ctx->needs_input_grad(added ? 3 : 2);
+    Tensor dy = grads[0], dh = added ? grads[1] : Tensor(), dx, dr, dw, db;
+    TORCH_CHECK(!has_tangent(dy) && !has_tangent(dh), "nsa_lnorm_bwd has no forward-mode derivative");
+    if (!dy.defined()) {   // only the sum was used: its gradient passes through
+      if (dh.defined()) {
+        dx = dh.to(xt);
+        dr = dh;
+        if (need_w) dw = at::zeros_like(w);
+        if (need_b) db = at::zeros_like(w);
+      }
+      return once({dx, dr, dw, db, Tensor(), Tensor()});
+    }
+    const int64_t D = h.size(-1), rows = h.numel() / D;
+    dy = dy.contiguous();
+    if (dh.defined()) dh = dh.contiguous();
+    dx = fresh(h.sizes(), h, xt);
+    const bool two = added && xt != h.scalar_type();
+    if (two) dr = fresh(h.sizes(), h, h.scalar_type());
+    if (need_w) dw = rows > 0 ? fresh(w.sizes(), w, w.scalar_type()) : at::zeros_like(w);
+    if (need_b) db = rows > 0 ? fresh(w.sizes(), w, w.scalar_type()) : at::zeros_like(w);
+    if (rows > 0) {
+      On on(h);
+      Tensor ws;
+      size_t bytes = 0;
+      if (need_w || need_b) {
+        bytes = p_nsa_lnorm_bwd_workspace(rows, (int)D, on.stream);
+        ws = fresh({(int64_t)bytes}, h, at::kByte);
+      }
+      check_backward(p_nsa_lnorm_bwd(dy.data_ptr(), at_of(dh), h.data_ptr(), w.data_ptr(), at_as<float>(stat),
+                                     dx.data_ptr(), at_of(dr), at_of(dw), at_of(db), at_of(ws), bytes, rows, (int)D,
+                                     code_of(xt), code_of(h.scalar_type()), code_of(w.scalar_type()),
+                                     code_of(dy.scalar_type()), on.stream),
+                     "nsa_lnorm_bwd");
+    }
+    if (added && !two) dr = dx;
+    return once({dx, dr, dw, db, Tensor(), Tensor()});
+  }
+};
+
+std::tuple<Tensor, Tensor> add_layer_norm(const Tensor& x, const OptTensor& res, const Tensor& w, const OptTensor& b,
+                                          double eps, std::optional<at::ScalarType> out_) {
+  const char* what = "add_layer_norm";
+  const double e = norm_args(x, res, w, eps, what);
+  if (b) {
+    no_tangent(has_tangent(*b), what);
+    NSA_ASSERT(b->sizes() == w.sizes() && b->scalar_type() == w.scalar_type() && b->device() == w.device(),
+               "add_layer_norm: bias must be like weight");
+  }
+  const auto out = out_ ? *out_ : res ? res->scalar_type() : x.scalar_type();
+  NSA_ASSERT(out == at::kFloat || out == at::kBFloat16, "add_layer_norm: out_dtype must be float32 or bfloat16");
+  if (!(wants_grad(x, res, w) || (at::GradMode::is_enabled() && b && b->requires_grad()))) {
+    LnOut o = lnorm_forward(x, res, w, b, e, out, false);
+    return {o.y, res ? o.h : x};
+  }
+  auto o = LnFn::apply(x, res, w, b, e, static_cast<int64_t>(out));
+  return {o[0], res ? o[1] : x};
+}
+
+// --- embedding -----------------------------------------------------------------
+// The gradient of one table from the rows' dy (index undefined: i % T).
+Tensor embed_gradient(const Tensor& index, const Tensor& dy, int64_t rows, at::ScalarType type, int64_t T, double scale) {
+  const int64_t D = dy.size(-1), n = dy.numel() / D;
+  Tensor dw = fresh({rows, D}, dy, type);
+  if (n == 0) return dw.zero_();
+  On on(dy);
+  const size_t bytes = p_nsa_embed_bwd_workspace(n, (int)D, index.defined());
+  const Tensor ws = fresh({(int64_t)bytes}, dy, at::kByte);
+  check_backward(p_nsa_embed_bwd(at_as<int64_t>(index), dy.data_ptr(), dw.data_ptr(), ws.data_ptr(), bytes, n, T, rows,
+                                 (int)D, (float)scale, code_of(dy.scalar_type()), code_of(type), on.stream),
+                 "nsa_embed_bwd");
+  return dw;
+}
+
+Tensor embed_forward(const Tensor& tokens, const Tensor& w_, const OptTensor& pw_, const OptTensor& pos, double scale,
+                     at::ScalarType out) {
+  const Tensor w = w_.contiguous(), pw = pw_ ? pw_->contiguous() : Tensor();
+  std::vector<int64_t> sizes(tokens.sizes().begin(), tokens.sizes().end());
+  sizes.push_back(w.size(1));
+  Tensor y = fresh(sizes, w, out);
+  On on(w);
+  check_status(p_nsa_embed_fwd(at_as<int64_t>(tokens), pos ? at_as<int64_t>(*pos) : nullptr, w.data_ptr(), at_of(pw),
+                               y.data_ptr(), tokens.numel(), tokens.dim() > 0 ? tokens.size(-1) : 1, w.size(0),
+                               pw.defined() ? pw.size(0) : 0, (int)w.size(1), (float)scale, code_of(w.scalar_type()),
+                               pw.defined() ? code_of(pw.scalar_type()) : NSA_F32, code_of(out), on.stream),
+               "nsa_embed_fwd");
+  return y;
+}
+
+struct EmbedFn : torch::autograd::Function<EmbedFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& tokens, const Tensor& w, const OptTensor& pw,
+                        const OptTensor& pos, double scale, int64_t out) {
+    ctx->save_for_backward({tokens, pos ? *pos : Tensor()});
+    ctx->saved_data["V"] = w.size(0);
+    ctx->saved_data["w"] = static_cast<int64_t>(w.scalar_type());
+    ctx->saved_data["P"] = pw ? pw->size(0) : (int64_t)0;
+    ctx->saved_data["pw"] = static_cast<int64_t>(pw ? pw->scalar_type() : at::kFloat);
+    ctx->saved_data["scale"] = scale;
+    return embed_forward(tokens, w, pw, pos, scale, static_cast<at::ScalarType>(out));
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &tokens = saved[0], &pos = saved[1];
+    TORCH_CHECK(!has_tangent(grads[0]), "nsa_embed_bwd has no forward-mode derivative");
+    const Tensor dy = grads[0].contiguous();
+    const int64_t T = tokens.dim() > 0 ? tokens.size(-1) : 1, P = ctx->saved_data["P"].toInt();
+    Tensor dw, dp;
+    if (ctx->needs_input_grad(1))
+      dw = embed_gradient(tokens, dy, ctx->saved_data["V"].toInt(),
+                          static_cast<at::ScalarType>(ctx->saved_data["w"].toInt()), T,
+                          ctx->saved_data["scale"].toDouble());
+    if (P > 0 && ctx->needs_input_grad(2))
+      dp = embed_gradient(pos, dy, P, static_cast<at::ScalarType>(ctx->saved_data["pw"].toInt()), T, 1.0);
+    return once({Tensor(), dw, dp, Tensor(), Tensor(), Tensor()});
+  }
+};
+
+Tensor embed(const Tensor& tokens_, const Tensor& w, double scale, const OptTensor& pw, const OptTensor& pos_,
+             std::optional<at::ScalarType> out_) {
+  no_tangent(has_tangent(w) || has_tangent(pw), "embed");
+  check_tensor(w, "embed: weight");
+  NSA_ASSERT(w.dim() == 2 && w.size(0) >= 1 && w.size(1) >= 1 && w.size(1) <= (1 << 20), "embed: weight must be [V, D]");
+  auto index = [&](const Tensor& t, const char* name) {
+    NSA_ASSERT(at::isIntegralType(t.scalar_type(), /*includeBool=*/false), std::string("embed: ") + name + " must be integers");
+    NSA_ASSERT(t.device() == w.device(), std::string("embed: ") + name + " on the weight's device");
+    return t.to(at::kLong).contiguous();
+  };
+  const Tensor tokens = index(tokens_, "tokens");
+  OptTensor pos;
+  if (pw) {
+    check_tensor(*pw, "embed: pos_weight");
+    NSA_ASSERT(pw->dim() == 2 && pw->size(0) >= 1 && pw->size(1) == w.size(1) && pw->device() == w.device(),
+               "embed: pos_weight must be [P, D] beside the weight");
+    if (pos_) {
+      NSA_ASSERT(pos_->sizes() == tokens.sizes(), "embed: one position for each token");
+      pos = index(*pos_, "positions");
+    } else {
+      NSA_ASSERT(tokens.dim() >= 1 && tokens.size(-1) <= pw->size(0), "embed: more tokens in a row than positions");
+    }
+  } else {
+    NSA_ASSERT(!pos_, "embed: positions without pos_weight");
+  }
+  const auto out = out_ ? *out_ : w.scalar_type();
+  NSA_ASSERT(out == at::kFloat || out == at::kBFloat16, "embed: out_dtype must be float32 or bfloat16");
+  if (at::GradMode::is_enabled() && (w.requires_grad() || (pw && pw->requires_grad())))
+    return EmbedFn::apply(tokens, w, pw, pos, scale, static_cast<int64_t>(out));
+  return embed_forward(tokens, w, pw, pos, scale, out);
+}
+
+// --- log probabilities from the rows behind the last norm ------------------------
+int on_16(const Tensor& x, const Tensor& w) {
+  return (reinterpret_cast<uintptr_t>(x.data_ptr()) | reinterpret_cast<uintptr_t>(w.data_ptr())) % 16 == 0;
+}
+
+std::tuple<Tensor, Tensor> head_forward(const Tensor& x, const Tensor& w, const OptTensor& targets) {
+  const int64_t N = x.size(0), V = w.size(0), D = x.size(1);
+  Tensor logp, lse = fresh({N}, x, at::kFloat);
+  if (targets) logp = fresh({N}, x, at::kFloat);
+  On on(x);
+  const int xc = code_of(x.scalar_type()), wc = code_of(w.scalar_type());
+  const size_t bytes = p_nsa_head_fwd_workspace(N, (int)V, (int)D, xc, wc, on_16(x, w), on.stream);
+  NSA_ASSERT(bytes > 0, "linear_logprobs: unsupported shape");
+  const Tensor ws = fresh({(int64_t)bytes}, x, at::kByte);
+  check_status(p_nsa_head_fwd(x.data_ptr(), w.data_ptr(), targets ? at_as<int64_t>(*targets) : nullptr,
+                              at_as<float>(logp), at_as<float>(lse), ws.data_ptr(), bytes, N, (int)V, (int)D, xc, wc,
+                              on.stream),
+               "nsa_head_fwd");
+  return {logp, lse};
+}
+
+struct HeadFn : torch::autograd::Function<HeadFn> {
+  // Outputs: lse, and with targets logp
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& targets) {
+    ctx->set_materialize_grads(false);
+    auto [logp, lse] = head_forward(x, w, targets);
+    ctx->save_for_backward({x, w, targets ? *targets : Tensor(), logp, lse});
+    if (targets) return {lse, logp};
+    return {lse};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &targets = saved[2], &logp = saved[3], &lse = saved[4];
+    Tensor dlse = grads[0], dlogp = targets.defined() ? grads[1] : Tensor(), dx, dw;
+    TORCH_CHECK(!has_tangent(dlogp) && !has_tangent(dlse), "nsa_head_bwd has no forward-mode derivative");
+    if (!dlogp.defined() && !dlse.defined()) return {Tensor(), Tensor(), Tensor()};
+    if (dlogp.defined()) dlogp = dlogp.contiguous();
+    if (dlse.defined()) dlse = dlse.contiguous();
+    const int64_t N = x.size(0);
+    if (ctx->needs_input_grad(0)) dx = fresh(x.sizes(), x, x.scalar_type());
+    if (ctx->needs_input_grad(1)) dw = N > 0 ? fresh(w.sizes(), w, w.scalar_type()) : at::zeros_like(w);
+    if (N > 0 && (dx.defined() || dw.defined())) {
+      On on(x);
+      const int xc = code_of(x.scalar_type()), wc = code_of(w.scalar_type());
+      const int V = (int)w.size(0), D = (int)w.size(1);
+      const size_t bytes = p_nsa_head_bwd_workspace(N, V, D, xc, wc, on_16(x, w), on.stream);
+      const Tensor ws = fresh({(int64_t)bytes}, x, at::kByte);
+      check_backward(p_nsa_head_bwd(x.data_ptr(), w.data_ptr(), at_as<int64_t>(targets), at_as<float>(logp),
+                                    at_as<float>(lse), at_as<float>(dlogp), at_as<float>(dlse), at_of(dx), at_of(dw),
+                                    ws.data_ptr(), bytes, N, V, D, xc, wc, on.stream),
+                     "nsa_head_bwd");
+    }
+    return once({dx, dw, Tensor()});
+  }
+};
+
+std::tuple<OptTensor, Tensor> linear_logprobs(const Tensor& x_, const Tensor& w_, const OptTensor& targets_) {
+  const char* what = "linear_logprobs";
+  no_tangent(has_tangent(x_) || has_tangent(w_), what);
+  check_tensor(x_, what);
+  check_tensor(w_, what);
+  NSA_ASSERT(w_.dim() == 2 && w_.size(0) >= 1 && w_.size(0) <= (1 << 28) && w_.size(1) >= 1 && w_.size(1) <= 65536,
+             "linear_logprobs: weight must be [V, D]");
+  const int64_t D = w_.size(1);
+  NSA_ASSERT(x_.dim() >= 1 && x_.size(-1) == D && x_.device() == w_.device(), "linear_logprobs: x must be [..., D]");
+  NSA_ASSERT(x_.numel() / D <= (1 << 22), "linear_logprobs: at most 2^22 rows");
+  const auto lead = x_.sizes().slice(0, x_.dim() - 1);
+  OptTensor targets;
+  if (targets_) {
+    NSA_ASSERT(targets_->device() == x_.device(), "linear_logprobs: targets on the rows' device");
+    NSA_ASSERT(at::isIntegralType(targets_->scalar_type(), /*includeBool=*/false),
+               "linear_logprobs: targets must be integers");
+    NSA_ASSERT(targets_->sizes() == lead, "linear_logprobs: one target for each row");
+    targets = targets_->reshape({-1}).to(at::kLong).contiguous();
+  }
+  const Tensor x = x_.dim() == 2 ? x_.contiguous() : x_.reshape({-1, D}).contiguous(), w = w_.contiguous();
+  Tensor logp, lse;
+  if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad())) {
+    auto out = HeadFn::apply(x, w, targets);
+    lse = out[0];
+    if (targets) logp = out[1];
+  } else {
+    std::tie(logp, lse) = head_forward(x, w, targets);
+  }
+  auto shaped = [&](const Tensor& t) { return lead.size() == 1 ? t : t.view(lead); };
+  return {targets ? OptTensor(shaped(logp)) : std::nullopt, shaped(lse)};
+}
+
 // --- one new token over a paged cache -----------------------------------------
 void check_pages(const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& lens) {
   NSA_ASSERT(kp.dim() == 4 && kp.is_cuda(), "paged: pages must be [n_pages, Hkv, page, D] on the GPU");
@@ -442,6 +742,9 @@ PYBIND11_MODULE(_nsa_torch, m) {
   m.def("add_rms_norm", &add_rms_norm);
   m.def("add_rms_norm_q8", &add_rms_norm_q8);
   m.def("token_logprobs", &token_logprobs);
+  m.def("add_layer_norm", &add_layer_norm);
+  m.def("embed", &embed);
+  m.def("linear_logprobs", &linear_logprobs);
   m.def("check_pages", &check_pages);
   m.def("no_tangent", [](const std::vector<Tensor>& ts, const std::string& what) {
     for (const Tensor& t : ts) no_tangent(has_tangent(t), what.c_str());

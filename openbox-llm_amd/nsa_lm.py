@@ -1,5 +1,5 @@
-"""What a decoder computes around its attention, on MI355X: the residual's
-addition with the root-mean-square norm, and the log probabilities of tokens.
+"""What a decoder computes around its attention, on MI355X: its embedding, the
+residual's addition with the norm, and the log probabilities of tokens.
 
 * ``add_rms_norm`` / ``add_rms_norm_q8``: ``x + branch`` and the norm of the
   sum in one pass (the reference adds and norms in ``Block.forward``,
@@ -9,6 +9,15 @@ addition with the root-mean-square norm, and the log probabilities of tokens.
   best alternatives of every row of logits, with the gradient; the loss over
   the vocabulary (nsa_model.py:504-507) is their mean.
   ``NSATransformer(loss_impl='fused')`` and ``NSATransformer.score`` use it.
+
+* ``add_layer_norm``: the same addition with the reference's own norm
+  (nsa_model.py:449-452); ``NSATransformer(norm_impl='joined')``.
+* ``embed``: rows of the token table with their positions' rows
+  (nsa_model.py:455-511), and both tables' gradients by sorted tokens;
+  ``NSATransformer(embed_impl='fused')``.
+* ``linear_logprobs``: log probabilities of given tokens from the rows behind the
+  last norm, without the logits, with the gradients;
+  ``NSATransformer(loss_impl='pieces')``.
 
 Tensors are float32 or bfloat16 on the GPU, at any alignment of their elements;
 rows that are not dense are made contiguous.  Sums and statistics are float32.
@@ -69,6 +78,42 @@ def add_rms_norm_q8(x, residual, weight, eps=None):
         return f(x, residual, weight, eps)
 
 
+def add_layer_norm(x, residual, weight, bias=None, eps=1e-5, out_dtype=None):
+    """``h = x + residual`` and ``y = (h - mean(h)) / sqrt(var(h) + eps) * weight +
+    bias`` over the last dimension -> ``(y, h)``; ``var`` is the mean square about
+    the mean, as in ``torch.nn.LayerNorm``.
+
+    Shapes, dtypes, rounding and derivatives as in ``add_rms_norm``; ``bias [D]``
+    (or None) in the weight's dtype.  The gradients of weight and bias have the
+    same bits on every run.  ``eps`` 0 makes a row of equal elements NaN."""
+    f = L.torch_side().add_layer_norm
+    if _ops._TIMER is None:
+        return f(x, residual, weight, bias, eps, out_dtype)
+    with _ops._span("nsa_lnorm_fwd"):
+        return f(x, residual, weight, bias, eps, out_dtype)
+
+
+# ---------------------------------------------------------------------------
+# embedding
+# ---------------------------------------------------------------------------
+
+def embed(tokens, weight, scale=1.0, pos_weight=None, positions=None, out_dtype=None):
+    """``scale * weight[tokens] + pos_weight[positions]`` -> ``[..., D]`` in
+    ``out_dtype`` (default: the weight's), formed in float32 and rounded once.
+
+    ``tokens [..., T]`` and ``positions`` (the same shape) are integers; without
+    ``positions`` the token at index t of the last dimension takes row t of
+    ``pos_weight [P, D]``, and without ``pos_weight`` there is no position.  A
+    token outside ``0 .. V-1`` (padding) adds nothing and has no gradient, nor has
+    a position outside ``0 .. P-1``.  Differentiable in both tables: dense
+    gradients, summed in float32, with the same bits on every run."""
+    f = L.torch_side().embed
+    if _ops._TIMER is None:
+        return f(tokens, weight, scale, pos_weight, positions, out_dtype)
+    with _ops._span("nsa_embed_fwd"):
+        return f(tokens, weight, scale, pos_weight, positions, out_dtype)
+
+
 # ---------------------------------------------------------------------------
 # log probabilities of tokens
 # ---------------------------------------------------------------------------
@@ -104,3 +149,32 @@ def token_logprobs(logits, targets=None, top=0):
         return TokenLogprobs(*f(logits, targets, top))
     with _ops._span("nsa_logprob_fwd"):
         return TokenLogprobs(*f(logits, targets, top))
+
+
+class LinearLogprobs(NamedTuple):
+    """Per row: ``logp`` (None without targets) and ``lse``."""
+
+    logp: Optional[torch.Tensor]
+    lse: torch.Tensor
+
+
+def linear_logprobs(x, weight, targets=None):
+    """Log probabilities under ``softmax(x @ weight.T)`` without forming the logits:
+    ``x [..., D]``, ``weight [V, D]`` -> ``LinearLogprobs`` of float32 ``[...]``.
+
+    ``lse`` is the logits' log-sum-exp and ``logp`` (with integer ``targets [...]``)
+    the target's log probability; a target outside ``0 .. V-1`` (``-100`` included)
+    leaves 0 and no gradient.  Differentiable in x and weight, from both outputs;
+    the backward forms the logits a second time, in pieces of the vocabulary that
+    take at most about half a GB, and has the same bits on every run.
+
+    float32 rows are computed in float32's precision.  bfloat16 rows are products of
+    bfloat16 with float32 sums, and the logits' gradient is rounded once to bfloat16
+    on its way into the products with x and weight; float32 weights beside bfloat16
+    rows are rounded to bfloat16 first (as under autocast) and have a float32
+    gradient.  At most 2^22 rows.  Rows with NaN or an infinite logit give NaN."""
+    f = L.torch_side().linear_logprobs
+    if _ops._TIMER is None:
+        return LinearLogprobs(*f(x, weight, targets))
+    with _ops._span("nsa_head_fwd"):
+        return LinearLogprobs(*f(x, weight, targets))
