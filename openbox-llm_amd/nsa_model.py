@@ -45,9 +45,11 @@ Keyword-only extensions, off by default (none is in the reference):
   queries and keys of every branch, keys rotated before pooling),
   ``tie_embeddings``, ``dense_impl='sdpa'`` (the dense arm through
   ``torch.nn.functional.scaled_dot_product_attention``);
-* ``norm_impl='fused'`` and ``loss_impl='fused'``: the residual additions with
-  the RMS norms, and the loss over the vocabulary, on the MI355X kernels
-  (``nsa_lm``);
+* ``norm_impl='joined'`` (``'fused'`` for RMS norms), ``embed_impl='fused'`` and
+  ``loss_impl='fused'``: the residual additions with the norms, the embedding with
+  its positions, and the loss over the vocabulary, on the MI355X kernels
+  (``nsa_lm``); ``loss_impl='pieces'`` takes the loss from the rows behind the last norm, and a
+  training step has no logits;
 * generation with the dense arm over paged caches (``nsa_paged``):
   ``NSATransformer.paged_caches``, ``prefill`` and ``step``; ``score`` for the log
   probabilities of given tokens.
@@ -667,8 +669,8 @@ class Block(nn.Module):
     def __init__(self, d_model, n_q_heads, n_kv_heads, ffn_mult=4, attn_type="nsa", *, norm="layer",
                  ffn="gelu", ffn_hidden=None, norm_impl="ref", **nsa_kw):
         super().__init__()
-        assert norm_impl in ("ref", "fused"), "norm_impl must be 'ref' or 'fused'"
-        assert norm_impl == "ref" or norm == "rms", "norm_impl='fused' needs norm='rms'"
+        assert norm_impl in ("ref", "fused", "joined"), "norm_impl must be 'ref', 'fused' or 'joined'"
+        assert norm_impl != "fused" or norm == "rms", "norm_impl='fused' needs norm='rms' ('joined' takes both norms)"
         self.norm_impl = norm_impl
         if attn_type == "full":
             nsa_kw = {k: v for k, v in nsa_kw.items() if k not in _NSA_ONLY}
@@ -685,7 +687,7 @@ class Block(nn.Module):
             self.ffn = nn.Sequential(Linear(d_model, hidden), nn.GELU(), Linear(hidden, d_model))
 
     def forward(self, x):
-        if self.norm_impl == "fused":
+        if self.norm_impl != "ref":
             x, f = self.pending(x, None)
             return x + f
         x = x + self.attn(self.ln1(x))
@@ -693,7 +695,7 @@ class Block(nn.Module):
 
     def pending(self, x, branch, attn=None):
         """The block with its additions left to the norms that follow them
-        (``norm_impl='fused'``): ``x`` and the branch still to be added to it
+        (``norm_impl='fused'`` or ``'joined'``): ``x`` and the branch still to be added to it
         (None: nothing) -> the same pair behind the block.  ``attn`` stands in
         for the attention (a generation step's)."""
         y, x = _fused_norm(self.ln1, branch, x)
@@ -704,7 +706,7 @@ class Block(nn.Module):
     def step(self, x, branch, cache):
         """One token of every sequence, ``x [B, d_model]``: the pair of
         ``pending`` (with ``norm_impl='ref'`` the branch is None throughout)."""
-        if self.norm_impl == "fused":
+        if self.norm_impl != "ref":
             return self.pending(x, branch, lambda y: self.attn.step(y, cache))
         x = x + self.attn.step(self.ln1(x), cache)
         return x + self.ffn(self.ln2(x)), None
@@ -720,9 +722,10 @@ def _fused_norm(ln, branch, x):
     dtype the products after it compute in (autocast's, where it is on)."""
     import nsa_lm
     out = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
-    if branch is None:
-        return nsa_lm.add_rms_norm(x, None, ln.weight, ln.eps, out)
-    return nsa_lm.add_rms_norm(branch, x, ln.weight, ln.eps, out)
+    pair = (x, None) if branch is None else (branch, x)
+    if isinstance(ln, nn.LayerNorm):
+        return nsa_lm.add_layer_norm(*pair, ln.weight, ln.bias, ln.eps, out)
+    return nsa_lm.add_rms_norm(*pair, ln.weight, ln.eps, out)
 
 
 class NSATransformer(nn.Module):
@@ -730,16 +733,19 @@ class NSATransformer(nn.Module):
     block: token embedding (+ learned positions unless ``pos='rope'``), the
     blocks, final norm, LM head tied to the embedding (nsa_model.py:455-511).
     ``forward(idx, targets=None) -> (logits, loss)``; ``grad_checkpoint``
-    recomputes each block in the backward."""
+    recomputes each block in the backward.  With ``loss_impl='pieces'`` the logits
+    are None where targets are given."""
 
     def __init__(self, vocab_size, d_model=512, n_layers=8, n_q_heads=8, n_kv_heads=2, max_seq_len=256,
                  ffn_mult=4, block_size=16, n_selected_blocks=4, window=32, attn_type="nsa", attn_impl="ref", *,
                  norm="layer", ffn="gelu", ffn_hidden=None, pos="learned", rope_base=10000.0, tie_embeddings=True,
                  dense_impl="ref", cmp_stride=None, sel_block=None, force_init=False, n_local=0, compressor="mean",
-                 cmp_hidden=None, norm_impl="ref", loss_impl="ref"):
+                 cmp_hidden=None, norm_impl="ref", loss_impl="ref", embed_impl="ref"):
         super().__init__()
-        assert loss_impl in ("ref", "fused"), "loss_impl must be 'ref' or 'fused'"
+        assert loss_impl in ("ref", "fused", "pieces"), "loss_impl must be 'ref', 'fused' or 'pieces'"
+        assert embed_impl in ("ref", "fused"), "embed_impl must be 'ref' or 'fused'"
         self.norm_impl = norm_impl
+        self.embed_impl = embed_impl
         self.loss_impl = loss_impl
         assert pos in ("learned", "rope"), "pos must be 'learned' or 'rope'"
         self.max_seq_len = max_seq_len
@@ -772,21 +778,38 @@ class NSATransformer(nn.Module):
             nn.init.zeros_(m.bias)
 
     def forward(self, idx, targets=None):
-        B, T = idx.shape
-        assert T <= self.max_seq_len
-        x = self.tok_emb(idx)
-        if hasattr(self, "pos_emb"):
-            x = x + self.pos_emb(torch.arange(T, device=idx.device))[None]
-        logits = self.lm_head(self._run_blocks(x))
+        x = self._run_blocks(self._embed(idx))
+        if targets is not None and self.loss_impl == "pieces":
+            return None, self._mean_loss(self._linear_logprobs(x, targets).logp, targets)
+        logits = self.lm_head(x)
         loss = None
         if targets is not None:
             loss = self._loss(logits, targets)
         return logits, loss
 
+    def _embed(self, idx):
+        """The rows ``[B, T, d_model]`` of the tokens ``idx [B, T]`` at positions 0 .. T-1."""
+        T = idx.shape[1]
+        assert T <= self.max_seq_len
+        learned = hasattr(self, "pos_emb")
+        if self.embed_impl == "fused":
+            import nsa_lm
+            return nsa_lm.embed(idx, self.tok_emb.weight, pos_weight=self.pos_emb.weight if learned else None)
+        x = self.tok_emb(idx)
+        return x + self.pos_emb(torch.arange(T, device=idx.device))[None] if learned else x
+
+    def _linear_logprobs(self, x, targets=None):
+        """``nsa_lm.linear_logprobs`` under the LM head, of the rows as its product takes
+        them (autocast's dtype, where it is on)."""
+        import nsa_lm
+        if torch.is_autocast_enabled("cuda"):
+            x = x.to(torch.get_autocast_dtype("cuda"))
+        return nsa_lm.linear_logprobs(x, self.lm_head.weight, targets)
+
     def _run_blocks(self, x):
         """The blocks and the final norm."""
         ckpt = self.grad_checkpoint and self.training
-        if self.norm_impl == "fused":
+        if self.norm_impl != "ref":
             branch = None
             for blk in self.blocks:
                 if ckpt:
@@ -808,11 +831,19 @@ class NSATransformer(nn.Module):
         without a wait for the host."""
         if self.loss_impl == "fused":
             import nsa_lm
-            logp = nsa_lm.token_logprobs(logits, targets).logp
-            kept = targets != -100
-            wrong = (kept & ((targets < 0) | (targets >= logits.shape[-1]))).any()
-            return -logp.sum() / kept.sum().float().masked_fill(wrong, float("nan"))
+            return self._mean_loss(nsa_lm.token_logprobs(logits, targets).logp, targets)
         return F.cross_entropy(logits.view(-1, logits.size(-1)), targets.view(-1))
+
+    def _mean_loss(self, logp, targets):
+        kept = targets != -100
+        wrong = (kept & ((targets < 0) | (targets >= self.lm_head.weight.shape[0]))).any()
+        return -logp.sum() / kept.sum().float().masked_fill(wrong, float("nan"))
+
+    @torch.no_grad()
+    def logprobs(self, idx, targets):
+        """``LinearLogprobs`` of the targets ``[B, T]`` behind the tokens ``idx [B, T]``:
+        log probabilities and log sums, without the logits that ``score`` forms."""
+        return self._linear_logprobs(self._run_blocks(self._embed(idx)), targets)
 
     @torch.no_grad()
     def score(self, idx, targets, top=0):
@@ -838,21 +869,17 @@ class NSATransformer(nn.Module):
     def prefill(self, idx, caches, lens=None):
         """``forward(idx)``'s logits ``[B, T, V]``, the keys and values of the first
         ``lens[b]`` tokens (default all) kept in the (empty, reserved) caches."""
-        B, T = idx.shape
-        assert T <= self.max_seq_len
         assert len(caches) == len(self.blocks), "one cache for each block"
-        x = self.tok_emb(idx)
-        if hasattr(self, "pos_emb"):
-            x = x + self.pos_emb(torch.arange(T, device=idx.device))[None]
+        x = self._embed(idx)
         lens = caches[0].counts(lens)
         branch = None
         for blk, cache in zip(self.blocks, caches):
-            if self.norm_impl == "fused":
+            if self.norm_impl != "ref":
                 x, branch = blk.pending(x, branch, lambda y: blk.attn.prefill(y, cache, lens))
             else:
                 x = x + blk.attn.prefill(blk.ln1(x), cache, lens)
                 x = x + blk.ffn(blk.ln2(x))
-        return self.lm_head(_fused_norm(self.ln_f, branch, x)[0] if self.norm_impl == "fused" else self.ln_f(x))
+        return self.lm_head(_fused_norm(self.ln_f, branch, x)[0] if self.norm_impl != "ref" else self.ln_f(x))
 
     @torch.no_grad()
     def step(self, tokens, caches):
@@ -862,13 +889,19 @@ class NSATransformer(nn.Module):
         sequence that is as long as its caches take no longer grows: its
         length tells (its logits then are of no position)."""
         assert len(caches) == len(self.blocks), "one cache for each block"
-        x = self.tok_emb(tokens)
-        if hasattr(self, "pos_emb"):
-            x = x + self.pos_emb(caches[0].lens.long().clamp(0, self.max_seq_len - 1))
+        at = caches[0].lens.long().clamp(0, self.max_seq_len - 1) if hasattr(self, "pos_emb") else None
+        if self.embed_impl == "fused":
+            import nsa_lm
+            x = nsa_lm.embed(tokens, self.tok_emb.weight, pos_weight=None if at is None else self.pos_emb.weight,
+                             positions=at)
+        else:
+            x = self.tok_emb(tokens)
+            if at is not None:
+                x = x + self.pos_emb(at)
         branch = None
         for blk, cache in zip(self.blocks, caches):
             x, branch = blk.step(x, branch, cache)
-        return self.lm_head(_fused_norm(self.ln_f, branch, x)[0] if self.norm_impl == "fused" else self.ln_f(x))
+        return self.lm_head(_fused_norm(self.ln_f, branch, x)[0] if self.norm_impl != "ref" else self.ln_f(x))
 
     def num_params(self):
         """The reference's parameter count (nsa_model.py:508-511): the unique
