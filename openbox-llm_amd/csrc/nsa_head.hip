@@ -23,8 +23,6 @@
 // the transposed LDS reads turn; no transposed copy is made.  Results have the
 // 32-row tile's rows permuted (perm32), so that a lane holds eight neighbouring
 // elements of an output row.
-#include <algorithm>
-
 #include "nsa_launch.h"
 #include "nsa_rows.h"
 #include "nsa_tile32.h"
@@ -32,7 +30,7 @@
 namespace nsa {
 
 constexpr int64_t kHeadRows = 1 << 22;       // most rows of x
-constexpr int kHeadVocab = 1 << 28;
+constexpr int kHeadVocab = 1 << 24;
 constexpr int kHeadWide = 1 << 16;           // widest row
 constexpr size_t kHeadPiece = 512u << 20;    // bytes of dz held at a time
 constexpr int64_t kHeadPieceMost = 1 << 20;  // most tokens of a piece: offsets within a stage have 32 bits
@@ -49,10 +47,10 @@ struct HeadOperand {
   int rows;        // rows (ROWS) or columns, for clamping: what lies past them is never stored
 };
 
-// One product C[m][n] = sum over plane pairs and k of A[m][k] B[n][k].
+// One product C[m][n] = sum over plane pairs and k < K of A[m][k] B[n][k].
 struct HeadProduct {
   HeadOperand a, b;
-  int k0, k1;      // contraction range of this workgroup; k0 a multiple of kStep
+  int K;
   int pa, pb;      // planes
 };
 
@@ -71,75 +69,85 @@ __device__ __forceinline__ void head_pair(int pa, int pb, int i, int& x, int& y)
   }
 }
 
-// A stage of one operand: T rows (ROWS) or columns x kStep contraction elements.
-// 16-byte chunks swizzled so that 16 neighbouring lanes' 16-byte reads, or the
-// transposed reads' 32-byte pieces of four rows, meet every bank once.
+// A stage of one operand: T rows (ROWS) or columns x kStep contraction elements, in
+// 16-byte chunks.  Chunks are swizzled so that 16 neighbouring lanes' 16-byte reads, or
+// the transposed reads' 32-byte pieces of four rows, meet every bank once.
 template <int T, bool ROWS>
 struct HeadTile {
   static constexpr int kElems = T * kStep;
-  static constexpr int kLoads = T * 8 / 256;   // 16-byte requests a thread
-  static constexpr int kCpr = ROWS ? 8 : T / 8;
-  static_assert(T % 32 == 0 && (ROWS || T >= 128), "a tile of whole requests");
+  static constexpr int kLoads = T * 8 / 256;      // requests a thread, 256 chunks each
+  static constexpr int kCpr = ROWS ? 8 : T / 8;   // chunks a row of the stage
+  static constexpr int kRows = 256 / kCpr;        // rows of the stage a request
+  static_assert(T % 32 == 0 && (ROWS || T == 256), "a tile of whole requests");
   static __device__ __forceinline__ int key(int r) {
     return ROWS ? (r >> 1) & 7 : 4 * (r & 3) + ((r >> 2) & 3);
   }
 
-  uint32_t off[kLoads];   // bytes from the stage's base
-
-  // rows (columns) first .. first + T - 1 of the operand
-  __device__ __forceinline__ void aim(const HeadOperand& o, int first, int tid) {
+  // Request j brings rows j kRows + tid / kCpr; the key of such a row depends on j
+  // through its parity alone (ROWS: not at all), so that two offsets serve all.
+  uint32_t off[2];
+  const bf16* base;   // the next stage's rows (columns) `first` .., elements k ..
+  int first, left;    // left: K - k
+  __device__ __forceinline__ void init(const HeadOperand& o, int tid) {
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int P = j * 256 + tid, r = P / kCpr, c = (P % kCpr) ^ key(r);
-      if (ROWS) {
-        const int last = o.rows - 1 - first;   // >= 0
-        off[j] = (uint32_t)((r < last ? r : last) * o.ld * 2 + c * 16);
-      } else {
-        const int col = first + 8 * c;
-        off[j] = (uint32_t)(r * o.ld * 2 + (col < o.rows ? 8 * c : 0) * 2);
-      }
+    for (int j = 0; j < 2; ++j) {
+      const int r = tid / kCpr, c = (tid % kCpr) ^ key(j * kRows + r);
+      off[j] = (uint32_t)(r * o.ld * 2 + c * 16);
     }
   }
-  // Request elements k .. k + 63 of plane `pl` (fewer before k1: the rest as zeros).
-  __device__ __forceinline__ void request(const HeadOperand& o, int first, int pl, int k, int k1, bf16* lds,
-                                          int tid) const {
-    const bf16* base = o.p + pl * o.plane + (ROWS ? (int64_t)first * o.ld + k : (int64_t)k * o.ld + first);
+  __device__ __forceinline__ void aim(const HeadOperand& o, int first_, int pl, int k, int K) {
+    first = first_;
+    left = K - k;
+    base = o.p + pl * o.plane + (ROWS ? (int64_t)first * o.ld + k : (int64_t)k * o.ld + first);
+  }
+  __device__ __forceinline__ void next(const HeadOperand& o) {
+    left -= kStep;
+    base += ROWS ? (int64_t)kStep : kStep * o.ld;
+  }
+  // Requests j0 .. j1 - 1: rows (columns) past the operand's last one are any, elements
+  // from K on zeros.
+  template <int J0, int J1>
+  __device__ __forceinline__ void request(const HeadOperand& o, bf16* lds, int tid) const {
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    if (k1 - k >= kStep) {
+    if (left >= kStep && first + T <= o.rows) {
 #pragma unroll
-      for (int j = 0; j < kLoads; ++j) lds_dma16_sbase(base, off[j], lds + (j * 256 + 64 * w) * 8);
+      for (int j = J0; j < J1; ++j)
+        lds_dma16_sbase(base + j * kRows * o.ld, off[j & 1], lds + (j * 256 + 64 * w) * 8);
     } else {
-      const int left = k1 - k;
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) {
-        const int P = j * 256 + tid, r = P / kCpr, c = (P % kCpr) ^ key(r);
-        const bool in = ROWS ? 8 * c < left : r < left;
-        const void* src = in ? reinterpret_cast<const char*>(base) + off[j] : reinterpret_cast<const char*>(&g_head_zero);
+      const int last = o.rows - 1 - first;   // >= 0
+#pragma unroll 1
+      for (int j = J0; j < J1; ++j) {
+        const int r = j * kRows + tid / kCpr, c = (tid % kCpr) ^ key(r);
+        const bf16* src = base + (ROWS ? (r < last ? r : last) * o.ld + 8 * c : r * o.ld + (8 * c <= last ? 8 * c : 0));
+        if (ROWS ? 8 * c >= left : r >= left) src = reinterpret_cast<const bf16*>(&g_head_zero);
         lds_dma16(src, lds + (j * 256 + 64 * w) * 8);
       }
     }
   }
-  // Fragment of the 32-row tile that starts at row r0: row r0 + m (PERM: perm32(m)),
-  // contraction elements 16 s + 8 h .. + 7.
+  // Fragments of a wave: of the 32-row tile i from row w0 on (a multiple of 32, of 128
+  // where there are several and not ROWS), row m (PERM: perm32(m)), contraction
+  // elements 16 s + 8 h .. + 7.  `at` is the lane's byte address in a stage for i = s =
+  // 0; i and s enter by addition, or by exclusive or where the swizzle has their bits.
   template <bool PERM>
-  static __device__ __forceinline__ bf16x8 frag(const bf16* lds, int r0, int s, int lane) {
+  static __device__ __forceinline__ uint32_t lane_at(int w0, int lane) {
+    if (ROWS) {
+      const int r = PERM ? perm32(lane & 31) : lane & 31;
+      return (uint32_t)((w0 + r) * kStep * 2 + (((lane >> 5) ^ key(r)) << 4));
+    }
+    const int g = lane >> 4, r = 8 * (g >> 1) + ((lane >> 2) & 3);
+    int q = lane & 3;
+    if (PERM) q = ((q & 1) << 1) | (q >> 1);   // perm32 swaps bits 2 and 3 of the row
+    const int col = w0 + 16 * (g & 1) + 4 * q;
+    return (uint32_t)(r * T * 2 + (((col >> 3) ^ key(r)) << 4) + (col & 7) * 2);
+  }
+  static __device__ __forceinline__ bf16x8 frag(const char* stage, uint32_t at, int i, int s) {
     if constexpr (ROWS) {
-      const int m = lane & 31, h = lane >> 5;
-      const int r = r0 + (PERM ? perm32(m) : m);
-      return *reinterpret_cast<const bf16x8*>(lds + r * kStep + (((2 * s + h) ^ key(r)) << 3));
+      return *reinterpret_cast<const bf16x8*>(stage + (at ^ (32 * s)) + 32 * i * kStep * 2);
     } else {
       typedef short s16x8 __attribute__((ext_vector_type(8)));
-      const int g = lane >> 4, jj = (lane >> 2) & 3;
-      int q = lane & 3;
-      if (PERM) q = ((q & 1) << 1) | (q >> 1);   // perm32 swaps bits 2 and 3 of the row
-      const int col = r0 + 16 * (g & 1) + 4 * q;
-      s16x4 v[2];
-#pragma unroll
-      for (int rd = 0; rd < 2; ++rd) {
-        const int r = 16 * s + 8 * (g >> 1) + 4 * rd + jj;
-        v[rd] = lds_read_tr16(lds + r * T + (((col >> 3) ^ key(r)) << 3) + (col & 7));
-      }
-      const s16x8 f = (s16x8){v[0][0], v[0][1], v[0][2], v[0][3], v[1][0], v[1][1], v[1][2], v[1][3]};
+      const uint32_t a0 = at ^ (64 * i), a1 = a0 ^ 16;   // (rows r + 4: another key by 1)
+      const s16x4 u = lds_read_tr16(stage + a0 + 16 * s * T * 2), v = lds_read_tr16(stage + a1 + (16 * s + 4) * T * 2);
+      const s16x8 f = (s16x8){u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
       return __builtin_bit_cast(bf16x8, f);
     }
   }
@@ -153,82 +161,148 @@ struct HeadShape {
   static_assert(WM * WN == 4 && MT >= 1 && NT >= 1 && NS >= 2, "four waves");
 };
 
-// The product of tiles m = m_first, m_first + m_step, .. < m_tiles (TM rows each) with
-// the tile at column n0; done(m, acc) takes each result.  All stages of all tiles
-// are one pipeline: while a tile is finished, the next one's stages are under way.
-template <class S, bool AROWS, bool BROWS, typename Done>
-__device__ __forceinline__ void head_product(const HeadProduct& pr, int m_first, int m_step, int m_tiles, int n0,
-                                             Done done) {
+// What a workgroup computes: tiles (m, n) of the result, each over the steps q0 .. q1 - 1
+// of its contraction (a step: kStep elements of one plane pair; pairs one after another).
+struct HeadSpan {
+  int m, n, q0, q1;
+};
+__device__ __forceinline__ int head_steps(const HeadProduct& pr) {
+  return head_pairs(pr.pa, pr.pb) * ((pr.K + kStep - 1) / kStep);
+}
+
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void head_each(F& f) {
+  f(std::integral_constant<int, I>{});
+  if constexpr (I + 1 < N) head_each<N, I + 1>(f);
+}
+
+// The spans i = 0 .. spans - 1, `total` steps in all; done(span, wm, wn, acc) takes each result.
+//
+// All steps of all spans are one pipeline of NS stages in LDS.  A wave holds the
+// fragments of 16 contraction elements while it reads those of the next 16; the
+// barrier between two stages stands before the products of a stage's last 16, whose
+// fragments are in registers by then, so that neither it nor the first reads of the
+// next stage leave the matrix units idle, and the stage's memory is asked to be
+// filled again at once.
+template <class S, bool AROWS, bool BROWS, typename Span, typename Done>
+__device__ __forceinline__ void head_product(const HeadProduct& pr, int spans, int total, Span span, Done done) {
   using TA = HeadTile<S::TM, AROWS>;
   using TB = HeadTile<S::TN, BROWS>;
-  constexpr int kLoads = TA::kLoads + TB::kLoads;
+  constexpr int kLoads = TA::kLoads + TB::kLoads, KS = kStep / 16;
+  static_assert(KS % 2 == 0, "two sets of fragments in turn");
   __shared__ __align__(1024) bf16 sa[S::NS][TA::kElems];
   __shared__ __align__(1024) bf16 sb[S::NS][TB::kElems];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = (w % S::WM) * S::MT * 32, wn = (w / S::WM) * S::NT * 32;
-  const int ksteps = (pr.k1 - pr.k0 + kStep - 1) / kStep;
-  const int pairs = head_pairs(pr.pa, pr.pb);
-  const int ntile = m_first < m_tiles ? (m_tiles - m_first + m_step - 1) / m_step : 0;
-  const int64_t total = (int64_t)ntile * pairs * ksteps;
-  // the request's place: tile, plane pair, step
+  const int ksteps = (pr.K + kStep - 1) / kStep;
+  // the next request: span, step of it, plane pair
   TA ta;
   TB tb;
-  int rm = m_first, rp = 0, rk = 0;
-  ta.aim(pr.a, rm * S::TM, tid);
-  tb.aim(pr.b, n0, tid);
-  int64_t asked = 0;
-  auto request = [&]() {
+  ta.init(pr.a, tid);
+  tb.init(pr.b, tid);
+  int ri = 0, rst = 0, asked = 0, rq, rp, pair_left;
+  HeadSpan rs;
+  auto aim = [&](int k) {
     int x, y;
     head_pair(pr.pa, pr.pb, rp, x, y);
-    const int k = pr.k0 + rk * kStep, st = (int)(asked % S::NS);
-    ta.request(pr.a, rm * S::TM, x, k, pr.k1, sa[st], tid);
-    tb.request(pr.b, n0, y, k, pr.k1, sb[st], tid);
-    ++asked;
-    if (++rk == ksteps) {
-      rk = 0;
-      if (++rp == pairs) {
-        rp = 0;
-        rm += m_step;
-        if (rm < m_tiles) ta.aim(pr.a, rm * S::TM, tid);
+    ta.aim(pr.a, rs.m * S::TM, x, k, pr.K);
+    tb.aim(pr.b, rs.n * S::TN, y, k, pr.K);
+  };
+  auto start = [&]() {
+    rs = span(ri);
+    rq = rs.q0, rp = rq / ksteps;
+    const int k = rq - rp * ksteps;
+    pair_left = ksteps - k;
+    aim(k * kStep);
+  };
+  start();
+  // part P of MT of the next stage's requests; the last one moves on
+  auto request = [&](auto part) {
+    constexpr int P = decltype(part)::value, PA = TA::kLoads, PB = TB::kLoads;
+    ta.template request<PA * P / S::MT, PA*(P + 1) / S::MT>(pr.a, sa[rst], tid);
+    tb.template request<PB * P / S::MT, PB*(P + 1) / S::MT>(pr.b, sb[rst], tid);
+    if constexpr (P == S::MT - 1) {
+      ++asked;
+      rst = rst + 1 == S::NS ? 0 : rst + 1;
+      ta.next(pr.a);
+      tb.next(pr.b);
+      if (++rq == rs.q1) {
+        if (++ri < spans) start();
+      } else if (--pair_left == 0) {
+        ++rp;
+        pair_left = ksteps;
+        aim(0);
       }
     }
   };
-  for (int i = 0; i < S::NS - 1 && asked < total; ++i) request();
+  bf16x8 fa[2][S::MT], fb[2][S::NT];
+  uint32_t la = TA::template lane_at<true>(wm, lane), lb = TB::template lane_at<false>(wn, lane);
+  auto read = [&](int set, int st, int ks) {
+    const char *A = reinterpret_cast<const char*>(sa[st]), *B = reinterpret_cast<const char*>(sb[st]);
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i) fa[set][i] = TA::frag(A, la, i, ks);
+#pragma unroll
+    for (int j = 0; j < S::NT; ++j) fb[set][j] = TB::frag(B, lb, j, ks);
+  };
+  auto meet = [&]() {   // (this wave's LDS reads are done, and everybody's)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < S::NS; ++i)
+    if (asked < total) head_each<S::MT>(request);
+  if (total >= S::NS)
+    vm_wait<(S::NS - 1) * kLoads>();
+  else
+    vm_wait<0>();
+  meet();
+  read(0, 0, 0);
   f32x16 acc[S::MT][S::NT];
-  int64_t it = 0;
-  for (int m = m_first; m < m_tiles; m += m_step) {
+  int it = 0, st = 0;
+  for (int sp = 0; sp < spans; ++sp) {
+    const HeadSpan cur = span(sp);
 #pragma unroll
     for (int i = 0; i < S::MT; ++i)
 #pragma unroll
       for (int j = 0; j < S::NT; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-    for (int s = 0; s < pairs * ksteps; ++s, ++it) {
-      // stage `it` has arrived when only the NS - 2 younger ones are outstanding
-      if (S::NS > 2 && it + S::NS - 2 < total)
-        vm_wait<(S::NS - 2) * kLoads>();
-      else
-        vm_wait<0>();
-      __syncthreads();   // everybody's part of it has; and nobody reads stage it - 1 any more
-      if (asked < total) request();
-      const bf16* A = sa[it % S::NS];
-      const bf16* B = sb[it % S::NS];
+    for (int q = cur.q0; q < cur.q1; ++q, ++it) {
+      asm volatile("" : "+v"(la), "+v"(lb));   // (addresses formed here, not kept for every stage)
 #pragma unroll
-      for (int ks = 0; ks < kStep / 16; ++ks) {
-        bf16x8 fa[S::MT], fb[S::NT];
-#pragma unroll
-        for (int i = 0; i < S::MT; ++i) fa[i] = TA::template frag<true>(A, wm + 32 * i, ks, lane);
-#pragma unroll
-        for (int j = 0; j < S::NT; ++j) fb[j] = TB::template frag<false>(B, wn + 32 * j, ks, lane);
-#pragma unroll
-        for (int i = 0; i < S::MT; ++i)
+      for (int ks = 0; ks < KS; ++ks) {
+        bool refill = false;
+        if (ks + 1 < KS) {
+          read((ks + 1) & 1, st, ks + 1);
+        } else if (it + 1 < total) {
+          // stage it + 1 has arrived when only the NS - 2 younger ones are outstanding
+          if (S::NS > 2 && it + S::NS - 1 < total)
+            vm_wait<(S::NS - 2) * kLoads>();
+          else
+            vm_wait<0>();
+          meet();
+          refill = asked < total;
+          st = st + 1 == S::NS ? 0 : st + 1;
+          read(0, st, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        auto rows = [&](auto row) {   // the requests between the products, which outlast them
+          constexpr int i = decltype(row)::value;
 #pragma unroll
           for (int j = 0; j < S::NT; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[ks & 1][i], fb[ks & 1][j], acc[i][j], 0, 0, 0);
+          if (ks + 1 == KS) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (refill) request(row);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        };
+        head_each<S::MT>(rows);
       }
     }
-    done(m, wm, wn, acc);
+    done(cur, wm, wn, acc);
   }
 }
 
@@ -250,6 +324,11 @@ __device__ __forceinline__ bool head_place(const HeadGrid& g, int bid, int& n, i
   return n < g.n_tiles;
 }
 
+// tiles of vocabulary lane `part` (at least one: split <= m_tiles)
+__device__ __forceinline__ int head_share(const HeadGrid& g, int part) {
+  return (g.m_tiles - part + g.split - 1) / g.split;
+}
+
 struct HeadFwd {
   HeadProduct pr;    // a: weights, b: rows
   HeadGrid g;
@@ -267,9 +346,11 @@ __global__ __launch_bounds__(256, 1) void k_head_fwd(const HeadFwd a) {
   float m[S::NT], l[S::NT];
 #pragma unroll
   for (int j = 0; j < S::NT; ++j) m[j] = kMaskScore, l[j] = 0.0f;
+  const int steps = head_steps(a.pr), tiles = head_share(a.g, part);
   head_product<S, true, true>(
-      a.pr, part, a.g.split, a.g.m_tiles, nt * S::TN, [&](int mt, int wm, int wn, f32x16(&acc)[S::MT][S::NT]) {
-        const int v0 = mt * S::TM + wm + 8 * h;
+      a.pr, tiles, tiles * steps, [&](int i) { return HeadSpan{part + i * a.g.split, nt, 0, steps}; },
+      [&](const HeadSpan& sp, int wm, int wn, f32x16(&acc)[S::MT][S::NT]) {
+        const int mt = sp.m, v0 = mt * S::TM + wm + 8 * h;
         if (mt * S::TM + S::TM > a.V) {   // past the vocabulary: no weight
 #pragma unroll
           for (int i = 0; i < S::MT; ++i)
@@ -296,6 +377,7 @@ __global__ __launch_bounds__(256, 1) void k_head_fwd(const HeadFwd a) {
             for (int r = 0; r < 16; ++r) s += fast_exp2(fmaf(acc[i][j][r], kLog2e, -mn));
           l[j] = l[j] * fast_exp2(m[j] - mn) + s;
           m[j] = mn;
+          __builtin_amdgcn_sched_barrier(0);   // (one row's values in registers at a time)
         }
       });
   // the halves of a wave, then the waves along the vocabulary
@@ -411,8 +493,12 @@ __global__ __launch_bounds__(256, 1) void k_head_dz(const HeadDz a) {
       if (a.dlogp != nullptr && head_real(a.target, n, a.V)) co[j] -= a.dlogp[n];
     }
   }
+  const int steps = head_steps(a.pr), tiles = head_share(a.g, part);
   head_product<S, true, true>(
-      a.pr, part, a.g.split, a.g.m_tiles, nt * S::TN, [&](int mt, int wm, int wn, f32x16(&acc)[S::MT][S::NT]) {
+      a.pr, tiles, tiles * steps, [&](int i) { return HeadSpan{part + i * a.g.split, nt, 0, steps}; },
+      [&](const HeadSpan& sp, int wm, int wn, f32x16(&acc)[S::MT][S::NT]) {
+        const int mt = sp.m;
+        const bool inside = mt * S::TM + S::TM <= a.vocab;   // else zeros past the vocabulary
 #pragma unroll
         for (int j = 0; j < S::NT; ++j) {
           const int n = nt * S::TN + wn + 32 * j + (lane & 31);
@@ -424,11 +510,14 @@ __global__ __launch_bounds__(256, 1) void k_head_dz(const HeadDz a) {
               const int v = mt * S::TM + wm + 32 * i + acc_elem(h, r0);
               float d[8];
 #pragma unroll
-              for (int r = 0; r < 8; ++r) {
-                d[r] = co[j] * fast_exp2(fmaf(acc[i][j][r0 + r], kLog2e, -off[j]));
-                if (v + r >= a.vocab) d[r] = 0.0f;
+              for (int r = 0; r < 8; ++r) d[r] = co[j] * fast_exp2(fmaf(acc[i][j][r0 + r], kLog2e, -off[j]));
+              if (!inside) {
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                  if (v + r >= a.vocab) d[r] = 0.0f;
               }
               store_planes<PLANES>(a.dz + (int64_t)n * a.ld + v, a.plane, d);
+              __builtin_amdgcn_sched_barrier(0);
             }
         }
       });
@@ -453,70 +542,135 @@ __global__ __launch_bounds__(256) void k_head_target(const HeadDz a, const float
   }
 }
 
-// dx (rows of x on n, columns of W on m) and dW's parts (tokens on n, columns of x on m)
+// dx (rows of x on n, columns of W on m) and dW (tokens on n, columns of x on m).  The
+// workgroups take whole tiles in rounds, neighbours on one XCD at the same steps, so
+// that its L2 serves them all; the tiles of a last round that would not fill the chip
+// are cut into `cuts` parts each, which go to `part` and are added by
+// k_head_join_tiles.  So do whole tiles that reach past D: their rows' ends are written
+// there.
 struct HeadGrad {
   HeadProduct pr;
-  void* out;             // [n][D]: float32 or, out_bf16, bf16
+  void* out;             // [N][D]: float32 or, out_bf16, bf16
   const float* add;      // float32 of the same shape to add, or null
-  int64_t part;          // elements between the parts of the contraction (blockIdx.z)
-  int k_part;            // contraction elements a part, a multiple of kStep
-  int N, D, m_tiles, n_tiles;
+  float* part;           // [cuts][tiles - whole][TN][TM], then [n_tiles][TN][TM] of the edge
+  int N, D, m_tiles, n_tiles, groups;
+  int whole, cuts;       // tiles taken whole, a multiple of groups
   bool out_bf16;
 };
+
 template <class S, bool BROWS>
 __global__ __launch_bounds__(256, 1) void k_head_grad(const HeadGrad a) {
-  const int bid = (int)xcd_remap(blockIdx.x, gridDim.x);
-  const int mt = bid % a.m_tiles, nt = bid / a.m_tiles;
-  HeadProduct pr = a.pr;
-  pr.k0 = (int)blockIdx.z * a.k_part;
-  pr.k1 = pr.k1 < pr.k0 + a.k_part ? pr.k1 : pr.k0 + a.k_part;
+  const int g = (int)xcd_remap(blockIdx.x, gridDim.x);
+  const int steps = head_steps(a.pr), rounds = a.whole / a.groups;
+  const int rest = a.m_tiles * a.n_tiles - a.whole, units = rest * a.cuts;
+  // whole tiles, then units g, g + groups, ..: unit u is part u / rest of tile whole + u % rest
+  auto span = [&](int i) {
+    int t = i * a.groups + g, q0 = 0, q1 = steps;
+    if (i >= rounds) {
+      const int u = (i - rounds) * a.groups + g, c = u / rest;
+      t = a.whole + u % rest;
+      q0 = (int)((int64_t)steps * c / a.cuts);
+      q1 = (int)((int64_t)steps * (c + 1) / a.cuts);
+    }
+    return HeadSpan{t % a.m_tiles, t / a.m_tiles, q0, q1};
+  };
+  const int spans = rounds + (g < units ? (units - g + a.groups - 1) / a.groups : 0);
+  int total = 0;
+  for (int i = 0; i < spans; ++i) {
+    const HeadSpan sp = span(i);
+    total += sp.q1 - sp.q0;
+  }
+  if (total == 0) return;
   const int lane = threadIdx.x & 63, h = lane >> 5;
-  const int64_t at = (int64_t)blockIdx.z * a.part;
   head_product<S, false, BROWS>(
-      pr, mt, 1, mt + 1, nt * S::TN, [&](int m, int wm, int wn, f32x16(&acc)[S::MT][S::NT]) {
+      a.pr, spans, total, span, [&](const HeadSpan& sp, int wm, int wn, f32x16(&acc)[S::MT][S::NT]) {
+        const int t = sp.n * a.m_tiles + sp.m;
+        float* part = nullptr;
+        if (sp.q1 - sp.q0 != steps) {   // (cuts <= steps: the part that ends at q1)
+          const int c = (int)(((int64_t)sp.q1 * a.cuts + steps - 1) / steps) - 1;
+          part = a.part + ((int64_t)c * rest + t - a.whole) * S::TM * S::TN;
+        }
+        if (part == nullptr && sp.m * S::TM + S::TM > a.D) part = a.part + ((int64_t)units + sp.n) * S::TM * S::TN;
+        auto each = [&](auto put) {
 #pragma unroll
-        for (int j = 0; j < S::NT; ++j) {
-          const int64_t n = nt * S::TN + wn + 32 * j + (lane & 31);
-          if (n >= a.N) continue;
+          for (int j = 0; j < S::NT; ++j) {
+            const int c = wn + 32 * j + (lane & 31);
+            if (sp.n * (int64_t)S::TN + c >= a.N) continue;
 #pragma unroll
-          for (int i = 0; i < S::MT; ++i)
+            for (int i = 0; i < S::MT; ++i)
 #pragma unroll
-            for (int r0 = 0; r0 < 16; r0 += 8) {
-              const int d = m * S::TM + wm + 32 * i + acc_elem(h, r0);
-              if (d >= a.D) continue;
-              float v[8];
+              for (int r0 = 0; r0 < 16; r0 += 8) {
+                float v[8];
 #pragma unroll
-              for (int r = 0; r < 8; ++r) v[r] = acc[i][j][r0 + r];
-              if (a.add != nullptr) {
-                float u[8];
-                load_run8(a.add + n * a.D + d, a.D - d, u);
-#pragma unroll
-                for (int r = 0; r < 8; ++r) v[r] += u[r];
+                for (int r = 0; r < 8; ++r) v[r] = acc[i][j][r0 + r];
+                put(c, wm + 32 * i + acc_elem(h, r0), v);
+                __builtin_amdgcn_sched_barrier(0);   // (few of the results in other registers at a time)
               }
-              if (a.out_bf16)
-                store_run8(static_cast<bf16*>(a.out) + at + n * a.D + d, a.D - d, v);
-              else
-                store_run8(static_cast<float*>(a.out) + at + n * a.D + d, a.D - d, v);
+          }
+        };
+        const int64_t at = (int64_t)sp.n * S::TN * a.D + sp.m * S::TM;
+        if (part != nullptr) {
+          each([&](int c, int e, float(&v)[8]) { store_run8(part + c * S::TM + e, v); });
+        } else if (a.out_bf16) {
+          each([&](int c, int e, float(&v)[8]) {
+            const int64_t o = at + (int64_t)c * a.D + e;
+            if (a.add != nullptr) {
+              float u[8];
+              load_run8(a.add + o, u);
+#pragma unroll
+              for (int r = 0; r < 8; ++r) v[r] += u[r];
             }
+            store_run8(static_cast<bf16*>(a.out) + o, v);
+          });
+        } else {
+          each([&](int c, int e, float(&v)[8]) {
+            const int64_t o = at + (int64_t)c * a.D + e;
+            if (a.add != nullptr) {
+              float u[8];
+              load_run8(a.add + o, u);
+#pragma unroll
+              for (int r = 0; r < 8; ++r) v[r] += u[r];
+            }
+            store_run8(static_cast<float*>(a.out) + o, v);
+          });
         }
       });
 }
 
-// out[i] = sum over the parts, in order
-__global__ __launch_bounds__(256) void k_head_sum(const float* part, int64_t stride, int nparts, void* out, bool bf,
-                                                  int64_t n) {
-  for (int64_t i = 8 * ((int64_t)blockIdx.x * 256 + threadIdx.x); i < n; i += 8 * 256 * (int64_t)gridDim.x) {
-    float s[8], v[8];
-    load_run8(part + i, (int)std::min<int64_t>(8, n - i), s);
-    for (int p = 1; p < nparts; ++p) {
-      load_run8(part + p * stride + i, (int)std::min<int64_t>(8, n - i), v);
+// The cut tiles' parts in order, and the tiles at the rows' ends.  Eight workgroups a
+// tile, a thread 8 elements at a time.
+template <class S>
+__global__ __launch_bounds__(256) void k_head_join_tiles(const HeadGrad a, int first) {
+  const int t = first + (int)blockIdx.x, rest = a.m_tiles * a.n_tiles - a.whole;
+  const int m0 = (t % a.m_tiles) * S::TM;
+  const bool cut = t >= a.whole && a.cuts > 1;
+  if (!cut && m0 + S::TM <= a.D) return;
+  const int64_t n0 = (int64_t)(t / a.m_tiles) * S::TN;
+  const float* part =
+      a.part + (cut ? (int64_t)t - a.whole : (int64_t)rest * a.cuts + t / a.m_tiles) * S::TM * S::TN;
+  const int64_t next = (int64_t)rest * S::TM * S::TN;
+  constexpr int kRuns = S::TM / 8;
+  for (int i = (int)blockIdx.y * 256 + threadIdx.x; i < S::TN * kRuns; i += 8 * 256) {
+    const int c = i / kRuns, e = i % kRuns * 8, d = m0 + e;
+    const int64_t n = n0 + c;
+    if (n >= a.N || d >= a.D) continue;
+    float v[8], u[8];
+    load_run8(part + c * S::TM + e, v);
+#pragma unroll 4
+    for (int g = 1; g < (cut ? a.cuts : 1); ++g) {
+      load_run8(part + g * next + c * S::TM + e, u);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] += v[j];
+      for (int r = 0; r < 8; ++r) v[r] += u[r];
     }
-    if (bf)
-      store_run8(static_cast<bf16*>(out) + i, (int)std::min<int64_t>(8, n - i), s);
+    if (a.add != nullptr) {
+      load_run8(a.add + n * a.D + d, a.D - d, u);
+#pragma unroll
+      for (int r = 0; r < 8; ++r) v[r] += u[r];
+    }
+    if (a.out_bf16)
+      store_run8(static_cast<bf16*>(a.out) + n * a.D + d, a.D - d, v);
     else
-      store_run8(static_cast<float*>(out) + i, (int)std::min<int64_t>(8, n - i), s);
+      store_run8(static_cast<float*>(a.out) + n * a.D + d, a.D - d, v);
   }
 }
 
@@ -538,7 +692,7 @@ __global__ __launch_bounds__(256) void k_head_pack(const void* x, bool x_bf16, b
 // host
 // ---------------------------------------------------------------------------
 using HeadBig = HeadShape<256, 256, 2, 2, 2>;
-using HeadMid = HeadShape<128, 128, 2, 2, 3>;
+using HeadMid = HeadShape<128, 128, 2, 2, 2>;
 using HeadFew = HeadShape<128, 32, 4, 1, 4>;
 
 static bool head_type(int dtype) { return dtype == NSA_F32 || dtype == NSA_BF16; }
@@ -601,28 +755,71 @@ static auto head_as(int kind, F f) {
   return f(HeadBig{});
 }
 
-// The backward's pieces: tokens of one, and parts of its contraction over the rows
+// The gradients' products: 256 x 256 tiles.  The last round's tiles are cut where that
+// saves more than a part costs: a tile's step takes about 1.1 us, writing and adding its
+// 256 KB part 26.
+using HeadGradShape = HeadBig;
+struct HeadCut {
+  int groups, whole, cuts;
+  int64_t parts;   // tiles of the part buffer
+};
+static HeadCut head_cut(int64_t rows, int D, int K, int pairs, int cu) {
+  using S = HeadGradShape;
+  const int64_t m = (D + S::TM - 1) / S::TM, n = (rows + S::TN - 1) / S::TN, tiles = m * n;
+  const int64_t steps = (int64_t)pairs * ((K + kStep - 1) / kStep);
+  HeadCut c{cu, (int)(tiles / cu * cu), 1, 0};
+  const int64_t rest = tiles - c.whole;
+  if (rest > 0) {
+    double best = 1e30;
+    for (int p = 1; p <= 64 && p * 4 <= steps + 3; ++p) {
+      const double time = (double)((rest * p + cu - 1) / cu) * (1.1 * steps / p) + (p > 1 ? 26.0 * rest * p / cu : 0.0);
+      if (time < best) best = time, c.cuts = p;
+    }
+    if (c.whole == 0 && rest * c.cuts < cu) c.groups = (int)(rest * c.cuts);
+  }
+  c.parts = (c.cuts > 1 ? rest * c.cuts : 0) + (D % S::TM == 0 ? 0 : n);
+  if (c.cuts == 1) c.parts += rest;   // (the edge's tiles lie behind `rest` unused ones)
+  return c;
+}
+static int head_pair_count(int pa, int pb) { return pb == 1 ? 1 : pa == 1 ? 3 : 6; }
+template <bool BROWS>
+static void head_grad(HeadGrad g, int cu, hipStream_t s) {
+  using S = HeadGradShape;
+  g.m_tiles = (g.D + S::TM - 1) / S::TM;
+  g.n_tiles = (g.N + S::TN - 1) / S::TN;
+  const HeadCut c = head_cut(g.N, g.D, g.pr.K, head_pair_count(g.pr.pa, g.pr.pb), cu);
+  g.groups = c.groups;
+  g.whole = c.whole;
+  g.cuts = c.cuts;
+  k_head_grad<S, BROWS><<<(unsigned)g.groups, 256, 0, s>>>(g);
+  const int tiles = g.m_tiles * g.n_tiles, first = g.D % S::TM != 0 ? 0 : c.cuts > 1 ? c.whole : tiles;
+  if (first < tiles) k_head_join_tiles<S><<<dim3((unsigned)(tiles - first), 8), 256, 0, s>>>(g, first);
+}
+
+// The backward's pieces of the vocabulary and its buffers
 struct HeadPlan {
   int piece;            // tokens of a piece, a multiple of 256
-  int w_parts, k_part;  // dW: parts, rows of x each
   size_t dz, acc, part; // bytes
 };
-static HeadPlan head_plan(int64_t N, int V, int D, int planes, bool x_bf16, int cu) {
+static HeadPlan head_plan(int64_t N, int V, int D, int planes, int pw, bool x_bf16, int cu) {
   HeadPlan p;
   const int64_t all = ((int64_t)V + 255) / 256 * 256;
   int64_t fit = (int64_t)(kHeadPiece / ((size_t)N * 2 * planes)) / 256 * 256;
   fit = fit < 256 ? 256 : fit < kHeadPieceMost ? fit : kHeadPieceMost;
   const int64_t pieces = (all + fit - 1) / fit;
   p.piece = (int)(((all + pieces - 1) / pieces + 255) / 256 * 256);
-  const int64_t tiles = (int64_t)(p.piece / 256) * ((D + 255) / 256);
-  int64_t parts = (cu + tiles - 1) / tiles;
-  const int64_t most = (N + 1023) / 1024;
-  if (parts > most) parts = most;
-  p.k_part = (int)(((N + parts - 1) / parts + kStep - 1) / kStep * kStep);
-  p.w_parts = (int)((N + p.k_part - 1) / p.k_part);
   p.dz = up16((size_t)planes * N * p.piece * 2);
-  p.acc = pieces > 1 && x_bf16 ? up16((size_t)N * D * 4) : 0;
-  p.part = p.w_parts > 1 ? up16((size_t)p.w_parts * p.piece * D * 4) : 0;
+  p.acc = all > p.piece && x_bf16 ? up16((size_t)N * D * 4) : 0;
+  // the parts of dx and dW of a whole piece and of the last one
+  const int last = (int)(V - (int64_t)(V - 1) / p.piece * p.piece);
+  int64_t parts = 0;
+  for (int vocab : {p.piece < V ? p.piece : V, last}) {
+    const int64_t dx = head_cut(N, D, vocab, head_pair_count(pw, planes), cu).parts;
+    const int64_t dw = head_cut(vocab, D, (int)N, head_pair_count(planes, planes), cu).parts;
+    parts = dx > parts ? dx : parts;
+    parts = dw > parts ? dw : parts;
+  }
+  p.part = (size_t)parts * HeadGradShape::TM * HeadGradShape::TN * 4;
   return p;
 }
 
@@ -667,8 +864,7 @@ extern "C" int nsa_head_fwd(const void* x, const void* w, const int64_t* target,
     HeadFwd a;
     a.pr.a = {l.pack_w ? wp : static_cast<const bf16*>(w), (int64_t)V * l.ld, l.pack_w ? l.ld : D, V};
     a.pr.b = {l.pack_x ? xp : static_cast<const bf16*>(x), N * l.ld, l.pack_x ? l.ld : D, (int)N};
-    a.pr.k0 = 0;
-    a.pr.k1 = D;
+    a.pr.K = D;
     a.pr.pa = l.pw;
     a.pr.pb = l.px;
     a.g = g;
@@ -689,7 +885,7 @@ extern "C" size_t nsa_head_bwd_workspace(int64_t N, int V, int D, int x_dtype, i
   if (N == 0) return 16;
   const void* at = reinterpret_cast<const void*>(aligned ? 16 : 1);
   const HeadLayout l = head_layout(N, V, D, at, at, x_dtype, w_dtype);
-  const HeadPlan p = head_plan(N, V, D, l.px, x_dtype == NSA_BF16, device_cu_count(static_cast<hipStream_t>(stream)));
+  const HeadPlan p = head_plan(N, V, D, l.px, l.pw, x_dtype == NSA_BF16, device_cu_count(static_cast<hipStream_t>(stream)));
   return l.x_bytes + l.w_bytes + p.dz + p.acc + p.part;
 }
 
@@ -704,7 +900,7 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int cu = device_cu_count(s);
   const HeadLayout l = head_layout(N, V, D, x, w, x_dtype, w_dtype);
-  const HeadPlan p = head_plan(N, V, D, l.px, x_dtype == NSA_BF16, cu);
+  const HeadPlan p = head_plan(N, V, D, l.px, l.pw, x_dtype == NSA_BF16, cu);
   NSA_CHECK(workspace != nullptr && workspace_bytes >= l.x_bytes + l.w_bytes + p.dz + p.acc + p.part,
             NSA_ERR_WORKSPACE);
   char* ws = static_cast<char*>(workspace);
@@ -728,8 +924,7 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
     HeadDz z;
     z.pr.a = {W + (int64_t)v0 * ldw, w_plane, ldw, vocab};
     z.pr.b = {X, x_plane, ldx, (int)N};
-    z.pr.k0 = 0;
-    z.pr.k1 = D;
+    z.pr.K = D;
     z.pr.pa = l.pw;
     z.pr.pb = l.px;
     z.lse = lse;
@@ -759,53 +954,25 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
     if (dx != nullptr) {
       HeadGrad g;
       const bool last = v0 + vocab >= V, lone = p.acc == 0;
-      g.pr.a = {W + (int64_t)v0 * ldw, w_plane, ldw, ldw};
-      g.pr.b = {dz, z_plane, p.piece, (int)N};
-      g.pr.k0 = 0;
-      g.pr.k1 = vocab;
-      g.pr.pa = l.pw;
-      g.pr.pb = l.px;
+      g.pr = {{W + (int64_t)v0 * ldw, w_plane, ldw, ldw}, {dz, z_plane, p.piece, (int)N}, vocab, l.pw, l.px};
       g.out = last || lone ? dx : static_cast<void*>(acc);
       g.out_bf16 = last && x_dtype == NSA_BF16;
       g.add = v0 == 0 ? nullptr : lone ? static_cast<const float*>(dx) : acc;
-      g.part = 0;
-      g.k_part = (vocab + kStep - 1) / kStep * kStep;
+      g.part = part;
       g.N = (int)N;
       g.D = D;
-      g.m_tiles = (D + 255) / 256;
-      g.n_tiles = (int)((N + 255) / 256);
-      if ((int64_t)g.m_tiles * g.n_tiles >= cu) {
-        k_head_grad<HeadBig, true><<<(unsigned)(g.m_tiles * g.n_tiles), 256, 0, s>>>(g);
-      } else {
-        g.m_tiles = (D + 127) / 128;
-        g.n_tiles = (int)((N + 127) / 128);
-        k_head_grad<HeadMid, true><<<(unsigned)(g.m_tiles * g.n_tiles), 256, 0, s>>>(g);
-      }
+      head_grad<true>(g, cu, s);
     }
     if (dw != nullptr) {
       HeadGrad g;
-      const bool one = p.w_parts == 1, to_bf16 = w_dtype == NSA_BF16;
-      char* to = static_cast<char*>(dw) + (int64_t)v0 * D * (to_bf16 ? 2 : 4);
-      g.pr.a = {X, x_plane, ldx, ldx};
-      g.pr.b = {dz, z_plane, p.piece, p.piece};
-      g.pr.k0 = 0;
-      g.pr.k1 = (int)N;
-      g.pr.pa = l.px;
-      g.pr.pb = l.px;
-      g.out = one ? static_cast<void*>(to) : static_cast<void*>(part);
-      g.out_bf16 = one && to_bf16;
+      g.pr = {{X, x_plane, ldx, ldx}, {dz, z_plane, p.piece, p.piece}, (int)N, l.px, l.px};
+      g.out = static_cast<char*>(dw) + (int64_t)v0 * D * (w_dtype == NSA_BF16 ? 2 : 4);
+      g.out_bf16 = w_dtype == NSA_BF16;
       g.add = nullptr;
-      g.part = (int64_t)p.piece * D;
-      g.k_part = p.k_part;
+      g.part = part;
       g.N = vocab;
       g.D = D;
-      g.m_tiles = (D + 255) / 256;
-      g.n_tiles = (vocab + 255) / 256;
-      k_head_grad<HeadBig, false><<<dim3((unsigned)(g.m_tiles * g.n_tiles), 1, (unsigned)p.w_parts), 256, 0, s>>>(g);
-      if (!one) {
-        const int64_t n = (int64_t)vocab * D, blocks = (n + 2047) / 2048;
-        k_head_sum<<<(unsigned)(blocks < 65536 ? blocks : 65536), 256, 0, s>>>(part, g.part, p.w_parts, to, to_bf16, n);
-      }
+      head_grad<false>(g, cu, s);
     }
   }
   return nsa_launch_status();

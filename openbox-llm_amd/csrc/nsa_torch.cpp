@@ -634,7 +634,7 @@ std::tuple<OptTensor, Tensor> linear_logprobs(const Tensor& x_, const Tensor& w_
   no_tangent(has_tangent(x_) || has_tangent(w_), what);
   check_tensor(x_, what);
   check_tensor(w_, what);
-  NSA_ASSERT(w_.dim() == 2 && w_.size(0) >= 1 && w_.size(0) <= (1 << 28) && w_.size(1) >= 1 && w_.size(1) <= 65536,
+  NSA_ASSERT(w_.dim() == 2 && w_.size(0) >= 1 && w_.size(0) <= (1 << 24) && w_.size(1) >= 1 && w_.size(1) <= 65536,
              "linear_logprobs: weight must be [V, D]");
   const int64_t D = w_.size(1);
   NSA_ASSERT(x_.dim() >= 1 && x_.size(-1) == D && x_.device() == w_.device(), "linear_logprobs: x must be [..., D]");

@@ -65,7 +65,7 @@ def test_head_refusals():
     def bwd(N=4, V=10, D=8, xt=1, wt=1, x=None, dlogp=None, dx=16):
         return lib.nsa_head_bwd(x, x, None, None, x, dlogp, None, dx, None, None, 0, N, V, D, xt, wt, None)
     assert fwd(N=0) == 0 and bwd(N=0) == SHAPE
-    for bad in (dict(N=-1), dict(N=(1 << 22) + 1), dict(V=0), dict(V=(1 << 28) + 1), dict(D=0), dict(D=65537)):
+    for bad in (dict(N=-1), dict(N=(1 << 22) + 1), dict(V=0), dict(V=(1 << 24) + 1), dict(D=0), dict(D=65537)):
         assert fwd(**bad) == SHAPE and bwd(**bad) == SHAPE, bad
         full = {**dict(N=4, V=10, D=8), **bad}
         assert lib.nsa_head_fwd_workspace(*full.values(), 1, 1, 1, None) == 0
