@@ -34,9 +34,6 @@ constexpr int kHeadVocab = 1 << 24;
 constexpr int kHeadWide = 1 << 16;           // widest row
 constexpr size_t kHeadPiece = 512u << 20;    // bytes of dz held at a time
 constexpr int64_t kHeadPieceMost = 1 << 20;  // most tokens of a piece: offsets within a stage have 32 bits
-constexpr int kStep = 64;                    // contraction elements of a stage
-
-__device__ const uint4 g_head_zero = {0, 0, 0, 0};   // what elements past an end are read from
 
 // An operand of a product: bf16 planes; ROWS: [rows][ld], contraction along a row;
 // otherwise [contraction][ld].
@@ -44,7 +41,8 @@ struct HeadOperand {
   const bf16* p;
   int64_t plane;   // elements between planes
   int64_t ld;      // elements between rows, a multiple of 8
-  int rows;        // rows (ROWS) or columns, for clamping: what lies past them is never stored
+  int rows;        // rows (ROWS) or columns: of the result
+  int k_rows;      // not ROWS: contraction elements that exist in memory (at least K)
 };
 
 // One product C[m][n] = sum over plane pairs and k < K of A[m][k] B[n][k].
@@ -72,62 +70,60 @@ __device__ __forceinline__ void head_pair(int pa, int pb, int i, int& x, int& y)
 // A stage of one operand: T rows (ROWS) or columns x kStep contraction elements, in
 // 16-byte chunks.  Chunks are swizzled so that 16 neighbouring lanes' 16-byte reads, or
 // the transposed reads' 32-byte pieces of four rows, meet every bank once.
-template <int T, bool ROWS>
+template <int T, int kStep, bool ROWS>
 struct HeadTile {
   static constexpr int kElems = T * kStep;
-  static constexpr int kLoads = T * 8 / 256;      // requests a thread, 256 chunks each
-  static constexpr int kCpr = ROWS ? 8 : T / 8;   // chunks a row of the stage
+  static constexpr int kLoads = kElems / 8 / 256;         // requests a thread, 256 chunks each
+  static constexpr int kCpr = ROWS ? kStep / 8 : T / 8;   // chunks a row of the stage
   static constexpr int kRows = 256 / kCpr;        // rows of the stage a request
-  static_assert(T % 32 == 0 && (ROWS || T == 256), "a tile of whole requests");
+  static_assert(kElems % 2048 == 0 && (ROWS || T == 256), "a tile of whole requests");
   static __device__ __forceinline__ int key(int r) {
-    return ROWS ? (r >> 1) & 7 : 4 * (r & 3) + ((r >> 2) & 3);
+    return !ROWS ? 4 * (r & 3) + ((r >> 2) & 3) : kStep == 64 ? (r >> 1) & 7 : (r >> 2) & 3;
   }
 
-  // Request j brings rows j kRows + tid / kCpr; the key of such a row depends on j
-  // through its parity alone (ROWS: not at all), so that two offsets serve all.
-  uint32_t off[2];
-  const bf16* base;   // the next stage's rows (columns) `first` .., elements k ..
-  int first, left;    // left: K - k
-  __device__ __forceinline__ void init(const HeadOperand& o, int tid) {
+  // Request j brings rows j kRows + tid / kCpr of the stage, each lane 16 bytes.  Past
+  // the operand its last row (first column) is read: what is past the result's last row
+  // (column) is never stored, and past the contraction's end one of the two operands
+  // (packed rows, dz) has zeros in memory up to a whole stage.
+  uint32_t off[kLoads];   // bytes from the stage's base
+  uint64_t base;          // the next stage's rows (columns) `first` .., elements k ..: wave-uniform
+  int first, left;        // left: contraction elements from k on that exist
+  __device__ __forceinline__ void place(const HeadOperand& o, int tid) {
+    const int last = o.rows - 1 - first, end = left - 1;   // >= 0
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int r = tid / kCpr, c = (tid % kCpr) ^ key(j * kRows + r);
-      off[j] = (uint32_t)(r * o.ld * 2 + c * 16);
+    for (int j = 0; j < kLoads; ++j) {
+      const int r = j * kRows + tid / kCpr, c = (tid % kCpr) ^ key(r);
+      if (ROWS)
+        off[j] = (uint32_t)((r < last ? r : last) * o.ld * 2 + c * 16);
+      else
+        off[j] = (uint32_t)((r < end ? r : end) * o.ld * 2 + (8 * c <= last ? c * 16 : 0));
     }
   }
-  __device__ __forceinline__ void aim(const HeadOperand& o, int first_, int pl, int k, int K) {
+  __device__ __forceinline__ void aim(const HeadOperand& o, int first_, int pl, int k, int tid) {
     first = first_;
-    left = K - k;
-    base = o.p + pl * o.plane + (ROWS ? (int64_t)first * o.ld + k : (int64_t)k * o.ld + first);
+    left = o.k_rows - k;
+    const bf16* p = o.p + pl * o.plane + (ROWS ? (int64_t)first * o.ld + k : (int64_t)k * o.ld + first);
+    base = (uint64_t)(uintptr_t)p;
+    base = u64_from_halves(__builtin_amdgcn_readfirstlane((uint32_t)base),
+                           __builtin_amdgcn_readfirstlane((uint32_t)(base >> 32)));
+    place(o, tid);
   }
-  __device__ __forceinline__ void next(const HeadOperand& o) {
+  __device__ __forceinline__ void next(const HeadOperand& o, int tid) {
     left -= kStep;
-    base += ROWS ? (int64_t)kStep : kStep * o.ld;
+    base += ROWS ? (uint64_t)(kStep * 2) : (uint64_t)o.ld * (kStep * 2);
+    if (!ROWS && left < kStep) place(o, tid);
   }
-  // Requests j0 .. j1 - 1: rows (columns) past the operand's last one are any, elements
-  // from K on zeros.
-  template <int J0, int J1>
-  __device__ __forceinline__ void request(const HeadOperand& o, bf16* lds, int tid) const {
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    if (left >= kStep && first + T <= o.rows) {
-#pragma unroll
-      for (int j = J0; j < J1; ++j)
-        lds_dma16_sbase(base + j * kRows * o.ld, off[j & 1], lds + (j * 256 + 64 * w) * 8);
-    } else {
-      const int last = o.rows - 1 - first;   // >= 0
-#pragma unroll 1
-      for (int j = J0; j < J1; ++j) {
-        const int r = j * kRows + tid / kCpr, c = (tid % kCpr) ^ key(r);
-        const bf16* src = base + (ROWS ? (r < last ? r : last) * o.ld + 8 * c : r * o.ld + (8 * c <= last ? 8 * c : 0));
-        if (ROWS ? 8 * c >= left : r >= left) src = reinterpret_cast<const bf16*>(&g_head_zero);
-        lds_dma16(src, lds + (j * 256 + 64 * w) * 8);
-      }
-    }
+  // Request J of a stage; lds: the wave's place in it.
+  template <int J>
+  __device__ __forceinline__ void request(uint32_t lds) const {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + J * 4096), "v"(off[J]),
+                 "s"(base)
+                 : "memory", "m0");
   }
   // Fragments of a wave: of the 32-row tile i from row w0 on (a multiple of 32, of 128
   // where there are several and not ROWS), row m (PERM: perm32(m)), contraction
-  // elements 16 s + 8 h .. + 7.  `at` is the lane's byte address in a stage for i = s =
-  // 0; i and s enter by addition, or by exclusive or where the swizzle has their bits.
+  // elements 16 s + 8 h .. + 7.  `at` is the lane's byte address in LDS (stages lie on
+  // 16 KB) for i = s = 0; i and s enter by addition, or by exclusive or where the swizzle has their bits.
   template <bool PERM>
   static __device__ __forceinline__ uint32_t lane_at(int w0, int lane) {
     if (ROWS) {
@@ -140,13 +136,16 @@ struct HeadTile {
     const int col = w0 + 16 * (g & 1) + 4 * q;
     return (uint32_t)(r * T * 2 + (((col >> 3) ^ key(r)) << 4) + (col & 7) * 2);
   }
-  static __device__ __forceinline__ bf16x8 frag(const char* stage, uint32_t at, int i, int s) {
+  static __device__ __forceinline__ bf16x8 frag(uint32_t at, int i, int s) {
+#define NSA_LDS(type, a) ((__attribute__((address_space(3))) type*)(uintptr_t)(a))
     if constexpr (ROWS) {
-      return *reinterpret_cast<const bf16x8*>(stage + (at ^ (32 * s)) + 32 * i * kStep * 2);
+      return *NSA_LDS(bf16x8, (at ^ (32 * s)) + 32 * i * kStep * 2);
     } else {
       typedef short s16x8 __attribute__((ext_vector_type(8)));
       const uint32_t a0 = at ^ (64 * i), a1 = a0 ^ 16;   // (rows r + 4: another key by 1)
-      const s16x4 u = lds_read_tr16(stage + a0 + 16 * s * T * 2), v = lds_read_tr16(stage + a1 + (16 * s + 4) * T * 2);
+      const s16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16(NSA_LDS(s16x4, a0 + 16 * s * T * 2));
+      const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(NSA_LDS(s16x4, a1 + (16 * s + 4) * T * 2));
+#undef NSA_LDS
       const s16x8 f = (s16x8){u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
       return __builtin_bit_cast(bf16x8, f);
     }
@@ -154,9 +153,9 @@ struct HeadTile {
 };
 
 // Tile shape: TM x TN of the result over WM x WN waves (four), NS stages.
-template <int TM_, int TN_, int WM_, int WN_, int NS_>
+template <int TM_, int TN_, int WM_, int WN_, int NS_, int KSTEP_, int PER_CU_>
 struct HeadShape {
-  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, NS = NS_;
+  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, NS = NS_, kStep = KSTEP_, kPerCu = PER_CU_;
   static constexpr int MT = TM / WM / 32, NT = TN / WN / 32;   // 32 x 32 tiles of a wave
   static_assert(WM * WN == 4 && MT >= 1 && NT >= 1 && NS >= 2, "four waves");
 };
@@ -166,48 +165,56 @@ struct HeadShape {
 struct HeadSpan {
   int m, n, q0, q1;
 };
+template <class S>
 __device__ __forceinline__ int head_steps(const HeadProduct& pr) {
-  return head_pairs(pr.pa, pr.pb) * ((pr.K + kStep - 1) / kStep);
+  return head_pairs(pr.pa, pr.pb) * ((pr.K + S::kStep - 1) / S::kStep);
 }
 
-template <int N, int I = 0, typename F>
-__device__ __forceinline__ void head_each(F& f) {
-  f(std::integral_constant<int, I>{});
-  if constexpr (I + 1 < N) head_each<N, I + 1>(f);
+// f(I), f(I + 1), .. f(N - 1) with constants
+template <int I, int N, typename F>
+__device__ __forceinline__ void head_range(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    head_range<I + 1, N>(f);
+  }
 }
 
 // The spans i = 0 .. spans - 1, `total` steps in all; done(span, wm, wn, acc) takes each result.
 //
-// All steps of all spans are one pipeline of NS stages in LDS.  A wave holds the
-// fragments of 16 contraction elements while it reads those of the next 16; the
-// barrier between two stages stands before the products of a stage's last 16, whose
-// fragments are in registers by then, so that neither it nor the first reads of the
-// next stage leave the matrix units idle, and the stage's memory is asked to be
-// filled again at once.
+// All steps of all spans are one pipeline of NS stages in LDS.  One wave a SIMD leaves
+// the matrix unit idle wherever more than half a dozen other instructions stand between
+// two products, so that everything else is spread: a wave reads the fragments of the
+// next 16 contraction elements and requests a part of a later stage behind each
+// product, with addresses that take one addition a stage.  The barrier between two
+// stages stands before the products of the last 16 elements of the older one, whose
+// fragments are in registers by then; its memory is requested anew from there on (the
+// last stages once more where there are none left, so that every step is alike).
 template <class S, bool AROWS, bool BROWS, typename Span, typename Done>
 __device__ __forceinline__ void head_product(const HeadProduct& pr, int spans, int total, Span span, Done done) {
-  using TA = HeadTile<S::TM, AROWS>;
-  using TB = HeadTile<S::TN, BROWS>;
-  constexpr int kLoads = TA::kLoads + TB::kLoads, KS = kStep / 16;
+  constexpr int kStep = S::kStep;
+  using TA = HeadTile<S::TM, kStep, AROWS>;
+  using TB = HeadTile<S::TN, kStep, BROWS>;
+  constexpr int kLoads = TA::kLoads + TB::kLoads, KS = kStep / 16, MT = S::MT, NT = S::NT;
   static_assert(KS % 2 == 0, "two sets of fragments in turn");
-  __shared__ __align__(1024) bf16 sa[S::NS][TA::kElems];
-  __shared__ __align__(1024) bf16 sb[S::NS][TB::kElems];
+  __shared__ __align__(16384) bf16 sa[S::NS][TA::kElems];
+  __shared__ __align__(16384) bf16 sb[S::NS][TB::kElems];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = (w % S::WM) * S::MT * 32, wn = (w / S::WM) * S::NT * 32;
+  const int wm = (w % S::WM) * MT * 32, wn = (w / S::WM) * NT * 32;
   const int ksteps = (pr.K + kStep - 1) / kStep;
-  // the next request: span, step of it, plane pair
+  const uint32_t at_a = lds_addr_uniform(sa), at_b = lds_addr_uniform(sb);
+  const uint32_t la = at_a + TA::template lane_at<true>(wm, lane), lb = at_b + TB::template lane_at<false>(wn, lane);
+  // the next request: span, step of it, plane pair, place
   TA ta;
   TB tb;
-  ta.init(pr.a, tid);
-  tb.init(pr.b, tid);
-  int ri = 0, rst = 0, asked = 0, rq, rp, pair_left;
+  int ri = 0, asked = 0, rq, rp, pair_left, rst = 0;
+  uint32_t ra = at_a + 1024 * w, rb = at_b + 1024 * w;
   HeadSpan rs;
   auto aim = [&](int k) {
     int x, y;
     head_pair(pr.pa, pr.pb, rp, x, y);
-    ta.aim(pr.a, rs.m * S::TM, x, k, pr.K);
-    tb.aim(pr.b, rs.n * S::TN, y, k, pr.K);
+    ta.aim(pr.a, rs.m * S::TM, x, k, tid);
+    tb.aim(pr.b, rs.n * S::TN, y, k, tid);
   };
   auto start = [&]() {
     rs = span(ri);
@@ -217,93 +224,114 @@ __device__ __forceinline__ void head_product(const HeadProduct& pr, int spans, i
     aim(k * kStep);
   };
   start();
-  // part P of MT of the next stage's requests; the last one moves on
-  auto request = [&](auto part) {
-    constexpr int P = decltype(part)::value, PA = TA::kLoads, PB = TB::kLoads;
-    ta.template request<PA * P / S::MT, PA*(P + 1) / S::MT>(pr.a, sa[rst], tid);
-    tb.template request<PB * P / S::MT, PB*(P + 1) / S::MT>(pr.b, sb[rst], tid);
-    if constexpr (P == S::MT - 1) {
-      ++asked;
-      rst = rst + 1 == S::NS ? 0 : rst + 1;
-      ta.next(pr.a);
-      tb.next(pr.b);
-      if (++rq == rs.q1) {
-        if (++ri < spans) start();
-      } else if (--pair_left == 0) {
-        ++rp;
-        pair_left = ksteps;
-        aim(0);
-      }
+  auto request_next = [&]() {   // behind the requests of a stage
+    rst = rst + 1 == S::NS ? 0 : rst + 1;
+    ra = at_a + 1024 * w + rst * TA::kElems * 2;
+    rb = at_b + 1024 * w + rst * TB::kElems * 2;
+    if (++asked >= total) return;
+    ++rq;
+    if (rq == rs.q1) {
+      ++ri;
+      start();
+    } else if (--pair_left == 0) {
+      ++rp;
+      pair_left = ksteps;
+      aim(0);
+    } else {
+      ta.next(pr.a, tid);
+      tb.next(pr.b, tid);
     }
   };
-  bf16x8 fa[2][S::MT], fb[2][S::NT];
-  uint32_t la = TA::template lane_at<true>(wm, lane), lb = TB::template lane_at<false>(wn, lane);
-  auto read = [&](int set, int st, int ks) {
-    const char *A = reinterpret_cast<const char*>(sa[st]), *B = reinterpret_cast<const char*>(sb[st]);
-#pragma unroll
-    for (int i = 0; i < S::MT; ++i) fa[set][i] = TA::frag(A, la, i, ks);
-#pragma unroll
-    for (int j = 0; j < S::NT; ++j) fb[set][j] = TB::frag(B, lb, j, ks);
+  // requests lo .. hi - 1 of a stage
+  auto request = [&](auto lo_, auto hi_) {
+    head_range<decltype(lo_)::value, decltype(hi_)::value>([&](auto d_) {
+      constexpr int d = decltype(d_)::value;
+      if constexpr (d < TA::kLoads)
+        ta.template request<d>(ra);
+      else
+        tb.template request<d - TA::kLoads>(rb);
+    });
   };
-  auto meet = [&]() {   // (this wave's LDS reads are done, and everybody's)
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  bf16x8 fa[2][MT], fb[2][NT];
+  f32x16 acc[MT][NT];
+  uint32_t sla = la, slb = lb;   // the stage being read
+  // Substep C's products, one a slot; behind them the fragments of substep R are read
+  // and the share of a stage's requests that slots S0 .. of kDmaSlots have is made.
+  constexpr int kSlots = MT * NT, kReadSlots = kSlots > 4 ? kSlots * 3 / 4 : kSlots;
+  constexpr int kDmaSlots = kSlots * (S::NS == 2 ? KS - 1 : KS);
+  auto substep = [&](auto c_, auto r_, auto s0_) {
+    constexpr int C = decltype(c_)::value, R = decltype(r_)::value, S0 = decltype(s0_)::value;
+    head_range<0, kSlots>([&](auto n_) {
+      constexpr int n = decltype(n_)::value, i = n / NT, j = n % NT;
+      acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[C & 1][i], fb[C & 1][j], acc[i][j], 0, 0, 0);
+      if constexpr (n < kReadSlots) {
+        constexpr int lo = (MT + NT) * n / kReadSlots, hi = (MT + NT) * (n + 1) / kReadSlots;
+#pragma unroll
+        for (int f = lo; f < hi; ++f) {
+          if (f < MT)
+            fa[R & 1][f] = TA::frag(sla, f, R);
+          else
+            fb[R & 1][f - MT] = TB::frag(slb, f - MT, R);
+        }
+      }
+      if constexpr (S0 + n < kDmaSlots)
+        request(std::integral_constant<int, kLoads*(S0 + n) / kDmaSlots>{},
+                std::integral_constant<int, kLoads*(S0 + n + 1) / kDmaSlots>{});
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  auto clear = [&]() {   // (a product of zeros writes 16 registers in the time of eight moves)
+    bf16x8 none = {0, 0, 0, 0, 0, 0, 0, 0};
+    const f32x16 zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        asm volatile("" : "+v"(none));
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(none, none, zero, 0, 0, 0);
+      }
+  };
+  auto arrive = [&]() {   // everybody's part of the next stage, behind which NS - 2 are under way
+    vm_wait<(S::NS - 2) * kLoads>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (this wave has read the stage before)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
+  constexpr std::integral_constant<int, 0> zero;
+  constexpr std::integral_constant<int, kLoads> all;
+  constexpr std::integral_constant<int, kLoads * kSlots / kDmaSlots> begun;   // requests made in the last substep
+#pragma unroll 1
+  for (int i = 0; i < S::NS - 1; ++i) {
+    request(zero, all);
+    request_next();
+  }
+  arrive();
 #pragma unroll
-  for (int i = 0; i < S::NS; ++i)
-    if (asked < total) head_each<S::MT>(request);
-  if (total >= S::NS)
-    vm_wait<(S::NS - 1) * kLoads>();
-  else
-    vm_wait<0>();
-  meet();
-  read(0, 0, 0);
-  f32x16 acc[S::MT][S::NT];
-  int it = 0, st = 0;
+  for (int i = 0; i < MT; ++i) fa[0][i] = TA::frag(sla, i, 0);
+#pragma unroll
+  for (int j = 0; j < NT; ++j) fb[0][j] = TB::frag(slb, j, 0);
+  request(zero, begun);
+  int st = 0;
+#pragma unroll 1
   for (int sp = 0; sp < spans; ++sp) {
     const HeadSpan cur = span(sp);
-#pragma unroll
-    for (int i = 0; i < S::MT; ++i)
-#pragma unroll
-      for (int j = 0; j < S::NT; ++j)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-    for (int q = cur.q0; q < cur.q1; ++q, ++it) {
-      asm volatile("" : "+v"(la), "+v"(lb));   // (addresses formed here, not kept for every stage)
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        bool refill = false;
-        if (ks + 1 < KS) {
-          read((ks + 1) & 1, st, ks + 1);
-        } else if (it + 1 < total) {
-          // stage it + 1 has arrived when only the NS - 2 younger ones are outstanding
-          if (S::NS > 2 && it + S::NS - 1 < total)
-            vm_wait<(S::NS - 2) * kLoads>();
-          else
-            vm_wait<0>();
-          meet();
-          refill = asked < total;
-          st = st + 1 == S::NS ? 0 : st + 1;
-          read(0, st, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        auto rows = [&](auto row) {   // the requests between the products, which outlast them
-          constexpr int i = decltype(row)::value;
-#pragma unroll
-          for (int j = 0; j < S::NT; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[ks & 1][i], fb[ks & 1][j], acc[i][j], 0, 0, 0);
-          if (ks + 1 == KS) {
-            __builtin_amdgcn_sched_barrier(0);
-            if (refill) request(row);
-            __builtin_amdgcn_sched_barrier(0);
-          }
-        };
-        head_each<S::MT>(rows);
-      }
+    clear();
+#pragma unroll 1
+    for (int left = cur.q1 - cur.q0; left > 0; --left) {
+      head_range<0, KS - 1>([&](auto k_) {
+        constexpr int k = decltype(k_)::value;
+        substep(k_, std::integral_constant<int, k + 1>{}, std::integral_constant<int, kSlots*(k + 1)>{});
+      });
+      request_next();
+      arrive();
+      st = st + 1 == S::NS ? 0 : st + 1;
+      sla = la + st * TA::kElems * 2;
+      slb = lb + st * TB::kElems * 2;
+      substep(std::integral_constant<int, KS - 1>{}, zero, zero);
     }
     done(cur, wm, wn, acc);
   }
+  vm_wait<0>();   // (nothing arrives in LDS that is another's by then)
 }
 
 // Workgroup -> (tile of x's rows, one of `split` lanes over the vocabulary's tiles).
@@ -339,46 +367,44 @@ struct HeadFwd {
 // Log sums over this workgroup's share of the vocabulary.  A lane holds one row of
 // x for each of its NT tiles and 16 MT logits of it at a time.
 template <class S>
-__global__ __launch_bounds__(256, 1) void k_head_fwd(const HeadFwd a) {
+__global__ __launch_bounds__(256, S::kPerCu) void k_head_fwd(const HeadFwd a) {
   int nt, part;
   if (!head_place(a.g, (int)blockIdx.x, nt, part)) return;
   const int lane = threadIdx.x & 63, h = lane >> 5;
   float m[S::NT], l[S::NT];
 #pragma unroll
   for (int j = 0; j < S::NT; ++j) m[j] = kMaskScore, l[j] = 0.0f;
-  const int steps = head_steps(a.pr), tiles = head_share(a.g, part);
+  const int steps = head_steps<S>(a.pr), tiles = head_share(a.g, part);
   head_product<S, true, true>(
       a.pr, tiles, tiles * steps, [&](int i) { return HeadSpan{part + i * a.g.split, nt, 0, steps}; },
       [&](const HeadSpan& sp, int wm, int wn, f32x16(&acc)[S::MT][S::NT]) {
-        const int mt = sp.m, v0 = mt * S::TM + wm + 8 * h;
-        if (mt * S::TM + S::TM > a.V) {   // past the vocabulary: no weight
+        const int left = a.V - (sp.m * S::TM + wm + 8 * h);   // tokens from the lane's first one on
+        auto add = [&](auto inside) {
 #pragma unroll
-          for (int i = 0; i < S::MT; ++i)
+          for (int j = 0; j < S::NT; ++j) {
+            auto z = [&](int i, int r) {   // past the vocabulary: no weight
+              return decltype(inside)::value || 32 * i + acc_elem(0, r) < left ? acc[i][j][r] : -__builtin_inff();
+            };
+            float t = z(0, 0);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const bool out = v0 + 32 * i + acc_elem(0, r) >= a.V;
+            for (int i = 0; i < S::MT; ++i)
 #pragma unroll
-              for (int j = 0; j < S::NT; ++j)
-                if (out) acc[i][j][r] = -__builtin_inff();
-            }
-        }
+              for (int r = 0; r < 16; ++r) t = fmaxf(t, z(i, r));
+            const float mn = fmaxf(m[j], t * kLog2e);
+            float s = 0.0f;
 #pragma unroll
-        for (int j = 0; j < S::NT; ++j) {
-          float t = acc[0][j][0];
+            for (int i = 0; i < S::MT; ++i)
 #pragma unroll
-          for (int i = 0; i < S::MT; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) t = fmaxf(t, acc[i][j][r]);
-          const float mn = fmaxf(m[j], t * kLog2e);
-          float s = 0.0f;
-#pragma unroll
-          for (int i = 0; i < S::MT; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s += fast_exp2(fmaf(acc[i][j][r], kLog2e, -mn));
-          l[j] = l[j] * fast_exp2(m[j] - mn) + s;
-          m[j] = mn;
-          __builtin_amdgcn_sched_barrier(0);   // (one row's values in registers at a time)
-        }
+              for (int r = 0; r < 16; ++r) s += fast_exp2(fmaf(z(i, r), kLog2e, -mn));
+            l[j] = l[j] * fast_exp2(m[j] - mn) + s;
+            m[j] = mn;
+            __builtin_amdgcn_sched_barrier(0);   // (one row's values in registers at a time)
+          }
+        };
+        if (sp.m * S::TM + S::TM <= a.V)
+          add(std::true_type{});
+        else
+          add(std::false_type{});
       });
   // the halves of a wave, then the waves along the vocabulary
   __shared__ float2 st[S::WM][S::TN];
@@ -454,11 +480,11 @@ struct HeadDz {
   HeadGrid g;
   const float *lse, *dlogp, *dlse;   // dlogp, dlse: or null
   const int64_t* target;             // or null
-  bf16* dz;                          // [planes][N][ld]
+  bf16* dz;                          // [planes][N rounded up to 64][ld], zeros past N and past the vocabulary
   int64_t ld, plane;
   int N, V, v0;                      // the piece starts at token v0 (V: of the whole vocabulary)
   int vocab;                         // ... and has so many
-  int planes;
+  int rows;                          // N rounded up to 64
 };
 __device__ __forceinline__ bool head_real(const int64_t* target, int64_t n, int V) {
   return target != nullptr && target[n] >= 0 && target[n] < V;
@@ -477,7 +503,7 @@ __device__ __forceinline__ void store_planes(bf16* p, int64_t plane, float (&v)[
   }
 }
 template <class S, int PLANES>
-__global__ __launch_bounds__(256, 1) void k_head_dz(const HeadDz a) {
+__global__ __launch_bounds__(256, S::kPerCu) void k_head_dz(const HeadDz a) {
   int nt, part;
   if (!head_place(a.g, (int)blockIdx.x, nt, part)) return;
   const int lane = threadIdx.x & 63, h = lane >> 5;
@@ -493,16 +519,17 @@ __global__ __launch_bounds__(256, 1) void k_head_dz(const HeadDz a) {
       if (a.dlogp != nullptr && head_real(a.target, n, a.V)) co[j] -= a.dlogp[n];
     }
   }
-  const int steps = head_steps(a.pr), tiles = head_share(a.g, part);
+  const int steps = head_steps<S>(a.pr), tiles = head_share(a.g, part);
   head_product<S, true, true>(
       a.pr, tiles, tiles * steps, [&](int i) { return HeadSpan{part + i * a.g.split, nt, 0, steps}; },
       [&](const HeadSpan& sp, int wm, int wn, f32x16(&acc)[S::MT][S::NT]) {
         const int mt = sp.m;
-        const bool inside = mt * S::TM + S::TM <= a.vocab;   // else zeros past the vocabulary
+        // else zeros past the vocabulary, and in the rows past N (of any sums, NaN among them)
+        const bool inside = mt * S::TM + S::TM <= a.vocab && nt * S::TN + S::TN <= a.N;
 #pragma unroll
         for (int j = 0; j < S::NT; ++j) {
           const int n = nt * S::TN + wn + 32 * j + (lane & 31);
-          if (n >= a.N) continue;
+          if (n >= a.rows) continue;
 #pragma unroll
           for (int i = 0; i < S::MT; ++i)
 #pragma unroll
@@ -514,7 +541,7 @@ __global__ __launch_bounds__(256, 1) void k_head_dz(const HeadDz a) {
               if (!inside) {
 #pragma unroll
                 for (int r = 0; r < 8; ++r)
-                  if (v + r >= a.vocab) d[r] = 0.0f;
+                  if (v + r >= a.vocab || n >= a.N) d[r] = 0.0f;
               }
               store_planes<PLANES>(a.dz + (int64_t)n * a.ld + v, a.plane, d);
               __builtin_amdgcn_sched_barrier(0);
@@ -559,9 +586,9 @@ struct HeadGrad {
 };
 
 template <class S, bool BROWS>
-__global__ __launch_bounds__(256, 1) void k_head_grad(const HeadGrad a) {
+__global__ __launch_bounds__(256, S::kPerCu) void k_head_grad(const HeadGrad a) {
   const int g = (int)xcd_remap(blockIdx.x, gridDim.x);
-  const int steps = head_steps(a.pr), rounds = a.whole / a.groups;
+  const int steps = head_steps<S>(a.pr), rounds = a.whole / a.groups;
   const int rest = a.m_tiles * a.n_tiles - a.whole, units = rest * a.cuts;
   // whole tiles, then units g, g + groups, ..: unit u is part u / rest of tile whole + u % rest
   auto span = [&](int i) {
@@ -691,9 +718,10 @@ __global__ __launch_bounds__(256) void k_head_pack(const void* x, bool x_bf16, b
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-using HeadBig = HeadShape<256, 256, 2, 2, 2>;
-using HeadMid = HeadShape<128, 128, 2, 2, 2>;
-using HeadFew = HeadShape<128, 32, 4, 1, 4>;
+using HeadBig = HeadShape<256, 256, 2, 2, 2, 64, 1>;
+using HeadTwo = HeadShape<256, 128, 2, 2, 3, 32, 2>;
+using HeadMid = HeadShape<128, 128, 2, 2, 2, 64, 2>;
+using HeadFew = HeadShape<128, 32, 4, 1, 4, 64, 1>;
 
 static bool head_type(int dtype) { return dtype == NSA_F32 || dtype == NSA_BF16; }
 static bool head_shape_ok(int64_t N, int V, int D) {
@@ -713,9 +741,9 @@ static HeadLayout head_layout(int64_t N, int V, int D, const void* x, const void
   l.px = wide ? 3 : 1;
   l.pw = wide && w_dtype == NSA_F32 ? 3 : 1;
   l.ld = (D + 63) / 64 * 64;
-  // rows are requested in aligned pieces of 16 bytes
-  l.pack_x = wide || D % 8 != 0 || reinterpret_cast<uintptr_t>(x) % 16 != 0;
-  l.pack_w = w_dtype == NSA_F32 || D % 8 != 0 || reinterpret_cast<uintptr_t>(w) % 16 != 0;
+  // rows are requested in whole stages, aligned pieces of 16 bytes
+  l.pack_x = wide || D % 64 != 0 || reinterpret_cast<uintptr_t>(x) % 16 != 0;
+  l.pack_w = w_dtype == NSA_F32 || D % 64 != 0 || reinterpret_cast<uintptr_t>(w) % 16 != 0;
   l.x_bytes = l.pack_x ? up16((size_t)l.px * N * l.ld * 2) : 0;
   l.w_bytes = l.pack_w ? up16((size_t)l.pw * V * l.ld * 2) : 0;
   return l;
@@ -766,7 +794,7 @@ struct HeadCut {
 static HeadCut head_cut(int64_t rows, int D, int K, int pairs, int cu) {
   using S = HeadGradShape;
   const int64_t m = (D + S::TM - 1) / S::TM, n = (rows + S::TN - 1) / S::TN, tiles = m * n;
-  const int64_t steps = (int64_t)pairs * ((K + kStep - 1) / kStep);
+  const int64_t steps = (int64_t)pairs * ((K + S::kStep - 1) / S::kStep);
   HeadCut c{cu, (int)(tiles / cu * cu), 1, 0};
   const int64_t rest = tiles - c.whole;
   if (rest > 0) {
@@ -804,11 +832,11 @@ struct HeadPlan {
 static HeadPlan head_plan(int64_t N, int V, int D, int planes, int pw, bool x_bf16, int cu) {
   HeadPlan p;
   const int64_t all = ((int64_t)V + 255) / 256 * 256;
-  int64_t fit = (int64_t)(kHeadPiece / ((size_t)N * 2 * planes)) / 256 * 256;
+  int64_t fit = (int64_t)(kHeadPiece / ((size_t)((N + 63) / 64 * 64) * 2 * planes)) / 256 * 256;
   fit = fit < 256 ? 256 : fit < kHeadPieceMost ? fit : kHeadPieceMost;
   const int64_t pieces = (all + fit - 1) / fit;
   p.piece = (int)(((all + pieces - 1) / pieces + 255) / 256 * 256);
-  p.dz = up16((size_t)planes * N * p.piece * 2);
+  p.dz = up16((size_t)planes * ((N + 63) / 64 * 64) * p.piece * 2);
   p.acc = all > p.piece && x_bf16 ? up16((size_t)N * D * 4) : 0;
   // the parts of dx and dW of a whole piece and of the last one
   const int last = (int)(V - (int64_t)(V - 1) / p.piece * p.piece);
@@ -862,8 +890,8 @@ extern "C" int nsa_head_fwd(const void* x, const void* w, const int64_t* target,
     if (l.pack_x) head_pack(x, x_dtype, xp, N, D, l.ld, l.px, s);
     if (l.pack_w) head_pack(w, w_dtype, wp, V, D, l.ld, l.pw, s);
     HeadFwd a;
-    a.pr.a = {l.pack_w ? wp : static_cast<const bf16*>(w), (int64_t)V * l.ld, l.pack_w ? l.ld : D, V};
-    a.pr.b = {l.pack_x ? xp : static_cast<const bf16*>(x), N * l.ld, l.pack_x ? l.ld : D, (int)N};
+    a.pr.a = {l.pack_w ? wp : static_cast<const bf16*>(w), (int64_t)V * l.ld, l.pack_w ? l.ld : D, V, 0};
+    a.pr.b = {l.pack_x ? xp : static_cast<const bf16*>(x), N * l.ld, l.pack_x ? l.ld : D, (int)N, 0};
     a.pr.K = D;
     a.pr.pa = l.pw;
     a.pr.pb = l.px;
@@ -918,12 +946,12 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
   const int ldx = l.pack_x ? l.ld : D, ldw = l.pack_w ? l.ld : D;
   const bf16* X = l.pack_x ? xp : static_cast<const bf16*>(x);
   const bf16* W = l.pack_w ? wp : static_cast<const bf16*>(w);
-  const int64_t x_plane = N * (int64_t)l.ld, w_plane = (int64_t)V * l.ld, z_plane = N * (int64_t)p.piece;
+  const int64_t x_plane = N * (int64_t)l.ld, w_plane = (int64_t)V * l.ld, z_plane = (N + 63) / 64 * 64 * (int64_t)p.piece;
   for (int v0 = 0; v0 < V; v0 += p.piece) {
     const int vocab = V - v0 < p.piece ? V - v0 : p.piece;
     HeadDz z;
-    z.pr.a = {W + (int64_t)v0 * ldw, w_plane, ldw, vocab};
-    z.pr.b = {X, x_plane, ldx, (int)N};
+    z.pr.a = {W + (int64_t)v0 * ldw, w_plane, ldw, vocab, 0};
+    z.pr.b = {X, x_plane, ldx, (int)N, 0};
     z.pr.K = D;
     z.pr.pa = l.pw;
     z.pr.pb = l.px;
@@ -938,15 +966,19 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
     z.V = V;
     z.v0 = v0;
     z.vocab = vocab;
-    z.planes = l.px;
-    head_as(head_kind(N, vocab, cu), [&](auto sh) {
+    z.rows = (int)((N + 63) / 64 * 64);
+    auto form = [&](auto sh) {   // (its tiles cover dz's rows of zeros)
       using S = decltype(sh);
       z.g = head_grid<S>(N, vocab, cu);
       if (l.px == 3)
         k_head_dz<S, 3><<<head_blocks(z.g), 256, 0, s>>>(z);
       else
         k_head_dz<S, 1><<<head_blocks(z.g), 256, 0, s>>>(z);
-    });
+    };
+    if (head_kind(N, vocab, cu) == kBig)
+      form(HeadBig{});
+    else
+      form(HeadMid{});
     if (l.px == 3)
       k_head_target<3><<<(unsigned)((N + 255) / 256), 256, 0, s>>>(z, logp);
     else
@@ -954,7 +986,7 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
     if (dx != nullptr) {
       HeadGrad g;
       const bool last = v0 + vocab >= V, lone = p.acc == 0;
-      g.pr = {{W + (int64_t)v0 * ldw, w_plane, ldw, ldw}, {dz, z_plane, p.piece, (int)N}, vocab, l.pw, l.px};
+      g.pr = {{W + (int64_t)v0 * ldw, w_plane, ldw, ldw, vocab}, {dz, z_plane, p.piece, (int)N, 0}, vocab, l.pw, l.px};
       g.out = last || lone ? dx : static_cast<void*>(acc);
       g.out_bf16 = last && x_dtype == NSA_BF16;
       g.add = v0 == 0 ? nullptr : lone ? static_cast<const float*>(dx) : acc;
@@ -965,7 +997,7 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
     }
     if (dw != nullptr) {
       HeadGrad g;
-      g.pr = {{X, x_plane, ldx, ldx}, {dz, z_plane, p.piece, p.piece}, (int)N, l.px, l.px};
+      g.pr = {{X, x_plane, ldx, ldx, (int)N}, {dz, z_plane, p.piece, p.piece, z.rows}, (int)N, l.px, l.px};
       g.out = static_cast<char*>(dw) + (int64_t)v0 * D * (w_dtype == NSA_BF16 ? 2 : 4);
       g.out_bf16 = w_dtype == NSA_BF16;
       g.add = nullptr;
