@@ -385,19 +385,29 @@ __global__ __launch_bounds__(256, S::kPerCu) void k_head_fwd(const HeadFwd a) {
             auto z = [&](int i, int r) {   // past the vocabulary: no weight
               return decltype(inside)::value || 32 * i + acc_elem(0, r) < left ? acc[i][j][r] : -__builtin_inff();
             };
-            float t = z(0, 0);
+            auto sum = [&](float ref) {
+              float s[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < S::MT; ++i)
+              for (int i = 0; i < S::MT; ++i)
 #pragma unroll
-              for (int r = 0; r < 16; ++r) t = fmaxf(t, z(i, r));
-            const float mn = fmaxf(m[j], t * kLog2e);
-            float s = 0.0f;
+                for (int r = 0; r < 16; ++r) s[r & 1] += fast_exp2(fmaf(z(i, r), kLog2e, -ref));
+              return s[0] + s[1];
+            };
+            // the maximum so far serves while the sum stays in range; the first tile, a
+            // row that grows by 40 bits and one with NaN take their own
+            float s = sum(m[j]);
+            if (__any(!(s < 0x1p40f))) {
+              float t = z(0, 0);
 #pragma unroll
-            for (int i = 0; i < S::MT; ++i)
+              for (int i = 0; i < S::MT; ++i)
 #pragma unroll
-              for (int r = 0; r < 16; ++r) s += fast_exp2(fmaf(z(i, r), kLog2e, -mn));
-            l[j] = l[j] * fast_exp2(m[j] - mn) + s;
-            m[j] = mn;
+                for (int r = 0; r < 16; ++r) t = fmaxf(t, z(i, r));
+              const float mn = fmaxf(m[j], t * kLog2e);
+              s = sum(mn);
+              l[j] *= fast_exp2(m[j] - mn);
+              m[j] = mn;
+            }
+            l[j] += s;
             __builtin_amdgcn_sched_barrier(0);   // (one row's values in registers at a time)
           }
         };
@@ -489,17 +499,19 @@ struct HeadDz {
 __device__ __forceinline__ bool head_real(const int64_t* target, int64_t n, int V) {
   return target != nullptr && target[n] >= 0 && target[n] < V;
 }
+// v as bf16 planes; neg: a sign bit to flip in all of them
 template <int PLANES>
-__device__ __forceinline__ void store_planes(bf16* p, int64_t plane, float (&v)[8]) {
+__device__ __forceinline__ void store_planes(bf16* p, int64_t plane, float (&v)[8], uint32_t neg = 0) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 #pragma unroll
   for (int q = 0; q < PLANES; ++q) {
     bf16x8 o;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       o[j] = (bf16)v[j];
-      v[j] -= (float)o[j];
+      if (q + 1 < PLANES) v[j] -= (float)o[j];
     }
-    *reinterpret_cast<bf16x8*>(p + q * plane) = o;
+    *reinterpret_cast<u32x4*>(p + q * plane) = __builtin_bit_cast(u32x4, o) ^ (neg | neg >> 16);
   }
 }
 template <class S, int PLANES>
@@ -508,15 +520,18 @@ __global__ __launch_bounds__(256, S::kPerCu) void k_head_dz(const HeadDz a) {
   if (!head_place(a.g, (int)blockIdx.x, nt, part)) return;
   const int lane = threadIdx.x & 63, h = lane >> 5;
   const int wn0 = ((threadIdx.x >> 6) / S::WM) * S::NT * 32;
-  float off[S::NT], co[S::NT];   // dz = co 2^(z log2 e - off)
+  float off[S::NT];      // |dz| = 2^(z log2 e - off)
+  uint32_t neg[S::NT];   // dz's sign bit
 #pragma unroll
   for (int j = 0; j < S::NT; ++j) {
     const int n = nt * S::TN + wn0 + 32 * j + (lane & 31);
-    off[j] = co[j] = 0.0f;
+    off[j] = __builtin_inff();   // (nothing weighs anything)
+    neg[j] = 0;
     if (n < a.N) {
-      off[j] = a.lse[n] * kLog2e;
-      co[j] = a.dlse != nullptr ? a.dlse[n] : 0.0f;
-      if (a.dlogp != nullptr && head_real(a.target, n, a.V)) co[j] -= a.dlogp[n];
+      float co = a.dlse != nullptr ? a.dlse[n] : 0.0f;
+      if (a.dlogp != nullptr && head_real(a.target, n, a.V)) co -= a.dlogp[n];
+      off[j] = a.lse[n] * kLog2e - __log2f(fabsf(co));
+      neg[j] = __float_as_uint(co) & 0x80000000u;
     }
   }
   const int steps = head_steps<S>(a.pr), tiles = head_share(a.g, part);
@@ -537,13 +552,13 @@ __global__ __launch_bounds__(256, S::kPerCu) void k_head_dz(const HeadDz a) {
               const int v = mt * S::TM + wm + 32 * i + acc_elem(h, r0);
               float d[8];
 #pragma unroll
-              for (int r = 0; r < 8; ++r) d[r] = co[j] * fast_exp2(fmaf(acc[i][j][r0 + r], kLog2e, -off[j]));
+              for (int r = 0; r < 8; ++r) d[r] = fast_exp2(fmaf(acc[i][j][r0 + r], kLog2e, -off[j]));
               if (!inside) {
 #pragma unroll
                 for (int r = 0; r < 8; ++r)
                   if (v + r >= a.vocab || n >= a.N) d[r] = 0.0f;
               }
-              store_planes<PLANES>(a.dz + (int64_t)n * a.ld + v, a.plane, d);
+              store_planes<PLANES>(a.dz + (int64_t)n * a.ld + v, a.plane, d, neg[j]);
               __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -769,8 +784,14 @@ static HeadGrid head_grid(int64_t N, int vocab, int cu) {
   HeadGrid g;
   g.n_tiles = (int)((N + S::TN - 1) / S::TN);
   g.m_tiles = (vocab + S::TM - 1) / S::TM;
-  const int want = (4 * cu + g.n_tiles - 1) / g.n_tiles;
-  g.split = want < g.m_tiles ? want : g.m_tiles;
+  // rounds of the chip's workgroups, a workgroup's tiles and half a tile to begin and end
+  const int64_t at_once = (int64_t)cu * S::kPerCu;
+  double best = 1e30;
+  g.split = 1;
+  for (int s = 1; s <= g.m_tiles && (s == 1 || (int64_t)s * g.n_tiles <= 4 * at_once); ++s) {
+    const double time = (double)((s * (int64_t)g.n_tiles + at_once - 1) / at_once) * ((g.m_tiles + s - 1) / s + 0.5);
+    if (time < best) best = time, g.split = s;
+  }
   return g;
 }
 static unsigned head_blocks(const HeadGrid& g) {
