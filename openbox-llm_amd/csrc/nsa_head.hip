@@ -76,7 +76,7 @@ struct HeadTile {
   static constexpr int kLoads = kElems / 8 / 256;         // requests a thread, 256 chunks each
   static constexpr int kCpr = ROWS ? kStep / 8 : T / 8;   // chunks a row of the stage
   static constexpr int kRows = 256 / kCpr;        // rows of the stage a request
-  static_assert(kElems % 2048 == 0 && (ROWS || T == 256), "a tile of whole requests");
+  static_assert(kElems % 2048 == 0 && (ROWS || T >= 128), "a tile of whole requests");
   static __device__ __forceinline__ int key(int r) {
     return !ROWS ? 4 * (r & 3) + ((r >> 2) & 3) : kStep == 64 ? (r >> 1) & 7 : (r >> 2) & 3;
   }
@@ -734,7 +734,6 @@ __global__ __launch_bounds__(256) void k_head_pack(const void* x, bool x_bf16, b
 // host
 // ---------------------------------------------------------------------------
 using HeadBig = HeadShape<256, 256, 2, 2, 2, 64, 1>;
-using HeadTwo = HeadShape<256, 128, 2, 2, 3, 32, 2>;
 using HeadMid = HeadShape<128, 128, 2, 2, 2, 64, 2>;
 using HeadFew = HeadShape<128, 32, 4, 1, 4, 64, 1>;
 
@@ -804,45 +803,65 @@ static auto head_as(int kind, F f) {
   return f(HeadBig{});
 }
 
-// The gradients' products: 256 x 256 tiles.  The last round's tiles are cut where that
-// saves more than a part costs: a tile's step takes about 1.1 us, writing and adding its
-// 256 KB part 26.
-using HeadGradShape = HeadBig;
+// The gradients' products: tiles of 256 x 256 or, where those are few, 128 x 128 with
+// two workgroups a compute unit.  The last round's tiles are cut where that saves more
+// than a part costs.  Measured: a step (64 elements) of a 256 x 256 tile 2.1 us, of two
+// 128 x 128 tiles side by side 1.2; writing and adding their parts 26 and 13.
 struct HeadCut {
+  bool big;
   int groups, whole, cuts;
-  int64_t parts;   // tiles of the part buffer
+  int64_t bytes;   // of the parts
 };
-static HeadCut head_cut(int64_t rows, int D, int K, int pairs, int cu) {
-  using S = HeadGradShape;
+template <class S>
+static double head_cut_as(HeadCut& c, int64_t rows, int D, int K, int pairs, int cu) {
+  const double step = S::TM == 256 ? 2.1 : 1.2, part = S::TM == 256 ? 26.0 : 13.0;
   const int64_t m = (D + S::TM - 1) / S::TM, n = (rows + S::TN - 1) / S::TN, tiles = m * n;
-  const int64_t steps = (int64_t)pairs * ((K + S::kStep - 1) / S::kStep);
-  HeadCut c{cu, (int)(tiles / cu * cu), 1, 0};
+  const int64_t steps = (int64_t)pairs * ((K + S::kStep - 1) / S::kStep), at_once = (int64_t)cu * S::kPerCu;
+  c.big = S::TM == 256;
+  c.groups = (int)at_once;
+  c.whole = (int)(tiles / at_once * at_once);
+  c.cuts = 1;
   const int64_t rest = tiles - c.whole;
+  double best = 0.0;
   if (rest > 0) {
-    double best = 1e30;
+    best = 1e30;
     for (int p = 1; p <= 64 && p * 4 <= steps + 3; ++p) {
-      const double time = (double)((rest * p + cu - 1) / cu) * (1.1 * steps / p) + (p > 1 ? 26.0 * rest * p / cu : 0.0);
+      const double rounds = (double)((rest * p + at_once - 1) / at_once);
+      const double time = rounds * (step * steps / p) + (p > 1 ? part * rest * p / at_once + 5.0 : 0.0);
       if (time < best) best = time, c.cuts = p;
     }
-    if (c.whole == 0 && rest * c.cuts < cu) c.groups = (int)(rest * c.cuts);
+    if (c.whole == 0 && rest * c.cuts < at_once) c.groups = (int)(rest * c.cuts);
   }
-  c.parts = (c.cuts > 1 ? rest * c.cuts : 0) + (D % S::TM == 0 ? 0 : n);
-  if (c.cuts == 1) c.parts += rest;   // (the edge's tiles lie behind `rest` unused ones)
-  return c;
+  // (with uncut tiles the edge's lie behind `rest` unused ones)
+  const int64_t parts = (c.cuts > 1 || D % S::TM != 0 ? rest * c.cuts : 0) + (D % S::TM == 0 ? 0 : n);
+  c.bytes = parts * S::TM * S::TN * 4;
+  return best + (double)(c.whole / at_once) * step * steps;
+}
+static HeadCut head_cut(int64_t rows, int D, int K, int pairs, int cu) {
+  HeadCut big, mid;
+  const double tb = head_cut_as<HeadBig>(big, rows, D, K, pairs, cu);
+  const double tm = head_cut_as<HeadMid>(mid, rows, D, K, pairs, cu);
+  return tb <= tm ? big : mid;
 }
 static int head_pair_count(int pa, int pb) { return pb == 1 ? 1 : pa == 1 ? 3 : 6; }
-template <bool BROWS>
-static void head_grad(HeadGrad g, int cu, hipStream_t s) {
-  using S = HeadGradShape;
+template <class S, bool BROWS>
+static void head_grad_as(HeadGrad g, const HeadCut& c, hipStream_t s) {
   g.m_tiles = (g.D + S::TM - 1) / S::TM;
   g.n_tiles = (g.N + S::TN - 1) / S::TN;
-  const HeadCut c = head_cut(g.N, g.D, g.pr.K, head_pair_count(g.pr.pa, g.pr.pb), cu);
   g.groups = c.groups;
   g.whole = c.whole;
   g.cuts = c.cuts;
   k_head_grad<S, BROWS><<<(unsigned)g.groups, 256, 0, s>>>(g);
   const int tiles = g.m_tiles * g.n_tiles, first = g.D % S::TM != 0 ? 0 : c.cuts > 1 ? c.whole : tiles;
   if (first < tiles) k_head_join_tiles<S><<<dim3((unsigned)(tiles - first), 8), 256, 0, s>>>(g, first);
+}
+template <bool BROWS>
+static void head_grad(const HeadGrad& g, int cu, hipStream_t s) {
+  const HeadCut c = head_cut(g.N, g.D, g.pr.K, head_pair_count(g.pr.pa, g.pr.pb), cu);
+  if (c.big)
+    head_grad_as<HeadBig, BROWS>(g, c, s);
+  else
+    head_grad_as<HeadMid, BROWS>(g, c, s);
 }
 
 // The backward's pieces of the vocabulary and its buffers
@@ -863,12 +882,12 @@ static HeadPlan head_plan(int64_t N, int V, int D, int planes, int pw, bool x_bf
   const int last = (int)(V - (int64_t)(V - 1) / p.piece * p.piece);
   int64_t parts = 0;
   for (int vocab : {p.piece < V ? p.piece : V, last}) {
-    const int64_t dx = head_cut(N, D, vocab, head_pair_count(pw, planes), cu).parts;
-    const int64_t dw = head_cut(vocab, D, (int)N, head_pair_count(planes, planes), cu).parts;
+    const int64_t dx = head_cut(N, D, vocab, head_pair_count(pw, planes), cu).bytes;
+    const int64_t dw = head_cut(vocab, D, (int)N, head_pair_count(planes, planes), cu).bytes;
     parts = dx > parts ? dx : parts;
     parts = dw > parts ? dw : parts;
   }
-  p.part = (size_t)parts * HeadGradShape::TM * HeadGradShape::TN * 4;
+  p.part = (size_t)parts;
   return p;
 }
 
