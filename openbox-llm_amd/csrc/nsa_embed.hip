@@ -10,7 +10,8 @@
 //
 //   1. (token, i) pairs are sorted by token with ties by ascending i: a radix sort
 //      of up to 9 bits a pass, each pass two launches (counts of every block of
-//      pairs; places from the counts, ranks within a wave by ballots).  Positions
+//      pairs; places from the counts, ranks within a wave by ballots), or one launch
+//      of one workgroup for up to 4096 pairs.  Positions
 //      0 .. T-1 of every sequence need no sort: the sorted list is a formula.
 //   2. The sorted list is cut into pieces of equal length, whatever the tokens'
 //      frequencies (in text one token can be a tenth of all): a workgroup adds the
@@ -37,29 +38,85 @@ struct EmbedArgs {
   bool w_bf16, pw_bf16, out_bf16;
 };
 
-// TPR threads a row, 256 / TPR rows a workgroup.
-template <int TPR>
+// E elements at any element-aligned address, `n` of them in the row from here on; a
+// float32 row goes by 4 a lane, so that neighbouring lanes' 16 bytes are neighbours.
+template <int E>
+__device__ __forceinline__ void load_some(const void* p, bool is_bf16, int64_t at, int n, float (&f)[E]) {
+  typedef bf16 bf16xE __attribute__((ext_vector_type(E), aligned(2)));
+  typedef float f32xE __attribute__((ext_vector_type(E), aligned(4)));
+  if (n >= E) {
+    if (is_bf16) {
+      const bf16xE v = *reinterpret_cast<const bf16xE*>(static_cast<const bf16*>(p) + at);
+#pragma unroll
+      for (int j = 0; j < E; ++j) f[j] = (float)v[j];
+    } else {
+      const f32xE v = *reinterpret_cast<const f32xE*>(static_cast<const float*>(p) + at);
+#pragma unroll
+      for (int j = 0; j < E; ++j) f[j] = v[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      f[j] = j >= n ? 0.0f : is_bf16 ? (float)static_cast<const bf16*>(p)[at + j] : static_cast<const float*>(p)[at + j];
+  }
+}
+template <int E>
+__device__ __forceinline__ void store_some(void* p, bool is_bf16, int64_t at, int n, const float (&f)[E]) {
+  typedef bf16 bf16xE __attribute__((ext_vector_type(E), aligned(2)));
+  typedef float f32xE __attribute__((ext_vector_type(E), aligned(4)));
+  if (n >= E) {
+    if (is_bf16) {
+      bf16xE v;
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = (bf16)f[j];
+      *reinterpret_cast<bf16xE*>(static_cast<bf16*>(p) + at) = v;
+    } else {
+      f32xE v;
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[j] = f[j];
+      *reinterpret_cast<f32xE*>(static_cast<float*>(p) + at) = v;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (j < n) {
+        if (is_bf16)
+          static_cast<bf16*>(p)[at + j] = (bf16)f[j];
+        else
+          static_cast<float*>(p)[at + j] = f[j];
+      }
+  }
+}
+
+// TPR threads a row, 256 / TPR rows a workgroup; a thread has two runs of E in flight.
+template <int E, int TPR>
 __global__ __launch_bounds__(256) void k_embed_fwd(const EmbedArgs a) {
   const int t = threadIdx.x & (TPR - 1);
   const int64_t i = a.first + (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
   if (i >= a.n) return;
   const int64_t tok = a.tokens[i];
   const bool real = tok >= 0 && tok < a.V;
-  const int64_t p = a.pw == nullptr ? 0 : a.pos != nullptr ? a.pos[i] : i % a.T;
+  // (fewer than 2^31 rows: a 32-bit remainder)
+  const int64_t p = a.pw == nullptr ? 0 : a.pos != nullptr ? a.pos[i] : (int64_t)((uint32_t)i % (uint32_t)a.T);
   const bool has_pos = a.pw != nullptr && p >= 0 && p < a.P;
   const int D = a.D;
-#pragma unroll 2
-  for (int c = 8 * t; c < D; c += 8 * TPR) {
-    const int n = D - c;
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0}, q[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (real) load_run8_of(a.w, a.w_bf16, tok * D + c, n, v);
-    if (has_pos) load_run8_of(a.pw, a.pw_bf16, p * D + c, n, q);
+  for (int c = E * t; c < D; c += 2 * E * TPR) {
+    float v[2][E], q[2][E];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = real ? fmaf(v[j], a.scale, q[j]) : q[j];
-    if (a.out_bf16)
-      store_run8(static_cast<bf16*>(a.out) + i * D + c, n, v);
-    else
-      store_run8(static_cast<float*>(a.out) + i * D + c, n, v);
+    for (int u = 0; u < 2; ++u) {
+      const int n = D - c - u * E * TPR;
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[u][j] = q[u][j] = 0.0f;
+      if (real) load_some<E>(a.w, a.w_bf16, tok * D + D - n, n, v[u]);
+      if (has_pos) load_some<E>(a.pw, a.pw_bf16, p * D + D - n, n, q[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int n = D - c - u * E * TPR;
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[u][j] = real ? fmaf(v[u][j], a.scale, q[u][j]) : q[u][j];
+      store_some<E>(a.out, a.out_bf16, i * D + D - n, n, v[u]);
+    }
   }
 }
 
@@ -110,20 +167,20 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_move(const SortPass a) {
   // places of the block's digits: all smaller digits, then this digit's earlier blocks
   constexpr int kPer = kSortBins / kSortThreads;
   uint32_t total[kPer], before[kPer], mine = 0;
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const int b = tid * kPer + k;
-    total[k] = before[k] = 0;
-    if (b < nb) {
-#pragma unroll 8
-      for (int g = 0; g < (int)gridDim.x; ++g) {
-        const uint32_t c = a.count[(int64_t)g * nb + b];
-        total[k] += c;
-        before[k] += g < (int)blockIdx.x ? c : 0u;
-      }
+  static_assert(kPer == 2, "two bins a thread");
+  total[0] = total[1] = before[0] = before[1] = 0;
+  if (2 * tid < nb) {
+#pragma unroll 16
+    for (int g = 0; g < (int)gridDim.x; ++g) {
+      const uint2 c = *reinterpret_cast<const uint2*>(a.count + (int64_t)g * nb + 2 * tid);
+      const bool earlier = g < (int)blockIdx.x;
+      total[0] += c.x;
+      total[1] += c.y;
+      before[0] += earlier ? c.x : 0u;
+      before[1] += earlier ? c.y : 0u;
     }
-    mine += total[k];
   }
+  mine = total[0] + total[1];
   uint32_t incl = mine;
 #pragma unroll
   for (int d = 1; d < kWave; d <<= 1) {
@@ -181,10 +238,86 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_move(const SortPass a) {
   }
 }
 
+// All passes of up to kSmallSort pairs in one workgroup of 16 waves, the pairs in LDS.
+constexpr int kSmallSort = 4096;
+__global__ __launch_bounds__(1024) void k_sort_small(const int64_t* tokens, uint32_t* key_out, uint32_t* val_out, int n,
+                                                     int64_t V, int passes, int bits) {
+  constexpr int W = 16;
+  __shared__ uint32_t key[2][kSmallSort], val[2][kSmallSort], seen[W][kSortBins], wsum[8];
+  const int tid = threadIdx.x, w = tid / kWave, lane = tid & (kWave - 1);
+  const int per = (n + 1023) / 1024, first = w * kWave * per;   // a wave owns `per` * 64 pairs in a row
+  for (int i = tid; i < n; i += 1024) {
+    const int64_t t = tokens[i];
+    key[0][i] = (uint32_t)(t >= 0 && t < V ? t : V);
+    val[0][i] = (uint32_t)i;
+  }
+  int from = 0, shift = 0;
+  for (int q = 0; q < passes; ++q, from ^= 1) {
+    const int b = (bits - shift + passes - q - 1) / (passes - q), nb = 1 << b;
+    for (int i = tid; i < W * kSortBins; i += 1024) (&seen[0][0])[i] = 0;
+    __syncthreads();
+    for (int r = 0; r < per; ++r) {
+      const int i = first + r * kWave + lane;
+      if (i < n) atomicAdd(&seen[w][(key[from][i] >> shift) & (nb - 1)], 1u);
+    }
+    __syncthreads();
+    // starts: all smaller digits, then the earlier waves
+    uint32_t total = 0, incl = 0;
+    if (tid < kSortBins) {
+#pragma unroll
+      for (int k = 0; k < W; ++k) total += seen[k][tid];
+      incl = total;
+#pragma unroll
+      for (int d = 1; d < kWave; d <<= 1) {
+        const uint32_t o = __shfl_up(incl, d, kWave);
+        if (lane >= d) incl += o;
+      }
+      if (lane == kWave - 1) wsum[w] = incl;
+    }
+    __syncthreads();
+    if (tid < kSortBins) {
+      uint32_t at = incl - total;
+      for (int k = 0; k < w; ++k) at += wsum[k];
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        const uint32_t c = seen[k][tid];
+        seen[k][tid] = at;
+        at += c;
+      }
+    }
+    __syncthreads();
+    for (int r = 0; r < per; ++r) {
+      const int i = first + r * kWave + lane;
+      const bool ok = i < n;
+      const uint32_t k = ok ? key[from][i] : 0u, dig = (k >> shift) & (nb - 1);
+      uint64_t same = __ballot(ok);
+      for (int x = 0; x < b; ++x) {
+        const uint64_t m = __ballot((dig >> x) & 1u);
+        same &= (dig >> x) & 1u ? m : ~m;
+      }
+      if (ok) {
+        const uint32_t to = seen[w][dig] + (uint32_t)__popcll(same & ((1ull << lane) - 1ull));
+        key[from ^ 1][to] = k;
+        val[from ^ 1][to] = val[from][i];
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // (as in k_sort_move)
+      if (ok && (same >> lane) == 1ull) seen[w][dig] += (uint32_t)__popcll(same);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    __syncthreads();
+    shift += b;
+  }
+  for (int i = tid; i < n; i += 1024) {
+    key_out[i] = key[from][i];
+    val_out[i] = val[from][i];
+  }
+}
+
 // ---------------------------------------------------------------------------
 // sums over the runs of the sorted list
 // ---------------------------------------------------------------------------
-constexpr int kAhead = 4;   // rows asked for at a time
+constexpr int kRunRows = 32;   // pairs of the sorted list in LDS
+constexpr int kAhead = 8;      // rows asked for at a time
 
 struct EmbedGrad {
   const uint32_t *key, *val;   // the sorted list; null: positions of B sequences of T
@@ -198,26 +331,24 @@ struct EmbedGrad {
   bool dy_bf16, w_bf16;
   // (fewer than 2^31 pairs: 32-bit divisions)
   __device__ __forceinline__ uint32_t key_at(int64_t s) const { return key != nullptr ? key[s] : (uint32_t)s / B; }
-  __device__ __forceinline__ int64_t row_at(int64_t s) const {
-    return key != nullptr ? (int64_t)val[s] : (int64_t)((uint32_t)s % B) * T + (uint32_t)s / B;
+  __device__ __forceinline__ uint32_t row_at(int64_t s) const {
+    return key != nullptr ? val[s] : (uint32_t)s % B * (uint32_t)T + (uint32_t)s / B;
   }
 };
 
-__device__ __forceinline__ void embed_store(const EmbedGrad& a, int64_t at, int n, const float (&v)[8]) {
-  float o[8];
+template <int E>
+__device__ __forceinline__ void embed_store(const EmbedGrad& a, int64_t at, int n, const float (&v)[E]) {
+  float o[E];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) o[j] = v[j] * a.scale;
-  if (a.w_bf16)
-    store_run8(static_cast<bf16*>(a.dw) + at, n, o);
-  else
-    store_run8(static_cast<float*>(a.dw) + at, n, o);
+  for (int j = 0; j < E; ++j) o[j] = v[j] * a.scale;
+  store_some<E>(a.dw, a.w_bf16, at, n, o);
 }
 
-// Clear the rows r0 .. r0 + 63 that have no token.
-template <int NTH>
-__device__ __forceinline__ void embed_clear(const EmbedGrad& a, int64_t r0) {
-  const int tid = threadIdx.x, D = a.D;
-  const int64_t v = r0 + (tid & 63);
+// Clear the rows r0 .. r0 + 63 that have no token, columns c ..
+template <int E>
+__device__ __forceinline__ void embed_clear(const EmbedGrad& a, int64_t r0, int c) {
+  const int n = a.D - c;
+  const int64_t v = r0 + (threadIdx.x & 63);
   bool empty = v < a.V;
   if (empty) {   // the first pair whose key is at least v
     int64_t lo = 0, hi = a.n;
@@ -231,70 +362,72 @@ __device__ __forceinline__ void embed_clear(const EmbedGrad& a, int64_t r0) {
     empty = lo >= a.n || a.key_at(lo) != (uint32_t)v;
   }
   uint64_t rows = __ballot(empty);   // (every wave of the workgroup: the same)
-  const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  float zero[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) zero[j] = 0.0f;
   while (rows != 0) {
-    const int64_t at = (r0 + __builtin_ctzll(rows)) * D;
+    const int64_t at = (r0 + __builtin_ctzll(rows)) * a.D + c;
     rows &= rows - 1;
-    for (int c = 8 * tid; c < D; c += 8 * NTH) {
-      if (a.w_bf16)
-        store_run8(static_cast<bf16*>(a.dw) + at + c, D - c, zero);
-      else
-        store_run8(static_cast<float*>(a.dw) + at + c, D - c, zero);
-    }
+    store_some<E>(a.dw, a.w_bf16, at, n, zero);
   }
 }
 
 // Workgroups below a.pieces add the rows of a piece; the others clear the rows
-// without a token, 64 rows of the table at a time.  A thread owns runs of 8 columns.
-template <int NTH>
-__global__ __launch_bounds__(NTH) void k_embed_runs(const EmbedGrad a) {
+// without a token, 64 rows of the table at a time.  A thread owns E columns.
+template <int E>
+__global__ __launch_bounds__(256) void k_embed_runs(const EmbedGrad a) {
+  __shared__ uint32_t keys[kRunRows + 1], rows[kRunRows];
   const int tid = threadIdx.x, D = a.D;
+  const int c = ((int)blockIdx.y * (int)blockDim.x + tid) * E, n = D - c;
   if ((int)blockIdx.x >= a.pieces) {
     for (int64_t r0 = ((int64_t)blockIdx.x - a.pieces) * 64; r0 < a.V; r0 += ((int64_t)gridDim.x - a.pieces) * 64)
-      embed_clear<NTH>(a, r0);
+      embed_clear<E>(a, r0, c);
     return;
   }
   const int64_t s0 = (int64_t)blockIdx.x * a.len, s1 = s0 + a.len < a.n ? s0 + a.len : a.n;
-  const uint32_t none = (uint32_t)a.V;
-  const uint32_t k_prev = s0 > 0 ? a.key_at(s0 - 1) : none + 1, k_next = s1 < a.n ? a.key_at(s1) : none + 1;
+  const uint32_t none = (uint32_t)a.V, end = none + 1;
+  const uint32_t k_prev = s0 > 0 ? a.key_at(s0 - 1) : end, k_next = s1 < a.n ? a.key_at(s1) : end;
   float* part = a.part + (int64_t)blockIdx.x * 2 * D;
-  for (int c = 8 * tid; c < D; c += 8 * NTH) {
-    const int n = D - c;
-    float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    uint32_t k = a.key_at(s0);
-    bool head = k == k_prev;   // the run began in an earlier piece
-    for (int64_t s = s0; s < s1 && k != none; s += kAhead) {
-      float v[kAhead][8];
-      uint32_t kn[kAhead];     // the key behind each row (none + 1 behind the piece)
+  float acc[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) acc[j] = 0.0f;
+  bool head = a.key_at(s0) == k_prev;   // the run began in an earlier piece
+  for (int64_t s = s0; s < s1; s += kRunRows) {
+    const int m = s1 - s < kRunRows ? (int)(s1 - s) : kRunRows;
+    __syncthreads();
+    if (tid <= m) keys[tid] = tid < m || s + m < s1 ? a.key_at(s + tid) : end;   // (the key behind each row; `end` behind the piece)
+    if (tid < m) rows[tid] = a.row_at(s + tid);
+    __syncthreads();
+    if (n <= 0) continue;
+    for (int u0 = 0; u0 < m; u0 += kAhead) {
+      float v[kAhead][E];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (u0 + u < m) load_some<E>(a.dy, a.dy_bf16, (int64_t)rows[u0 + u] * D + c, n, v[u]);
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        if (s + u < s1) load_run8_of(a.dy, a.dy_bf16, a.row_at(s + u) * D + c, n, v[u]);
-        kn[u] = s + u + 1 < s1 ? a.key_at(s + u + 1) : none + 1;
-      }
+        if (u0 + u >= m) continue;
+        const uint32_t k = keys[u0 + u], kn = keys[u0 + u + 1];
+        if (k == none) continue;
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        if (s + u >= s1 || k == none) continue;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] += v[u][j];
-        if (kn[u] == k) continue;
+        for (int j = 0; j < E; ++j) acc[j] += v[u][j];
+        if (kn == k) continue;
         if (head)
-          store_run8(part + c, n, acc);
-        else if (s + u + 1 == s1 && k == k_next)   // the run goes on in the next piece
-          store_run8(part + D + c, n, acc);
+          store_some<E>(part, false, c, n, acc);
+        else if (kn == end && k == k_next)   // the run goes on in the next piece
+          store_some<E>(part, false, D + c, n, acc);
         else
-          embed_store(a, (int64_t)k * D + c, n, acc);
+          embed_store<E>(a, (int64_t)k * D + c, n, acc);
         head = false;
-        k = kn[u];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
+        for (int j = 0; j < E; ++j) acc[j] = 0.0f;
       }
     }
   }
 }
 
 // The cut runs: one workgroup for each piece in which one begins.
-template <int NTH>
-__global__ __launch_bounds__(NTH) void k_embed_join(const EmbedGrad a) {
+__global__ __launch_bounds__(256) void k_embed_join(const EmbedGrad a) {
   const int tid = threadIdx.x, lane = tid & (kWave - 1), D = a.D;
   const int64_t p = blockIdx.x;
   const int64_t s0 = p * a.len, s1 = s0 + a.len;      // (the last piece begins none that is cut)
@@ -310,18 +443,23 @@ __global__ __launch_bounds__(NTH) void k_embed_join(const EmbedGrad a) {
     more += m == ~0ull ? 64 : __builtin_ctzll(~m);
     if (m != ~0ull) break;
   }
-  for (int c = 8 * tid; c < D; c += 8 * NTH) {
+  for (int c = 4 * tid; c < D; c += 4 * (int)blockDim.x) {
     const int n = D - c;
-    float acc[8];
-    load_run8(a.part + (p * 2 + 1) * D + c, n, acc);
-#pragma unroll 4
-    for (int64_t q = 1; q <= more; ++q) {
-      float v[8];
-      load_run8(a.part + (p + q) * 2 * D + c, n, v);
+    float acc[4];
+    load_some<4>(a.part, false, (p * 2 + 1) * D + c, n, acc);
+    for (int64_t q0 = 1; q0 <= more; q0 += 16) {
+      float v[16][4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] += v[j];
+      for (int u = 0; u < 16; ++u)
+        if (q0 + u <= more) load_some<4>(a.part, false, (p + q0 + u) * 2 * D + c, n, v[u]);
+#pragma unroll
+      for (int u = 0; u < 16; ++u)
+        if (q0 + u <= more) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[j] += v[u][j];
+        }
     }
-    embed_store(a, (int64_t)k * D + c, n, acc);
+    embed_store<4>(a, (int64_t)k * D + c, n, acc);
   }
 }
 
@@ -336,10 +474,10 @@ static int sort_blocks(int64_t n) {
   const int64_t per = (int64_t)kSortThreads * sort_per(n);
   return (int)((n + per - 1) / per);
 }
-// Pairs a piece: 32, more where the pieces would be more than 4096
+// Pairs a piece: 8, more where the pieces would be more than 2048
 static int embed_piece(int64_t n) {
-  int64_t len = 32;
-  while (n / len > 4096) len *= 2;
+  int64_t len = 8;
+  while (n / len > 2048) len *= 2;
   return (int)len;
 }
 struct EmbedPlan {
@@ -373,22 +511,29 @@ extern "C" int nsa_embed_fwd(const int64_t* tokens, const int64_t* pos, const vo
   if (n == 0) return NSA_OK;
   NSA_CHECK(tokens != nullptr && w != nullptr && out != nullptr, NSA_ERR_ARG);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const int runs = (D + 7) / 8;
   // 2^24 rows a launch: a grid holds less than 2^32 threads
   for (int64_t r0 = 0; r0 < n; r0 += 1 << 24) {
     const int64_t end = n - r0 < (1 << 24) ? n : r0 + (1 << 24);
     const EmbedArgs a{tokens, pos, w, pw, out, r0, end, T, V, P, D, scale, w_dtype == NSA_BF16, pw_dtype == NSA_BF16,
                       out_dtype == NSA_BF16};
-    auto grid = [&](int tpr) { return (unsigned)((end - r0 + 256 / tpr - 1) / (256 / tpr)); };
-    // the fewest threads that hold a row with one run each, 64 at most
-    if (runs <= 4)
-      k_embed_fwd<4><<<grid(4), 256, 0, s>>>(a);
-    else if (runs <= 16)
-      k_embed_fwd<16><<<grid(16), 256, 0, s>>>(a);
-    else if (runs <= 32)
-      k_embed_fwd<32><<<grid(32), 256, 0, s>>>(a);
+    auto go = [&](auto e, auto tpr) {
+      constexpr int E = decltype(e)::value, TPR = decltype(tpr)::value;
+      k_embed_fwd<E, TPR><<<(unsigned)((end - r0 + 256 / TPR - 1) / (256 / TPR)), 256, 0, s>>>(a);
+    };
+    // the fewest threads that hold a row with two runs each, 64 at most
+    auto pick = [&](auto e) {
+      const int runs = (D + decltype(e)::value - 1) / decltype(e)::value;
+      if (runs <= 8)
+        go(e, std::integral_constant<int, 4>{});
+      else if (runs <= 32)
+        go(e, std::integral_constant<int, 16>{});
+      else
+        go(e, std::integral_constant<int, 64>{});
+    };
+    if (w_dtype == NSA_BF16)
+      pick(std::integral_constant<int, 8>{});
     else
-      k_embed_fwd<64><<<grid(64), 256, 0, s>>>(a);
+      pick(std::integral_constant<int, 4>{});
     const int rc = nsa_launch_status();
     if (rc != NSA_OK) return rc;
   }
@@ -420,8 +565,9 @@ extern "C" int nsa_embed_bwd(const int64_t* index, const void* dy, void* dw, voi
     int bits = 1;   // of the keys 0 .. V
     while ((V >> bits) != 0) ++bits;
     const int passes = (bits + kSortBits - 1) / kSortBits;
+    if (n <= kSmallSort) k_sort_small<<<1, 1024, 0, s>>>(index, ka, va, (int)n, V, passes, bits);
     const unsigned blocks = (unsigned)sort_blocks(n);
-    for (int q = 0, shift = 0; q < passes; ++q) {
+    for (int q = 0, shift = 0; n > kSmallSort && q < passes; ++q) {
       const int b = (bits - shift + passes - q - 1) / (passes - q);
       const SortPass a{q == 0 ? index : nullptr, ka, va, kb, vb, count, n, V, sort_per(n), shift, b};
       k_sort_count<<<blocks, kSortThreads, 0, s>>>(a);
@@ -437,17 +583,13 @@ extern "C" int nsa_embed_bwd(const int64_t* index, const void* dy, void* dw, voi
                     D, p.len, p.pieces, scale, dy_dtype == NSA_BF16, w_dtype == NSA_BF16};
   const int64_t clear = (V + 63) / 64;
   const unsigned grid = (unsigned)(p.pieces + (clear < (1 << 16) ? clear : 1 << 16));
-  auto go = [&](auto nth) {
-    constexpr int N = decltype(nth)::value;
-    k_embed_runs<N><<<grid, N, 0, s>>>(g);
-    if (p.pieces > 1) k_embed_join<N><<<(unsigned)(p.pieces - 1), N, 0, s>>>(g);
-  };
-  // threads that hold a row with one run each, 256 at most
-  if (D <= 512)
-    go(std::integral_constant<int, 64>{});
-  else if (D <= 1024)
-    go(std::integral_constant<int, 128>{});
+  const int E = g.dy_bf16 ? 8 : 4, runs = (D + E - 1) / E;
+  const int nth = runs >= 256 ? 256 : (runs + 63) / 64 * 64;
+  const dim3 all(grid, (unsigned)((runs + nth - 1) / nth));
+  if (g.dy_bf16)
+    k_embed_runs<8><<<all, nth, 0, s>>>(g);
   else
-    go(std::integral_constant<int, 256>{});
+    k_embed_runs<4><<<all, nth, 0, s>>>(g);
+  if (p.pieces > 1) k_embed_join<<<(unsigned)(p.pieces - 1), nth, 0, s>>>(g);
   return nsa_launch_status();
 }
