@@ -60,7 +60,8 @@ __device__ __forceinline__ void load_some(const void* p, bool is_bf16, int64_t a
       f[j] = j >= n ? 0.0f : is_bf16 ? (float)static_cast<const bf16*>(p)[at + j] : static_cast<const float*>(p)[at + j];
   }
 }
-template <int E>
+// (PAST: the caches keep nothing of it)
+template <int E, bool PAST = false>
 __device__ __forceinline__ void store_some(void* p, bool is_bf16, int64_t at, int n, const float (&f)[E]) {
   typedef bf16 bf16xE __attribute__((ext_vector_type(E), aligned(2)));
   typedef float f32xE __attribute__((ext_vector_type(E), aligned(4)));
@@ -69,12 +70,18 @@ __device__ __forceinline__ void store_some(void* p, bool is_bf16, int64_t at, in
       bf16xE v;
 #pragma unroll
       for (int j = 0; j < E; ++j) v[j] = (bf16)f[j];
-      *reinterpret_cast<bf16xE*>(static_cast<bf16*>(p) + at) = v;
+      if (PAST)
+        __builtin_nontemporal_store(v, reinterpret_cast<bf16xE*>(static_cast<bf16*>(p) + at));
+      else
+        *reinterpret_cast<bf16xE*>(static_cast<bf16*>(p) + at) = v;
     } else {
       f32xE v;
 #pragma unroll
       for (int j = 0; j < E; ++j) v[j] = f[j];
-      *reinterpret_cast<f32xE*>(static_cast<float*>(p) + at) = v;
+      if (PAST)
+        __builtin_nontemporal_store(v, reinterpret_cast<f32xE*>(static_cast<float*>(p) + at));
+      else
+        *reinterpret_cast<f32xE*>(static_cast<float*>(p) + at) = v;
     }
   } else {
 #pragma unroll
@@ -88,8 +95,8 @@ __device__ __forceinline__ void store_some(void* p, bool is_bf16, int64_t at, in
   }
 }
 
-// TPR threads a row, 256 / TPR rows a workgroup; a thread has two runs of E in flight.
-template <int E, int TPR>
+// TPR threads a row, 256 / TPR rows a workgroup; a thread has 16 elements of each table in flight.
+template <int E, int TPR, bool PAST>
 __global__ __launch_bounds__(256) void k_embed_fwd(const EmbedArgs a) {
   const int t = threadIdx.x & (TPR - 1);
   const int64_t i = a.first + (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
@@ -100,10 +107,11 @@ __global__ __launch_bounds__(256) void k_embed_fwd(const EmbedArgs a) {
   const int64_t p = a.pw == nullptr ? 0 : a.pos != nullptr ? a.pos[i] : (int64_t)((uint32_t)i % (uint32_t)a.T);
   const bool has_pos = a.pw != nullptr && p >= 0 && p < a.P;
   const int D = a.D;
-  for (int c = E * t; c < D; c += 2 * E * TPR) {
-    float v[2][E], q[2][E];
+  constexpr int U = E == 4 ? 4 : 2;
+  for (int c = E * t; c < D; c += U * E * TPR) {
+    float v[U][E], q[U][E];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int n = D - c - u * E * TPR;
 #pragma unroll
       for (int j = 0; j < E; ++j) v[u][j] = q[u][j] = 0.0f;
@@ -111,11 +119,11 @@ __global__ __launch_bounds__(256) void k_embed_fwd(const EmbedArgs a) {
       if (has_pos) load_some<E>(a.pw, a.pw_bf16, p * D + D - n, n, q[u]);
     }
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < U; ++u) {
       const int n = D - c - u * E * TPR;
 #pragma unroll
       for (int j = 0; j < E; ++j) v[u][j] = real ? fmaf(v[u][j], a.scale, q[u][j]) : q[u][j];
-      store_some<E>(a.out, a.out_bf16, i * D + D - n, n, v[u]);
+      store_some<E, PAST>(a.out, a.out_bf16, i * D + D - n, n, v[u]);
     }
   }
 }
@@ -127,6 +135,7 @@ constexpr int kSortThreads = 256;
 constexpr int kSortWaves = kSortThreads / kWave;
 constexpr int kSortBits = 9;
 constexpr int kSortBins = 1 << kSortBits;
+constexpr int kSortAhead = 4;   // pairs a thread asks for at a time; `per` is a multiple of it
 
 struct SortPass {
   const int64_t* tokens;              // first pass: keys from here, i in order; else null
@@ -150,9 +159,18 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_count(const SortPass a) {
   for (int b = threadIdx.x; b < nb; b += kSortThreads) bins[b] = 0;
   __syncthreads();
   const int64_t first = (int64_t)blockIdx.x * kSortThreads * a.per;
-  for (int r = 0; r < a.per; ++r) {
-    const int64_t i = first + (int64_t)r * kSortThreads + threadIdx.x;
-    if (i < a.n) atomicAdd(&bins[(sort_key(a, i) >> a.shift) & (nb - 1)], 1u);
+  for (int r0 = 0; r0 < a.per; r0 += kSortAhead) {
+    uint32_t key[kSortAhead];
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u) {
+      const int64_t i = first + (int64_t)(r0 + u) * kSortThreads + threadIdx.x;
+      key[u] = i < a.n ? sort_key(a, i) : 0u;
+    }
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u) {
+      const int64_t i = first + (int64_t)(r0 + u) * kSortThreads + threadIdx.x;
+      if (i < a.n) atomicAdd(&bins[(key[u] >> a.shift) & (nb - 1)], 1u);
+    }
   }
   __syncthreads();
   for (int b = threadIdx.x; b < nb; b += kSortThreads) a.count[(int64_t)blockIdx.x * nb + b] = bins[b];
@@ -164,6 +182,18 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_move(const SortPass a) {
   __shared__ uint32_t base[kSortBins];
   __shared__ uint32_t wsum[kSortWaves];
   const int nb = 1 << a.bits, tid = threadIdx.x, w = tid / kWave, lane = tid & (kWave - 1);
+  const int64_t first = (int64_t)blockIdx.x * kSortThreads * a.per + (int64_t)w * kWave * a.per;
+  auto at_of = [&](int r) { return first + (int64_t)r * kWave + lane; };
+  uint32_t key[kSortAhead], val[kSortAhead];
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u) {
+      const int64_t i = at_of(r0 + u);
+      key[u] = i < a.n ? sort_key(a, i) : 0u;
+      val[u] = a.tokens != nullptr || i >= a.n ? (uint32_t)i : a.val_in[i];
+    }
+  };
+  load(0);
   // places of the block's digits: all smaller digits, then this digit's earlier blocks
   constexpr int kPer = kSortBins / kSortThreads;
   uint32_t total[kPer], before[kPer], mine = 0;
@@ -197,11 +227,12 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_move(const SortPass a) {
     base[tid * kPer + k] = at + before[k];
     at += total[k];
   }
-  const int64_t first = (int64_t)blockIdx.x * kSortThreads * a.per + (int64_t)w * kWave * a.per;
   // 1st walk: how many pairs of each digit every wave has
-  for (int r = 0; r < a.per; ++r) {
-    const int64_t i = first + (int64_t)r * kWave + lane;
-    if (i < a.n) atomicAdd(&seen[w][(sort_key(a, i) >> a.shift) & (nb - 1)], 1u);
+  for (int r0 = 0; r0 < a.per; r0 += kSortAhead) {
+    if (r0 > 0) load(r0);
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u)
+      if (at_of(r0 + u) < a.n) atomicAdd(&seen[w][(key[u] >> a.shift) & (nb - 1)], 1u);
   }
   __syncthreads();
   // the waves' starts of each digit
@@ -216,25 +247,27 @@ __global__ __launch_bounds__(kSortThreads) void k_sort_move(const SortPass a) {
   }
   __syncthreads();
   // 2nd walk: a pair's place is its wave's next of the digit, plus its rank among the 64
-  for (int r = 0; r < a.per; ++r) {
-    const int64_t i = first + (int64_t)r * kWave + lane;
-    const bool ok = i < a.n;
-    const uint32_t key = ok ? sort_key(a, i) : 0u;
-    const uint32_t dig = (key >> a.shift) & (nb - 1);
-    uint64_t same = __ballot(ok);
-    for (int b = 0; b < a.bits; ++b) {
-      const uint64_t m = __ballot((dig >> b) & 1u);
-      same &= (dig >> b) & 1u ? m : ~m;
+  for (int r0 = 0; r0 < a.per; r0 += kSortAhead) {
+    if (a.per > kSortAhead) load(r0);
+#pragma unroll
+    for (int u = 0; u < kSortAhead; ++u) {
+      const bool ok = at_of(r0 + u) < a.n;
+      const uint32_t dig = (key[u] >> a.shift) & (nb - 1);
+      uint64_t same = __ballot(ok);
+      for (int b = 0; b < a.bits; ++b) {
+        const uint64_t m = __ballot((dig >> b) & 1u);
+        same &= (dig >> b) & 1u ? m : ~m;
+      }
+      if (ok) {
+        const uint32_t to = seen[w][dig] + (uint32_t)__popcll(same & ((1ull << lane) - 1ull));
+        a.key_out[to] = key[u];
+        a.val_out[to] = val[u];
+      }
+      // (LDS accesses of a wave keep their order: all have read before one adds)
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (ok && (same >> lane) == 1ull) seen[w][dig] += (uint32_t)__popcll(same);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    if (ok) {
-      const uint32_t rank = (uint32_t)__popcll(same & ((1ull << lane) - 1ull));
-      const uint32_t to = seen[w][dig] + rank;
-      a.key_out[to] = key;
-      a.val_out[to] = a.tokens != nullptr ? (uint32_t)i : a.val_in[i];
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // (LDS accesses of a wave keep their order: all have read before one adds)
-    if (ok && (same >> lane) == 1ull) seen[w][dig] += (uint32_t)__popcll(same);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
 
@@ -426,14 +459,19 @@ __global__ __launch_bounds__(256) void k_embed_runs(const EmbedGrad a) {
   }
 }
 
-// The cut runs: one workgroup for each piece in which one begins.
-__global__ __launch_bounds__(256) void k_embed_join(const EmbedGrad a) {
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), D = a.D;
+// The cut runs: one workgroup for each piece in which one begins.  Its two halves add
+// every other group of kJoin parts, then the second half's sum goes to the first's.
+constexpr int kJoin = 16;
+__global__ __launch_bounds__(512) void k_embed_join(const EmbedGrad a) {
+  __shared__ float half[4][256];
+  const int lane = threadIdx.x & (kWave - 1), D = a.D, nth = (int)blockDim.x / 2;
+  const int h = threadIdx.x >= nth, tid = threadIdx.x - h * nth;
   const int64_t p = blockIdx.x;
   const int64_t s0 = p * a.len, s1 = s0 + a.len;      // (the last piece begins none that is cut)
-  const uint32_t k = a.key_at(s1 - 1);
-  if (k == (uint32_t)a.V || a.key_at(s1) != k) return;               // nothing goes on behind this piece
-  if (a.key_at(s0) == k && s0 > 0 && a.key_at(s0 - 1) == k) return;  // the run began before it
+  const uint32_t k = a.key_at(s1 - 1), k_next = a.key_at(s1), k0 = a.key_at(s0);
+  const uint32_t k_prev = s0 > 0 ? a.key_at(s0 - 1) : (uint32_t)a.V + 1;
+  if (k == (uint32_t)a.V || k_next != k) return;   // nothing goes on behind this piece
+  if (k0 == k && k_prev == k) return;              // the run began before it
   // pieces that the run goes on in: the next one, and every one that starts with it
   int64_t more = 1;
   for (;;) {
@@ -443,23 +481,35 @@ __global__ __launch_bounds__(256) void k_embed_join(const EmbedGrad a) {
     more += m == ~0ull ? 64 : __builtin_ctzll(~m);
     if (m != ~0ull) break;
   }
-  for (int c = 4 * tid; c < D; c += 4 * (int)blockDim.x) {
-    const int n = D - c;
-    float acc[4];
-    load_some<4>(a.part, false, (p * 2 + 1) * D + c, n, acc);
-    for (int64_t q0 = 1; q0 <= more; q0 += 16) {
-      float v[16][4];
+  for (int c0 = 0; c0 < D; c0 += 4 * nth) {
+    const int c = c0 + 4 * tid, n = D - c;
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (h == 0) load_some<4>(a.part, false, (p * 2 + 1) * D + c, n, acc);
+    for (int64_t q0 = 1 + h * kJoin; q0 <= more; q0 += 2 * kJoin) {
+      float v[kJoin][4];
 #pragma unroll
-      for (int u = 0; u < 16; ++u)
+      for (int u = 0; u < kJoin; ++u)
         if (q0 + u <= more) load_some<4>(a.part, false, (p + q0 + u) * 2 * D + c, n, v[u]);
 #pragma unroll
-      for (int u = 0; u < 16; ++u)
+      for (int u = 0; u < kJoin; ++u)
         if (q0 + u <= more) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[j] += v[u][j];
         }
     }
-    embed_store<4>(a, (int64_t)k * D + c, n, acc);
+    if (more > kJoin) {   // (else the second half has nothing)
+      __syncthreads();
+      if (h == 1) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) half[j][tid] = acc[j];
+      }
+      __syncthreads();
+      if (h == 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] += half[j][tid];
+      }
+    }
+    if (h == 0) embed_store<4>(a, (int64_t)k * D + c, n, acc);
   }
 }
 
@@ -468,7 +518,7 @@ static bool embed_type(int dtype) { return dtype == NSA_F32 || dtype == NSA_BF16
 // Pairs a thread of the sort (4, more past 256 blocks), and its blocks
 static int sort_per(int64_t n) {
   const int64_t per = (n + kSortThreads * 256 - 1) / (kSortThreads * 256);
-  return per < 4 ? 4 : (int)per;
+  return (int)((per + kSortAhead - 1) / kSortAhead * kSortAhead);
 }
 static int sort_blocks(int64_t n) {
   const int64_t per = (int64_t)kSortThreads * sort_per(n);
@@ -514,18 +564,24 @@ extern "C" int nsa_embed_fwd(const int64_t* tokens, const int64_t* pos, const vo
   // 2^24 rows a launch: a grid holds less than 2^32 threads
   for (int64_t r0 = 0; r0 < n; r0 += 1 << 24) {
     const int64_t end = n - r0 < (1 << 24) ? n : r0 + (1 << 24);
+    // an output that the caches cannot hold leaves them to the tables (8 x 4096 rows of 768
+    // in float32: 37 us, 42 through the caches)
+    const bool past = (double)n * D * (out_dtype == NSA_BF16 ? 2 : 4) > (double)(64 << 20);
     const EmbedArgs a{tokens, pos, w, pw, out, r0, end, T, V, P, D, scale, w_dtype == NSA_BF16, pw_dtype == NSA_BF16,
                       out_dtype == NSA_BF16};
     auto go = [&](auto e, auto tpr) {
       constexpr int E = decltype(e)::value, TPR = decltype(tpr)::value;
-      k_embed_fwd<E, TPR><<<(unsigned)((end - r0 + 256 / TPR - 1) / (256 / TPR)), 256, 0, s>>>(a);
+      const unsigned grid = (unsigned)((end - r0 + 256 / TPR - 1) / (256 / TPR));
+      if (past)
+        k_embed_fwd<E, TPR, true><<<grid, 256, 0, s>>>(a);
+      else
+        k_embed_fwd<E, TPR, false><<<grid, 256, 0, s>>>(a);
     };
-    // the fewest threads that hold a row with two runs each, 64 at most
+    // the fewest threads that hold a row with 16 elements each, 64 at most
     auto pick = [&](auto e) {
-      const int runs = (D + decltype(e)::value - 1) / decltype(e)::value;
-      if (runs <= 8)
+      if (D <= 64)
         go(e, std::integral_constant<int, 4>{});
-      else if (runs <= 32)
+      else if (D <= 256)
         go(e, std::integral_constant<int, 16>{});
       else
         go(e, std::integral_constant<int, 64>{});
@@ -590,6 +646,7 @@ extern "C" int nsa_embed_bwd(const int64_t* index, const void* dy, void* dw, voi
     k_embed_runs<8><<<all, nth, 0, s>>>(g);
   else
     k_embed_runs<4><<<all, nth, 0, s>>>(g);
-  if (p.pieces > 1) k_embed_join<<<(unsigned)(p.pieces - 1), nth, 0, s>>>(g);
+  const int quads = (D + 3) / 4, jth = quads >= 256 ? 256 : (quads + 63) / 64 * 64;
+  if (p.pieces > 1) k_embed_join<<<(unsigned)(p.pieces - 1), 2 * jth, 0, s>>>(g);
   return nsa_launch_status();
 }

@@ -128,6 +128,32 @@ struct LnBwdArgs {
   bool w_bf16, dx_bf16;
 };
 
+// A run of 8 elements as it lies in memory; elements past the row's end are 0.
+template <typename T> struct RawRun;
+template <> struct RawRun<bf16> {
+  bf16x8u v;
+  __device__ __forceinline__ void load(const bf16* p, int n) {
+    if (n >= 8) {
+      v = *reinterpret_cast<const bf16x8u*>(p);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : (bf16)0.0f;
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (float)v[j];
+  }
+};
+template <> struct RawRun<float> {
+  float v[8];
+  __device__ __forceinline__ void load(const float* p, int n) { load_run8(p, n, v); }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = v[j];
+  }
+};
+
 // Sums of two values over a row's N threads; `buf` as in row_sum, twice as long.
 template <int N>
 __device__ __forceinline__ void row_sum2(float& u, float& v, float* buf) {
@@ -167,9 +193,33 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_ln_bwd(const LnBwdArg
     for (int j = 0; j < 8; ++j) dw[i][j] = db[i][j] = 0.0f;
   }
   int turn = 0;
-  for (int64_t row = (int64_t)blockIdx.x * RPG + sub; row < a.rows; row += (int64_t)gridDim.x * RPG) {
+  const int64_t step = (int64_t)gridDim.x * RPG;
+  // a row of several waves is asked for before the sums of the row ahead of it, whose barrier
+  // would leave the memory idle; wider rows (two runs a thread) have no registers for that
+  constexpr bool kNext = kHold && TPR > kWave;
+  struct Row {
+    RawRun<RT> h, d;
+    RawRun<YT> g;
+    float mu, rstd;
+  };
+  Row ahead[kNext ? NV : 1];
+  auto ask = [&](int64_t row) {
     const int64_t base = row * D;
-    const float mu = a.stat[2 * row], rstd = a.stat[2 * row + 1];
+#pragma unroll
+    for (int i = 0; i < (kNext ? NV : 0); ++i) {
+      const int c = 8 * (i * TPR + t), n = D - c;
+      ahead[i].h.load(static_cast<const RT*>(a.h) + base + c, n);
+      ahead[i].g.load(static_cast<const YT*>(a.dy) + base + c, n);
+      if (a.dh != nullptr) ahead[i].d.load(static_cast<const RT*>(a.dh) + base + c, n);
+    }
+    ahead[0].mu = a.stat[2 * row];
+    ahead[0].rstd = a.stat[2 * row + 1];
+  };
+  int64_t row = (int64_t)blockIdx.x * RPG + sub;
+  if (kNext && row < a.rows) ask(row);
+  for (; row < a.rows; row += step) {
+    const int64_t base = row * D;
+    const float mu = kNext ? ahead[0].mu : a.stat[2 * row], rstd = kNext ? ahead[0].rstd : a.stat[2 * row + 1];
     float n_[NV][8], g[NV][8], d[kHold ? NV : 1][8];
     float s1 = 0.0f, s2 = 0.0f;
     auto load_dh = [&](int i, float(&v)[8]) {
@@ -184,10 +234,22 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_ln_bwd(const LnBwdArg
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = 8 * (i * TPR + t), n = D - c;
-      load_run8(static_cast<const RT*>(a.h) + base + c, n, n_[i]);
-      load_run8(static_cast<const YT*>(a.dy) + base + c, n, g[i]);   // (0 past the row's end)
-      if (kHold) load_dh(i, d[i]);
+      if constexpr (kNext) {
+        ahead[i].h.get(n_[i]);
+        ahead[i].g.get(g[i]);
+        if (a.dh != nullptr) {
+          ahead[i].d.get(d[i]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) d[i][j] = 0.0f;
+        }
+      } else {
+        load_run8(static_cast<const RT*>(a.h) + base + c, n, n_[i]);
+        load_run8(static_cast<const YT*>(a.dy) + base + c, n, g[i]);   // (0 past the row's end)
+        if (kHold) load_dh(i, d[kHold ? i : 0]);
+      }
     }
+    if (kNext && row + step < a.rows) ask(row + step);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float(&wi)[8] = w[kHold ? i : 0];
