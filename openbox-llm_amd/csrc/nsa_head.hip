@@ -32,7 +32,8 @@ namespace nsa {
 constexpr int64_t kHeadRows = 1 << 22;       // most rows of x
 constexpr int kHeadVocab = 1 << 24;
 constexpr int kHeadWide = 1 << 16;           // widest row
-constexpr size_t kHeadPiece = 512u << 20;    // bytes of dz held at a time
+constexpr size_t kHeadPiece = 1u << 30;      // bytes of dz held at a time: 32768 x 32000 x d768 takes 6.3 ms, 6.9 with
+                                             // half of them (the parts of dx and more partial rounds), 6.1 in one piece
 constexpr int64_t kHeadPieceMost = 1 << 20;  // most tokens of a piece: offsets within a stage have 32 bits
 
 // An operand of a product: bf16 planes; ROWS: [rows][ld], contraction along a row;
@@ -452,36 +453,37 @@ __global__ __launch_bounds__(256) void k_head_join(const HeadJoin a) {
   const int lane = threadIdx.x & 63;
   const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (n >= a.N) return;
+  const int64_t t = a.target != nullptr ? a.target[n] : -1;
   float m = kMaskScore, l = 0.0f;
-  bool nan = false;
+#pragma unroll 4
   for (int s = lane; s < a.split; s += kWave) {
     const float2 p = a.part[(int64_t)s * a.N + n];
     const float mx = fmaxf(m, p.x);
     l = l * fast_exp2(m - mx) + p.y * fast_exp2(p.x - mx);
     m = mx;
   }
+  const bool real = t >= 0 && t < a.V;
+  float dot = 0.0f;
+  if (real) {
+#pragma unroll 2
+    for (int c = 8 * lane; c < a.D; c += 8 * kWave) {
+      float u[8], v[8];
+      load_run8_of(a.x, a.x_bf16, n * a.D + c, a.D - c, u);
+      load_run8_of(a.w, a.w_bf16, t * a.D + c, a.D - c, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dot += u[j] * (a.w_round ? (float)(bf16)v[j] : v[j]);
+    }
+    dot = wave_sum(dot);
+  }
   const float mx = wave_max(m);
-  nan = l != l;
+  const bool nan = l != l;   // (a maximum passes NaN over: its sum shows it)
   l = wave_sum(l * fast_exp2(m - mx));
   if (__any(nan)) l = __builtin_nanf("");
   const float lse = (mx + __log2f(l)) * kLn2;
-  if (a.target != nullptr) {
-    const int64_t t = a.target[n];
-    float dot = 0.0f;
-    const bool real = t >= 0 && t < a.V;
-    if (real) {
-      for (int c = 8 * lane; c < a.D; c += 8 * kWave) {
-        float u[8], v[8];
-        load_run8_of(a.x, a.x_bf16, n * a.D + c, a.D - c, u);
-        load_run8_of(a.w, a.w_bf16, t * a.D + c, a.D - c, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) dot += u[j] * (a.w_round ? (float)(bf16)v[j] : v[j]);
-      }
-      dot = wave_sum(dot);
-    }
-    if (lane == 0) a.logp[n] = real ? dot - lse : 0.0f;
+  if (lane == 0) {
+    if (a.target != nullptr) a.logp[n] = real ? dot - lse : 0.0f;
+    a.lse[n] = lse;
   }
-  if (lane == 0) a.lse[n] = lse;
 }
 
 // dz of a piece of the vocabulary, as the gradients' operand
@@ -545,11 +547,13 @@ __global__ __launch_bounds__(256, S::kPerCu) void k_head_dz(const HeadDz a) {
         for (int j = 0; j < S::NT; ++j) {
           const int n = nt * S::TN + wn + 32 * j + (lane & 31);
           if (n >= a.rows) continue;
+          bf16* const at = a.dz + (int64_t)n * a.ld + mt * S::TM + wm + 8 * h;
+          const int v0 = mt * S::TM + wm + 8 * h;
 #pragma unroll
           for (int i = 0; i < S::MT; ++i)
 #pragma unroll
             for (int r0 = 0; r0 < 16; r0 += 8) {
-              const int v = mt * S::TM + wm + 32 * i + acc_elem(h, r0);
+              const int v = v0 + 32 * i + 2 * r0;
               float d[8];
 #pragma unroll
               for (int r = 0; r < 8; ++r) d[r] = fast_exp2(fmaf(acc[i][j][r0 + r], kLog2e, -off[j]));
@@ -558,7 +562,7 @@ __global__ __launch_bounds__(256, S::kPerCu) void k_head_dz(const HeadDz a) {
                 for (int r = 0; r < 8; ++r)
                   if (v + r >= a.vocab || n >= a.N) d[r] = 0.0f;
               }
-              store_planes<PLANES>(a.dz + (int64_t)n * a.ld + v, a.plane, d, neg[j]);
+              store_planes<PLANES>(at + 32 * i + 2 * r0, a.plane, d, neg[j]);
               __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -633,11 +637,13 @@ __global__ __launch_bounds__(256, S::kPerCu) void k_head_grad(const HeadGrad a) 
           part = a.part + ((int64_t)c * rest + t - a.whole) * S::TM * S::TN;
         }
         if (part == nullptr && sp.m * S::TM + S::TM > a.D) part = a.part + ((int64_t)units + sp.n) * S::TM * S::TN;
-        auto each = [&](auto put) {
+        // a lane's runs of a row: 32 i + 2 r0 elements from its first one on
+        auto each = [&](auto to, auto put) {
 #pragma unroll
           for (int j = 0; j < S::NT; ++j) {
             const int c = wn + 32 * j + (lane & 31);
             if (sp.n * (int64_t)S::TN + c >= a.N) continue;
+            const auto at = to(c, wm + 8 * h);
 #pragma unroll
             for (int i = 0; i < S::MT; ++i)
 #pragma unroll
@@ -645,35 +651,32 @@ __global__ __launch_bounds__(256, S::kPerCu) void k_head_grad(const HeadGrad a) 
                 float v[8];
 #pragma unroll
                 for (int r = 0; r < 8; ++r) v[r] = acc[i][j][r0 + r];
-                put(c, wm + 32 * i + acc_elem(h, r0), v);
+                put(at, 32 * i + 2 * r0, v);
                 __builtin_amdgcn_sched_barrier(0);   // (few of the results in other registers at a time)
               }
           }
         };
-        const int64_t at = (int64_t)sp.n * S::TN * a.D + sp.m * S::TM;
-        if (part != nullptr) {
-          each([&](int c, int e, float(&v)[8]) { store_run8(part + c * S::TM + e, v); });
-        } else if (a.out_bf16) {
-          each([&](int c, int e, float(&v)[8]) {
-            const int64_t o = at + (int64_t)c * a.D + e;
-            if (a.add != nullptr) {
-              float u[8];
-              load_run8(a.add + o, u);
+        auto in_out = [&](int c, int e) {
+          return ((int64_t)sp.n * S::TN + c) * a.D + sp.m * S::TM + e;
+        };
+        auto added = [&](int64_t at, int o, float(&v)[8]) {
+          float u[8];
+          load_run8(a.add + at + o, u);
 #pragma unroll
-              for (int r = 0; r < 8; ++r) v[r] += u[r];
-            }
-            store_run8(static_cast<bf16*>(a.out) + o, v);
+          for (int r = 0; r < 8; ++r) v[r] += u[r];
+        };
+        if (part != nullptr) {
+          each([&](int c, int e) { return part + c * S::TM + e; },
+               [&](float* at, int o, float(&v)[8]) { store_run8(at + o, v); });
+        } else if (a.out_bf16) {
+          each(in_out, [&](int64_t at, int o, float(&v)[8]) {
+            if (a.add != nullptr) added(at, o, v);
+            store_run8(static_cast<bf16*>(a.out) + at + o, v);
           });
         } else {
-          each([&](int c, int e, float(&v)[8]) {
-            const int64_t o = at + (int64_t)c * a.D + e;
-            if (a.add != nullptr) {
-              float u[8];
-              load_run8(a.add + o, u);
-#pragma unroll
-              for (int r = 0; r < 8; ++r) v[r] += u[r];
-            }
-            store_run8(static_cast<float*>(a.out) + o, v);
+          each(in_out, [&](int64_t at, int o, float(&v)[8]) {
+            if (a.add != nullptr) added(at, o, v);
+            store_run8(static_cast<float*>(a.out) + at + o, v);
           });
         }
       });
