@@ -71,13 +71,13 @@ __device__ __forceinline__ void head_pair(int pa, int pb, int i, int& x, int& y)
 // A stage of one operand: T rows (ROWS) or columns x kStep contraction elements, in
 // 16-byte chunks.  Chunks are swizzled so that 16 neighbouring lanes' 16-byte reads, or
 // the transposed reads' 32-byte pieces of four rows, meet every bank once.
-template <int T, int kStep, bool ROWS>
+template <int T, int kStep, int kThreads, bool ROWS>
 struct HeadTile {
   static constexpr int kElems = T * kStep;
-  static constexpr int kLoads = kElems / 8 / 256;         // requests a thread, 256 chunks each
+  static constexpr int kLoads = kElems / 8 / kThreads;    // requests a thread, kThreads chunks each
   static constexpr int kCpr = ROWS ? kStep / 8 : T / 8;   // chunks a row of the stage
-  static constexpr int kRows = 256 / kCpr;        // rows of the stage a request
-  static_assert(kElems % 2048 == 0 && (ROWS || T >= 128), "a tile of whole requests");
+  static constexpr int kRows = kThreads / kCpr;   // rows of the stage a request
+  static_assert(kElems % (8 * kThreads) == 0 && (ROWS || T >= 128), "a tile of whole requests");
   static __device__ __forceinline__ int key(int r) {
     return !ROWS ? 4 * (r & 3) + ((r >> 2) & 3) : kStep == 64 ? (r >> 1) & 7 : (r >> 2) & 3;
   }
@@ -117,7 +117,7 @@ struct HeadTile {
   // Request J of a stage; lds: the wave's place in it.
   template <int J>
   __device__ __forceinline__ void request(uint32_t lds) const {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + J * 4096), "v"(off[J]),
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds + J * kThreads * 16), "v"(off[J]),
                  "s"(base)
                  : "memory", "m0");
   }
@@ -153,12 +153,13 @@ struct HeadTile {
   }
 };
 
-// Tile shape: TM x TN of the result over WM x WN waves (four), NS stages.
+// Tile shape: TM x TN of the result over WM x WN waves, NS stages, kPerCu workgroups a CU.
 template <int TM_, int TN_, int WM_, int WN_, int NS_, int KSTEP_, int PER_CU_>
 struct HeadShape {
   static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, NS = NS_, kStep = KSTEP_, kPerCu = PER_CU_;
+  static constexpr int kThreads = WM * WN * 64, kPerSimd = kPerCu * WM * WN / 4;   // waves a SIMD
   static constexpr int MT = TM / WM / 32, NT = TN / WN / 32;   // 32 x 32 tiles of a wave
-  static_assert(WM * WN == 4 && MT >= 1 && NT >= 1 && NS >= 2, "four waves");
+  static_assert(WM * WN % 4 == 0 && MT >= 1 && NT >= 1 && NS >= 2, "whole waves a SIMD");
 };
 
 // What a workgroup computes: tiles (m, n) of the result, each over the steps q0 .. q1 - 1
@@ -182,9 +183,9 @@ __device__ __forceinline__ void head_range(F&& f) {
 
 // The spans i = 0 .. spans - 1, `total` steps in all; done(span, wm, wn, acc) takes each result.
 //
-// All steps of all spans are one pipeline of NS stages in LDS.  One wave a SIMD leaves
-// the matrix unit idle wherever more than half a dozen other instructions stand between
-// two products, so that everything else is spread: a wave reads the fragments of the
+// All steps of all spans are one pipeline of NS stages in LDS.  One or two waves a SIMD leave
+// the matrix unit idle wherever more than a few other instructions stand between two
+// products, so that everything else is spread: a wave reads the fragments of the
 // next 16 contraction elements and requests a part of a later stage behind each
 // product, with addresses that take one addition a stage.  The barrier between two
 // stages stands before the products of the last 16 elements of the older one, whose
@@ -193,8 +194,8 @@ __device__ __forceinline__ void head_range(F&& f) {
 template <class S, bool AROWS, bool BROWS, typename Span, typename Done>
 __device__ __forceinline__ void head_product(const HeadProduct& pr, int spans, int total, Span span, Done done) {
   constexpr int kStep = S::kStep;
-  using TA = HeadTile<S::TM, kStep, AROWS>;
-  using TB = HeadTile<S::TN, kStep, BROWS>;
+  using TA = HeadTile<S::TM, kStep, S::kThreads, AROWS>;
+  using TB = HeadTile<S::TN, kStep, S::kThreads, BROWS>;
   constexpr int kLoads = TA::kLoads + TB::kLoads, KS = kStep / 16, MT = S::MT, NT = S::NT;
   static_assert(KS % 2 == 0, "two sets of fragments in turn");
   __shared__ __align__(16384) bf16 sa[S::NS][TA::kElems];
@@ -368,7 +369,7 @@ struct HeadFwd {
 // Log sums over this workgroup's share of the vocabulary.  A lane holds one row of
 // x for each of its NT tiles and 16 MT logits of it at a time.
 template <class S>
-__global__ __launch_bounds__(256, S::kPerCu) void k_head_fwd(const HeadFwd a) {
+__global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_fwd(const HeadFwd a) {
   int nt, part;
   if (!head_place(a.g, (int)blockIdx.x, nt, part)) return;
   const int lane = threadIdx.x & 63, h = lane >> 5;
@@ -428,7 +429,7 @@ __global__ __launch_bounds__(256, S::kPerCu) void k_head_fwd(const HeadFwd a) {
     if (h == 0) st[wmi][wn + 32 * j + (lane & 31)] = make_float2(mx, s);
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < S::TN; c += 256) {
+  for (int c = threadIdx.x; c < S::TN; c += S::kThreads) {
     const int n = nt * S::TN + c;
     float mx = kMaskScore, s = 0.0f;
 #pragma unroll
@@ -501,23 +502,18 @@ struct HeadDz {
 __device__ __forceinline__ bool head_real(const int64_t* target, int64_t n, int V) {
   return target != nullptr && target[n] >= 0 && target[n] < V;
 }
-// v as bf16 planes; neg: a sign bit to flip in all of them
-template <int PLANES>
-__device__ __forceinline__ void store_planes(bf16* p, int64_t plane, float (&v)[8], uint32_t neg = 0) {
-  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// The bf16 plane of v that comes next; v becomes what it leaves.  neg: a sign bit to flip.
+__device__ __forceinline__ u32x4 next_plane(float (&v)[8], uint32_t neg) {
+  bf16x8 o;
 #pragma unroll
-  for (int q = 0; q < PLANES; ++q) {
-    bf16x8 o;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      o[j] = (bf16)v[j];
-      if (q + 1 < PLANES) v[j] -= (float)o[j];
-    }
-    *reinterpret_cast<u32x4*>(p + q * plane) = __builtin_bit_cast(u32x4, o) ^ (neg | neg >> 16);
+  for (int j = 0; j < 8; ++j) {
+    o[j] = (bf16)v[j];
+    v[j] -= (float)o[j];
   }
+  return __builtin_bit_cast(u32x4, o) ^ (neg | neg >> 16);
 }
 template <class S, int PLANES>
-__global__ __launch_bounds__(256, S::kPerCu) void k_head_dz(const HeadDz a) {
+__global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_dz(const HeadDz a) {
   int nt, part;
   if (!head_place(a.g, (int)blockIdx.x, nt, part)) return;
   const int lane = threadIdx.x & 63, h = lane >> 5;
@@ -536,6 +532,10 @@ __global__ __launch_bounds__(256, S::kPerCu) void k_head_dz(const HeadDz a) {
       neg[j] = __float_as_uint(co) & 0x80000000u;
     }
   }
+  // Results turn in LDS, 32 tokens x 64 of the vocabulary a wave at a time, so that eight
+  // lanes store 128 bytes in a row: a store of 32 rows takes the caches four times as many requests.
+  static_assert(S::MT % 2 == 0, "64 of the vocabulary");
+  __shared__ __align__(16) char turn[S::kThreads / 64 * 4096];
   const int steps = head_steps<S>(a.pr), tiles = head_share(a.g, part);
   head_product<S, true, true>(
       a.pr, tiles, tiles * steps, [&](int i) { return HeadSpan{part + i * a.g.split, nt, 0, steps}; },
@@ -543,28 +543,47 @@ __global__ __launch_bounds__(256, S::kPerCu) void k_head_dz(const HeadDz a) {
         const int mt = sp.m;
         // else zeros past the vocabulary, and in the rows past N (of any sums, NaN among them)
         const bool inside = mt * S::TM + S::TM <= a.vocab && nt * S::TN + S::TN <= a.N;
+        char* const mine = turn + (threadIdx.x >> 6) * 4096;
+        char* const put = mine + (lane & 31) * 128;
+        const int put_key = (lane >> 1) & 7;
+        const int v0 = mt * S::TM + wm, n0 = nt * S::TN + wn;
 #pragma unroll
         for (int j = 0; j < S::NT; ++j) {
-          const int n = nt * S::TN + wn + 32 * j + (lane & 31);
-          if (n >= a.rows) continue;
-          bf16* const at = a.dz + (int64_t)n * a.ld + mt * S::TM + wm + 8 * h;
-          const int v0 = mt * S::TM + wm + 8 * h;
+          const bool real = n0 + 32 * j + (lane & 31) < a.N;
 #pragma unroll
-          for (int i = 0; i < S::MT; ++i)
+          for (int i = 0; i < S::MT; i += 2) {
+            float d[4][8];
 #pragma unroll
-            for (int r0 = 0; r0 < 16; r0 += 8) {
-              const int v = v0 + 32 * i + 2 * r0;
-              float d[8];
+            for (int q = 0; q < PLANES; ++q) {
 #pragma unroll
-              for (int r = 0; r < 8; ++r) d[r] = fast_exp2(fmaf(acc[i][j][r0 + r], kLog2e, -off[j]));
-              if (!inside) {
+              for (int c = 0; c < 4; ++c) {   // 8 elements from v0 + 32 i + 16 c + 8 h on
+                if (q == 0) {
 #pragma unroll
-                for (int r = 0; r < 8; ++r)
-                  if (v + r >= a.vocab || n >= a.N) d[r] = 0.0f;
+                  for (int r = 0; r < 8; ++r)
+                    d[c][r] = fast_exp2(fmaf(acc[i + c / 2][j][8 * (c % 2) + r], kLog2e, -off[j]));
+                  if (!inside) {
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+                      if (v0 + 32 * i + 16 * c + 8 * h + r >= a.vocab || !real) d[c][r] = 0.0f;
+                  }
+                }
+                *reinterpret_cast<u32x4*>(put + (((2 * c + h) ^ put_key) << 4)) = next_plane(d[c], neg[j]);
+                __builtin_amdgcn_sched_barrier(0);
               }
-              store_planes<PLANES>(at + 32 * i + 2 * r0, a.plane, d, neg[j]);
-              __builtin_amdgcn_sched_barrier(0);
+              // (a wave's LDS requests are served in order: the compiler alone has to keep it)
+              asm volatile("" ::: "memory");
+              __builtin_amdgcn_wave_barrier();
+#pragma unroll
+              for (int t = 0; t < 4; ++t) {
+                const int r = 8 * t + (lane >> 3), n = n0 + 32 * j + r;
+                const u32x4 o = *reinterpret_cast<const u32x4*>(mine + r * 128 + (((lane & 7) ^ ((r >> 1) & 7)) << 4));
+                if (n < a.rows)
+                  *reinterpret_cast<u32x4*>(a.dz + q * a.plane + (int64_t)n * a.ld + v0 + 32 * i + 8 * (lane & 7)) = o;
+              }
+              asm volatile("" ::: "memory");
+              __builtin_amdgcn_wave_barrier();
             }
+          }
         }
       });
 }
@@ -605,7 +624,7 @@ struct HeadGrad {
 };
 
 template <class S, bool BROWS>
-__global__ __launch_bounds__(256, S::kPerCu) void k_head_grad(const HeadGrad a) {
+__global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_grad(const HeadGrad a) {
   const int g = (int)xcd_remap(blockIdx.x, gridDim.x);
   const int steps = head_steps<S>(a.pr), rounds = a.whole / a.groups;
   const int rest = a.m_tiles * a.n_tiles - a.whole, units = rest * a.cuts;
@@ -729,14 +748,15 @@ __global__ __launch_bounds__(256) void k_head_pack(const void* x, bool x_bf16, b
     const int c = (int)(i % runs) * 8;
     float v[8];
     load_run8_of(x, x_bf16, r * D + c, D - c, v);
-    store_planes<PLANES>(out + r * ld + c, plane, v);
+#pragma unroll
+    for (int q = 0; q < PLANES; ++q) *reinterpret_cast<u32x4*>(out + q * plane + r * ld + c) = next_plane(v, 0);
   }
 }
 
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-using HeadBig = HeadShape<256, 256, 2, 2, 2, 64, 1>;
+using HeadBig = HeadShape<256, 256, 2, 4, 2, 64, 1>;
 using HeadMid = HeadShape<128, 128, 2, 2, 2, 64, 2>;
 using HeadFew = HeadShape<128, 32, 4, 1, 4, 64, 1>;
 
@@ -854,7 +874,7 @@ static void head_grad_as(HeadGrad g, const HeadCut& c, hipStream_t s) {
   g.groups = c.groups;
   g.whole = c.whole;
   g.cuts = c.cuts;
-  k_head_grad<S, BROWS><<<(unsigned)g.groups, 256, 0, s>>>(g);
+  k_head_grad<S, BROWS><<<(unsigned)g.groups, S::kThreads, 0, s>>>(g);
   const int tiles = g.m_tiles * g.n_tiles, first = g.D % S::TM != 0 ? 0 : c.cuts > 1 ? c.whole : tiles;
   if (first < tiles) k_head_join_tiles<S><<<dim3((unsigned)(tiles - first), 8), 256, 0, s>>>(g, first);
 }
@@ -942,7 +962,7 @@ extern "C" int nsa_head_fwd(const void* x, const void* w, const int64_t* target,
     a.part = part;
     a.N = (int)N;
     a.V = V;
-    k_head_fwd<S><<<head_blocks(g), 256, 0, s>>>(a);
+    k_head_fwd<S><<<head_blocks(g), S::kThreads, 0, s>>>(a);
     const HeadJoin j{part, x, w, target, logp, lse, N, g.split, V, D, x_dtype == NSA_BF16, w_dtype == NSA_BF16,
                      x_dtype == NSA_BF16 && w_dtype == NSA_F32};
     k_head_join<<<(unsigned)((N + 3) / 4), 256, 0, s>>>(j);
@@ -1014,9 +1034,9 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
       using S = decltype(sh);
       z.g = head_grid<S>(N, vocab, cu);
       if (l.px == 3)
-        k_head_dz<S, 3><<<head_blocks(z.g), 256, 0, s>>>(z);
+        k_head_dz<S, 3><<<head_blocks(z.g), S::kThreads, 0, s>>>(z);
       else
-        k_head_dz<S, 1><<<head_blocks(z.g), 256, 0, s>>>(z);
+        k_head_dz<S, 1><<<head_blocks(z.g), S::kThreads, 0, s>>>(z);
     };
     if (head_kind(N, vocab, cu) == kBig)
       form(HeadBig{});
