@@ -555,7 +555,7 @@ extern "C" int nsa_embed_fwd(const int64_t* tokens, const int64_t* pos, const vo
   NSA_CHECK(n >= 0 && n <= kEmbedRows && V >= 1 && V <= kEmbedRows && D >= 1 && D <= kEmbedWide, NSA_ERR_SHAPE);
   NSA_CHECK(embed_type(w_dtype) && embed_type(out_dtype), NSA_ERR_DTYPE);
   if (pw != nullptr) {
-    NSA_CHECK(P >= 1 && P <= kEmbedRows && (pos != nullptr || T >= 1), NSA_ERR_SHAPE);
+    NSA_CHECK(P >= 1 && P <= kEmbedRows && (n == 0 || pos != nullptr || T >= 1), NSA_ERR_SHAPE);
     NSA_CHECK(embed_type(pw_dtype), NSA_ERR_DTYPE);
   }
   if (n == 0) return NSA_OK;

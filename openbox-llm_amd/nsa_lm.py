@@ -165,8 +165,8 @@ def linear_logprobs(x, weight, targets=None):
     ``lse`` is the logits' log-sum-exp and ``logp`` (with integer ``targets [...]``)
     the target's log probability; a target outside ``0 .. V-1`` (``-100`` included)
     leaves 0 and no gradient.  Differentiable in x and weight, from both outputs;
-    the backward forms the logits a second time, in pieces of the vocabulary that
-    take at most about 1 GB, and has the same bits on every run.
+    the backward forms the logits a second time, in pieces of 1 GB at most (or 256
+    of the vocabulary), and has the same bits on every run.
 
     float32 rows are computed in float32's precision.  bfloat16 rows are products of
     bfloat16 with float32 sums, and the logits' gradient is rounded once to bfloat16

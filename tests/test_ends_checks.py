@@ -56,6 +56,12 @@ def test_embed_refusals():
     assert size(1000, 64, 1) > size(1000, 64, 0) >= 2 * 64 * 4
 
 
+def test_embed_of_no_tokens():
+    lib = _lib()
+    for T in (0, 4):   # [.., 0] and [0, 4], by position
+        assert lib.nsa_embed_fwd(None, None, None, 16, None, 0, T, 10, 3, 8, 1.0, 0, 0, 0, None) == 0
+
+
 def test_head_refusals():
     lib = _lib()
 

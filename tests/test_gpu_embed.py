@@ -154,6 +154,19 @@ def test_integer_types_strides_and_alignment():
     assert torch.equal(a, torch.bincount((t % 9).view(-1), minlength=9).float()[:, None].expand(9, D))
 
 
+@pytest.mark.parametrize("shape", [(0,), (4, 0), (0, 4)], ids=str)
+@pytest.mark.parametrize("pos", ["none", "given", "index"])
+def test_no_tokens(shape, pos):
+    import nsa_lm
+    dev = require_gpu()
+    t = torch.empty(shape, dtype=torch.long, device=dev)
+    w, p = (torch.randn(n, 12, device=dev, requires_grad=True) for n in (7, 5))
+    y = nsa_lm.embed(t, w, 1.0, None if pos == "none" else p, t if pos == "given" else None)
+    assert y.shape == (*shape, 12)
+    y.sum().backward()
+    assert not w.grad.any() and (pos == "none" or not p.grad.any())
+
+
 def test_nan_rows_stay_where_they_are():
     import nsa_lm
     dev = require_gpu()
