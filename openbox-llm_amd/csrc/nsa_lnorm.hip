@@ -41,55 +41,138 @@ struct LnArgs {
   bool w_bf16, y_bf16;
 };
 
+// A run of 8 elements as it lies in memory, `n` of them in the row: of rows in which every
+// thread's runs are whole, of others, and of rows of less than 8 elements.  The run at a
+// row's end is asked for as the row's last 8 elements, like any other, and shifted when it
+// is used: an element at a time it would hold up all loads behind it (66974 x 501 bf16,
+// backward: 186 us so, 75 now).
+enum { kWhole, kEdge, kTiny };
+template <int EDGE>
+struct RunAt {
+  uint32_t off;   // what is loaded, from the row's first element on
+  int n;
+  __device__ __forceinline__ RunAt(int D, int c) : off((uint32_t)(EDGE == kEdge && D - c < 8 ? D - 8 : c)), n(D - c) {}
+};
+template <typename T>
+struct RawRun {
+  typedef T vec __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  vec v;
+  template <int EDGE>
+  __device__ __forceinline__ void load(const T* row, const RunAt<EDGE>& at) {
+    if constexpr (EDGE != kTiny) {
+      v = *reinterpret_cast<const vec*>(row + at.off);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j < at.n ? row[at.off + j] : (T)0.0f;
+    }
+  }
+  template <int EDGE>
+  __device__ __forceinline__ void get(float (&f)[8], const RunAt<EDGE>& at) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (float)v[j];
+    if constexpr (EDGE == kEdge) {
+      if (at.n > 0 && at.n < 8) {
+        const int by = 8 - at.n;
+#pragma unroll
+        for (int k = 4; k >= 1; k >>= 1)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = by & k ? (j + k < 8 ? f[j + k] : 0.0f) : f[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = at.n > 0 ? f[j] : 0.0f;
+    }
+  }
+};
+// Weights, of either type.
+template <int EDGE>
+__device__ __forceinline__ void ln_weights(const void* w, bool is_bf16, const RunAt<EDGE>& at, float (&f)[8]) {
+  if (is_bf16) {
+    RawRun<bf16> r;
+    r.load(static_cast<const bf16*>(w), at);
+    r.get(f, at);
+  } else {
+    RawRun<float> r;
+    r.load(static_cast<const float*>(w), at);
+    r.get(f, at);
+  }
+}
+
+// Sums of K values over a row's threads: TPR of them, or past a wave the workgroup's
+// (whole waves, TPR at most).  buf: K * TPR / 64 floats.
+template <int TPR, int K>
+__device__ __forceinline__ void row_sums(float (&v)[K], float* buf) {
+  static_assert(TPR <= 16 * kWave, "sixteen waves");
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = wave_sum<(TPR < kWave ? TPR : kWave)>(v[k]);
+  if (TPR <= kWave) return;
+  const int tid = threadIdx.x;
+  if ((tid & (kWave - 1)) == 0) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) buf[K * (tid / kWave) + k] = v[k];
+  }
+  __syncthreads();
+  // (every lane of 16 takes one wave's)
+  const int i = tid & 15;
+  const bool there = i < (int)(blockDim.x / kWave);
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = wave_sum<16>(there ? buf[K * i + k] : 0.0f);
+}
+
 // h of one run: x + r rounded to r's type (RES), or x itself
-template <typename XT, typename RT, bool RES>
-__device__ __forceinline__ void ln_sum8(const LnArgs& a, int64_t at, int n, float (&h)[8]) {
-  load_run8(static_cast<const XT*>(a.x) + at, n, h);
+template <typename XT, typename RT, bool RES, int EDGE>
+__device__ __forceinline__ void ln_sum8(const LnArgs& a, int64_t base, const RunAt<EDGE>& at, float (&h)[8]) {
+  RawRun<XT> x;
+  RawRun<RT> res;
+  x.load(static_cast<const XT*>(a.x) + base, at);
+  if (RES) res.load(static_cast<const RT*>(a.res) + base, at);
+  x.get(h, at);
   if (RES) {
     float r[8];
-    load_run8(static_cast<const RT*>(a.res) + at, n, r);
+    res.get(r, at);
 #pragma unroll
     for (int j = 0; j < 8; ++j) h[j] = (float)(RT)(h[j] + r[j]);
   }
 }
 
-// TPR threads a row, NV runs of 8 a thread (NV = 0: any length, h formed again for every pass).
-template <typename XT, typename RT, bool RES, int TPR, int NV>
+// TPR threads a row (past 64: the workgroup's, TPR at most), NV runs of 8 a thread (NV = 0:
+// any length, h formed again for every pass).
+template <typename XT, typename RT, bool RES, int TPR, int NV, int EDGE>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_ln_fwd(const LnArgs a) {
   constexpr int W = TPR > kWave ? TPR / kWave : 1;
   __shared__ float red[2][W];
-  const int t = threadIdx.x & (TPR - 1);
+  const int nth = TPR <= 64 ? TPR : (int)blockDim.x, t = TPR <= 64 ? threadIdx.x & (TPR - 1) : threadIdx.x;
   const int64_t row = TPR <= 64 ? (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR : (int64_t)blockIdx.x;
   if (TPR <= 64 && row >= a.rows) return;   // (all of a row's lanes; no barrier follows for these)
   const int D = a.D;
   const int64_t base = row * D;
-  const int nrun = NV > 0 ? NV : (D + 8 * TPR - 1) / (8 * TPR);
+  const int nrun = NV > 0 ? NV : (D + 8 * nth - 1) / (8 * nth);
   float h[NV > 0 ? NV : 1][8];
-  float s = 0.0f;
+  float s[1] = {0.0f};
 #pragma unroll
   for (int i = 0; i < nrun; ++i) {
     float(&hi)[8] = h[NV > 0 ? i : 0];
-    const int c = 8 * (i * TPR + t), n = D - c;
-    ln_sum8<XT, RT, RES>(a, base + c, n, hi);
+    const int c = 8 * (i * nth + t), n = D - c;
+    ln_sum8<XT, RT, RES>(a, base, RunAt<EDGE>(D, c), hi);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s += hi[j];
+    for (int j = 0; j < 8; ++j) s[0] += hi[j];
     if (RES && n > 0) store_run8(static_cast<RT*>(a.h) + base + c, n, hi);
   }
-  const float mu = row_sum<TPR>(s, red[0]) * a.inv_d;
-  float ss = 0.0f;
+  row_sums<TPR>(s, red[0]);
+  const float mu = s[0] * a.inv_d;
+  float ss[1] = {0.0f};
 #pragma unroll
   for (int i = 0; i < nrun; ++i) {
     float(&hi)[8] = h[NV > 0 ? i : 0];
-    const int c = 8 * (i * TPR + t), n = D - c;
-    if (NV == 0) ln_sum8<XT, RT, RES>(a, base + c, n, hi);
+    const int c = 8 * (i * nth + t), n = D - c;
+    if (NV == 0) ln_sum8<XT, RT, RES>(a, base, RunAt<EDGE>(D, c), hi);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       hi[j] -= mu;
-      ss += j < n ? hi[j] * hi[j] : 0.0f;
+      ss[0] += j < n ? hi[j] * hi[j] : 0.0f;
     }
   }
-  ss = row_sum<TPR>(ss, red[1]);
-  const float rstd = 1.0f / sqrtf(ss * a.inv_d + a.eps);
+  row_sums<TPR>(ss, red[1]);
+  const float rstd = 1.0f / sqrtf(ss[0] * a.inv_d + a.eps);
   if (a.stat != nullptr && t == 0) {
     a.stat[2 * row] = mu;
     a.stat[2 * row + 1] = rstd;
@@ -97,15 +180,15 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_ln_fwd(const LnArgs a
 #pragma unroll
   for (int i = 0; i < nrun; ++i) {
     float(&hi)[8] = h[NV > 0 ? i : 0];
-    const int c = 8 * (i * TPR + t), n = D - c;
+    const int c = 8 * (i * nth + t), n = D - c;
     if (NV == 0) {
-      ln_sum8<XT, RT, RES>(a, base + c, n, hi);
+      ln_sum8<XT, RT, RES>(a, base, RunAt<EDGE>(D, c), hi);
 #pragma unroll
       for (int j = 0; j < 8; ++j) hi[j] -= mu;
     }
     float wv[8], bv[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    load_run8_of(a.w, a.w_bf16, c, n, wv);
-    if (a.b != nullptr) load_run8_of(a.b, a.w_bf16, c, n, bv);
+    ln_weights(a.w, a.w_bf16, RunAt<EDGE>(D, c), wv);
+    if (a.b != nullptr) ln_weights(a.b, a.w_bf16, RunAt<EDGE>(D, c), bv);
 #pragma unroll
     for (int j = 0; j < 8; ++j) hi[j] = (hi[j] * rstd) * wv[j] + bv[j];
     if (n > 0) {
@@ -128,67 +211,23 @@ struct LnBwdArgs {
   bool w_bf16, dx_bf16;
 };
 
-// A run of 8 elements as it lies in memory; elements past the row's end are 0.
-template <typename T> struct RawRun;
-template <> struct RawRun<bf16> {
-  bf16x8u v;
-  __device__ __forceinline__ void load(const bf16* p, int n) {
-    if (n >= 8) {
-      v = *reinterpret_cast<const bf16x8u*>(p);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : (bf16)0.0f;
-    }
-  }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = (float)v[j];
-  }
-};
-template <> struct RawRun<float> {
-  float v[8];
-  __device__ __forceinline__ void load(const float* p, int n) { load_run8(p, n, v); }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = v[j];
-  }
-};
-
-// Sums of two values over a row's N threads; `buf` as in row_sum, twice as long.
-template <int N>
-__device__ __forceinline__ void row_sum2(float& u, float& v, float* buf) {
-  u = wave_sum<(N < kWave ? N : kWave)>(u);
-  v = wave_sum<(N < kWave ? N : kWave)>(v);
-  if (N <= kWave) return;
-  if ((threadIdx.x & (kWave - 1)) == 0) {
-    buf[2 * (threadIdx.x / kWave)] = u;
-    buf[2 * (threadIdx.x / kWave) + 1] = v;
-  }
-  __syncthreads();
-  u = v = 0.0f;
-#pragma unroll
-  for (int i = 0; i < N / kWave; ++i) {
-    u += buf[2 * i];
-    v += buf[2 * i + 1];
-  }
-}
-
 // YT: dy; RT: h, dh and dres.  dres is null where dx serves both (one type).
-template <typename YT, typename RT, int TPR, int NV>
+template <typename YT, typename RT, int TPR, int NV, int EDGE>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_ln_bwd(const LnBwdArgs a) {
   constexpr int W = TPR > kWave ? TPR / kWave : 1;
   constexpr int RPG = TPR <= 64 ? 256 / TPR : 1;   // rows at a time
   __shared__ float red[2][2 * W];
   __shared__ float sums[RPG > 1 ? 8 * TPR * NV : 1];
-  const int t = threadIdx.x & (TPR - 1);
-  const int sub = threadIdx.x / TPR;
+  const int nth = TPR <= 64 ? TPR : (int)blockDim.x, t = TPR <= 64 ? threadIdx.x & (TPR - 1) : threadIdx.x;
+  const int sub = TPR <= 64 ? threadIdx.x / TPR : 0;
   const int D = a.D;
+  auto run_at = [&](int i) { return RunAt<EDGE>(D, 8 * (i * nth + t)); };
   // where the registers hold them: the weights for all rows, and dh asked for with the rest of a row
   constexpr bool kHold = NV * TPR <= 1024;
   float w[kHold ? NV : 1][8], dw[NV][8], db[NV][8];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if (kHold) load_run8_of(a.w, a.w_bf16, 8 * (i * TPR + t), D - 8 * (i * TPR + t), w[kHold ? i : 0]);
+    if (kHold) ln_weights(a.w, a.w_bf16, run_at(i), w[kHold ? i : 0]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) dw[i][j] = db[i][j] = 0.0f;
   }
@@ -197,83 +236,82 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_ln_bwd(const LnBwdArg
   // a row of several waves is asked for before the sums of the row ahead of it, whose barrier
   // would leave the memory idle; wider rows (two runs a thread) have no registers for that
   constexpr bool kNext = kHold && TPR > kWave;
-  struct Row {
+  struct Run {
     RawRun<RT> h, d;
     RawRun<YT> g;
-    float mu, rstd;
-  };
-  Row ahead[kNext ? NV : 1];
+  } ahead[kHold ? NV : 1];
+  float mu_next = 0.0f, rstd_next = 0.0f;
   auto ask = [&](int64_t row) {
     const int64_t base = row * D;
 #pragma unroll
-    for (int i = 0; i < (kNext ? NV : 0); ++i) {
-      const int c = 8 * (i * TPR + t), n = D - c;
-      ahead[i].h.load(static_cast<const RT*>(a.h) + base + c, n);
-      ahead[i].g.load(static_cast<const YT*>(a.dy) + base + c, n);
-      if (a.dh != nullptr) ahead[i].d.load(static_cast<const RT*>(a.dh) + base + c, n);
+    for (int i = 0; i < (kHold ? NV : 0); ++i) {
+      const RunAt<EDGE> at = run_at(i);
+      ahead[i].h.load(static_cast<const RT*>(a.h) + base, at);
+      ahead[i].g.load(static_cast<const YT*>(a.dy) + base, at);
+      if (a.dh != nullptr) ahead[i].d.load(static_cast<const RT*>(a.dh) + base, at);
     }
-    ahead[0].mu = a.stat[2 * row];
-    ahead[0].rstd = a.stat[2 * row + 1];
+    mu_next = a.stat[2 * row];
+    rstd_next = a.stat[2 * row + 1];
   };
   int64_t row = (int64_t)blockIdx.x * RPG + sub;
   if (kNext && row < a.rows) ask(row);
   for (; row < a.rows; row += step) {
     const int64_t base = row * D;
-    const float mu = kNext ? ahead[0].mu : a.stat[2 * row], rstd = kNext ? ahead[0].rstd : a.stat[2 * row + 1];
+    if (!kNext) ask(row);
+    const float mu = mu_next, rstd = rstd_next;
     float n_[NV][8], g[NV][8], d[kHold ? NV : 1][8];
-    float s1 = 0.0f, s2 = 0.0f;
-    auto load_dh = [&](int i, float(&v)[8]) {
-      const int c = 8 * (i * TPR + t);
-      if (a.dh != nullptr) {
-        load_run8(static_cast<const RT*>(a.dh) + base + c, D - c, v);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-      }
-    };
+    float sum[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = 8 * (i * TPR + t), n = D - c;
-      if constexpr (kNext) {
-        ahead[i].h.get(n_[i]);
-        ahead[i].g.get(g[i]);
+      const RunAt<EDGE> at = run_at(i);
+      if constexpr (kHold) {
+        ahead[i].h.get(n_[i], at);
+        ahead[i].g.get(g[i], at);
         if (a.dh != nullptr) {
-          ahead[i].d.get(d[i]);
+          ahead[i].d.get(d[i], at);
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j) d[i][j] = 0.0f;
         }
       } else {
-        load_run8(static_cast<const RT*>(a.h) + base + c, n, n_[i]);
-        load_run8(static_cast<const YT*>(a.dy) + base + c, n, g[i]);   // (0 past the row's end)
-        if (kHold) load_dh(i, d[kHold ? i : 0]);
+        Run& r = ahead[0];
+        r.h.load(static_cast<const RT*>(a.h) + base, at);
+        r.g.load(static_cast<const YT*>(a.dy) + base, at);
+        r.h.get(n_[i], at);
+        r.g.get(g[i], at);
       }
     }
     if (kNext && row + step < a.rows) ask(row + step);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float(&wi)[8] = w[kHold ? i : 0];
-      if (!kHold) load_run8_of(a.w, a.w_bf16, 8 * (i * TPR + t), D - 8 * (i * TPR + t), wi);
+      if (!kHold) ln_weights(a.w, a.w_bf16, run_at(i), wi);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         n_[i][j] = (n_[i][j] - mu) * rstd;
         db[i][j] += g[i][j];
         dw[i][j] += g[i][j] * n_[i][j];
         g[i][j] *= wi[j];
-        s1 += g[i][j];
-        s2 += g[i][j] * n_[i][j];
+        sum[0] += g[i][j];
+        sum[1] += g[i][j] * n_[i][j];
       }
     }
     // two buffers in turn: the next row's sums are not written over those still being read
-    row_sum2<TPR>(s1, s2, red[turn & 1]);
-    s1 *= a.inv_d;
-    s2 *= a.inv_d;
+    row_sums<TPR>(sum, red[turn & 1]);
+    const float s1 = sum[0] * a.inv_d, s2 = sum[1] * a.inv_d;
     ++turn;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = 8 * (i * TPR + t), n = D - c;
+      const int c = 8 * (i * nth + t), n = D - c;
       float(&di)[8] = d[kHold ? i : 0];
-      if (!kHold) load_dh(i, di);
+      if (!kHold) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) di[j] = 0.0f;
+        if (a.dh != nullptr) {
+          ahead[0].d.load(static_cast<const RT*>(a.dh) + base, run_at(i));
+          ahead[0].d.get(di, run_at(i));
+        }
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) di[j] += rstd * (g[i][j] - s1 - n_[i][j] * s2);
       if (n > 0) {
@@ -291,7 +329,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_ln_bwd(const LnBwdArg
   if constexpr (RPG == 1) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = 8 * (i * TPR + t);
+      const int c = 8 * (i * nth + t);
       if (c < D) {
         store_run8(out + c, D - c, dw[i]);
         store_run8(out + next + c, D - c, db[i]);
@@ -327,13 +365,13 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_ln_bwd(const LnBwdArg
 // Rows past kLnBwdMax: one workgroup a row, read twice.
 template <typename YT, typename RT>
 __global__ __launch_bounds__(1024) void k_ln_bwd_long(const LnBwdArgs a) {
-  __shared__ float red[2][32];
+  __shared__ float red[2][32];   // (rows past kLnBwdMax only: wide)
   const int D = a.D;
   int turn = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, ++turn) {
     const int64_t base = row * D;
     const float mu = a.stat[2 * row], rstd = a.stat[2 * row + 1];
-    float s1 = 0.0f, s2 = 0.0f;
+    float sum[2] = {0.0f, 0.0f};
     for (int c = 8 * threadIdx.x; c < D; c += 8 * 1024) {
       float h[8], g[8], w[8];
       load_run8(static_cast<const RT*>(a.h) + base + c, D - c, h);
@@ -342,13 +380,12 @@ __global__ __launch_bounds__(1024) void k_ln_bwd_long(const LnBwdArgs a) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float v = g[j] * w[j];
-        s1 += v;
-        s2 += v * ((h[j] - mu) * rstd);
+        sum[0] += v;
+        sum[1] += v * ((h[j] - mu) * rstd);
       }
     }
-    row_sum2<1024>(s1, s2, red[turn & 1]);
-    s1 *= a.inv_d;
-    s2 *= a.inv_d;
+    row_sums<1024>(sum, red[turn & 1]);
+    const float s1 = sum[0] * a.inv_d, s2 = sum[1] * a.inv_d;
     for (int c = 8 * threadIdx.x; c < D; c += 8 * 1024) {
       const int n = D - c;
       float h[8], g[8], w[8], d[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -421,8 +458,10 @@ __global__ __launch_bounds__(1024) void k_ln_dw(const float* __restrict__ part, 
   }
 }
 
-// Threads a row and runs a thread: the fewest threads that hold the row with one
-// run each; past 8192 elements two or four runs in 1024.
+// Threads a row (the most, from which the kernel's registers follow) and runs a thread:
+// the fewest threads that hold the row with one run each; past 8192 elements two or
+// four runs.  Past a wave as many waves are launched as the row needs (8184 x 4100
+// bf16 in 9 waves: forward 46 us, backward 76; 75 and 110 in 16).
 struct LnShape {
   int tpr, nv;
 };
@@ -436,14 +475,34 @@ static LnShape ln_shape(int D) {
   return {1024, D <= kLnRegMax ? 4 : 0};
 }
 
+static int ln_threads(LnShape s, int D) {
+  if (s.tpr <= 64) return 256;
+  if (s.nv == 0) return s.tpr;
+  return ((D + 7) / 8 + s.nv * kWave - 1) / (s.nv * kWave) * kWave;
+}
+
+// How a row's runs lie in its threads
+template <int TPR, typename F>
+static void ln_edge(LnShape s, int D, F f) {
+  const int threads = TPR <= 64 ? TPR : ln_threads(s, D);
+  if (D == threads * s.nv * 8) return f(std::integral_constant<int, kWhole>{});
+  if constexpr (TPR == 8) {
+    if (D < 8) return f(std::integral_constant<int, kTiny>{});
+  }
+  f(std::integral_constant<int, kEdge>{});
+}
+
 template <typename XT, typename RT, bool RES>
 static int ln_fwd_launch(const LnArgs& a, hipStream_t s) {
   const LnShape sh = ln_shape(a.D);
-#define NSA_LN_CASE(TPR, NV)                                                                 \
-  if (sh.tpr == TPR && sh.nv == NV) {                                                        \
-    const int64_t grid = TPR <= 64 ? (a.rows + 256 / TPR - 1) / (256 / TPR) : a.rows;        \
-    k_ln_fwd<XT, RT, RES, TPR, NV><<<(unsigned)grid, TPR <= 64 ? 256 : TPR, 0, s>>>(a);      \
-    return nsa_launch_status();                                                              \
+  const int threads = ln_threads(sh, a.D);
+#define NSA_LN_CASE(TPR, NV)                                                                                   \
+  if (sh.tpr == TPR && sh.nv == NV) {                                                                          \
+    const unsigned grid = (unsigned)(TPR <= 64 ? (a.rows + 256 / TPR - 1) / (256 / TPR) : a.rows);             \
+    ln_edge<TPR>(sh, a.D, [&](auto e) {                                                                        \
+      k_ln_fwd<XT, RT, RES, TPR, NV, decltype(e)::value><<<grid, threads, 0, s>>>(a);                          \
+    });                                                                                                        \
+    return nsa_launch_status();                                                                                \
   }
   NSA_LN_SHAPES(NSA_LN_CASE) NSA_LN_CASE(1024, 4) NSA_LN_CASE(1024, 0)
 #undef NSA_LN_CASE
@@ -464,7 +523,8 @@ static int64_t ln_bwd_groups(int64_t rows, int D, int cu) {
   const LnShape sh = ln_shape(D);
   const int rpg = sh.tpr <= 64 ? 256 / sh.tpr : 1;
   const int64_t groups = (rows + rpg - 1) / rpg;
-  const int64_t most = (int64_t)cu * (sh.tpr <= 256 ? 8 : 2048 / sh.tpr);
+  const int threads = ln_threads(sh, D);
+  const int64_t most = (int64_t)cu * (threads <= 256 ? 8 : 2048 / threads);
   return groups < most ? groups : most;
 }
 
@@ -480,10 +540,13 @@ static int ln_bwd_launch(LnBwdArgs a, void* dw, void* db, hipStream_t s) {
       k_ln_dw_wide<YT, RT><<<dim3((unsigned)((a.D + 2047) / 2048), (unsigned)grid), 256, 0, s>>>(a);
     done = true;
   }
-#define NSA_LN_CASE(TPR, NV)                                                            \
-  if (!done && sh.tpr == TPR && sh.nv == NV) {                                          \
-    k_ln_bwd<YT, RT, TPR, NV><<<(unsigned)grid, TPR <= 64 ? 256 : TPR, 0, s>>>(a);      \
-    done = true;                                                                        \
+  const int threads = ln_threads(sh, a.D);
+#define NSA_LN_CASE(TPR, NV)                                                                       \
+  if (!done && sh.tpr == TPR && sh.nv == NV) {                                                     \
+    ln_edge<TPR>(sh, a.D, [&](auto e) {                                                            \
+      k_ln_bwd<YT, RT, TPR, NV, decltype(e)::value><<<(unsigned)grid, threads, 0, s>>>(a);         \
+    });                                                                                            \
+    done = true;                                                                                   \
   }
   NSA_LN_SHAPES(NSA_LN_CASE)
 #undef NSA_LN_CASE
