@@ -759,6 +759,8 @@ __global__ __launch_bounds__(256) void k_head_pack(const void* x, bool x_bf16, b
 using HeadBig = HeadShape<256, 256, 2, 4, 2, 64, 1>;
 using HeadMid = HeadShape<128, 128, 2, 2, 2, 64, 2>;
 using HeadFew = HeadShape<128, 32, 4, 1, 4, 64, 1>;
+using HeadFew64 = HeadShape<128, 64, 2, 2, 3, 64, 2>;
+using HeadFew128 = HeadShape<128, 128, 2, 2, 4, 64, 1>;
 
 static bool head_type(int dtype) { return dtype == NSA_F32 || dtype == NSA_BF16; }
 static bool head_shape_ok(int64_t N, int V, int D) {
@@ -794,12 +796,16 @@ static void head_pack(const void* x, int dtype, void* out, int64_t rows, int D, 
     k_head_pack<1><<<grid, 256, 0, s>>>(x, dtype == NSA_BF16, static_cast<bf16*>(out), rows, D, ld);
 }
 
-// Tile of the product over the vocabulary: 256 x 256 where that gives every compute
-// unit a tile, 32 rows of x where there are no more, 128 x 128 between.
-enum { kFew, kMid, kBig };
+// Tile of the product over the vocabulary: 256 x 256 where that gives every compute unit
+// a tile, else 128 x 128.  The forward of up to 128 rows, one tile across, waits for W: it
+// takes the narrowest of 32, 64 and 128 rows, with stages for more of W under way (bf16, W
+// 32000 x 4096, 64 and 128 rows: 50 and 53 us, 67 and 71 in the common 128 x 128).
+enum { kFew, kFew64, kFew128, kMid, kBig };
 static int head_kind(int64_t N, int V, int cu) {
-  if (N <= 32) return kFew;
-  return ((N + 255) / 256) * ((V + 255) / 256) >= cu ? kBig : kMid;
+  return ((N + 255) / 256) * ((V + 255) / 256) >= cu && N > 128 ? kBig : kMid;
+}
+static int head_fwd_kind(int64_t N, int V, int cu) {
+  return N <= 32 ? kFew : N <= 64 ? kFew64 : N <= 128 ? kFew128 : head_kind(N, V, cu);
 }
 template <class S>
 static HeadGrid head_grid(int64_t N, int vocab, int cu) {
@@ -822,6 +828,8 @@ static unsigned head_blocks(const HeadGrid& g) {
 template <typename F>
 static auto head_as(int kind, F f) {
   if (kind == kFew) return f(HeadFew{});
+  if (kind == kFew64) return f(HeadFew64{});
+  if (kind == kFew128) return f(HeadFew128{});
   if (kind == kMid) return f(HeadMid{});
   return f(HeadBig{});
 }
@@ -925,7 +933,7 @@ extern "C" size_t nsa_head_fwd_workspace(int64_t N, int V, int D, int x_dtype, i
   const void* at = reinterpret_cast<const void*>(aligned ? 16 : 1);
   const HeadLayout l = head_layout(N, V, D, at, at, x_dtype, w_dtype);
   const int cu = device_cu_count(static_cast<hipStream_t>(stream));
-  const int split = head_as(head_kind(N, V, cu), [&](auto s) { return head_grid<decltype(s)>(N, V, cu).split; });
+  const int split = head_as(head_fwd_kind(N, V, cu), [&](auto s) { return head_grid<decltype(s)>(N, V, cu).split; });
   return l.x_bytes + l.w_bytes + (size_t)split * N * sizeof(float2);
 }
 
@@ -940,7 +948,7 @@ extern "C" int nsa_head_fwd(const void* x, const void* w, const int64_t* target,
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int cu = device_cu_count(s);
   const HeadLayout l = head_layout(N, V, D, x, w, x_dtype, w_dtype);
-  return head_as(head_kind(N, V, cu), [&](auto sh) -> int {
+  return head_as(head_fwd_kind(N, V, cu), [&](auto sh) -> int {
     using S = decltype(sh);
     const HeadGrid g = head_grid<S>(N, V, cu);
     NSA_CHECK(workspace != nullptr &&

@@ -112,6 +112,12 @@ def test_large_tiles(N, V, D, xd):
     _check(N, V, D, xd, xd, seed=N)
 
 
+@pytest.mark.parametrize("N,V,D,xd", [(32, 140001, 72, BF), (64, 140001, 72, BF), (65, 70001, 136, BF), (128, 70001, 40, F32)])
+def test_few_rows_of_many_tokens(N, V, D, xd):
+    """Several tiles of the vocabulary one after another in a workgroup."""
+    _check(N, V, D, xd, xd, seed=N)
+
+
 @pytest.mark.parametrize("N,V,D,xd", [(22100, 13000, 64, BF), (8000, 13001, 40, F32)])
 def test_several_pieces_of_the_vocabulary(N, V, D, xd):
     _check(N, V, D, xd, xd, seed=V)
