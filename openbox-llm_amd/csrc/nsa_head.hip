@@ -7,16 +7,18 @@
 //
 //   dz_nv = a_n e^{z_nv - lse_n} + b_n [v = t_n],   dx = dz W,   dW = dz^T x.
 //
-// Four products, each on v_mfma_f32_32x32x16_bf16 with float32 sums: z for the
+// Four products on the matrix instructions with float32 sums (bf16: 32x32x16): z for the
 // log sums (a running maximum and sum in registers), z again for dz, and the two
-// of the gradients.  dz exists for a piece of the vocabulary at a time, rounded once
-// to bf16 as the products' operand (the relative rounding of a probability and of
-// an operand are the same; a sum over the vocabulary or the rows averages it).
+// of the gradients.  dz exists for a piece of the vocabulary at a time; beside bf16 rows
+// it is rounded once to bf16 as the products' operand (the relative rounding of a
+// probability and of an operand are the same; a sum over the vocabulary or the rows
+// averages it), beside float32 rows it is float32 or its planes.
 //
-// float32 operands go as three bf16 planes p0 + p1 + p2 = x, |x - p0 - p1 - p2| <=
-// 2^-27 |x|: six products of planes (i + j <= 2) leave out terms below 2^-26 of the
-// product, less than float32's own rounding.  A bf16 operand beside float32 rows is
-// one plane; float32 weights beside bf16 rows are rounded to bf16 first.
+// float32 rows and weights of few rows go through v_mfma_f32_32x32x2_f32 as they are; of many
+// as three bf16 planes p0 + p1 + p2 = x, |x - p0 - p1 - p2| <= 2^-27 |x|: six products of
+// planes (i + j <= 2) leave out terms below 2^-26 of the product, less than float32's own
+// rounding.  A bf16 operand beside float32 rows is one plane; float32 weights beside bf16 rows
+// are rounded to bf16 first.
 //
 // Layout: an operand is read either along its rows (the contraction runs along
 // memory) into a [rows][64] tile, or across them into a [64][columns] tile that
@@ -39,7 +41,7 @@ constexpr int64_t kHeadPieceMost = 1 << 20;  // most tokens of a piece: offsets 
 // An operand of a product: bf16 planes; ROWS: [rows][ld], contraction along a row;
 // otherwise [contraction][ld].
 struct HeadOperand {
-  const bf16* p;
+  const void* p;   // bf16, or float32 where the shape's elements are
   int64_t plane;   // elements between planes
   int64_t ld;      // elements between rows, a multiple of 8
   int rows;        // rows (ROWS) or columns: of the result
@@ -68,18 +70,40 @@ __device__ __forceinline__ void head_pair(int pa, int pb, int i, int& x, int& y)
   }
 }
 
+// What a product's operands are made of.  A step of the contraction is 128 bytes of a
+// row; a fragment is 16 bytes a lane: 8 elements of bf16 for one matrix instruction,
+// 4 of float32 for four.
+template <typename E> struct HeadType;
+template <> struct HeadType<bf16> {
+  typedef bf16x8 Frag;
+  static __device__ __forceinline__ f32x16 product(Frag a, Frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct HeadType<float> {
+  typedef f32x4 Frag;
+  static __device__ __forceinline__ f32x16 product(Frag a, Frag b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
 // A stage of one operand: T rows (ROWS) or columns x kStep contraction elements, in
-// 16-byte chunks.  Chunks are swizzled so that 16 neighbouring lanes' 16-byte reads, or
-// the transposed reads' 32-byte pieces of four rows, meet every bank once.
-template <int T, int kStep, int kThreads, bool ROWS>
+// 16-byte chunks.  Chunks are swizzled so that 16 neighbouring lanes' 16-byte reads, the
+// transposed reads' 32-byte pieces of four rows, or 32 neighbouring columns of two rows
+// meet every bank once.
+template <typename E, int T, int kThreads, bool ROWS>
 struct HeadTile {
-  static constexpr int kElems = T * kStep;
-  static constexpr int kLoads = kElems / 8 / kThreads;    // requests a thread, kThreads chunks each
-  static constexpr int kCpr = ROWS ? kStep / 8 : T / 8;   // chunks a row of the stage
-  static constexpr int kRows = kThreads / kCpr;   // rows of the stage a request
-  static_assert(kElems % (8 * kThreads) == 0 && (ROWS || T >= 128), "a tile of whole requests");
+  typedef typename HeadType<E>::Frag Frag;
+  static constexpr bool kWide = sizeof(E) == 4;
+  static constexpr int kB = sizeof(E), kChunk = 16 / kB, kStep = 128 / kB, kBytes = T * 128;
+  static constexpr int kLoads = kBytes / 16 / kThreads;   // requests a thread, kThreads chunks each
+  static constexpr int kCpr = ROWS ? 8 : T / kChunk;      // chunks a row of the stage
+  static constexpr int kRows = kThreads / kCpr;           // rows of the stage a request
+  static_assert(kBytes % (16 * kThreads) == 0 && (ROWS || T >= 128), "a tile of whole requests");
   static __device__ __forceinline__ int key(int r) {
-    return !ROWS ? 4 * (r & 3) + ((r >> 2) & 3) : kStep == 64 ? (r >> 1) & 7 : (r >> 2) & 3;
+    return ROWS ? (r >> 1) & 7 : kWide ? 8 * ((r >> 2) & 1) : 4 * (r & 3) + ((r >> 2) & 3);
   }
 
   // Request j brings rows j kRows + tid / kCpr of the stage, each lane 16 bytes.  Past
@@ -95,15 +119,15 @@ struct HeadTile {
     for (int j = 0; j < kLoads; ++j) {
       const int r = j * kRows + tid / kCpr, c = (tid % kCpr) ^ key(r);
       if (ROWS)
-        off[j] = (uint32_t)((r < last ? r : last) * o.ld * 2 + c * 16);
+        off[j] = (uint32_t)((r < last ? r : last) * o.ld * kB + c * 16);
       else
-        off[j] = (uint32_t)((r < end ? r : end) * o.ld * 2 + (8 * c <= last ? c * 16 : 0));
+        off[j] = (uint32_t)((r < end ? r : end) * o.ld * kB + (kChunk * c <= last ? c * 16 : 0));
     }
   }
   __device__ __forceinline__ void aim(const HeadOperand& o, int first_, int pl, int k, int tid) {
     first = first_;
     left = o.k_rows - k;
-    const bf16* p = o.p + pl * o.plane + (ROWS ? (int64_t)first * o.ld + k : (int64_t)k * o.ld + first);
+    const E* p = static_cast<const E*>(o.p) + pl * o.plane + (ROWS ? (int64_t)first * o.ld + k : (int64_t)k * o.ld + first);
     base = (uint64_t)(uintptr_t)p;
     base = u64_from_halves(__builtin_amdgcn_readfirstlane((uint32_t)base),
                            __builtin_amdgcn_readfirstlane((uint32_t)(base >> 32)));
@@ -111,7 +135,7 @@ struct HeadTile {
   }
   __device__ __forceinline__ void next(const HeadOperand& o, int tid) {
     left -= kStep;
-    base += ROWS ? (uint64_t)(kStep * 2) : (uint64_t)o.ld * (kStep * 2);
+    base += ROWS ? 128 : (uint64_t)o.ld * 128;
     if (!ROWS && left < kStep) place(o, tid);
   }
   // Request J of a stage; lds: the wave's place in it.
@@ -121,15 +145,17 @@ struct HeadTile {
                  "s"(base)
                  : "memory", "m0");
   }
-  // Fragments of a wave: of the 32-row tile i from row w0 on (a multiple of 32, of 128
-  // where there are several and not ROWS), row m (PERM: perm32(m)), contraction
-  // elements 16 s + 8 h .. + 7.  `at` is the lane's byte address in LDS (stages lie on
+  // Fragments of a wave: of the 32-row tile i from row w0 on (a multiple of 32, of 32 MT
+  // where there are MT and not ROWS), row m (PERM: perm32(m)), 16 bytes of the contraction
+  // from chunk 2 s + h of the step on.  `at` is the lane's byte address in LDS (stages lie on
   // 16 KB) for i = s = 0; i and s enter by addition, or by exclusive or where the swizzle has their bits.
   template <bool PERM>
   static __device__ __forceinline__ uint32_t lane_at(int w0, int lane) {
-    if (ROWS) {
-      const int r = PERM ? perm32(lane & 31) : lane & 31;
-      return (uint32_t)((w0 + r) * kStep * 2 + (((lane >> 5) ^ key(r)) << 4));
+    const int m = PERM ? perm32(lane & 31) : lane & 31, h = lane >> 5;
+    if (ROWS) return (uint32_t)((w0 + m) * 128 + ((h ^ key(m)) << 4));
+    if (kWide) {
+      const int col = w0 + m;
+      return (uint32_t)(4 * h * T * 4 + (((col >> 2) ^ key(4 * h)) << 4) + (col & 3) * 4);
     }
     const int g = lane >> 4, r = 8 * (g >> 1) + ((lane >> 2) & 3);
     int q = lane & 3;
@@ -137,10 +163,15 @@ struct HeadTile {
     const int col = w0 + 16 * (g & 1) + 4 * q;
     return (uint32_t)(r * T * 2 + (((col >> 3) ^ key(r)) << 4) + (col & 7) * 2);
   }
-  static __device__ __forceinline__ bf16x8 frag(uint32_t at, int i, int s) {
+  static __device__ __forceinline__ Frag frag(uint32_t at, int i, int s) {
 #define NSA_LDS(type, a) ((__attribute__((address_space(3))) type*)(uintptr_t)(a))
     if constexpr (ROWS) {
-      return *NSA_LDS(bf16x8, (at ^ (32 * s)) + 32 * i * kStep * 2);
+      return *NSA_LDS(Frag, (at ^ (32 * s)) + 32 * i * 128);
+    } else if constexpr (kWide) {
+      Frag f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] = *NSA_LDS(float, (at ^ (128 * i)) + (8 * s + j) * T * 4);
+      return f;
     } else {
       typedef short s16x8 __attribute__((ext_vector_type(8)));
       const uint32_t a0 = at ^ (64 * i), a1 = a0 ^ 16;   // (rows r + 4: another key by 1)
@@ -154,9 +185,10 @@ struct HeadTile {
 };
 
 // Tile shape: TM x TN of the result over WM x WN waves, NS stages, kPerCu workgroups a CU.
-template <int TM_, int TN_, int WM_, int WN_, int NS_, int KSTEP_, int PER_CU_>
+template <int TM_, int TN_, int WM_, int WN_, int NS_, int PER_CU_, typename E_ = bf16>
 struct HeadShape {
-  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, NS = NS_, kStep = KSTEP_, kPerCu = PER_CU_;
+  typedef E_ E;
+  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, NS = NS_, kStep = 128 / (int)sizeof(E), kPerCu = PER_CU_;
   static constexpr int kThreads = WM * WN * 64, kPerSimd = kPerCu * WM * WN / 4;   // waves a SIMD
   static constexpr int MT = TM / WM / 32, NT = TN / WN / 32;   // 32 x 32 tiles of a wave
   static_assert(WM * WN % 4 == 0 && MT >= 1 && NT >= 1 && NS >= 2, "whole waves a SIMD");
@@ -194,12 +226,14 @@ __device__ __forceinline__ void head_range(F&& f) {
 template <class S, bool AROWS, bool BROWS, typename Span, typename Done>
 __device__ __forceinline__ void head_product(const HeadProduct& pr, int spans, int total, Span span, Done done) {
   constexpr int kStep = S::kStep;
-  using TA = HeadTile<S::TM, kStep, S::kThreads, AROWS>;
-  using TB = HeadTile<S::TN, kStep, S::kThreads, BROWS>;
-  constexpr int kLoads = TA::kLoads + TB::kLoads, KS = kStep / 16, MT = S::MT, NT = S::NT;
+  typedef typename S::E E;
+  typedef HeadType<E> Type;
+  using TA = HeadTile<E, S::TM, S::kThreads, AROWS>;
+  using TB = HeadTile<E, S::TN, S::kThreads, BROWS>;
+  constexpr int kLoads = TA::kLoads + TB::kLoads, KS = 4, MT = S::MT, NT = S::NT;
   static_assert(KS % 2 == 0, "two sets of fragments in turn");
-  __shared__ __align__(16384) bf16 sa[S::NS][TA::kElems];
-  __shared__ __align__(16384) bf16 sb[S::NS][TB::kElems];
+  __shared__ __align__(16384) char sa[S::NS][TA::kBytes];
+  __shared__ __align__(16384) char sb[S::NS][TB::kBytes];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = (w % S::WM) * MT * 32, wn = (w / S::WM) * NT * 32;
@@ -228,8 +262,8 @@ __device__ __forceinline__ void head_product(const HeadProduct& pr, int spans, i
   start();
   auto request_next = [&]() {   // behind the requests of a stage
     rst = rst + 1 == S::NS ? 0 : rst + 1;
-    ra = at_a + 1024 * w + rst * TA::kElems * 2;
-    rb = at_b + 1024 * w + rst * TB::kElems * 2;
+    ra = at_a + 1024 * w + rst * TA::kBytes;
+    rb = at_b + 1024 * w + rst * TB::kBytes;
     if (++asked >= total) return;
     ++rq;
     if (rq == rs.q1) {
@@ -254,10 +288,10 @@ __device__ __forceinline__ void head_product(const HeadProduct& pr, int spans, i
         tb.template request<d - TA::kLoads>(rb);
     });
   };
-  bf16x8 fa[2][MT], fb[2][NT];
+  typename Type::Frag fa[2][MT], fb[2][NT];
   f32x16 acc[MT][NT];
   uint32_t sla = la, slb = lb;   // the stage being read
-  // Substep C's products, one a slot; behind them the fragments of substep R are read
+  // Substep C's products, one pair of fragments a slot; behind them the fragments of substep R are read
   // and the share of a stage's requests that slots S0 .. of kDmaSlots have is made.
   constexpr int kSlots = MT * NT, kReadSlots = kSlots > 4 ? kSlots * 3 / 4 : kSlots;
   constexpr int kDmaSlots = kSlots * (S::NS == 2 ? KS - 1 : KS);
@@ -265,7 +299,7 @@ __device__ __forceinline__ void head_product(const HeadProduct& pr, int spans, i
     constexpr int C = decltype(c_)::value, R = decltype(r_)::value, S0 = decltype(s0_)::value;
     head_range<0, kSlots>([&](auto n_) {
       constexpr int n = decltype(n_)::value, i = n / NT, j = n % NT;
-      acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[C & 1][i], fb[C & 1][j], acc[i][j], 0, 0, 0);
+      acc[i][j] = Type::product(fa[C & 1][i], fb[C & 1][j], acc[i][j]);
       if constexpr (n < kReadSlots) {
         constexpr int lo = (MT + NT) * n / kReadSlots, hi = (MT + NT) * (n + 1) / kReadSlots;
 #pragma unroll
@@ -327,8 +361,8 @@ __device__ __forceinline__ void head_product(const HeadProduct& pr, int spans, i
       request_next();
       arrive();
       st = st + 1 == S::NS ? 0 : st + 1;
-      sla = la + st * TA::kElems * 2;
-      slb = lb + st * TB::kElems * 2;
+      sla = la + st * TA::kBytes;
+      slb = lb + st * TB::kBytes;
       substep(std::integral_constant<int, KS - 1>{}, zero, zero);
     }
     done(cur, wm, wn, acc);
@@ -359,10 +393,15 @@ __device__ __forceinline__ int head_share(const HeadGrid& g, int part) {
   return (g.m_tiles - part + g.split - 1) / g.split;
 }
 
+__device__ __forceinline__ bool head_real(const int64_t* target, int64_t n, int V) {
+  return target != nullptr && target[n] >= 0 && target[n] < V;
+}
 struct HeadFwd {
   HeadProduct pr;    // a: weights, b: rows
   HeadGrid g;
   float2* part;      // [split][N]: maximum (log2 units) and sum of 2^(z - maximum)
+  const int64_t* target;   // or null
+  float* zt;         // [N]: the target's z, where there is one
   int N, V;
 };
 
@@ -376,6 +415,12 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_fwd(const Hea
   float m[S::NT], l[S::NT];
 #pragma unroll
   for (int j = 0; j < S::NT; ++j) m[j] = kMaskScore, l[j] = 0.0f;
+  int t[S::NT];   // the rows' targets
+#pragma unroll
+  for (int j = 0; j < S::NT; ++j) {
+    const int n = nt * S::TN + ((int)threadIdx.x >> 6) / S::WM * S::NT * 32 + 32 * j + (lane & 31);
+    t[j] = a.target != nullptr && n < a.N && head_real(a.target, n, a.V) ? (int)a.target[n] : -1;
+  }
   const int steps = head_steps<S>(a.pr), tiles = head_share(a.g, part);
   head_product<S, true, true>(
       a.pr, tiles, tiles * steps, [&](int i) { return HeadSpan{part + i * a.g.split, nt, 0, steps}; },
@@ -410,6 +455,17 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_fwd(const Hea
               m[j] = mn;
             }
             l[j] += s;
+            // the target's own z: logp is its difference from the sum of the same numbers
+            const int at = t[j] - (a.V - left);
+            const bool mine = t[j] >= 0 && at >= 0 && at < 32 * S::MT && (at & 8) == 0;
+            if (__any(mine)) {
+              float zt = 0.0f;
+#pragma unroll
+              for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) zt = at == 32 * i + acc_elem(0, r) ? acc[i][j][r] : zt;
+              if (mine) a.zt[nt * S::TN + wn + 32 * j + (lane & 31)] = zt;
+            }
             __builtin_amdgcn_sched_barrier(0);   // (one row's values in registers at a time)
           }
         };
@@ -440,21 +496,19 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_fwd(const Hea
   }
 }
 
-// Joins the shares and takes the target's own product: a wave a row.
+// Joins the shares of a row: a wave a row.
 struct HeadJoin {
   const float2* part;
-  const void *x, *w;
+  const float* zt;
   const int64_t* target;   // or null
   float *logp, *lse;
   int64_t N;
-  int split, V, D;
-  bool x_bf16, w_bf16, w_round;   // w_round: float32 weights taken as bf16
+  int split, V;
 };
 __global__ __launch_bounds__(256) void k_head_join(const HeadJoin a) {
   const int lane = threadIdx.x & 63;
   const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (n >= a.N) return;
-  const int64_t t = a.target != nullptr ? a.target[n] : -1;
   float m = kMaskScore, l = 0.0f;
 #pragma unroll 4
   for (int s = lane; s < a.split; s += kWave) {
@@ -463,26 +517,13 @@ __global__ __launch_bounds__(256) void k_head_join(const HeadJoin a) {
     l = l * fast_exp2(m - mx) + p.y * fast_exp2(p.x - mx);
     m = mx;
   }
-  const bool real = t >= 0 && t < a.V;
-  float dot = 0.0f;
-  if (real) {
-#pragma unroll 2
-    for (int c = 8 * lane; c < a.D; c += 8 * kWave) {
-      float u[8], v[8];
-      load_run8_of(a.x, a.x_bf16, n * a.D + c, a.D - c, u);
-      load_run8_of(a.w, a.w_bf16, t * a.D + c, a.D - c, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) dot += u[j] * (a.w_round ? (float)(bf16)v[j] : v[j]);
-    }
-    dot = wave_sum(dot);
-  }
   const float mx = wave_max(m);
   const bool nan = l != l;   // (a maximum passes NaN over: its sum shows it)
   l = wave_sum(l * fast_exp2(m - mx));
   if (__any(nan)) l = __builtin_nanf("");
   const float lse = (mx + __log2f(l)) * kLn2;
   if (lane == 0) {
-    if (a.target != nullptr) a.logp[n] = real ? dot - lse : 0.0f;
+    if (a.target != nullptr) a.logp[n] = head_real(a.target, n, a.V) ? a.zt[n] - lse : 0.0f;
     a.lse[n] = lse;
   }
 }
@@ -493,15 +534,12 @@ struct HeadDz {
   HeadGrid g;
   const float *lse, *dlogp, *dlse;   // dlogp, dlse: or null
   const int64_t* target;             // or null
-  bf16* dz;                          // [planes][N rounded up to 64][ld], zeros past N and past the vocabulary
+  void* dz;                          // [planes][N rounded up to 64][ld], zeros past N and past the vocabulary
   int64_t ld, plane;
   int N, V, v0;                      // the piece starts at token v0 (V: of the whole vocabulary)
   int vocab;                         // ... and has so many
   int rows;                          // N rounded up to 64
 };
-__device__ __forceinline__ bool head_real(const int64_t* target, int64_t n, int V) {
-  return target != nullptr && target[n] >= 0 && target[n] < V;
-}
 // The bf16 plane of v that comes next; v becomes what it leaves.  neg: a sign bit to flip.
 __device__ __forceinline__ u32x4 next_plane(float (&v)[8], uint32_t neg) {
   bf16x8 o;
@@ -532,9 +570,11 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_dz(const Head
       neg[j] = __float_as_uint(co) & 0x80000000u;
     }
   }
-  // Results turn in LDS, 32 tokens x 64 of the vocabulary a wave at a time, so that eight
+  // Results turn in LDS, 32 tokens x 128 bytes of the vocabulary a wave at a time, so that eight
   // lanes store 128 bytes in a row: a store of 32 rows takes the caches four times as many requests.
-  static_assert(S::MT % 2 == 0, "64 of the vocabulary");
+  typedef typename S::E E;
+  constexpr int kC = 16 / (int)sizeof(E), kI = 4 / (int)sizeof(E);   // elements of 16 bytes; 32-row tiles of 128
+  static_assert(S::MT % kI == 0 && (kI == 2 || PLANES == 1), "128 bytes of the vocabulary");
   __shared__ __align__(16) char turn[S::kThreads / 64 * 4096];
   const int steps = head_steps<S>(a.pr), tiles = head_share(a.g, part);
   head_product<S, true, true>(
@@ -551,12 +591,12 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_dz(const Head
         for (int j = 0; j < S::NT; ++j) {
           const bool real = n0 + 32 * j + (lane & 31) < a.N;
 #pragma unroll
-          for (int i = 0; i < S::MT; i += 2) {
-            float d[4][8];
+          for (int i = 0; i < S::MT; i += kI) {
+            float d[2 * kI][8];
 #pragma unroll
             for (int q = 0; q < PLANES; ++q) {
 #pragma unroll
-              for (int c = 0; c < 4; ++c) {   // 8 elements from v0 + 32 i + 16 c + 8 h on
+              for (int c = 0; c < 2 * kI; ++c) {   // 8 elements from v0 + 32 i + 16 c + 8 h on
                 if (q == 0) {
 #pragma unroll
                   for (int r = 0; r < 8; ++r)
@@ -567,7 +607,16 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_dz(const Head
                       if (v0 + 32 * i + 16 * c + 8 * h + r >= a.vocab || !real) d[c][r] = 0.0f;
                   }
                 }
-                *reinterpret_cast<u32x4*>(put + (((2 * c + h) ^ put_key) << 4)) = next_plane(d[c], neg[j]);
+                if constexpr (kC == 8) {
+                  *reinterpret_cast<u32x4*>(put + (((2 * c + h) ^ put_key) << 4)) = next_plane(d[c], neg[j]);
+                } else {
+#pragma unroll
+                  for (int x = 0; x < 2; ++x) {
+                    const f32x4 o = {d[c][4 * x], d[c][4 * x + 1], d[c][4 * x + 2], d[c][4 * x + 3]};
+                    *reinterpret_cast<u32x4*>(put + (((4 * c + 2 * h + x) ^ put_key) << 4)) =
+                        __builtin_bit_cast(u32x4, o) ^ neg[j];
+                  }
+                }
                 __builtin_amdgcn_sched_barrier(0);
               }
               // (a wave's LDS requests are served in order: the compiler alone has to keep it)
@@ -578,7 +627,8 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_dz(const Head
                 const int r = 8 * t + (lane >> 3), n = n0 + 32 * j + r;
                 const u32x4 o = *reinterpret_cast<const u32x4*>(mine + r * 128 + (((lane & 7) ^ ((r >> 1) & 7)) << 4));
                 if (n < a.rows)
-                  *reinterpret_cast<u32x4*>(a.dz + q * a.plane + (int64_t)n * a.ld + v0 + 32 * i + 8 * (lane & 7)) = o;
+                  *reinterpret_cast<u32x4*>(static_cast<E*>(a.dz) + q * a.plane + (int64_t)n * a.ld + v0 + 32 * i +
+                                            kC * (lane & 7)) = o;
               }
               asm volatile("" ::: "memory");
               __builtin_amdgcn_wave_barrier();
@@ -589,7 +639,7 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_dz(const Head
 }
 
 // The target's own element, where the piece has it: a p_t + b.
-template <int PLANES>
+template <typename E, int PLANES>
 __global__ __launch_bounds__(256) void k_head_target(const HeadDz a, const float* logp) {
   const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (n >= a.N || a.dlogp == nullptr || !head_real(a.target, n, a.V)) return;
@@ -598,10 +648,10 @@ __global__ __launch_bounds__(256) void k_head_target(const HeadDz a, const float
   const float b = a.dlogp[n], dl = a.dlse != nullptr ? a.dlse[n] : 0.0f, lp = logp[n];
   // (dlse - b) p + b with 1 - p from expm1: p near 1 leaves no digits in 1 - p otherwise
   float d = dl * expf(lp) - b * expm1f(lp);
-  bf16* p = a.dz + n * a.ld + v;
+  E* p = static_cast<E*>(a.dz) + n * a.ld + v;
 #pragma unroll
   for (int q = 0; q < PLANES; ++q) {
-    const bf16 o = (bf16)d;
+    const E o = (E)d;
     p[q * a.plane] = o;
     d -= (float)o;
   }
@@ -738,9 +788,9 @@ __global__ __launch_bounds__(256) void k_head_join_tiles(const HeadGrad a, int f
   }
 }
 
-// Rows as bf16 planes with a pitch of ld: [planes][rows][ld], zeros past a row.
-template <int PLANES>
-__global__ __launch_bounds__(256) void k_head_pack(const void* x, bool x_bf16, bf16* out, int64_t rows, int D, int ld) {
+// Rows as bf16 planes or float32 with a pitch of ld: [planes][rows][ld], zeros past a row.
+template <typename E, int PLANES>
+__global__ __launch_bounds__(256) void k_head_pack(const void* x, bool x_bf16, E* out, int64_t rows, int D, int ld) {
   const int runs = ld / 8;
   const int64_t total = rows * runs, plane = rows * ld;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
@@ -748,53 +798,30 @@ __global__ __launch_bounds__(256) void k_head_pack(const void* x, bool x_bf16, b
     const int c = (int)(i % runs) * 8;
     float v[8];
     load_run8_of(x, x_bf16, r * D + c, D - c, v);
+    if constexpr (sizeof(E) == 4) {
+      store_run8(out + r * ld + c, v);
+    } else {
 #pragma unroll
-    for (int q = 0; q < PLANES; ++q) *reinterpret_cast<u32x4*>(out + q * plane + r * ld + c) = next_plane(v, 0);
+      for (int q = 0; q < PLANES; ++q) *reinterpret_cast<u32x4*>(out + q * plane + r * ld + c) = next_plane(v, 0);
+    }
   }
 }
 
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
-using HeadBig = HeadShape<256, 256, 2, 4, 2, 64, 1>;
-using HeadMid = HeadShape<128, 128, 2, 2, 2, 64, 2>;
-using HeadFew = HeadShape<128, 32, 4, 1, 4, 64, 1>;
-using HeadFew64 = HeadShape<128, 64, 2, 2, 3, 64, 2>;
-using HeadFew128 = HeadShape<128, 128, 2, 2, 4, 64, 1>;
+template <typename E> using HeadBig = HeadShape<256, 256, 2, 4, 2, 1, E>;
+template <typename E> using HeadMid = HeadShape<128, 128, 2, 2, 2, 2, E>;
+template <typename E> using HeadFew = HeadShape<128, 32, 4, 1, 4, 1, E>;
+template <typename E> using HeadFew64 = HeadShape<128, 64, 2, 2, 3, 2, E>;
+using HeadFewBack = HeadShape<128, 64, 2, 2, 3, 1, float>;   // (the backward's, up to 64 rows)
+template <typename E> using HeadFew128 = HeadShape<128, 128, 2, 2, 4, 1, E>;
 
 static bool head_type(int dtype) { return dtype == NSA_F32 || dtype == NSA_BF16; }
 static bool head_shape_ok(int64_t N, int V, int D) {
   return N >= 0 && N <= kHeadRows && V >= 1 && V <= kHeadVocab && D >= 1 && D <= kHeadWide;
 }
 static size_t up16(size_t n) { return (n + 255) / 256 * 256; }
-
-// How the operands lie: as given, or packed (planes, padded rows).
-struct HeadLayout {
-  bool pack_x, pack_w;
-  int px, pw, ld;               // planes; pitch of a packed row
-  size_t x_bytes, w_bytes;      // of the packed copies
-};
-static HeadLayout head_layout(int64_t N, int V, int D, const void* x, const void* w, int x_dtype, int w_dtype) {
-  HeadLayout l;
-  const bool wide = x_dtype == NSA_F32;
-  l.px = wide ? 3 : 1;
-  l.pw = wide && w_dtype == NSA_F32 ? 3 : 1;
-  l.ld = (D + 63) / 64 * 64;
-  // rows are requested in whole stages, aligned pieces of 16 bytes
-  l.pack_x = wide || D % 64 != 0 || reinterpret_cast<uintptr_t>(x) % 16 != 0;
-  l.pack_w = w_dtype == NSA_F32 || D % 64 != 0 || reinterpret_cast<uintptr_t>(w) % 16 != 0;
-  l.x_bytes = l.pack_x ? up16((size_t)l.px * N * l.ld * 2) : 0;
-  l.w_bytes = l.pack_w ? up16((size_t)l.pw * V * l.ld * 2) : 0;
-  return l;
-}
-static void head_pack(const void* x, int dtype, void* out, int64_t rows, int D, int ld, int planes, hipStream_t s) {
-  const int64_t blocks = (rows * (ld / 8) + 255) / 256;
-  const unsigned grid = (unsigned)(blocks < 65536 ? blocks : 65536);
-  if (planes == 3)
-    k_head_pack<3><<<grid, 256, 0, s>>>(x, dtype == NSA_BF16, static_cast<bf16*>(out), rows, D, ld);
-  else
-    k_head_pack<1><<<grid, 256, 0, s>>>(x, dtype == NSA_BF16, static_cast<bf16*>(out), rows, D, ld);
-}
 
 // Tile of the product over the vocabulary: 256 x 256 where that gives every compute unit
 // a tile, else 128 x 128.  The forward of up to 128 rows, one tile across, waits for W: it
@@ -807,6 +834,51 @@ static int head_kind(int64_t N, int V, int cu) {
 static int head_fwd_kind(int64_t N, int V, int cu) {
   return N <= 32 ? kFew : N <= 64 ? kFew64 : N <= 128 ? kFew128 : head_kind(N, V, cu);
 }
+// Whether float32 rows and weights go through the float32 instructions rather than as
+// planes.  Planes take six products of bf16 at 870 to 1150 TFLOP/s together and a copy of
+// W of 1.5 times its size, the float32 instructions up to 140 TFLOP/s and no copy: they win
+// where rows are few and the tiles of 128 x 128 half fill the chip (W 32000 x 768, 64, 512 and
+// 2048 rows: forward 35, 201, 720 us, planes 92, 217, 528; 128, 256 and 512 rows: backward
+// 202, 344, 607, planes 258, 323, 571).
+static bool head_native(int64_t N, int V, int most, int cu) {
+  return N <= 64 || (N <= most && (N + 127) / 128 * ((V + 127) / 128) * 2 >= cu);
+}
+constexpr int kNativeFwd = 512, kNativeBwd = 256;
+
+// How the operands lie: as given, or packed (planes, padded rows).
+struct HeadLayout {
+  bool native, pack_x, pack_w;  // native: products of float32
+  int px, pw, ld;               // planes; pitch of a packed row
+  size_t x_bytes, w_bytes;      // of the packed copies
+};
+static HeadLayout head_layout(int64_t N, int V, int D, const void* x, const void* w, int x_dtype, int w_dtype, int native, int cu) {
+  HeadLayout l;
+  const bool wide = x_dtype == NSA_F32, both = wide && w_dtype == NSA_F32;
+  l.native = both && head_native(N, V, native, cu);
+  l.px = wide && !l.native ? 3 : 1;
+  l.pw = both && !l.native ? 3 : 1;
+  l.ld = (D + 63) / 64 * 64;
+  // rows are requested in whole stages, aligned pieces of 16 bytes
+  const int step = l.native ? 32 : 64, size = l.native ? 4 : 2;
+  l.pack_x = l.px == 3 || D % step != 0 || reinterpret_cast<uintptr_t>(x) % 16 != 0;
+  l.pack_w = (w_dtype == NSA_F32 && !l.native) || D % step != 0 || reinterpret_cast<uintptr_t>(w) % 16 != 0;
+  l.x_bytes = l.pack_x ? up16((size_t)l.px * N * l.ld * size) : 0;
+  l.w_bytes = l.pack_w ? up16((size_t)l.pw * V * l.ld * size) : 0;
+  return l;
+}
+static void head_pack(const void* x, int dtype, void* out, int64_t rows, int D, int ld, int planes, bool native,
+                      hipStream_t s) {
+  const int64_t blocks = (rows * (ld / 8) + 255) / 256;
+  const unsigned grid = (unsigned)(blocks < 65536 ? blocks : 65536);
+  const bool half = dtype == NSA_BF16;
+  if (native)
+    k_head_pack<float, 1><<<grid, 256, 0, s>>>(x, half, static_cast<float*>(out), rows, D, ld);
+  else if (planes == 3)
+    k_head_pack<bf16, 3><<<grid, 256, 0, s>>>(x, half, static_cast<bf16*>(out), rows, D, ld);
+  else
+    k_head_pack<bf16, 1><<<grid, 256, 0, s>>>(x, half, static_cast<bf16*>(out), rows, D, ld);
+}
+
 template <class S>
 static HeadGrid head_grid(int64_t N, int vocab, int cu) {
   HeadGrid g;
@@ -825,19 +897,26 @@ static HeadGrid head_grid(int64_t N, int vocab, int cu) {
 static unsigned head_blocks(const HeadGrid& g) {
   return (unsigned)((g.n_tiles >= 8 ? (g.n_tiles + 7) / 8 * 8 : g.n_tiles) * (int64_t)g.split);
 }
+// f with the shape of the forward's tiles
 template <typename F>
-static auto head_as(int kind, F f) {
-  if (kind == kFew) return f(HeadFew{});
-  if (kind == kFew64) return f(HeadFew64{});
-  if (kind == kFew128) return f(HeadFew128{});
-  if (kind == kMid) return f(HeadMid{});
-  return f(HeadBig{});
+static auto head_as(int kind, bool native, F f) {
+  if (native)
+    return kind == kFew     ? f(HeadFew<float>{})
+           : kind == kFew64 ? f(HeadFew64<float>{})
+           : kind == kFew128 ? f(HeadFew128<float>{})
+                             : f(HeadMid<float>{});
+  return kind == kFew     ? f(HeadFew<bf16>{})
+         : kind == kFew64 ? f(HeadFew64<bf16>{})
+         : kind == kFew128 ? f(HeadFew128<bf16>{})
+         : kind == kMid    ? f(HeadMid<bf16>{})
+                           : f(HeadBig<bf16>{});
 }
 
 // The gradients' products: tiles of 256 x 256 or, where those are few, 128 x 128 with
 // two workgroups a compute unit.  The last round's tiles are cut where that saves more
 // than a part costs.  Measured: a step (64 elements) of a 256 x 256 tile 2.1 us, of two
-// 128 x 128 tiles side by side 1.2; writing and adding their parts 26 and 13.
+// 128 x 128 tiles side by side 1.2; writing and adding their parts 26 and 13.  Of float32 (32
+// elements) two 128 x 128 tiles 3.6, one of 64 rows 1.0, its parts 4.
 struct HeadCut {
   bool big;
   int groups, whole, cuts;
@@ -845,7 +924,9 @@ struct HeadCut {
 };
 template <class S>
 static double head_cut_as(HeadCut& c, int64_t rows, int D, int K, int pairs, int cu) {
-  const double step = S::TM == 256 ? 2.1 : 1.2, part = S::TM == 256 ? 26.0 : 13.0;
+  constexpr bool kWide = sizeof(typename S::E) == 4;
+  const double step = kWide ? S::TN == 64 ? 1.0 : 3.6 : S::TM == 256 ? 2.1 : 1.2;
+  const double part = S::TM == 256 ? 26.0 : S::TN == 64 ? 4.0 : 13.0;
   const int64_t m = (D + S::TM - 1) / S::TM, n = (rows + S::TN - 1) / S::TN, tiles = m * n;
   const int64_t steps = (int64_t)pairs * ((K + S::kStep - 1) / S::kStep), at_once = (int64_t)cu * S::kPerCu;
   c.big = S::TM == 256;
@@ -868,10 +949,18 @@ static double head_cut_as(HeadCut& c, int64_t rows, int D, int K, int pairs, int
   c.bytes = parts * S::TM * S::TN * 4;
   return best + (double)(c.whole / at_once) * step * steps;
 }
-static HeadCut head_cut(int64_t rows, int D, int K, int pairs, int cu) {
+static bool head_few_back(int64_t N, bool native) { return native && N <= 64; }   // dz and dx
+static HeadCut head_cut(int64_t rows, int D, int K, int pairs, bool native, bool few, int cu) {
   HeadCut big, mid;
-  const double tb = head_cut_as<HeadBig>(big, rows, D, K, pairs, cu);
-  const double tm = head_cut_as<HeadMid>(mid, rows, D, K, pairs, cu);
+  if (native) {
+    if (few)
+      head_cut_as<HeadFewBack>(mid, rows, D, K, pairs, cu);
+    else
+      head_cut_as<HeadMid<float>>(mid, rows, D, K, pairs, cu);
+    return mid;
+  }
+  const double tb = head_cut_as<HeadBig<bf16>>(big, rows, D, K, pairs, cu);
+  const double tm = head_cut_as<HeadMid<bf16>>(mid, rows, D, K, pairs, cu);
   return tb <= tm ? big : mid;
 }
 static int head_pair_count(int pa, int pb) { return pb == 1 ? 1 : pa == 1 ? 3 : 6; }
@@ -887,12 +976,17 @@ static void head_grad_as(HeadGrad g, const HeadCut& c, hipStream_t s) {
   if (first < tiles) k_head_join_tiles<S><<<dim3((unsigned)(tiles - first), 8), 256, 0, s>>>(g, first);
 }
 template <bool BROWS>
-static void head_grad(const HeadGrad& g, int cu, hipStream_t s) {
-  const HeadCut c = head_cut(g.N, g.D, g.pr.K, head_pair_count(g.pr.pa, g.pr.pb), cu);
-  if (c.big)
-    head_grad_as<HeadBig, BROWS>(g, c, s);
+static void head_grad(const HeadGrad& g, bool native, int cu, hipStream_t s) {
+  const bool few = BROWS && head_few_back(g.N, native);
+  const HeadCut c = head_cut(g.N, g.D, g.pr.K, head_pair_count(g.pr.pa, g.pr.pb), native, few, cu);
+  if constexpr (BROWS)
+    if (few) return head_grad_as<HeadFewBack, true>(g, c, s);
+  if (native)
+    head_grad_as<HeadMid<float>, BROWS>(g, c, s);
+  else if (c.big)
+    head_grad_as<HeadBig<bf16>, BROWS>(g, c, s);
   else
-    head_grad_as<HeadMid, BROWS>(g, c, s);
+    head_grad_as<HeadMid<bf16>, BROWS>(g, c, s);
 }
 
 // The backward's pieces of the vocabulary and its buffers
@@ -900,21 +994,23 @@ struct HeadPlan {
   int piece;            // tokens of a piece, a multiple of 256
   size_t dz, acc, part; // bytes
 };
-static HeadPlan head_plan(int64_t N, int V, int D, int planes, int pw, bool x_bf16, int cu) {
+static HeadPlan head_plan(int64_t N, int V, int D, const HeadLayout& l, bool x_bf16, int cu) {
   HeadPlan p;
+  const int planes = l.px, pw = l.pw;
+  const size_t size = l.native ? 4 : 2;
   const int64_t all = ((int64_t)V + 255) / 256 * 256;
-  int64_t fit = (int64_t)(kHeadPiece / ((size_t)((N + 63) / 64 * 64) * 2 * planes)) / 256 * 256;
+  int64_t fit = (int64_t)(kHeadPiece / ((size_t)((N + 63) / 64 * 64) * size * planes)) / 256 * 256;
   fit = fit < 256 ? 256 : fit < kHeadPieceMost ? fit : kHeadPieceMost;
   const int64_t pieces = (all + fit - 1) / fit;
   p.piece = (int)(((all + pieces - 1) / pieces + 255) / 256 * 256);
-  p.dz = up16((size_t)planes * ((N + 63) / 64 * 64) * p.piece * 2);
+  p.dz = up16((size_t)planes * ((N + 63) / 64 * 64) * p.piece * size);
   p.acc = all > p.piece && x_bf16 ? up16((size_t)N * D * 4) : 0;
   // the parts of dx and dW of a whole piece and of the last one
   const int last = (int)(V - (int64_t)(V - 1) / p.piece * p.piece);
   int64_t parts = 0;
   for (int vocab : {p.piece < V ? p.piece : V, last}) {
-    const int64_t dx = head_cut(N, D, vocab, head_pair_count(pw, planes), cu).bytes;
-    const int64_t dw = head_cut(vocab, D, (int)N, head_pair_count(planes, planes), cu).bytes;
+    const int64_t dx = head_cut(N, D, vocab, head_pair_count(pw, planes), l.native, head_few_back(N, l.native), cu).bytes;
+    const int64_t dw = head_cut(vocab, D, (int)N, head_pair_count(planes, planes), l.native, false, cu).bytes;
     parts = dx > parts ? dx : parts;
     parts = dw > parts ? dw : parts;
   }
@@ -931,10 +1027,10 @@ extern "C" size_t nsa_head_fwd_workspace(int64_t N, int V, int D, int x_dtype, i
   if (!head_shape_ok(N, V, D) || !head_type(x_dtype) || !head_type(w_dtype)) return 0;
   if (N == 0) return 16;
   const void* at = reinterpret_cast<const void*>(aligned ? 16 : 1);
-  const HeadLayout l = head_layout(N, V, D, at, at, x_dtype, w_dtype);
   const int cu = device_cu_count(static_cast<hipStream_t>(stream));
-  const int split = head_as(head_fwd_kind(N, V, cu), [&](auto s) { return head_grid<decltype(s)>(N, V, cu).split; });
-  return l.x_bytes + l.w_bytes + (size_t)split * N * sizeof(float2);
+  const HeadLayout l = head_layout(N, V, D, at, at, x_dtype, w_dtype, kNativeFwd, cu);
+  const int split = head_as(head_fwd_kind(N, V, cu), l.native, [&](auto s) { return head_grid<decltype(s)>(N, V, cu).split; });
+  return l.x_bytes + l.w_bytes + up16((size_t)split * N * sizeof(float2)) + (size_t)N * 4;
 }
 
 extern "C" int nsa_head_fwd(const void* x, const void* w, const int64_t* target, float* logp, float* lse,
@@ -947,32 +1043,32 @@ extern "C" int nsa_head_fwd(const void* x, const void* w, const int64_t* target,
   NSA_CHECK(x != nullptr && w != nullptr && lse != nullptr && (target == nullptr) == (logp == nullptr), NSA_ERR_ARG);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int cu = device_cu_count(s);
-  const HeadLayout l = head_layout(N, V, D, x, w, x_dtype, w_dtype);
-  return head_as(head_fwd_kind(N, V, cu), [&](auto sh) -> int {
+  const HeadLayout l = head_layout(N, V, D, x, w, x_dtype, w_dtype, kNativeFwd, cu);
+  return head_as(head_fwd_kind(N, V, cu), l.native, [&](auto sh) -> int {
     using S = decltype(sh);
     const HeadGrid g = head_grid<S>(N, V, cu);
     NSA_CHECK(workspace != nullptr &&
-                  workspace_bytes >= l.x_bytes + l.w_bytes + (size_t)g.split * N * sizeof(float2),
+                  workspace_bytes >= l.x_bytes + l.w_bytes + up16((size_t)g.split * N * sizeof(float2)) + (size_t)N * 4,
               NSA_ERR_WORKSPACE);
     char* ws = static_cast<char*>(workspace);
-    bf16* xp = reinterpret_cast<bf16*>(ws);
-    bf16* wp = reinterpret_cast<bf16*>(ws + l.x_bytes);
+    char *const xp = ws, *const wp = ws + l.x_bytes;
     float2* part = reinterpret_cast<float2*>(ws + l.x_bytes + l.w_bytes);
-    if (l.pack_x) head_pack(x, x_dtype, xp, N, D, l.ld, l.px, s);
-    if (l.pack_w) head_pack(w, w_dtype, wp, V, D, l.ld, l.pw, s);
+    if (l.pack_x) head_pack(x, x_dtype, xp, N, D, l.ld, l.px, l.native, s);
+    if (l.pack_w) head_pack(w, w_dtype, wp, V, D, l.ld, l.pw, l.native, s);
     HeadFwd a;
-    a.pr.a = {l.pack_w ? wp : static_cast<const bf16*>(w), (int64_t)V * l.ld, l.pack_w ? l.ld : D, V, 0};
-    a.pr.b = {l.pack_x ? xp : static_cast<const bf16*>(x), N * l.ld, l.pack_x ? l.ld : D, (int)N, 0};
+    a.pr.a = {l.pack_w ? wp : w, (int64_t)V * l.ld, l.pack_w ? l.ld : D, V, 0};
+    a.pr.b = {l.pack_x ? xp : x, N * l.ld, l.pack_x ? l.ld : D, (int)N, 0};
     a.pr.K = D;
     a.pr.pa = l.pw;
     a.pr.pb = l.px;
     a.g = g;
     a.part = part;
+    a.target = target;
+    a.zt = reinterpret_cast<float*>(ws + l.x_bytes + l.w_bytes + up16((size_t)g.split * N * sizeof(float2)));
     a.N = (int)N;
     a.V = V;
     k_head_fwd<S><<<head_blocks(g), S::kThreads, 0, s>>>(a);
-    const HeadJoin j{part, x, w, target, logp, lse, N, g.split, V, D, x_dtype == NSA_BF16, w_dtype == NSA_BF16,
-                     x_dtype == NSA_BF16 && w_dtype == NSA_F32};
+    const HeadJoin j{part, a.zt, target, logp, lse, N, g.split, V};
     k_head_join<<<(unsigned)((N + 3) / 4), 256, 0, s>>>(j);
     return nsa_launch_status();
   });
@@ -983,8 +1079,9 @@ extern "C" size_t nsa_head_bwd_workspace(int64_t N, int V, int D, int x_dtype, i
   if (!head_shape_ok(N, V, D) || !head_type(x_dtype) || !head_type(w_dtype)) return 0;
   if (N == 0) return 16;
   const void* at = reinterpret_cast<const void*>(aligned ? 16 : 1);
-  const HeadLayout l = head_layout(N, V, D, at, at, x_dtype, w_dtype);
-  const HeadPlan p = head_plan(N, V, D, l.px, l.pw, x_dtype == NSA_BF16, device_cu_count(static_cast<hipStream_t>(stream)));
+  const int cu = device_cu_count(static_cast<hipStream_t>(stream));
+  const HeadLayout l = head_layout(N, V, D, at, at, x_dtype, w_dtype, kNativeBwd, cu);
+  const HeadPlan p = head_plan(N, V, D, l, x_dtype == NSA_BF16, cu);
   return l.x_bytes + l.w_bytes + p.dz + p.acc + p.part;
 }
 
@@ -998,30 +1095,30 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
   NSA_CHECK(dlogp == nullptr || (target != nullptr && logp != nullptr), NSA_ERR_ARG);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int cu = device_cu_count(s);
-  const HeadLayout l = head_layout(N, V, D, x, w, x_dtype, w_dtype);
-  const HeadPlan p = head_plan(N, V, D, l.px, l.pw, x_dtype == NSA_BF16, cu);
+  const HeadLayout l = head_layout(N, V, D, x, w, x_dtype, w_dtype, kNativeBwd, cu);
+  const HeadPlan p = head_plan(N, V, D, l, x_dtype == NSA_BF16, cu);
   NSA_CHECK(workspace != nullptr && workspace_bytes >= l.x_bytes + l.w_bytes + p.dz + p.acc + p.part,
             NSA_ERR_WORKSPACE);
   char* ws = static_cast<char*>(workspace);
-  bf16* xp = reinterpret_cast<bf16*>(ws);
+  char* const xp = ws;
   ws += l.x_bytes;
-  bf16* wp = reinterpret_cast<bf16*>(ws);
+  char* const wp = ws;
   ws += l.w_bytes;
-  bf16* dz = reinterpret_cast<bf16*>(ws);
+  char* const dz = ws;
   ws += p.dz;
   float* acc = reinterpret_cast<float*>(ws);
   ws += p.acc;
   float* part = reinterpret_cast<float*>(ws);
-  if (l.pack_x) head_pack(x, x_dtype, xp, N, D, l.ld, l.px, s);
-  if (l.pack_w) head_pack(w, w_dtype, wp, V, D, l.ld, l.pw, s);
+  if (l.pack_x) head_pack(x, x_dtype, xp, N, D, l.ld, l.px, l.native, s);
+  if (l.pack_w) head_pack(w, w_dtype, wp, V, D, l.ld, l.pw, l.native, s);
   const int ldx = l.pack_x ? l.ld : D, ldw = l.pack_w ? l.ld : D;
-  const bf16* X = l.pack_x ? xp : static_cast<const bf16*>(x);
-  const bf16* W = l.pack_w ? wp : static_cast<const bf16*>(w);
+  const void* X = l.pack_x ? xp : x;
+  const char* W = l.pack_w ? wp : static_cast<const char*>(w);
   const int64_t x_plane = N * (int64_t)l.ld, w_plane = (int64_t)V * l.ld, z_plane = (N + 63) / 64 * 64 * (int64_t)p.piece;
   for (int v0 = 0; v0 < V; v0 += p.piece) {
     const int vocab = V - v0 < p.piece ? V - v0 : p.piece;
     HeadDz z;
-    z.pr.a = {W + (int64_t)v0 * ldw, w_plane, ldw, vocab, 0};
+    z.pr.a = {W + (int64_t)v0 * ldw * (l.native ? 4 : 2), w_plane, ldw, vocab, 0};
     z.pr.b = {X, x_plane, ldx, (int)N, 0};
     z.pr.K = D;
     z.pr.pa = l.pw;
@@ -1041,30 +1138,36 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
     auto form = [&](auto sh) {   // (its tiles cover dz's rows of zeros)
       using S = decltype(sh);
       z.g = head_grid<S>(N, vocab, cu);
-      if (l.px == 3)
-        k_head_dz<S, 3><<<head_blocks(z.g), S::kThreads, 0, s>>>(z);
-      else
-        k_head_dz<S, 1><<<head_blocks(z.g), S::kThreads, 0, s>>>(z);
+      if constexpr (sizeof(typename S::E) == 2)
+        if (l.px == 3) return k_head_dz<S, 3><<<head_blocks(z.g), S::kThreads, 0, s>>>(z);
+      k_head_dz<S, 1><<<head_blocks(z.g), S::kThreads, 0, s>>>(z);
     };
-    if (head_kind(N, vocab, cu) == kBig)
-      form(HeadBig{});
+    if (head_few_back(N, l.native))
+      form(HeadFewBack{});
+    else if (l.native)
+      form(HeadMid<float>{});
+    else if (head_kind(N, vocab, cu) == kBig)
+      form(HeadBig<bf16>{});
     else
-      form(HeadMid{});
-    if (l.px == 3)
-      k_head_target<3><<<(unsigned)((N + 255) / 256), 256, 0, s>>>(z, logp);
+      form(HeadMid<bf16>{});
+    const unsigned rows = (unsigned)((N + 255) / 256);
+    if (l.native)
+      k_head_target<float, 1><<<rows, 256, 0, s>>>(z, logp);
+    else if (l.px == 3)
+      k_head_target<bf16, 3><<<rows, 256, 0, s>>>(z, logp);
     else
-      k_head_target<1><<<(unsigned)((N + 255) / 256), 256, 0, s>>>(z, logp);
+      k_head_target<bf16, 1><<<rows, 256, 0, s>>>(z, logp);
     if (dx != nullptr) {
       HeadGrad g;
       const bool last = v0 + vocab >= V, lone = p.acc == 0;
-      g.pr = {{W + (int64_t)v0 * ldw, w_plane, ldw, ldw, vocab}, {dz, z_plane, p.piece, (int)N, 0}, vocab, l.pw, l.px};
+      g.pr = {{W + (int64_t)v0 * ldw * (l.native ? 4 : 2), w_plane, ldw, ldw, vocab}, {dz, z_plane, p.piece, (int)N, 0}, vocab, l.pw, l.px};
       g.out = last || lone ? dx : static_cast<void*>(acc);
       g.out_bf16 = last && x_dtype == NSA_BF16;
       g.add = v0 == 0 ? nullptr : lone ? static_cast<const float*>(dx) : acc;
       g.part = part;
       g.N = (int)N;
       g.D = D;
-      head_grad<true>(g, cu, s);
+      head_grad<true>(g, l.native, cu, s);
     }
     if (dw != nullptr) {
       HeadGrad g;
@@ -1075,7 +1178,7 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
       g.part = part;
       g.N = vocab;
       g.D = D;
-      head_grad<false>(g, cu, s);
+      head_grad<false>(g, l.native, cu, s);
     }
   }
   return nsa_launch_status();

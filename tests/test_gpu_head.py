@@ -112,7 +112,9 @@ def test_large_tiles(N, V, D, xd):
     _check(N, V, D, xd, xd, seed=N)
 
 
-@pytest.mark.parametrize("N,V,D,xd", [(32, 140001, 72, BF), (64, 140001, 72, BF), (65, 70001, 136, BF), (128, 70001, 40, F32)])
+@pytest.mark.parametrize("N,V,D,xd", [(32, 140001, 72, BF), (64, 140001, 72, BF), (65, 70001, 136, BF), (128, 70001, 40, F32),
+                                      (32, 70001, 64, F32), (64, 70001, 72, F32), (200, 20001, 96, F32), (500, 40001, 72, F32),
+                                      (16, 1100001, 32, F32), (16, 1100001, 32, BF)])
 def test_few_rows_of_many_tokens(N, V, D, xd):
     """Several tiles of the vocabulary one after another in a workgroup."""
     _check(N, V, D, xd, xd, seed=N)
