@@ -642,10 +642,14 @@ extern "C" int nsa_embed_bwd(const int64_t* index, const void* dy, void* dw, voi
       va = vb, vb = t;
     }
   }
-  const EmbedGrad g{index != nullptr ? ka : nullptr, va, dy, dw, part, n, T, V, (uint32_t)(index != nullptr ? 1 : n / T),
-                    D, p.len, p.pieces, scale, dy_dtype == NSA_BF16, w_dtype == NSA_BF16};
+  // positions 0 .. T-1 of up to 64 sequences: whole runs a piece, none to join
+  const int64_t B = index != nullptr ? 1 : n / T;
+  const bool whole = index == nullptr && B <= 64;
+  const int len = whole ? (int)((p.len + B - 1) / B * B) : p.len, pieces = (int)((n + len - 1) / len);
+  const EmbedGrad g{index != nullptr ? ka : nullptr, va, dy, dw, part, n, T, V, (uint32_t)B,
+                    D, len, pieces, scale, dy_dtype == NSA_BF16, w_dtype == NSA_BF16};
   const int64_t clear = (V + 63) / 64;
-  const unsigned grid = (unsigned)(p.pieces + (clear < (1 << 16) ? clear : 1 << 16));
+  const unsigned grid = (unsigned)(pieces + (clear < (1 << 16) ? clear : 1 << 16));
   const int E = g.dy_bf16 ? 8 : 4, runs = (D + E - 1) / E;
   const int nth = runs >= 256 ? 256 : (runs + 63) / 64 * 64;
   const dim3 all(grid, (unsigned)((runs + nth - 1) / nth));
@@ -653,7 +657,7 @@ extern "C" int nsa_embed_bwd(const int64_t* index, const void* dy, void* dw, voi
     k_embed_runs<8><<<all, nth, 0, s>>>(g);
   else
     k_embed_runs<4><<<all, nth, 0, s>>>(g);
-  if (p.pieces > 1)
-    k_embed_join<<<dim3((unsigned)(p.pieces - 1), (unsigned)((D + 255) / 256)), 64 * kJoinWaves, 0, s>>>(g);
+  if (pieces > 1 && !whole)
+    k_embed_join<<<dim3((unsigned)(pieces - 1), (unsigned)((D + 255) / 256)), 64 * kJoinWaves, 0, s>>>(g);
   return nsa_launch_status();
 }
