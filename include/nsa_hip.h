@@ -601,8 +601,8 @@ int nsa_embed_fwd(const int64_t* tokens, const int64_t* pos, const void* w, cons
 /* The gradient of one table, all V rows of it: dw[v] = scale sum of dy[i] over the i
  * with index[i] = v, summed in an order fixed by the indices (rows without one: 0);
  * index outside the table: none.  index null: i % T (n a multiple of T, T <= V).
- * workspace: nsa_embed_bwd_workspace bytes (0: unsupported shape), `sorted` 0 where
- * index is null. */
+ * workspace: 16-byte aligned, nsa_embed_bwd_workspace bytes (0: unsupported shape),
+ * `sorted` 0 where index is null. */
 size_t nsa_embed_bwd_workspace(int64_t n, int D, int sorted);
 int nsa_embed_bwd(const int64_t* index, const void* dy, void* dw, void* workspace, size_t workspace_bytes, int64_t n,
                   int64_t T, int64_t V, int D, float scale, int dy_dtype, int w_dtype, void* stream);
@@ -614,8 +614,8 @@ int nsa_embed_bwd(const int64_t* index, const void* dy, void* dw, void* workspac
  * float [N] each; target and logp both null: lse alone.  float rows: float's
  * precision; bf16 rows: products of bf16, summed in float (float weights are rounded
  * to bf16 first).  N <= 2^22, V <= 2^24, D <= 65536; any element-aligned addresses.
- * workspace: nsa_head_fwd_workspace bytes (0: unsupported shape); `aligned` 1 only
- * where x and w lie on 16 bytes. */
+ * workspace: 16-byte aligned, nsa_head_fwd_workspace bytes (0: unsupported shape);
+ * `aligned` 1 only where x and w lie on 16 bytes. */
 size_t nsa_head_fwd_workspace(int64_t N, int V, int D, int x_dtype, int w_dtype, int aligned, void* stream);
 int nsa_head_fwd(const void* x, const void* w, const int64_t* target, float* logp, float* lse, void* workspace,
                  size_t workspace_bytes, int64_t N, int V, int D, int x_dtype, int w_dtype, void* stream);

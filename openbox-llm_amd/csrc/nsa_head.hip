@@ -25,6 +25,12 @@
 // the transposed LDS reads turn; no transposed copy is made.  Results have the
 // 32-row tile's rows permuted (perm32), so that a lane holds eight neighbouring
 // elements of an output row.
+//
+// Large products are bound by the matrix unit: 32768 x 32000 x d768 in bf16, 1.61 TFLOP a
+// product: z with its log sums 1.33 to 1.41 ms (1140 to 1210 TFLOP/s), dz 1.64 to 1.73 with
+// its exponentials and 2.1 GB of stores, dx and dW 1.40 each (1150); a library product of these
+// shapes takes 1.45 (z), 1.47 (dx) and 2.00 (dW).  At d4096 (8192 x 8192) all four run at
+// 1310.  Few rows are bound by W: 32 x 32000 x d768 reads its 49 MB in 11 us.
 #include "nsa_launch.h"
 #include "nsa_rows.h"
 #include "nsa_tile32.h"
@@ -1050,6 +1056,7 @@ extern "C" int nsa_head_fwd(const void* x, const void* w, const int64_t* target,
     NSA_CHECK(workspace != nullptr &&
                   workspace_bytes >= l.x_bytes + l.w_bytes + up16((size_t)g.split * N * sizeof(float2)) + (size_t)N * 4,
               NSA_ERR_WORKSPACE);
+    NSA_CHECK(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, NSA_ERR_ARG);
     char* ws = static_cast<char*>(workspace);
     char *const xp = ws, *const wp = ws + l.x_bytes;
     float2* part = reinterpret_cast<float2*>(ws + l.x_bytes + l.w_bytes);
@@ -1099,6 +1106,7 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
   const HeadPlan p = head_plan(N, V, D, l, x_dtype == NSA_BF16, cu);
   NSA_CHECK(workspace != nullptr && workspace_bytes >= l.x_bytes + l.w_bytes + p.dz + p.acc + p.part,
             NSA_ERR_WORKSPACE);
+  NSA_CHECK(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, NSA_ERR_ARG);
   char* ws = static_cast<char*>(workspace);
   char* const xp = ws;
   ws += l.x_bytes;

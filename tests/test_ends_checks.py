@@ -82,6 +82,14 @@ def test_head_refusals():
     assert bwd() == ARG and bwd(x=16, dx=None) == ARG and bwd(x=16, dlogp=16) == ARG and bwd(x=16) == WORKSPACE
 
 
+def test_workspaces_off_16_bytes_are_refused():
+    lib = _lib()
+    big = 1 << 40
+    assert lib.nsa_head_fwd(16, 16, None, None, 16, 24, big, 4, 10, 8, 1, 1, None) == ARG
+    assert lib.nsa_head_bwd(16, 16, None, None, 16, None, 16, 16, None, 24, big, 4, 10, 8, 1, 1, None) == ARG
+    assert lib.nsa_embed_bwd(16, 16, 16, 24, big, 4, 2, 10, 8, 1.0, 0, 0, None) == ARG
+
+
 def test_the_backward_never_holds_the_logits():
     """What the backward takes beside its results stays near 1 GB of dz, however large
     the vocabulary: dz of 32768 rows x 131072 tokens would be 8.6 GB in bf16."""
