@@ -24,7 +24,7 @@
 // Measured: 8 x 4096 rows of 768 in float32 with their positions, table of 32000: 38 us
 // forward (300 MB less what the caches hold of the table; a copy's rate is 5.4 TB/s); 49 for
 // the tokens' sums (200 MB, 4.1 TB/s), 20 for their sort (four launches of one dependent
-// chain each), 9 for the joins, 18 for the positions' sums. 8191 x 4096 bf16 rows: 22 us.
+// chain each), 11 for the joins, 18 for the positions' sums. 8191 x 4096 bf16 rows: 22 us.
 #include "nsa_launch.h"
 #include "nsa_rows.h"
 
