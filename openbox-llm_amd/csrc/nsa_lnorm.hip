@@ -23,8 +23,8 @@
 // by a second launch, so that both have the same bits on every run.
 //
 // Measured, against a copy's 5.4 TB/s: 32768 x 768 (bf16 branch, float32 stream) 59 us
-// forward (5.1 TB/s), 78 backward (5.2) and 7 for the 2048 parts of dw and db; 8191 x 8192
-// bf16 96 (5.6), 114 (4.7) and 13.
+// forward (5.1 TB/s), 78 backward (5.2) and 6.5 for the 2048 parts of dw and db; 8191 x 8192
+// bf16 96 (5.6), 114 (4.7) and 8.4.
 #include "nsa_launch.h"
 #include "nsa_rows.h"
 
@@ -430,28 +430,28 @@ __global__ __launch_bounds__(256) void k_ln_dw_wide(const LnBwdArgs a) {
   store_run8(a.part + ((int64_t)gridDim.y + blockIdx.y) * a.D + c, n, db);
 }
 
-// out[c] = sum of part[p][c] (dw for blockIdx.y = 0, db for 1): 16 columns a workgroup
-// (64-byte pieces of a part), 64 interleaved sums over the parts, added in order.
+// out[c] = sum of part[p][c] (dw for blockIdx.y = 0, db for 1): 32 columns a workgroup (a
+// part's cache lines, each in one L2: 512 parts of 8192 8.4 us, 13.8 with half lines), 32
+// interleaved sums over the parts, added in order.
 __global__ __launch_bounds__(1024) void k_ln_dw(const float* __restrict__ part, int nparts, int D, void* dw, void* db,
                                                 bool w_bf16) {
-  __shared__ float acc[64][17];
-  const int x = threadIdx.x & 15, s = threadIdx.x >> 4;
-  const int c = blockIdx.x * 16 + x;
+  __shared__ float acc[32][33];
+  const int x = threadIdx.x & 31, s = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + x;
   void* out = blockIdx.y == 0 ? dw : db;
   if (out == nullptr) return;
   part += (int64_t)blockIdx.y * nparts * D;
   float v = 0.0f;
   if (c < D) {
 #pragma unroll 8
-    for (int p = s; p < nparts; p += 64) v += part[(int64_t)p * D + c];
+    for (int p = s; p < nparts; p += 32) v += part[(int64_t)p * D + c];
   }
   acc[s][x] = v;
   __syncthreads();
-  if (s < 4) {   // 16 sums each by the first wave, then those four
+  if (s < 2) {   // 16 sums each by the halves of the first wave, then those two
     float t = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) t += acc[16 * s + i][x];
-    t += __shfl_xor(t, 16, kWave);
     t += __shfl_xor(t, 32, kWave);
     if (s == 0 && c < D) {
       if (w_bf16)
@@ -556,7 +556,7 @@ static int ln_bwd_launch(LnBwdArgs a, void* dw, void* db, hipStream_t s) {
 #undef NSA_LN_CASE
   if (!done) return NSA_ERR_SHAPE;
   if (a.part != nullptr)
-    k_ln_dw<<<dim3((unsigned)((a.D + 15) / 16), 2), 1024, 0, s>>>(a.part, (int)grid, a.D, dw, db, a.w_bf16);
+    k_ln_dw<<<dim3((unsigned)((a.D + 31) / 32), 2), 1024, 0, s>>>(a.part, (int)grid, a.D, dw, db, a.w_bf16);
   return nsa_launch_status();
 }
 
