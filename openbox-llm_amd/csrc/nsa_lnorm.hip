@@ -520,16 +520,22 @@ static int ln_fwd_as(const LnArgs& a, hipStream_t s) {
   return NSA_ERR_DTYPE;
 }
 
-// Parts of dw and db: a workgroup of the backward each, eight to a compute unit or
-// what its waves hold; past kLnBwdMax a row group of k_ln_dw_wide.
+// Parts of dw and db: a workgroup of the backward each; past kLnBwdMax a row group of
+// k_ln_dw_wide.  A part is written and read once more, 16 bytes an element against the 8 or 16
+// of a row's in bf16 or float32: workgroups take 16 rows in turn (4 where rows are few), while
+// they are eight waves a compute unit and one workgroup each, and no more than the chip holds
+// (bf16, 2048 x 768 10 us, 16.5 with a row each; 4096 x 4096 26 and 36; 8192 x 2048 26 and 35).
 static int64_t ln_bwd_groups(int64_t rows, int D, int cu) {
   if (D > kLnBwdMax) return rows < 128 ? rows : 128;
   const LnShape sh = ln_shape(D);
-  const int rpg = sh.tpr <= 64 ? 256 / sh.tpr : 1;
-  const int64_t groups = (rows + rpg - 1) / rpg;
-  const int threads = ln_threads(sh, D);
-  const int64_t most = (int64_t)cu * (threads <= 256 ? 8 : 2048 / threads);
-  return groups < most ? groups : most;
+  const int rpg = sh.tpr <= 64 ? 256 / sh.tpr : 1, threads = ln_threads(sh, D);
+  const int64_t turns = (rows + rpg - 1) / rpg;   // of one workgroup
+  const int64_t most = (int64_t)cu * (threads <= 256 ? 8 : 2048 / threads), eight = (int64_t)cu * 512 / threads;
+  int64_t groups = turns / 16 > eight ? turns / 16 : eight;
+  groups = groups < turns / 4 ? groups : turns / 4;
+  groups = groups > cu ? groups : cu;
+  groups = groups < most ? groups : most;
+  return groups < turns ? groups : turns;
 }
 
 template <typename YT, typename RT>
