@@ -829,13 +829,14 @@ static bool head_shape_ok(int64_t N, int V, int D) {
 }
 static size_t up16(size_t n) { return (n + 255) / 256 * 256; }
 
-// Tile of the product over the vocabulary: 256 x 256 where that gives every compute unit
-// a tile, else 128 x 128.  The forward of up to 128 rows, one tile across, waits for W: it
+// Tile of the product over the vocabulary: 256 x 256 where that gives five of eight compute
+// units a tile (16000 x 768, 700 rows, 0.74 of them: 29.5 us, 33 in 128 x 128; 8192 x 768, 1024 rows,
+// 0.5: 28 and 25), else 128 x 128.  The forward of up to 128 rows, one tile across, waits for W: it
 // takes the narrowest of 32, 64 and 128 rows, with stages for more of W under way (bf16, W
 // 32000 x 4096, 64 and 128 rows: 50 and 53 us, 67 and 71 in the common 128 x 128).
 enum { kFew, kFew64, kFew128, kMid, kBig };
 static int head_kind(int64_t N, int V, int cu) {
-  return ((N + 255) / 256) * ((V + 255) / 256) >= cu && N > 128 ? kBig : kMid;
+  return ((N + 255) / 256) * ((V + 255) / 256) * 8 >= (int64_t)cu * 5 && N > 128 ? kBig : kMid;
 }
 static int head_fwd_kind(int64_t N, int V, int cu) {
   return N <= 32 ? kFew : N <= 64 ? kFew64 : N <= 128 ? kFew128 : head_kind(N, V, cu);
