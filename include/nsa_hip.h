@@ -613,7 +613,8 @@ int nsa_embed_bwd(const int64_t* index, const void* dy, void* dw, void* workspac
  *   lse   ln sum_v e^{z_nv},  logp  z_{n, target[n]} - lse_n (0: target outside 0 .. V-1)
  * float [N] each; target and logp both null: lse alone.  float rows: float's
  * precision; bf16 rows: products of bf16, summed in float (float weights are rounded
- * to bf16 first).  N <= 2^22, V <= 2^24, D <= 65536; any element-aligned addresses.
+ * to bf16 first).  Logits of any finite size; rows with NaN or plus infinity are NaN.
+ * N <= 2^22, V <= 2^24, D <= 65536; any element-aligned addresses.
  * workspace: 16-byte aligned, nsa_head_fwd_workspace bytes (0: unsupported shape);
  * `aligned` 1 only where x and w lie on 16 bytes. */
 size_t nsa_head_fwd_workspace(int64_t N, int V, int D, int x_dtype, int w_dtype, int aligned, void* stream);

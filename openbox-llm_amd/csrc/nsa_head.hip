@@ -402,10 +402,28 @@ __device__ __forceinline__ int head_share(const HeadGrid& g, int part) {
 __device__ __forceinline__ bool head_real(const int64_t* target, int64_t n, int V) {
   return target != nullptr && target[n] >= 0 && target[n] < V;
 }
+// What a row's weights refer to: 2^((z - a) log2 e - b), from a maximum m that is one of the
+// row's logits.  Near zero a = 0 and b = m log2 e, so that a weight is one multiply-add and an exponential;
+// the rounding of b (half a step of it, at most 2^-11) is in every weight alike.  Far off zero that
+// rounding would be any power of two: there a = m, b = 0.  m starts at the lowest finite value, never at a sentinel
+// that a finite logit can lie below.
+constexpr float kHeadFar = 4096.0f;
+constexpr float kHeadLowest = -3.402823466e38f;
+__device__ __forceinline__ bool head_far(float m) { return !(fabsf(m) < kHeadFar); }
+struct HeadRef {
+  float a, b;
+  __device__ __forceinline__ explicit HeadRef(float m) : a(head_far(m) ? m : 0.0f), b(head_far(m) ? 0.0f : m * kLog2e) {}
+  __device__ __forceinline__ float weight(float z) const { return fast_exp2(fmaf(z - a, kLog2e, -b)); }
+  // what a sum of such weights is multiplied with to refer to `to`
+  __device__ __forceinline__ float factor(const HeadRef& to) const {
+    return fast_exp2(fmaf(a - to.a, kLog2e, b - to.b));
+  }
+};
+
 struct HeadFwd {
   HeadProduct pr;    // a: weights, b: rows
   HeadGrid g;
-  float2* part;      // [split][N]: maximum (log2 units) and sum of 2^(z - maximum)
+  float2* part;      // [split][N]: maximum and sum of the weights that refer to it
   const int64_t* target;   // or null
   float* zt;         // [N]: the target's z, where there is one
   int N, V;
@@ -420,7 +438,7 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_fwd(const Hea
   const int lane = threadIdx.x & 63, h = lane >> 5;
   float m[S::NT], l[S::NT];
 #pragma unroll
-  for (int j = 0; j < S::NT; ++j) m[j] = kMaskScore, l[j] = 0.0f;
+  for (int j = 0; j < S::NT; ++j) m[j] = kHeadLowest, l[j] = 0.0f;
   int t[S::NT];   // the rows' targets
 #pragma unroll
   for (int j = 0; j < S::NT; ++j) {
@@ -447,17 +465,22 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_fwd(const Hea
               return s[0] + s[1];
             };
             // the maximum so far serves while the sum stays in range; the first tile, a
-            // row that grows by 40 bits and one with NaN take their own
-            float s = sum(m[j]);
+            // row that grows by 40 bits, one far off zero and one with NaN take their own
+            float s = sum(head_far(m[j]) ? __builtin_nanf("") : m[j] * kLog2e);
             if (__any(!(s < 0x1p40f))) {
               float t = z(0, 0);
 #pragma unroll
               for (int i = 0; i < S::MT; ++i)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) t = fmaxf(t, z(i, r));
-              const float mn = fmaxf(m[j], t * kLog2e);
-              s = sum(mn);
-              l[j] *= fast_exp2(m[j] - mn);
+              const float mn = fmaxf(m[j], t);
+              const HeadRef to(mn);
+              s = 0.0f;
+#pragma unroll
+              for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s += to.weight(z(i, r));
+              l[j] *= HeadRef(m[j]).factor(to);
               m[j] = mn;
             }
             l[j] += s;
@@ -487,17 +510,19 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_fwd(const Hea
   for (int j = 0; j < S::NT; ++j) {
     const float mo = __shfl_xor(m[j], 32, kWave), lo = __shfl_xor(l[j], 32, kWave);
     const float mx = fmaxf(m[j], mo);
-    const float s = l[j] * fast_exp2(m[j] - mx) + lo * fast_exp2(mo - mx);
+    const HeadRef to(mx);
+    const float s = l[j] * HeadRef(m[j]).factor(to) + lo * HeadRef(mo).factor(to);
     if (h == 0) st[wmi][wn + 32 * j + (lane & 31)] = make_float2(mx, s);
   }
   __syncthreads();
   for (int c = threadIdx.x; c < S::TN; c += S::kThreads) {
     const int n = nt * S::TN + c;
-    float mx = kMaskScore, s = 0.0f;
+    float mx = kHeadLowest, s = 0.0f;
 #pragma unroll
     for (int i = 0; i < S::WM; ++i) mx = fmaxf(mx, st[i][c].x);
+    const HeadRef to(mx);
 #pragma unroll
-    for (int i = 0; i < S::WM; ++i) s += st[i][c].y * fast_exp2(st[i][c].x - mx);
+    for (int i = 0; i < S::WM; ++i) s += st[i][c].y * HeadRef(st[i][c].x).factor(to);
     if (n < a.N) a.part[(int64_t)part * a.N + n] = make_float2(mx, s);
   }
 }
@@ -515,19 +540,21 @@ __global__ __launch_bounds__(256) void k_head_join(const HeadJoin a) {
   const int lane = threadIdx.x & 63;
   const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (n >= a.N) return;
-  float m = kMaskScore, l = 0.0f;
+  float m = kHeadLowest, l = 0.0f;
 #pragma unroll 4
   for (int s = lane; s < a.split; s += kWave) {
     const float2 p = a.part[(int64_t)s * a.N + n];
     const float mx = fmaxf(m, p.x);
-    l = l * fast_exp2(m - mx) + p.y * fast_exp2(p.x - mx);
+    const HeadRef to(mx);
+    l = l * HeadRef(m).factor(to) + p.y * HeadRef(p.x).factor(to);
     m = mx;
   }
   const float mx = wave_max(m);
+  const HeadRef ref(mx);
   const bool nan = l != l;   // (a maximum passes NaN over: its sum shows it)
-  l = wave_sum(l * fast_exp2(m - mx));
-  if (__any(nan)) l = __builtin_nanf("");
-  const float lse = (mx + __log2f(l)) * kLn2;
+  l = wave_sum(l * HeadRef(m).factor(ref));
+  if (__any(nan) || l == 0.0f) l = __builtin_nanf("");   // (no weight at all: every logit is minus infinity)
+  const float lse = fmaf(ref.b + __log2f(l), kLn2, ref.a);
   if (lane == 0) {
     if (a.target != nullptr) a.logp[n] = head_real(a.target, n, a.V) ? a.zt[n] - lse : 0.0f;
     a.lse[n] = lse;
@@ -562,8 +589,9 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_dz(const Head
   if (!head_place(a.g, (int)blockIdx.x, nt, part)) return;
   const int lane = threadIdx.x & 63, h = lane >> 5;
   const int wn0 = ((threadIdx.x >> 6) / S::WM) * S::NT * 32;
-  float off[S::NT];      // |dz| = 2^(z log2 e - off)
+  float off[S::NT];      // |dz| = 2^(z log2 e - off), of a row far off zero with z - lse (<= 0) for z
   uint32_t neg[S::NT];   // dz's sign bit
+  bool far = false;
 #pragma unroll
   for (int j = 0; j < S::NT; ++j) {
     const int n = nt * S::TN + wn0 + 32 * j + (lane & 31);
@@ -572,7 +600,9 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_dz(const Head
     if (n < a.N) {
       float co = a.dlse != nullptr ? a.dlse[n] : 0.0f;
       if (a.dlogp != nullptr && head_real(a.target, n, a.V)) co -= a.dlogp[n];
-      off[j] = a.lse[n] * kLog2e - __log2f(fabsf(co));
+      const float lse = a.lse[n];
+      far = far || head_far(lse);
+      off[j] = (head_far(lse) ? lse - lse : lse * kLog2e) - __log2f(fabsf(co));   // (lse - lse: NaN stays NaN)
       neg[j] = __float_as_uint(co) & 0x80000000u;
     }
   }
@@ -583,10 +613,23 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_dz(const Head
   static_assert(S::MT % kI == 0 && (kI == 2 || PLANES == 1), "128 bytes of the vocabulary");
   __shared__ __align__(16) char turn[S::kThreads / 64 * 4096];
   const int steps = head_steps<S>(a.pr), tiles = head_share(a.g, part);
+  const bool any_far = __any(far) != 0;
   head_product<S, true, true>(
       a.pr, tiles, tiles * steps, [&](int i) { return HeadSpan{part + i * a.g.split, nt, 0, steps}; },
       [&](const HeadSpan& sp, int wm, int wn, f32x16(&acc)[S::MT][S::NT]) {
         const int mt = sp.m;
+        if (any_far) {
+#pragma unroll
+          for (int j = 0; j < S::NT; ++j) {
+            const int n = nt * S::TN + wn + 32 * j + (lane & 31);
+            const float lse = n < a.N ? a.lse[n] : 0.0f;
+            const float from = head_far(lse) ? lse : 0.0f, most = head_far(lse) ? 0.0f : __builtin_inff();
+#pragma unroll
+            for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) acc[i][j][r] = fminf(acc[i][j][r] - from, most);
+          }
+        }
         // else zeros past the vocabulary, and in the rows past N (of any sums, NaN among them)
         const bool inside = mt * S::TM + S::TM <= a.vocab && nt * S::TN + S::TN <= a.N;
         char* const mine = turn + (threadIdx.x >> 6) * 4096;

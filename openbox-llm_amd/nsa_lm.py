@@ -172,7 +172,11 @@ def linear_logprobs(x, weight, targets=None):
     bfloat16 with float32 sums, and the logits' gradient is rounded once to bfloat16
     on its way into the products with x and weight; float32 weights beside bfloat16
     rows are rounded to bfloat16 first (as under autocast) and have a float32
-    gradient.  At most 2^22 rows.  Rows with NaN or an infinite logit give NaN."""
+    gradient.  At most 2^22 rows.
+
+    Every finite logit counts, whatever its size.  A row with NaN or plus infinity among
+    its logits, or with minus infinity alone, is NaN.  The backward's probabilities are
+    formed from ``lse`` as float32 holds it: within ``|lse| 2^-23`` of their size."""
     f = L.torch_side().linear_logprobs
     if _ops._TIMER is None:
         return LinearLogprobs(*f(x, weight, targets))
