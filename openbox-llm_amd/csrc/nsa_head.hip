@@ -464,10 +464,11 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_fwd(const Hea
                 for (int r = 0; r < 16; ++r) s[r & 1] += fast_exp2(fmaf(z(i, r), kLog2e, -ref));
               return s[0] + s[1];
             };
-            // the maximum so far serves while the sum stays in range; the first tile, a
-            // row that grows by 40 bits, one far off zero and one with NaN take their own
+            // the maximum so far serves while no weight has grown past 8 bits (its exponent is rounded
+            // to 2^-22 then; a longer way from the maximum would cost the sum digits); the first tile, a
+            // row that grows further, one far off zero and one with NaN take their own
             float s = sum(head_far(m[j]) ? __builtin_nanf("") : m[j] * kLog2e);
-            if (__any(!(s < 0x1p40f))) {
+            if (__any(!(s < 0x1p8f))) {
               float t = z(0, 0);
 #pragma unroll
               for (int i = 0; i < S::MT; ++i)
@@ -554,11 +555,24 @@ __global__ __launch_bounds__(256) void k_head_join(const HeadJoin a) {
   const bool nan = l != l;   // (a maximum passes NaN over: its sum shows it)
   l = wave_sum(l * HeadRef(m).factor(ref));
   if (__any(nan) || l == 0.0f) l = __builtin_nanf("");   // (no weight at all: every logit is minus infinity)
-  const float lse = fmaf(ref.b + __log2f(l), kLn2, ref.a);
-  if (lane == 0) {
-    if (a.target != nullptr) a.logp[n] = head_real(a.target, n, a.V) ? a.zt[n] - lse : 0.0f;
-    a.lse[n] = lse;
+  if (lane != 0) return;
+  // l = f 2^e with f about 1.  The target's distance from the maximum and e are joined in 64 bits, so that logp is
+  // off by a few 2^-24 however large the logits are (less lse it would have an error of lse's size:
+  // 8e-6 at 100, of either sign).
+  int e;
+  float f = frexpf(l, &e);
+  if (f < 0.70710678f) f *= 2.0f, --e;
+  const float log_f = __log2f(f);
+  constexpr double kPerBit = 1.0 / (double)kLog2e;
+  a.lse[n] = (float)((double)ref.a + ((double)ref.b + (double)e + (double)log_f) * kPerBit);
+  if (a.target == nullptr) return;
+  float logp = 0.0f;
+  if (head_real(a.target, n, a.V)) {
+    const double d = fma((double)a.zt[n] - (double)ref.a, (double)kLog2e, -(double)ref.b) - (double)e;
+    logp = ((float)d - log_f) * (float)kPerBit;
+    logp = logp > 0.0f ? 0.0f : logp;   // (NaN stays)
   }
+  a.logp[n] = logp;
 }
 
 // dz of a piece of the vocabulary, as the gradients' operand
@@ -695,7 +709,7 @@ __global__ __launch_bounds__(256) void k_head_target(const HeadDz a, const float
   const int64_t v = a.target[n] - a.v0;
   if (v < 0 || v >= a.vocab) return;
   const float b = a.dlogp[n], dl = a.dlse != nullptr ? a.dlse[n] : 0.0f, lp = logp[n];
-  // (dlse - b) p + b with 1 - p from expm1: p near 1 leaves no digits in 1 - p otherwise
+  // (dlse - b) p + b with 1 - p from expm1: within a few 2^-24 as logp is, not of the size of the logits
   float d = dl * expf(lp) - b * expm1f(lp);
   E* p = static_cast<E*>(a.dz) + n * a.ld + v;
 #pragma unroll
