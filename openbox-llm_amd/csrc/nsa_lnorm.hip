@@ -9,6 +9,10 @@
 //   dh = dh_out + rstd (g - mean_j g_j - n mean_j(g_j n_j));   dx = dr = dh
 //   dw = sum over rows of dy n,   db = sum over rows of dy
 //
+// The mean is summed in 64 bits and rounded once: a sum in 32, or its product with a rounded 1 / D, is off by steps of
+// the elements' size, which rows far off zero show beside their deviation (41 times 16384 came out as 0.19, not
+// 0).
+//
 // Every kernel is bound by the bytes it moves: one read of x and r (dy, dh_out and
 // h in the backward), one write of h and y (dx, dr).  A row stays in registers, so
 // that the squares are taken about the mean itself (a sum of squares less the
@@ -42,6 +46,7 @@ struct LnArgs {
   int64_t rows;
   int D;
   float eps, inv_d;
+  double inv_d64;
   bool w_bf16, y_bf16;
 };
 
@@ -102,9 +107,9 @@ __device__ __forceinline__ void ln_weights(const void* w, bool is_bf16, const Ru
 }
 
 // Sums of K values over a row's threads: TPR of them, or past a wave the workgroup's
-// (whole waves, TPR at most).  buf: K * TPR / 64 floats.
-template <int TPR, int K>
-__device__ __forceinline__ void row_sums(float (&v)[K], float* buf) {
+// (whole waves, TPR at most).  buf: K * TPR / 64 values.
+template <int TPR, typename T, int K>
+__device__ __forceinline__ void row_sums(T (&v)[K], T* buf) {
   static_assert(TPR <= 16 * kWave, "sixteen waves");
 #pragma unroll
   for (int k = 0; k < K; ++k) v[k] = wave_sum<(TPR < kWave ? TPR : kWave)>(v[k]);
@@ -119,7 +124,7 @@ __device__ __forceinline__ void row_sums(float (&v)[K], float* buf) {
   const int i = tid & 15;
   const bool there = i < (int)(blockDim.x / kWave);
 #pragma unroll
-  for (int k = 0; k < K; ++k) v[k] = wave_sum<16>(there ? buf[K * i + k] : 0.0f);
+  for (int k = 0; k < K; ++k) v[k] = wave_sum<16>(there ? buf[K * i + k] : (T)0);
 }
 
 // h of one run: x + r rounded to r's type (RES), or x itself
@@ -143,7 +148,8 @@ __device__ __forceinline__ void ln_sum8(const LnArgs& a, int64_t base, const Run
 template <typename XT, typename RT, bool RES, int TPR, int NV, int EDGE>
 __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_ln_fwd(const LnArgs a) {
   constexpr int W = TPR > kWave ? TPR / kWave : 1;
-  __shared__ float red[2][W];
+  __shared__ double red64[W];
+  __shared__ float red[W];
   const int nth = TPR <= 64 ? TPR : (int)blockDim.x, t = TPR <= 64 ? threadIdx.x & (TPR - 1) : threadIdx.x;
   const int64_t row = TPR <= 64 ? (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR : (int64_t)blockIdx.x;
   if (TPR <= 64 && row >= a.rows) return;   // (all of a row's lanes; no barrier follows for these)
@@ -151,18 +157,18 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_ln_fwd(const LnArgs a
   const int64_t base = row * D;
   const int nrun = NV > 0 ? NV : (D + 8 * nth - 1) / (8 * nth);
   float h[NV > 0 ? NV : 1][8];
-  float s[1] = {0.0f};
+  double s[1] = {0.0};
 #pragma unroll
   for (int i = 0; i < nrun; ++i) {
     float(&hi)[8] = h[NV > 0 ? i : 0];
     const int c = 8 * (i * nth + t), n = D - c;
     ln_sum8<XT, RT, RES>(a, base, RunAt<EDGE>(D, c), hi);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[0] += hi[j];
+    for (int j = 0; j < 8; ++j) s[0] += (double)hi[j];
     if (RES && n > 0) store_run8(static_cast<RT*>(a.h) + base + c, n, hi);
   }
-  row_sums<TPR>(s, red[0]);
-  const float mu = s[0] * a.inv_d;
+  row_sums<TPR>(s, red64);
+  const float mu = (float)(s[0] * a.inv_d64);
   float ss[1] = {0.0f};
 #pragma unroll
   for (int i = 0; i < nrun; ++i) {
@@ -175,7 +181,7 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_ln_fwd(const LnArgs a
       ss[0] += j < n ? hi[j] * hi[j] : 0.0f;
     }
   }
-  row_sums<TPR>(ss, red[1]);
+  row_sums<TPR>(ss, red);
   const float rstd = 1.0f / sqrtf(ss[0] * a.inv_d + a.eps);
   if (a.stat != nullptr && t == 0) {
     a.stat[2 * row] = mu;
@@ -592,7 +598,7 @@ extern "C" int nsa_lnorm_fwd(const void* x, const void* res, const void* w, cons
                    h == nullptr ? nullptr : static_cast<char*>(h) + at * hs,
                    static_cast<char*>(y) + at * ys,
                    stat == nullptr ? nullptr : stat + 2 * r0,
-                   n, D, eps, 1.0f / (float)D, w_dtype == NSA_BF16, y_dtype == NSA_BF16};
+                   n, D, eps, 1.0f / (float)D, 1.0 / (double)D, w_dtype == NSA_BF16, y_dtype == NSA_BF16};
     int rc;
     if (x_dtype == NSA_BF16)
       rc = h_dtype == NSA_BF16 ? ln_fwd_as<bf16, bf16>(a, s) : ln_fwd_as<bf16, float>(a, s);

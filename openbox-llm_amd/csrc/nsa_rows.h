@@ -94,6 +94,29 @@ __device__ __forceinline__ uint32_t lanes_all(uint32_t v, Op op) {
   }
   return v;
 }
+// (a 64-bit value moves as its halves)
+template <int N>
+__device__ __forceinline__ double wave_sum(double v) {
+  auto dpp = [](double x, auto ctrl) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)u, decltype(ctrl)::value, 0xF, 0xF, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(u >> 32), decltype(ctrl)::value, 0xF, 0xF, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+  };
+  auto rows = [](double x, auto swap) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const auto lo = swap((uint32_t)u), hi = swap((uint32_t)(u >> 32));
+    return __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) +
+           __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+  };
+  v += dpp(v, std::integral_constant<int, 0xB1>{});
+  v += dpp(v, std::integral_constant<int, 0x4E>{});
+  v += dpp(v, std::integral_constant<int, 0x141>{});
+  if (N >= 16) v += dpp(v, std::integral_constant<int, 0x140>{});
+  if (N >= 32) v = rows(v, [](uint32_t x) { return __builtin_amdgcn_permlane16_swap(x, x, false, false); });
+  if (N >= 64) v = rows(v, [](uint32_t x) { return __builtin_amdgcn_permlane32_swap(x, x, false, false); });
+  return v;
+}
 template <int N = kWave>
 __device__ __forceinline__ float wave_sum(float v) {
   return __uint_as_float(lanes_all<N>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
