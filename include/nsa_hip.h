@@ -594,7 +594,7 @@ int nsa_lnorm_bwd(const void* dy, const void* dh, const void* h, const void* w, 
  *   out[i] = scale w[tokens[i]] + pw[pos[i]]      (float, rounded once to out_dtype)
  * for n rows of D elements; w [V][D], pw [P][D] (nullable: no positions).  pos null:
  * position i % T.  A token or position outside its table adds nothing.
- * n, V, P < 2^31 - 16, D <= 2^20; any element-aligned addresses. */
+ * n, V, P, T <= 2^31 - 16, D <= 2^20; any element-aligned addresses. */
 int nsa_embed_fwd(const int64_t* tokens, const int64_t* pos, const void* w, const void* pw, void* out, int64_t n,
                   int64_t T, int64_t V, int64_t P, int D, float scale, int w_dtype, int pw_dtype, int out_dtype,
                   void* stream);

@@ -116,7 +116,7 @@ __global__ __launch_bounds__(256) void k_embed_fwd(const EmbedArgs a) {
   if (i >= a.n) return;
   const int64_t tok = a.tokens[i];
   const bool real = tok >= 0 && tok < a.V;
-  // (fewer than 2^31 rows: a 32-bit remainder)
+  // (fewer than 2^31 rows, and T too: a 32-bit remainder)
   const int64_t p = a.pw == nullptr ? 0 : a.pos != nullptr ? a.pos[i] : (int64_t)((uint32_t)i % (uint32_t)a.T);
   const bool has_pos = a.pw != nullptr && p >= 0 && p < a.P;
   const int D = a.D;
@@ -567,7 +567,7 @@ extern "C" int nsa_embed_fwd(const int64_t* tokens, const int64_t* pos, const vo
   NSA_CHECK(n >= 0 && n <= kEmbedRows && V >= 1 && V <= kEmbedRows && D >= 1 && D <= kEmbedWide, NSA_ERR_SHAPE);
   NSA_CHECK(embed_type(w_dtype) && embed_type(out_dtype), NSA_ERR_DTYPE);
   if (pw != nullptr) {
-    NSA_CHECK(P >= 1 && P <= kEmbedRows && (n == 0 || pos != nullptr || T >= 1), NSA_ERR_SHAPE);
+    NSA_CHECK(P >= 1 && P <= kEmbedRows && (n == 0 || pos != nullptr || (T >= 1 && T <= kEmbedRows)), NSA_ERR_SHAPE);
     NSA_CHECK(embed_type(pw_dtype), NSA_ERR_DTYPE);
   }
   if (n == 0) return NSA_OK;
