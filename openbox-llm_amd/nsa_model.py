@@ -158,6 +158,20 @@ class Linear(nn.Linear):
         return _linear(x, self.weight, self.bias)
 
 
+def _plain(m, *kinds):
+    """Whether calling the module is its class's own computation on its parameters: no
+    subclass, parametrization or wrapper, no hooks, no ``forward`` set on it.  What takes
+    the parameters in the module's place (``norm_impl``, ``embed_impl``,
+    ``loss_impl='pieces'``) asks for that."""
+    return type(m) in kinds and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or
+                                     m._backward_pre_hooks or "forward" in m.__dict__)
+
+
+def _plain_table(m):
+    return (_plain(m, nn.Embedding) and m.padding_idx is None and m.max_norm is None and not m.scale_grad_by_freq and
+            not m.sparse)
+
+
 class BlockCompressor(nn.Module):
     """Learned pooling of one span of ``block_size`` tokens into one token:
     ``proj(sum_p softmax(pool_logits)_p * (x_p + intra_pos_p))``
@@ -719,7 +733,11 @@ def _norm(kind, d_model):
 
 def _fused_norm(ln, branch, x):
     """``(ln(x + branch), x + branch)`` in one kernel; the norm's rows in the
-    dtype the products after it compute in (autocast's, where it is on)."""
+    dtype the products after it compute in (autocast's, where it is on).  A norm
+    that is not a plain one (``_plain``) is called."""
+    if not (_plain(ln, nn.LayerNorm, nn.RMSNorm) and ln.weight is not None and len(ln.normalized_shape) == 1):
+        x = x if branch is None else x + branch
+        return ln(x), x
     import nsa_lm
     out = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
     pair = (x, None) if branch is None else (branch, x)
@@ -792,15 +810,23 @@ class NSATransformer(nn.Module):
         T = idx.shape[1]
         assert T <= self.max_seq_len
         learned = hasattr(self, "pos_emb")
-        if self.embed_impl == "fused":
+        if self._fused_embed():
             import nsa_lm
             return nsa_lm.embed(idx, self.tok_emb.weight, pos_weight=self.pos_emb.weight if learned else None)
         x = self.tok_emb(idx)
         return x + self.pos_emb(torch.arange(T, device=idx.device))[None] if learned else x
 
+    def _fused_embed(self):
+        """``embed_impl='fused'``, of plain tables: others are called."""
+        return (self.embed_impl == "fused" and _plain_table(self.tok_emb) and
+                (not hasattr(self, "pos_emb") or _plain_table(self.pos_emb)))
+
     def _linear_logprobs(self, x, targets=None):
         """``nsa_lm.linear_logprobs`` under the LM head, of the rows as its product takes
         them (autocast's dtype, where it is on)."""
+        assert _plain(self.lm_head, Linear, nn.Linear) and self.lm_head.bias is None, \
+            "log probabilities without logits take lm_head's weight alone: an lm_head with a bias, with hooks or with a " \
+            "forward of its own needs loss_impl='ref' or 'fused' (score for logprobs)"
         import nsa_lm
         if torch.is_autocast_enabled("cuda"):
             x = x.to(torch.get_autocast_dtype("cuda"))
@@ -890,7 +916,7 @@ class NSATransformer(nn.Module):
         length tells (its logits then are of no position)."""
         assert len(caches) == len(self.blocks), "one cache for each block"
         at = caches[0].lens.long().clamp(0, self.max_seq_len - 1) if hasattr(self, "pos_emb") else None
-        if self.embed_impl == "fused":
+        if self._fused_embed():
             import nsa_lm
             x = nsa_lm.embed(tokens, self.tok_emb.weight, pos_weight=None if at is None else self.pos_emb.weight,
                              positions=at)
