@@ -40,8 +40,8 @@ namespace nsa {
 constexpr int64_t kHeadRows = 1 << 22;       // most rows of x
 constexpr int kHeadVocab = 1 << 24;
 constexpr int kHeadWide = 1 << 16;           // widest row
-constexpr size_t kHeadPiece = 1u << 30;      // bytes of dz held at a time: 32768 x 32000 x d768 takes 6.3 ms, 6.9 with
-                                             // half of them (the parts of dx and more partial rounds), 6.1 in one piece
+constexpr size_t kHeadPiece = 1u << 30;      // bytes of dz held at a time: the backward of 32768 x 32000 x d768 takes 4.55 ms, 5.03
+                                             // with half of them (the parts of dx and more partial rounds), 4.36 in one piece
 constexpr int64_t kHeadPieceMost = 1 << 20;  // most tokens of a piece: offsets within a stage have 32 bits
 
 // An operand of a product: bf16 planes; ROWS: [rows][ld], contraction along a row;
@@ -901,9 +901,14 @@ static int head_fwd_kind(int64_t N, int V, int cu) {
 // Whether float32 rows and weights go through the float32 instructions rather than as
 // planes.  Planes take six products of bf16 at 870 to 1150 TFLOP/s together and a copy of
 // W of 1.5 times its size, the float32 instructions up to 140 TFLOP/s and no copy: they win
-// where rows are few and the tiles of 128 x 128 half fill the chip (W 32000 x 768, 64, 512 and
-// 2048 rows: forward 35, 201, 720 us, planes 92, 217, 528; 128, 256 and 512 rows: backward
-// 202, 344, 607, planes 258, 323, 571).
+// where rows are few and the tiles of 128 x 128 half fill the chip.  Measured, us of the instructions
+// and of planes, in the order of the W's 32000 x 768, 50257 x 1024, 8192 x 4096 and 128000 x 2048:
+//   forward   128 rows  59  90   130  210   247 248    498 1010
+//             512      186 167   474  380   248 443   1876 1760
+//             768      275 241   594  516   468 438   2813 2331
+//   backward  128 rows 203 245   378  467   486 493   1587 2275
+//             256      309 322   671  646   530 613   2933 2898
+//             512      571 539  1251 1020   755 830   5651 4735
 static bool head_native(int64_t N, int V, int most, int cu) {
   return N <= 64 || (N <= most && (N + 127) / 128 * ((V + 127) / 128) * 2 >= cu);
 }
