@@ -476,11 +476,12 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_fwd(const Hea
                 for (int r = 0; r < 16; ++r) t = fmaxf(t, z(i, r));
               const float mn = fmaxf(m[j], t);
               const HeadRef to(mn);
-              s = 0.0f;
+              float own[2] = {0.0f, 0.0f};
 #pragma unroll
               for (int i = 0; i < S::MT; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s += to.weight(z(i, r));
+                for (int r = 0; r < 16; ++r) own[r & 1] += to.weight(z(i, r));
+              s = own[0] + own[1];
               l[j] *= HeadRef(m[j]).factor(to);
               m[j] = mn;
             }
@@ -541,19 +542,30 @@ __global__ __launch_bounds__(256) void k_head_join(const HeadJoin a) {
   const int lane = threadIdx.x & 63;
   const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (n >= a.N) return;
+  const bool real = head_real(a.target, n, a.V);
+  const float zt = a.zt[n];   // (asked for here, not behind the sums; of no meaning where there is no target)
   float m = kHeadLowest, l = 0.0f;
-#pragma unroll 4
-  for (int s = lane; s < a.split; s += kWave) {
-    const float2 p = a.part[(int64_t)s * a.N + n];
-    const float mx = fmaxf(m, p.x);
+  constexpr int kAtOnce = 4;
+  for (int s0 = 0; s0 < a.split; s0 += kAtOnce * kWave) {
+    float2 p[kAtOnce];
+    float mx = m;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int s = s0 + u * kWave + lane;
+      p[u] = s < a.split ? a.part[(int64_t)s * a.N + n] : make_float2(kHeadLowest, 0.0f);
+    }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) mx = fmaxf(mx, p[u].x);
+    mx = wave_max(mx);
     const HeadRef to(mx);
-    l = l * HeadRef(m).factor(to) + p.y * HeadRef(p.x).factor(to);
+    l *= HeadRef(m).factor(to);
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) l += p[u].y * HeadRef(p[u].x).factor(to);
     m = mx;
   }
-  const float mx = wave_max(m);
-  const HeadRef ref(mx);
+  const HeadRef ref(m);
   const bool nan = l != l;   // (a maximum passes NaN over: its sum shows it)
-  l = wave_sum(l * HeadRef(m).factor(ref));
+  l = wave_sum(l);
   if (__any(nan) || l == 0.0f) l = __builtin_nanf("");   // (no weight at all: every logit is minus infinity)
   if (lane != 0) return;
   // l = f 2^e with f about 1.  The target's distance from the maximum and e are joined in 64 bits, so that logp is
@@ -567,8 +579,8 @@ __global__ __launch_bounds__(256) void k_head_join(const HeadJoin a) {
   a.lse[n] = (float)((double)ref.a + ((double)ref.b + (double)e + (double)log_f) * kPerBit);
   if (a.target == nullptr) return;
   float logp = 0.0f;
-  if (head_real(a.target, n, a.V)) {
-    const double d = fma((double)a.zt[n] - (double)ref.a, (double)kLog2e, -(double)ref.b) - (double)e;
+  if (real) {
+    const double d = fma((double)zt - (double)ref.a, (double)kLog2e, -(double)ref.b) - (double)e;
     logp = ((float)d - log_f) * (float)kPerBit;
     logp = logp > 0.0f ? 0.0f : logp;   // (NaN stays)
   }
