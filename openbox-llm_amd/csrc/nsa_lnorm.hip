@@ -163,8 +163,10 @@ __global__ __launch_bounds__(TPR <= 64 ? 256 : TPR) void k_ln_fwd(const LnArgs a
     float(&hi)[8] = h[NV > 0 ? i : 0];
     const int c = 8 * (i * nth + t), n = D - c;
     ln_sum8<XT, RT, RES>(a, base, RunAt<EDGE>(D, c), hi);
+    double q[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[0] += (double)hi[j];
+    for (int j = 0; j < 8; ++j) q[j] = (double)hi[j];
+    s[0] += ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
     if (RES && n > 0) store_run8(static_cast<RT*>(a.h) + base + c, n, hi);
   }
   row_sums<TPR>(s, red64);
