@@ -628,7 +628,7 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_dz(const Head
       if (a.dlogp != nullptr && head_real(a.target, n, a.V)) co -= a.dlogp[n];
       const float lse = a.lse[n];
       far = far || head_far(lse);
-      off[j] = (head_far(lse) ? lse - lse : lse * kLog2e) - __log2f(fabsf(co));   // (lse - lse: NaN stays NaN)
+      if (co != 0.0f) off[j] = (head_far(lse) ? lse - lse : lse * kLog2e) - __log2f(fabsf(co));   // (lse - lse: NaN stays NaN)
       neg[j] = __float_as_uint(co) & 0x80000000u;
     }
   }
@@ -653,7 +653,8 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_dz(const Head
 #pragma unroll
             for (int i = 0; i < S::MT; ++i)
 #pragma unroll
-              for (int r = 0; r < 16; ++r) acc[i][j][r] = fminf(acc[i][j][r] - from, most);
+              for (int r = 0; r < 16; ++r)   // (a row without weight has no gradient, whatever its logits)
+                acc[i][j][r] = off[j] == __builtin_inff() ? 0.0f : fminf(acc[i][j][r] - from, most);
           }
         }
         // else zeros past the vocabulary, and in the rows past N (of any sums, NaN among them)
@@ -721,6 +722,7 @@ __global__ __launch_bounds__(256) void k_head_target(const HeadDz a, const float
   const int64_t v = a.target[n] - a.v0;
   if (v < 0 || v >= a.vocab) return;
   const float b = a.dlogp[n], dl = a.dlse != nullptr ? a.dlse[n] : 0.0f, lp = logp[n];
+  if (b == 0.0f && dl == 0.0f) return;   // (0 already)
   // (dlse - b) p + b with 1 - p from expm1: within a few 2^-24 as logp is, not of the size of the logits
   float d = dl * expf(lp) - b * expm1f(lp);
   E* p = static_cast<E*>(a.dz) + n * a.ld + v;

@@ -175,8 +175,10 @@ def linear_logprobs(x, weight, targets=None):
     gradient.  At most 2^22 rows.
 
     Every finite logit counts, whatever its size.  A row with NaN or plus infinity among
-    its logits, or with minus infinity alone, is NaN.  The backward's probabilities are
-    formed from ``lse`` as float32 holds it: within ``|lse| 2^-23`` of their size."""
+    its logits, or with minus infinity alone, is NaN, and so is its gradient where it has
+    one (an ignored row's is 0; ``weight``'s sums that 0 times the row of x).  The backward's
+    probabilities are formed from ``lse`` as float32 holds it: within ``|lse| 2^-23`` of
+    their size."""
     f = L.torch_side().linear_logprobs
     if _ops._TIMER is None:
         return LinearLogprobs(*f(x, weight, targets))

@@ -115,3 +115,38 @@ def test_infinite_logits():
         w[250, 0] = float("inf")
         got = nsa_lm.linear_logprobs(x, w, t)
         assert got.lse.isnan().all() and got.logp.isnan().all()
+
+
+@pytest.mark.parametrize("N", [5, 60, 200, 2100])
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_ignored_rows_have_no_gradient_whatever_their_logits(N, dtype):
+    """Rows whose products pass float32 (x is finite), and rows with NaN: 0 where they are ignored
+    or their results' gradients are 0; the other rows' gradients are as without them."""
+    import nsa_lm
+    dev = require_gpu()
+    V, D = 5300 if N > 2000 else 300, 64
+    g = torch.Generator().manual_seed(N)
+    x, w = torch.randn(N, D, generator=g).to(dtype).to(dev), torch.randn(V, D, generator=g).to(dtype).to(dev)
+    t = torch.randint(0, V, (N,), generator=g).to(dev)
+    dlogp = -torch.rand(N, generator=g).to(dev)
+    bad = torch.zeros(N, dtype=torch.bool, device=dev)
+    bad[1::3] = True
+    t[bad] = -100
+    last = int(bad.nonzero()[-1])
+    t[last], dlogp[last] = 7, 0.0                                  # not ignored, of no weight
+
+    def grads(x):
+        xs, ws = x.clone().requires_grad_(), w.clone().requires_grad_()
+        r = nsa_lm.linear_logprobs(xs, ws, t)
+        return r, torch.autograd.grad(r.logp, (xs, ws), dlogp)
+    tame = x.clone()
+    tame[bad] = 0
+    _, (dx0, dw0) = grads(tame)
+    wild = tame.clone()
+    wild[bad] = 3e38
+    r, (dx, dw) = grads(wild)
+    assert not r.lse[bad].isfinite().any() and r.lse[~bad].isfinite().all()
+    assert torch.equal(dx, dx0) and torch.equal(dw, dw0)
+    wild[bad] = float("nan")
+    r, (dx, _) = grads(wild)
+    assert r.lse[bad].isnan().all() and torch.equal(dx, dx0)
