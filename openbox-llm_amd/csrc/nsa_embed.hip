@@ -21,10 +21,15 @@
 //      table is written once.
 //   3. The parts of every cut run are added in the order of the pieces.
 //
+// The same lists give sums of weighted rows by token (nsa_token_sums), for the gradient of a head's
+// weights: a token's sum then lies at its run's place in the sorted list, not at the token.
+//
 // Measured: 8 x 4096 rows of 768 in float32 with their positions, table of 32000: 38 us
 // forward (300 MB less what the caches hold of the table; a copy's rate is 5.4 TB/s); 49 for
 // the tokens' sums (200 MB, 4.1 TB/s), 20 for their sort (four launches of one dependent
 // chain each), 11 for the joins, 18 for the positions' sums. 8191 x 4096 bf16 rows: 22 us.
+#include <utility>
+
 #include "nsa_launch.h"
 #include "nsa_rows.h"
 
@@ -375,6 +380,9 @@ struct EmbedGrad {
   int D, len, pieces;          // len: pairs a piece
   float scale;
   bool dy_bf16, w_bf16;
+  const float* weight;         // [n], sums by token: of every row; dw then has a row a pair, a run's at its first pair
+  int* first;                  // [V], sums by token: a token's first pair, of those that have one,
+  uint64_t* there;             // ... whose bits these are
   // (fewer than 2^31 pairs: 32-bit divisions)
   __device__ __forceinline__ uint32_t key_at(int64_t s) const { return key != nullptr ? key[s] : (uint32_t)s / B; }
   __device__ __forceinline__ uint32_t row_at(int64_t s) const {
@@ -390,8 +398,8 @@ __device__ __forceinline__ void embed_store(const EmbedGrad& a, int64_t at, int 
   store_some<E>(a.dw, a.w_bf16, at, n, o);
 }
 
-// Clear the rows r0 .. r0 + 63 that have no token, columns c ..
-template <int E>
+// Clear the rows r0 .. r0 + 63 that have no token, columns c ..  SUMS: note these tokens' first pairs.
+template <int E, bool SUMS>
 __device__ __forceinline__ void embed_clear(const EmbedGrad& a, int64_t r0, int c) {
   const int n = a.D - c;
   const int64_t v = r0 + (threadIdx.x & 63);
@@ -406,6 +414,12 @@ __device__ __forceinline__ void embed_clear(const EmbedGrad& a, int64_t r0, int 
         hi = mid;
     }
     empty = lo >= a.n || a.key_at(lo) != (uint32_t)v;
+    if (SUMS && !empty && threadIdx.x < 64 && blockIdx.y == 0) a.first[v] = (int)lo;
+  }
+  if (SUMS) {
+    const uint64_t there = __ballot(v < a.V && !empty);
+    if (threadIdx.x == 0 && blockIdx.y == 0) a.there[r0 / 64] = there;
+    return;
   }
   uint64_t rows = __ballot(empty);   // (every wave of the workgroup: the same)
   if (n <= 0) return;
@@ -421,14 +435,15 @@ __device__ __forceinline__ void embed_clear(const EmbedGrad& a, int64_t r0, int 
 
 // Workgroups below a.pieces add the rows of a piece; the others clear the rows
 // without a token, 64 rows of the table at a time.  A thread owns E columns.
-template <int E>
+template <int E, bool SUMS>
 __global__ __launch_bounds__(256) void k_embed_runs(const EmbedGrad a) {
   __shared__ uint32_t keys[kRunRows + 1], rows[kRunRows];
+  __shared__ float weights[SUMS ? kRunRows : 1];
   const int tid = threadIdx.x, D = a.D;
   const int ct = ((int)blockIdx.y * (int)blockDim.x + tid) * E, c = ct < D ? run_start<E>(ct, D) : D, n = D - c;
   if ((int)blockIdx.x >= a.pieces) {
     for (int64_t r0 = ((int64_t)blockIdx.x - a.pieces) * 64; r0 < a.V; r0 += ((int64_t)gridDim.x - a.pieces) * 64)
-      embed_clear<E>(a, r0, c);
+      embed_clear<E, SUMS>(a, r0, c);
     return;
   }
   const int64_t s0 = (int64_t)blockIdx.x * a.len, s1 = s0 + a.len < a.n ? s0 + a.len : a.n;
@@ -439,11 +454,15 @@ __global__ __launch_bounds__(256) void k_embed_runs(const EmbedGrad a) {
 #pragma unroll
   for (int j = 0; j < E; ++j) acc[j] = 0.0f;
   bool head = a.key_at(s0) == k_prev;   // the run began in an earlier piece
+  int64_t start = s0;                   // ... else here
   for (int64_t s = s0; s < s1; s += kRunRows) {
     const int m = s1 - s < kRunRows ? (int)(s1 - s) : kRunRows;
     __syncthreads();
     if (tid <= m) keys[tid] = tid < m || s + m < s1 ? a.key_at(s + tid) : end;   // (the key behind each row; `end` behind the piece)
-    if (tid < m) rows[tid] = a.row_at(s + tid);
+    if (tid < m) {
+      rows[tid] = a.row_at(s + tid);
+      if (SUMS) weights[tid] = a.weight[rows[tid]];
+    }
     __syncthreads();
     if (n <= 0) continue;
     for (int u0 = 0; u0 < m; u0 += kAhead) {
@@ -457,15 +476,16 @@ __global__ __launch_bounds__(256) void k_embed_runs(const EmbedGrad a) {
         const uint32_t k = keys[u0 + u], kn = keys[u0 + u + 1];
         if (k == none) continue;
 #pragma unroll
-        for (int j = 0; j < E; ++j) acc[j] += v[u][j];
+        for (int j = 0; j < E; ++j) acc[j] = SUMS ? fmaf(weights[u0 + u], v[u][j], acc[j]) : acc[j] + v[u][j];
         if (kn == k) continue;
         if (head)
           store_some<E>(part, false, c, n, acc);
         else if (kn == end && k == k_next)   // the run goes on in the next piece
           store_some<E>(part, false, D + c, n, acc);
         else
-          embed_store<E>(a, (int64_t)k * D + c, n, acc);
+          embed_store<E>(a, (SUMS ? start : (int64_t)k) * D + c, n, acc);
         head = false;
+        start = s + u0 + u + 1;
 #pragma unroll
         for (int j = 0; j < E; ++j) acc[j] = 0.0f;
       }
@@ -476,6 +496,7 @@ __global__ __launch_bounds__(256) void k_embed_runs(const EmbedGrad a) {
 // The cut runs: a workgroup for each piece in which one begins and 256 columns.  Its waves
 // take kJoin parts each in turn, then the first adds the others' sums in order.
 constexpr int kJoin = 16, kJoinWaves = 4;
+template <bool SUMS>
 __global__ __launch_bounds__(64 * kJoinWaves) void k_embed_join(const EmbedGrad a) {
   __shared__ float sums[kJoinWaves - 1][4][64];
   const int lane = threadIdx.x & (kWave - 1), w = threadIdx.x / kWave, D = a.D;
@@ -522,7 +543,19 @@ __global__ __launch_bounds__(64 * kJoinWaves) void k_embed_join(const EmbedGrad 
         for (int j = 0; j < 4; ++j) acc[j] += sums[g][j][lane];
     }
   }
-  if (w == 0) embed_store<4>(a, (int64_t)k * D + c, n, acc);
+  int64_t at = k;
+  if (SUMS) {   // the run's first pair
+    int64_t lo = s0, hi = s1 - 1;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (a.key_at(mid) < k)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    at = lo;
+  }
+  if (w == 0) embed_store<4>(a, at * D + c, n, acc);
 }
 
 static bool embed_type(int dtype) { return dtype == NSA_F32 || dtype == NSA_BF16; }
@@ -537,9 +570,9 @@ static int sort_blocks(int64_t n) {
   return (int)((n + per - 1) / per);
 }
 // Pairs a piece: 8, more where the pieces would be more than 2048
-static int embed_piece(int64_t n) {
+static int embed_piece(int64_t n, int most = 2048) {
   int64_t len = 8;
-  while (n / len > 2048) len *= 2;
+  while (n / len > most) len *= 2;
   return (int)len;
 }
 struct EmbedPlan {
@@ -548,14 +581,54 @@ struct EmbedPlan {
   int len, pieces;
   size_t bytes() const { return (size_t)(4 * pairs + counts + parts) * 4; }
 };
-static EmbedPlan embed_plan(int64_t n, int D, bool sorted) {
+static EmbedPlan embed_plan(int64_t n, int D, bool sorted, int most = 2048) {
   EmbedPlan p;
   p.pairs = sorted ? (n + 3) / 4 * 4 : 0;
   p.counts = sorted ? sort_blocks(n) * kSortBins : 0;
-  p.len = embed_piece(n);
+  p.len = embed_piece(n, most);
   p.pieces = (int)((n + p.len - 1) / p.len);
   p.parts = (int64_t)p.pieces * 2 * D;
   return p;
+}
+
+// The workspace of such a plan: two buffers of pairs in turn, the sort's counts, the runs' parts.
+struct EmbedLists {
+  uint32_t *key, *val, *key2, *val2, *count;
+  float* part;
+  EmbedLists(void* ws, const EmbedPlan& p)
+      : key(static_cast<uint32_t*>(ws)), val(key + p.pairs), key2(val + p.pairs), val2(key2 + p.pairs), count(val2 + p.pairs),
+        part(reinterpret_cast<float*>(count + p.counts)) {}
+};
+
+// (index, i) sorted into key and val
+static void embed_sort(EmbedLists& at, const int64_t* index, int64_t n, int64_t V, hipStream_t s) {
+  int bits = 1;   // of the keys 0 .. V
+  while ((V >> bits) != 0) ++bits;
+  const int passes = (bits + kSortBits - 1) / kSortBits;
+  if (n <= kSmallSort) {
+    k_sort_small<<<1, 1024, 0, s>>>(index, at.key, at.val, (int)n, V, passes, bits);
+    return;
+  }
+  const unsigned blocks = (unsigned)sort_blocks(n);
+  for (int q = 0, shift = 0; q < passes; ++q) {
+    const int b = (bits - shift + passes - q - 1) / (passes - q);
+    const SortPass a{q == 0 ? index : nullptr, at.key, at.val, at.key2, at.val2, at.count, n, V, sort_per(n), shift, b};
+    k_sort_count<<<blocks, kSortThreads, 0, s>>>(a);
+    k_sort_move<<<blocks, kSortThreads, 0, s>>>(a);
+    shift += b;
+    std::swap(at.key, at.key2);
+    std::swap(at.val, at.val2);
+  }
+}
+
+template <int E, bool SUMS>
+static void embed_sums(const EmbedGrad& g, bool join, hipStream_t s) {
+  const int64_t clear = (g.V + 63) / 64;
+  const unsigned grid = (unsigned)(g.pieces + (clear < (1 << 16) ? clear : 1 << 16));
+  const int runs = (g.D + E - 1) / E, nth = runs >= 256 ? 256 : (runs + 63) / 64 * 64;
+  k_embed_runs<E, SUMS><<<dim3(grid, (unsigned)((runs + nth - 1) / nth)), nth, 0, s>>>(g);
+  if (g.pieces > 1 && join)
+    k_embed_join<SUMS><<<dim3((unsigned)(g.pieces - 1), (unsigned)((g.D + 255) / 256)), 64 * kJoinWaves, 0, s>>>(g);
 }
 
 }  // namespace nsa
@@ -627,43 +700,35 @@ extern "C" int nsa_embed_bwd(const int64_t* index, const void* dy, void* dw, voi
   NSA_CHECK(workspace != nullptr && workspace_bytes >= p.bytes(), NSA_ERR_WORKSPACE);
   NSA_CHECK(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, NSA_ERR_ARG);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  uint32_t* ws = static_cast<uint32_t*>(workspace);
-  uint32_t *ka = ws, *va = ka + p.pairs, *kb = va + p.pairs, *vb = kb + p.pairs, *count = vb + p.pairs;
-  float* part = reinterpret_cast<float*>(count + p.counts);
-  if (index != nullptr) {
-    int bits = 1;   // of the keys 0 .. V
-    while ((V >> bits) != 0) ++bits;
-    const int passes = (bits + kSortBits - 1) / kSortBits;
-    if (n <= kSmallSort) k_sort_small<<<1, 1024, 0, s>>>(index, ka, va, (int)n, V, passes, bits);
-    const unsigned blocks = (unsigned)sort_blocks(n);
-    for (int q = 0, shift = 0; n > kSmallSort && q < passes; ++q) {
-      const int b = (bits - shift + passes - q - 1) / (passes - q);
-      const SortPass a{q == 0 ? index : nullptr, ka, va, kb, vb, count, n, V, sort_per(n), shift, b};
-      k_sort_count<<<blocks, kSortThreads, 0, s>>>(a);
-      k_sort_move<<<blocks, kSortThreads, 0, s>>>(a);
-      shift += b;
-      uint32_t* t = ka;
-      ka = kb, kb = t;
-      t = va;
-      va = vb, vb = t;
-    }
-  }
+  EmbedLists at(workspace, p);
+  if (index != nullptr) embed_sort(at, index, n, V, s);
   // positions 0 .. T-1 of up to 64 sequences: whole runs a piece, none to join
   const int64_t B = index != nullptr ? 1 : n / T;
   const bool whole = index == nullptr && B <= 64;
   const int len = whole ? (int)((p.len + B - 1) / B * B) : p.len, pieces = (int)((n + len - 1) / len);
-  const EmbedGrad g{index != nullptr ? ka : nullptr, va, dy, dw, part, n, T, V, (uint32_t)B,
-                    D, len, pieces, scale, dy_dtype == NSA_BF16, w_dtype == NSA_BF16};
-  const int64_t clear = (V + 63) / 64;
-  const unsigned grid = (unsigned)(pieces + (clear < (1 << 16) ? clear : 1 << 16));
-  const int E = g.dy_bf16 ? 8 : 4, runs = (D + E - 1) / E;
-  const int nth = runs >= 256 ? 256 : (runs + 63) / 64 * 64;
-  const dim3 all(grid, (unsigned)((runs + nth - 1) / nth));
+  const EmbedGrad g{index != nullptr ? at.key : nullptr, at.val, dy, dw, at.part, n, T, V, (uint32_t)B,
+                    D, len, pieces, scale, dy_dtype == NSA_BF16, w_dtype == NSA_BF16, nullptr, nullptr, nullptr};
   if (g.dy_bf16)
-    k_embed_runs<8><<<all, nth, 0, s>>>(g);
+    embed_sums<8, false>(g, !whole, s);
   else
-    k_embed_runs<4><<<all, nth, 0, s>>>(g);
-  if (pieces > 1 && !whole)
-    k_embed_join<<<dim3((unsigned)(pieces - 1), (unsigned)((D + 255) / 256)), 64 * kJoinWaves, 0, s>>>(g);
+    embed_sums<4, false>(g, !whole, s);
+  return nsa_launch_status();
+}
+
+// (fewer and longer pieces of wide rows, which several workgroups share: 8192 x 4096 in 42 us, 52 with 1024 pieces;
+// 32768 x 768 in 33 with 2048, 59 with 512)
+static nsa::EmbedPlan token_sums_plan(int64_t n, int D) { return nsa::embed_plan(n, D, true, D > 2048 ? 512 : 2048); }
+
+size_t nsa_token_sums_workspace(int64_t n, int D) { return token_sums_plan(n, D).bytes(); }
+
+int nsa_token_sums(const int64_t* index, const float* weight, const void* rows, void* sums, int* first, uint64_t* there,
+                   void* workspace, int64_t n, int64_t V, int D, void* stream) {
+  using namespace nsa;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const EmbedPlan p = token_sums_plan(n, D);
+  EmbedLists at(workspace, p);
+  embed_sort(at, index, n, V, s);
+  const EmbedGrad g{at.key, at.val, rows, sums, at.part, n, 1, V, 1, D, p.len, p.pieces, 1.0f, true, true, weight, first, there};
+  embed_sums<8, true>(g, true, s);
   return nsa_launch_status();
 }

@@ -9,10 +9,13 @@
 //
 // Four products on the matrix instructions with float32 sums (bf16: 32x32x16): z for the
 // log sums (a running maximum and sum in registers), z again for dz, and the two
-// of the gradients.  dz exists for a piece of the vocabulary at a time; beside bf16 rows
-// it is rounded once to bf16 as the products' operand (the relative rounding of a
-// probability and of an operand are the same; a sum over the vocabulary or the rows
-// averages it), beside float32 rows it is float32 or its planes.
+// of the gradients.  dz exists for a piece of the vocabulary at a time; beside float32 rows it
+// is float32 or its planes, beside bf16 rows it is rounded once to bf16 as the products'
+// operand.  Most of both gradients is the target's own element, whose rounding no sum
+// averages: what it leaves, rest_n, goes to the results in float32, as rest_n W_{t_n} to
+// dx and, summed over a token's rows, as rest_n x_n to dW.  (Root of the squares' sum, 40 cases of 1 to
+// 19900 rows and 128 to 183000 tokens: both gradients are 1.00 times as far off 64 bits as their
+// rounding to bf16 makes them, 1.16 at most; 1.36 and up to 1.8 without the rests. 1 to 2% of the time of large calls.)
 //
 // float32 rows and weights of few rows go through v_mfma_f32_32x32x2_f32 as they are; of many
 // as three bf16 planes p0 + p1 + p2 = x, |x - p0 - p1 - p2| <= 2^-27 |x|: six products of
@@ -219,7 +222,8 @@ __device__ __forceinline__ void head_range(F&& f) {
   }
 }
 
-// The spans i = 0 .. spans - 1, `total` steps in all; done(span, wm, wn, acc) takes each result.
+// The spans i = 0 .. spans - 1, `total` steps in all; done(span, wm, wn, acc) takes each result,
+// begin(span, wn) may ask for what that needs.
 //
 // All steps of all spans are one pipeline of NS stages in LDS.  One or two waves a SIMD leave
 // the matrix unit idle wherever more than a few other instructions stand between two
@@ -229,8 +233,12 @@ __device__ __forceinline__ void head_range(F&& f) {
 // stages stands before the products of the last 16 elements of the older one, whose
 // fragments are in registers by then; its memory is requested anew from there on (the
 // last stages once more where there are none left, so that every step is alike).
-template <class S, bool AROWS, bool BROWS, typename Span, typename Done>
-__device__ __forceinline__ void head_product(const HeadProduct& pr, int spans, int total, Span span, Done done) {
+struct HeadNoBegin {
+  __device__ __forceinline__ void operator()(const HeadSpan&, int) const {}
+};
+template <class S, bool AROWS, bool BROWS, typename Span, typename Done, typename Begin = HeadNoBegin>
+__device__ __forceinline__ void head_product(const HeadProduct& pr, int spans, int total, Span span, Done done,
+                                             Begin begin = Begin()) {
   constexpr int kStep = S::kStep;
   typedef typename S::E E;
   typedef HeadType<E> Type;
@@ -357,6 +365,7 @@ __device__ __forceinline__ void head_product(const HeadProduct& pr, int spans, i
 #pragma unroll 1
   for (int sp = 0; sp < spans; ++sp) {
     const HeadSpan cur = span(sp);
+    begin(cur, wn);
     clear();
 #pragma unroll 1
     for (int left = cur.q1 - cur.q0; left > 0; --left) {
@@ -714,17 +723,23 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_dz(const Head
       });
 }
 
-// The target's own element, where the piece has it: a p_t + b.
+// The target's own element, a p_t + b, of a row that has one.
+__device__ __forceinline__ float head_target(float b, float dl, float lp) {
+  if (b == 0.0f && dl == 0.0f) return 0.0f;   // (whatever the row's logits)
+  // (dlse - b) p + b with 1 - p from expm1: within a few 2^-24 as logp is, not of the size of the logits
+  return dl * expf(lp) - b * expm1f(lp);
+}
+__device__ __forceinline__ float head_target(const HeadDz& a, const float* logp, int64_t n) {
+  return head_target(a.dlogp[n], a.dlse != nullptr ? a.dlse[n] : 0.0f, logp[n]);
+}
+// ... where the piece has it
 template <typename E, int PLANES>
 __global__ __launch_bounds__(256) void k_head_target(const HeadDz a, const float* logp) {
   const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (n >= a.N || a.dlogp == nullptr || !head_real(a.target, n, a.V)) return;
   const int64_t v = a.target[n] - a.v0;
   if (v < 0 || v >= a.vocab) return;
-  const float b = a.dlogp[n], dl = a.dlse != nullptr ? a.dlse[n] : 0.0f, lp = logp[n];
-  if (b == 0.0f && dl == 0.0f) return;   // (0 already)
-  // (dlse - b) p + b with 1 - p from expm1: within a few 2^-24 as logp is, not of the size of the logits
-  float d = dl * expf(lp) - b * expm1f(lp);
+  float d = head_target(a, logp, n);
   E* p = static_cast<E*>(a.dz) + n * a.ld + v;
 #pragma unroll
   for (int q = 0; q < PLANES; ++q) {
@@ -732,6 +747,202 @@ __global__ __launch_bounds__(256) void k_head_target(const HeadDz a, const float
     p[q * a.plane] = o;
     d -= (float)o;
   }
+}
+
+// What its rounding to bf16 leaves of it, and its token; 0 and -1 without one.
+__global__ __launch_bounds__(256) void k_head_rest(const HeadDz a, const float* logp, float* rest, int* token) {
+  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (n >= a.N) return;
+  const bool real = head_real(a.target, n, a.V);
+  const float d = real ? head_target(a, logp, n) : 0.0f;
+  rest[n] = d - (float)(bf16)d;
+  token[n] = real ? (int)a.target[n] : -1;
+}
+
+// Both for up to 1024 rows of x, and the rests' sums by token, in one launch: the sort, sums and joins of
+// more rows would take 20 us beside the products of few rows (512 rows of W 8192 x 1024: 9 us of 91).  A workgroup takes 16 rows, each by a
+// wave; the first row of a token sums them all, a wave those of a token of few rows, the workgroup those of one of
+// many.  sums[n] where n is such a row; first[t_n] = n, and other tokens' `first` is left as it was: `there`
+// has the tokens' bits, 65536 of them a workgroup.
+constexpr int kFewRows = 1024, kFewThreads = 1024, kFewWaves = kFewThreads / 64, kFewAlone = 8;
+constexpr int kFewBits = 1 << 16;
+struct HeadFewRows {
+  HeadDz z;
+  const float* logp;
+  const bf16* x;
+  float* rest;
+  int* token;
+  bf16* sums;          // null: no sums
+  int* first;
+  uint64_t* there;     // [V rounded up to 256, / 64]
+  int D;
+};
+__global__ __launch_bounds__(kFewThreads) void k_head_few(const HeadFewRows a) {
+  constexpr int kPer = kFewRows / kFewThreads, kWords = kFewRows / 64;
+  __shared__ int token[kFewRows];
+  __shared__ float weight[kFewRows];
+  __shared__ uint64_t same[kFewWaves][kWords];   // of the wave's row: the rows of its token, 64 a word
+  __shared__ int count[kFewWaves];               // ... how many, 0 but for its first
+  __shared__ float part[kFewWaves][512];
+  unsigned* const bits = reinterpret_cast<unsigned*>(part);
+  static_assert(sizeof(part) >= kFewBits / 8, "a workgroup's bits");
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, N = a.z.N, D = a.D;
+  const int words = (N + 63) / 64, n = (int)blockIdx.x * kFewWaves + w;
+  // all that one waits for at once: the rows' numbers, and the wave's own row of x
+  constexpr int kOwn = 2;
+  bf16x8u own[kOwn];
+#pragma unroll
+  for (int u = 0; u < kOwn; ++u) {
+    const int c = 8 * (64 * u + lane);
+    if (n < N && c + 8 <= D) own[u] = *reinterpret_cast<const bf16x8u*>(a.x + (int64_t)n * D + c);
+  }
+  int64_t t[kPer];
+  float b[kPer], dl[kPer], lp[kPer];
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
+    const int i = u * kFewThreads + tid;
+    t[u] = i < N ? a.z.target[i] : -1;
+    b[u] = i < N ? a.z.dlogp[i] : 0.0f;
+    dl[u] = i < N && a.z.dlse != nullptr ? a.z.dlse[i] : 0.0f;
+    lp[u] = i < N ? a.logp[i] : 0.0f;
+  }
+  const int64_t bit0 = (int64_t)blockIdx.x * kFewBits;
+  const bool has_bits = bit0 < a.z.V;
+  if (has_bits)
+    for (int i = tid; i < kFewBits / 32; i += kFewThreads) bits[i] = 0;
+#pragma unroll
+  for (int u = 0; u < kPer; ++u) {
+    const int i = u * kFewThreads + tid;
+    if (u * kFewThreads >= N) break;
+    const bool real = t[u] >= 0 && t[u] < a.z.V;
+    const float d = real ? head_target(b[u], dl[u], lp[u]) : 0.0f;
+    const bf16 o = (bf16)d;
+    token[i] = real ? (int)t[u] : -1;
+    weight[i] = d - (float)o;
+    if (i < N && i / kFewWaves == (int)blockIdx.x) {
+      a.rest[i] = d - (float)o;
+      a.token[i] = real ? (int)t[u] : -1;
+      const int64_t v = t[u] - a.z.v0;
+      if (real && v >= 0 && v < a.z.vocab) static_cast<bf16*>(a.z.dz)[i * a.z.ld + v] = o;
+    }
+  }
+  if (a.sums == nullptr) return;
+  __syncthreads();
+  if (has_bits) {   // the tokens that are there, of this workgroup's
+    for (int i = tid; i < N; i += kFewThreads) {
+      const int64_t v = token[i] - bit0;
+      if (token[i] >= 0 && v >= 0 && v < kFewBits) atomicOr(&bits[v / 32], 1u << (v & 31));
+    }
+  }
+  const int mine = n < N ? token[n] : -1;
+  int found = 0;
+  if (mine >= 0) {   // (uniform over the wave)
+    bool before = false;
+#pragma unroll 8
+    for (int k = 0; k < words; ++k) {
+      const uint64_t m = __ballot(64 * k + lane < N && token[64 * k + lane] == mine);
+      before = before || (64 * k + 63 < n ? m : 64 * k > n ? 0 : m & ((1ull << (n & 63)) - 1ull)) != 0;
+      found += __popcll(m);
+      if (lane == 0) same[w][k] = m;
+    }
+    if (before) found = 0;
+    if (lane == 0 && found > 0) a.first[mine] = n;
+  }
+  if (lane == 0) count[w] = found;
+  __syncthreads();
+  if (has_bits) {
+    const int64_t all = ((int64_t)a.z.V + 255) / 256 * 4, at = bit0 / 64;
+    for (int i = tid; i < kFewBits / 64 && at + i < all; i += kFewThreads)
+      a.there[at + i] = (uint64_t)bits[2 * i + 1] << 32 | bits[2 * i];
+  }
+  // the rows of `m` (rows 64 k ..), in order, 8 columns a lane from c on
+  auto add = [&](float(&acc)[8], uint64_t m, int k, int c) {
+    while (m != 0) {
+      float v[4][8], f[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int r = 64 * k + (m != 0 ? __builtin_ctzll(m) : 0);
+        f[u] = m != 0 ? weight[r] : 0.0f;
+        load_run8(a.x + (int64_t)r * D + c, m != 0 ? D - c : 0, v[u]);
+        m &= m - 1;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = fmaf(f[u], v[u][j], acc[j]);
+    }
+  };
+  if (found == 1) {
+    const float f = weight[n];
+    auto store = [&](int c, float(&v)[8]) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= f;
+      store_run8(a.sums + (int64_t)n * D + c, D - c, v);
+    };
+#pragma unroll
+    for (int u = 0; u < kOwn; ++u) {
+      const int c = 8 * (64 * u + lane);
+      if (c >= D) continue;
+      float v[8];
+      if (c + 8 <= D) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (float)own[u][j];
+      } else {
+        load_run8(a.x + (int64_t)n * D + c, D - c, v);
+      }
+      store(c, v);
+    }
+#pragma unroll 4
+    for (int c = 8 * (64 * kOwn + lane); c < D; c += 512) {
+      float v[8];
+      load_run8(a.x + (int64_t)n * D + c, D - c, v);
+      store(c, v);
+    }
+  } else if (found > 0 && found <= kFewAlone) {
+    for (int c = 8 * lane; c < D; c += 512) {
+      float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      for (int k = n / 64; k < words; ++k) add(acc, same[w][k], k, c);
+      store_run8(a.sums + (int64_t)n * D + c, D - c, acc);
+    }
+  }
+  uint64_t many = __ballot(lane < kFewWaves && count[lane & (kFewWaves - 1)] > kFewAlone);   // (every wave: the same)
+  while (many != 0) {
+    const int q = __builtin_ctzll(many);
+    many &= many - 1;
+    const int64_t row = (int64_t)blockIdx.x * kFewWaves + q;
+    for (int c0 = 0; c0 < D; c0 += 512) {
+      float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (c0 + 8 * lane < D)
+        for (int k = w; k < words; k += kFewWaves) add(acc, same[q][k], k, c0 + 8 * lane);
+      __syncthreads();   // (`part` is read no more)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) part[w][8 * lane + j] = acc[j];
+      __syncthreads();
+      const int c = c0 + tid;
+      if (tid < 512 && c < D) {
+        float t = 0.0f;
+        for (int k = 0; k < kFewWaves; ++k) t += part[k][tid];
+        a.sums[row * D + c] = (bf16)t;
+      }
+    }
+  }
+}
+
+// Rows of bf16 that go to the results' rows beside the products: W_{t_n} with the weight rest_n to row n
+// of dx, the sum of a token's rest_n x_n (rounded to bf16: of a part that is 2^-8 of the whole) to its row of dW.
+struct HeadMore {
+  const bf16* rows;          // null: none
+  int64_t ld;
+  const int* token;          // dx: of every row, or -1
+  const float* weight;
+  const int* first;          // dW: a token's row,
+  const uint64_t* there;     // ... of the tokens that have one: a bit each
+};
+// The bits of 32 tokens from n0 (the same in a wave) on, by a scalar load: a vector load would wait for the product's
+// requests ahead of it, also where no token has a row.
+__device__ __forceinline__ uint32_t head_there(const HeadMore& a, int64_t n0) {
+  typedef const __attribute__((address_space(4))) uint32_t* Words;
+  return ((Words)(uintptr_t)a.there)[__builtin_amdgcn_readfirstlane((int)(n0 / 32))];
 }
 
 // dx (rows of x on n, columns of W on m) and dW (tokens on n, columns of x on m).  The
@@ -748,6 +959,7 @@ struct HeadGrad {
   int N, D, m_tiles, n_tiles, groups;
   int whole, cuts;       // tiles taken whole, a multiple of groups
   bool out_bf16;
+  HeadMore more;
 };
 
 template <class S, bool BROWS>
@@ -774,6 +986,25 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_grad(const He
   }
   if (total == 0) return;
   const int lane = threadIdx.x & 63, h = lane >> 5;
+  constexpr bool kMore = sizeof(typename S::E) == 2;   // (float32 operands: none)
+  // asked for a tile ahead: dx: the rows' tokens and weights; dW: the tokens' bits
+  int token[S::NT];
+  float weight[S::NT];
+  uint32_t there[S::NT];
+  const bool more = kMore && a.more.rows != nullptr;
+  auto begin = [&](const HeadSpan& sp, int wn) {
+    if (!more) return;
+#pragma unroll
+    for (int j = 0; j < S::NT; ++j) {
+      const int64_t n0 = (int64_t)sp.n * S::TN + wn + 32 * j, n = n0 + (lane & 31) < a.N ? n0 + (lane & 31) : a.N - 1;
+      if (BROWS) {
+        token[j] = a.more.token[n];
+        weight[j] = a.more.weight[n];
+      } else {
+        there[j] = head_there(a.more, n0 < a.N ? n0 : 0);
+      }
+    }
+  };
   head_product<S, false, BROWS>(
       a.pr, spans, total, span, [&](const HeadSpan& sp, int wm, int wn, f32x16(&acc)[S::MT][S::NT]) {
         const int t = sp.n * a.m_tiles + sp.m;
@@ -783,54 +1014,87 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_grad(const He
           part = a.part + ((int64_t)c * rest + t - a.whole) * S::TM * S::TN;
         }
         if (part == nullptr && sp.m * S::TM + S::TM > a.D) part = a.part + ((int64_t)units + sp.n) * S::TM * S::TN;
-        // a lane's runs of a row: 32 i + 2 r0 elements from its first one on
-        auto each = [&](auto to, auto put) {
+        // a lane's runs of a row: 32 i + 2 r0 elements from its first one on, two tiles' at a time
+        constexpr int kAhead = S::MT % 2 == 0 ? 4 : 2;
+        auto each = [&](auto to, auto ask, auto put) {
 #pragma unroll
           for (int j = 0; j < S::NT; ++j) {
             const int c = wn + 32 * j + (lane & 31);
             if (sp.n * (int64_t)S::TN + c >= a.N) continue;
-            const auto at = to(c, wm + 8 * h);
+            const auto at = to(c, wm + 8 * h, j);
 #pragma unroll
-            for (int i = 0; i < S::MT; ++i)
+            for (int k0 = 0; k0 < 2 * S::MT; k0 += kAhead) {
+              bf16x8u u[kAhead];
 #pragma unroll
-              for (int r0 = 0; r0 < 16; r0 += 8) {
+              for (int k = 0; k < kAhead; ++k) ask(at, 16 * (k0 + k), u[k]);
+              __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+              for (int k = 0; k < kAhead; ++k) {
                 float v[8];
 #pragma unroll
-                for (int r = 0; r < 8; ++r) v[r] = acc[i][j][r0 + r];
-                put(at, 32 * i + 2 * r0, v);
+                for (int r = 0; r < 8; ++r) v[r] = acc[(k0 + k) / 2][j][8 * (k & 1) + r];
+                put(at, 16 * (k0 + k), u[k], v);
                 __builtin_amdgcn_sched_barrier(0);   // (few of the results in other registers at a time)
               }
+            }
           }
         };
-        auto in_out = [&](int c, int e) {
-          return ((int64_t)sp.n * S::TN + c) * a.D + sp.m * S::TM + e;
+        struct At {
+          int64_t at;
+          const bf16* more;
+          float weight;
+          bool some;   // the wave has any
         };
-        auto added = [&](int64_t at, int o, float(&v)[8]) {
-          float u[8];
-          load_run8(a.add + at + o, u);
+        auto in_out = [&](int c, int e, int j) {
+          At to{((int64_t)sp.n * S::TN + c) * a.D + sp.m * S::TM + e, nullptr, 0.0f, false};
+          if (more && (BROWS || there[j] != 0)) {
+            to.some = true;
+            int row = -1;
+            if (BROWS)
+              row = token[j];
+            else if ((there[j] >> (lane & 31)) & 1u)
+              row = a.more.first[(int64_t)sp.n * S::TN + c];
+            if (row >= 0) to.more = a.more.rows + row * a.more.ld + sp.m * S::TM + e;
+            to.weight = BROWS ? weight[j] : 1.0f;
+          }
+          return to;
+        };
+        auto ask = [&](const At& to, int o, bf16x8u& u) {
+          if (to.some && to.more != nullptr) u = *reinterpret_cast<const bf16x8u*>(to.more + o);
+        };
+        auto added = [&](const At& to, int o, const bf16x8u& u, float(&v)[8]) {
+          if (a.add != nullptr) {
+            float f[8];
+            load_run8(a.add + to.at + o, f);
 #pragma unroll
-          for (int r = 0; r < 8; ++r) v[r] += u[r];
+            for (int r = 0; r < 8; ++r) v[r] += f[r];
+          }
+          if (to.some && to.more != nullptr) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r) v[r] = fmaf(to.weight, (float)u[r], v[r]);
+          }
         };
         if (part != nullptr) {
-          each([&](int c, int e) { return part + c * S::TM + e; },
-               [&](float* at, int o, float(&v)[8]) { store_run8(at + o, v); });
+          each([&](int c, int e, int) { return part + c * S::TM + e; }, [](float*, int, bf16x8u&) {},
+               [&](float* at, int o, const bf16x8u&, float(&v)[8]) { store_run8(at + o, v); });
         } else if (a.out_bf16) {
-          each(in_out, [&](int64_t at, int o, float(&v)[8]) {
-            if (a.add != nullptr) added(at, o, v);
-            store_run8(static_cast<bf16*>(a.out) + at + o, v);
+          each(in_out, ask, [&](const At& to, int o, const bf16x8u& u, float(&v)[8]) {
+            added(to, o, u, v);
+            store_run8(static_cast<bf16*>(a.out) + to.at + o, v);
           });
         } else {
-          each(in_out, [&](int64_t at, int o, float(&v)[8]) {
-            if (a.add != nullptr) added(at, o, v);
-            store_run8(static_cast<float*>(a.out) + at + o, v);
+          each(in_out, ask, [&](const At& to, int o, const bf16x8u& u, float(&v)[8]) {
+            added(to, o, u, v);
+            store_run8(static_cast<float*>(a.out) + to.at + o, v);
           });
         }
-      });
+      },
+      begin);
 }
 
 // The cut tiles' parts in order, and the tiles at the rows' ends.  Eight workgroups a
 // tile, a thread 8 elements at a time.
-template <class S>
+template <class S, bool DX>
 __global__ __launch_bounds__(256) void k_head_join_tiles(const HeadGrad a, int first) {
   const int t = first + (int)blockIdx.x, rest = a.m_tiles * a.n_tiles - a.whole;
   const int m0 = (t % a.m_tiles) * S::TM;
@@ -857,6 +1121,19 @@ __global__ __launch_bounds__(256) void k_head_join_tiles(const HeadGrad a, int f
       load_run8(a.add + n * a.D + d, a.D - d, u);
 #pragma unroll
       for (int r = 0; r < 8; ++r) v[r] += u[r];
+    }
+    if (a.more.rows != nullptr) {
+      int row = -1;
+      if (DX)
+        row = a.more.token[n];
+      else if ((reinterpret_cast<const uint32_t*>(a.more.there)[n / 32] >> (n & 31)) & 1u)
+        row = a.more.first[n];
+      if (row >= 0) {
+        const float weight = DX ? a.more.weight[n] : 1.0f;
+        load_run8(a.more.rows + row * a.more.ld + d, a.D - d, u);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) v[r] = fmaf(weight, u[r], v[r]);
+      }
     }
     if (a.out_bf16)
       store_run8(static_cast<bf16*>(a.out) + n * a.D + d, a.D - d, v);
@@ -1056,7 +1333,7 @@ static void head_grad_as(HeadGrad g, const HeadCut& c, hipStream_t s) {
   g.cuts = c.cuts;
   k_head_grad<S, BROWS><<<(unsigned)g.groups, S::kThreads, 0, s>>>(g);
   const int tiles = g.m_tiles * g.n_tiles, first = g.D % S::TM != 0 ? 0 : c.cuts > 1 ? c.whole : tiles;
-  if (first < tiles) k_head_join_tiles<S><<<dim3((unsigned)(tiles - first), 8), 256, 0, s>>>(g, first);
+  if (first < tiles) k_head_join_tiles<S, BROWS><<<dim3((unsigned)(tiles - first), 8), 256, 0, s>>>(g, first);
 }
 template <bool BROWS>
 static void head_grad(const HeadGrad& g, bool native, int cu, hipStream_t s) {
@@ -1076,6 +1353,10 @@ static void head_grad(const HeadGrad& g, bool native, int cu, hipStream_t s) {
 struct HeadPlan {
   int piece;            // tokens of a piece, a multiple of 256
   size_t dz, acc, part; // bytes
+  size_t rest, sums, first, there, lists;   // of the targets' rests (and tokens), their sums by token and what forms those
+  size_t bytes(const HeadLayout& l) const {
+    return l.x_bytes + l.w_bytes + dz + acc + part + rest + sums + first + there + lists;
+  }
 };
 static HeadPlan head_plan(int64_t N, int V, int D, const HeadLayout& l, bool x_bf16, int cu) {
   HeadPlan p;
@@ -1098,6 +1379,11 @@ static HeadPlan head_plan(int64_t N, int V, int D, const HeadLayout& l, bool x_b
     parts = dw > parts ? dw : parts;
   }
   p.part = (size_t)parts;
+  p.rest = x_bf16 ? up16((size_t)N * 8) : 0;
+  p.sums = x_bf16 ? up16((size_t)N * D * 2) : 0;
+  p.first = x_bf16 ? up16((size_t)V * 4) : 0;
+  p.there = x_bf16 ? up16((size_t)all / 8) : 0;
+  p.lists = x_bf16 && N > kFewRows ? nsa_token_sums_workspace(N, D) : 0;
   return p;
 }
 
@@ -1166,7 +1452,7 @@ extern "C" size_t nsa_head_bwd_workspace(int64_t N, int V, int D, int x_dtype, i
   const int cu = device_cu_count(static_cast<hipStream_t>(stream));
   const HeadLayout l = head_layout(N, V, D, at, at, x_dtype, w_dtype, kNativeBwd, cu);
   const HeadPlan p = head_plan(N, V, D, l, x_dtype == NSA_BF16, cu);
-  return l.x_bytes + l.w_bytes + p.dz + p.acc + p.part;
+  return p.bytes(l);
 }
 
 extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target, const float* logp, const float* lse,
@@ -1181,8 +1467,7 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
   const int cu = device_cu_count(s);
   const HeadLayout l = head_layout(N, V, D, x, w, x_dtype, w_dtype, kNativeBwd, cu);
   const HeadPlan p = head_plan(N, V, D, l, x_dtype == NSA_BF16, cu);
-  NSA_CHECK(workspace != nullptr && workspace_bytes >= l.x_bytes + l.w_bytes + p.dz + p.acc + p.part,
-            NSA_ERR_WORKSPACE);
+  NSA_CHECK(workspace != nullptr && workspace_bytes >= p.bytes(l), NSA_ERR_WORKSPACE);
   NSA_CHECK(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, NSA_ERR_ARG);
   char* ws = static_cast<char*>(workspace);
   char* const xp = ws;
@@ -1194,8 +1479,34 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
   float* acc = reinterpret_cast<float*>(ws);
   ws += p.acc;
   float* part = reinterpret_cast<float*>(ws);
+  ws += p.part;
+  float* rest = reinterpret_cast<float*>(ws);
+  int* token = reinterpret_cast<int*>(rest + N);
+  ws += p.rest;
+  char* const sums = ws;
+  ws += p.sums;
+  int* first = reinterpret_cast<int*>(ws);
+  ws += p.first;
+  uint64_t* there = reinterpret_cast<uint64_t*>(ws);
+  ws += p.there;
   if (l.pack_x) head_pack(x, x_dtype, xp, N, D, l.ld, l.px, l.native, s);
   if (l.pack_w) head_pack(w, w_dtype, wp, V, D, l.ld, l.pw, l.native, s);
+  const unsigned rows = (unsigned)((N + 255) / 256);
+  // the targets' rests: of few rows with the targets' elements of the first piece, else here
+  const bool rests = x_dtype == NSA_BF16 && dlogp != nullptr, few = rests && N <= kFewRows;
+  if (rests && !few) {
+    HeadDz z{};
+    z.dlogp = dlogp;
+    z.dlse = dlse;
+    z.target = target;
+    z.N = (int)N;
+    z.V = V;
+    k_head_rest<<<rows, 256, 0, s>>>(z, logp, rest, token);
+    if (dw != nullptr) {
+      const int rc = nsa_token_sums(target, rest, x, sums, first, there, ws, N, V, D, stream);
+      if (rc != NSA_OK) return rc;
+    }
+  }
   const int ldx = l.pack_x ? l.ld : D, ldw = l.pack_w ? l.ld : D;
   const void* X = l.pack_x ? xp : x;
   const char* W = l.pack_w ? wp : static_cast<const char*>(w);
@@ -1235,8 +1546,12 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
       form(HeadBig<bf16>{});
     else
       form(HeadMid<bf16>{});
-    const unsigned rows = (unsigned)((N + 255) / 256);
-    if (l.native)
+    if (few && v0 == 0) {
+      const HeadFewRows f{z, logp, static_cast<const bf16*>(x), rest, token, dw != nullptr ? reinterpret_cast<bf16*>(sums) : nullptr,
+                          first, there, D};
+      const int64_t own = (N + kFewWaves - 1) / kFewWaves, bits = dw != nullptr ? ((int64_t)V + kFewBits - 1) / kFewBits : 0;
+      k_head_few<<<(unsigned)(own > bits ? own : bits), kFewThreads, 0, s>>>(f);
+    } else if (l.native)
       k_head_target<float, 1><<<rows, 256, 0, s>>>(z, logp);
     else if (l.px == 3)
       k_head_target<bf16, 3><<<rows, 256, 0, s>>>(z, logp);
@@ -1252,6 +1567,7 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
       g.part = part;
       g.N = (int)N;
       g.D = D;
+      g.more = {rests && last ? reinterpret_cast<const bf16*>(W) : nullptr, ldw, token, rest, nullptr, nullptr};
       head_grad<true>(g, l.native, cu, s);
     }
     if (dw != nullptr) {
@@ -1263,6 +1579,7 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
       g.part = part;
       g.N = vocab;
       g.D = D;
+      g.more = {rests ? reinterpret_cast<const bf16*>(sums) : nullptr, D, nullptr, nullptr, first + v0, there + v0 / 64};
       head_grad<false>(g, l.native, cu, s);
     }
   }
