@@ -21,8 +21,8 @@
 //      table is written once.
 //   3. The parts of every cut run are added in the order of the pieces.
 //
-// The same lists give sums of weighted rows by token (nsa_token_sums), for the gradient of a head's
-// weights: a token's sum then lies at its run's place in the sorted list, not at the token.
+// The same lists give sums of weighted rows by token (nsa_token_sums), for the gradient of
+// a head's weights: a token's sum then lies at its run's place in the sorted list.
 //
 // Measured: 8 x 4096 rows of 768 in float32 with their positions, table of 32000: 38 us
 // forward (300 MB less what the caches hold of the table; a copy's rate is 5.4 TB/s); 49 for
@@ -596,7 +596,11 @@ struct EmbedLists {
   uint32_t *key, *val, *key2, *val2, *count;
   float* part;
   EmbedLists(void* ws, const EmbedPlan& p)
-      : key(static_cast<uint32_t*>(ws)), val(key + p.pairs), key2(val + p.pairs), val2(key2 + p.pairs), count(val2 + p.pairs),
+      : key(static_cast<uint32_t*>(ws)),
+        val(key + p.pairs),
+        key2(val + p.pairs),
+        val2(key2 + p.pairs),
+        count(val2 + p.pairs),
         part(reinterpret_cast<float*>(count + p.counts)) {}
 };
 
@@ -715,8 +719,8 @@ extern "C" int nsa_embed_bwd(const int64_t* index, const void* dy, void* dw, voi
   return nsa_launch_status();
 }
 
-// (fewer and longer pieces of wide rows, which several workgroups share: 8192 x 4096 in 42 us, 52 with 1024 pieces;
-// 32768 x 768 in 33 with 2048, 59 with 512)
+// (fewer and longer pieces of wide rows, which several workgroups share: 8192 x 4096 in 40 us,
+// 52 with 1024 pieces; 32768 x 768 in 31 with 2048, 59 with 512)
 static nsa::EmbedPlan token_sums_plan(int64_t n, int D) { return nsa::embed_plan(n, D, true, D > 2048 ? 512 : 2048); }
 
 size_t nsa_token_sums_workspace(int64_t n, int D) { return token_sums_plan(n, D).bytes(); }
@@ -728,7 +732,8 @@ int nsa_token_sums(const int64_t* index, const float* weight, const void* rows, 
   const EmbedPlan p = token_sums_plan(n, D);
   EmbedLists at(workspace, p);
   embed_sort(at, index, n, V, s);
-  const EmbedGrad g{at.key, at.val, rows, sums, at.part, n, 1, V, 1, D, p.len, p.pieces, 1.0f, true, true, weight, first, there};
+  const EmbedGrad g{at.key, at.val, rows,     sums, at.part, n,    1,      V,     1,
+                    D,      p.len,  p.pieces, 1.0f, true,    true, weight, first, there};
   embed_sums<8, true>(g, true, s);
   return nsa_launch_status();
 }

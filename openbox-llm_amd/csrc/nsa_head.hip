@@ -43,8 +43,9 @@ namespace nsa {
 constexpr int64_t kHeadRows = 1 << 22;       // most rows of x
 constexpr int kHeadVocab = 1 << 24;
 constexpr int kHeadWide = 1 << 16;           // widest row
-constexpr size_t kHeadPiece = 1u << 30;      // bytes of dz held at a time: the backward of 32768 x 32000 x d768 takes 4.55 ms, 5.03
-                                             // with half of them (the parts of dx and more partial rounds), 4.36 in one piece
+constexpr size_t kHeadPiece = 1u << 30;      // bytes of dz held at a time: the backward of 32768 x 32000 x d768 takes
+                                             // 4.55 ms, 5.03 with half of them (the parts of dx and more partial
+                                             // rounds), 4.36 in one piece
 constexpr int64_t kHeadPieceMost = 1 << 20;  // most tokens of a piece: offsets within a stage have 32 bits
 
 // An operand of a product: bf16 planes; ROWS: [rows][ld], contraction along a row;
@@ -412,10 +413,10 @@ __device__ __forceinline__ bool head_real(const int64_t* target, int64_t n, int 
   return target != nullptr && target[n] >= 0 && target[n] < V;
 }
 // What a row's weights refer to: 2^((z - a) log2 e - b), from a maximum m that is one of the
-// row's logits.  Near zero a = 0 and b = m log2 e, so that a weight is one multiply-add and an exponential;
-// the rounding of b (half a step of it, at most 2^-11) is in every weight alike.  Far off zero that
-// rounding would be any power of two: there a = m, b = 0.  m starts at the lowest finite value, never at a sentinel
-// that a finite logit can lie below.
+// row's logits.  Near zero a = 0 and b = m log2 e, so that a weight is one multiply-add and an
+// exponential; the rounding of b (half a step of it, at most 2^-12) is in every weight alike.
+// Far off zero that rounding would be any power of two: there a = m, b = 0.  m starts at the
+// lowest finite value, never at a sentinel that a finite logit can lie below.
 constexpr float kHeadFar = 4096.0f;
 constexpr float kHeadLowest = -3.402823466e38f;
 __device__ __forceinline__ bool head_far(float m) { return !(fabsf(m) < kHeadFar); }
@@ -577,9 +578,9 @@ __global__ __launch_bounds__(256) void k_head_join(const HeadJoin a) {
   l = wave_sum(l);
   if (__any(nan) || l == 0.0f) l = __builtin_nanf("");   // (no weight at all: every logit is minus infinity)
   if (lane != 0) return;
-  // l = f 2^e with f about 1.  The target's distance from the maximum and e are joined in 64 bits, so that logp is
-  // off by a few 2^-24 however large the logits are (less lse it would have an error of lse's size:
-  // 8e-6 at 100, of either sign).
+  // l = f 2^e with f about 1.  The target's distance from the maximum and e are joined in 64
+  // bits, so that logp is off by a few 2^-24 however large the logits are (less lse it would
+  // have an error of lse's size: 8e-6 at 100, of either sign).
   int e;
   float f = frexpf(l, &e);
   if (f < 0.70710678f) f *= 2.0f, --e;
@@ -637,7 +638,8 @@ __global__ __launch_bounds__(S::kThreads, S::kPerSimd) void k_head_dz(const Head
       if (a.dlogp != nullptr && head_real(a.target, n, a.V)) co -= a.dlogp[n];
       const float lse = a.lse[n];
       far = far || head_far(lse);
-      if (co != 0.0f) off[j] = (head_far(lse) ? lse - lse : lse * kLog2e) - __log2f(fabsf(co));   // (lse - lse: NaN stays NaN)
+      // (lse - lse: NaN stays NaN)
+      if (co != 0.0f) off[j] = (head_far(lse) ? lse - lse : lse * kLog2e) - __log2f(fabsf(co));
       neg[j] = __float_as_uint(co) & 0x80000000u;
     }
   }
@@ -759,11 +761,12 @@ __global__ __launch_bounds__(256) void k_head_rest(const HeadDz a, const float* 
   token[n] = real ? (int)a.target[n] : -1;
 }
 
-// Both for up to 1024 rows of x, and the rests' sums by token, in one launch: the sort, sums and joins of
-// more rows would take 20 us beside the products of few rows (512 rows of W 8192 x 1024: 9 us of 91).  A workgroup takes 16 rows, each by a
-// wave; the first row of a token sums them all, a wave those of a token of few rows, the workgroup those of one of
-// many.  sums[n] where n is such a row; first[t_n] = n, and other tokens' `first` is left as it was: `there`
-// has the tokens' bits, 65536 of them a workgroup.
+// Both for up to 1024 rows of x, and the rests' sums by token, in one launch: the sort, sums
+// and joins of more rows would take 20 us beside the products of few rows (512 rows of W
+// 8192 x 1024: 9 us of 91).  A workgroup takes 16 rows, each by a wave; the first row of a
+// token sums them all, a wave those of a token of few rows, the workgroup those of one of
+// many.  sums[n] where n is such a row; first[t_n] = n, and other tokens' `first` is left as
+// it was: `there` has the tokens' bits, 65536 of them a workgroup.
 constexpr int kFewRows = 1024, kFewThreads = 1024, kFewWaves = kFewThreads / 64, kFewAlone = 8;
 constexpr int kFewBits = 1 << 16;
 struct HeadFewRows {
@@ -928,8 +931,9 @@ __global__ __launch_bounds__(kFewThreads) void k_head_few(const HeadFewRows a) {
   }
 }
 
-// Rows of bf16 that go to the results' rows beside the products: W_{t_n} with the weight rest_n to row n
-// of dx, the sum of a token's rest_n x_n (rounded to bf16: of a part that is 2^-8 of the whole) to its row of dW.
+// Rows of bf16 that go to the results' rows beside the products: W_{t_n} with the weight
+// rest_n to row n of dx, the sum of a token's rest_n x_n (rounded to bf16: of a part that is
+// 2^-8 of the whole) to its row of dW.
 struct HeadMore {
   const bf16* rows;          // null: none
   int64_t ld;
@@ -1353,7 +1357,7 @@ static void head_grad(const HeadGrad& g, bool native, int cu, hipStream_t s) {
 struct HeadPlan {
   int piece;            // tokens of a piece, a multiple of 256
   size_t dz, acc, part; // bytes
-  size_t rest, sums, first, there, lists;   // of the targets' rests (and tokens), their sums by token and what forms those
+  size_t rest, sums, first, there, lists;   // of the targets' rests and tokens, and the rests' sums by token
   size_t bytes(const HeadLayout& l) const {
     return l.x_bytes + l.w_bytes + dz + acc + part + rest + sums + first + there + lists;
   }
@@ -1547,9 +1551,10 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
     else
       form(HeadMid<bf16>{});
     if (few && v0 == 0) {
-      const HeadFewRows f{z, logp, static_cast<const bf16*>(x), rest, token, dw != nullptr ? reinterpret_cast<bf16*>(sums) : nullptr,
-                          first, there, D};
-      const int64_t own = (N + kFewWaves - 1) / kFewWaves, bits = dw != nullptr ? ((int64_t)V + kFewBits - 1) / kFewBits : 0;
+      bf16* const out = dw != nullptr ? reinterpret_cast<bf16*>(sums) : nullptr;
+      const HeadFewRows f{z, logp, static_cast<const bf16*>(x), rest, token, out, first, there, D};
+      const int64_t own = (N + kFewWaves - 1) / kFewWaves;
+      const int64_t bits = dw != nullptr ? ((int64_t)V + kFewBits - 1) / kFewBits : 0;
       k_head_few<<<(unsigned)(own > bits ? own : bits), kFewThreads, 0, s>>>(f);
     } else if (l.native)
       k_head_target<float, 1><<<rows, 256, 0, s>>>(z, logp);

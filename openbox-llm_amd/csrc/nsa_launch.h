@@ -51,10 +51,11 @@ int nsa_pool_fwd_set(const void* const* x, void* const* out, int m, int B, int H
 int nsa_pool_bwd_set(const void* const* dpool, int dpool_dtype, void* const* dx, int m, int B, int H, int T, int D,
                      int l, int d, int dtype, void* stream);
 
-// Sums of weighted bf16 rows [n][D] by token (nsa_embed.hip): of the tokens v < V that some index[i] names, and whose bits
-// `there` ([V rounded up to 64, / 64]) has, first[v] is the row of `sums` ([n][D], bf16, rounded once) that holds the
-// sum of weight[i] rows[i] over the i with index[i] = v, in an order fixed by the indices; other elements of
-// `first` are left as they were.  n >= 1, the limits of nsa_embed_bwd; workspace on 16 bytes.
+// Sums of weighted bf16 rows [n][D] by token (nsa_embed.hip): of the tokens v < V that some
+// index[i] names, and whose bits `there` ([V rounded up to 64, / 64]) has, first[v] is the row
+// of `sums` ([n][D], bf16, rounded once) that holds the sum of weight[i] rows[i] over the i
+// with index[i] = v, in an order fixed by the indices; other elements of `first` are left as
+// they were.  n >= 1, the limits of nsa_embed_bwd; workspace on 16 bytes.
 size_t nsa_token_sums_workspace(int64_t n, int D);
 int nsa_token_sums(const int64_t* index, const float* weight, const void* rows, void* sums, int* first, uint64_t* there,
                    void* workspace, int64_t n, int64_t V, int D, void* stream);

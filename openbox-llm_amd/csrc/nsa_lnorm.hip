@@ -9,9 +9,9 @@
 //   dh = dh_out + rstd (g - mean_j g_j - n mean_j(g_j n_j));   dx = dr = dh
 //   dw = sum over rows of dy n,   db = sum over rows of dy
 //
-// The mean is summed in 64 bits and rounded once: a sum in 32, or its product with a rounded 1 / D, is off by steps of
-// the elements' size, which rows far off zero show beside their deviation (41 times 16384 came out as 0.19, not
-// 0).
+// The mean is summed in 64 bits and rounded once: a sum in 32, or its product with a
+// rounded 1 / D, is off by steps of the elements' size, which rows far off zero show
+// beside their deviation (41 times 16384 came out as 0.19, not 0).
 //
 // Every kernel is bound by the bytes it moves: one read of x and r (dy, dh_out and
 // h in the backward), one write of h and y (dx, dr).  A row stays in registers, so
@@ -26,9 +26,10 @@
 // columns' parts of dw and db in registers; the parts are added in workgroup order
 // by a second launch, so that both have the same bits on every run.
 //
-// Measured, against a copy's 5.4 TB/s: 32768 x 768 (bf16 branch, float32 stream) 59 us
-// forward (5.1 TB/s), 78 backward (5.2) and 6.5 for the 2048 parts of dw and db; 8191 x 8192
-// bf16 96 (5.6), 114 (4.7) and 8.4.
+// Measured, against a copy's 5.4 TB/s: 32768 x 768 (bf16 branch, float32 stream) 60 us
+// forward (5.1 TB/s), 79 backward (5.2) and 6.4 for the 2048 parts of dw and db; 8191 x 8192
+// bf16 97 (5.5), 116 (4.6) and 10.6; 1024 x 32768 52 and 99 (the backward reads h and dy
+// for the rows' sums, for dx and for the columns' sums), 512 x 65536 88 and 119.
 #include "nsa_launch.h"
 #include "nsa_rows.h"
 
@@ -439,7 +440,7 @@ __global__ __launch_bounds__(256) void k_ln_dw_wide(const LnBwdArgs a) {
 }
 
 // out[c] = sum of part[p][c] (dw for blockIdx.y = 0, db for 1): 32 columns a workgroup (a
-// part's cache lines, each in one L2: 512 parts of 8192 8.4 us, 13.8 with half lines), 32
+// part's cache lines, each in one L2: 512 parts of 8192 8.4 us in a loop, 13.8 with half lines), 32
 // interleaved sums over the parts, added in order.
 __global__ __launch_bounds__(1024) void k_ln_dw(const float* __restrict__ part, int nparts, int D, void* dw, void* db,
                                                 bool w_bf16) {

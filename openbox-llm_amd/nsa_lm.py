@@ -171,8 +171,9 @@ def linear_logprobs(x, weight, targets=None):
     float32 rows are computed in float32's precision.  bfloat16 rows are products of
     bfloat16 with float32 sums, and the logits' gradient is rounded once to bfloat16
     on its way into the products with x and weight, but for the targets' own elements,
-    which keep float32's digits in both; float32 weights beside bfloat16 rows are rounded to bfloat16 first (as under autocast) and have a float32
-    gradient.  At most 2^22 rows.
+    which keep float32's digits in both; float32 weights beside bfloat16 rows are
+    rounded to bfloat16 first (as under autocast) and have a float32 gradient.  At most
+    2^22 rows.
 
     Every finite logit counts, whatever its size.  A row with NaN or plus infinity among
     its logits, or with minus infinity alone, is NaN, and so is its gradient where it has

@@ -1,5 +1,5 @@
-"""CPU checks of the decoder's ends at the limits of their 32-bit indices: the C entry points refuse what lies past them before
-any launch."""
+"""CPU checks of the decoder's ends at the limits of their 32-bit indices: the C entry points
+refuse what lies past them before any launch."""
 
 import os
 
