@@ -58,3 +58,37 @@ def test_captured_steps_have_the_eager_bits(B, T, V, D, rows, table):
             assert torch.equal(a, b), (k, i)
             assert bool(a.isfinite().all()) and bool(a.any()), (k, i)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("N,V,D,rows,table", [(5, 300, 64, BF, BF), (300, 1009, 200, BF, F32), (1500, 2500, 256, BF, BF), (40, 500, 72, F32, F32),
+                                              (700, 3000, 96, F32, F32), (9000, 200000, 64, BF, BF)])
+def test_nothing_is_read_that_was_not_written(N, V, D, rows, table):
+    """Workspaces and outputs that start as 0xff bytes and NaN: the same bits."""
+    import nsa_lm
+    dev = require_gpu()
+    g = torch.Generator(dev).manual_seed(N)
+    w = torch.randn(V, D, generator=g, device=dev).to(table).requires_grad_()
+    p = torch.randn(N, D, generator=g, device=dev).to(table).requires_grad_()
+    a = (1 + 0.1 * torch.randn(D, generator=g, device=dev)).to(table).requires_grad_()
+    tok = torch.randint(-2, V // 3, (1, N), generator=g, device=dev)
+    tgt = torch.randint(-5, V, (1, N), generator=g, device=dev)
+
+    def step():
+        x = nsa_lm.embed(tok, w, 1.0, p, out_dtype=rows)
+        y, h = nsa_lm.add_layer_norm(x, x, a, a, out_dtype=rows)
+        r = nsa_lm.linear_logprobs(y, w, tgt)
+        return [x.detach(), y.detach(), h.detach(), r.logp.detach(), r.lse.detach(),
+                *torch.autograd.grad((r.logp, r.lse), (w, p, a), (torch.ones_like(r.logp), 0.5 * torch.ones_like(r.lse)))]
+    want = step()
+    was = torch.are_deterministic_algorithms_enabled(), torch.is_deterministic_algorithms_warn_only_enabled()
+    fill = torch.utils.deterministic.fill_uninitialized_memory
+    try:
+        torch.use_deterministic_algorithms(True, warn_only=True)
+        torch.utils.deterministic.fill_uninitialized_memory = True
+        assert torch.empty(4, device=dev).isnan().all()
+        got = step()
+    finally:
+        torch.utils.deterministic.fill_uninitialized_memory = fill
+        torch.use_deterministic_algorithms(was[0], warn_only=was[1])
+    for i, (b, c) in enumerate(zip(want, got)):
+        assert torch.equal(b, c), i

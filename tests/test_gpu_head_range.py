@@ -150,3 +150,49 @@ def test_ignored_rows_have_no_gradient_whatever_their_logits(N, dtype):
     wild[bad] = float("nan")
     r, (dx, _) = grads(wild)
     assert r.lse[bad].isnan().all() and torch.equal(dx, dx0)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("N,V", SHAPES)
+def test_one_logit_far_from_the_others(N, V, dtype):
+    """Logits within 4 of 0 and one, late in the vocabulary, far above or (in rows of x = -1) far below them all: the maximum passes
+    from near zero to far off it.  Above, its probability is 1; below it is 0 and the row is as without it, bit for bit
+    where the same wave has rows of the other kind."""
+    import nsa_lm
+    dev = require_gpu()
+    g = torch.Generator().manual_seed(V)
+    w = torch.randn(V, 64, generator=g)
+    w[:, 0] = (torch.randint(-32, 33, (V,), generator=g) / 8.0)
+    x = torch.zeros(N, 64)
+    x[:, 0] = torch.tensor([1.0, -1.0, -1.0])[torch.arange(N) % 3]
+    t = torch.randint(0, V - 8, (N,), generator=g)
+    x, t = x.to(dtype).to(dev), t.to(dev)
+    up = x[:, 0] > 0
+    for size in (300.0, 4095.0, 4100.0, 1e6, 1e30, 2.0 ** 126):
+        for at in (V - 3, V // 2):
+            w2 = w.to(dtype).to(dev)
+            w2[at, 0] = size
+            tt = torch.where(up & (torch.arange(N, device=dev) % 2 == 0), at, torch.where(t == at, t + 1, t))
+            z = x[:, :1].double() * w2[:, 0].double()[None]
+            lse = torch.logsumexp(z, 1)
+            want = z.gather(1, tt[:, None])[:, 0] - lse
+            xs, ws = x.clone().requires_grad_(), w2.clone().requires_grad_()
+            r = nsa_lm.linear_logprobs(xs, ws, tt)
+            tol = (284 + 8 * lse.abs()) * U
+            assert ((r.lse.double() - lse).abs() <= tol).all(), (size, at)
+            assert ((r.logp.double() - want).abs() <= tol + 2 * U * want.abs()).all(), (size, at)
+            one = torch.ones(N, device=dev)
+            dx, dw = torch.autograd.grad((r.logp, r.lse), (xs, ws), (one, 0.25 * one))
+            assert dx[~up].isfinite().all() and dw[:at].isfinite().all()
+            # dz of the row above: 1 at its target, -3/4 at the far token; columns of w that x does not see
+            other = w2[:, 1:].double()
+            ref = other[tt] - 0.75 * other[at]
+            err = (dx[:, 1:].double() - ref).abs() - 2.0 ** -7 * (other[tt].abs() + other[at].abs())
+            assert (err[up] <= 0).all(), (size, at)
+            xi = x.clone()
+            xi[up] = 0                                   # the far rows gone: the others' bits stay
+            xs = xi.requires_grad_()
+            r2 = nsa_lm.linear_logprobs(xs, ws, tt)
+            d2, = torch.autograd.grad((r2.logp, r2.lse), xs, (one, 0.25 * one))
+            assert torch.equal(r2.lse[~up], r.lse[~up]) and torch.equal(r2.logp[~up], r.logp[~up])
+            assert torch.equal(d2[~up], dx[~up]), (size, at)
