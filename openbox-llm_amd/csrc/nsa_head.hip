@@ -734,14 +734,20 @@ __device__ __forceinline__ float head_target(float b, float dl, float lp) {
 __device__ __forceinline__ float head_target(const HeadDz& a, const float* logp, int64_t n) {
   return head_target(a.dlogp[n], a.dlse != nullptr ? a.dlse[n] : 0.0f, logp[n]);
 }
-// ... where the piece has it
+// ... where the piece has it, and (rest: not null) what its rounding to bf16 leaves of it with
+// its token; 0 and -1 without one.
 template <typename E, int PLANES>
-__global__ __launch_bounds__(256) void k_head_target(const HeadDz a, const float* logp) {
+__global__ __launch_bounds__(256) void k_head_target(const HeadDz a, const float* logp, float* rest, int* token) {
   const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (n >= a.N || a.dlogp == nullptr || !head_real(a.target, n, a.V)) return;
-  const int64_t v = a.target[n] - a.v0;
-  if (v < 0 || v >= a.vocab) return;
-  float d = head_target(a, logp, n);
+  if (n >= a.N || a.dlogp == nullptr) return;
+  const bool real = head_real(a.target, n, a.V);
+  const int64_t t = real ? a.target[n] : -1, v = t - a.v0;
+  float d = real ? head_target(a, logp, n) : 0.0f;
+  if (rest != nullptr) {
+    rest[n] = d - (float)(bf16)d;
+    token[n] = (int)t;
+  }
+  if (!real || v < 0 || v >= a.vocab) return;
   E* p = static_cast<E*>(a.dz) + n * a.ld + v;
 #pragma unroll
   for (int q = 0; q < PLANES; ++q) {
@@ -751,23 +757,12 @@ __global__ __launch_bounds__(256) void k_head_target(const HeadDz a, const float
   }
 }
 
-// What its rounding to bf16 leaves of it, and its token; 0 and -1 without one.
-__global__ __launch_bounds__(256) void k_head_rest(const HeadDz a, const float* logp, float* rest, int* token) {
-  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (n >= a.N) return;
-  const bool real = head_real(a.target, n, a.V);
-  const float d = real ? head_target(a, logp, n) : 0.0f;
-  rest[n] = d - (float)(bf16)d;
-  token[n] = real ? (int)a.target[n] : -1;
-}
-
-// Both for up to 1024 rows of x, and the rests' sums by token, in one launch: the sort, sums
-// and joins of more rows would take 20 us beside the products of few rows (512 rows of W
-// 8192 x 1024: 9 us of 91).  A workgroup takes 16 rows, each by a wave; the first row of a
-// token sums them all, a wave those of a token of few rows, the workgroup those of one of
-// many.  sums[n] where n is such a row; first[t_n] = n, and other tokens' `first` is left as
-// it was: `there` has the tokens' bits, 65536 of them a workgroup.
-constexpr int kFewRows = 1024, kFewThreads = 1024, kFewWaves = kFewThreads / 64, kFewAlone = 8;
+// Both for up to 2048 rows of x, and the rests' sums by token, in one launch.  More rows are
+// sorted by token (2048 rows of 768: 22 us, 29 sorted; 4096: 45 and 38).  A workgroup takes 16
+// rows, each by a wave; the first row of a token sums them all, a wave those of a token of few
+// rows, the workgroup those of one of many.  sums[n] where n is such a row; first[t_n] = n, and
+// other tokens' `first` is left as it was: `there` has the tokens' bits, 65536 of them a workgroup.
+constexpr int kFewRows = 2048, kFewThreads = 1024, kFewWaves = kFewThreads / 64, kFewAlone = 8;
 constexpr int kFewBits = 1 << 16;
 struct HeadFewRows {
   HeadDz z;
@@ -1496,21 +1491,8 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
   if (l.pack_x) head_pack(x, x_dtype, xp, N, D, l.ld, l.px, l.native, s);
   if (l.pack_w) head_pack(w, w_dtype, wp, V, D, l.ld, l.pw, l.native, s);
   const unsigned rows = (unsigned)((N + 255) / 256);
-  // the targets' rests: of few rows with the targets' elements of the first piece, else here
+  // the targets' rests come with the targets' elements of the first piece
   const bool rests = x_dtype == NSA_BF16 && dlogp != nullptr, few = rests && N <= kFewRows;
-  if (rests && !few) {
-    HeadDz z{};
-    z.dlogp = dlogp;
-    z.dlse = dlse;
-    z.target = target;
-    z.N = (int)N;
-    z.V = V;
-    k_head_rest<<<rows, 256, 0, s>>>(z, logp, rest, token);
-    if (dw != nullptr) {
-      const int rc = nsa_token_sums(target, rest, x, sums, first, there, ws, N, V, D, stream);
-      if (rc != NSA_OK) return rc;
-    }
-  }
   const int ldx = l.pack_x ? l.ld : D, ldw = l.pack_w ? l.ld : D;
   const void* X = l.pack_x ? xp : x;
   const char* W = l.pack_w ? wp : static_cast<const char*>(w);
@@ -1556,12 +1538,18 @@ extern "C" int nsa_head_bwd(const void* x, const void* w, const int64_t* target,
       const int64_t own = (N + kFewWaves - 1) / kFewWaves;
       const int64_t bits = dw != nullptr ? ((int64_t)V + kFewBits - 1) / kFewBits : 0;
       k_head_few<<<(unsigned)(own > bits ? own : bits), kFewThreads, 0, s>>>(f);
-    } else if (l.native)
-      k_head_target<float, 1><<<rows, 256, 0, s>>>(z, logp);
-    else if (l.px == 3)
-      k_head_target<bf16, 3><<<rows, 256, 0, s>>>(z, logp);
-    else
-      k_head_target<bf16, 1><<<rows, 256, 0, s>>>(z, logp);
+    } else if (l.native) {
+      k_head_target<float, 1><<<rows, 256, 0, s>>>(z, logp, nullptr, nullptr);
+    } else if (l.px == 3) {
+      k_head_target<bf16, 3><<<rows, 256, 0, s>>>(z, logp, nullptr, nullptr);
+    } else {
+      const bool all = rests && v0 == 0;
+      k_head_target<bf16, 1><<<rows, 256, 0, s>>>(z, logp, all ? rest : nullptr, token);
+      if (all && dw != nullptr) {
+        const int rc = nsa_token_sums(target, rest, x, sums, first, there, ws, N, V, D, stream);
+        if (rc != NSA_OK) return rc;
+      }
+    }
     if (dx != nullptr) {
       HeadGrad g;
       const bool last = v0 + vocab >= V, lone = p.acc == 0;

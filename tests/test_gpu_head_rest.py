@@ -37,7 +37,8 @@ def _targets(N, V, kind, g):
 @pytest.mark.parametrize("kind", ["any", "text", "one"])
 @pytest.mark.parametrize("N,V,D", [(1, 1, 1), (1, 130, 64), (7, 40, 33), (40, 1000, 64), (300, 700, 136), (2100, 5300, 72), (4096, 500, 128),
                                    (4097, 9000, 100), (9000, 301, 520), (22100, 13000, 64), (16, 70001, 768), (50, 30, 1300),
-                                   (1024, 2000, 1100), (1025, 2000, 1100), (5000, 3000, 2100)])
+                                   (1024, 2000, 1100), (1025, 2000, 1100), (2048, 70, 600), (2049, 70, 600),
+                                   (5000, 3000, 2100)])
 def test_the_targets_elements(N, V, D, kind, wd):
     import nsa_lm
     dev = require_gpu()
